@@ -1,0 +1,372 @@
+// Attention of a tile of query rows to 64-key tiles, shared by the sliding-window
+// and the paged-cache kernels (bf16 and fp32, head dim 64 / 128).
+//
+// A wave holds 32 query rows as the columns of S^T = K . Q^T on 32x32 MFMA
+// tiles: lane l has column l % 32, and of each 32-key tile the 16 keys of its
+// half l / 32.  Row maxima and sums are then in-lane but for one exchange
+// between the halves, and the probabilities are already the B operand of
+// O^T += V^T . P^T: nothing moves between lanes.  The rows of one KV head's
+// query heads are flattened (row r = token r / G, head r % G), so every group
+// size fills the tiles and the heads of a group share the staged keys.
+//
+// Softmax: running maximum and sum in fp32, in units of log2.  The sums (O, l)
+// are rescaled only when a row's maximum grows by more than 8 (a factor of 256,
+// far from fp32's range), so most tiles do no rescaling.
+//
+// Masked keys have probability 0; a NaN or infinity of V in a masked place
+// would still spoil 0 * V.  Whether that happened shows in the result, so a
+// workgroup whose rows come out non-finite computes them once more key by key,
+// where a masked key takes no part (attend_each).  Finite inputs pay nothing but
+// the check of the result.
+#pragma once
+
+#include "hba_common.h"
+#include "hba_dma.h"
+
+namespace hba {
+namespace rows {
+
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef unsigned int u32x4r __attribute__((ext_vector_type(4)));
+
+constexpr int KT = 64;            // keys per tile
+constexpr int NW = 4;             // waves per workgroup
+constexpr int RW = 32;            // query rows per wave
+constexpr int RT = NW * RW;       // query rows per workgroup
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LAZY = 8.0f;      // log2 units a maximum may grow before O and l are rescaled
+
+__device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
+
+// The value of lane l ^ 32.
+__device__ __forceinline__ float other_half(float v) {
+    const uint32_t x = __float_as_uint(v);
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+
+// Operand fragments of a 16-deep step: 8 elements of one row or column, lane l
+// those of its half, elements 8 (l / 32) .. + 7.  mma adds a 32x32 product.
+// Lane l of the result: column l % 32, rows 8 (r / 4) + 4 (l / 32) + r % 4.
+// fp32 takes eight 2-deep steps: in step e half h supplies element 8 h + e.
+template <int DT> struct Op;
+template <> struct Op<1> {
+    typedef bf16x8 F;
+    static __device__ __forceinline__ f32x16 mma(F a, F b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+    // the probabilities enter the product in bf16, as the matrix cores take them: a
+    // relative 2^-9 each, which averages out over a row's keys
+    static __device__ __forceinline__ F pack(const float (&x)[8]) {
+        F r;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r[e] = (__bf16)x[e];
+        return r;
+    }
+    static __device__ __forceinline__ F load(const void *p) {
+        return __builtin_bit_cast(F, *reinterpret_cast<const u32x4r *>(p));
+    }
+    static __device__ __forceinline__ void unpack(F f, float (&x)[8]) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = (float)f[e];
+    }
+};
+template <> struct Op<0> {
+    typedef f32x8 F;
+    static __device__ __forceinline__ f32x16 mma(F a, F b, f32x16 c) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+        return c;
+    }
+    static __device__ __forceinline__ F pack(const float (&x)[8]) {
+        F r;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r[e] = x[e];
+        return r;
+    }
+    static __device__ __forceinline__ F load(const void *p) {
+        const f32x4 a = reinterpret_cast<const f32x4 *>(p)[0], b = reinterpret_cast<const f32x4 *>(p)[1];
+        return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    static __device__ __forceinline__ void unpack(F f, float (&x)[8]) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = f[e];
+    }
+};
+
+// Elements 8u .. 8u+7 of a 32x32 result as the operand of the step over its
+// rows' u-th half.
+template <int DT> __device__ __forceinline__ typename Op<DT>::F half16(const f32x16 &p, int u) {
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = p[8 * u + e];
+    return Op<DT>::pack(x);
+}
+
+// ------------------------------------------------------------ staged rows --
+// R rows of D elements in LDS, 16-byte chunk c of row r at place c ^ (r & 7) of
+// its row: the eight lanes that an LDS cycle serves then read eight different
+// bank groups, whether they read one chunk of eight rows (an operand along the
+// rows) or, transposed, four rows' pieces.
+template <int DT, int D> struct Tile {
+    typedef typename St<DT>::T T;
+    typedef typename Op<DT>::F F;
+    static constexpr int ESZ = DT == 1 ? 2 : 4;
+    static constexpr int NCH = D * ESZ / 16;          // chunks per row
+    static constexpr int ROWB = D * ESZ;              // bytes per row
+
+    static __device__ __forceinline__ int at(int r, int c) { return r * ROWB + ((c ^ (r & 7)) * 16); }
+
+    // Row r, elements 16 ks + 8 (lane / 32) .. + 7.
+    static __device__ __forceinline__ F row(const char *t, int r, int ks, int hf) {
+        if constexpr (DT == 1) {
+            return Op<1>::load(t + at(r, 2 * ks + hf));
+        } else {
+            const f32x4 a = *reinterpret_cast<const f32x4 *>(t + at(r, 4 * ks + 2 * hf));
+            const f32x4 b = *reinterpret_cast<const f32x4 *>(t + at(r, 4 * ks + 2 * hf + 1));
+            return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+    // Column 32 dt + lane % 32 over rows r0 + 4 hf + 0..3 and r0 + 8 + 4 hf + 0..3: the
+    // rows that registers 8u .. 8u+7 of a result hold, r0 = 32 tile + 16 u.
+    static __device__ __forceinline__ F col(const char *t, int r0, int dt, int lane) {
+        const int hf = lane >> 5;
+        if constexpr (DT == 1) {
+            const int r = r0 + 4 * hf + ((lane & 15) >> 2);
+            const int x = 32 * dt + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+            const int c = x >> 3, o = (x & 7) * 2;
+            return ld_tr8(reinterpret_cast<const bf16_t *>(t + at(r, c) + o),
+                          reinterpret_cast<const bf16_t *>(t + at(r + 8, c) + o));
+        } else {
+            const int x = 32 * dt + (lane & 31), c = x >> 2, o = (x & 3) * 4;
+            F f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                f[e] = *reinterpret_cast<const float *>(t + at(r0 + 4 * hf + (e & 3) + 8 * (e >> 2), c) + o);
+            return f;
+        }
+    }
+    // Stage rows j0 .. j0 + R - 1 of a strided array (`bytes` from row to row); rows past
+    // `last` read row `last`.  Called by all NW waves.
+    template <int R>
+    static __device__ __forceinline__ void stage(const char *base, int64_t bytes, int j0, int last, uint32_t lds) {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+        for (int i = 0; i < R * NCH / 64 / NW; ++i) {
+            const int p = (i * NW + wave) * 64 + lane;
+            const int r = p / NCH, c = (p % NCH) ^ (r & 7);
+            const int j = min(j0 + r, last);
+            dma16(base + (int64_t)j * bytes + c * 16, lds + (i * NW + wave) * 1024);
+        }
+    }
+};
+
+// Keys and values of one KV head as strided rows.
+template <int DT, int D> struct DenseKV {
+    typedef typename Op<DT>::F F;
+    typedef Tile<DT, D> TL;
+    static constexpr int BYTES = 2 * KT * TL::ROWB;   // a staged tile: keys, then values
+    const char *k, *v;
+    int64_t kb, vb;                                   // bytes from row to row
+    int last;                                         // the last row that may be read
+
+    __device__ __forceinline__ void stage(int tile, uint32_t lds) const {
+        TL::template stage<KT>(k, kb, tile * KT, last, lds);
+        TL::template stage<KT>(v, vb, tile * KT, last, lds + KT * TL::ROWB);
+    }
+    // the key (of 32) that register r of half hf holds
+    static __device__ __forceinline__ int key(int r, int hf) { return 8 * (r >> 2) + 4 * hf + (r & 3); }
+    static __device__ __forceinline__ F kf(const char *t, int kt, int ks, int lane) {
+        return TL::row(t, 32 * kt + (lane & 31), ks, lane >> 5);
+    }
+    static __device__ __forceinline__ F vf(const char *t, int kt, int dt, int u, int lane) {
+        return TL::col(t + KT * TL::ROWB, 32 * kt + 16 * u, dt, lane);
+    }
+    template <bool LO>
+    __device__ __forceinline__ float dot(const F (&q)[D / 16], const F *, int j, int hf) const;
+    __device__ __forceinline__ void add(f32x16 (&o)[D / 32], int j, float p, int hf) const;
+};
+
+// What a row (a lane's column) and its wave see: keys j < hi with j >= lo or
+// j < S.  The wave's bounds cover its valid rows.
+struct Sees {
+    int lo, hi, S;
+    int lo_min, lo_max, hi_min, hi_max;
+};
+
+template <int DT, int D> struct RowAcc {
+    f32x16 O[D / 32];
+    float m, l;       // running maximum (log2 units; -inf: nothing seen yet), and this half's part of the sum
+};
+
+// One pass of the workgroup's rows over tiles it0 .. it1 - 1 of their list
+// (tile it < ns: sinks, tile it; else tile wt0 + it - ns).  c: logits to log2
+// units.  LO: the queries' low parts, added to the scores.  Every wave of the
+// workgroup calls it; it leaves no wave reading LDS.
+template <int DT, int D, bool LO, class Src>
+__device__ __forceinline__ void attend(const Src &src, char *smem, const typename Op<DT>::F (&q)[D / 16],
+                                       const typename Op<DT>::F *qlo, float c, int it0, int it1, int ns, int wt0,
+                                       const Sees &w, RowAcc<DT, D> &a) {
+    constexpr int NKS = D / 16, NDT = D / 32;
+    const int lane = threadIdx.x & 63, hf = lane >> 5;
+    const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) a.O[dt] = zero;
+    a.m = -INFINITY;
+    a.l = 0.0f;
+    float mc = 0.0f;   // the exponent's shift: m, or 0 while nothing is seen
+    const uint32_t lds = lds_offset(smem);
+    if (it0 < it1) src.stage(it0 < ns ? it0 : wt0 + it0 - ns, lds);
+#pragma unroll 1
+    for (int it = it0; it < it1; ++it) {
+        wait_vm<0>();
+        __syncthreads();   // this tile is staged, and the other buffer is read no more
+        const int cur = (it - it0) & 1, nx = it + 1;
+        if (nx < it1) src.stage(nx < ns ? nx : wt0 + nx - ns, lds + (cur ^ 1) * Src::BYTES);
+        const int j0 = (it < ns ? it : wt0 + it - ns) * KT;
+        if (j0 >= w.hi_max || (j0 + KT <= w.lo_min && j0 >= w.S)) continue;   // nothing the wave's rows see
+        const char *t = smem + cur * Src::BYTES;
+        f32x16 s[2];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+            s[kt] = zero;
+#pragma unroll
+            for (int ks = 0; ks < NKS; ++ks) {
+                const typename Op<DT>::F kf = Src::kf(t, kt, ks, lane);
+                s[kt] = Op<DT>::mma(kf, q[ks], s[kt]);
+                if constexpr (LO) s[kt] = Op<DT>::mma(kf, qlo[ks], s[kt]);
+            }
+        }
+        const bool whole = j0 + KT <= w.hi_min && (j0 >= w.lo_max || j0 + KT <= w.S);
+        if (!whole) {
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int j = j0 + 32 * kt + Src::key(r, hf);
+                    if (!(j < w.hi && (j >= w.lo || j < w.S))) s[kt][r] = -INFINITY;
+                }
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kt][r]);
+        mx = fmaxf(mx, other_half(mx)) * c;
+        const bool grow = mx > a.m + LAZY;   // m = -inf: whenever something is seen
+        if (__ballot(grow)) {
+            const float mn = grow ? mx : a.m;
+            const float al = (a.m == -INFINITY) ? 0.0f : ex2(a.m - mn);   // nothing to rescale yet
+            a.l *= al;
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) a.O[dt][r] *= al;
+            a.m = mn;
+            mc = (mn == -INFINITY) ? 0.0f : mn;
+        }
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float p = ex2(fmaf(s[kt][r], c, -mc));
+                s[kt][r] = p;
+                a.l += p;
+            }
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const typename Op<DT>::F pf = half16<DT>(s[kt], u);
+#pragma unroll
+                for (int dt = 0; dt < NDT; ++dt) a.O[dt] = Op<DT>::mma(Src::vf(t, kt, dt, u, lane), pf, a.O[dt]);
+            }
+    }
+    __syncthreads();
+}
+
+// Sum over both halves of a fragment pair: the dot product of two rows.
+template <int DT, int D>
+__device__ __forceinline__ float dot_rows(const typename Op<DT>::F (&x)[D / 16], const char *p, int hf) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+        float u[8], y[8];
+        Op<DT>::unpack(x[ks], u);
+        Op<DT>::unpack(Op<DT>::load(p + (16 * ks + 8 * hf) * Tile<DT, D>::ESZ), y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = fmaf(u[e], y[e], sum);
+    }
+    return sum + other_half(sum);
+}
+
+// o += f * (row p) on the elements 32 dt + 8 g + 4 hf + i of registers 4 g + i.
+template <int DT, int D>
+__device__ __forceinline__ void add_row(f32x16 (&o)[D / 32], const char *p, float f, int hf) {
+    typedef typename St<DT>::T T;
+    const T *x = reinterpret_cast<const T *>(p);
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[dt][r] = fmaf(f, St<DT>::ld(x, 32 * dt + 8 * (r >> 2) + 4 * hf + (r & 3)), o[dt][r]);
+}
+
+template <int DT, int D>
+template <bool LO>
+__device__ __forceinline__ float DenseKV<DT, D>::dot(const F (&q)[D / 16], const F *, int j, int hf) const {
+    return dot_rows<DT, D>(q, k + (int64_t)min(j, last) * kb, hf);
+}
+template <int DT, int D>
+__device__ __forceinline__ void DenseKV<DT, D>::add(f32x16 (&o)[D / 32], int j, float p, int hf) const {
+    add_row<DT, D>(o, v + (int64_t)min(j, last) * vb, p, hf);
+}
+
+// attend, one key at a time: for rows that came out non-finite.  Each lane adds
+// the visible keys only, so nothing of a masked key reaches its row.
+template <int DT, int D, bool LO, class Src>
+__device__ __noinline__ void attend_each(const Src &src, const typename Op<DT>::F (&q)[D / 16],
+                                         const typename Op<DT>::F *qlo, float c, int it0, int it1, int ns, int wt0,
+                                         const Sees &w, RowAcc<DT, D> &a) {
+    const int hf = (threadIdx.x & 63) >> 5;
+    const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) a.O[dt] = zero;
+    a.m = -INFINITY;
+    a.l = 0.0f;
+#pragma unroll 1
+    for (int it = it0; it < it1; ++it) {
+        const int j0 = (it < ns ? it : wt0 + it - ns) * KT;
+#pragma unroll 1
+        for (int j = j0; j < min(j0 + KT, w.hi_max); ++j) {
+            float s = src.template dot<LO>(q, qlo, j, hf) * c;
+            if (!(j < w.hi && (j >= w.lo || j < w.S))) continue;
+            if (s != s) {   // a NaN makes the row NaN
+                a.l = s;
+                continue;
+            }
+            const float mn = fmaxf(a.m, s), al = a.m == -INFINITY ? 0.0f : ex2(a.m - mn);
+            const float p = mn == -INFINITY ? 0.0f : ex2(s - mn);   // +inf: inf - inf, a NaN
+            a.l = fmaf(a.l, al, hf ? 0.0f : p);
+#pragma unroll
+            for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) a.O[dt][r] *= al;
+            a.m = mn;
+            src.add(a.O, j, p, hf);
+        }
+    }
+}
+
+// The list of 64-key tiles that rows with first visible key lo (the smallest),
+// one past the last hi (the largest) and S sinks see: ns tiles of sinks, then
+// tiles wt0 ...; returns how many.
+__device__ __forceinline__ int tile_list(int lo, int hi, int S, int &ns, int &wt0) {
+    wt0 = lo / KT;
+    ns = min((min(S, hi) + KT - 1) / KT, wt0);
+    const int wt1 = (hi + KT - 1) / KT;
+    return ns + max(wt1 - wt0, 0);
+}
+
+}  // namespace rows
+}  // namespace hba

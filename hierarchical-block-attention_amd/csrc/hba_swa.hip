@@ -1,0 +1,616 @@
+// Sliding-window attention with sinks: row i of a head sees the keys j <= i with
+// j > i - W or j < S, on queries and keys as they are given (any positions or
+// norms already applied), forward and backward, any length.
+//
+//   o_i = sum_j p_ij v_j,  p_ij = exp(scale q_i . k_j - lse_i)
+//   dv_j = sum_i p_ij do_i,  ds_ij = p_ij (do_i . v_j - do_i . o_i)
+//   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i
+//
+// Forward and dq: a workgroup has 128 rows of one KV head's query heads
+// (hba_rows.h) and walks the 64-key tiles that they see.  dk and dv: a workgroup
+// has 128 keys as the columns of S = Q . K^T and walks its KV head's query heads
+// and their 64-token tiles, so the sum over the heads of a group stays in
+// registers and nothing is added by atomics: the gradients are the same bits
+// from run to run.  A tile whose keys many rows see (sinks: every later row) is
+// cut into parts that sum into a workspace and are joined in order by a second
+// kernel.
+#include "hba_abi.h"
+#include "hba_common.h"
+#include "hba_rows.h"
+#include "hba_xcd.h"
+
+namespace hba {
+namespace swa {
+
+using namespace rows;
+
+struct Args {
+    const char *q, *k, *v, *dout;       // strided rows; byte strides of batch, token, head
+    int64_t qs[3], ks[3], vs[3], dos[3];
+    const int32_t *lens;                // rows of each sequence (nullptr: n)
+    int n, Hq, Hkv, G, W, S;
+    float scale, c;                     // c: logits to log2 units
+    int Cn, ntiles, xmap;               // B * Hkv, row tiles of one of them, workgroup map
+    char *out;                          // [B, n, Hq, D]
+    float *lse, *delta;                 // [B, Hq, n]: log2-sum-exp2 (+inf: no row), do . o
+    char *dq, *dk, *dv;
+    float *part;                        // dk / dv sums of tiles in several parts
+    int nst, Ps, Pn, chunk;             // tiles of sinks, parts of those and of the others, steps of a part
+};
+
+__device__ __forceinline__ int seq_len(const Args &a, int b) {
+    return a.lens ? max(0, min(a.n, a.lens[b])) : a.n;
+}
+
+// The rows of this wave: its lane's column and what they see.
+struct Rows {
+    int b, g, tok, head, len, lo, hi;   // lo .. hi: tiles' bounds over the workgroup
+    bool in, valid;                     // a row of the batch; one of its sequence
+    Sees w;
+};
+
+template <int D> __device__ __forceinline__ bool find_rows(const Args &a, Rows &x) {
+    int combo, tile;
+    xcd_map(blockIdx.x, a.Cn, a.ntiles, a.xmap, combo, tile);
+    if (tile >= a.ntiles || combo >= a.Cn) return false;
+    x.b = combo / a.Hkv;
+    x.g = combo % a.Hkv;
+    x.len = seq_len(a, x.b);
+    const int nr = a.n * a.G, vr = x.len * a.G;          // rows there are, rows of the sequence
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r0 = tile * RT, rw = r0 + wave * RW, r = rw + (threadIdx.x & 31);
+    x.in = r < nr;
+    x.valid = r < vr;
+    x.tok = min(r, nr - 1) / a.G;
+    x.head = x.g * a.G + min(r, nr - 1) % a.G;
+    // the workgroup's and the wave's tokens
+    const int t0 = r0 / a.G, t1 = (min(r0 + RT, vr) - 1) / a.G;
+    x.lo = max(0, t0 - a.W + 1);
+    x.hi = r0 < vr ? t1 + 1 : 0;
+    const int u0 = rw / a.G, u1 = (min(rw + RW, vr) - 1) / a.G;
+    x.w.S = a.S;
+    x.w.lo = max(0, x.tok - a.W + 1);
+    x.w.hi = x.valid ? x.tok + 1 : 0;
+    x.w.lo_min = max(0, u0 - a.W + 1);
+    x.w.lo_max = max(0, u1 - a.W + 1);
+    x.w.hi_min = u0 + 1;
+    x.w.hi_max = rw < vr ? u1 + 1 : 0;
+    return true;
+}
+
+template <int DT, int D>
+__device__ __forceinline__ void load_rows(const char *p, bool ok, typename Op<DT>::F (&f)[D / 16]) {
+    const int hf = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+        float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        f[ks] = ok ? Op<DT>::load(p + (16 * ks + 8 * hf) * Tile<DT, D>::ESZ) : Op<DT>::pack(z);
+    }
+}
+
+// A 32-column result, columns as rows of memory: registers 4g .. 4g+3 of block dt
+// are elements 32 dt + 8 g + 4 hf + 0..3.
+template <int DT, int D>
+__device__ __forceinline__ void store_rows(char *p, const f32x16 (&o)[D / 32], float f) {
+    const int hf = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int e = 32 * dt + 8 * g + 4 * hf;
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = o[dt][4 * g + i] * f;
+            if constexpr (DT == 1)
+                *reinterpret_cast<uint2 *>(p + 2 * e) = make_uint2(pk_bf16(x[0], x[1]), pk_bf16(x[2], x[3]));
+            else
+                *reinterpret_cast<float4 *>(p + 4 * e) = make_float4(x[0], x[1], x[2], x[3]);
+        }
+}
+
+template <int D> __device__ __forceinline__ bool any_bad(const f32x16 (&o)[D / 32]) {
+    float x = 0.0f;   // 0 * finite is 0, 0 * anything else NaN
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x = fmaf(0.0f, o[dt][r], x);
+    return !(x == 0.0f);
+}
+
+template <int DT, int D> __device__ __forceinline__ DenseKV<DT, D> keys(const Args &a, const Rows &x) {
+    DenseKV<DT, D> s;
+    s.k = a.k + x.b * a.ks[0] + x.g * a.ks[2];
+    s.v = a.v + x.b * a.vs[0] + x.g * a.vs[2];
+    s.kb = a.ks[1];
+    s.vb = a.vs[1];
+    s.last = max(x.len, 1) - 1;
+    return s;
+}
+
+template <int DT, int D> __global__ __launch_bounds__(64 * NW) void swa_fwd(const Args a) {
+    extern __shared__ __align__(16) char smem[];
+    constexpr int ESZ = Tile<DT, D>::ESZ;
+    Rows x;
+    if (!find_rows<D>(a, x)) return;
+    typename Op<DT>::F q[D / 16];
+    load_rows<DT, D>(a.q + x.b * a.qs[0] + x.tok * a.qs[1] + x.head * a.qs[2], x.valid, q);
+    const DenseKV<DT, D> src = keys<DT, D>(a, x);
+    int ns, wt0;
+    const int nt = tile_list(x.lo, x.hi, a.S, ns, wt0);
+    RowAcc<DT, D> acc;
+    float l, inv;
+    attend<DT, D, false>(src, smem, q, nullptr, a.c, 0, nt, ns, wt0, x.w, acc);
+    l = acc.l + other_half(acc.l);
+    if (__ballot(x.valid && (any_bad<D>(acc.O) || !finite(l)))) {
+        attend_each<DT, D, false>(src, q, nullptr, a.c, 0, nt, ns, wt0, x.w, acc);
+        l = acc.l + other_half(acc.l);
+    }
+    inv = x.valid ? 1.0f / l : 0.0f;
+    if (!x.in) return;
+    if (!x.valid) {   // a row behind its sequence: 0
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) acc.O[dt] = acc.O[dt] - acc.O[dt];
+    }
+    const int64_t row = ((int64_t)x.b * a.n + x.tok) * a.Hq + x.head;
+    store_rows<DT, D>(a.out + row * D * ESZ, acc.O, inv);
+    if (a.lse && (threadIdx.x & 32) == 0)
+        a.lse[((int64_t)x.b * a.Hq + x.head) * a.n + x.tok] = x.valid ? acc.m + __log2f(l) : INFINITY;
+}
+
+// The probabilities' gradient from the forward's log-sum-exps, and dq; delta =
+// do . o on the way, for dk and dv.
+template <int DT, int D> __global__ __launch_bounds__(64 * NW) void swa_dq(const Args a) {
+    extern __shared__ __align__(16) char smem[];
+    typedef Tile<DT, D> TL;
+    typedef typename Op<DT>::F F;
+    constexpr int ESZ = TL::ESZ, NKS = D / 16, NDT = D / 32;
+    const int lane = threadIdx.x & 63, hf = lane >> 5;
+    Rows x;
+    if (!find_rows<D>(a, x)) return;
+    F q[NKS], dO[NKS];
+    load_rows<DT, D>(a.q + x.b * a.qs[0] + x.tok * a.qs[1] + x.head * a.qs[2], x.valid, q);
+    load_rows<DT, D>(a.dout + x.b * a.dos[0] + x.tok * a.dos[1] + x.head * a.dos[2], x.valid, dO);
+    const int64_t row = ((int64_t)x.b * a.n + x.tok) * a.Hq + x.head;
+    const int64_t hrow = ((int64_t)x.b * a.Hq + x.head) * a.n + x.tok;
+    float delta = 0.0f;
+    {
+        F o[NKS];
+        load_rows<DT, D>(a.out + row * D * ESZ, x.valid, o);
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) {
+            float u[8], w[8];
+            Op<DT>::unpack(o[ks], u);
+            Op<DT>::unpack(dO[ks], w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) delta = fmaf(u[e], w[e], delta);
+        }
+        delta += other_half(delta);
+        if (x.valid && hf == 0) a.delta[hrow] = delta;
+    }
+    const float lse = x.valid ? a.lse[hrow] : INFINITY;
+    const DenseKV<DT, D> src = keys<DT, D>(a, x);
+    int ns, wt0;
+    const int nt = tile_list(x.lo, x.hi, a.S, ns, wt0);
+    const uint32_t lds = lds_offset(smem);
+    const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    f32x16 acc[NDT];
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) acc[dt] = zero;
+    if (nt > 0) src.stage(0 < ns ? 0 : wt0, lds);
+#pragma unroll 1
+    for (int it = 0; it < nt; ++it) {
+        wait_vm<0>();
+        __syncthreads();
+        const int cur = it & 1, nx = it + 1;
+        if (nx < nt) src.stage(nx < ns ? nx : wt0 + nx - ns, lds + (cur ^ 1) * src.BYTES);
+        const int j0 = (it < ns ? it : wt0 + it - ns) * KT;
+        if (j0 >= x.w.hi_max || (j0 + KT <= x.w.lo_min && j0 >= a.S)) continue;
+        const char *t = smem + cur * src.BYTES;
+        const bool whole = j0 + KT <= x.w.hi_min && (j0 >= x.w.lo_max || j0 + KT <= a.S);
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+            f32x16 s = zero, dp = zero;
+#pragma unroll
+            for (int ks = 0; ks < NKS; ++ks) {
+                s = Op<DT>::mma(src.kf(t, kt, ks, lane), q[ks], s);
+                dp = Op<DT>::mma(TL::row(t + KT * TL::ROWB, 32 * kt + (lane & 31), ks, hf), dO[ks], dp);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = ex2(fmaf(s[r], a.c, -lse)) * (dp[r] - delta);
+            if (!whole) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int j = j0 + 32 * kt + src.key(r, hf);
+                    if (!(j < x.w.hi && (j >= x.w.lo || j < a.S))) s[r] = 0.0f;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const F df = half16<DT>(s, u);
+#pragma unroll
+                for (int dt = 0; dt < NDT; ++dt)
+                    acc[dt] = Op<DT>::mma(TL::col(t, 32 * kt + 16 * u, dt, lane), df, acc[dt]);
+            }
+        }
+    }
+    if (__ballot(x.valid && any_bad<D>(acc))) {   // key by key, the masked ones left out
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) acc[dt] = zero;
+#pragma unroll 1
+        for (int it = 0; it < nt; ++it) {
+            const int j0 = (it < ns ? it : wt0 + it - ns) * KT;
+#pragma unroll 1
+            for (int j = j0; j < min(j0 + KT, x.w.hi_max); ++j) {
+                const char *kj = src.k + (int64_t)min(j, src.last) * src.kb;
+                const float s = dot_rows<DT, D>(q, kj, hf);
+                const float dp = dot_rows<DT, D>(dO, src.v + (int64_t)min(j, src.last) * src.vb, hf);
+                if (j < x.w.hi && (j >= x.w.lo || j < a.S))
+                    add_row<DT, D>(acc, kj, ex2(fmaf(s, a.c, -lse)) * (dp - delta), hf);
+            }
+        }
+    }
+    if (!x.in) return;
+    if (!x.valid) {
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) acc[dt] = zero;
+    }
+    store_rows<DT, D>(a.dq + row * D * ESZ, acc, a.scale);
+}
+
+constexpr int KB = 32 * NW;   // keys of a dk / dv workgroup
+constexpr int TT = 64;        // tokens of its steps
+
+// One past the last token that sees keys k0 .. k0 + KB - 1, and the steps over them.
+__device__ __forceinline__ int last_token(int k0, int len, int W, int S) {
+    return k0 < S ? len : min(len, k0 + KB - 1 + W);
+}
+__device__ __forceinline__ int steps(int k0, int len, int W, int S) {
+    return max(0, (last_token(k0, len, W, S) + TT - 1) / TT - k0 / TT);
+}
+
+// The workgroup's key tile and part of it: tiles of sinks first.
+__device__ __forceinline__ void find_part(const Args &a, int slot, int &tile, int &part) {
+    const int sinks = a.nst * a.Ps;
+    if (slot < sinks) {
+        tile = slot / a.Ps;
+        part = slot % a.Ps;
+    } else {
+        tile = a.nst + (slot - sinks) / a.Pn;
+        part = (slot - sinks) % a.Pn;
+    }
+}
+
+template <int DT, int D> __global__ __launch_bounds__(64 * NW) void swa_dkv(const Args a) {
+    extern __shared__ __align__(16) char smem[];
+    typedef Tile<DT, D> TL;
+    typedef typename Op<DT>::F F;
+    constexpr int ESZ = TL::ESZ, NKS = D / 16, NDT = D / 32, BYTES = 2 * TT * TL::ROWB + 2 * TT * 4;
+    const int lane = threadIdx.x & 63, hf = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int combo = blockIdx.x % a.Cn, slot = blockIdx.x / a.Cn;
+    int tile, part;
+    find_part(a, slot, tile, part);
+    const int b = combo / a.Hkv, g = combo % a.Hkv, len = seq_len(a, b);
+    const int k0 = tile * KB, kw = k0 + 32 * wave, j = kw + (lane & 31);
+    const int nst = steps(k0, len, a.W, a.S), all = nst * a.G;
+    const int parts = tile < a.nst ? a.Ps : a.Pn;
+    const int i0 = part * a.chunk, i1 = min(all, i0 + a.chunk);
+    if (i0 >= i1 && (parts > 1 || part > 0)) return;   // a part with nothing to sum is not read either
+    const bool valid = j < len;
+    F kf[NKS], vf[NKS];
+    load_rows<DT, D>(a.k + b * a.ks[0] + (int64_t)min(j, a.n - 1) * a.ks[1] + g * a.ks[2], valid, kf);
+    load_rows<DT, D>(a.v + b * a.vs[0] + (int64_t)min(j, a.n - 1) * a.vs[1] + g * a.vs[2], valid, vf);
+    const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    f32x16 dk[NDT], dv[NDT];
+    const uint32_t lds = lds_offset(smem);
+    const int last = max(len, 1) - 1;
+
+    auto stage = [&](int it, int buf) {
+        const int h = g * a.G + it / nst, t0 = (k0 / TT + it % nst) * TT;
+        const uint32_t to = lds + buf * BYTES;
+        TL::template stage<TT>(a.q + b * a.qs[0] + h * a.qs[2], a.qs[1], t0, last, to);
+        TL::template stage<TT>(a.dout + b * a.dos[0] + h * a.dos[2], a.dos[1], t0, last, to + TT * TL::ROWB);
+        float *ld = reinterpret_cast<float *>(smem + buf * BYTES + 2 * TT * TL::ROWB);
+        if (threadIdx.x < 2 * TT) {
+            const int t = min(t0 + ((int)threadIdx.x & (TT - 1)), last);
+            ld[threadIdx.x] = (threadIdx.x < TT ? a.lse : a.delta)[((int64_t)b * a.Hq + h) * a.n + t];
+        }
+    };
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) dk[dt] = dv[dt] = zero;
+    if (i0 < i1) stage(i0, 0);
+#pragma unroll 1
+    for (int it = i0; it < i1; ++it) {
+        wait_vm<0>();
+        __syncthreads();
+        const int cur = (it - i0) & 1;
+        if (it + 1 < i1) stage(it + 1, cur ^ 1);
+        const int t0 = (k0 / TT + it % nst) * TT;
+        if (t0 + TT <= kw || (t0 >= kw + 31 + a.W && kw >= a.S) || t0 >= len) continue;
+        const char *tq = smem + cur * BYTES, *td = tq + TT * TL::ROWB;
+        const float *ld = reinterpret_cast<const float *>(td + TT * TL::ROWB);
+        const bool whole = t0 >= kw + 31 && t0 + TT <= len && (t0 + TT <= kw + a.W || kw + 32 <= a.S);
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt) {
+            f32x16 s = zero, dp = zero;
+#pragma unroll
+            for (int ks = 0; ks < NKS; ++ks) {
+                s = Op<DT>::mma(TL::row(tq, 32 * rt + (lane & 31), ks, hf), kf[ks], s);
+                dp = Op<DT>::mma(TL::row(td, 32 * rt + (lane & 31), ks, hf), vf[ks], dp);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int tr = 32 * rt + 8 * (r >> 2) + 4 * hf + (r & 3);
+                s[r] = ex2(fmaf(s[r], a.c, -ld[tr]));
+                dp[r] = s[r] * (dp[r] - ld[TT + tr]);
+            }
+            if (!whole) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int t = t0 + 32 * rt + 8 * (r >> 2) + 4 * hf + (r & 3);
+                    if (!(t >= j && t < len && (t < j + a.W || j < a.S))) s[r] = dp[r] = 0.0f;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const F pf = half16<DT>(s, u), df = half16<DT>(dp, u);
+#pragma unroll
+                for (int dt = 0; dt < NDT; ++dt) {
+                    dv[dt] = Op<DT>::mma(TL::col(td, 32 * rt + 16 * u, dt, lane), pf, dv[dt]);
+                    dk[dt] = Op<DT>::mma(TL::col(tq, 32 * rt + 16 * u, dt, lane), df, dk[dt]);
+                }
+            }
+        }
+    }
+    if (__ballot(valid && (any_bad<D>(dk) || any_bad<D>(dv)))) {   // token by token, the masked ones left out
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) dk[dt] = dv[dt] = zero;
+#pragma unroll 1
+        for (int it = i0; it < i1; ++it) {
+            const int h = g * a.G + it / nst, t0 = (k0 / TT + it % nst) * TT;
+#pragma unroll 1
+            for (int t = t0; t < min(t0 + TT, len); ++t) {
+                const char *qt = a.q + b * a.qs[0] + t * a.qs[1] + h * a.qs[2];
+                const char *dt_ = a.dout + b * a.dos[0] + t * a.dos[1] + h * a.dos[2];
+                const int64_t at = ((int64_t)b * a.Hq + h) * a.n + t;
+                const float p = ex2(fmaf(dot_rows<DT, D>(kf, qt, hf), a.c, -a.lse[at]));
+                const float ds = p * (dot_rows<DT, D>(vf, dt_, hf) - a.delta[at]);
+                if (t >= j && (t < j + a.W || j < a.S)) {
+                    add_row<DT, D>(dv, dt_, p, hf);
+                    add_row<DT, D>(dk, qt, ds, hf);
+                }
+            }
+        }
+    }
+    if (parts > 1) {   // the sums as they are, for swa_join
+        const int64_t at = ((int64_t)combo * (a.nst * a.Ps + (a.ntiles - a.nst) * a.Pn) + slot) * KB + 32 * wave +
+                           (lane & 31);
+        store_rows<0, D>(reinterpret_cast<char *>(a.part + at * 2 * D), dk, 1.0f);
+        store_rows<0, D>(reinterpret_cast<char *>(a.part + at * 2 * D + D), dv, 1.0f);
+        return;
+    }
+    if (j >= a.n) return;
+    if (!valid) {
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) dk[dt] = dv[dt] = zero;
+    }
+    const int64_t row = (((int64_t)b * a.n + j) * a.Hkv + g) * D * ESZ;
+    store_rows<DT, D>(a.dk + row, dk, a.scale);
+    store_rows<DT, D>(a.dv + row, dv, 1.0f);
+}
+
+// dk and dv of the tiles in several parts: the parts' sums, in order.  One
+// workgroup per key tile and KV head; 4 elements per thread and pass.
+template <int DT, int D> __global__ __launch_bounds__(256) void swa_join(const Args a, int first) {
+    typedef typename St<DT>::T T;
+    const int combo = blockIdx.x % a.Cn, tile = first + blockIdx.x / a.Cn;
+    const int b = combo / a.Hkv, g = combo % a.Hkv, len = seq_len(a, b), k0 = tile * KB;
+    const int P = tile < a.nst ? a.Ps : a.Pn;
+    const int used = min(P, (steps(k0, len, a.W, a.S) * a.G + a.chunk - 1) / a.chunk);
+    const int slot = tile < a.nst ? tile * a.Ps : a.nst * a.Ps + (tile - a.nst) * a.Pn;
+    const int64_t slots = a.nst * a.Ps + (a.ntiles - a.nst) * a.Pn;
+    const float *base = a.part + ((int64_t)combo * slots + slot) * KB * 2 * D;
+    for (int e = threadIdx.x * 4; e < KB * 2 * D; e += 1024) {
+        const int r = e / (2 * D), x = e % (2 * D), j = k0 + r;
+        if (j >= a.n) break;
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+        if (j < len)
+            for (int p = 0; p < used; ++p)
+                sum = sum + *reinterpret_cast<const f32x4 *>(base + (int64_t)p * KB * 2 * D + e);
+        const float f = x < D ? a.scale : 1.0f;
+        T *to = reinterpret_cast<T *>(x < D ? a.dk : a.dv) + (((int64_t)b * a.n + j) * a.Hkv + g) * D + x % D;
+        if constexpr (DT == 1)
+            *reinterpret_cast<uint2 *>(to) = make_uint2(pk_bf16(sum[0] * f, sum[1] * f), pk_bf16(sum[2] * f, sum[3] * f));
+        else
+            *reinterpret_cast<f32x4 *>(to) = sum * f;
+    }
+}
+
+// How dk and dv are cut: steps of a part, so that some 1024 workgroups share the
+// work, never more than a tile without sinks takes.
+struct Cut {
+    int ntiles, nst, Ps, Pn, chunk;
+    int64_t slots;
+};
+static Cut cut(int64_t Cn, int64_t n, int64_t G, int64_t W, int64_t S) {
+    Cut c;
+    c.ntiles = (int)((n + KB - 1) / KB);
+    c.nst = (int)((S < n ? S : n) + KB - 1) / KB;
+    const int64_t most = G * ((n + TT - 1) / TT);                     // steps of a tile of sinks
+    int64_t usual = G * ((KB + W - 1 + TT - 1) / TT + 1);             // of another
+    if (usual > most) usual = most;
+    const int64_t total = Cn * (c.nst * most + (c.ntiles - c.nst) * usual);
+    int64_t ch = (total + 1023) / 1024;
+    if (ch < 8) ch = 8;
+    if (ch > usual) ch = usual;
+    c.chunk = (int)ch;
+    c.Ps = (int)((most + ch - 1) / ch);
+    c.Pn = (int)((usual + ch - 1) / ch);
+    c.slots = (int64_t)c.nst * c.Ps + (int64_t)(c.ntiles - c.nst) * c.Pn;
+    return c;
+}
+
+template <int DT, int D, class K> static int lds_room(K kern, size_t bytes) {
+    if (bytes <= 65536) return HBA_OK;
+    return hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
+                               (int)bytes) == hipSuccess
+               ? HBA_OK
+               : HBA_ERR_LAUNCH;
+}
+
+template <int DT, int D> static int launch_fwd(const Args &a, int64_t grid, hipStream_t s) {
+    constexpr size_t lds = 2 * DenseKV<DT, D>::BYTES;
+    if (int st = lds_room<DT, D>(swa_fwd<DT, D>, lds)) return st;
+    hipLaunchKernelGGL((swa_fwd<DT, D>), dim3((unsigned)grid), dim3(64 * NW), lds, s, a);
+    HBA_LAUNCH_CHECK();
+    return HBA_OK;
+}
+
+template <int DT, int D> static int launch_bwd(Args a, int64_t grid, const Cut &c, hipStream_t s) {
+    constexpr size_t lds = 2 * DenseKV<DT, D>::BYTES, ldk = lds + 2 * 2 * TT * 4;
+    if (int st = lds_room<DT, D>(swa_dq<DT, D>, lds)) return st;
+    if (int st = lds_room<DT, D>(swa_dkv<DT, D>, ldk)) return st;
+    hipLaunchKernelGGL((swa_dq<DT, D>), dim3((unsigned)grid), dim3(64 * NW), lds, s, a);
+    HBA_LAUNCH_CHECK();
+    a.ntiles = c.ntiles;
+    hipLaunchKernelGGL((swa_dkv<DT, D>), dim3((unsigned)(c.slots * a.Cn)), dim3(64 * NW), ldk, s, a);
+    HBA_LAUNCH_CHECK();
+    const int first = c.Ps > 1 ? 0 : c.nst, end = c.Pn > 1 ? c.ntiles : c.nst;
+    if (first < end) {
+        hipLaunchKernelGGL((swa_join<DT, D>), dim3((unsigned)((end - first) * a.Cn)), dim3(256), 0, s, a, first);
+        HBA_LAUNCH_CHECK();
+    }
+    return HBA_OK;
+}
+
+static void set_strides(int64_t (&to)[3], const int64_t *from, int64_t esz) {
+    for (int i = 0; i < 3; ++i) to[i] = from[i] * esz;
+}
+
+static int check(int dtype, int64_t B, int64_t n, int64_t Hq, int64_t Hkv, int64_t d, int64_t W, int64_t S,
+                 float scale) {
+    if (int st = abi::check_dtype_dim(dtype, d)) return st;
+    if (B <= 0 || n <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || W < 1 || S < 0) return HBA_ERR_INVALID_ARG;
+    if (!(scale > 0.0f) || !(scale < INFINITY)) return HBA_ERR_INVALID_ARG;
+    // rows, steps and workgroups are counted in 32 bits
+    if (n > (1 << 28) || n * (Hq / Hkv) > 0x7fffff00 || B * Hq * ((n + 31) / 32 + 8) > 0x7fffffff)
+        return HBA_ERR_UNSUPPORTED;
+    return HBA_OK;
+}
+
+}  // namespace swa
+}  // namespace hba
+
+using namespace hba;
+
+extern "C" int hba_swa_fwd(int dtype, const void *q, const int64_t q_strides[3], const void *k,
+                           const int64_t k_strides[3], const void *v, const int64_t v_strides[3],
+                           const int32_t *lens, int64_t B, int64_t n, int64_t Hq, int64_t Hkv, int64_t d, int64_t W,
+                           int64_t S, float scale, void *out, float *lse, void *stream) {
+    if (int st = swa::check(dtype, B, n, Hq, Hkv, d, W, S, scale)) return st;
+    if (!q || !k || !v || !q_strides || !k_strides || !v_strides || !out) return HBA_ERR_INVALID_ARG;
+    if (!abi::rows_aligned(dtype, q, q_strides) || !abi::rows_aligned(dtype, k, k_strides) ||
+        !abi::rows_aligned(dtype, v, v_strides) || !abi::aligned16(out))
+        return HBA_ERR_UNSUPPORTED;
+    const int64_t e = abi::elem_size(dtype);
+    swa::Args a = {};
+    a.q = (const char *)q;
+    a.k = (const char *)k;
+    a.v = (const char *)v;
+    swa::set_strides(a.qs, q_strides, e);
+    swa::set_strides(a.ks, k_strides, e);
+    swa::set_strides(a.vs, v_strides, e);
+    a.lens = lens;
+    a.n = (int)n;
+    a.Hq = (int)Hq;
+    a.Hkv = (int)Hkv;
+    a.G = (int)(Hq / Hkv);
+    a.W = (int)(W < n ? W : n);
+    a.S = (int)(S < n ? S : n);
+    a.scale = scale;
+    a.c = scale * rows::LOG2E;
+    a.Cn = (int)(B * Hkv);
+    a.ntiles = (int)((n * a.G + rows::RT - 1) / rows::RT);
+    int64_t grid;
+    a.xmap = xcd_pick(a.Cn, a.ntiles, grid);
+    a.out = (char *)out;
+    a.lse = lse;
+    int st = HBA_OK;
+#define HBA_SWA(DT, D) st = swa::launch_fwd<DT, D>(a, grid, (hipStream_t)stream)
+    HBA_DISPATCH_DT_D(dtype, d, HBA_SWA);
+#undef HBA_SWA
+    return st;
+}
+
+extern "C" int hba_swa_bwd_workspace_bytes(int64_t B, int64_t n, int64_t Hq, int64_t Hkv, int64_t d, int64_t W,
+                                           int64_t S, size_t *bytes) {
+    if (!bytes) return HBA_ERR_INVALID_ARG;
+    if (int st = swa::check(HBA_DTYPE_F32, B, n, Hq, Hkv, d, W, S, 1.0f)) return st;
+    if (W > n) W = n;
+    if (S > n) S = n;
+    const swa::Cut c = swa::cut(B * Hkv, n, Hq / Hkv, W, S);
+    const size_t delta = ((size_t)(B * Hq * n) * 4 + 255) / 256 * 256;
+    const size_t part = c.Ps > 1 || c.Pn > 1 ? (size_t)(B * Hkv) * c.slots * swa::KB * 2 * d * 4 : 0;
+    *bytes = delta + part;
+    return HBA_OK;
+}
+
+extern "C" int hba_swa_bwd(int dtype, const void *q, const int64_t q_strides[3], const void *k,
+                           const int64_t k_strides[3], const void *v, const int64_t v_strides[3], const void *out,
+                           const float *lse, const void *dout, const int64_t dout_strides[3], const int32_t *lens,
+                           int64_t B, int64_t n, int64_t Hq, int64_t Hkv, int64_t d, int64_t W, int64_t S,
+                           float scale, void *workspace, size_t ws_bytes, void *dq, void *dk, void *dv,
+                           void *stream) {
+    if (int st = swa::check(dtype, B, n, Hq, Hkv, d, W, S, scale)) return st;
+    if (!q || !k || !v || !q_strides || !k_strides || !v_strides || !out || !lse || !dout || !dout_strides ||
+        !workspace || !dq || !dk || !dv)
+        return HBA_ERR_INVALID_ARG;
+    size_t need = 0;
+    if (int st = hba_swa_bwd_workspace_bytes(B, n, Hq, Hkv, d, W, S, &need)) return st;
+    if (ws_bytes < need) return HBA_ERR_INVALID_ARG;
+    if (!abi::rows_aligned(dtype, q, q_strides) || !abi::rows_aligned(dtype, k, k_strides) ||
+        !abi::rows_aligned(dtype, v, v_strides) || !abi::rows_aligned(dtype, dout, dout_strides) ||
+        !abi::aligned16(out) || !abi::aligned16(dq) || !abi::aligned16(dk) || !abi::aligned16(dv) ||
+        !abi::aligned16(workspace))
+        return HBA_ERR_UNSUPPORTED;
+    const int64_t e = abi::elem_size(dtype);
+    swa::Args a = {};
+    a.q = (const char *)q;
+    a.k = (const char *)k;
+    a.v = (const char *)v;
+    a.dout = (const char *)dout;
+    swa::set_strides(a.qs, q_strides, e);
+    swa::set_strides(a.ks, k_strides, e);
+    swa::set_strides(a.vs, v_strides, e);
+    swa::set_strides(a.dos, dout_strides, e);
+    a.lens = lens;
+    a.n = (int)n;
+    a.Hq = (int)Hq;
+    a.Hkv = (int)Hkv;
+    a.G = (int)(Hq / Hkv);
+    a.W = (int)(W < n ? W : n);
+    a.S = (int)(S < n ? S : n);
+    a.scale = scale;
+    a.c = scale * rows::LOG2E;
+    a.Cn = (int)(B * Hkv);
+    a.ntiles = (int)((n * a.G + rows::RT - 1) / rows::RT);
+    int64_t grid;
+    a.xmap = xcd_pick(a.Cn, a.ntiles, grid);
+    a.out = (char *)const_cast<void *>(out);
+    a.lse = const_cast<float *>(lse);
+    a.delta = (float *)workspace;
+    a.part = (float *)((char *)workspace + ((size_t)(B * Hq * n) * 4 + 255) / 256 * 256);
+    a.dq = (char *)dq;
+    a.dk = (char *)dk;
+    a.dv = (char *)dv;
+    const swa::Cut c = swa::cut(a.Cn, n, a.G, a.W, a.S);
+    a.nst = c.nst;
+    a.Ps = c.Ps;
+    a.Pn = c.Pn;
+    a.chunk = c.chunk;
+    if (c.slots * a.Cn > 0x7fffffff) return HBA_ERR_UNSUPPORTED;
+    int st = HBA_OK;
+#define HBA_SWA(DT, D) st = swa::launch_bwd<DT, D>(a, grid, c, (hipStream_t)stream)
+    HBA_DISPATCH_DT_D(dtype, d, HBA_SWA);
+#undef HBA_SWA
+    return st;
+}

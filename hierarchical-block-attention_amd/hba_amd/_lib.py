@@ -66,6 +66,11 @@ SIGNATURES = {
                        _vp, _vp, _vp, _vp],
     "hba_decode_fwd_noalloc": [_i, _vp, _vp, _f, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64,
                                _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp],
+    "hba_swa_fwd": [_i, _vp, _c_i64p, _vp, _c_i64p, _vp, _c_i64p, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f,
+                    _vp, _vp, _vp],
+    "hba_swa_bwd_workspace_bytes": [_i64, _i64, _i64, _i64, _i64, _i64, _i64, ctypes.POINTER(ctypes.c_size_t)],
+    "hba_swa_bwd": [_i, _vp, _c_i64p, _vp, _c_i64p, _vp, _c_i64p, _vp, _vp, _vp, _c_i64p, _vp, _i64, _i64, _i64,
+                    _i64, _i64, _i64, _i64, _f, _vp, ctypes.c_size_t, _vp, _vp, _vp, _vp],
 }
 
 _LIB = None
@@ -103,3 +108,8 @@ _I64X3 = ctypes.c_int64 * 3
 def strides3(t):
     """First three strides (elements) of a 4-D [B, n, H, d] view as a ctypes array."""
     return _I64X3(*t.stride()[:3])
+
+
+def used_strides3(t):
+    """strides3 with 0 for dims of one element, whose stride no address uses."""
+    return _I64X3(*(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape)))

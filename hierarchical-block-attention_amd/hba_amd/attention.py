@@ -250,6 +250,39 @@ def equiv_attention(q, k, v, cos, sin, cfg, qkn):
     return ops.attn_fwd(q, qg, kg, qeps, kc, kr, vt, cos, sin, idx, cnt, 0, n, scale)
 
 
+class _Sliding(torch.autograd.Function):
+    """sliding_attention with hba_swa_bwd behind it."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, lens, window, sinks, scale):
+        out, lse = ops._swa_fwd(q, k, v, lens, window, sinks, scale)
+        ctx.save_for_backward(q, k, v, out, lse, lens)
+        ctx.meta = (window, sinks, scale)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse, lens = ctx.saved_tensors
+        return (*ops._swa_bwd(q, k, v, out, lse, dout, lens, *ctx.meta), None, None, None, None)
+
+
+def sliding_attention(q, k, v, window, sinks=0, scale=None, lens=None):
+    """Sliding-window attention with sinks, the attention of a model's window
+    layers: query i of q [B, n, Hq, d] attends to the keys j <= i with
+    j > i - window or j < sinks, of k, v [B, n, Hkv, d] (query head h uses KV
+    head h / (Hq / Hkv)).  Queries and keys enter as they are: any norm or
+    rotation is the caller's.  Any n, any strides; float32 or bfloat16, head
+    dim 64 or 128.  scale: of the logits, positive (default d ** -0.5).  lens
+    [B]: rows at and past lens[b] are padding, whose output and gradients are
+    0.  Returns a new tensor of q's shape and dtype; differentiable in q, k
+    and v, with gradients that are the same bits from run to run."""
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _Sliding.apply(q, k, v, lens, int(window), int(sinks), scale)
+    return ops._swa_fwd(q, k, v, lens, int(window), int(sinks), scale)[0]
+
+
 def hba_attention_eval(q, k, v, cos, sin, cfg, summ, qkn, cap=None, hier=False, equiv=False):
     """Gathered union attention with flat or hierarchical selection; `cap`
     (the reference's memory cap for its chunk loop) is accepted and unused.

@@ -18,6 +18,8 @@ device.
     hba::summarize_pages  summaries of listed pages (mutates summ_pages)
     hba::summarize_filled summaries of the pages the last append filled (mutates summ_pages)
     hba::decode_fwd       decode step over the paged cache
+    hba::swa_fwd          sliding-window attention with sinks, forward
+    hba::swa_bwd          its backward (dq, dk, dv)
 """
 import ctypes
 from typing import Optional, Tuple
@@ -25,7 +27,7 @@ from typing import Optional, Tuple
 import torch
 from torch import Tensor
 
-from ._lib import BF16, F32, check, lib, strides3
+from ._lib import BF16, F32, check, lib, strides3, used_strides3
 
 BLOCK = 64
 _DT = {torch.float32: F32, torch.bfloat16: BF16}
@@ -548,6 +550,113 @@ def attn_bwd(q: Tensor, k: Tensor, v: Tensor, kc: Tensor, kr: Tensor, q_gain: Op
 def _(q, k, v, kc, kr, q_gain, k_gain, eps, cos, sin, idx, cnt, out, dout, sinks, window, scale, block=64):
     return (q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape),
             q.new_empty(q.shape[2], dtype=torch.float32), k.new_empty(k.shape[2], dtype=torch.float32))
+
+
+# -------------------------------------------------- sliding-window attention ----
+def _rows16(t):
+    """t, or a copy of it, with a contiguous last dim and rows on 16-byte boundaries."""
+    q = 16 // t.element_size()
+    st, sz = t.stride(), t.shape
+    if (st[-1] == 1 and t.data_ptr() % 16 == 0
+            and all(s % q == 0 or n == 1 for s, n in zip(st[:-1], sz[:-1]))):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _swa_args(q, k, v, lens, window, sinks, scale):
+    """Checks the arguments of swa_fwd / swa_bwd; returns (device, B, n, Hq, Hkv, d, lens)."""
+    dev = _dev(q)
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError("q, k and v: expected [B, n, H, d] tensors")
+    B, n, Hq, d = q.shape
+    Hkv = k.shape[2]
+    if k.shape[0] != B or k.shape[1] != n or k.shape[3] != d or v.shape != k.shape or Hkv == 0 or Hq % Hkv:
+        raise ValueError(f"k {tuple(k.shape)} / v {tuple(v.shape)} do not match q {tuple(q.shape)}")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError("q, k and v must share one dtype")
+    if k.device != dev or v.device != dev:
+        raise ValueError(f"q, k and v must be on one device ({dev})")
+    if window < 1 or sinks < 0:
+        raise ValueError(f"window must be at least 1 and sinks at least 0, got {window} and {sinks}")
+    if not 0.0 < scale < float("inf"):
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if lens is not None:
+        if tuple(lens.shape) != (B,) or lens.dtype.is_floating_point or lens.dtype == torch.bool:
+            raise ValueError(f"lens: expected {B} whole numbers")
+        lens = lens.to(device=dev, dtype=torch.int32).contiguous()
+    return dev, B, n, Hq, Hkv, d, lens
+
+
+def _swa_fwd(q, k, v, lens, window, sinks, scale):
+    dev, B, n, Hq, Hkv, d, lens = _swa_args(q, k, v, lens, window, sinks, scale)
+    code = _code(q)
+    out = torch.empty(B, n, Hq, d, dtype=q.dtype, device=dev)
+    lse = torch.empty(B, Hq, n, dtype=torch.float32, device=dev)
+    if out.numel() == 0:
+        return out, lse
+    q, k, v = _rows16(q), _rows16(k), _rows16(v)
+    with _on(dev):
+        st = lib().hba_swa_fwd(code, _p(q), used_strides3(q), _p(k), used_strides3(k), _p(v), used_strides3(v),
+                               _p(lens), B, n, Hq, Hkv, d, min(window, n), min(sinks, n), scale, _p(out), _p(lse),
+                               _stream(dev))
+    check(st, "hba_swa_fwd")
+    return out, lse
+
+
+def _swa_bwd(q, k, v, out, lse, dout, lens, window, sinks, scale):
+    dev, B, n, Hq, Hkv, d, lens = _swa_args(q, k, v, lens, window, sinks, scale)
+    code = _code(q)
+    if out.shape != q.shape or dout.shape != q.shape or tuple(lse.shape) != (B, Hq, n):
+        raise ValueError("out, dout and lse do not match q")
+    if out.dtype != q.dtype or dout.dtype != q.dtype or lse.dtype != torch.float32:
+        raise TypeError("out and dout must have q's dtype, lse float32")
+    if out.device != dev or dout.device != dev or lse.device != dev:
+        raise ValueError(f"out, dout and lse must be on {dev}")
+    dq = torch.empty(B, n, Hq, d, dtype=q.dtype, device=dev)
+    dk = torch.empty(B, n, Hkv, d, dtype=q.dtype, device=dev)
+    dv = torch.empty_like(dk)
+    if dq.numel() == 0:
+        return dq, dk, dv
+    W, S = min(window, n), min(sinks, n)
+    q, k, v, dout, out, lse = _rows16(q), _rows16(k), _rows16(v), _rows16(dout), _c16(out), lse.contiguous()
+    nbytes = ctypes.c_size_t(0)
+    check(lib().hba_swa_bwd_workspace_bytes(B, n, Hq, Hkv, d, W, S, ctypes.byref(nbytes)),
+          "hba_swa_bwd_workspace_bytes")
+    ws = torch.empty(int(nbytes.value), dtype=torch.uint8, device=dev)
+    with _on(dev):
+        st = lib().hba_swa_bwd(code, _p(q), used_strides3(q), _p(k), used_strides3(k), _p(v), used_strides3(v),
+                               _p(out), _p(lse), _p(dout), used_strides3(dout), _p(lens), B, n, Hq, Hkv, d, W, S,
+                               scale, _p(ws), int(nbytes.value), _p(dq), _p(dk), _p(dv), _stream(dev))
+    check(st, "hba_swa_bwd")
+    return dq, dk, dv
+
+
+@torch.library.custom_op("hba::swa_fwd", mutates_args=(), device_types="cuda")
+def swa_fwd(q: Tensor, k: Tensor, v: Tensor, lens: Optional[Tensor], window: int, sinks: int,
+            scale: float) -> Tuple[Tensor, Tensor]:
+    """Attention of q [B, n, Hq, d] to the keys j <= i with j > i - window or
+    j < sinks (k, v [B, n, Hkv, d]): (out, lse), lse fp32 [B, Hq, n] in units
+    of log2.  lens int32 [B]: rows at and past lens[b] are padding (out 0)."""
+    return _swa_fwd(q, k, v, lens, window, sinks, scale)
+
+
+@swa_fwd.register_fake
+def _(q, k, v, lens, window, sinks, scale):
+    B, n, Hq, d = q.shape
+    return q.new_empty(B, n, Hq, d), q.new_empty(B, Hq, n, dtype=torch.float32)
+
+
+@torch.library.custom_op("hba::swa_bwd", mutates_args=(), device_types="cuda")
+def swa_bwd(q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor, dout: Tensor, lens: Optional[Tensor],
+            window: int, sinks: int, scale: float) -> Tuple[Tensor, Tensor, Tensor]:
+    """dq, dk, dv of swa_fwd from its inputs, its out and lse and the output's
+    cotangent dout; the same bits from run to run."""
+    return _swa_bwd(q, k, v, out, lse, dout, lens, window, sinks, scale)
+
+
+@swa_bwd.register_fake
+def _(q, k, v, out, lse, dout, lens, window, sinks, scale):
+    return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
 
 
 # ---------------------------------------------------------------- decode ----

@@ -490,6 +490,45 @@ int hba_attn_bwd_workspace_full_bytes(int dtype, int64_t B, int64_t n, int64_t H
  * Hkv <= Hq (for callers that size one workspace for any call). */
 int hba_attn_bwd_workspace_size(int64_t B, int64_t n, int64_t Hq, int64_t d, size_t *bytes);
 
+/*
+ * Sliding-window attention with sinks (a model's window layers): query i of
+ * q [B, n, Hq, d] attends to the keys j <= i with j > i - W or j < S of k, v
+ * [B, n, Hkv, d], all with element strides (rows on 16-byte boundaries).
+ * Queries and keys enter as they are (no norm, no rotation).  Any n >= 1, any
+ * Hq / Hkv, d = 64 or 128, W >= 1, S >= 0, scale > 0.  lens int32 [B] (NULL: n
+ * each; values are clamped to 0 .. n): rows at and past lens[b] are padding,
+ * whose out is 0; their q, k and v are not used and may hold anything.  out
+ * [B, n, Hq, d] contiguous; lse (NULL to skip) fp32 [B, Hq, n]: log2 of the sum
+ * of 2^(log2(e) scale q.k) over the keys a row sees, +inf for padding.  A NaN
+ * or infinity of a key or value that a row does not see has no effect on it.
+ * bf16: products on bf16 matrix cores, the probabilities rounded to bf16, sums
+ * in fp32.  No counterpart in the reference.
+ */
+int hba_swa_fwd(int dtype, const void *q, const int64_t q_strides[3], const void *k,
+                const int64_t k_strides[3], const void *v, const int64_t v_strides[3],
+                const int32_t *lens, int64_t B, int64_t n, int64_t Hq, int64_t Hkv, int64_t d,
+                int64_t W, int64_t S, float scale, void *out, float *lse, void *stream);
+
+/* Scratch bytes of hba_swa_bwd: <dout, out> of every row (fp32 [B, Hq, n]) and
+ * the partial sums of dk and dv where key tiles are cut into parts. */
+int hba_swa_bwd_workspace_bytes(int64_t B, int64_t n, int64_t Hq, int64_t Hkv, int64_t d,
+                                int64_t W, int64_t S, size_t *bytes);
+
+/*
+ * Gradients of hba_swa_fwd: dq [B, n, Hq, d], dk, dv [B, n, Hkv, d] (contiguous,
+ * storage dtype, overwritten; 0 in padding) from its inputs, its out
+ * (contiguous) and lse, and the cotangent dout (element strides).  workspace:
+ * 16-byte aligned, no initial contents.  Every sum runs in a fixed order, so
+ * the gradients are the same bits from run to run.  bf16: the probabilities
+ * and their gradients enter the products rounded to bf16, sums in fp32.
+ */
+int hba_swa_bwd(int dtype, const void *q, const int64_t q_strides[3], const void *k,
+                const int64_t k_strides[3], const void *v, const int64_t v_strides[3],
+                const void *out, const float *lse, const void *dout,
+                const int64_t dout_strides[3], const int32_t *lens, int64_t B, int64_t n,
+                int64_t Hq, int64_t Hkv, int64_t d, int64_t W, int64_t S, float scale,
+                void *workspace, size_t ws_bytes, void *dq, void *dk, void *dv, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
