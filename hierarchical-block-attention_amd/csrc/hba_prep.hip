@@ -8,6 +8,8 @@
 //   kv_append        decode-cache append (no reference counterpart)
 //   kv_append_advance  the decode loop's append: token, page summary when it
 //                    fills a page, seq_lens += 1 and the new length's scale
+//   kv_append_ragged any number of tokens per sequence, and the summaries of
+//                    every page they fill
 //
 // All of these are HBM-bound elementwise / tiny-GEMM work: one thread per key
 // row (prep), d/8 lanes per key row (append), one workgroup per 64-key block
@@ -15,6 +17,7 @@
 #include "hba_common.h"
 #include "hba_abi.h"
 #include "hba_generic.h"
+#include "hba_ragged.h"
 
 namespace hba {
 
@@ -581,6 +584,154 @@ __global__ __launch_bounds__(256) void kv_append_advance_kernel(
     }
 }
 
+// ---------------------------------------------------------- ragged append --
+struct RaggedArgs {
+    const char *k, *v;              // [T, Hkv, D]; byte strides of token and head
+    int64_t kst, ksh, vst, vsh;
+    const int32_t *cu;
+    int T, Bd, Hkv, maxp, m;
+    const float *kgain, *cosT, *sinT, *probes, *proj;
+    float eps, att_scale;
+    int64_t n_tab, pages;
+    const int32_t *ptab, *lens;
+    char *kc, *kr, *vp, *summ;      // kc, summ may be nullptr
+};
+
+// Tokens of sequence s that are appended: positions first .. last - 1, token i of
+// them at place c0 + i of the batch.  Positions outside the page table or past
+// the rotation tables, or below 0 (a length below the token count) are not.
+struct NewTokens {
+    int c0, first, last;
+};
+__device__ __forceinline__ NewTokens new_tokens(const RaggedArgs &a, int s) {
+    NewTokens x;
+    const int n = ragged::tokens(a.cu, s, a.T, x.c0);
+    const int64_t most = min((int64_t)a.maxp * 64, a.n_tab), L = a.lens[s];
+    int64_t first = L - n;
+    if (first < 0) {
+        x.c0 -= (int)max(first, -(int64_t)n);
+        first = 0;
+    }
+    x.first = (int)min(first, most);
+    x.last = (int)max((int64_t)x.first, min(L, most));
+    return x;
+}
+
+// One workgroup per (page that gets tokens, KV head): D/8 lanes a row as in
+// prep_tile (the same chain for the norm, so kc has the bits of every other way
+// to append it), 256 / (D/8) rows at a time.  kr is rounded once, from the
+// normalised key in fp32.  The values go through LDS, so that a page's 8-token
+// chunks are written whole where the batch has all 8.  The page's summaries
+// follow when its last token is among the new ones (the earlier keys are read
+// back: no other workgroup writes this page).
+// HBM-bound: k and v read once, kc, kr and v written once.
+template <int DT, int D, bool SUMM>
+__global__ __launch_bounds__(256) void kv_append_ragged_kernel(const RaggedArgs a) {
+    using T = typename St<DT>::T;
+    constexpr int TPH = D / 8, RPP = 256 / TPH, ESZ = DT == 1 ? 2 : 4, VS = 64 + 16 / ESZ;
+    __shared__ __align__(16) T vs[D][VS];
+    __shared__ SummSmem<SUMM ? D : 1, false> sm;
+    const int tid = threadIdx.x, g = blockIdx.y;
+    int slot;
+    const int s = ragged::find(blockIdx.x, a.Bd, [&](int i) {
+        const NewTokens x = new_tokens(a, i);
+        return x.last > x.first ? (x.last - 1) / 64 - x.first / 64 + 1 : 0;
+    }, slot);
+    if (s < 0) return;
+    const NewTokens x = new_tokens(a, s);
+    const int lp = x.first / 64 + slot, p0 = lp * 64;
+    const int ja = max(x.first - p0, 0), jb = min(x.last - p0, 64);   // the page's new tokens
+    const int64_t page = a.ptab[(int64_t)s * a.maxp + lp];
+    if (page < 0 || page >= a.pages) return;                          // not a page of this cache
+    const int64_t base = (page * a.Hkv + g) * 64 * D;
+    T *kcp = reinterpret_cast<T *>(a.kc) + base, *krp = reinterpret_cast<T *>(a.kr) + base;
+    T *vp = reinterpret_cast<T *>(a.vp) + base;
+    const bool fills = SUMM && jb == 64;
+    const int jl = tid % TPH, t0 = 8 * jl;
+    const bool lo = t0 < D / 2;
+    const float gn = a.kgain ? a.kgain[g] : 0.0f;
+#pragma unroll
+    for (int pass = 0; pass < 64 / RPP; ++pass) {
+        const int j = pass * RPP + tid / TPH;
+        if (pass * RPP >= jb || pass * RPP + RPP <= ja) continue;     // uniform
+        const bool act = j >= ja && j < jb;
+        const int64_t tok = x.c0 + (p0 + (act ? j : ja) - x.first), pos = p0 + (act ? j : ja);
+        float y[8], vv[8];
+        load8<DT>(reinterpret_cast<const T *>(a.k + tok * a.kst + g * a.ksh) + t0, y);
+        load8<DT>(reinterpret_cast<const T *>(a.v + tok * a.vst + g * a.vsh) + t0, vv);
+        if (a.kgain) {
+            float run = 0.0f;
+#pragma unroll
+            for (int step = 0; step < TPH; ++step) {
+                const float in = __builtin_bit_cast(
+                    float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, run), 0x111, 0xf, 0xf, false));
+                if (jl == step) {
+                    float c = (jl == 0) ? 0.0f : in;
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) c = fmaf(y[u], y[u], c);
+                    run = c;
+                }
+            }
+            const float ss = __shfl(run, (tid & 63) | (TPH - 1), 64);   // the row's last lane
+            float ms = ss / (float)D;
+            if (ms < a.eps) ms = a.eps;
+            const float rr = sqrtf(ms);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) y[u] = (y[u] / rr) * gn;
+        }
+        float cs[8], sn[8], z[8];
+        load8<0>(a.cosT + pos * D + t0, cs);
+        load8<0>(a.sinT + pos * D + t0, sn);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const float part = __shfl_xor(y[u], TPH / 2, 64);
+            z[u] = y[u] * cs[u] + (lo ? -part : part) * sn[u];
+        }
+        if (act) {
+            const int64_t o = page_key_off(j, t0, D);
+            if (a.kc) store8<DT>(kcp + o, y);
+            store8<DT>(krp + o, z);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) St<DT>::st(&vs[t0 + u][0], j, vv[u]);
+            if constexpr (SUMM)
+                if (fills)
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) sm.kb[j][t0 + u] = St<DT>::rnd(y[u]);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int c = tid; c < 8 * D; c += 256) {
+        int t, j0;
+        page_val_chunk(c, t, j0);
+        if (j0 >= ja && j0 + 8 <= jb) {
+            if constexpr (DT == 1) {
+                *reinterpret_cast<uint4 *>(vp + 8 * c) = *reinterpret_cast<const uint4 *>(&vs[t][j0]);
+            } else {
+                reinterpret_cast<float4 *>(vp + 8 * c)[0] = *reinterpret_cast<const float4 *>(&vs[t][j0]);
+                reinterpret_cast<float4 *>(vp + 8 * c)[1] = *reinterpret_cast<const float4 *>(&vs[t][j0 + 4]);
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if (j0 + u >= ja && j0 + u < jb) vp[8 * c + u] = vs[t][j0 + u];
+        }
+    }
+    if constexpr (SUMM) {
+        if (!fills) return;
+        for (int c = tid; c < 8 * D; c += 256) {   // the keys that were there
+            int j, e0;
+            page_key_chunk(c, D, j, e0);
+            if (j >= ja) continue;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) sm.kb[j][e0 + u] = St<DT>::ld(kcp, 8 * c + u);
+        }
+        __syncthreads();
+        summarize_staged<DT, D, false>(sm, a.probes + (int64_t)g * a.m * D, a.proj + (int64_t)g * D * D, a.m,
+                                       a.att_scale, reinterpret_cast<T *>(a.summ) + (page * a.Hkv + g) * a.m * D, tid);
+    }
+}
+
 }  // namespace hba
 
 using namespace hba;
@@ -825,6 +976,71 @@ extern "C" int hba_kv_append(int dtype, const void *k_new, const void *v_new, co
                        (St<DT>::T *)kr_pages, (St<DT>::T *)v_pages)
     HBA_DISPATCH_DT_D(dtype, d, HBA_APP);
 #undef HBA_APP
+    HBA_LAUNCH_CHECK();
+    return HBA_OK;
+}
+
+extern "C" int hba_kv_append_ragged(int dtype, const void *k, const int64_t k_strides[2], const void *v,
+                                    const int64_t v_strides[2], const int32_t *cu, int64_t T, const float *k_gain,
+                                    float eps, const float *cos_tab, const float *sin_tab, int64_t n_tab,
+                                    const int32_t *page_table, int64_t max_pages, const int32_t *seq_lens, int64_t Bd,
+                                    int64_t Hkv, int64_t d, int64_t Bk, int64_t num_pages, void *kc_pages,
+                                    void *kr_pages, void *v_pages, const float *probes, const float *proj, int64_t m,
+                                    void *summ_pages, void *stream) {
+    int st = abi::check_dtype_dim(dtype, d);
+    if (st) return st;
+    if (!k || !k_strides || !v || !v_strides || !cu || !cos_tab || !sin_tab || !page_table || !seq_lens || !kr_pages ||
+        !v_pages || T < 0 || Bd <= 0 || Hkv <= 0 || max_pages <= 0 || n_tab <= 0 || num_pages <= 0)
+        return HBA_ERR_INVALID_ARG;
+    if (summ_pages && (!kc_pages || !probes || !proj)) return HBA_ERR_INVALID_ARG;
+    if (Bk != 64 || (summ_pages && (m < 1 || m > 8))) return HBA_ERR_UNSUPPORTED;
+    if (T > (1 << 30) || Bd > (1 << 24) || Hkv > 65535 || max_pages > (1 << 24)) return HBA_ERR_UNSUPPORTED;
+    const int64_t e = abi::elem_size(dtype), al = 16 / e;
+    if (!abi::aligned16(k) || !abi::aligned16(v) || k_strides[0] % al || k_strides[1] % al || v_strides[0] % al ||
+        v_strides[1] % al || !abi::aligned16(cos_tab) || !abi::aligned16(sin_tab) || !abi::aligned16(kc_pages) ||
+        !abi::aligned16(kr_pages) || !abi::aligned16(v_pages))
+        return HBA_ERR_UNSUPPORTED;
+    if (T == 0) return HBA_OK;
+    RaggedArgs a = {};
+    a.k = (const char *)k;
+    a.v = (const char *)v;
+    a.kst = k_strides[0] * e;
+    a.ksh = k_strides[1] * e;
+    a.vst = v_strides[0] * e;
+    a.vsh = v_strides[1] * e;
+    a.cu = cu;
+    a.T = (int)T;
+    a.Bd = (int)Bd;
+    a.Hkv = (int)Hkv;
+    a.maxp = (int)max_pages;
+    a.m = (int)m;
+    a.kgain = k_gain;
+    a.cosT = cos_tab;
+    a.sinT = sin_tab;
+    a.probes = probes;
+    a.proj = proj;
+    a.eps = eps;
+    a.att_scale = (float)(1.0 / __builtin_sqrt((double)d));
+    a.n_tab = n_tab;
+    a.pages = num_pages;
+    a.ptab = page_table;
+    a.lens = seq_lens;
+    a.kc = (char *)kc_pages;
+    a.kr = (char *)kr_pages;
+    a.vp = (char *)v_pages;
+    a.summ = (char *)summ_pages;
+    // c tokens touch at most c and at most c / 64 + 2 pages
+    const int64_t slots = T < T / 64 + 2 * Bd ? T : T / 64 + 2 * Bd;
+    const dim3 grid((unsigned)slots, (unsigned)Hkv);
+#define HBA_APPR(DT, D)                                                                                       \
+    do {                                                                                                      \
+        if (summ_pages)                                                                                       \
+            hipLaunchKernelGGL((kv_append_ragged_kernel<DT, D, true>), grid, dim3(256), 0, (hipStream_t)stream, a);  \
+        else                                                                                                  \
+            hipLaunchKernelGGL((kv_append_ragged_kernel<DT, D, false>), grid, dim3(256), 0, (hipStream_t)stream, a); \
+    } while (0)
+    HBA_DISPATCH_DT_D(dtype, d, HBA_APPR);
+#undef HBA_APPR
     HBA_LAUNCH_CHECK();
     return HBA_OK;
 }

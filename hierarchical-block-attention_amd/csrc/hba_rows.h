@@ -171,6 +171,7 @@ template <int DT, int D> struct DenseKV {
     int64_t kb, vb;                                   // bytes from row to row
     int last;                                         // the last row that may be read
 
+    __device__ __forceinline__ void next(int) {}
     __device__ __forceinline__ void stage(int tile, uint32_t lds) const {
         TL::template stage<KT>(k, kb, tile * KT, last, lds);
         TL::template stage<KT>(v, vb, tile * KT, last, lds + KT * TL::ROWB);
@@ -187,6 +188,104 @@ template <int DT, int D> struct DenseKV {
     __device__ __forceinline__ float dot(const F (&q)[D / 16], const F *, int j, int hf) const;
     __device__ __forceinline__ void add(f32x16 (&o)[D / 32], int j, float p, int hf) const;
 };
+
+// Keys and values of one KV head in 64-token pages (page_key_off, page_val_off):
+// a tile is a page as it lies in memory.  Row l % 32 of a key operand is the
+// token for which the result's registers 8u .. 8u+7 of half h are the tokens
+// 16 u + 8 h .. + 7, the order in which the pages hold values.
+template <int DT, int D> struct PageKV {
+    typedef typename Op<DT>::F F;
+    static constexpr int ESZ = DT == 1 ? 2 : 4, HALF = KT * D * ESZ, BYTES = 2 * HALF;
+    const char *k, *v;            // the KV head's place in page 0
+    int64_t page;                 // bytes from page to page
+    const int32_t *table;         // the sequence's pages
+    int64_t pages;                // pages there are
+    int64_t id;                   // the page of the tile that is staged next
+
+    __device__ __forceinline__ int64_t at(int tile) const {
+        const int64_t p = table[tile];
+        return p < 0 ? 0 : (p < pages ? p : pages - 1);   // never outside the cache
+    }
+    __device__ __forceinline__ void next(int tile) { id = at(tile); }
+    __device__ __forceinline__ void stage(int, uint32_t lds) const {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+        for (int i = 0; i < HALF / 1024 / NW; ++i) {
+            const int c = (i * NW + wave) * 1024;
+            dma16(k + id * page + c + lane * 16, lds + c);
+            dma16(v + id * page + c + lane * 16, lds + HALF + c);
+        }
+    }
+    static __device__ __forceinline__ int key(int r, int hf) {
+        return 16 * (r >> 3) + 8 * hf + 4 * ((r >> 2) & 1) + (r & 3);
+    }
+    static __device__ __forceinline__ F kf(const char *t, int kt, int ks, int lane) {
+        const int r = lane & 31, l16 = 8 * (r >> 4) + 4 * ((r >> 2) & 1) + (r & 3), mt = 2 * kt + ((r >> 3) & 1);
+        return Op<DT>::load(t + ((mt * (D / 32) + (ks >> 1)) * 64 + l16 + 16 * (2 * (ks & 1) + (lane >> 5))) * 8 * ESZ);
+    }
+    static __device__ __forceinline__ F vf(const char *t, int kt, int dt, int u, int lane) {
+        const int x = 32 * dt + (lane & 31);
+        return Op<DT>::load(t + HALF + (((x >> 4) * 2 + kt) * 64 + (x & 15) + 16 * (2 * u + (lane >> 5))) * 8 * ESZ);
+    }
+    // one key, for attend_each
+    __device__ __forceinline__ float dot_one(const F (&q)[D / 16], int j, int hf) const {
+        const char *t = k + at(j / KT) * page;
+        float sum = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+            float a[8], b[8];
+            Op<DT>::unpack(q[ks], a);
+            Op<DT>::unpack(Op<DT>::load(t + page_key_off(j % KT, 16 * ks + 8 * hf, D) * ESZ), b);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum = fmaf(a[e], b[e], sum);
+        }
+        return sum + other_half(sum);
+    }
+    template <bool LO> __device__ __forceinline__ float dot(const F (&q)[D / 16], const F *qlo, int j, int hf) const {
+        float s = dot_one(q, j, hf);
+        if constexpr (LO) s += dot_one(*reinterpret_cast<const F(*)[D / 16]>(qlo), j, hf);
+        return s;
+    }
+    __device__ __forceinline__ void add(f32x16 (&o)[D / 32], int j, float p, int hf) const {
+        typedef typename St<DT>::T T;
+        const T *t = reinterpret_cast<const T *>(v + at(j / KT) * page);
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                o[dt][r] = fmaf(p, St<DT>::ld(t, page_val_off(j % KT, 32 * dt + 8 * (r >> 2) + 4 * hf + (r & 3))),
+                                o[dt][r]);
+    }
+};
+
+// A 32-column result, columns as rows of memory: registers 4g .. 4g+3 of block dt
+// are elements 32 dt + 8 g + 4 hf + 0..3.
+template <int DT, int D>
+__device__ __forceinline__ void store_rows(char *p, const f32x16 (&o)[D / 32], float f) {
+    const int hf = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int e = 32 * dt + 8 * g + 4 * hf;
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = o[dt][4 * g + i] * f;
+            if constexpr (DT == 1)
+                *reinterpret_cast<uint2 *>(p + 2 * e) = make_uint2(pk_bf16(x[0], x[1]), pk_bf16(x[2], x[3]));
+            else
+                *reinterpret_cast<float4 *>(p + 4 * e) = make_float4(x[0], x[1], x[2], x[3]);
+        }
+}
+
+template <int D> __device__ __forceinline__ bool any_bad(const f32x16 (&o)[D / 32]) {
+    float x = 0.0f;   // 0 * finite is 0, 0 * anything else NaN
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x = fmaf(0.0f, o[dt][r], x);
+    return !(x == 0.0f);
+}
 
 // What a row (a lane's column) and its wave see: keys j < hi with j >= lo or
 // j < S.  The wave's bounds cover its valid rows.
@@ -205,7 +304,7 @@ template <int DT, int D> struct RowAcc {
 // units.  LO: the queries' low parts, added to the scores.  Every wave of the
 // workgroup calls it; it leaves no wave reading LDS.
 template <int DT, int D, bool LO, class Src>
-__device__ __forceinline__ void attend(const Src &src, char *smem, const typename Op<DT>::F (&q)[D / 16],
+__device__ __forceinline__ void attend(Src &src, char *smem, const typename Op<DT>::F (&q)[D / 16],
                                        const typename Op<DT>::F *qlo, float c, int it0, int it1, int ns, int wt0,
                                        const Sees &w, RowAcc<DT, D> &a) {
     constexpr int NKS = D / 16, NDT = D / 32;
@@ -217,14 +316,22 @@ __device__ __forceinline__ void attend(const Src &src, char *smem, const typenam
     a.l = 0.0f;
     float mc = 0.0f;   // the exponent's shift: m, or 0 while nothing is seen
     const uint32_t lds = lds_offset(smem);
-    if (it0 < it1) src.stage(it0 < ns ? it0 : wt0 + it0 - ns, lds);
+    const auto tile = [&](int it) { return it < ns ? it : wt0 + it - ns; };
+    if (it0 < it1) {
+        src.next(tile(it0));
+        src.stage(tile(it0), lds);
+        src.next(tile(min(it0 + 1, it1 - 1)));
+    }
 #pragma unroll 1
     for (int it = it0; it < it1; ++it) {
         wait_vm<0>();
         __syncthreads();   // this tile is staged, and the other buffer is read no more
         const int cur = (it - it0) & 1, nx = it + 1;
-        if (nx < it1) src.stage(nx < ns ? nx : wt0 + nx - ns, lds + (cur ^ 1) * Src::BYTES);
-        const int j0 = (it < ns ? it : wt0 + it - ns) * KT;
+        if (nx < it1) {
+            src.stage(tile(nx), lds + (cur ^ 1) * Src::BYTES);
+            src.next(tile(min(nx + 1, it1 - 1)));
+        }
+        const int j0 = tile(it) * KT;
         if (j0 >= w.hi_max || (j0 + KT <= w.lo_min && j0 >= w.S)) continue;   // nothing the wave's rows see
         const char *t = smem + cur * Src::BYTES;
         f32x16 s[2];

@@ -88,35 +88,6 @@ __device__ __forceinline__ void load_rows(const char *p, bool ok, typename Op<DT
     }
 }
 
-// A 32-column result, columns as rows of memory: registers 4g .. 4g+3 of block dt
-// are elements 32 dt + 8 g + 4 hf + 0..3.
-template <int DT, int D>
-__device__ __forceinline__ void store_rows(char *p, const f32x16 (&o)[D / 32], float f) {
-    const int hf = (threadIdx.x & 63) >> 5;
-#pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int e = 32 * dt + 8 * g + 4 * hf;
-            float x[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = o[dt][4 * g + i] * f;
-            if constexpr (DT == 1)
-                *reinterpret_cast<uint2 *>(p + 2 * e) = make_uint2(pk_bf16(x[0], x[1]), pk_bf16(x[2], x[3]));
-            else
-                *reinterpret_cast<float4 *>(p + 4 * e) = make_float4(x[0], x[1], x[2], x[3]);
-        }
-}
-
-template <int D> __device__ __forceinline__ bool any_bad(const f32x16 (&o)[D / 32]) {
-    float x = 0.0f;   // 0 * finite is 0, 0 * anything else NaN
-#pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) x = fmaf(0.0f, o[dt][r], x);
-    return !(x == 0.0f);
-}
-
 template <int DT, int D> __device__ __forceinline__ DenseKV<DT, D> keys(const Args &a, const Rows &x) {
     DenseKV<DT, D> s;
     s.k = a.k + x.b * a.ks[0] + x.g * a.ks[2];
@@ -134,7 +105,7 @@ template <int DT, int D> __global__ __launch_bounds__(64 * NW) void swa_fwd(cons
     if (!find_rows<D>(a, x)) return;
     typename Op<DT>::F q[D / 16];
     load_rows<DT, D>(a.q + x.b * a.qs[0] + x.tok * a.qs[1] + x.head * a.qs[2], x.valid, q);
-    const DenseKV<DT, D> src = keys<DT, D>(a, x);
+    DenseKV<DT, D> src = keys<DT, D>(a, x);
     int ns, wt0;
     const int nt = tile_list(x.lo, x.hi, a.S, ns, wt0);
     RowAcc<DT, D> acc;

@@ -66,6 +66,12 @@ SIGNATURES = {
                        _vp, _vp, _vp, _vp],
     "hba_decode_fwd_noalloc": [_i, _vp, _vp, _f, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64,
                                _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp],
+    "hba_kv_append_ragged": [_i, _vp, _c_i64p, _vp, _c_i64p, _vp, _i64, _vp, _f, _vp, _vp, _i64, _vp, _i64, _vp, _i64,
+                             _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp],
+    "hba_paged_attn_workspace_bytes": [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i, _i64,
+                                       ctypes.POINTER(ctypes.c_size_t)],
+    "hba_paged_attn": [_i, _vp, _c_i64p, _vp, _f, _vp, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i64,
+                       _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, ctypes.c_size_t, _vp, _vp],
     "hba_swa_fwd": [_i, _vp, _c_i64p, _vp, _c_i64p, _vp, _c_i64p, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f,
                     _vp, _vp, _vp],
     "hba_swa_bwd_workspace_bytes": [_i64, _i64, _i64, _i64, _i64, _i64, _i64, ctypes.POINTER(ctypes.c_size_t)],
@@ -102,6 +108,7 @@ def check(status, what):
         raise HBAError(f"{what}: {msg} (status {status})")
 
 
+_I64X2 = ctypes.c_int64 * 2
 _I64X3 = ctypes.c_int64 * 3
 
 
@@ -113,3 +120,8 @@ def strides3(t):
 def used_strides3(t):
     """strides3 with 0 for dims of one element, whose stride no address uses."""
     return _I64X3(*(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape)))
+
+
+def used_strides2(t):
+    """First two strides of a 3-D [T, H, d] view, 0 for dims of one element."""
+    return _I64X2(*(s if n > 1 else 0 for s, n in zip(t.stride()[:2], t.shape)))

@@ -73,6 +73,7 @@ class PagedKVCache:
         self.lens = [0] * batch
         self._table = [[] for _ in range(batch)]
         self._free = list(range(P - 1, -1, -1))
+        self._held = set()               # pages that several sequences begin with
         self._scale_tabs = {}
         self._scales = torch.zeros(batch, dtype=torch.float32, device=device)   # written by append
         self._scales_ok = False          # _scales holds the scales of the current lengths
@@ -103,6 +104,8 @@ class PagedKVCache:
         outputs: hba_prep_keys' kc and kr), and summarise its full pages.
         Setup path: plain tensor copies."""
         L = kc_seq.shape[0]
+        if self._held.intersection(self._table[s]):
+            raise ValueError(f"sequence {s} begins with pages that others read; load would overwrite them")
         self._ensure_pages(s, L)
         pages = torch.tensor(self._table[s], dtype=torch.long, device=self.kc_pages.device)
         npg = (L + PAGE - 1) // PAGE
@@ -158,6 +161,68 @@ class PagedKVCache:
         self._scales_ok = True
         for s in range(self.batch):
             self.lens[s] += 1
+
+    def extend(self, k, v, counts, qkn, summ, cos, sin):
+        """Append counts[s] tokens to each sequence s (raw k, v [sum(counts),
+        Hkv, d], one sequence behind the other; any strides) in one launch: a
+        part of a prompt, or several accepted tokens.  The same cache as that
+        many appends, but that a bf16 kr is rounded once from the fp32 normalised
+        key (append: after every step).  Returns the int32 [batch + 1] offsets
+        of the sequences' tokens on the device, as cache_attention takes them."""
+        counts = [int(c) for c in counts]
+        kp = self.kr_pages
+        for x, what in ((k, "k"), (v, "v")):
+            if x.dim() != 3 or tuple(x.shape[1:]) != (self.cfg.n_kv, self.cfg.head_dim) or x.shape[0] != k.shape[0] \
+                    or x.dtype != kp.dtype or x.device != kp.device:
+                raise ValueError(f"{what}: expected a {kp.dtype} tensor [tokens, {self.cfg.n_kv}, "
+                                 f"{self.cfg.head_dim}] on {kp.device}")
+        if len(counts) != self.batch or min(counts) < 0 or sum(counts) != k.shape[0]:
+            raise ValueError(f"counts: expected {self.batch} numbers that sum to the {k.shape[0]} tokens of k")
+        need = max(n + c for n, c in zip(self.lens, counts))
+        if need > self.max_len:
+            raise ValueError(f"length {need} exceeds max_len {self.max_len}")
+        if cos.shape[0] < need:
+            raise ValueError(f"cos/sin tables cover {cos.shape[0]} positions, need {need}")
+        cu = [0]
+        for c in counts:
+            cu.append(cu[-1] + c)
+        if cu[-1] == 0:
+            return torch.zeros(self.batch + 1, dtype=torch.int32, device=self.kc_pages.device)
+        lens = [n + c for n, c in zip(self.lens, counts)]
+        short = sum(max(0, (n + PAGE - 1) // PAGE - len(t)) for n, t in zip(lens, self._table))
+        if short > len(self._free):
+            raise RuntimeError("paged KV cache is out of pages")
+        if any([self._ensure_pages(s, n) for s, n in enumerate(lens)]):
+            rows = [t + [0] * (self.max_pages - len(t)) for t in self._table]
+            self.page_table.copy_(torch.tensor(rows, dtype=torch.int32))
+        # one transfer: the offsets, then the new lengths
+        both = torch.tensor(cu + lens, dtype=torch.int32).to(self.kc_pages.device)
+        cu = both[:self.batch + 1]
+        self.seq_lens.copy_(both[self.batch + 1:])
+        cfg = self.cfg
+        kg = qkn.k.gain if getattr(cfg, "qknorm", False) else None
+        keps = float(qkn.k.eps) if kg is not None else 1e-6
+        ops.kv_append_ragged(k, v, cu, kg, keps, cos, sin, self.page_table, self.seq_lens, self.kc_pages,
+                             self.kr_pages, self.v_pages, summ.probes, summ.proj, self.summ_pages)
+        self.lens = lens
+        self._scales_ok = False
+        return cu
+
+    def share(self, src, tokens, dsts):
+        """Begin the empty sequences dsts with the first `tokens` tokens of
+        sequence src (whole pages): the same pages, their summaries included,
+        without a copy.  Appends go to pages of each sequence's own."""
+        if tokens < 0 or tokens % PAGE or tokens > self.lens[src]:
+            raise ValueError(f"share: whole pages of {PAGE} tokens that sequence {src} holds; got {tokens}")
+        if any(s == src or self.lens[s] or self._table[s] for s in dsts) or len(set(dsts)) != len(dsts):
+            raise ValueError("share: the other sequences must be empty and named once")
+        head = self._table[src][:tokens // PAGE]
+        for s in dsts:
+            self._table[s] = list(head)
+            self.lens[s] = tokens
+        if dsts and head:
+            self._held.update(head)
+        self._sync_table()
 
     def key_rows(self, pages, rotated=False):
         """Keys of physical pages (int or index tensor) as token rows
@@ -216,6 +281,33 @@ def hba_decode_step(q, cache, cfg, qkn, cos, sin, scales=None, max_len=None):
     return ops.decode_fwd(q, qg, qeps, cache.kc_pages, cache.kr_pages, cache.v_pages, cache.summ_pages,
                           cache.page_table, cache.seq_lens, cos, sin, sc, cfg.sinks, cfg.window, cfg.k_blocks,
                           max_len)
+
+
+def cache_attention(q, cache, cfg, qkn, cos, sin, window=None, sinks=0, cu=None, shared=0, scales=None, max_len=None):
+    """Attention of each sequence's newest tokens over the paged cache, no
+    selection: the equiv mode's and a window layer's serving form.  The cache
+    holds the tokens' keys already (append or extend first).  q [T, Hq, d] raw
+    (QKNorm, rotation and the union scale of each sequence's length in the
+    kernel, as hba_decode_step).  One token per sequence, or with cu (extend's
+    result) several.  window None: every key; else the last `window` keys and
+    the first `sinks`.  shared: tokens whose pages every sequence shares
+    (PagedKVCache.share), read once for the batch.  Returns [T, Hq, d]."""
+    qg = qkn.q.gain if getattr(cfg, "qknorm", False) else None
+    qeps = float(qkn.q.eps) if qg is not None else 1e-6
+    if window is not None and window < 1:
+        raise ValueError(f"window must be at least 1, got {window}")
+    if shared:
+        head = cache._table[0][:shared // PAGE]
+        if shared % PAGE or len(head) < shared // PAGE or any(t[:len(head)] != head for t in cache._table):
+            raise ValueError(f"the sequences do not share their first {shared} tokens' pages")
+    longest = max(cache.lens)
+    if max_len is None:
+        max_len = max(longest, 1)
+    elif max_len < longest:
+        raise ValueError(f"max_len {max_len} is below the longest sequence ({longest})")
+    sc = cache.scales(cfg) if scales is None else scales
+    return ops.paged_attn(q, qg, qeps, cache.kr_pages, cache.v_pages, cache.page_table, cache.seq_lens, cos, sin, sc,
+                          max_len, 0 if window is None else window, sinks, cu, shared)
 
 
 class DecodeLoop:

@@ -20,6 +20,13 @@ device.
     hba::decode_fwd       decode step over the paged cache
     hba::swa_fwd          sliding-window attention with sinks, forward
     hba::swa_bwd          its backward (dq, dk, dv)
+    hba::kv_append_ragged paged-cache append of any number of tokens per sequence
+                          (mutates the pages and their summaries)
+    hba::paged_attn       attention of new tokens over the paged cache: decode and
+                          parts of prompts, whole or windowed, shared first pages
+
+The last two also run without the dispatcher, under their plain Python names (a
+call through it costs some 20 us of host time).
 """
 import ctypes
 from typing import Optional, Tuple
@@ -27,7 +34,7 @@ from typing import Optional, Tuple
 import torch
 from torch import Tensor
 
-from ._lib import BF16, F32, check, lib, strides3, used_strides3
+from ._lib import BF16, F32, check, lib, strides3, used_strides2, used_strides3
 
 BLOCK = 64
 _DT = {torch.float32: F32, torch.bfloat16: BF16}
@@ -905,3 +912,162 @@ def _(q, q_gain, eps, kc_pages, kr_pages, v_pages, summ_pages, page_table, seq_l
     Bd, Hkv = q.shape[0], summ_pages.shape[1]
     return (q.new_empty(q.shape), q.new_empty(Bd, Hkv, k, dtype=torch.int32),
             q.new_empty(Bd, Hkv, dtype=torch.int32))
+
+
+# ------------------------------------------------- ragged append, paged attention ----
+def _i32(t, shape, dev, what):
+    if t.dtype != torch.int32 or t.device != dev or not t.is_contiguous() or tuple(t.shape) != shape:
+        raise ValueError(f"{what}: expected a contiguous int32 tensor {list(shape)} on {dev}")
+
+
+def _pages(t, dt, dev, P, Hkv, width, what):
+    if t.dtype != dt or t.device != dev or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous {dt} tensor on {dev}")
+    if t.dim() < 2 or t.shape[0] != P or t.shape[1] != Hkv or t.numel() != P * Hkv * width or P == 0:
+        raise ValueError(f"{what}: expected {P} pages of {Hkv} KV heads, {width} elements each")
+
+
+def kv_append_ragged(k, v, cu, k_gain, eps, cos, sin, page_table, seq_lens, kc_pages, kr_pages, v_pages, probes, proj,
+                     summ_pages):
+    """Append a ragged batch of tokens to the paged cache: tokens cu[s] ..
+    cu[s + 1] - 1 of k, v [T, Hkv, d] (raw; any strides) are the last ones of
+    sequence s, whose length seq_lens[s] counts them already, so they go to
+    positions seq_lens[s] - (cu[s + 1] - cu[s]) ...: QKNorm (k_gain None: none)
+    into kc_pages, its rotation at the position into kr_pages, v into v_pages,
+    and the summaries of every page that they fill into summ_pages.  kc_pages
+    and summ_pages (with probes and proj) may be None: a cache without the
+    unrotated keys or the summaries.  cu int32 [Bd + 1], page_table int32 [Bd,
+    max_pages], seq_lens int32 [Bd] on the device; cos/sin fp32 [n_tab, d].
+    Positions past the page table or the cos/sin tables are not appended; a
+    page belongs to one sequence while tokens are appended to it."""
+    if torch.compiler.is_compiling():
+        return torch.ops.hba.kv_append_ragged(k, v, cu, k_gain, eps, cos, sin, page_table, seq_lens, kc_pages,
+                                              kr_pages, v_pages, probes, proj, summ_pages)
+    dev = _dev(k)
+    if k.dim() != 3 or v.shape != k.shape or v.dtype != k.dtype or v.device != dev:
+        raise ValueError("k and v: expected two [T, Hkv, d] tensors of one type and device")
+    T, Hkv, d = k.shape
+    dt = k.dtype
+    code = _code(k)
+    P = kr_pages.shape[0]
+    for t, what in ((kc_pages, "kc_pages"), (kr_pages, "kr_pages"), (v_pages, "v_pages")):
+        if t is not None or what != "kc_pages":
+            _pages(t, dt, dev, P, Hkv, BLOCK * d, what)
+    m = 0
+    pr = pj = None
+    if summ_pages is not None:
+        if probes is None or proj is None or kc_pages is None:
+            raise ValueError("summaries need kc_pages, probes and proj")
+        m = probes.shape[1]
+        pr = _f32c(probes, dev, Hkv * m * d, "probes")
+        pj = _f32c(proj, dev, Hkv * d * d, "proj")
+        _pages(summ_pages, dt, dev, P, Hkv, m * d, "summ_pages")
+    if page_table.dim() != 2:
+        raise ValueError("page_table: expected [Bd, max_pages]")
+    Bd, maxp = page_table.shape
+    _i32(page_table, (Bd, maxp), dev, "page_table")
+    _i32(seq_lens, (Bd,), dev, "seq_lens")
+    _i32(cu, (Bd + 1,), dev, "cu")
+    cos, sin = _tables(cos, sin, 1, d, dev)
+    kg = _f32c(k_gain, dev, Hkv, "k_gain")
+    if T == 0 or Bd == 0:
+        return
+    k, v = _rows16(k), _rows16(v)
+    with _on(dev):
+        st = lib().hba_kv_append_ragged(code, _p(k), used_strides2(k), _p(v), used_strides2(v), _p(cu), T, _p(kg), eps,
+                                        _p(cos), _p(sin), cos.shape[0], _p(page_table), maxp, _p(seq_lens), Bd, Hkv, d,
+                                        BLOCK, P, _p(kc_pages), _p(kr_pages), _p(v_pages), _p(pr), _p(pj), m,
+                                        _p(summ_pages), _stream(dev))
+    check(st, "hba_kv_append_ragged")
+
+
+@torch.library.custom_op("hba::kv_append_ragged", mutates_args=("kc_pages", "kr_pages", "v_pages", "summ_pages"),
+                         device_types="cuda")
+def _kv_append_ragged_op(k: Tensor, v: Tensor, cu: Tensor, k_gain: Optional[Tensor], eps: float, cos: Tensor,
+                         sin: Tensor, page_table: Tensor, seq_lens: Tensor, kc_pages: Optional[Tensor],
+                         kr_pages: Tensor, v_pages: Tensor, probes: Optional[Tensor], proj: Optional[Tensor],
+                         summ_pages: Optional[Tensor]) -> None:
+    kv_append_ragged(k, v, cu, k_gain, eps, cos, sin, page_table, seq_lens, kc_pages, kr_pages, v_pages, probes, proj,
+                     summ_pages)
+
+
+def paged_attn(q, q_gain, eps, kr_pages, v_pages, page_table, seq_lens, cos, sin, scales, max_len, window=0, sinks=0,
+               cu=None, shared=0):
+    """Attention of each sequence's newest tokens over the paged cache (which
+    holds their keys already): q [T, Hq, d] raw, QKNorm (q_gain None: none),
+    the rotation at each token's position (cos None: none) and the logits'
+    scale scales[s] (fp32 [Bd]) applied in the kernel.  cu None: one token per
+    sequence, T = Bd; cu int32 [Bd + 1]: tokens cu[s] .. cu[s + 1] - 1 are the
+    last ones of sequence s.  The token at position i sees the keys j <= i;
+    with window > 0 those with j > i - window or j < sinks.  shared: the first
+    `shared` tokens (whole pages) are the same pages in every sequence; they
+    are read through page_table[0], once for the batch.  max_len bounds every
+    seq_lens[s] (a longer one is read as max_len).  Returns [T, Hq, d]; a
+    token that sees nothing gives 0."""
+    if torch.compiler.is_compiling():
+        return torch.ops.hba.paged_attn(q, q_gain, eps, kr_pages, v_pages, page_table, seq_lens, cos, sin, scales,
+                                        max_len, window, sinks, cu, shared)
+    dev = _dev(q)
+    if q.dim() != 3:
+        raise ValueError("q: expected [T, Hq, d]")
+    T, Hq, d = q.shape
+    P, Hkv = kr_pages.shape[:2]
+    code = _code(q)
+    _pages(kr_pages, q.dtype, dev, P, Hkv, BLOCK * d, "kr_pages")
+    _pages(v_pages, q.dtype, dev, P, Hkv, BLOCK * d, "v_pages")
+    if Hkv == 0 or Hq % Hkv:
+        raise ValueError(f"{Hq} query heads do not divide over {Hkv} KV heads")
+    if page_table.dim() != 2:
+        raise ValueError("page_table: expected [Bd, max_pages]")
+    Bd, maxp = page_table.shape
+    _i32(page_table, (Bd, maxp), dev, "page_table")
+    _i32(seq_lens, (Bd,), dev, "seq_lens")
+    if cu is not None:
+        _i32(cu, (Bd + 1,), dev, "cu")
+    elif T != Bd:
+        raise ValueError(f"one token per sequence expected: {T} tokens, {Bd} sequences (give cu for more)")
+    if window < 0 or sinks < 0 or (sinks and not window):
+        raise ValueError(f"window and sinks must not be negative, and sinks need a window: {window}, {sinks}")
+    if shared < 0 or shared % BLOCK or shared > BLOCK * maxp or (shared and window):
+        raise ValueError(f"shared: whole pages of {BLOCK} tokens within the page table, and no window; got {shared}")
+    if max_len < 1:
+        raise ValueError(f"max_len must be positive, got {max_len}")
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin go together")
+    n_tab = 0
+    if cos is not None:
+        cos, sin = _tables(cos, sin, min(max_len, BLOCK * maxp), d, dev)
+        n_tab = cos.shape[0]
+    qg = _f32c(q_gain, dev, Hq, "q_gain")
+    sc = _f32c(scales, dev, Bd, "scales")
+    out = torch.empty(T, Hq, d, dtype=q.dtype, device=dev)
+    if out.numel() == 0:
+        return out
+    q = _rows16(q)
+    L = lib()
+    nbytes = ctypes.c_size_t(0)
+    check(L.hba_paged_attn_workspace_bytes(T, Bd, Hq, Hkv, d, window, sinks, shared // BLOCK, cu is None, max_len,
+                                           ctypes.byref(nbytes)), "hba_paged_attn_workspace_bytes")
+    nbytes = nbytes.value
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with _on(dev):
+        st = L.hba_paged_attn(code, _p(q), used_strides2(q), _p(qg), eps, _p(cos), _p(sin), n_tab, _p(kr_pages),
+                              _p(v_pages), P, _p(page_table), maxp, _p(seq_lens), _p(sc), _p(cu), T, Bd, Hq, Hkv, d,
+                              BLOCK, window, sinks, shared // BLOCK, max_len, _p(ws), nbytes, _p(out), _stream(dev))
+    check(st, "hba_paged_attn")
+    return out
+
+
+@torch.library.custom_op("hba::paged_attn", mutates_args=(), device_types="cuda")
+def _paged_attn_op(q: Tensor, q_gain: Optional[Tensor], eps: float, kr_pages: Tensor, v_pages: Tensor,
+                   page_table: Tensor, seq_lens: Tensor, cos: Optional[Tensor], sin: Optional[Tensor],
+                   scales: Tensor, max_len: int, window: int = 0, sinks: int = 0, cu: Optional[Tensor] = None,
+                   shared: int = 0) -> Tensor:
+    return paged_attn(q, q_gain, eps, kr_pages, v_pages, page_table, seq_lens, cos, sin, scales, max_len, window,
+                      sinks, cu, shared)
+
+
+@_paged_attn_op.register_fake
+def _(q, q_gain, eps, kr_pages, v_pages, page_table, seq_lens, cos, sin, scales, max_len, window=0, sinks=0, cu=None,
+      shared=0):
+    return q.new_empty(q.shape)

@@ -491,6 +491,65 @@ int hba_attn_bwd_workspace_full_bytes(int dtype, int64_t B, int64_t n, int64_t H
 int hba_attn_bwd_workspace_size(int64_t B, int64_t n, int64_t Hq, int64_t d, size_t *bytes);
 
 /*
+ * Append a ragged batch of tokens to the paged cache: tokens cu[s] .. cu[s+1]-1
+ * of k, v (element strides of token and head; rows on 16-byte boundaries) are
+ * the last ones of sequence s, whose seq_lens[s] counts them already (as in
+ * hba_kv_append): they go to positions seq_lens[s] - (cu[s+1] - cu[s]) and on.
+ * QKNorm of k into kc_pages, its rotation at the position into kr_pages, v into
+ * v_pages, and the slot summaries of every page whose last token is among them
+ * into summ_pages (as hba_summarize_pages).  kc, v and the summaries have the
+ * bits of hba_kv_append and hba_summarize_pages; a bf16 kr is rounded once, from
+ * the fp32 normalised key (hba_kv_append's after every step).  Everything else
+ * in the pages stays as it is.  kc_pages and summ_pages may be NULL (summ_pages
+ * needs kc_pages, probes and proj).  cu int32 [Bd+1] rises from 0 to T; tokens
+ * at positions < 0, past the page table, at/after n_tab, or on a page outside
+ * 0 .. num_pages-1 are not appended.  A page is appended to by one sequence.
+ * The call changes no length, so repeating it gives the same cache.  No
+ * counterpart in the reference, which has no KV cache.
+ */
+int hba_kv_append_ragged(int dtype, const void *k, const int64_t k_strides[2], const void *v,
+                         const int64_t v_strides[2], const int32_t *cu, int64_t T,
+                         const float *k_gain, float eps, const float *cos_tab,
+                         const float *sin_tab, int64_t n_tab, const int32_t *page_table,
+                         int64_t max_pages, const int32_t *seq_lens, int64_t Bd, int64_t Hkv,
+                         int64_t d, int64_t Bk, int64_t num_pages, void *kc_pages, void *kr_pages,
+                         void *v_pages, const float *probes, const float *proj, int64_t m,
+                         void *summ_pages, void *stream);
+
+/*
+ * Attention of each sequence's newest tokens over the paged cache (kr_pages,
+ * v_pages; the tokens' own keys are in it already).  q (element strides of token
+ * and head, rows on 16-byte boundaries) is raw: QKNorm with q_gain (NULL: none),
+ * the rotation at the token's position (cos_tab, sin_tab NULL: none; a position
+ * past n_tab takes the last row) and scales[s], the logits' scale, are applied in
+ * fp32 in the kernel.  cu NULL: one token per sequence (T = Bd), at position
+ * seq_lens[s] - 1; else int32 [Bd+1]: tokens cu[s] .. cu[s+1]-1 are sequence s's
+ * last ones.  The token at position i sees the keys j <= i (W = 0), or those
+ * with j > i - W or j < S (W > 0; W = 1 is the token itself and the sinks).
+ * shared_pages > 0 (W = 0 only): the first shared_pages pages of all sequences
+ * are the same; they are read through page_table's first row, once for the whole
+ * batch, and joined with each sequence's own by their log-sum-exps.  max_len
+ * bounds every seq_lens[s] (a longer one is read as max_len).  A page id outside
+ * 0 .. num_pages-1 is clamped into it.  out [T, Hq, d] contiguous; a token that
+ * sees nothing (position < 0) gives 0.  Whatever lies in the pages at or past a
+ * sequence's length has no effect.  bf16: logits from queries of two bf16 parts
+ * (16 bits of mantissa), probabilities rounded to bf16, sums in fp32.
+ * workspace: 16-byte aligned, no initial contents, at least
+ * hba_paged_attn_workspace_bytes (one_each: cu is NULL); 0 means none is needed.
+ * No counterpart in the reference, which has no KV cache.
+ */
+int hba_paged_attn_workspace_bytes(int64_t T, int64_t Bd, int64_t Hq, int64_t Hkv, int64_t d,
+                                   int64_t W, int64_t S, int64_t shared_pages, int one_each,
+                                   int64_t max_len, size_t *bytes);
+int hba_paged_attn(int dtype, const void *q, const int64_t q_strides[2], const float *q_gain,
+                   float eps, const float *cos_tab, const float *sin_tab, int64_t n_tab,
+                   const void *kr_pages, const void *v_pages, int64_t num_pages,
+                   const int32_t *page_table, int64_t max_pages, const int32_t *seq_lens,
+                   const float *scales, const int32_t *cu, int64_t T, int64_t Bd, int64_t Hq,
+                   int64_t Hkv, int64_t d, int64_t Bk, int64_t W, int64_t S, int64_t shared_pages,
+                   int64_t max_len, void *workspace, size_t ws_bytes, void *out, void *stream);
+
+/*
  * Sliding-window attention with sinks (a model's window layers): query i of
  * q [B, n, Hq, d] attends to the keys j <= i with j > i - W or j < S of k, v
  * [B, n, Hkv, d], all with element strides (rows on 16-byte boundaries).

@@ -39,10 +39,10 @@ def visible(i, j, window, sinks):
     return see
 
 
-def attend(q, k, v, see, scale, u, dout=None):
+def attend(q, k, v, see, scale, u, dout=None, qerr=None):
     """One KV head: q [rows, G, d], k, v [keys, d], see [rows, keys]; rows that see
     nothing are 0.  Returns (o, bound) and with dout ((o, dq, dk, dv), bounds); inputs
-    of any type, computed in 64 bits."""
+    of any type, computed in 64 bits.  qerr: how far the kernel's queries may be from q."""
     q, k, v = q.double(), k.double(), v.double()
     G, d = q.shape[1:]
     N = see.shape[1] + G * see.shape[0]
@@ -52,6 +52,8 @@ def attend(q, k, v, see, scale, u, dout=None):
     some = see.any(1)[None, :, None]
     p = torch.where(some, torch.softmax(x, -1).nan_to_num(0.0), torch.zeros((), dtype=torch.float64))
     dx = (d + 4) * E * scale * 1.4427 * (qh.abs() @ k.abs().T)
+    if qerr is not None:
+        dx = dx + scale * 1.4427 * (qerr.double().transpose(0, 1) @ k.abs().T)
     dx = torch.where(sees, dx, torch.zeros((), dtype=torch.float64)).amax(-1, keepdim=True)
     r = 2 * dx + 8 * E
     o = p @ v
@@ -72,6 +74,24 @@ def attend(q, k, v, see, scale, u, dout=None):
     bv = bv.sum(0) + (u + 2 * E) * dv.abs() + F
     t = lambda z: z.transpose(0, 1)  # noqa: E731
     return (t(o), t(dq), dk, dv), (t(bo), t(bq), bk, bv)
+
+
+def norm_rotate(x, gain, eps, cos, sin, u):
+    """QKNorm (gain None: none) and rotation of x [rows, H, d] with cos, sin [rows, d]
+    in 64 bits: (normalised, rotated, error of the rotated in fp32 and one rounding u).
+    The norm: d e / 2 from the sum of squares, 6 e from root, division, gain, scale; the
+    rotation 3 e of both products' magnitudes."""
+    x = x.double()
+    d = x.shape[-1]
+    if gain is not None:
+        x = x / x.square().mean(-1, keepdim=True).clamp_min(eps).sqrt() * gain.double()[:, None]
+    if cos is None:
+        return x, x, (d / 2 + 6 + u / E) * E * x.abs()
+    h = d // 2
+    c, s = cos.double()[:, None], sin.double()[:, None]
+    other = torch.cat((-x[..., h:], x[..., :h]), -1)
+    y = x * c + other * s
+    return x, y, (d / 2 + 9) * E * (x.abs() * c.abs() + other.abs() * s.abs()) + u * y.abs()
 
 
 def sliding(q, k, v, window, sinks, scale, lens, u, dout=None):
