@@ -288,7 +288,7 @@ template <int DT, int D, int UK> __global__ __launch_bounds__(64 * DW) void deco
 // SHARED: the rows of all tokens over the shared pages (blockIdx.x: 128-row
 // tile); else the rows of one sequence's tokens over its own pages (blockIdx.x:
 // tile of the ragged batch).  blockIdx.y: KV head, blockIdx.z: part of the tiles.
-template <int DT, int D, bool SHARED> __global__ __launch_bounds__(64 * rows::NW) void rows_kernel(const Args a) {
+template <int DT, int D, bool SHARED> __global__ __launch_bounds__(64 * rows::NW, (rows::WAVES<DT, D>)) void rows_kernel(const Args a) {
     extern __shared__ __align__(16) char smem[];
     typedef typename Op<DT>::F F;
     constexpr int ESZ = DT == 1 ? 2 : 4, NKS = D / 16;

@@ -33,6 +33,10 @@ constexpr int KT = 64;            // keys per tile
 constexpr int NW = 4;             // waves per workgroup
 constexpr int RW = 32;            // query rows per wave
 constexpr int RT = NW * RW;       // query rows per workgroup
+// Waves per SIMD that a row kernel's registers leave room for.  At two or more the
+// compiler also keeps the MFMA results in the registers that vector instructions
+// read, without a move each.
+template <int DT, int D> constexpr int WAVES = DT == 1 ? 2 : (D == 64 ? 2 : 1);
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LAZY = 8.0f;      // log2 units a maximum may grow before O and l are rescaled
 
@@ -287,6 +291,22 @@ template <int D> __device__ __forceinline__ bool any_bad(const f32x16 (&o)[D / 3
     return !(x == 0.0f);
 }
 
+// The first n of 64 bits.
+__device__ __forceinline__ uint64_t first_bits(int n) {
+    return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1;
+}
+// Places lo .. hi - 1 and those below both s and hi, of the 64 from j0.
+__device__ __forceinline__ uint64_t seen_bits(int lo, int hi, int s, int j0) {
+    return (first_bits(hi - j0) & ~first_bits(lo - j0)) | first_bits(min(s, hi) - j0);
+}
+// x where bit b of the mask is set, else `other`: two instructions (a bit field
+// extract, a bitwise select).
+__device__ __forceinline__ float keep(float x, uint64_t bits, int b, float other) {
+    const uint32_t w = b < 32 ? (uint32_t)bits : (uint32_t)(bits >> 32);
+    const uint32_t t = (uint32_t)((int32_t)(w << (31 - (b & 31))) >> 31);
+    return __uint_as_float((__float_as_uint(x) & t) | (__float_as_uint(other) & ~t));
+}
+
 // What a row (a lane's column) and its wave see: keys j < hi with j >= lo or
 // j < S.  The wave's bounds cover its valid rows.
 struct Sees {
@@ -347,13 +367,11 @@ __device__ __forceinline__ void attend(Src &src, char *smem, const typename Op<D
         }
         const bool whole = j0 + KT <= w.hi_min && (j0 >= w.lo_max || j0 + KT <= w.S);
         if (!whole) {
+            const uint64_t see = seen_bits(w.lo, w.hi, w.S, j0) >> Src::key(0, hf);
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int j = j0 + 32 * kt + Src::key(r, hf);
-                    if (!(j < w.hi && (j >= w.lo || j < w.S))) s[kt][r] = -INFINITY;
-                }
+                for (int r = 0; r < 16; ++r) s[kt][r] = keep(s[kt][r], see, 32 * kt + Src::key(r, 0), -INFINITY);
         }
         float mx = s[0][0];
 #pragma unroll
@@ -432,7 +450,7 @@ __device__ __forceinline__ void DenseKV<DT, D>::add(f32x16 (&o)[D / 32], int j, 
 // attend, one key at a time: for rows that came out non-finite.  Each lane adds
 // the visible keys only, so nothing of a masked key reaches its row.
 template <int DT, int D, bool LO, class Src>
-__device__ __noinline__ void attend_each(const Src &src, const typename Op<DT>::F (&q)[D / 16],
+__device__ __forceinline__ void attend_each(const Src &src, const typename Op<DT>::F (&q)[D / 16],
                                          const typename Op<DT>::F *qlo, float c, int it0, int it1, int ns, int wt0,
                                          const Sees &w, RowAcc<DT, D> &a) {
     const int hf = (threadIdx.x & 63) >> 5;

@@ -98,7 +98,7 @@ template <int DT, int D> __device__ __forceinline__ DenseKV<DT, D> keys(const Ar
     return s;
 }
 
-template <int DT, int D> __global__ __launch_bounds__(64 * NW) void swa_fwd(const Args a) {
+template <int DT, int D> __global__ __launch_bounds__(64 * NW, (DT == 1 && D == 64 ? 3 : WAVES<DT, D>)) void swa_fwd(const Args a) {
     extern __shared__ __align__(16) char smem[];
     constexpr int ESZ = Tile<DT, D>::ESZ;
     Rows x;
@@ -130,7 +130,7 @@ template <int DT, int D> __global__ __launch_bounds__(64 * NW) void swa_fwd(cons
 
 // The probabilities' gradient from the forward's log-sum-exps, and dq; delta =
 // do . o on the way, for dk and dv.
-template <int DT, int D> __global__ __launch_bounds__(64 * NW) void swa_dq(const Args a) {
+template <int DT, int D> __global__ __launch_bounds__(64 * NW, DT == 1 ? 2 : 1) void swa_dq(const Args a) {
     extern __shared__ __align__(16) char smem[];
     typedef Tile<DT, D> TL;
     typedef typename Op<DT>::F F;
@@ -189,11 +189,9 @@ template <int DT, int D> __global__ __launch_bounds__(64 * NW) void swa_dq(const
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = ex2(fmaf(s[r], a.c, -lse)) * (dp[r] - delta);
             if (!whole) {
+                const uint64_t see = seen_bits(x.w.lo, x.w.hi, a.S, j0 + 32 * kt) >> src.key(0, hf);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int j = j0 + 32 * kt + src.key(r, hf);
-                    if (!(j < x.w.hi && (j >= x.w.lo || j < a.S))) s[r] = 0.0f;
-                }
+                for (int r = 0; r < 16; ++r) s[r] = keep(s[r], see, src.key(r, 0), 0.0f);
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
@@ -251,7 +249,7 @@ __device__ __forceinline__ void find_part(const Args &a, int slot, int &tile, in
     }
 }
 
-template <int DT, int D> __global__ __launch_bounds__(64 * NW) void swa_dkv(const Args a) {
+template <int DT, int D> __global__ __launch_bounds__(64 * NW, DT == 1 && D == 64 ? 2 : 1) void swa_dkv(const Args a) {
     extern __shared__ __align__(16) char smem[];
     typedef Tile<DT, D> TL;
     typedef typename Op<DT>::F F;
@@ -314,11 +312,12 @@ template <int DT, int D> __global__ __launch_bounds__(64 * NW) void swa_dkv(cons
                 s[r] = ex2(fmaf(s[r], a.c, -ld[tr]));
                 dp[r] = s[r] * (dp[r] - ld[TT + tr]);
             }
-            if (!whole) {
+            if (!whole) {   // tokens j .. that see key j
+                const uint64_t see = seen_bits(j, j < a.S ? len : min(len, j + a.W), 0, t0 + 32 * rt) >> (4 * hf);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const int t = t0 + 32 * rt + 8 * (r >> 2) + 4 * hf + (r & 3);
-                    if (!(t >= j && t < len && (t < j + a.W || j < a.S))) s[r] = dp[r] = 0.0f;
+                    s[r] = keep(s[r], see, 8 * (r >> 2) + (r & 3), 0.0f);
+                    dp[r] = keep(dp[r], see, 8 * (r >> 2) + (r & 3), 0.0f);
                 }
             }
 #pragma unroll
