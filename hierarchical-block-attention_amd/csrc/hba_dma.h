@@ -24,6 +24,15 @@ __device__ __forceinline__ void dma16(const void *src, uint32_t lds_addr) {
                  : "memory");
 }
 
+// The same from a wave-uniform base and a lane's 32-bit byte offset.
+__device__ __forceinline__ void dma16s(const void *base, uint32_t off, uint32_t lds_addr) {
+    const uint32_t a = __builtin_amdgcn_readfirstlane(lds_addr);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"(a), "v"(off), "s"(base)
+                 : "memory");
+}
+
 // vmcnt(N) with the other counters left alone (gfx9 s_waitcnt encoding)
 template <int N>
 __device__ __forceinline__ void wait_vm() {

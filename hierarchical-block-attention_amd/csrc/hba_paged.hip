@@ -396,36 +396,75 @@ template <int DT, int D, bool SHARED> __global__ __launch_bounds__(64 * rows::NW
 }
 
 // out = sum of the parts' O 2^(m - max) over sum of their l 2^(m - max); a row
-// without keys 0.  One wave per row.
-template <int DT, int D> __global__ __launch_bounds__(256) void join_kernel(const Args a, int64_t nrows) {
-    const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= nrows) return;
-    const float *ml = a.pml + row * a.slots * 2;
-    float mm = -INFINITY;
-    for (int i = lane; i < a.slots; i += 64) mm = fmaxf(mm, ml[2 * i]);
-    mm = wave_max(mm);
-    constexpr int V = D / 64;   // elements of a lane
-    float o[V], ll = 0.0f;
+// without keys 0.  D / 4 threads a part, SG parts of a row at a time (all of a
+// workgroup where a row has many parts, one where rows are many), each with sums
+// of its own that LDS joins.
+template <int DT, int D, int SG> __global__ __launch_bounds__(256) void join_kernel(const Args a, int64_t nrows) {
+    constexpr int TP = D / 4, RB = 256 / (TP * SG);   // threads of a part, rows of a workgroup
+    __shared__ float so[SG > 1 ? SG : 1][SG > 1 ? D : 1];
+    __shared__ float sm[SG], sl[SG];
+    const int x = threadIdx.x % TP * 4, sg = threadIdx.x / TP % SG;
+    const int64_t row = (int64_t)blockIdx.x * RB + threadIdx.x / (TP * SG);
+    if (row >= nrows) return;                         // SG > 1: the workgroup's one row
+    const float *ml = a.pml + row * a.slots * 2, *po = a.po + row * a.slots * D + x;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.0f;
+    for (int i = sg; i < a.slots; i += 4 * SG) {      // four parts at a time
+        float pm[4], pl[4];
+        f32x4 px[4];
+        float mn = m;
 #pragma unroll
-    for (int e = 0; e < V; ++e) o[e] = 0.0f;
-    for (int i = 0; i < a.slots; ++i) {
-        const float m = ml[2 * i], l = ml[2 * i + 1];
-        if (m == -INFINITY && l == 0.0f) continue;   // no keys here, or none that counts
-        const float f = ex2(m - mm);
-        ll = fmaf(l, f, ll);
+        for (int e = 0; e < 4; ++e) {
+            const int p = min(i + e * SG, a.slots - 1);
+            const bool in = i + e * SG < a.slots;
+            pm[e] = in ? ml[2 * p] : -INFINITY;
+            pl[e] = in ? ml[2 * p + 1] : 0.0f;
+            px[e] = *reinterpret_cast<const f32x4 *>(po + (int64_t)p * D);
+            mn = fmaxf(mn, pm[e]);
+        }
+        const float al = m == -INFINITY ? 0.0f : ex2(m - mn);
+        l *= al;
+        o = o * al;
 #pragma unroll
-        for (int e = 0; e < V; ++e) o[e] = fmaf(a.po[(row * a.slots + i) * D + lane * V + e], f, o[e]);
+        for (int e = 0; e < 4; ++e) {
+            if (pm[e] == -INFINITY && pl[e] == 0.0f) continue;   // no keys here, or none that counts
+            const float f = ex2(pm[e] - mn);
+            l = fmaf(pl[e], f, l);
+            o = o + px[e] * f;
+        }
+        m = mn;
+    }
+    if constexpr (SG > 1) {
+        *reinterpret_cast<f32x4 *>(&so[sg][x]) = o;
+        if (x == 0) {
+            sm[sg] = m;
+            sl[sg] = l;
+        }
+        __syncthreads();
+        if (sg) return;
+        float mm = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < SG; ++i) mm = fmaxf(mm, sm[i]);
+        o = f32x4{0.f, 0.f, 0.f, 0.f};
+        l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < SG; ++i) {
+            if (sm[i] == -INFINITY && sl[i] == 0.0f) continue;
+            const float f = ex2(sm[i] - mm);
+            l = fmaf(sl[i], f, l);
+            o = o + *reinterpret_cast<const f32x4 *>(&so[i][x]) * f;
+        }
     }
     // what the row sees: nothing gives 0, scores that are all -inf NaN
     const int t = (int)(row / a.Hq), s = a.cu ? ragged::sequence(a.cu, a.Bd, t) : t;
     int first = t, cnt = 1;
     if (a.cu) cnt = ragged::tokens(a.cu, s, a.T, first);
-    const bool some = length(a, s) - cnt + t - first >= 0;
-    typedef typename St<DT>::T T;
-    T *to = reinterpret_cast<T *>(a.out) + row * D + lane * V;
-#pragma unroll
-    for (int e = 0; e < V; ++e) St<DT>::st(to, e, some ? o[e] / ll : 0.0f);
+    const f32x4 r = length(a, s) - cnt + t - first >= 0 ? o / l : f32x4{0.f, 0.f, 0.f, 0.f};
+    char *to = a.out + (row * D + x) * (DT == 1 ? 2 : 4);
+    if constexpr (DT == 1)
+        *reinterpret_cast<uint2 *>(to) = make_uint2(pk_bf16(r[0], r[1]), pk_bf16(r[2], r[3]));
+    else
+        *reinterpret_cast<f32x4 *>(to) = r;
 }
 
 // ------------------------------------------------------------------- plan ----
@@ -504,7 +543,12 @@ template <int DT, int D> static int launch(Args a, const Plan &p, hipStream_t s)
     HBA_LAUNCH_CHECK();
     if (a.slots > 1) {
         const int64_t nrows = (int64_t)a.T * a.Hq;
-        hipLaunchKernelGGL((join_kernel<DT, D>), dim3((unsigned)((nrows + 3) / 4)), dim3(256), 0, s, a, nrows);
+        constexpr int SG = 1024 / D, RB = 1024 / D;   // parts at a time, or rows
+        if (a.slots > 8)
+            hipLaunchKernelGGL((join_kernel<DT, D, SG>), dim3((unsigned)nrows), dim3(256), 0, s, a, nrows);
+        else
+            hipLaunchKernelGGL((join_kernel<DT, D, 1>), dim3((unsigned)((nrows + RB - 1) / RB)), dim3(256), 0, s, a,
+                               nrows);
         HBA_LAUNCH_CHECK();
     }
     return HBA_OK;

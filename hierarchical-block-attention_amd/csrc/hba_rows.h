@@ -9,9 +9,11 @@
 // query heads are flattened (row r = token r / G, head r % G), so every group
 // size fills the tiles and the heads of a group share the staged keys.
 //
-// Softmax: running maximum and sum in fp32, in units of log2.  The sums (O, l)
-// are rescaled only when a row's maximum grows by more than 8 (a factor of 256,
-// far from fp32's range), so most tiles do no rescaling.
+// Softmax: a shift m and the sums O and l in fp32, in units of log2.  m is a maximum
+// of the row, but not of the newest tiles: a tile's probabilities are taken
+// with the m there is, and only where their sum passes 2^16 (far from any
+// range's end), or nothing was seen before, the wave takes the tile's maximum as
+// m, rescales and does the tile once more.  So most tiles compute no maximum.
 //
 // Masked keys have probability 0; a NaN or infinity of V in a masked place
 // would still spoil 0 * V.  Whether that happened shows in the result, so a
@@ -38,7 +40,7 @@ constexpr int RT = NW * RW;       // query rows per workgroup
 // read, without a move each.
 template <int DT, int D> constexpr int WAVES = DT == 1 ? 2 : (D == 64 ? 2 : 1);
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float LAZY = 8.0f;      // log2 units a maximum may grow before O and l are rescaled
+constexpr float MOST = 65536.0f;  // sum of a tile's probabilities that calls for a new maximum
 
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
@@ -75,6 +77,15 @@ template <> struct Op<1> {
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = (float)f[e];
     }
+    // acc + the sum of f's elements, two at a time
+    static __device__ __forceinline__ float sum(F f, float acc) {
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        const bf16x2 one = {(__bf16)1.0f, (__bf16)1.0f};
+        acc = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(f, f, 0, 1), one, acc, false);
+        acc = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(f, f, 2, 3), one, acc, false);
+        acc = __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(f, f, 4, 5), one, acc, false);
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_shufflevector(f, f, 6, 7), one, acc, false);
+    }
 };
 template <> struct Op<0> {
     typedef f32x8 F;
@@ -97,6 +108,11 @@ template <> struct Op<0> {
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = f[e];
     }
+    static __device__ __forceinline__ float sum(F f, float acc) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc += f[e];
+        return acc;
+    }
 };
 
 // Elements 8u .. 8u+7 of a 32x32 result as the operand of the step over its
@@ -109,10 +125,10 @@ template <int DT> __device__ __forceinline__ typename Op<DT>::F half16(const f32
 }
 
 // ------------------------------------------------------------ staged rows --
-// R rows of D elements in LDS, 16-byte chunk c of row r at place c ^ (r & 7) of
-// its row: the eight lanes that an LDS cycle serves then read eight different
-// bank groups, whether they read one chunk of eight rows (an operand along the
-// rows) or, transposed, four rows' pieces.
+// R rows of D elements in LDS, 16-byte chunk c of row r at place c ^ swz(r) of its
+// row, swz(r) = 2 (r % 4) + r / 4 % 2: eight rows' chunks c lie in eight
+// different places (an operand along the rows reads those in one LDS cycle), and
+// so do the chunk pairs 2c, 2c + 1 of four rows r, r + 1 .. (a transposed operand).
 template <int DT, int D> struct Tile {
     typedef typename St<DT>::T T;
     typedef typename Op<DT>::F F;
@@ -120,7 +136,10 @@ template <int DT, int D> struct Tile {
     static constexpr int NCH = D * ESZ / 16;          // chunks per row
     static constexpr int ROWB = D * ESZ;              // bytes per row
 
-    static __device__ __forceinline__ int at(int r, int c) { return r * ROWB + ((c ^ (r & 7)) * 16); }
+    static constexpr int RPI = 64 * NW / NCH;         // rows that the workgroup stages at once (a multiple of 8)
+
+    static __device__ __forceinline__ int swz(int r) { return ((r & 3) << 1) | ((r >> 2) & 1); }
+    static __device__ __forceinline__ int at(int r, int c) { return r * ROWB + ((c ^ swz(r)) * 16); }
 
     // Row r, elements 16 ks + 8 (lane / 32) .. + 7.
     static __device__ __forceinline__ F row(const char *t, int r, int ks, int hf) {
@@ -151,17 +170,26 @@ template <int DT, int D> struct Tile {
             return f;
         }
     }
-    // Stage rows j0 .. j0 + R - 1 of a strided array (`bytes` from row to row); rows past
-    // `last` read row `last`.  Called by all NW waves.
+    // The thread's first chunk of a staging pass, as an offset from the first row.
+    static __device__ __forceinline__ uint32_t offset(int64_t bytes) {
+        const int r = threadIdx.x / NCH;
+        return (uint32_t)(r * (int)bytes) + ((threadIdx.x % NCH) ^ swz(r)) * 16;
+    }
+    // Stage rows j0 .. j0 + R - 1 of a strided array (`bytes` from row to row, off =
+    // offset(bytes)); rows past `last` read row `last`.  Called by all NW waves.
     template <int R>
-    static __device__ __forceinline__ void stage(const char *base, int64_t bytes, int j0, int last, uint32_t lds) {
-        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    static __device__ __forceinline__ void stage(const char *base, int64_t bytes, uint32_t off, int j0, int last,
+                                                 uint32_t lds) {
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        if (j0 + R - 1 <= last) {
+            const char *p = base + j0 * bytes;
 #pragma unroll
-        for (int i = 0; i < R * NCH / 64 / NW; ++i) {
-            const int p = (i * NW + wave) * 64 + lane;
-            const int r = p / NCH, c = (p % NCH) ^ (r & 7);
-            const int j = min(j0 + r, last);
-            dma16(base + (int64_t)j * bytes + c * 16, lds + (i * NW + wave) * 1024);
+            for (int i = 0; i < R / RPI; ++i) dma16s(p + i * RPI * bytes, off, lds + (i * NW + wave) * 1024);
+        } else {
+            const int r = threadIdx.x / NCH, c = (threadIdx.x % NCH) ^ swz(r);
+#pragma unroll
+            for (int i = 0; i < R / RPI; ++i)
+                dma16(base + (int64_t)min(j0 + r + i * RPI, last) * bytes + c * 16, lds + (i * NW + wave) * 1024);
         }
     }
 };
@@ -174,11 +202,12 @@ template <int DT, int D> struct DenseKV {
     const char *k, *v;
     int64_t kb, vb;                                   // bytes from row to row
     int last;                                         // the last row that may be read
+    uint32_t ko, vo;                                  // TL::offset of kb, vb
 
     __device__ __forceinline__ void next(int) {}
     __device__ __forceinline__ void stage(int tile, uint32_t lds) const {
-        TL::template stage<KT>(k, kb, tile * KT, last, lds);
-        TL::template stage<KT>(v, vb, tile * KT, last, lds + KT * TL::ROWB);
+        TL::template stage<KT>(k, kb, ko, tile * KT, last, lds);
+        TL::template stage<KT>(v, vb, vo, tile * KT, last, lds + KT * TL::ROWB);
     }
     // the key (of 32) that register r of half hf holds
     static __device__ __forceinline__ int key(int r, int hf) { return 8 * (r >> 2) + 4 * hf + (r & 3); }
@@ -207,17 +236,19 @@ template <int DT, int D> struct PageKV {
     int64_t id;                   // the page of the tile that is staged next
 
     __device__ __forceinline__ int64_t at(int tile) const {
-        const int64_t p = table[tile];
+        const int p = __builtin_amdgcn_readfirstlane(table[tile]);
         return p < 0 ? 0 : (p < pages ? p : pages - 1);   // never outside the cache
     }
     __device__ __forceinline__ void next(int tile) { id = at(tile); }
     __device__ __forceinline__ void stage(int, uint32_t lds) const {
-        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const uint32_t off = (threadIdx.x & 63) * 16;
+        const char *kp = k + id * page, *vp = v + id * page;
 #pragma unroll
         for (int i = 0; i < HALF / 1024 / NW; ++i) {
             const int c = (i * NW + wave) * 1024;
-            dma16(k + id * page + c + lane * 16, lds + c);
-            dma16(v + id * page + c + lane * 16, lds + HALF + c);
+            dma16s(kp + c, off, lds + c);
+            dma16s(vp + c, off, lds + HALF + c);
         }
     }
     static __device__ __forceinline__ int key(int r, int hf) {
@@ -321,12 +352,14 @@ template <int DT, int D> struct RowAcc {
 
 // One pass of the workgroup's rows over tiles it0 .. it1 - 1 of their list
 // (tile it < ns: sinks, tile it; else tile wt0 + it - ns).  c: logits to log2
-// units.  LO: the queries' low parts, added to the scores.  Every wave of the
-// workgroup calls it; it leaves no wave reading LDS.
+// units.  LO: the queries come as two parts in log2 units already (c = 1); their
+// products then start from -m instead of 0.  Every wave of the workgroup calls
+// it; it leaves no wave reading LDS.
 template <int DT, int D, bool LO, class Src>
 __device__ __forceinline__ void attend(Src &src, char *smem, const typename Op<DT>::F (&q)[D / 16],
                                        const typename Op<DT>::F *qlo, float c, int it0, int it1, int ns, int wt0,
                                        const Sees &w, RowAcc<DT, D> &a) {
+    typedef typename Op<DT>::F F;
     constexpr int NKS = D / 16, NDT = D / 32;
     const int lane = threadIdx.x & 63, hf = lane >> 5;
     const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -334,7 +367,7 @@ __device__ __forceinline__ void attend(Src &src, char *smem, const typename Op<D
     for (int dt = 0; dt < NDT; ++dt) a.O[dt] = zero;
     a.m = -INFINITY;
     a.l = 0.0f;
-    float mc = 0.0f;   // the exponent's shift: m, or 0 while nothing is seen
+    float shift = INFINITY;   // -m: every probability is infinite (or NaN) while nothing is seen
     const uint32_t lds = lds_offset(smem);
     const auto tile = [&](int it) { return it < ns ? it : wt0 + it - ns; };
     if (it0 < it1) {
@@ -354,59 +387,81 @@ __device__ __forceinline__ void attend(Src &src, char *smem, const typename Op<D
         const int j0 = tile(it) * KT;
         if (j0 >= w.hi_max || (j0 + KT <= w.lo_min && j0 >= w.S)) continue;   // nothing the wave's rows see
         const char *t = smem + cur * Src::BYTES;
-        f32x16 s[2];
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-            s[kt] = zero;
-#pragma unroll
-            for (int ks = 0; ks < NKS; ++ks) {
-                const typename Op<DT>::F kf = Src::kf(t, kt, ks, lane);
-                s[kt] = Op<DT>::mma(kf, q[ks], s[kt]);
-                if constexpr (LO) s[kt] = Op<DT>::mma(kf, qlo[ks], s[kt]);
-            }
-        }
         const bool whole = j0 + KT <= w.hi_min && (j0 >= w.lo_max || j0 + KT <= w.S);
-        if (!whole) {
-            const uint64_t see = seen_bits(w.lo, w.hi, w.S, j0) >> Src::key(0, hf);
+        // the tile's logits (LO: in log2 units, above `from`), masked
+        const auto logits = [&](f32x16 (&s)[2], float from) {
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+                s[kt] = zero;
+                if constexpr (LO) s[kt] = s[kt] + from;
+#pragma unroll
+                for (int ks = 0; ks < NKS; ++ks) {
+                    const F kf = src.kf(t, kt, ks, lane);
+                    s[kt] = Op<DT>::mma(kf, q[ks], s[kt]);
+                    if constexpr (LO) s[kt] = Op<DT>::mma(kf, qlo[ks], s[kt]);
+                }
+            }
+            if (!whole) {
+                const uint64_t see = seen_bits(w.lo, w.hi, w.S, j0) >> Src::key(0, hf);
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[kt][r] = keep(s[kt][r], see, 32 * kt + Src::key(r, 0), -INFINITY);
+            }
+        };
+        // probabilities 2^(c s + by) as operands, and this half's sum of them
+        const auto weights = [&](const f32x16 (&s)[2], float by, F (&p)[2][2]) {
+            float sum = 0.0f;
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[kt][r] = keep(s[kt][r], see, 32 * kt + Src::key(r, 0), -INFINITY);
-        }
-        float mx = s[0][0];
+                for (int u = 0; u < 2; ++u) {
+                    float x[8];
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
+                    for (int e = 0; e < 8; ++e) {
+                        const float y = s[kt][8 * u + e];
+                        x[e] = ex2(LO ? y : fmaf(y, c, by));
+                    }
+                    p[kt][u] = Op<DT>::pack(x);
+                    sum = Op<DT>::sum(p[kt][u], sum);
+                }
+            return sum;
+        };
+        f32x16 s[2];
+        F p[2][2];
+        logits(s, shift);
+        float sum = weights(s, shift, p);
+        if (__ballot(!(sum <= MOST))) {   // a new maximum
+            asm volatile("" ::: "memory");   // the keys once more from LDS: registers for them would be held in every tile
+            logits(s, 0.0f);
+            float mx = s[0][0];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kt][r]);
-        mx = fmaxf(mx, other_half(mx)) * c;
-        const bool grow = mx > a.m + LAZY;   // m = -inf: whenever something is seen
-        if (__ballot(grow)) {
-            const float mn = grow ? mx : a.m;
-            const float al = (a.m == -INFINITY) ? 0.0f : ex2(a.m - mn);   // nothing to rescale yet
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kt][r]);
+            mx = fmaxf(a.m, fmaxf(mx, other_half(mx)) * c);
+            const float al = a.m == -INFINITY ? 0.0f : ex2(a.m - mx);   // nothing to rescale yet
             a.l *= al;
 #pragma unroll
             for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) a.O[dt][r] *= al;
-            a.m = mn;
-            mc = (mn == -INFINITY) ? 0.0f : mn;
+            a.m = mx;
+            shift = -mx;
+            const float by = mx == -INFINITY ? 0.0f : -mx;   // rows that still see nothing: 2^-inf
+            if constexpr (LO) {
+                s[0] = s[0] + by;
+                s[1] = s[1] + by;
+            }
+            sum = weights(s, by, p);
         }
+        a.l += sum;
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float p = ex2(fmaf(s[kt][r], c, -mc));
-                s[kt][r] = p;
-                a.l += p;
-            }
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const typename Op<DT>::F pf = half16<DT>(s[kt], u);
-#pragma unroll
-                for (int dt = 0; dt < NDT; ++dt) a.O[dt] = Op<DT>::mma(Src::vf(t, kt, dt, u, lane), pf, a.O[dt]);
-            }
+                for (int dt = 0; dt < NDT; ++dt) a.O[dt] = Op<DT>::mma(src.vf(t, kt, dt, u, lane), p[kt][u], a.O[dt]);
     }
     __syncthreads();
 }

@@ -95,6 +95,8 @@ template <int DT, int D> __device__ __forceinline__ DenseKV<DT, D> keys(const Ar
     s.kb = a.ks[1];
     s.vb = a.vs[1];
     s.last = max(x.len, 1) - 1;
+    s.ko = Tile<DT, D>::offset(s.kb);
+    s.vo = Tile<DT, D>::offset(s.vb);
     return s;
 }
 
@@ -272,12 +274,13 @@ template <int DT, int D> __global__ __launch_bounds__(64 * NW, DT == 1 && D == 6
     f32x16 dk[NDT], dv[NDT];
     const uint32_t lds = lds_offset(smem);
     const int last = max(len, 1) - 1;
+    const uint32_t qo = TL::offset(a.qs[1]), doo = TL::offset(a.dos[1]);
 
     auto stage = [&](int it, int buf) {
         const int h = g * a.G + it / nst, t0 = (k0 / TT + it % nst) * TT;
         const uint32_t to = lds + buf * BYTES;
-        TL::template stage<TT>(a.q + b * a.qs[0] + h * a.qs[2], a.qs[1], t0, last, to);
-        TL::template stage<TT>(a.dout + b * a.dos[0] + h * a.dos[2], a.dos[1], t0, last, to + TT * TL::ROWB);
+        TL::template stage<TT>(a.q + b * a.qs[0] + h * a.qs[2], a.qs[1], qo, t0, last, to);
+        TL::template stage<TT>(a.dout + b * a.dos[0] + h * a.dos[2], a.dos[1], doo, t0, last, to + TT * TL::ROWB);
         float *ld = reinterpret_cast<float *>(smem + buf * BYTES + 2 * TT * TL::ROWB);
         if (threadIdx.x < 2 * TT) {
             const int t = min(t0 + ((int)threadIdx.x & (TT - 1)), last);
@@ -368,31 +371,31 @@ template <int DT, int D> __global__ __launch_bounds__(64 * NW, DT == 1 && D == 6
     store_rows<DT, D>(a.dv + row, dv, 1.0f);
 }
 
-// dk and dv of the tiles in several parts: the parts' sums, in order.  One
-// workgroup per key tile and KV head; 4 elements per thread and pass.
-template <int DT, int D> __global__ __launch_bounds__(256) void swa_join(const Args a, int first) {
+// dk and dv of the tiles in several parts: the parts' sums, in order.  A workgroup
+// takes 1024 elements of one key tile and KV head, 4 a thread, so that there
+// are enough of them to keep HBM busy.
+constexpr int JE = 1024;
+template <int DT, int D> __global__ __launch_bounds__(JE / 4) void swa_join(const Args a, int first) {
     typedef typename St<DT>::T T;
-    const int combo = blockIdx.x % a.Cn, tile = first + blockIdx.x / a.Cn;
-    const int b = combo / a.Hkv, g = combo % a.Hkv, len = seq_len(a, b), k0 = tile * KB;
+    constexpr int PER = KB * 2 * D / JE;
+    const int e = blockIdx.x % PER * JE + threadIdx.x * 4, r = e / (2 * D), x = e % (2 * D);
+    const int combo = blockIdx.x / PER % a.Cn, tile = first + blockIdx.x / PER / a.Cn;
+    const int b = combo / a.Hkv, g = combo % a.Hkv, len = seq_len(a, b), k0 = tile * KB, j = k0 + r;
+    if (j >= a.n) return;
     const int P = tile < a.nst ? a.Ps : a.Pn;
-    const int used = min(P, (steps(k0, len, a.W, a.S) * a.G + a.chunk - 1) / a.chunk);
+    const int used = j < len ? min(P, (steps(k0, len, a.W, a.S) * a.G + a.chunk - 1) / a.chunk) : 0;
     const int slot = tile < a.nst ? tile * a.Ps : a.nst * a.Ps + (tile - a.nst) * a.Pn;
     const int64_t slots = a.nst * a.Ps + (a.ntiles - a.nst) * a.Pn;
-    const float *base = a.part + ((int64_t)combo * slots + slot) * KB * 2 * D;
-    for (int e = threadIdx.x * 4; e < KB * 2 * D; e += 1024) {
-        const int r = e / (2 * D), x = e % (2 * D), j = k0 + r;
-        if (j >= a.n) break;
-        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-        if (j < len)
-            for (int p = 0; p < used; ++p)
-                sum = sum + *reinterpret_cast<const f32x4 *>(base + (int64_t)p * KB * 2 * D + e);
-        const float f = x < D ? a.scale : 1.0f;
-        T *to = reinterpret_cast<T *>(x < D ? a.dk : a.dv) + (((int64_t)b * a.n + j) * a.Hkv + g) * D + x % D;
-        if constexpr (DT == 1)
-            *reinterpret_cast<uint2 *>(to) = make_uint2(pk_bf16(sum[0] * f, sum[1] * f), pk_bf16(sum[2] * f, sum[3] * f));
-        else
-            *reinterpret_cast<f32x4 *>(to) = sum * f;
-    }
+    const float *p = a.part + ((int64_t)combo * slots + slot) * KB * 2 * D + e;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = 0; i < used; ++i) sum = sum + *reinterpret_cast<const f32x4 *>(p + (int64_t)i * KB * 2 * D);
+    const float f = x < D ? a.scale : 1.0f;
+    T *to = reinterpret_cast<T *>(x < D ? a.dk : a.dv) + (((int64_t)b * a.n + j) * a.Hkv + g) * D + x % D;
+    if constexpr (DT == 1)
+        *reinterpret_cast<uint2 *>(to) = make_uint2(pk_bf16(sum[0] * f, sum[1] * f), pk_bf16(sum[2] * f, sum[3] * f));
+    else
+        *reinterpret_cast<f32x4 *>(to) = sum * f;
 }
 
 // How dk and dv are cut: steps of a part, so that some 1024 workgroups share the
@@ -446,11 +449,15 @@ template <int DT, int D> static int launch_bwd(Args a, int64_t grid, const Cut &
     HBA_LAUNCH_CHECK();
     const int first = c.Ps > 1 ? 0 : c.nst, end = c.Pn > 1 ? c.ntiles : c.nst;
     if (first < end) {
-        hipLaunchKernelGGL((swa_join<DT, D>), dim3((unsigned)((end - first) * a.Cn)), dim3(256), 0, s, a, first);
+        hipLaunchKernelGGL((swa_join<DT, D>), dim3((unsigned)((end - first) * a.Cn * (KB * 2 * D / JE))),
+                           dim3(JE / 4), 0, s, a, first);
         HBA_LAUNCH_CHECK();
     }
     return HBA_OK;
 }
+
+// Rows whose strides the kernels' 32-bit offsets within a tile can span.
+static bool rows_near(const int64_t *st, int64_t esz) { return st[1] * esz < (1 << 24); }
 
 static void set_strides(int64_t (&to)[3], const int64_t *from, int64_t esz) {
     for (int i = 0; i < 3; ++i) to[i] = from[i] * esz;
@@ -482,6 +489,7 @@ extern "C" int hba_swa_fwd(int dtype, const void *q, const int64_t q_strides[3],
         !abi::rows_aligned(dtype, v, v_strides) || !abi::aligned16(out))
         return HBA_ERR_UNSUPPORTED;
     const int64_t e = abi::elem_size(dtype);
+    if (!swa::rows_near(k_strides, e) || !swa::rows_near(v_strides, e)) return HBA_ERR_UNSUPPORTED;
     swa::Args a = {};
     a.q = (const char *)q;
     a.k = (const char *)k;
@@ -543,6 +551,9 @@ extern "C" int hba_swa_bwd(int dtype, const void *q, const int64_t q_strides[3],
         !abi::aligned16(workspace))
         return HBA_ERR_UNSUPPORTED;
     const int64_t e = abi::elem_size(dtype);
+    if (!swa::rows_near(q_strides, e) || !swa::rows_near(k_strides, e) || !swa::rows_near(v_strides, e) ||
+        !swa::rows_near(dout_strides, e))
+        return HBA_ERR_UNSUPPORTED;
     swa::Args a = {};
     a.q = (const char *)q;
     a.k = (const char *)k;

@@ -561,10 +561,11 @@ def _(q, k, v, kc, kr, q_gain, k_gain, eps, cos, sin, idx, cnt, out, dout, sinks
 
 # -------------------------------------------------- sliding-window attention ----
 def _rows16(t):
-    """t, or a copy of it, with a contiguous last dim and rows on 16-byte boundaries."""
+    """t, or a copy of it, with a contiguous last dim, rows on 16-byte boundaries and less
+    than 16 MiB from token to token."""
     q = 16 // t.element_size()
     st, sz = t.stride(), t.shape
-    if (st[-1] == 1 and t.data_ptr() % 16 == 0
+    if (st[-1] == 1 and t.data_ptr() % 16 == 0 and st[-3] * t.element_size() < 1 << 24
             and all(s % q == 0 or n == 1 for s, n in zip(st[:-1], sz[:-1]))):
         return t
     return t.clone(memory_format=torch.contiguous_format)
