@@ -49,7 +49,7 @@ struct Args {
 
 // A row's position and what it sees of its sequence.
 __device__ __forceinline__ int length(const Args &a, int s) {
-    return max(0, min(min(a.lens[s], a.max_len), a.maxp * rows::KT));
+    return max(0, min(min(a.lens[s], a.max_len), a.maxp * rows::PAGE));
 }
 
 // QKNorm, rotation at pos and scale of a row's elements x[ks][e] = element
@@ -122,8 +122,8 @@ struct Pages {
 __device__ __forceinline__ Pages page_list(const Args &a, int L) {
     Pages p;
     p.L = L;
-    p.lo = a.W > 0 ? max(0, L - a.W) : a.shared * rows::KT;
-    p.n = rows::tile_list(p.lo, L, a.W > 0 ? a.S : 0, p.ns, p.w0);
+    p.lo = a.W > 0 ? max(0, L - a.W) : a.shared * rows::PAGE;
+    p.n = rows::tile_list<rows::PAGE>(p.lo, L, a.W > 0 ? a.S : 0, p.ns, p.w0);
     return p;
 }
 
@@ -132,7 +132,7 @@ __device__ __forceinline__ Pages page_list(const Args &a, int L) {
 // registers.
 template <int DT, int D, int UK> __global__ __launch_bounds__(64 * DW) void decode_kernel(const Args a) {
     typedef typename Op<DT>::F F;
-    constexpr int ESZ = DT == 1 ? 2 : 4, NKS = D / 32, NDT = D / 16, NH = UK / 32, UP = rows::KT / UK;
+    constexpr int ESZ = DT == 1 ? 2 : 4, NKS = D / 32, NDT = D / 16, NH = UK / 32, UP = rows::PAGE / UK;
     __shared__ float so[DW][16][D + 4];
     __shared__ float sm[DW][16], sl[DW][16];
     const int lane = threadIdx.x & 63, l16 = lane & 15, lg = lane >> 4;
@@ -156,8 +156,8 @@ template <int DT, int D, int UK> __global__ __launch_bounds__(64 * DW) void deco
 #pragma unroll
         for (int ks = 0; ks < NKS; ++ks) split<DT>(x[ks], qh[ks], ql[ks]);
     }
-    const char *kb = a.kr + (int64_t)g * rows::KT * D * ESZ, *vb = a.v + (int64_t)g * rows::KT * D * ESZ;
-    const int64_t pstep = (int64_t)a.Hkv * rows::KT * D * ESZ;
+    const char *kb = a.kr + (int64_t)g * rows::PAGE * D * ESZ, *vb = a.v + (int64_t)g * rows::PAGE * D * ESZ;
+    const int64_t pstep = (int64_t)a.Hkv * rows::PAGE * D * ESZ;
     const int32_t *table = a.table + (int64_t)s * a.maxp;
     f32x4 O[NDT];
 #pragma unroll
@@ -168,7 +168,7 @@ template <int DT, int D, int UK> __global__ __launch_bounds__(64 * DW) void deco
         const int i = u / UP, h0 = UP == 1 ? 0 : u % UP, pl = i < pg.ns ? i : pg.w0 + i - pg.ns;
         const int64_t id = max((int64_t)0, min((int64_t)table[pl], a.pages - 1));
         const char *kp = kb + id * pstep, *vp = vb + id * pstep;
-        const int j0 = pl * rows::KT + 32 * h0;
+        const int j0 = pl * rows::PAGE + 32 * h0;
         F kf[2 * NH][NKS], vf[NDT][NH];
 #pragma unroll
         for (int mt = 0; mt < 2 * NH; ++mt)
@@ -316,8 +316,8 @@ template <int DT, int D, bool SHARED> __global__ __launch_bounds__(64 * rows::NW
     w.S = a.W > 0 ? a.S : 0;
     w.hi = in && pos >= 0 ? pos + 1 : 0;
     w.lo = a.W > 0 ? max(0, pos + 1 - a.W) : 0;
-    if constexpr (SHARED) w.hi = min(w.hi, a.shared * rows::KT);
-    else if (a.shared) w.lo = a.shared * rows::KT;
+    if constexpr (SHARED) w.hi = min(w.hi, a.shared * rows::PAGE);
+    else if (a.shared) w.lo = a.shared * rows::PAGE;
     // the wave's and the workgroup's bounds, over the rows that see anything
     int v[4] = {w.hi ? w.lo : 0x7fffffff, w.hi ? w.lo : 0, in ? w.hi : 0x7fffffff, w.hi};
 #pragma unroll
@@ -344,7 +344,7 @@ template <int DT, int D, bool SHARED> __global__ __launch_bounds__(64 * rows::NW
         hi = max(hi, bounds[i][1]);
     }
     int ns = 0, wt0 = 0;
-    const int nt = hi > 0 ? rows::tile_list(lo, hi, w.S, ns, wt0) : 0;
+    const int nt = hi > 0 ? rows::tile_list<rows::KEYS<DT, D>>(lo, hi, w.S, ns, wt0) : 0;
     const int z = blockIdx.z, it0 = (int)((int64_t)nt * z / a.part), it1 = (int)((int64_t)nt * (z + 1) / a.part);
 
     F qh[NKS], ql[NKS];
@@ -360,9 +360,9 @@ template <int DT, int D, bool SHARED> __global__ __launch_bounds__(64 * rows::NW
         for (int ks = 0; ks < NKS; ++ks) split<DT>(x[ks], qh[ks], ql[ks]);
     }
     rows::PageKV<DT, D> src;
-    src.page = (int64_t)a.Hkv * rows::KT * D * ESZ;
-    src.k = a.kr + (int64_t)g * rows::KT * D * ESZ;
-    src.v = a.v + (int64_t)g * rows::KT * D * ESZ;
+    src.page = (int64_t)a.Hkv * rows::PAGE * D * ESZ;
+    src.k = a.kr + (int64_t)g * rows::PAGE * D * ESZ;
+    src.v = a.v + (int64_t)g * rows::PAGE * D * ESZ;
     src.table = a.table + (SHARED ? 0 : (int64_t)s * a.maxp);
     src.pages = a.pages;
     rows::RowAcc<DT, D> acc;
@@ -478,7 +478,7 @@ struct Plan {
 static Plan plan(int64_t T, int64_t Bd, int64_t Hq, int64_t Hkv, int64_t W, int64_t S, int64_t shared, bool one,
                  int64_t max_len) {
     Plan p = {};
-    const int64_t G = Hq / Hkv, KT = rows::KT;
+    const int64_t G = Hq / Hkv, KT = rows::PAGE;
     int64_t keys = max_len - shared * KT;
     if (W > 0 && W < keys) keys = W;
     if (keys < 1) keys = 1;
@@ -591,7 +591,7 @@ extern "C" int hba_paged_attn(int dtype, const void *q, const int64_t q_strides[
                               int64_t shared_pages, int64_t max_len, void *workspace, size_t ws_bytes, void *out,
                               void *stream) {
     if (int st = abi::check_dtype_dim(dtype, d)) return st;
-    if (Bk != rows::KT) return HBA_ERR_UNSUPPORTED;
+    if (Bk != rows::PAGE) return HBA_ERR_UNSUPPORTED;
     if (int st = paged::check(T, Bd, Hq, Hkv, d, W, S, shared_pages, cu == nullptr, max_len, max_pages)) return st;
     if (!q || !q_strides || !kr_pages || !v_pages || !page_table || !seq_lens || !scales || !out || num_pages <= 0 ||
         !cos_tab != !sin_tab || (cos_tab && n_tab <= 0))

@@ -1,4 +1,4 @@
-// Attention of a tile of query rows to 64-key tiles, shared by the sliding-window
+// Attention of a tile of query rows to tiles of keys, shared by the sliding-window
 // and the paged-cache kernels (bf16 and fp32, head dim 64 / 128).
 //
 // A wave holds 32 query rows as the columns of S^T = K . Q^T on 32x32 MFMA
@@ -31,7 +31,10 @@ namespace rows {
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef unsigned int u32x4r __attribute__((ext_vector_type(4)));
 
-constexpr int KT = 64;            // keys per tile
+constexpr int PAGE = 64;          // tokens of a cache page
+// Keys per staged tile: 8 KB of keys and as much of values, but 32 keys at least,
+// so that two buffers leave LDS for as many workgroups as the registers do.
+template <int DT, int D> constexpr int KEYS = D * (DT == 1 ? 2 : 4) <= 128 ? 64 : 32;
 constexpr int NW = 4;             // waves per workgroup
 constexpr int RW = 32;            // query rows per wave
 constexpr int RT = NW * RW;       // query rows per workgroup
@@ -198,7 +201,7 @@ template <int DT, int D> struct Tile {
 template <int DT, int D> struct DenseKV {
     typedef typename Op<DT>::F F;
     typedef Tile<DT, D> TL;
-    static constexpr int BYTES = 2 * KT * TL::ROWB;   // a staged tile: keys, then values
+    static constexpr int KT = KEYS<DT, D>, BYTES = 2 * KT * TL::ROWB;   // a staged tile: keys, then values
     const char *k, *v;
     int64_t kb, vb;                                   // bytes from row to row
     int last;                                         // the last row that may be read
@@ -223,32 +226,39 @@ template <int DT, int D> struct DenseKV {
 };
 
 // Keys and values of one KV head in 64-token pages (page_key_off, page_val_off):
-// a tile is a page as it lies in memory.  Row l % 32 of a key operand is the
+// a tile is a page or half of one as it lies in memory (the tokens of a half are
+// a run of the keys and every other KB of the values).  Row l % 32 of a key operand is the
 // token for which the result's registers 8u .. 8u+7 of half h are the tokens
 // 16 u + 8 h .. + 7, the order in which the pages hold values.
 template <int DT, int D> struct PageKV {
     typedef typename Op<DT>::F F;
+    static constexpr int KT = KEYS<DT, D>, TP = PAGE / KT;   // tiles of a page
     static constexpr int ESZ = DT == 1 ? 2 : 4, HALF = KT * D * ESZ, BYTES = 2 * HALF;
     const char *k, *v;            // the KV head's place in page 0
     int64_t page;                 // bytes from page to page
     const int32_t *table;         // the sequence's pages
     int64_t pages;                // pages there are
     int64_t id;                   // the page of the tile that is staged next
+    int half;                     // and the tile's place in it
 
-    __device__ __forceinline__ int64_t at(int tile) const {
-        const int p = __builtin_amdgcn_readfirstlane(table[tile]);
+    __device__ __forceinline__ int64_t at(int lp) const {
+        const int p = __builtin_amdgcn_readfirstlane(table[lp]);
         return p < 0 ? 0 : (p < pages ? p : pages - 1);   // never outside the cache
     }
-    __device__ __forceinline__ void next(int tile) { id = at(tile); }
+    __device__ __forceinline__ void next(int tile) {
+        id = at(tile / TP);
+        half = tile % TP;
+    }
     __device__ __forceinline__ void stage(int, uint32_t lds) const {
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const uint32_t off = (threadIdx.x & 63) * 16;
-        const char *kp = k + id * page, *vp = v + id * page;
+        const char *kp = k + id * page + half * HALF, *vp = v + id * page + half * 512 * ESZ;
 #pragma unroll
         for (int i = 0; i < HALF / 1024 / NW; ++i) {
             const int c = (i * NW + wave) * 1024;
             dma16s(kp + c, off, lds + c);
-            dma16s(vp + c, off, lds + HALF + c);
+            // chunk run dt * 2 + half of a page becomes run dt of a half tile
+            dma16s(vp + (TP == 1 ? c : c / (512 * ESZ) * (1024 * ESZ) + c % (512 * ESZ)), off, lds + HALF + c);
         }
     }
     static __device__ __forceinline__ int key(int r, int hf) {
@@ -260,17 +270,17 @@ template <int DT, int D> struct PageKV {
     }
     static __device__ __forceinline__ F vf(const char *t, int kt, int dt, int u, int lane) {
         const int x = 32 * dt + (lane & 31);
-        return Op<DT>::load(t + HALF + (((x >> 4) * 2 + kt) * 64 + (x & 15) + 16 * (2 * u + (lane >> 5))) * 8 * ESZ);
+        return Op<DT>::load(t + HALF + (((x >> 4) * (KT / 32) + kt) * 64 + (x & 15) + 16 * (2 * u + (lane >> 5))) * 8 * ESZ);
     }
     // one key, for attend_each
     __device__ __forceinline__ float dot_one(const F (&q)[D / 16], int j, int hf) const {
-        const char *t = k + at(j / KT) * page;
+        const char *t = k + at(j / PAGE) * page;
         float sum = 0.0f;
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
             float a[8], b[8];
             Op<DT>::unpack(q[ks], a);
-            Op<DT>::unpack(Op<DT>::load(t + page_key_off(j % KT, 16 * ks + 8 * hf, D) * ESZ), b);
+            Op<DT>::unpack(Op<DT>::load(t + page_key_off(j % PAGE, 16 * ks + 8 * hf, D) * ESZ), b);
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum = fmaf(a[e], b[e], sum);
         }
@@ -283,12 +293,12 @@ template <int DT, int D> struct PageKV {
     }
     __device__ __forceinline__ void add(f32x16 (&o)[D / 32], int j, float p, int hf) const {
         typedef typename St<DT>::T T;
-        const T *t = reinterpret_cast<const T *>(v + at(j / KT) * page);
+        const T *t = reinterpret_cast<const T *>(v + at(j / PAGE) * page);
 #pragma unroll
         for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-                o[dt][r] = fmaf(p, St<DT>::ld(t, page_val_off(j % KT, 32 * dt + 8 * (r >> 2) + 4 * hf + (r & 3))),
+                o[dt][r] = fmaf(p, St<DT>::ld(t, page_val_off(j % PAGE, 32 * dt + 8 * (r >> 2) + 4 * hf + (r & 3))),
                                 o[dt][r]);
     }
 };
@@ -360,14 +370,14 @@ __device__ __forceinline__ void attend(Src &src, char *smem, const typename Op<D
                                        const typename Op<DT>::F *qlo, float c, int it0, int it1, int ns, int wt0,
                                        const Sees &w, RowAcc<DT, D> &a) {
     typedef typename Op<DT>::F F;
-    constexpr int NKS = D / 16, NDT = D / 32;
+    constexpr int NKS = D / 16, NDT = D / 32, KT = Src::KT;
     const int lane = threadIdx.x & 63, hf = lane >> 5;
     const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) a.O[dt] = zero;
     a.m = -INFINITY;
     a.l = 0.0f;
-    float shift = INFINITY;   // -m: every probability is infinite (or NaN) while nothing is seen
+    float shift = 0.0f;   // -m, or 0 while nothing is seen
     const uint32_t lds = lds_offset(smem);
     const auto tile = [&](int it) { return it < ns ? it : wt0 + it - ns; };
     if (it0 < it1) {
@@ -387,81 +397,63 @@ __device__ __forceinline__ void attend(Src &src, char *smem, const typename Op<D
         const int j0 = tile(it) * KT;
         if (j0 >= w.hi_max || (j0 + KT <= w.lo_min && j0 >= w.S)) continue;   // nothing the wave's rows see
         const char *t = smem + cur * Src::BYTES;
-        const bool whole = j0 + KT <= w.hi_min && (j0 >= w.lo_max || j0 + KT <= w.S);
-        // the tile's logits (LO: in log2 units, above `from`), masked
-        const auto logits = [&](f32x16 (&s)[2], float from) {
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt) {
-                s[kt] = zero;
-                if constexpr (LO) s[kt] = s[kt] + from;
+        for (int kt = 0; kt < KT / 32; ++kt) {   // 32 keys at a time: fewer registers, and halves that no row sees cost nothing
+            const int jh = j0 + 32 * kt;
+            if (jh >= w.hi_max || (jh + 32 <= w.lo_min && jh >= w.S)) continue;
+            f32x16 s = zero;
+            if constexpr (LO) s = s + shift;
 #pragma unroll
-                for (int ks = 0; ks < NKS; ++ks) {
-                    const F kf = src.kf(t, kt, ks, lane);
-                    s[kt] = Op<DT>::mma(kf, q[ks], s[kt]);
-                    if constexpr (LO) s[kt] = Op<DT>::mma(kf, qlo[ks], s[kt]);
-                }
+            for (int ks = 0; ks < NKS; ++ks) {
+                const F kf = src.kf(t, kt, ks, lane);
+                s = Op<DT>::mma(kf, q[ks], s);
+                if constexpr (LO) s = Op<DT>::mma(kf, qlo[ks], s);
             }
-            if (!whole) {
-                const uint64_t see = seen_bits(w.lo, w.hi, w.S, j0) >> Src::key(0, hf);
+            if (!(jh + 32 <= w.hi_min && (jh >= w.lo_max || jh + 32 <= w.S))) {
+                const uint64_t see = seen_bits(w.lo, w.hi, w.S, jh) >> Src::key(0, hf);
 #pragma unroll
-                for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[kt][r] = keep(s[kt][r], see, 32 * kt + Src::key(r, 0), -INFINITY);
+                for (int r = 0; r < 16; ++r) s[r] = keep(s[r], see, Src::key(r, 0), -INFINITY);
             }
-        };
-        // probabilities 2^(c s + by) as operands, and this half's sum of them
-        const auto weights = [&](const f32x16 (&s)[2], float by, F (&p)[2][2]) {
-            float sum = 0.0f;
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
+            // probabilities 2^(c s + by) as operands, and this half's sum of them
+            F p[2];
+            const auto weights = [&](float by) {
+                float sum = 0.0f;
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     float x[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float y = s[kt][8 * u + e];
-                        x[e] = ex2(LO ? y : fmaf(y, c, by));
-                    }
-                    p[kt][u] = Op<DT>::pack(x);
-                    sum = Op<DT>::sum(p[kt][u], sum);
+                    for (int e = 0; e < 8; ++e)
+                        x[e] = ex2(LO ? s[8 * u + e] : fmaf(s[8 * u + e], c, by));
+                    p[u] = Op<DT>::pack(x);
+                    sum = Op<DT>::sum(p[u], sum);
                 }
-            return sum;
-        };
-        f32x16 s[2];
-        F p[2][2];
-        logits(s, shift);
-        float sum = weights(s, shift, p);
-        if (__ballot(!(sum <= MOST))) {   // a new maximum
-            asm volatile("" ::: "memory");   // the keys once more from LDS: registers for them would be held in every tile
-            logits(s, 0.0f);
-            float mx = s[0][0];
+                return sum;
+            };
+            float sum = weights(shift);
+            if (__ballot(!(sum <= MOST) || a.m == -INFINITY)) {   // a new maximum
+                float mx = s[0];
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
+                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[r]);
+                mx = fmaxf(mx, other_half(mx));
+                mx = fmaxf(a.m, LO ? mx - shift : mx * c);
+                const float al = a.m == -INFINITY ? 0.0f : ex2(a.m - mx);   // nothing to rescale yet
+                a.l *= al;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kt][r]);
-            mx = fmaxf(a.m, fmaxf(mx, other_half(mx)) * c);
-            const float al = a.m == -INFINITY ? 0.0f : ex2(a.m - mx);   // nothing to rescale yet
-            a.l *= al;
+                for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
-            for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) a.O[dt][r] *= al;
-            a.m = mx;
-            shift = -mx;
-            const float by = mx == -INFINITY ? 0.0f : -mx;   // rows that still see nothing: 2^-inf
-            if constexpr (LO) {
-                s[0] = s[0] + by;
-                s[1] = s[1] + by;
+                    for (int r = 0; r < 16; ++r) a.O[dt][r] *= al;
+                a.m = mx;
+                const float by = mx == -INFINITY ? 0.0f : -mx;   // rows that still see nothing: 2^-inf
+                if constexpr (LO) s = s + (by - shift);
+                shift = by;
+                sum = weights(shift);
             }
-            sum = weights(s, by, p);
-        }
-        a.l += sum;
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
+            a.l += sum;
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int dt = 0; dt < NDT; ++dt) a.O[dt] = Op<DT>::mma(src.vf(t, kt, dt, u, lane), p[kt][u], a.O[dt]);
+                for (int dt = 0; dt < NDT; ++dt) a.O[dt] = Op<DT>::mma(src.vf(t, kt, dt, u, lane), p[u], a.O[dt]);
+        }
     }
     __syncthreads();
 }
@@ -516,9 +508,9 @@ __device__ __forceinline__ void attend_each(const Src &src, const typename Op<DT
     a.l = 0.0f;
 #pragma unroll 1
     for (int it = it0; it < it1; ++it) {
-        const int j0 = (it < ns ? it : wt0 + it - ns) * KT;
+        const int j0 = (it < ns ? it : wt0 + it - ns) * Src::KT;
 #pragma unroll 1
-        for (int j = j0; j < min(j0 + KT, w.hi_max); ++j) {
+        for (int j = j0; j < min(j0 + Src::KT, w.hi_max); ++j) {
             float s = src.template dot<LO>(q, qlo, j, hf) * c;
             if (!(j < w.hi && (j >= w.lo || j < w.S))) continue;
             if (s != s) {   // a NaN makes the row NaN
@@ -538,10 +530,10 @@ __device__ __forceinline__ void attend_each(const Src &src, const typename Op<DT
     }
 }
 
-// The list of 64-key tiles that rows with first visible key lo (the smallest),
+// The list of KT-key tiles that rows with first visible key lo (the smallest),
 // one past the last hi (the largest) and S sinks see: ns tiles of sinks, then
 // tiles wt0 ...; returns how many.
-__device__ __forceinline__ int tile_list(int lo, int hi, int S, int &ns, int &wt0) {
+template <int KT> __device__ __forceinline__ int tile_list(int lo, int hi, int S, int &ns, int &wt0) {
     wt0 = lo / KT;
     ns = min((min(S, hi) + KT - 1) / KT, wt0);
     const int wt1 = (hi + KT - 1) / KT;

@@ -7,7 +7,7 @@
 //   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i
 //
 // Forward and dq: a workgroup has 128 rows of one KV head's query heads
-// (hba_rows.h) and walks the 64-key tiles that they see.  dk and dv: a workgroup
+// (hba_rows.h) and walks the tiles of keys that they see.  dk and dv: a workgroup
 // has 128 keys as the columns of S = Q . K^T and walks its KV head's query heads
 // and their 64-token tiles, so the sum over the heads of a group stays in
 // registers and nothing is added by atomics: the gradients are the same bits
@@ -109,7 +109,7 @@ template <int DT, int D> __global__ __launch_bounds__(64 * NW, (DT == 1 && D == 
     load_rows<DT, D>(a.q + x.b * a.qs[0] + x.tok * a.qs[1] + x.head * a.qs[2], x.valid, q);
     DenseKV<DT, D> src = keys<DT, D>(a, x);
     int ns, wt0;
-    const int nt = tile_list(x.lo, x.hi, a.S, ns, wt0);
+    const int nt = tile_list<KEYS<DT, D>>(x.lo, x.hi, a.S, ns, wt0);
     RowAcc<DT, D> acc;
     float l, inv;
     attend<DT, D, false>(src, smem, q, nullptr, a.c, 0, nt, ns, wt0, x.w, acc);
@@ -136,7 +136,7 @@ template <int DT, int D> __global__ __launch_bounds__(64 * NW, DT == 1 ? 2 : 1) 
     extern __shared__ __align__(16) char smem[];
     typedef Tile<DT, D> TL;
     typedef typename Op<DT>::F F;
-    constexpr int ESZ = TL::ESZ, NKS = D / 16, NDT = D / 32;
+    constexpr int ESZ = TL::ESZ, NKS = D / 16, NDT = D / 32, KT = KEYS<DT, D>;
     const int lane = threadIdx.x & 63, hf = lane >> 5;
     Rows x;
     if (!find_rows<D>(a, x)) return;
@@ -163,7 +163,7 @@ template <int DT, int D> __global__ __launch_bounds__(64 * NW, DT == 1 ? 2 : 1) 
     const float lse = x.valid ? a.lse[hrow] : INFINITY;
     const DenseKV<DT, D> src = keys<DT, D>(a, x);
     int ns, wt0;
-    const int nt = tile_list(x.lo, x.hi, a.S, ns, wt0);
+    const int nt = tile_list<KEYS<DT, D>>(x.lo, x.hi, a.S, ns, wt0);
     const uint32_t lds = lds_offset(smem);
     const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     f32x16 acc[NDT];
@@ -179,9 +179,10 @@ template <int DT, int D> __global__ __launch_bounds__(64 * NW, DT == 1 ? 2 : 1) 
         const int j0 = (it < ns ? it : wt0 + it - ns) * KT;
         if (j0 >= x.w.hi_max || (j0 + KT <= x.w.lo_min && j0 >= a.S)) continue;
         const char *t = smem + cur * src.BYTES;
-        const bool whole = j0 + KT <= x.w.hi_min && (j0 >= x.w.lo_max || j0 + KT <= a.S);
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
+        for (int kt = 0; kt < KT / 32; ++kt) {
+            const int jh = j0 + 32 * kt;
+            if (jh >= x.w.hi_max || (jh + 32 <= x.w.lo_min && jh >= a.S)) continue;
             f32x16 s = zero, dp = zero;
 #pragma unroll
             for (int ks = 0; ks < NKS; ++ks) {
@@ -190,8 +191,8 @@ template <int DT, int D> __global__ __launch_bounds__(64 * NW, DT == 1 ? 2 : 1) 
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = ex2(fmaf(s[r], a.c, -lse)) * (dp[r] - delta);
-            if (!whole) {
-                const uint64_t see = seen_bits(x.w.lo, x.w.hi, a.S, j0 + 32 * kt) >> src.key(0, hf);
+            if (!(jh + 32 <= x.w.hi_min && (jh >= x.w.lo_max || jh + 32 <= a.S))) {
+                const uint64_t see = seen_bits(x.w.lo, x.w.hi, a.S, jh) >> src.key(0, hf);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = keep(s[r], see, src.key(r, 0), 0.0f);
             }
@@ -439,7 +440,7 @@ template <int DT, int D> static int launch_fwd(const Args &a, int64_t grid, hipS
 }
 
 template <int DT, int D> static int launch_bwd(Args a, int64_t grid, const Cut &c, hipStream_t s) {
-    constexpr size_t lds = 2 * DenseKV<DT, D>::BYTES, ldk = lds + 2 * 2 * TT * 4;
+    constexpr size_t lds = 2 * DenseKV<DT, D>::BYTES, ldk = 2 * (2 * TT * Tile<DT, D>::ROWB + 2 * TT * 4);
     if (int st = lds_room<DT, D>(swa_dq<DT, D>, lds)) return st;
     if (int st = lds_room<DT, D>(swa_dkv<DT, D>, ldk)) return st;
     hipLaunchKernelGGL((swa_dq<DT, D>), dim3((unsigned)grid), dim3(64 * NW), lds, s, a);
