@@ -469,6 +469,7 @@ __device__ __forceinline__ float dot_rows(const typename Op<DT>::F (&x)[D / 16],
         Op<DT>::unpack(Op<DT>::load(p + (16 * ks + 8 * hf) * Tile<DT, D>::ESZ), y);
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum = fmaf(u[e], y[e], sum);
+        __builtin_amdgcn_sched_barrier(0);   // few registers, not speed: see attend_each
     }
     return sum + other_half(sum);
 }
@@ -479,9 +480,11 @@ __device__ __forceinline__ void add_row(f32x16 (&o)[D / 32], const char *p, floa
     typedef typename St<DT>::T T;
     const T *x = reinterpret_cast<const T *>(p);
 #pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
+    for (int dt = 0; dt < D / 32; ++dt) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[dt][r] = fmaf(f, St<DT>::ld(x, 32 * dt + 8 * (r >> 2) + 4 * hf + (r & 3)), o[dt][r]);
+        __builtin_amdgcn_sched_barrier(0);
+    }
 }
 
 template <int DT, int D>
@@ -495,7 +498,8 @@ __device__ __forceinline__ void DenseKV<DT, D>::add(f32x16 (&o)[D / 32], int j, 
 }
 
 // attend, one key at a time: for rows that came out non-finite.  Each lane adds
-// the visible keys only, so nothing of a masked key reaches its row.
+// the visible keys only, so nothing of a masked key reaches its row.  It is kept
+// from loading ahead: its registers would cost the kernels that hold it waves.
 template <int DT, int D, bool LO, class Src>
 __device__ __forceinline__ void attend_each(const Src &src, const typename Op<DT>::F (&q)[D / 16],
                                          const typename Op<DT>::F *qlo, float c, int it0, int it1, int ns, int wt0,

@@ -35,6 +35,7 @@ struct Args {
     float *lse, *delta;                 // [B, Hq, n]: log2-sum-exp2 (+inf: no row), do . o
     char *dq, *dk, *dv;
     float *part;                        // dk / dv sums of tiles in several parts
+    int32_t *marks;                     // waves of swa_dkv whose sums are not finite
     int nst, Ps, Pn, chunk;             // tiles of sinks, parts of those and of the others, steps of a part
 };
 
@@ -100,76 +101,134 @@ template <int DT, int D> __device__ __forceinline__ DenseKV<DT, D> keys(const Ar
     return s;
 }
 
-template <int DT, int D> __global__ __launch_bounds__(64 * NW, (DT == 1 && D == 64 ? 3 : WAVES<DT, D>)) void swa_fwd(const Args a) {
-    extern __shared__ __align__(16) char smem[];
-    constexpr int ESZ = Tile<DT, D>::ESZ;
-    Rows x;
-    if (!find_rows<D>(a, x)) return;
-    typename Op<DT>::F q[D / 16];
-    load_rows<DT, D>(a.q + x.b * a.qs[0] + x.tok * a.qs[1] + x.head * a.qs[2], x.valid, q);
-    DenseKV<DT, D> src = keys<DT, D>(a, x);
-    int ns, wt0;
-    const int nt = tile_list<KEYS<DT, D>>(x.lo, x.hi, a.S, ns, wt0);
-    RowAcc<DT, D> acc;
-    float l, inv;
-    attend<DT, D, false>(src, smem, q, nullptr, a.c, 0, nt, ns, wt0, x.w, acc);
-    l = acc.l + other_half(acc.l);
-    if (__ballot(x.valid && (any_bad<D>(acc.O) || !finite(l)))) {
-        attend_each<DT, D, false>(src, q, nullptr, a.c, 0, nt, ns, wt0, x.w, acc);
-        l = acc.l + other_half(acc.l);
-    }
-    inv = x.valid ? 1.0f / l : 0.0f;
+template <int DT, int D>
+__device__ __forceinline__ void store_fwd(const Args &a, const Rows &x, RowAcc<DT, D> &acc, float l) {
     if (!x.in) return;
     if (!x.valid) {   // a row behind its sequence: 0
 #pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt) acc.O[dt] = acc.O[dt] - acc.O[dt];
+        for (int dt = 0; dt < D / 32; ++dt) acc.O[dt] = f32x16{0.0f};
     }
     const int64_t row = ((int64_t)x.b * a.n + x.tok) * a.Hq + x.head;
-    store_rows<DT, D>(a.out + row * D * ESZ, acc.O, inv);
+    store_rows<DT, D>(a.out + row * D * Tile<DT, D>::ESZ, acc.O, x.valid ? 1.0f / l : 0.0f);
     if (a.lse && (threadIdx.x & 32) == 0)
         a.lse[((int64_t)x.b * a.Hq + x.head) * a.n + x.tok] = x.valid ? acc.m + __log2f(l) : INFINITY;
 }
 
+template <int DT, int D>
+__device__ __forceinline__ const char *q_row(const Args &a, const Rows &x) {
+    return a.q + x.b * a.qs[0] + x.tok * a.qs[1] + x.head * a.qs[2];
+}
+template <int DT, int D>
+__device__ __forceinline__ const char *dout_row(const Args &a, const Rows &x) {
+    return a.dout + x.b * a.dos[0] + x.tok * a.dos[1] + x.head * a.dos[2];
+}
+
+template <int DT, int D>
+__global__ __launch_bounds__(64 * NW, (DT == 1 && D == 64 ? 3 : WAVES<DT, D>)) void swa_fwd(const Args a) {
+    extern __shared__ __align__(16) char smem[];
+    Rows x;
+    if (!find_rows<D>(a, x)) return;
+    typename Op<DT>::F q[D / 16];
+    load_rows<DT, D>(q_row<DT, D>(a, x), x.valid, q);
+    DenseKV<DT, D> src = keys<DT, D>(a, x);
+    int ns, wt0;
+    const int nt = tile_list<KEYS<DT, D>>(x.lo, x.hi, a.S, ns, wt0);
+    RowAcc<DT, D> acc;
+    attend<DT, D, false>(src, smem, q, nullptr, a.c, 0, nt, ns, wt0, x.w, acc);
+    float l = acc.l + other_half(acc.l);
+    if (__ballot(x.valid && (any_bad<D>(acc.O) || !finite(l)))) {
+        attend_each<DT, D, false>(src, q, nullptr, a.c, 0, nt, ns, wt0, x.w, acc);
+        l = acc.l + other_half(acc.l);
+    }
+    store_fwd<DT, D>(a, x, acc, l);
+}
+
 // The probabilities' gradient from the forward's log-sum-exps, and dq; delta =
 // do . o on the way, for dk and dv.
+template <int DT, int D>
+__device__ __forceinline__ float row_delta(const Args &a, const Rows &x, const typename Op<DT>::F (&dO)[D / 16]) {
+    typename Op<DT>::F o[D / 16];
+    load_rows<DT, D>(a.out + (((int64_t)x.b * a.n + x.tok) * a.Hq + x.head) * D * Tile<DT, D>::ESZ, x.valid, o);
+    float delta = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+        float u[8], w[8];
+        Op<DT>::unpack(o[ks], u);
+        Op<DT>::unpack(dO[ks], w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) delta = fmaf(u[e], w[e], delta);
+    }
+    return delta + other_half(delta);
+}
+
+template <int DT, int D>
+__device__ __forceinline__ void store_dq(const Args &a, const Rows &x, f32x16 (&acc)[D / 32]) {
+    if (!x.in) return;
+    if (!x.valid) {
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) acc[dt] = f32x16{0.0f};
+    }
+    store_rows<DT, D>(a.dq + (((int64_t)x.b * a.n + x.tok) * a.Hq + x.head) * D * Tile<DT, D>::ESZ, acc, a.scale);
+}
+
+// The wave's rows of swa_dq key by key, the masked ones left out.  It finds its rows
+// again: what swa_dq would hold for it through its loop costs a wave per SIMD.
+template <int DT, int D> __device__ __forceinline__ void dq_each(const Args a) {
+    typedef typename Op<DT>::F F;
+    constexpr int KT = KEYS<DT, D>;
+    const int hf = (threadIdx.x & 63) >> 5;
+    Rows x;
+    find_rows<D>(a, x);
+    F q[D / 16], dO[D / 16];
+    load_rows<DT, D>(q_row<DT, D>(a, x), x.valid, q);
+    load_rows<DT, D>(dout_row<DT, D>(a, x), x.valid, dO);
+    const float delta = row_delta<DT, D>(a, x, dO);
+    const float lse = x.valid ? a.lse[((int64_t)x.b * a.Hq + x.head) * a.n + x.tok] : INFINITY;
+    const DenseKV<DT, D> src = keys<DT, D>(a, x);
+    int ns, wt0;
+    const int nt = tile_list<KT>(x.lo, x.hi, a.S, ns, wt0);
+    f32x16 acc[D / 32];
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) acc[dt] = f32x16{0.0f};
+#pragma unroll 1
+    for (int it = 0; it < nt; ++it) {
+        const int j0 = (it < ns ? it : wt0 + it - ns) * KT;
+#pragma unroll 1
+        for (int j = j0; j < min(j0 + KT, x.w.hi_max); ++j) {
+            const char *kj = src.k + (int64_t)min(j, src.last) * src.kb;
+            const float s = dot_rows<DT, D>(q, kj, hf);
+            const float dp = dot_rows<DT, D>(dO, src.v + (int64_t)min(j, src.last) * src.vb, hf);
+            if (j < x.w.hi && (j >= x.w.lo || j < a.S))
+                add_row<DT, D>(acc, kj, ex2(fmaf(s, a.c, -lse)) * (dp - delta), hf);
+        }
+    }
+    store_dq<DT, D>(a, x, acc);
+}
+
 template <int DT, int D> __global__ __launch_bounds__(64 * NW, DT == 1 ? 2 : 1) void swa_dq(const Args a) {
     extern __shared__ __align__(16) char smem[];
     typedef Tile<DT, D> TL;
     typedef typename Op<DT>::F F;
-    constexpr int ESZ = TL::ESZ, NKS = D / 16, NDT = D / 32, KT = KEYS<DT, D>;
+    constexpr int NKS = D / 16, NDT = D / 32, KT = KEYS<DT, D>;
     const int lane = threadIdx.x & 63, hf = lane >> 5;
     Rows x;
     if (!find_rows<D>(a, x)) return;
-    F q[NKS], dO[NKS];
-    load_rows<DT, D>(a.q + x.b * a.qs[0] + x.tok * a.qs[1] + x.head * a.qs[2], x.valid, q);
-    load_rows<DT, D>(a.dout + x.b * a.dos[0] + x.tok * a.dos[1] + x.head * a.dos[2], x.valid, dO);
-    const int64_t row = ((int64_t)x.b * a.n + x.tok) * a.Hq + x.head;
-    const int64_t hrow = ((int64_t)x.b * a.Hq + x.head) * a.n + x.tok;
-    float delta = 0.0f;
-    {
-        F o[NKS];
-        load_rows<DT, D>(a.out + row * D * ESZ, x.valid, o);
-#pragma unroll
-        for (int ks = 0; ks < NKS; ++ks) {
-            float u[8], w[8];
-            Op<DT>::unpack(o[ks], u);
-            Op<DT>::unpack(dO[ks], w);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) delta = fmaf(u[e], w[e], delta);
-        }
-        delta += other_half(delta);
-        if (x.valid && hf == 0) a.delta[hrow] = delta;
-    }
-    const float lse = x.valid ? a.lse[hrow] : INFINITY;
     const DenseKV<DT, D> src = keys<DT, D>(a, x);
     int ns, wt0;
-    const int nt = tile_list<KEYS<DT, D>>(x.lo, x.hi, a.S, ns, wt0);
+    const int nt = tile_list<KT>(x.lo, x.hi, a.S, ns, wt0);
     const uint32_t lds = lds_offset(smem);
-    const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (nt > 0) src.stage(0 < ns ? 0 : wt0, lds);
+    F q[NKS], dO[NKS];
+    load_rows<DT, D>(q_row<DT, D>(a, x), x.valid, q);
+    load_rows<DT, D>(dout_row<DT, D>(a, x), x.valid, dO);
+    const int64_t hrow = ((int64_t)x.b * a.Hq + x.head) * a.n + x.tok;
+    const float delta = row_delta<DT, D>(a, x, dO);
+    if (x.valid && hf == 0) a.delta[hrow] = delta;
+    const float lse = x.valid ? a.lse[hrow] : INFINITY;
+    const f32x16 zero = {0.0f};
     f32x16 acc[NDT];
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) acc[dt] = zero;
-    if (nt > 0) src.stage(0 < ns ? 0 : wt0, lds);
 #pragma unroll 1
     for (int it = 0; it < nt; ++it) {
         wait_vm<0>();
@@ -184,13 +243,14 @@ template <int DT, int D> __global__ __launch_bounds__(64 * NW, DT == 1 ? 2 : 1) 
             const int jh = j0 + 32 * kt;
             if (jh >= x.w.hi_max || (jh + 32 <= x.w.lo_min && jh >= a.S)) continue;
             f32x16 s = zero, dp = zero;
+            dp = dp - delta;
 #pragma unroll
             for (int ks = 0; ks < NKS; ++ks) {
                 s = Op<DT>::mma(src.kf(t, kt, ks, lane), q[ks], s);
                 dp = Op<DT>::mma(TL::row(t + KT * TL::ROWB, 32 * kt + (lane & 31), ks, hf), dO[ks], dp);
             }
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = ex2(fmaf(s[r], a.c, -lse)) * (dp[r] - delta);
+            for (int r = 0; r < 16; ++r) s[r] = ex2(fmaf(s[r], a.c, -lse)) * dp[r];
             if (!(jh + 32 <= x.w.hi_min && (jh >= x.w.lo_max || jh + 32 <= a.S))) {
                 const uint64_t see = seen_bits(x.w.lo, x.w.hi, a.S, jh) >> src.key(0, hf);
 #pragma unroll
@@ -205,32 +265,19 @@ template <int DT, int D> __global__ __launch_bounds__(64 * NW, DT == 1 ? 2 : 1) 
             }
         }
     }
-    if (__ballot(x.valid && any_bad<D>(acc))) {   // key by key, the masked ones left out
-#pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) acc[dt] = zero;
-#pragma unroll 1
-        for (int it = 0; it < nt; ++it) {
-            const int j0 = (it < ns ? it : wt0 + it - ns) * KT;
-#pragma unroll 1
-            for (int j = j0; j < min(j0 + KT, x.w.hi_max); ++j) {
-                const char *kj = src.k + (int64_t)min(j, src.last) * src.kb;
-                const float s = dot_rows<DT, D>(q, kj, hf);
-                const float dp = dot_rows<DT, D>(dO, src.v + (int64_t)min(j, src.last) * src.vb, hf);
-                if (j < x.w.hi && (j >= x.w.lo || j < a.S))
-                    add_row<DT, D>(acc, kj, ex2(fmaf(s, a.c, -lse)) * (dp - delta), hf);
-            }
-        }
+    if (__ballot(x.valid && any_bad<D>(acc))) {
+        dq_each<DT, D>(a);
+        return;
     }
-    if (!x.in) return;
-    if (!x.valid) {
-#pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) acc[dt] = zero;
-    }
-    store_rows<DT, D>(a.dq + row * D * ESZ, acc, a.scale);
+    store_dq<DT, D>(a, x, acc);
 }
 
 constexpr int KB = 32 * NW;   // keys of a dk / dv workgroup
-constexpr int TT = 64;        // tokens of its steps
+constexpr int TT = 32;        // tokens of its steps
+
+// Whether the keys' operands come from LDS each time: where keys, values and both
+// sums would leave registers for one wave per SIMD only.
+template <int DT, int D> constexpr bool keys_in_lds() { return DT == 1 && D == 128; }
 
 // One past the last token that sees keys k0 .. k0 + KB - 1, and the steps over them.
 __device__ __forceinline__ int last_token(int k0, int len, int W, int S) {
@@ -252,72 +299,141 @@ __device__ __forceinline__ void find_part(const Args &a, int slot, int &tile, in
     }
 }
 
-template <int DT, int D> __global__ __launch_bounds__(64 * NW, DT == 1 && D == 64 ? 2 : 1) void swa_dkv(const Args a) {
+// A dk / dv workgroup's keys, and this lane's.
+struct Keys {
+    int b, g, len, k0, kw, j;     // k0: the workgroup's first key, kw: the wave's, j: the lane's
+    int nst, i0, i1, parts;       // token tiles, this part's steps (head, token tile), the tile's parts
+    int64_t at;                   // the lane's place among the parts
+};
+
+__device__ __forceinline__ void find_keys(const Args &a, Keys &x) {
+    const int combo = blockIdx.x % a.Cn, slot = blockIdx.x / a.Cn;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    int tile, part;
+    find_part(a, slot, tile, part);
+    x.b = combo / a.Hkv;
+    x.g = combo % a.Hkv;
+    x.len = seq_len(a, x.b);
+    x.k0 = tile * KB;
+    x.kw = x.k0 + 32 * wave;
+    x.j = x.kw + (lane & 31);
+    x.nst = steps(x.k0, x.len, a.W, a.S);
+    x.parts = tile < a.nst ? a.Ps : a.Pn;
+    x.i0 = part * a.chunk;
+    x.i1 = min(x.nst * a.G, x.i0 + a.chunk);
+    x.at = ((int64_t)combo * (a.nst * a.Ps + (a.ntiles - a.nst) * a.Pn) + slot) * KB + 32 * wave + (lane & 31);
+}
+
+template <int DT, int D>
+__device__ __forceinline__ void load_keys(const Args &a, const Keys &x, typename Op<DT>::F (&kf)[D / 16],
+                                          typename Op<DT>::F (&vf)[D / 16]) {
+    const int64_t j = min(x.j, a.n - 1);
+    load_rows<DT, D>(a.k + x.b * a.ks[0] + j * a.ks[1] + x.g * a.ks[2], x.j < x.len, kf);
+    load_rows<DT, D>(a.v + x.b * a.vs[0] + j * a.vs[1] + x.g * a.vs[2], x.j < x.len, vf);
+}
+
+template <int DT, int D>
+__device__ __forceinline__ void store_keys(const Args &a, const Keys &x, f32x16 (&dk)[D / 32], f32x16 (&dv)[D / 32]) {
+    if (x.parts > 1) {   // the sums as they are, for swa_join
+        store_rows<0, D>(reinterpret_cast<char *>(a.part + x.at * 2 * D), dk, 1.0f);
+        store_rows<0, D>(reinterpret_cast<char *>(a.part + x.at * 2 * D + D), dv, 1.0f);
+        return;
+    }
+    if (x.j >= a.n) return;
+    if (x.j >= x.len) {
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) dk[dt] = dv[dt] = f32x16{0.0f};
+    }
+    const int64_t row = (((int64_t)x.b * a.n + x.j) * a.Hkv + x.g) * D * Tile<DT, D>::ESZ;
+    store_rows<DT, D>(a.dk + row, dk, a.scale);
+    store_rows<DT, D>(a.dv + row, dv, 1.0f);
+}
+
+template <int DT, int D> __global__ __launch_bounds__(64 * NW, DT == 1 ? 2 : 1) void swa_dkv(const Args a) {
     extern __shared__ __align__(16) char smem[];
     typedef Tile<DT, D> TL;
     typedef typename Op<DT>::F F;
-    constexpr int ESZ = TL::ESZ, NKS = D / 16, NDT = D / 32, BYTES = 2 * TT * TL::ROWB + 2 * TT * 4;
-    const int lane = threadIdx.x & 63, hf = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int combo = blockIdx.x % a.Cn, slot = blockIdx.x / a.Cn;
-    int tile, part;
-    find_part(a, slot, tile, part);
-    const int b = combo / a.Hkv, g = combo % a.Hkv, len = seq_len(a, b);
-    const int k0 = tile * KB, kw = k0 + 32 * wave, j = kw + (lane & 31);
-    const int nst = steps(k0, len, a.W, a.S), all = nst * a.G;
-    const int parts = tile < a.nst ? a.Ps : a.Pn;
-    const int i0 = part * a.chunk, i1 = min(all, i0 + a.chunk);
-    if (i0 >= i1 && (parts > 1 || part > 0)) return;   // a part with nothing to sum is not read either
-    const bool valid = j < len;
-    F kf[NKS], vf[NKS];
-    load_rows<DT, D>(a.k + b * a.ks[0] + (int64_t)min(j, a.n - 1) * a.ks[1] + g * a.ks[2], valid, kf);
-    load_rows<DT, D>(a.v + b * a.vs[0] + (int64_t)min(j, a.n - 1) * a.vs[1] + g * a.vs[2], valid, vf);
-    const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    f32x16 dk[NDT], dv[NDT];
+    constexpr int NKS = D / 16, NDT = D / 32, BYTES = 2 * TT * TL::ROWB + 2 * TT * 4;
+    constexpr bool KL = keys_in_lds<DT, D>();
+    const int lane = threadIdx.x & 63, hf = lane >> 5;
+    Keys x;
+    find_keys(a, x);
+    if (x.i0 >= x.i1 && x.parts > 1) {   // a part with nothing to sum is not read either
+        if (lane == 0) a.marks[blockIdx.x * NW + (threadIdx.x >> 6)] = 0;
+        return;
+    }
     const uint32_t lds = lds_offset(smem);
-    const int last = max(len, 1) - 1;
+    const int last = max(x.len, 1) - 1;
     const uint32_t qo = TL::offset(a.qs[1]), doo = TL::offset(a.dos[1]);
-
-    auto stage = [&](int it, int buf) {
-        const int h = g * a.G + it / nst, t0 = (k0 / TT + it % nst) * TT;
+    // the step that is staged next: head h, token tile tt of it
+    int h = x.g * a.G + (x.nst ? x.i0 / x.nst : 0), tt = x.nst ? x.i0 % x.nst : 0;
+    const auto stage = [&](int buf) {
+        const int t0 = (x.k0 / TT + tt) * TT;
         const uint32_t to = lds + buf * BYTES;
-        TL::template stage<TT>(a.q + b * a.qs[0] + h * a.qs[2], a.qs[1], qo, t0, last, to);
-        TL::template stage<TT>(a.dout + b * a.dos[0] + h * a.dos[2], a.dos[1], doo, t0, last, to + TT * TL::ROWB);
+        TL::template stage<TT>(a.q + x.b * a.qs[0] + h * a.qs[2], a.qs[1], qo, t0, last, to);
+        TL::template stage<TT>(a.dout + x.b * a.dos[0] + h * a.dos[2], a.dos[1], doo, t0, last, to + TT * TL::ROWB);
         float *ld = reinterpret_cast<float *>(smem + buf * BYTES + 2 * TT * TL::ROWB);
-        if (threadIdx.x < 2 * TT) {
+        if (threadIdx.x < 2 * TT) {   // -lse, -delta
             const int t = min(t0 + ((int)threadIdx.x & (TT - 1)), last);
-            ld[threadIdx.x] = (threadIdx.x < TT ? a.lse : a.delta)[((int64_t)b * a.Hq + h) * a.n + t];
+            ld[threadIdx.x] = -(threadIdx.x < TT ? a.lse : a.delta)[((int64_t)x.b * a.Hq + h) * a.n + t];
+        }
+        if (++tt == x.nst) {
+            tt = 0;
+            ++h;
         }
     };
+    int ct = tt;   // token tile of the step that is computed
+    char *tk = smem + 2 * BYTES;
+    if (x.i0 < x.i1) {
+        stage(0);
+        if constexpr (KL)
+            TL::template stage<KB>(a.k + x.b * a.ks[0] + x.g * a.ks[2], a.ks[1], TL::offset(a.ks[1]), x.k0, last,
+                                   lds + 2 * BYTES);
+    }
+    F kf[NKS], vf[NKS];
+    load_keys<DT, D>(a, x, kf, vf);
+    const f32x16 zero = {0.0f};
+    f32x16 dk[NDT], dv[NDT];
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) dk[dt] = dv[dt] = zero;
-    if (i0 < i1) stage(i0, 0);
+    const int tend = x.kw < a.S ? x.len : min(x.len, x.kw + 31 + a.W);   // tokens that see one of the wave's keys
 #pragma unroll 1
-    for (int it = i0; it < i1; ++it) {
+    for (int it = x.i0; it < x.i1; ++it) {
         wait_vm<0>();
         __syncthreads();
-        const int cur = (it - i0) & 1;
-        if (it + 1 < i1) stage(it + 1, cur ^ 1);
-        const int t0 = (k0 / TT + it % nst) * TT;
-        if (t0 + TT <= kw || (t0 >= kw + 31 + a.W && kw >= a.S) || t0 >= len) continue;
+        const int cur = (it - x.i0) & 1, t0 = (x.k0 / TT + ct) * TT;
+        ct = ct + 1 == x.nst ? 0 : ct + 1;
+        if (it + 1 < x.i1) stage(cur ^ 1);
         const char *tq = smem + cur * BYTES, *td = tq + TT * TL::ROWB;
         const float *ld = reinterpret_cast<const float *>(td + TT * TL::ROWB);
-        const bool whole = t0 >= kw + 31 && t0 + TT <= len && (t0 + TT <= kw + a.W || kw + 32 <= a.S);
+        if (t0 + TT <= x.kw || t0 >= tend) continue;
+        {
+            const int th = t0;
+            f32x16 s = zero, dp;
 #pragma unroll
-        for (int rt = 0; rt < 2; ++rt) {
-            f32x16 s = zero, dp = zero;
+            for (int g = 0; g < 4; ++g) {   // do . v starts from -delta
+                const f32x4 dl = *reinterpret_cast<const f32x4 *>(ld + TT + 8 * g + 4 * hf);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) dp[4 * g + e] = dl[e];
+            }
 #pragma unroll
             for (int ks = 0; ks < NKS; ++ks) {
-                s = Op<DT>::mma(TL::row(tq, 32 * rt + (lane & 31), ks, hf), kf[ks], s);
-                dp = Op<DT>::mma(TL::row(td, 32 * rt + (lane & 31), ks, hf), vf[ks], dp);
+                s = Op<DT>::mma(TL::row(tq, lane & 31, ks, hf), KL ? TL::row(tk, x.kw - x.k0 + (lane & 31), ks, hf) : kf[ks], s);
+                dp = Op<DT>::mma(TL::row(td, lane & 31, ks, hf), vf[ks], dp);
             }
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int tr = 32 * rt + 8 * (r >> 2) + 4 * hf + (r & 3);
-                s[r] = ex2(fmaf(s[r], a.c, -ld[tr]));
-                dp[r] = s[r] * (dp[r] - ld[TT + tr]);
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 ls = *reinterpret_cast<const f32x4 *>(ld + 8 * g + 4 * hf);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[4 * g + e] = ex2(fmaf(s[4 * g + e], a.c, ls[e]));
+                    dp[4 * g + e] *= s[4 * g + e];
+                }
             }
-            if (!whole) {   // tokens j .. that see key j
-                const uint64_t see = seen_bits(j, j < a.S ? len : min(len, j + a.W), 0, t0 + 32 * rt) >> (4 * hf);
+            if (!(th >= x.kw + 31 && th + 32 <= x.len && (th + 32 <= x.kw + a.W || x.kw + 32 <= a.S))) {
+                // tokens j .. that see key j
+                const uint64_t see =
+                    seen_bits(x.j, x.j < a.S ? x.len : min(x.len, x.j + a.W), 0, th) >> (4 * hf);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     s[r] = keep(s[r], see, 8 * (r >> 2) + (r & 3), 0.0f);
@@ -329,99 +445,122 @@ template <int DT, int D> __global__ __launch_bounds__(64 * NW, DT == 1 && D == 6
                 const F pf = half16<DT>(s, u), df = half16<DT>(dp, u);
 #pragma unroll
                 for (int dt = 0; dt < NDT; ++dt) {
-                    dv[dt] = Op<DT>::mma(TL::col(td, 32 * rt + 16 * u, dt, lane), pf, dv[dt]);
-                    dk[dt] = Op<DT>::mma(TL::col(tq, 32 * rt + 16 * u, dt, lane), df, dk[dt]);
+                    dv[dt] = Op<DT>::mma(TL::col(td, 16 * u, dt, lane), pf, dv[dt]);
+                    dk[dt] = Op<DT>::mma(TL::col(tq, 16 * u, dt, lane), df, dk[dt]);
                 }
             }
         }
     }
-    if (__ballot(valid && (any_bad<D>(dk) || any_bad<D>(dv)))) {   // token by token, the masked ones left out
-#pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) dk[dt] = dv[dt] = zero;
-#pragma unroll 1
-        for (int it = i0; it < i1; ++it) {
-            const int h = g * a.G + it / nst, t0 = (k0 / TT + it % nst) * TT;
-#pragma unroll 1
-            for (int t = t0; t < min(t0 + TT, len); ++t) {
-                const char *qt = a.q + b * a.qs[0] + t * a.qs[1] + h * a.qs[2];
-                const char *dt_ = a.dout + b * a.dos[0] + t * a.dos[1] + h * a.dos[2];
-                const int64_t at = ((int64_t)b * a.Hq + h) * a.n + t;
-                const float p = ex2(fmaf(dot_rows<DT, D>(kf, qt, hf), a.c, -a.lse[at]));
-                const float ds = p * (dot_rows<DT, D>(vf, dt_, hf) - a.delta[at]);
-                if (t >= j && (t < j + a.W || j < a.S)) {
-                    add_row<DT, D>(dv, dt_, p, hf);
-                    add_row<DT, D>(dk, qt, ds, hf);
-                }
-            }
-        }
-    }
-    if (parts > 1) {   // the sums as they are, for swa_join
-        const int64_t at = ((int64_t)combo * (a.nst * a.Ps + (a.ntiles - a.nst) * a.Pn) + slot) * KB + 32 * wave +
-                           (lane & 31);
-        store_rows<0, D>(reinterpret_cast<char *>(a.part + at * 2 * D), dk, 1.0f);
-        store_rows<0, D>(reinterpret_cast<char *>(a.part + at * 2 * D + D), dv, 1.0f);
-        return;
-    }
-    if (j >= a.n) return;
-    if (!valid) {
-#pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) dk[dt] = dv[dt] = zero;
-    }
-    const int64_t row = (((int64_t)b * a.n + j) * a.Hkv + g) * D * ESZ;
-    store_rows<DT, D>(a.dk + row, dk, a.scale);
-    store_rows<DT, D>(a.dv + row, dv, 1.0f);
+    const uint64_t bad = __ballot(x.j < x.len && (any_bad<D>(dk) || any_bad<D>(dv)));
+    if (lane == 0) a.marks[blockIdx.x * NW + (threadIdx.x >> 6)] = bad != 0;
+    store_keys<DT, D>(a, x, dk, dv);
 }
 
 // dk and dv of the tiles in several parts: the parts' sums, in order.  A workgroup
 // takes 1024 elements of one key tile and KV head, 4 a thread, so that there
 // are enough of them to keep HBM busy.
+//
+// Keys of a wave that swa_dkv marked are computed here instead, token by token,
+// the masked ones left out: 2D / 4 threads a key, those of its dk with q . k, those
+// of its dv with do . v.  (Inlined in swa_dkv that path's registers cost it a wave
+// per SIMD: 8192 tokens, d = 128, 390 us and 735; 2000 tokens, d = 64, 39 and 52.)
 constexpr int JE = 1024;
-template <int DT, int D> __global__ __launch_bounds__(JE / 4) void swa_join(const Args a, int first) {
+template <int DT, int D> __global__ __launch_bounds__(JE / 4) void swa_join(const Args a) {
     typedef typename St<DT>::T T;
-    constexpr int PER = KB * 2 * D / JE;
-    const int e = blockIdx.x % PER * JE + threadIdx.x * 4, r = e / (2 * D), x = e % (2 * D);
-    const int combo = blockIdx.x / PER % a.Cn, tile = first + blockIdx.x / PER / a.Cn;
-    const int b = combo / a.Hkv, g = combo % a.Hkv, len = seq_len(a, b), k0 = tile * KB, j = k0 + r;
-    if (j >= a.n) return;
+    constexpr int PER = KB * 2 * D / JE, ESZ = Tile<DT, D>::ESZ;
+    const int e = blockIdx.x % PER * JE + threadIdx.x * 4, r = e / (2 * D), x = e % (2 * D), xd = x % D;
+    const int combo = blockIdx.x / PER % a.Cn, tile = blockIdx.x / PER / a.Cn;
     const int P = tile < a.nst ? a.Ps : a.Pn;
-    const int used = j < len ? min(P, (steps(k0, len, a.W, a.S) * a.G + a.chunk - 1) / a.chunk) : 0;
     const int slot = tile < a.nst ? tile * a.Ps : a.nst * a.Ps + (tile - a.nst) * a.Pn;
-    const int64_t slots = a.nst * a.Ps + (a.ntiles - a.nst) * a.Pn;
-    const float *p = a.part + ((int64_t)combo * slots + slot) * KB * 2 * D + e;
+    const int b = combo / a.Hkv, g = combo % a.Hkv, len = seq_len(a, b), k0 = tile * KB, j = k0 + r;
+    const int used = min(P, (steps(k0, len, a.W, a.S) * a.G + a.chunk - 1) / a.chunk);
+    bool marked = false;   // the same for the threads of a key
+    for (int i = 0; i < used; ++i) marked |= a.marks[((slot + i) * a.Cn + combo) * NW + r / 32] != 0;
+    if (j >= a.n || (P == 1 && !marked)) return;
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    if (marked && j < len) {
+        // this thread's 4 elements of the key (x < D) or the value
+        const char *kv = x < D ? a.k + b * a.ks[0] + j * a.ks[1] + g * a.ks[2]
+                               : a.v + b * a.vs[0] + j * a.vs[1] + g * a.vs[2];
+        f32x4 own;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) own[i] = St<DT>::ld(reinterpret_cast<const T *>(kv), xd + i);
+        const int t1 = j < a.S ? len : min(len, j + a.W);
+        for (int h = g * a.G; h < (g + 1) * a.G; ++h)
+            for (int t = j; t < t1; ++t) {
+                const char *qt = a.q + b * a.qs[0] + t * a.qs[1] + h * a.qs[2];
+                const char *ot = a.dout + b * a.dos[0] + t * a.dos[1] + h * a.dos[2];
+                f32x4 qo;   // the query's elements for the key's threads, do's for the value's, and the other way round
+                float dot = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    qo[i] = St<DT>::ld(reinterpret_cast<const T *>(x < D ? qt : ot), xd + i);
+                    dot = fmaf(own[i], qo[i], dot);
+                }
+#pragma unroll
+                for (int o = 1; o < D / 4; o <<= 1) dot += __shfl_xor(dot, o, 64);
+                const float other = __shfl_xor(dot, D / 4, 64);
+                const int64_t at = ((int64_t)b * a.Hq + h) * a.n + t;
+                const float p = ex2(fmaf(x < D ? dot : other, a.c, -a.lse[at]));
+                const float w = x < D ? p * (other - a.delta[at]) : p;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[i] = fmaf(w, qo[i], sum[i]);
+            }
+    } else if (j < len) {
+        const int64_t slots = a.nst * a.Ps + (a.ntiles - a.nst) * a.Pn;
+        const float *p = a.part + ((int64_t)combo * slots + slot) * KB * 2 * D + e;
 #pragma unroll 4
-    for (int i = 0; i < used; ++i) sum = sum + *reinterpret_cast<const f32x4 *>(p + (int64_t)i * KB * 2 * D);
+        for (int i = 0; i < used; ++i) sum = sum + *reinterpret_cast<const f32x4 *>(p + (int64_t)i * KB * 2 * D);
+    }
     const float f = x < D ? a.scale : 1.0f;
-    T *to = reinterpret_cast<T *>(x < D ? a.dk : a.dv) + (((int64_t)b * a.n + j) * a.Hkv + g) * D + x % D;
+    char *to = (x < D ? a.dk : a.dv) + ((((int64_t)b * a.n + j) * a.Hkv + g) * D + xd) * ESZ;
     if constexpr (DT == 1)
         *reinterpret_cast<uint2 *>(to) = make_uint2(pk_bf16(sum[0] * f, sum[1] * f), pk_bf16(sum[2] * f, sum[3] * f));
     else
         *reinterpret_cast<f32x4 *>(to) = sum * f;
 }
 
-// How dk and dv are cut: steps of a part, so that some 1024 workgroups share the
-// work, never more than a tile without sinks takes.
+// How dk and dv are cut.  The workgroups run in rounds of as many as the card holds;
+// a tile without sinks is cut into the number of parts for which rounds times
+// steps of a part (and a part's start and end, worth some 4 steps), and the
+// traffic of the parts' sums, take least.  A step takes about 0.9 us at d = 64,
+// 1.8 at d = 128 (bf16; fp32 eight times that).  Measured at 8192 tokens, 28 / 4
+// heads, d = 128, kernel and join: 2 parts 481 us, 3 (taken) 370, 4 410, 8 412.
 struct Cut {
     int ntiles, nst, Ps, Pn, chunk;
     int64_t slots;
 };
-static Cut cut(int64_t Cn, int64_t n, int64_t G, int64_t W, int64_t S) {
-    Cut c;
+static Cut cut(int dtype, int64_t d, int64_t Cn, int64_t n, int64_t G, int64_t W, int64_t S) {
+    Cut c = {}, best = {};
     c.ntiles = (int)((n + KB - 1) / KB);
-    c.nst = (int)((S < n ? S : n) + KB - 1) / KB;
+    c.nst = (int)(((S < n ? S : n) + KB - 1) / KB);
     const int64_t most = G * ((n + TT - 1) / TT);                     // steps of a tile of sinks
     int64_t usual = G * ((KB + W - 1 + TT - 1) / TT + 1);             // of another
     if (usual > most) usual = most;
-    const int64_t total = Cn * (c.nst * most + (c.ntiles - c.nst) * usual);
-    int64_t ch = (total + 1023) / 1024;
-    if (ch < 8) ch = 8;
-    if (ch > usual) ch = usual;
-    c.chunk = (int)ch;
-    c.Ps = (int)((most + ch - 1) / ch);
-    c.Pn = (int)((usual + ch - 1) / ch);
-    c.slots = (int64_t)c.nst * c.Ps + (int64_t)(c.ntiles - c.nst) * c.Pn;
-    return c;
+    const int64_t room = dtype == HBA_DTYPE_BF16 && d == 64 ? 768 : d == 64 || dtype == HBA_DTYPE_BF16 ? 512 : 256;
+    const double step = (double)d / 64 * 0.9 * (dtype == HBA_DTYPE_BF16 ? 1 : 8);
+    double least = 0;
+    for (int64_t P = 1; P <= 32 && P <= usual; ++P) {
+        const int64_t ch = (usual + P - 1) / P;
+        c.chunk = (int)ch;
+        c.Pn = (int)((usual + ch - 1) / ch);
+        c.Ps = (int)((most + ch - 1) / ch);
+        c.slots = (int64_t)c.nst * c.Ps + (int64_t)(c.ntiles - c.nst) * c.Pn;
+        const int64_t parts = (c.Ps > 1 ? (int64_t)c.nst * c.Ps : 0) + (c.Pn > 1 ? (int64_t)(c.ntiles - c.nst) * c.Pn : 0);
+        const double us = (double)((c.slots * Cn + room - 1) / room) * (ch + 4) * step +
+                          (double)(parts * Cn) * KB * 2 * d * 8 / 4e6;
+        if (P == 1 || us < least) {
+            least = us;
+            best = c;
+        }
+    }
+    return best;
 }
+
+// The workspace: delta, marks, parts.
+static size_t round256(size_t x) { return (x + 255) & ~(size_t)255; }
+static size_t delta_bytes(int64_t B, int64_t n, int64_t Hq) { return round256((size_t)(B * Hq * n) * 4); }
+static size_t mark_bytes(int64_t Cn, const Cut &c) { return round256((size_t)(Cn * c.slots) * NW * 4); }
 
 template <int DT, int D, class K> static int lds_room(K kern, size_t bytes) {
     if (bytes <= 65536) return HBA_OK;
@@ -440,7 +579,8 @@ template <int DT, int D> static int launch_fwd(const Args &a, int64_t grid, hipS
 }
 
 template <int DT, int D> static int launch_bwd(Args a, int64_t grid, const Cut &c, hipStream_t s) {
-    constexpr size_t lds = 2 * DenseKV<DT, D>::BYTES, ldk = 2 * (2 * TT * Tile<DT, D>::ROWB + 2 * TT * 4);
+    constexpr size_t lds = 2 * DenseKV<DT, D>::BYTES, ldk = 2 * (2 * TT * Tile<DT, D>::ROWB + 2 * TT * 4) +
+                         (keys_in_lds<DT, D>() ? KB * Tile<DT, D>::ROWB : 0);
     if (int st = lds_room<DT, D>(swa_dq<DT, D>, lds)) return st;
     if (int st = lds_room<DT, D>(swa_dkv<DT, D>, ldk)) return st;
     hipLaunchKernelGGL((swa_dq<DT, D>), dim3((unsigned)grid), dim3(64 * NW), lds, s, a);
@@ -448,12 +588,9 @@ template <int DT, int D> static int launch_bwd(Args a, int64_t grid, const Cut &
     a.ntiles = c.ntiles;
     hipLaunchKernelGGL((swa_dkv<DT, D>), dim3((unsigned)(c.slots * a.Cn)), dim3(64 * NW), ldk, s, a);
     HBA_LAUNCH_CHECK();
-    const int first = c.Ps > 1 ? 0 : c.nst, end = c.Pn > 1 ? c.ntiles : c.nst;
-    if (first < end) {
-        hipLaunchKernelGGL((swa_join<DT, D>), dim3((unsigned)((end - first) * a.Cn * (KB * 2 * D / JE))),
-                           dim3(JE / 4), 0, s, a, first);
-        HBA_LAUNCH_CHECK();
-    }
+    hipLaunchKernelGGL((swa_join<DT, D>), dim3((unsigned)((int64_t)c.ntiles * a.Cn * (KB * 2 * D / JE))), dim3(JE / 4),
+                       0, s, a);
+    HBA_LAUNCH_CHECK();
     return HBA_OK;
 }
 
@@ -520,16 +657,15 @@ extern "C" int hba_swa_fwd(int dtype, const void *q, const int64_t q_strides[3],
     return st;
 }
 
-extern "C" int hba_swa_bwd_workspace_bytes(int64_t B, int64_t n, int64_t Hq, int64_t Hkv, int64_t d, int64_t W,
+extern "C" int hba_swa_bwd_workspace_bytes(int dtype, int64_t B, int64_t n, int64_t Hq, int64_t Hkv, int64_t d, int64_t W,
                                            int64_t S, size_t *bytes) {
     if (!bytes) return HBA_ERR_INVALID_ARG;
-    if (int st = swa::check(HBA_DTYPE_F32, B, n, Hq, Hkv, d, W, S, 1.0f)) return st;
+    if (int st = swa::check(dtype, B, n, Hq, Hkv, d, W, S, 1.0f)) return st;
     if (W > n) W = n;
     if (S > n) S = n;
-    const swa::Cut c = swa::cut(B * Hkv, n, Hq / Hkv, W, S);
-    const size_t delta = ((size_t)(B * Hq * n) * 4 + 255) / 256 * 256;
+    const swa::Cut c = swa::cut(dtype, d, B * Hkv, n, Hq / Hkv, W, S);
     const size_t part = c.Ps > 1 || c.Pn > 1 ? (size_t)(B * Hkv) * c.slots * swa::KB * 2 * d * 4 : 0;
-    *bytes = delta + part;
+    *bytes = swa::delta_bytes(B, n, Hq) + swa::mark_bytes(B * Hkv, c) + part;
     return HBA_OK;
 }
 
@@ -544,7 +680,7 @@ extern "C" int hba_swa_bwd(int dtype, const void *q, const int64_t q_strides[3],
         !workspace || !dq || !dk || !dv)
         return HBA_ERR_INVALID_ARG;
     size_t need = 0;
-    if (int st = hba_swa_bwd_workspace_bytes(B, n, Hq, Hkv, d, W, S, &need)) return st;
+    if (int st = hba_swa_bwd_workspace_bytes(dtype, B, n, Hq, Hkv, d, W, S, &need)) return st;
     if (ws_bytes < need) return HBA_ERR_INVALID_ARG;
     if (!abi::rows_aligned(dtype, q, q_strides) || !abi::rows_aligned(dtype, k, k_strides) ||
         !abi::rows_aligned(dtype, v, v_strides) || !abi::rows_aligned(dtype, dout, dout_strides) ||
@@ -580,16 +716,17 @@ extern "C" int hba_swa_bwd(int dtype, const void *q, const int64_t q_strides[3],
     a.out = (char *)const_cast<void *>(out);
     a.lse = const_cast<float *>(lse);
     a.delta = (float *)workspace;
-    a.part = (float *)((char *)workspace + ((size_t)(B * Hq * n) * 4 + 255) / 256 * 256);
+    a.marks = (int32_t *)((char *)workspace + swa::delta_bytes(B, n, Hq));
     a.dq = (char *)dq;
     a.dk = (char *)dk;
     a.dv = (char *)dv;
-    const swa::Cut c = swa::cut(a.Cn, n, a.G, a.W, a.S);
+    const swa::Cut c = swa::cut(dtype, d, a.Cn, n, a.G, a.W, a.S);
+    a.part = (float *)((char *)a.marks + swa::mark_bytes(a.Cn, c));
     a.nst = c.nst;
     a.Ps = c.Ps;
     a.Pn = c.Pn;
     a.chunk = c.chunk;
-    if (c.slots * a.Cn > 0x7fffffff) return HBA_ERR_UNSUPPORTED;
+    if (c.slots * a.Cn * rows::NW > 0x7fffffff || (int64_t)c.ntiles * a.Cn * (swa::KB * 2 * d / swa::JE) > 0x7fffffff) return HBA_ERR_UNSUPPORTED;
     int st = HBA_OK;
 #define HBA_SWA(DT, D) st = swa::launch_bwd<DT, D>(a, grid, c, (hipStream_t)stream)
     HBA_DISPATCH_DT_D(dtype, d, HBA_SWA);

@@ -74,7 +74,7 @@ SIGNATURES = {
                        _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, ctypes.c_size_t, _vp, _vp],
     "hba_swa_fwd": [_i, _vp, _c_i64p, _vp, _c_i64p, _vp, _c_i64p, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f,
                     _vp, _vp, _vp],
-    "hba_swa_bwd_workspace_bytes": [_i64, _i64, _i64, _i64, _i64, _i64, _i64, ctypes.POINTER(ctypes.c_size_t)],
+    "hba_swa_bwd_workspace_bytes": [_i, _i64, _i64, _i64, _i64, _i64, _i64, _i64, ctypes.POINTER(ctypes.c_size_t)],
     "hba_swa_bwd": [_i, _vp, _c_i64p, _vp, _c_i64p, _vp, _c_i64p, _vp, _vp, _vp, _c_i64p, _vp, _i64, _i64, _i64,
                     _i64, _i64, _i64, _i64, _f, _vp, ctypes.c_size_t, _vp, _vp, _vp, _vp],
 }

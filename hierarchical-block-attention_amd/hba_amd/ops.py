@@ -628,7 +628,7 @@ def _swa_bwd(q, k, v, out, lse, dout, lens, window, sinks, scale):
     W, S = min(window, n), min(sinks, n)
     q, k, v, dout, out, lse = _rows16(q), _rows16(k), _rows16(v), _rows16(dout), _c16(out), lse.contiguous()
     nbytes = ctypes.c_size_t(0)
-    check(lib().hba_swa_bwd_workspace_bytes(B, n, Hq, Hkv, d, W, S, ctypes.byref(nbytes)),
+    check(lib().hba_swa_bwd_workspace_bytes(code, B, n, Hq, Hkv, d, W, S, ctypes.byref(nbytes)),
           "hba_swa_bwd_workspace_bytes")
     ws = torch.empty(int(nbytes.value), dtype=torch.uint8, device=dev)
     with _on(dev):

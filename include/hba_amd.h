@@ -568,10 +568,11 @@ int hba_swa_fwd(int dtype, const void *q, const int64_t q_strides[3], const void
                 const int32_t *lens, int64_t B, int64_t n, int64_t Hq, int64_t Hkv, int64_t d,
                 int64_t W, int64_t S, float scale, void *out, float *lse, void *stream);
 
-/* Scratch bytes of hba_swa_bwd: <dout, out> of every row (fp32 [B, Hq, n]) and
- * the partial sums of dk and dv where key tiles are cut into parts. */
-int hba_swa_bwd_workspace_bytes(int64_t B, int64_t n, int64_t Hq, int64_t Hkv, int64_t d,
-                                int64_t W, int64_t S, size_t *bytes);
+/* Scratch bytes of hba_swa_bwd: <dout, out> of every row (fp32 [B, Hq, n]), marks of
+ * sums that are not finite, and the partial sums of dk and dv where key tiles are
+ * cut into parts. */
+int hba_swa_bwd_workspace_bytes(int dtype, int64_t B, int64_t n, int64_t Hq, int64_t Hkv,
+                                int64_t d, int64_t W, int64_t S, size_t *bytes);
 
 /*
  * Gradients of hba_swa_fwd: dq [B, n, Hq, d], dk, dv [B, n, Hkv, d] (contiguous,
