@@ -42,7 +42,7 @@ struct Args {
     const float *scales;
     int T, Bd, Hq, Hkv, G, maxp, max_len, W, S;   // W: 0 for every key
     int shared;                         // pages that all sequences begin with
-    int slots, slot0, part;             // parts of a row: how many, this launch's first, its parts (rows) or pages of one (decode)
+    int slots, slot0, part;             // parts of a row: how many, this launch's first, pages of one of them
     char *out;                          // [T, Hq, D]
     float *po, *pml;                    // parts: [T, Hq, slots, D] sums, [T, Hq, slots, 2] maximum (log2 units) and sum
 };
@@ -288,7 +288,7 @@ template <int DT, int D, int UK> __global__ __launch_bounds__(64 * DW) void deco
 // SHARED: the rows of all tokens over the shared pages (blockIdx.x: 128-row
 // tile); else the rows of one sequence's tokens over its own pages (blockIdx.x:
 // tile of the ragged batch).  blockIdx.y: KV head, blockIdx.z: part of the tiles.
-template <int DT, int D, bool SHARED> __global__ __launch_bounds__(64 * rows::NW, (rows::WAVES<DT, D>)) void rows_kernel(const Args a) {
+template <int DT, int D, bool SHARED> __global__ __launch_bounds__(64 * rows::NW, (DT == 1 && D == 64 ? 3 : rows::WAVES<DT, D>)) void rows_kernel(const Args a) {
     extern __shared__ __align__(16) char smem[];
     typedef typename Op<DT>::F F;
     constexpr int ESZ = DT == 1 ? 2 : 4, NKS = D / 16;
@@ -345,7 +345,16 @@ template <int DT, int D, bool SHARED> __global__ __launch_bounds__(64 * rows::NW
     }
     int ns = 0, wt0 = 0;
     const int nt = hi > 0 ? rows::tile_list<rows::KEYS<DT, D>>(lo, hi, w.S, ns, wt0) : 0;
-    const int z = blockIdx.z, it0 = (int)((int64_t)nt * z / a.part), it1 = (int)((int64_t)nt * (z + 1) / a.part);
+    constexpr int TP = rows::PAGE / rows::KEYS<DT, D>;   // tiles of a page
+    const int z = blockIdx.z, it0 = z * a.part * TP, it1 = min(nt, it0 + a.part * TP);
+    const int64_t row = (int64_t)t * a.Hq + head, at = row * a.slots + a.slot0 + z;
+    if (it0 >= it1 && a.slots > 1) {   // nothing of the row's keys in this part
+        if (in && hf == 0) {
+            a.pml[2 * at] = -INFINITY;
+            a.pml[2 * at + 1] = 0.0f;
+        }
+        return;
+    }
 
     F qh[NKS], ql[NKS];
     {
@@ -353,9 +362,9 @@ template <int DT, int D, bool SHARED> __global__ __launch_bounds__(64 * rows::NW
         const char *row = a.q + (int64_t)t * a.qst + head * a.qsh;
 #pragma unroll
         for (int ks = 0; ks < NKS; ++ks) Op<DT>::unpack(Op<DT>::load(row + (16 * ks + 8 * hf) * ESZ), x[ks]);
-        const int64_t at = max((int64_t)0, min((int64_t)pos, a.n_tab - 1)) * D;
-        finish_q<D, 16>(x, 8 * hf, a.gain ? a.gain + head : nullptr, a.eps, a.cos ? a.cos + at : nullptr,
-                        a.sin ? a.sin + at : nullptr, a.scales[sq] * LOG2E);
+        const int64_t turn = max((int64_t)0, min((int64_t)pos, a.n_tab - 1)) * D;
+        finish_q<D, 16>(x, 8 * hf, a.gain ? a.gain + head : nullptr, a.eps, a.cos ? a.cos + turn : nullptr,
+                        a.sin ? a.sin + turn : nullptr, a.scales[sq] * LOG2E);
 #pragma unroll
         for (int ks = 0; ks < NKS; ++ks) split<DT>(x[ks], qh[ks], ql[ks]);
     }
@@ -382,11 +391,9 @@ template <int DT, int D, bool SHARED> __global__ __launch_bounds__(64 * rows::NW
         acc.m = -INFINITY;
         l = 0.0f;
     }
-    const int64_t row = (int64_t)t * a.Hq + head;
     if (a.slots == 1) {
         rows::store_rows<DT, D>(a.out + row * D * ESZ, acc.O, valid ? 1.0f / l : 0.0f);
     } else {
-        const int64_t at = row * a.slots + a.slot0 + z;
         rows::store_rows<0, D>(reinterpret_cast<char *>(a.po + at * D), acc.O, 1.0f);
         if (hf == 0) {
             a.pml[2 * at] = acc.m;
@@ -468,44 +475,49 @@ template <int DT, int D, int SG> __global__ __launch_bounds__(256) void join_ker
 }
 
 // ------------------------------------------------------------------- plan ----
-// How the rows' keys are cut into parts.
+// How the rows' keys are cut into parts: runs of pages, so that long sequences have
+// more of them than short ones.
 struct Plan {
-    int prefix, own;       // parts over the shared pages, and over each sequence's own
-    int part_pages;        // decode: pages of one of the latter
-    int64_t tiles, ptiles; // 128-row tiles: of the ragged batch (at most), of all tokens
+    int prefix, own;              // parts over the shared pages, and over each sequence's own, at most
+    int prefix_pages, own_pages;  // pages of one
+    int64_t tiles, ptiles;        // 128-row tiles: of the ragged batch (at most), of all tokens
     int slots() const { return prefix + own; }
 };
+#ifndef AIMR
+#define AIMR 1024
+#endif
+#ifndef AIMP
+#define AIMP 512
+#endif
+#ifndef MINP
+#define MINP 4
+#endif
+static int parts_of(int64_t pages, int64_t parts, int64_t least, int &per) {
+    if (parts > pages / least) parts = pages / least;
+    if (parts < 1) parts = 1;
+    per = (int)((pages + parts - 1) / parts);
+    return (int)((pages + per - 1) / per);
+}
 static Plan plan(int64_t T, int64_t Bd, int64_t Hq, int64_t Hkv, int64_t W, int64_t S, int64_t shared, bool one,
                  int64_t max_len) {
     Plan p = {};
     const int64_t G = Hq / Hkv, KT = rows::PAGE;
     int64_t keys = max_len - shared * KT;
     if (W > 0 && W < keys) keys = W;
+    if (W > 0 && !one) keys = max_len;   // a part of a prompt may span any number of windows
     if (keys < 1) keys = 1;
     int64_t pages = (keys + KT - 1) / KT + 1 + (W > 0 ? (S + KT - 1) / KT : 0);
     const int64_t all = (max_len + KT - 1) / KT;
     if (pages > all) pages = all > 0 ? all : 1;
     p.ptiles = (T * G + rows::RT - 1) / rows::RT;
     if (one) {
-        // Enough workgroups to fill 256 CUs several times over, and at least 4 pages
-        // (one a wave) for each.
         const int64_t groups = Bd * Hkv * ((G + 15) / 16);
-        int64_t parts = (2048 + groups - 1) / groups;
-        if (parts > pages / 4) parts = pages / 4;
-        if (parts < 1) parts = 1;
-        p.part_pages = (int)((pages + parts - 1) / parts);
-        p.own = (int)((pages + p.part_pages - 1) / p.part_pages);
+        p.own = parts_of(pages, (2048 + groups - 1) / groups, 4, p.own_pages);
     } else {
-        p.tiles = (T * G + rows::RT - 1) / rows::RT + Bd;
-        int64_t parts = 512 / (p.ptiles * Hkv);
-        if (parts > pages / 8) parts = pages / 8;
-        p.own = (int)(parts < 1 ? 1 : parts);
+        p.tiles = p.ptiles + Bd;
+        p.own = parts_of(pages, AIMR / (p.ptiles * Hkv), 8, p.own_pages);
     }
-    if (shared) {
-        int64_t parts = 512 / (p.ptiles * Hkv);
-        if (parts > shared / 4) parts = shared / 4;
-        p.prefix = (int)(parts < 1 ? 1 : parts);
-    }
+    if (shared) p.prefix = parts_of(shared, AIMP / (p.ptiles * Hkv), MINP, p.prefix_pages);
     return p;
 }
 
@@ -523,7 +535,7 @@ template <int DT, int D> static int launch(Args a, const Plan &p, hipStream_t s)
     a.slots = p.slots();
     if (p.prefix) {
         a.slot0 = 0;
-        a.part = p.prefix;
+        a.part = p.prefix_pages;
         if (int st = lds_room(rows_kernel<DT, D, true>, lds)) return st;
         hipLaunchKernelGGL((rows_kernel<DT, D, true>), dim3((unsigned)p.ptiles, (unsigned)a.Hkv, (unsigned)p.prefix),
                            dim3(64 * rows::NW), lds, s, a);
@@ -531,12 +543,12 @@ template <int DT, int D> static int launch(Args a, const Plan &p, hipStream_t s)
     }
     a.slot0 = p.prefix;
     if (a.cu) {
-        a.part = p.own;
+        a.part = p.own_pages;
         if (int st = lds_room(rows_kernel<DT, D, false>, lds)) return st;
         hipLaunchKernelGGL((rows_kernel<DT, D, false>), dim3((unsigned)p.tiles, (unsigned)a.Hkv, (unsigned)p.own),
                            dim3(64 * rows::NW), lds, s, a);
     } else {
-        a.part = p.part_pages;
+        a.part = p.own_pages;
         const int64_t groups = (int64_t)a.Bd * a.Hkv * ((a.G + 15) / 16);
         hipLaunchKernelGGL((decode_kernel<DT, D, UK>), dim3((unsigned)groups, (unsigned)p.own), dim3(64 * DW), 0, s, a);
     }

@@ -241,8 +241,10 @@ template <int DT, int D> struct PageKV {
     int64_t id;                   // the page of the tile that is staged next
     int half;                     // and the tile's place in it
 
+    // A scalar load: a vector load's wait would be one for the DMA before it as well.
     __device__ __forceinline__ int64_t at(int lp) const {
-        const int p = __builtin_amdgcn_readfirstlane(table[lp]);
+        typedef const __attribute__((address_space(4))) int32_t *uniform;
+        const int p = ((uniform)(uintptr_t)table)[__builtin_amdgcn_readfirstlane(lp)];
         return p < 0 ? 0 : (p < pages ? p : pages - 1);   // never outside the cache
     }
     __device__ __forceinline__ void next(int tile) {
