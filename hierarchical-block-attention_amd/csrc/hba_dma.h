@@ -27,9 +27,13 @@ __device__ __forceinline__ void dma16(const void *src, uint32_t lds_addr) {
 // The same from a wave-uniform base and a lane's 32-bit byte offset.
 __device__ __forceinline__ void dma16s(const void *base, uint32_t off, uint32_t lds_addr) {
     const uint32_t a = __builtin_amdgcn_readfirstlane(lds_addr);
+    // in scalar registers whatever the compiler computed it in (no instruction where it is)
+    const uint64_t p = (uint64_t)(uintptr_t)base;
+    const uint64_t b = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(p >> 32)) << 32 |
+                       (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)p);
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                  :
-                 : "s"(a), "v"(off), "s"(base)
+                 : "s"(a), "v"(off), "s"(b)
                  : "memory");
 }
 

@@ -9,14 +9,18 @@
 // logits keep fp32-like queries: one bf16 rounding would move a logit by 2^-9 of
 // |q||k| and cost as much accuracy as all that follows.
 //
-//   decode_kernel  one token per sequence: memory-bound.  A wave takes a page of
+//   decode_part    one token per sequence: memory-bound.  A wave takes a page of
 //                  one KV head in operand order straight into registers (its
-//                  heads are the 16 columns), workgroups share a sequence's pages
-//                  when there are few sequences.
-//   rows_kernel    128 rows (token, head) a workgroup over staged pages
+//                  heads are the 16 columns), the next one's loads in flight;
+//                  workgroups share a sequence's pages when there are few
+//                  sequences.
+//   rows_part      128 rows (token, head) a workgroup over staged pages
 //                  (hba_rows.h): parts of prompts, and the shared pages for the
 //                  rows of the whole batch.
 //   join_kernel    the parts of a row, by their maxima and sums.
+//
+// With shared pages, both parts of the work are one launch (shared_kernel): neither
+// fills the card alone.
 #include "hba_abi.h"
 #include "hba_common.h"
 #include "hba_ragged.h"
@@ -42,7 +46,7 @@ struct Args {
     const float *scales;
     int T, Bd, Hq, Hkv, G, maxp, max_len, W, S;   // W: 0 for every key
     int shared;                         // pages that all sequences begin with
-    int slots, slot0, part;             // parts of a row: how many, this launch's first, pages of one of them
+    int slots, slot0, part;             // parts of a row: how many, the first of these, pages of one of them
     char *out;                          // [T, Hq, D]
     float *po, *pml;                    // parts: [T, Hq, slots, D] sums, [T, Hq, slots, 2] maximum (log2 units) and sum
 };
@@ -112,8 +116,6 @@ template <> struct Mma16<0> {   // eight 4-deep steps: in step e lane group lg s
     }
 };
 
-constexpr int DW = 4;   // waves of a decode workgroup
-
 // Which pages of its sequence the newest token sees: page i of the list is
 // i < ns ? i : w0 + i - ns (sinks, then the window or everything from `shared`).
 struct Pages {
@@ -127,22 +129,60 @@ __device__ __forceinline__ Pages page_list(const Args &a, int L) {
     return p;
 }
 
-// blockIdx.x: (sequence, KV head, 16 of its heads); blockIdx.y: part.  Units of
-// UK keys: a page, or half of one where a page's operands would fill the
-// registers.
-template <int DT, int D, int UK> __global__ __launch_bounds__(64 * DW) void decode_kernel(const Args a) {
+// group: (sequence, KV head, 16 of its heads); part: a run of a.part pages of its
+// list.  Units of UK keys: a page, or half of one where a page's operands would
+// fill the registers.  DW waves take the part's units in turn.
+template <int DT, int D> constexpr int UNIT = DT == 1 && D == 64 ? 64 : 32;
+template <int D> struct DecodeLds {
+    float o[4][16][D + 4], m[4][16], l[4][16];
+};
+template <int DT, int D, int DW>
+__device__ __forceinline__ void decode_part(const Args &a, DecodeLds<D> &lds, int group, int part) {
     typedef typename Op<DT>::F F;
-    constexpr int ESZ = DT == 1 ? 2 : 4, NKS = D / 32, NDT = D / 16, NH = UK / 32, UP = rows::PAGE / UK;
-    __shared__ float so[DW][16][D + 4];
-    __shared__ float sm[DW][16], sl[DW][16];
+    constexpr int ESZ = DT == 1 ? 2 : 4, UK = UNIT<DT, D>;
+    constexpr int NKS = D / 32, NDT = D / 16, NH = UK / 32, UP = rows::PAGE / UK;
+    typedef const __attribute__((address_space(4))) int32_t *uniform;
     const int lane = threadIdx.x & 63, l16 = lane & 15, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ct = (a.G + 15) / 16;
-    const int s = blockIdx.x / (a.Hkv * ct), g = blockIdx.x / ct % a.Hkv, c0 = blockIdx.x % ct * 16;
+    const int s = group / (a.Hkv * ct), g = group / ct % a.Hkv, c0 = group % ct * 16;
     const int L = length(a, s);
     const Pages pg = page_list(a, L);
-    const int u0 = blockIdx.y * a.part * UP, u1 = min(pg.n, (int)(blockIdx.y + 1) * a.part) * UP;
+    const int u0 = part * a.part * UP, u1 = min(pg.n, (part + 1) * a.part) * UP;
     const int hl = c0 + l16, head = g * a.G + min(hl, a.G - 1);
+    const char *kb = a.kr + (int64_t)g * rows::PAGE * D * ESZ, *vb = a.v + (int64_t)g * rows::PAGE * D * ESZ;
+    const int64_t pstep = (int64_t)a.Hkv * rows::PAGE * D * ESZ;
+    const uniform table = (uniform)(uintptr_t)(a.table + (int64_t)s * a.maxp);
+
+    struct Unit {
+        F k[2 * NH][NKS], v[NDT][NH];
+    };
+    // the logical page of unit u (the last one past the end), its place in the cache
+    const auto logical = [&](int u) {
+        const int i = min(u, u1 - 1) / UP;
+        return i < pg.ns ? i : pg.w0 + i - pg.ns;
+    };
+    const auto place = [&](int u) { return max((int64_t)0, min((int64_t)table[logical(u)], a.pages - 1)); };
+    const auto load = [&](Unit &x, int u, int64_t id) {
+        const int h0 = UP == 1 ? 0 : u % UP;
+        const char *kp = kb + id * pstep, *vp = vb + id * pstep;
+#pragma unroll
+        for (int mt = 0; mt < 2 * NH; ++mt)
+#pragma unroll
+            for (int ks = 0; ks < NKS; ++ks)
+                x.k[mt][ks] = Op<DT>::load(kp + (((2 * h0 + mt) * NKS + ks) * 64 + lane) * 8 * ESZ);
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+            for (int h = 0; h < NH; ++h) x.v[dt][h] = Op<DT>::load(vp + ((dt * 2 + h0 + h) * 64 + lane) * 8 * ESZ);
+    };
+    int u = u0 + wave;
+    Unit xa, xb;
+    int64_t next = 0;   // the place of unit u + DW
+    if (u < u1) {
+        load(xa, u, place(u));
+        next = place(u + DW);
+    }
 
     F qh[NKS], ql[NKS];
     {
@@ -156,37 +196,20 @@ template <int DT, int D, int UK> __global__ __launch_bounds__(64 * DW) void deco
 #pragma unroll
         for (int ks = 0; ks < NKS; ++ks) split<DT>(x[ks], qh[ks], ql[ks]);
     }
-    const char *kb = a.kr + (int64_t)g * rows::PAGE * D * ESZ, *vb = a.v + (int64_t)g * rows::PAGE * D * ESZ;
-    const int64_t pstep = (int64_t)a.Hkv * rows::PAGE * D * ESZ;
-    const int32_t *table = a.table + (int64_t)s * a.maxp;
     f32x4 O[NDT];
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) O[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.0f;
-#pragma unroll 1
-    for (int u = u0 + wave; u < u1; u += DW) {
-        const int i = u / UP, h0 = UP == 1 ? 0 : u % UP, pl = i < pg.ns ? i : pg.w0 + i - pg.ns;
-        const int64_t id = max((int64_t)0, min((int64_t)table[pl], a.pages - 1));
-        const char *kp = kb + id * pstep, *vp = vb + id * pstep;
-        const int j0 = pl * rows::PAGE + 32 * h0;
-        F kf[2 * NH][NKS], vf[NDT][NH];
-#pragma unroll
-        for (int mt = 0; mt < 2 * NH; ++mt)
-#pragma unroll
-            for (int ks = 0; ks < NKS; ++ks)
-                kf[mt][ks] = Op<DT>::load(kp + (((2 * h0 + mt) * NKS + ks) * 64 + lane) * 8 * ESZ);
-#pragma unroll
-        for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-            for (int h = 0; h < NH; ++h) vf[dt][h] = Op<DT>::load(vp + ((dt * 2 + h0 + h) * 64 + lane) * 8 * ESZ);
+    const auto use = [&](Unit &x, int at) {
+        const int j0 = logical(at) * rows::PAGE + (UP == 1 ? 0 : at % UP * UK);
         f32x4 S[2 * NH];
 #pragma unroll
         for (int mt = 0; mt < 2 * NH; ++mt) {
             S[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int ks = 0; ks < NKS; ++ks) {
-                S[mt] = Mma16<DT>::mma(kf[mt][ks], qh[ks], S[mt]);
-                if constexpr (DT == 1) S[mt] = Mma16<DT>::mma(kf[mt][ks], ql[ks], S[mt]);
+                S[mt] = Mma16<DT>::mma(x.k[mt][ks], qh[ks], S[mt]);
+                if constexpr (DT == 1) S[mt] = Mma16<DT>::mma(x.k[mt][ks], ql[ks], S[mt]);
             }
         }
         // S[mt][e]: key j0 + 32 (mt / 2) + 8 lg + 4 (mt % 2) + e
@@ -203,11 +226,11 @@ template <int DT, int D, int UK> __global__ __launch_bounds__(64 * DW) void deco
                 }
 #pragma unroll
                 for (int dt = 0; dt < NDT; ++dt) {
-                    float x[8];
-                    Op<DT>::unpack(vf[dt][h], x);
+                    float y[8];
+                    Op<DT>::unpack(x.v[dt][h], y);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = see[e] ? x[e] : 0.0f;
-                    vf[dt][h] = Op<DT>::pack(x);
+                    for (int e = 0; e < 8; ++e) y[e] = see[e] ? y[e] : 0.0f;
+                    x.v[dt][h] = Op<DT>::pack(y);
                 }
             }
         }
@@ -236,33 +259,73 @@ template <int DT, int D, int UK> __global__ __launch_bounds__(64 * DW) void deco
             }
             const F pf = Op<DT>::pack(p);
 #pragma unroll
-            for (int dt = 0; dt < NDT; ++dt) O[dt] = Mma16<DT>::mma(vf[dt][h], pf, O[dt]);
+            for (int dt = 0; dt < NDT; ++dt) O[dt] = Mma16<DT>::mma(x.v[dt][h], pf, O[dt]);
         }
+    };
+    if constexpr (DT == 0 && D == 128) {   // two units would fill the registers
+#pragma unroll 1
+        while (u < u1) {
+            use(xa, u);
+            u += DW;
+            if (u < u1) load(xa, u, next);
+            if (u < u1) next = place(u + DW);
+        }
+    }
+#pragma unroll 1
+    for (; u < u1; u += 2 * DW) {
+        if (u + DW < u1) {
+            load(xb, u + DW, next);
+            next = place(u + 2 * DW);
+        }
+        use(xa, u);
+        if (u + DW >= u1) break;
+        if (u + 2 * DW < u1) {
+            load(xa, u + 2 * DW, next);
+            next = place(u + 3 * DW);
+        }
+        use(xb, u + DW);
     }
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
-    if (lg == 0) {
-        sm[wave][l16] = m;
-        sl[wave][l16] = l;
-    }
+    // the waves' sums meet in LDS: those of waves 4 and up fold into the first four's
+    const auto put = [&](int w) {
+        if (lg == 0) {
+            lds.m[w][l16] = m;
+            lds.l[w][l16] = l;
+        }
 #pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) *reinterpret_cast<f32x4 *>(&so[wave][l16][16 * dt + 4 * lg]) = O[dt];
+        for (int dt = 0; dt < NDT; ++dt) *reinterpret_cast<f32x4 *>(&lds.o[w][l16][16 * dt + 4 * lg]) = O[dt];
+    };
+    if constexpr (DW > 4) {
+        if (wave >= 4) put(wave - 4);
+        __syncthreads();
+        if (wave < 4) {
+            const float om = lds.m[wave][l16], ol = lds.l[wave][l16], mn = fmaxf(m, om);
+            const float fa = m == -INFINITY ? 0.0f : ex2(m - mn), fb = om == -INFINITY ? 0.0f : ex2(om - mn);
+            l = fmaf(ol, fb, l * fa);
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt)
+                O[dt] = O[dt] * fa + *reinterpret_cast<const f32x4 *>(&lds.o[wave][l16][16 * dt + 4 * lg]) * fb;
+            m = mn;
+        }
+    }
+    if (wave < 4) put(wave);   // its own place: nobody else has read it
     __syncthreads();
-    // the waves' parts: thread (head, 4 elements)
+    // thread (head, 4 elements)
     for (int x = threadIdx.x; x < 16 * D / 4; x += 64 * DW) {
         const int hc = x / (D / 4), e = x % (D / 4) * 4;
         if (c0 + hc >= a.G) break;
         float mm = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < DW; ++w) mm = fmaxf(mm, sm[w][hc]);
+        for (int w = 0; w < 4; ++w) mm = fmaxf(mm, lds.m[w][hc]);
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
         float ll = 0.0f;
 #pragma unroll
-        for (int w = 0; w < DW; ++w) {
-            const float f = sm[w][hc] == -INFINITY ? 0.0f : ex2(sm[w][hc] - mm);
-            // a wave without keys has zeros; one whose scores are all -inf as well
-            ll = fmaf(sl[w][hc], f, ll);
-            o = o + *reinterpret_cast<const f32x4 *>(&so[w][hc][e]) * f;
+        for (int w = 0; w < 4; ++w) {
+            // a wave without keys, or with scores that are all -inf, has zeros
+            const float f = lds.m[w][hc] == -INFINITY ? 0.0f : ex2(lds.m[w][hc] - mm);
+            ll = fmaf(lds.l[w][hc], f, ll);
+            o = o + *reinterpret_cast<const f32x4 *>(&lds.o[w][hc][e]) * f;
         }
         const int64_t row = (int64_t)s * a.Hq + g * a.G + c0 + hc;
         if (a.slots == 1) {
@@ -274,7 +337,7 @@ template <int DT, int D, int UK> __global__ __launch_bounds__(64 * DW) void deco
             else
                 *reinterpret_cast<f32x4 *>(a.out + (row * D + e) * 4) = r;
         } else {
-            const int64_t at = row * a.slots + a.slot0 + blockIdx.y;
+            const int64_t at = row * a.slots + a.slot0 + part;
             *reinterpret_cast<f32x4 *>(a.po + at * D + e) = o;
             if (e == 0) {
                 a.pml[2 * at] = mm;
@@ -284,25 +347,41 @@ template <int DT, int D, int UK> __global__ __launch_bounds__(64 * DW) void deco
     }
 }
 
+constexpr int DW = 8;   // waves of a decode workgroup
+template <int DT, int D> __global__ __launch_bounds__(64 * DW) void decode_kernel(const Args a) {
+    __shared__ DecodeLds<D> lds;
+    decode_part<DT, D, DW>(a, lds, blockIdx.x, blockIdx.y);
+}
+
 // -------------------------------------------------------------------- rows ----
-// SHARED: the rows of all tokens over the shared pages (blockIdx.x: 128-row
-// tile); else the rows of one sequence's tokens over its own pages (blockIdx.x:
-// tile of the ragged batch).  blockIdx.y: KV head, blockIdx.z: part of the tiles.
-template <int DT, int D, bool SHARED> __global__ __launch_bounds__(64 * rows::NW, (DT == 1 && D == 64 ? 3 : rows::WAVES<DT, D>)) void rows_kernel(const Args a) {
-    extern __shared__ __align__(16) char smem[];
+// SHARED: the rows of all tokens over the shared pages (x: 128-row tile); else the
+// rows of one sequence's tokens over its own pages (x: tile of the ragged batch).
+// g: KV head, z: part, a run of a.part pages.
+template <int DT, int D, bool SHARED>
+__device__ __forceinline__ void rows_part(const Args &a, char *smem, int x, int g, int z) {
     typedef typename Op<DT>::F F;
-    constexpr int ESZ = DT == 1 ? 2 : 4, NKS = D / 16;
+    constexpr int ESZ = DT == 1 ? 2 : 4, NKS = D / 16, KT = rows::KEYS<DT, D>, TP = rows::PAGE / KT;
     constexpr bool LO = DT == 1;
     const int lane = threadIdx.x & 63, hf = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int g = blockIdx.y;
-    int s = 0, tile = blockIdx.x, first = 0, cnt = a.T;
-    if constexpr (!SHARED) {
-        s = ragged::find(blockIdx.x, a.Bd, [&](int i) {
+    rows::PageKV<DT, D> src;
+    src.page = (int64_t)a.Hkv * rows::PAGE * D * ESZ;
+    src.k = a.kr + (int64_t)g * rows::PAGE * D * ESZ;
+    src.v = a.v + (int64_t)g * rows::PAGE * D * ESZ;
+    src.pages = a.pages;
+    const int it0 = z * a.part * TP;
+    int s = 0, tile = x, first = 0, cnt = a.T, it1 = 0, ns = 0, wt0 = 0;
+    if constexpr (SHARED) {   // every tile of the part, whatever the rows see of it: it can be staged at once
+        src.table = a.table;
+        it1 = min(a.shared * TP, it0 + a.part * TP);
+        rows::attend_begin(src, smem, it0, it1, 0, 0);
+    } else {
+        s = ragged::find(x, a.Bd, [&](int i) {
             int f;
             return (ragged::tokens(a.cu, i, a.T, f) * a.G + rows::RT - 1) / rows::RT;
         }, tile);
         if (s < 0) return;
         cnt = ragged::tokens(a.cu, s, a.T, first);
+        src.table = a.table + (int64_t)s * a.maxp;
     }
     const int nr = cnt * a.G, r0 = tile * rows::RT, rw = r0 + wave * rows::RW, r = rw + (lane & 31);
     const bool in = r < nr;
@@ -331,49 +410,43 @@ template <int DT, int D, bool SHARED> __global__ __launch_bounds__(64 * rows::NW
     w.lo_max = __builtin_amdgcn_readfirstlane(v[1]);
     w.hi_min = __builtin_amdgcn_readfirstlane(v[2]);
     w.hi_max = __builtin_amdgcn_readfirstlane(v[3]);
-    __shared__ int bounds[rows::NW][2];
-    if (lane == 0) {
-        bounds[wave][0] = w.lo_min;
-        bounds[wave][1] = w.hi_max;
-    }
-    __syncthreads();
-    int lo = 0x7fffffff, hi = 0;
-#pragma unroll
-    for (int i = 0; i < rows::NW; ++i) {
-        lo = min(lo, bounds[i][0]);
-        hi = max(hi, bounds[i][1]);
-    }
-    int ns = 0, wt0 = 0;
-    const int nt = hi > 0 ? rows::tile_list<rows::KEYS<DT, D>>(lo, hi, w.S, ns, wt0) : 0;
-    constexpr int TP = rows::PAGE / rows::KEYS<DT, D>;   // tiles of a page
-    const int z = blockIdx.z, it0 = z * a.part * TP, it1 = min(nt, it0 + a.part * TP);
     const int64_t row = (int64_t)t * a.Hq + head, at = row * a.slots + a.slot0 + z;
-    if (it0 >= it1 && a.slots > 1) {   // nothing of the row's keys in this part
-        if (in && hf == 0) {
-            a.pml[2 * at] = -INFINITY;
-            a.pml[2 * at + 1] = 0.0f;
+    if constexpr (!SHARED) {
+        __shared__ int bounds[rows::NW][2];
+        if (lane == 0) {
+            bounds[wave][0] = w.lo_min;
+            bounds[wave][1] = w.hi_max;
         }
-        return;
+        __syncthreads();
+        int lo = 0x7fffffff, hi = 0;
+#pragma unroll
+        for (int i = 0; i < rows::NW; ++i) {
+            lo = min(lo, bounds[i][0]);
+            hi = max(hi, bounds[i][1]);
+        }
+        const int nt = hi > 0 ? rows::tile_list<KT>(lo, hi, w.S, ns, wt0) : 0;
+        it1 = min(nt, it0 + a.part * TP);
+        if (it0 >= it1 && a.slots > 1) {   // nothing of the rows' keys in this part
+            if (in && hf == 0) {
+                a.pml[2 * at] = -INFINITY;
+                a.pml[2 * at + 1] = 0.0f;
+            }
+            return;
+        }
+        rows::attend_begin(src, smem, it0, it1, ns, wt0);
     }
-
     F qh[NKS], ql[NKS];
     {
-        float x[NKS][8];
-        const char *row = a.q + (int64_t)t * a.qst + head * a.qsh;
+        float y[NKS][8];
+        const char *q = a.q + (int64_t)t * a.qst + head * a.qsh;
 #pragma unroll
-        for (int ks = 0; ks < NKS; ++ks) Op<DT>::unpack(Op<DT>::load(row + (16 * ks + 8 * hf) * ESZ), x[ks]);
+        for (int ks = 0; ks < NKS; ++ks) Op<DT>::unpack(Op<DT>::load(q + (16 * ks + 8 * hf) * ESZ), y[ks]);
         const int64_t turn = max((int64_t)0, min((int64_t)pos, a.n_tab - 1)) * D;
-        finish_q<D, 16>(x, 8 * hf, a.gain ? a.gain + head : nullptr, a.eps, a.cos ? a.cos + turn : nullptr,
+        finish_q<D, 16>(y, 8 * hf, a.gain ? a.gain + head : nullptr, a.eps, a.cos ? a.cos + turn : nullptr,
                         a.sin ? a.sin + turn : nullptr, a.scales[sq] * LOG2E);
 #pragma unroll
-        for (int ks = 0; ks < NKS; ++ks) split<DT>(x[ks], qh[ks], ql[ks]);
+        for (int ks = 0; ks < NKS; ++ks) split<DT>(y[ks], qh[ks], ql[ks]);
     }
-    rows::PageKV<DT, D> src;
-    src.page = (int64_t)a.Hkv * rows::PAGE * D * ESZ;
-    src.k = a.kr + (int64_t)g * rows::PAGE * D * ESZ;
-    src.v = a.v + (int64_t)g * rows::PAGE * D * ESZ;
-    src.table = a.table + (SHARED ? 0 : (int64_t)s * a.maxp);
-    src.pages = a.pages;
     rows::RowAcc<DT, D> acc;
     rows::attend<DT, D, LO>(src, smem, qh, ql, 1.0f, it0, it1, ns, wt0, w, acc);
     float l = acc.l + rows::other_half(acc.l);
@@ -385,9 +458,7 @@ template <int DT, int D, bool SHARED> __global__ __launch_bounds__(64 * rows::NW
     if (!in) return;
     if (!valid) {
 #pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc.O[dt][e] = 0.0f;
+        for (int dt = 0; dt < D / 32; ++dt) acc.O[dt] = f32x16{0.0f};
         acc.m = -INFINITY;
         l = 0.0f;
     }
@@ -400,6 +471,27 @@ template <int DT, int D, bool SHARED> __global__ __launch_bounds__(64 * rows::NW
             a.pml[2 * at + 1] = l;
         }
     }
+}
+
+template <int DT, int D, bool SHARED>
+__global__ __launch_bounds__(64 * rows::NW, (DT == 1 && D == 64 ? 3 : rows::WAVES<DT, D>)) void rows_kernel(
+    const Args a) {
+    extern __shared__ __align__(16) char smem[];
+    rows_part<DT, D, SHARED>(a, smem, blockIdx.x, blockIdx.y, blockIdx.z);
+}
+
+// The shared pages for all rows (the first nshared workgroups, which take longest)
+// and every sequence's own pages for its newest token.
+template <int DT, int D>
+__global__ __launch_bounds__(64 * rows::NW, (rows::WAVES<DT, D>)) void shared_kernel(
+    const Args a, const Args own, int ptiles, int nshared, int groups) {
+    extern __shared__ __align__(16) char smem[];
+    const int i = blockIdx.x;
+    if (i < nshared)
+        rows_part<DT, D, true>(a, smem, i % ptiles, i / ptiles % a.Hkv, i / (ptiles * a.Hkv));
+    else
+        decode_part<DT, D, rows::NW>(own, *reinterpret_cast<DecodeLds<D> *>(smem), (i - nshared) % groups,
+                                     (i - nshared) / groups);
 }
 
 // out = sum of the parts' O 2^(m - max) over sum of their l 2^(m - max); a row
@@ -512,7 +604,8 @@ static Plan plan(int64_t T, int64_t Bd, int64_t Hq, int64_t Hkv, int64_t W, int6
     p.ptiles = (T * G + rows::RT - 1) / rows::RT;
     if (one) {
         const int64_t groups = Bd * Hkv * ((G + 15) / 16);
-        p.own = parts_of(pages, (2048 + groups - 1) / groups, 4, p.own_pages);
+        // some 1024 workgroups of 8 waves; but up to 32 pages, 4 a wave, need no join
+        p.own = parts_of(pages, (1024 + groups - 1) / groups, shared ? 4 : pages <= 32 ? 32 : 8, p.own_pages);
     } else {
         p.tiles = p.ptiles + Bd;
         p.own = parts_of(pages, AIMR / (p.ptiles * Hkv), 8, p.own_pages);
@@ -521,36 +614,33 @@ static Plan plan(int64_t T, int64_t Bd, int64_t Hq, int64_t Hkv, int64_t W, int6
     return p;
 }
 
-template <class K> static int lds_room(K kern, size_t bytes) {
-    if (bytes <= 65536) return HBA_OK;
-    return hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
-                               (int)bytes) == hipSuccess
-               ? HBA_OK
-               : HBA_ERR_LAUNCH;
-}
-
 template <int DT, int D> static int launch(Args a, const Plan &p, hipStream_t s) {
     constexpr size_t lds = 2 * rows::PageKV<DT, D>::BYTES;
-    constexpr int UK = DT == 1 && D == 64 ? 64 : 32;
+    static_assert(sizeof(DecodeLds<D>) <= 65536 && lds <= 65536, "LDS without an attribute");
+    const int64_t groups = (int64_t)a.Bd * a.Hkv * ((a.G + 15) / 16);
     a.slots = p.slots();
-    if (p.prefix) {
-        a.slot0 = 0;
-        a.part = p.prefix_pages;
-        if (int st = lds_room(rows_kernel<DT, D, true>, lds)) return st;
-        hipLaunchKernelGGL((rows_kernel<DT, D, true>), dim3((unsigned)p.ptiles, (unsigned)a.Hkv, (unsigned)p.prefix),
-                           dim3(64 * rows::NW), lds, s, a);
-        HBA_LAUNCH_CHECK();
-    }
-    a.slot0 = p.prefix;
-    if (a.cu) {
-        a.part = p.own_pages;
-        if (int st = lds_room(rows_kernel<DT, D, false>, lds)) return st;
-        hipLaunchKernelGGL((rows_kernel<DT, D, false>), dim3((unsigned)p.tiles, (unsigned)a.Hkv, (unsigned)p.own),
-                           dim3(64 * rows::NW), lds, s, a);
+    Args own = a;
+    own.slot0 = p.prefix;
+    own.part = p.own_pages;
+    a.part = p.prefix_pages;
+    if (p.prefix && !a.cu) {
+        const int64_t nshared = p.ptiles * a.Hkv * p.prefix, grid = nshared + groups * p.own;
+        if (grid > 0x7fffffff) return HBA_ERR_UNSUPPORTED;
+        constexpr size_t both = lds > sizeof(DecodeLds<D>) ? lds : sizeof(DecodeLds<D>);
+        hipLaunchKernelGGL((shared_kernel<DT, D>), dim3((unsigned)grid), dim3(64 * rows::NW), both, s, a, own,
+                           (int)p.ptiles, (int)nshared, (int)groups);
     } else {
-        a.part = p.own_pages;
-        const int64_t groups = (int64_t)a.Bd * a.Hkv * ((a.G + 15) / 16);
-        hipLaunchKernelGGL((decode_kernel<DT, D, UK>), dim3((unsigned)groups, (unsigned)p.own), dim3(64 * DW), 0, s, a);
+        if (p.prefix)
+            hipLaunchKernelGGL((rows_kernel<DT, D, true>),
+                               dim3((unsigned)p.ptiles, (unsigned)a.Hkv, (unsigned)p.prefix), dim3(64 * rows::NW), lds,
+                               s, a);
+        HBA_LAUNCH_CHECK();
+        if (a.cu)
+            hipLaunchKernelGGL((rows_kernel<DT, D, false>), dim3((unsigned)p.tiles, (unsigned)a.Hkv, (unsigned)p.own),
+                               dim3(64 * rows::NW), lds, s, own);
+        else
+            hipLaunchKernelGGL((decode_kernel<DT, D>), dim3((unsigned)groups, (unsigned)p.own), dim3(64 * DW), 0, s,
+                               own);
     }
     HBA_LAUNCH_CHECK();
     if (a.slots > 1) {

@@ -362,8 +362,19 @@ template <int DT, int D> struct RowAcc {
     float m, l;       // running maximum (log2 units; -inf: nothing seen yet), and this half's part of the sum
 };
 
-// One pass of the workgroup's rows over tiles it0 .. it1 - 1 of their list
-// (tile it < ns: sinks, tile it; else tile wt0 + it - ns).  c: logits to log2
+// Stages the first of tiles it0 .. it1 - 1 of a list (tile it < ns: sinks, tile it;
+// else tile wt0 + it - ns): attend goes on from there.  What a kernel loads in
+// between comes while the tile does.
+template <class Src>
+__device__ __forceinline__ void attend_begin(Src &src, char *smem, int it0, int it1, int ns, int wt0) {
+    const auto tile = [&](int it) { return it < ns ? it : wt0 + it - ns; };
+    if (it0 >= it1) return;
+    src.next(tile(it0));
+    src.stage(tile(it0), lds_offset(smem));
+    src.next(tile(min(it0 + 1, it1 - 1)));
+}
+
+// One pass of the workgroup's rows over the tiles.  c: logits to log2
 // units.  LO: the queries come as two parts in log2 units already (c = 1); their
 // products then start from -m instead of 0.  Every wave of the workgroup calls
 // it; it leaves no wave reading LDS.
@@ -382,11 +393,6 @@ __device__ __forceinline__ void attend(Src &src, char *smem, const typename Op<D
     float shift = 0.0f;   // -m, or 0 while nothing is seen
     const uint32_t lds = lds_offset(smem);
     const auto tile = [&](int it) { return it < ns ? it : wt0 + it - ns; };
-    if (it0 < it1) {
-        src.next(tile(it0));
-        src.stage(tile(it0), lds);
-        src.next(tile(min(it0 + 1, it1 - 1)));
-    }
 #pragma unroll 1
     for (int it = it0; it < it1; ++it) {
         wait_vm<0>();

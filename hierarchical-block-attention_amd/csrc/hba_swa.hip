@@ -128,11 +128,12 @@ __global__ __launch_bounds__(64 * NW, (DT == 1 && D == 64 ? 3 : WAVES<DT, D>)) v
     extern __shared__ __align__(16) char smem[];
     Rows x;
     if (!find_rows<D>(a, x)) return;
-    typename Op<DT>::F q[D / 16];
-    load_rows<DT, D>(q_row<DT, D>(a, x), x.valid, q);
     DenseKV<DT, D> src = keys<DT, D>(a, x);
     int ns, wt0;
     const int nt = tile_list<KEYS<DT, D>>(x.lo, x.hi, a.S, ns, wt0);
+    attend_begin(src, smem, 0, nt, ns, wt0);
+    typename Op<DT>::F q[D / 16];
+    load_rows<DT, D>(q_row<DT, D>(a, x), x.valid, q);
     RowAcc<DT, D> acc;
     attend<DT, D, false>(src, smem, q, nullptr, a.c, 0, nt, ns, wt0, x.w, acc);
     float l = acc.l + other_half(acc.l);
