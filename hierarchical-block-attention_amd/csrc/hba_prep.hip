@@ -227,15 +227,70 @@ template <int D, bool LONE> struct SummSmem {
     float prl[LONE ? 8 : 1][D];
 };
 
+// summarize_staged's pooling and projection: thread tid has column tid % D of slots
+// tid / D, tid / D + 256 / D, ... (NQ of them), one chain each.
+template <int D, int NQ, class SM> __device__ __forceinline__ void pool_columns(SM &sm, int m, int tid) {
+    const int dd = tid % D, s0 = __builtin_amdgcn_readfirstlane(tid / D);
+    if (s0 >= m) return;
+    float acc[NQ];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) acc[q] = 0.0f;
+#pragma unroll 8
+    for (int t = 0; t < 64; ++t) {
+        const float x = sm.kb[t][dd];
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) acc[q] = fmaf(sm.att[min(s0 + q * (256 / D), m - 1)][t], x, acc[q]);
+    }
+#pragma unroll
+    for (int q = 0; q < NQ; ++q)
+        if (s0 + q * (256 / D) < m) sm.pooled[s0 + q * (256 / D)][dd] = acc[q];
+}
+template <int DT, int D, int NQ, class SM>
+__device__ __forceinline__ void project_columns(SM &sm, const float *__restrict__ pj, int m,
+                                                typename St<DT>::T *__restrict__ dst, int tid) {
+    const int ee = tid % D, s0 = __builtin_amdgcn_readfirstlane(tid / D);
+    if (s0 >= m) return;
+    float acc[NQ];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) acc[q] = 0.0f;
+#pragma unroll 1
+    for (int d0 = 0; d0 < D; d0 += 16) {
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = pj[(d0 + i) * D + ee];
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+#pragma unroll
+            for (int q = 0; q < NQ; ++q)
+                acc[q] = fmaf(sm.pooled[min(s0 + q * (256 / D), m - 1)][d0 + i], x[i], acc[q]);
+    }
+#pragma unroll
+    for (int q = 0; q < NQ; ++q)
+        if (s0 + q * (256 / D) < m) St<DT>::st(dst, (int64_t)(s0 + q * (256 / D)) * D + ee, acc[q]);
+}
+template <int D, class SM> __device__ __forceinline__ void summarize_columns(SM &sm, int m, int tid) {
+    if (m * D <= 256) pool_columns<D, 1>(sm, m, tid);
+    else if (m * D <= 512) pool_columns<D, 2>(sm, m, tid);
+    else pool_columns<D, 4>(sm, m, tid);
+}
+template <int DT, int D, class SM>
+__device__ __forceinline__ void summarize_project(SM &sm, const float *__restrict__ pj, int m,
+                                                  typename St<DT>::T *__restrict__ dst, int tid) {
+    if (m * D <= 256) project_columns<DT, D, 1>(sm, pj, m, dst, tid);
+    else if (m * D <= 512) project_columns<DT, D, 2>(sm, pj, m, dst, tid);
+    else project_columns<DT, D, 4>(sm, pj, m, dst, tid);
+}
+
 // Slot summaries of one block whose 64 key rows are staged in sm.kb: slot
 // scores, softmax over the 64 keys of each slot, pooling, projection.  Every
 // output is one sequential fma chain in the index order of the sums
 // (probes . key, att . keys, pooled . proj), so both forms below give the
 // same bits.  256 threads; starts after the staging barrier; its callers
 // barrier before restaging sm.kb.
-//   LONE = false (many workgroups, prefill and page lists): probes and the
-//     projection are read from global memory inside the chains; other
-//     workgroups hide the load latency.
+//   LONE = false (many workgroups, prefill and page lists): probes come as
+//     scalar loads (a wave has one slot), the projection from global memory 16
+//     rows at a time; a thread's outputs share a column, so each key element and
+//     projection element is read once for all of them.
 //   LONE = true (a workgroup or two, the decode loop's page fill): probes and
 //     the projection are staged through LDS in coalesced bulk loads (the
 //     projection in chunks over sm.kb's space), so the workgroup waits on a
@@ -256,7 +311,9 @@ __device__ __forceinline__ void summarize_staged(SummSmem<D, LONE> &sm, const fl
 #pragma unroll 16
             for (int dd = 0; dd < D; ++dd) acc = fmaf(sm.prl[s][dd], sm.kb[t][dd], acc);
         } else {
-            for (int dd = 0; dd < D; ++dd) acc = fmaf(pr[s * D + dd], sm.kb[t][dd], acc);
+            const float *row = pr + __builtin_amdgcn_readfirstlane(s) * D;   // 64 keys of one slot to a wave
+#pragma unroll 16
+            for (int dd = 0; dd < D; ++dd) acc = fmaf(row[dd], sm.kb[t][dd], acc);
         }
         sm.att[s][t] = acc * att_scale;
     }
@@ -272,20 +329,19 @@ __device__ __forceinline__ void summarize_staged(SummSmem<D, LONE> &sm, const fl
         }
     }
     __syncthreads();
-    for (int e = tid; e < m * D; e += 256) {
-        int s = e / D, dd = e % D;
-        float acc = 0.0f;
-        for (int t = 0; t < BK; ++t) acc = fmaf(sm.att[s][t], sm.kb[t][dd], acc);
-        sm.pooled[s][dd] = acc;
+    if constexpr (LONE) {
+        for (int e = tid; e < m * D; e += 256) {
+            int s = e / D, dd = e % D;
+            float acc = 0.0f;
+            for (int t = 0; t < BK; ++t) acc = fmaf(sm.att[s][t], sm.kb[t][dd], acc);
+            sm.pooled[s][dd] = acc;
+        }
+    } else {
+        summarize_columns<D>(sm, m, tid);
     }
     __syncthreads();
     if constexpr (!LONE) {
-        for (int e = tid; e < m * D; e += 256) {
-            int s = e / D, ee = e % D;
-            float acc = 0.0f;
-            for (int dd = 0; dd < D; ++dd) acc = fmaf(sm.pooled[s][dd], pj[dd * D + ee], acc);
-            St<DT>::st(dst, (int64_t)s * D + ee, acc);
-        }
+        summarize_project<DT, D>(sm, pj, m, dst, tid);
     } else {
         // up to 4 outputs per thread (m * D <= 1024); pj rows staged CHR at a
         // time into the key tile's space (65 or 64 rows fit; CHR divides D)
