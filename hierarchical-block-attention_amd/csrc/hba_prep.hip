@@ -673,23 +673,95 @@ __device__ __forceinline__ NewTokens new_tokens(const RaggedArgs &a, int s) {
     return x;
 }
 
+// A page's keys in LDS: 8 elements of a key together, keys beside one another, a
+// chunk of room after every 64.  Written by rows, read by columns and by rows, all
+// without bank conflicts.
+template <int DT, int D> struct KeyTile {
+    using T = typename St<DT>::T;
+    __align__(16) T x[D / 8 * 65 * 8];
+    __device__ __forceinline__ T *at(int j, int t) { return x + ((t / 8) * 65 + j) * 8 + t % 8; }
+};
+
+// Slot summaries of the page whose 64 keys are in a tile: summarize_staged's chains
+// in the same order, so the same bits, from the keys as stored.  A thread has 4
+// columns of one slot's pooled row.
+template <int DT, int D, class SM>
+__device__ __forceinline__ void summarize_tile(SM &sm, const float *__restrict__ pr, const float *__restrict__ pj,
+                                               int m, float att_scale, typename St<DT>::T *__restrict__ dst, int tid) {
+    for (int e = tid; e < m * 64; e += 256) {
+        const int s = __builtin_amdgcn_readfirstlane(e / 64), t = e % 64;
+        float acc = 0.0f;
+#pragma unroll 4
+        for (int c = 0; c < D / 8; ++c) {
+            float x[8];
+            load8<DT>(sm.keys.at(t, 8 * c), x);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) acc = fmaf(pr[s * D + 8 * c + u], x[u], acc);
+        }
+        sm.att[s][t] = acc * att_scale;
+    }
+    __syncthreads();
+    for (int s = tid / 64; s < m; s += 4) {   // softmax over the 64 keys: one wave per slot
+        const float x = sm.att[s][tid % 64], e = expf(x - wave_max(x));
+        sm.att[s][tid % 64] = e / wave_sum(e);
+    }
+    __syncthreads();
+    for (int e = tid; e < m * (D / 4); e += 256) {
+        const int s = e / (D / 4), t0 = 4 * (e % (D / 4));
+        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+        for (int t = 0; t < 64; ++t) {
+            const float w = sm.att[s][t];
+            const auto *x = sm.keys.at(t, t0);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) acc[u] = fmaf(w, St<DT>::ld(x, u), acc[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) sm.pooled[s][t0 + u] = acc[u];
+    }
+    __syncthreads();
+    summarize_project<DT, D>(sm, pj, m, dst, tid);
+}
+
+template <class T> __device__ __forceinline__ void load_raw(T (&x)[8], const T *p) {
+    using V = uint32_t __attribute__((ext_vector_type(2 * sizeof(T))));
+    const V v = *reinterpret_cast<const V *>(p);
+    __builtin_memcpy(x, &v, sizeof v);
+}
+
 // One workgroup per (page that gets tokens, KV head): D/8 lanes a row as in
 // prep_tile (the same chain for the norm, so kc has the bits of every other way
 // to append it), 256 / (D/8) rows at a time.  kr is rounded once, from the
-// normalised key in fp32.  The values go through LDS, so that a page's 8-token
-// chunks are written whole where the batch has all 8.  The page's summaries
-// follow when its last token is among the new ones (the earlier keys are read
-// back: no other workgroup writes this page).
-// HBM-bound: k and v read once, kc, kr and v written once.
+// normalised key in fp32.  The page's summaries follow when its last token is
+// among the new ones (the earlier keys are read back: no other workgroup writes
+// this page).
+// HBM-bound in the large: k and v read once, kc, kr and v written once.  14000
+// tokens, 4 KV heads, d = 128, bf16 with summaries: 37 us, 21 at a copy's rate;
+// 59 before each of these:
+//   - values, rotated keys and keys go through LDS in turn, and a wave writes 1 KB
+//     runs of the page where rows written as they come fill 64 bytes of a line at a
+//     time; the summary reads the same keys there;
+//   - 22 KB of LDS, so that all 1088 workgroups are there at once (at 40 KB four to
+//     a CU, 1024, and the rest follow as a second round: 46 us);
+//   - workgroups of one page's heads run on one XCD, whose L2 then has their rows
+//     of the cos/sin tables.
 template <int DT, int D, bool SUMM>
 __global__ __launch_bounds__(256) void kv_append_ragged_kernel(const RaggedArgs a) {
     using T = typename St<DT>::T;
     constexpr int TPH = D / 8, RPP = 256 / TPH, ESZ = DT == 1 ? 2 : 4, VS = 64 + 16 / ESZ;
-    __shared__ __align__(16) T vs[D][VS];
-    __shared__ SummSmem<SUMM ? D : 1, false> sm;
-    const int tid = threadIdx.x, g = blockIdx.y;
+    // values, rotated keys, keys in turn: 22 KB (bf16, d = 128)
+    __shared__ union {
+        __align__(16) T vs[D][VS];
+        struct {
+            KeyTile<DT, D> keys;
+            float att[SUMM ? 8 : 1][64], pooled[SUMM ? 8 : 1][D];
+        } sm;
+    } lds;
+    auto &vs = lds.vs;
+    auto &sm = lds.sm;
+    const int tid = threadIdx.x, g = blockIdx.x / 8 % a.Hkv;
     int slot;
-    const int s = ragged::find(blockIdx.x, a.Bd, [&](int i) {
+    const int s = ragged::find(blockIdx.x / 8 / a.Hkv * 8 + blockIdx.x % 8, a.Bd, [&](int i) {
         const NewTokens x = new_tokens(a, i);
         return x.last > x.first ? (x.last - 1) / 64 - x.first / 64 + 1 : 0;
     }, slot);
@@ -706,15 +778,52 @@ __global__ __launch_bounds__(256) void kv_append_ragged_kernel(const RaggedArgs 
     const int jl = tid % TPH, t0 = 8 * jl;
     const bool lo = t0 < D / 2;
     const float gn = a.kgain ? a.kgain[g] : 0.0f;
+    // all loads of a kind at once: a row outside the new ones repeats one of those
+    T kx[64 / RPP][8], vx[64 / RPP][8];
+#pragma unroll
+    for (int pass = 0; pass < 64 / RPP; ++pass) {
+        const int64_t tok = x.c0 + (p0 + min(max(pass * RPP + tid / TPH, ja), jb - 1) - x.first);
+        load_raw(kx[pass], reinterpret_cast<const T *>(a.k + tok * a.kst + g * a.ksh) + t0);
+        load_raw(vx[pass], reinterpret_cast<const T *>(a.v + tok * a.vst + g * a.vsh) + t0);
+    }
+#pragma unroll
+    for (int pass = 0; pass < 64 / RPP; ++pass) {
+        const int j = pass * RPP + tid / TPH;
+        if (j >= ja && j < jb) {
+#pragma unroll
+            for (int u = 0; u < 8; ++u) vs[t0 + u][j ^ (8 * (jl % 8))] = vx[pass][u];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int c = tid; c < 8 * D; c += 256) {
+        int t, j0;
+        page_val_chunk(c, t, j0);
+        const int jp = j0 ^ (8 * (t / 8 % 8));
+        if (j0 >= ja && j0 + 8 <= jb) {
+            if constexpr (DT == 1) {
+                *reinterpret_cast<uint4 *>(vp + 8 * c) = *reinterpret_cast<const uint4 *>(&vs[t][jp]);
+            } else {
+                reinterpret_cast<float4 *>(vp + 8 * c)[0] = *reinterpret_cast<const float4 *>(&vs[t][jp]);
+                reinterpret_cast<float4 *>(vp + 8 * c)[1] = *reinterpret_cast<const float4 *>(&vs[t][jp + 4]);
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if (j0 + u >= ja && j0 + u < jb) vp[8 * c + u] = vs[t][jp + u];
+        }
+    }
+    __syncthreads();   // vs becomes sm
 #pragma unroll
     for (int pass = 0; pass < 64 / RPP; ++pass) {
         const int j = pass * RPP + tid / TPH;
         if (pass * RPP >= jb || pass * RPP + RPP <= ja) continue;     // uniform
-        const bool act = j >= ja && j < jb;
-        const int64_t tok = x.c0 + (p0 + (act ? j : ja) - x.first), pos = p0 + (act ? j : ja);
-        float y[8], vv[8];
-        load8<DT>(reinterpret_cast<const T *>(a.k + tok * a.kst + g * a.ksh) + t0, y);
-        load8<DT>(reinterpret_cast<const T *>(a.v + tok * a.vst + g * a.vsh) + t0, vv);
+        const int64_t pos = p0 + min(max(j, ja), jb - 1);
+        float cs[8], sn[8], y[8], z[8];
+        load8<0>(a.cosT + pos * D + t0, cs);
+        load8<0>(a.sinT + pos * D + t0, sn);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) y[u] = St<DT>::ld(kx[pass], u);
         if (a.kgain) {
             float run = 0.0f;
 #pragma unroll
@@ -735,56 +844,41 @@ __global__ __launch_bounds__(256) void kv_append_ragged_kernel(const RaggedArgs 
 #pragma unroll
             for (int u = 0; u < 8; ++u) y[u] = (y[u] / rr) * gn;
         }
-        float cs[8], sn[8], z[8];
-        load8<0>(a.cosT + pos * D + t0, cs);
-        load8<0>(a.sinT + pos * D + t0, sn);
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             const float part = __shfl_xor(y[u], TPH / 2, 64);
             z[u] = y[u] * cs[u] + (lo ? -part : part) * sn[u];
+            St<DT>::st(kx[pass], u, y[u]);
         }
-        if (act) {
-            const int64_t o = page_key_off(j, t0, D);
-            if (a.kc) store8<DT>(kcp + o, y);
-            store8<DT>(krp + o, z);
-#pragma unroll
-            for (int u = 0; u < 8; ++u) St<DT>::st(&vs[t0 + u][0], j, vv[u]);
-            if constexpr (SUMM)
-                if (fills)
-#pragma unroll
-                    for (int u = 0; u < 8; ++u) sm.kb[j][t0 + u] = St<DT>::rnd(y[u]);
-        }
+        if (j >= ja && j < jb) store8<DT>(sm.keys.at(j, t0), z);
     }
     __syncthreads();
 #pragma unroll
     for (int c = tid; c < 8 * D; c += 256) {
-        int t, j0;
-        page_val_chunk(c, t, j0);
-        if (j0 >= ja && j0 + 8 <= jb) {
-            if constexpr (DT == 1) {
-                *reinterpret_cast<uint4 *>(vp + 8 * c) = *reinterpret_cast<const uint4 *>(&vs[t][j0]);
-            } else {
-                reinterpret_cast<float4 *>(vp + 8 * c)[0] = *reinterpret_cast<const float4 *>(&vs[t][j0]);
-                reinterpret_cast<float4 *>(vp + 8 * c)[1] = *reinterpret_cast<const float4 *>(&vs[t][j0 + 4]);
-            }
-        } else {
+        int j, e0;
+        page_key_chunk(c, D, j, e0);
+        if (j >= ja && j < jb) __builtin_memcpy(krp + 8 * c, sm.keys.at(j, e0), 8 * sizeof(T));
+    }
+    if (!a.kc) return;
+    __syncthreads();
 #pragma unroll
-            for (int u = 0; u < 8; ++u)
-                if (j0 + u >= ja && j0 + u < jb) vp[8 * c + u] = vs[t][j0 + u];
-        }
+    for (int pass = 0; pass < 64 / RPP; ++pass) {
+        const int j = pass * RPP + tid / TPH;
+        if (j >= ja && j < jb) __builtin_memcpy(sm.keys.at(j, t0), kx[pass], sizeof kx[pass]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int c = tid; c < 8 * D; c += 256) {
+        int j, e0;
+        page_key_chunk(c, D, j, e0);
+        if (j >= ja && j < jb) __builtin_memcpy(kcp + 8 * c, sm.keys.at(j, e0), 8 * sizeof(T));
+        else if (SUMM && fills) __builtin_memcpy(sm.keys.at(j, e0), kcp + 8 * c, 8 * sizeof(T));   // it was there
     }
     if constexpr (SUMM) {
         if (!fills) return;
-        for (int c = tid; c < 8 * D; c += 256) {   // the keys that were there
-            int j, e0;
-            page_key_chunk(c, D, j, e0);
-            if (j >= ja) continue;
-#pragma unroll
-            for (int u = 0; u < 8; ++u) sm.kb[j][e0 + u] = St<DT>::ld(kcp, 8 * c + u);
-        }
         __syncthreads();
-        summarize_staged<DT, D, false>(sm, a.probes + (int64_t)g * a.m * D, a.proj + (int64_t)g * D * D, a.m,
-                                       a.att_scale, reinterpret_cast<T *>(a.summ) + (page * a.Hkv + g) * a.m * D, tid);
+        summarize_tile<DT, D>(sm, a.probes + (int64_t)g * a.m * D, a.proj + (int64_t)g * D * D, a.m, a.att_scale,
+                              reinterpret_cast<T *>(a.summ) + (page * a.Hkv + g) * a.m * D, tid);
     }
 }
 
@@ -1087,7 +1181,8 @@ extern "C" int hba_kv_append_ragged(int dtype, const void *k, const int64_t k_st
     a.summ = (char *)summ_pages;
     // c tokens touch at most c and at most c / 64 + 2 pages
     const int64_t slots = T < T / 64 + 2 * Bd ? T : T / 64 + 2 * Bd;
-    const dim3 grid((unsigned)slots, (unsigned)Hkv);
+    if ((slots + 7) / 8 * 8 * Hkv > 0x7fffffff) return HBA_ERR_UNSUPPORTED;
+    const dim3 grid((unsigned)((slots + 7) / 8 * 8 * Hkv));
 #define HBA_APPR(DT, D)                                                                                       \
     do {                                                                                                      \
         if (summ_pages)                                                                                       \
