@@ -11,9 +11,9 @@
 //
 //   decode_part    one token per sequence: memory-bound.  A wave takes a page of
 //                  one KV head in operand order straight into registers (its
-//                  heads are the 16 columns), the next one's loads in flight;
-//                  workgroups share a sequence's pages when there are few
-//                  sequences.
+//                  heads are the 16 columns), the next one's loads in flight.
+//                  Long sequences' pages are one list that the workgroups share
+//                  evenly (even_kernel).
 //   rows_part      128 rows (token, head) a workgroup over staged pages
 //                  (hba_rows.h): parts of prompts, and the shared pages for the
 //                  rows of the whole batch.
@@ -48,7 +48,9 @@ struct Args {
     int shared;                         // pages that all sequences begin with
     int slots, slot0, part;             // parts of a row: how many, the first of these, pages of one of them
     char *out;                          // [T, Hq, D]
-    float *po, *pml;                    // parts: [T, Hq, slots, D] sums, [T, Hq, slots, 2] maximum (log2 units) and sum
+    // parts: [T, Hq, slots, D] sums, [T, Hq, slots, 2] maximum (log2 units) and sum; of even shares (slots of
+    // them, part pages at least): [slots, 2, 16, D] and [slots, 2, 16, 2], see even_kernel
+    float *po, *pml;
 };
 
 // A row's position and what it sees of its sequence.
@@ -129,15 +131,17 @@ __device__ __forceinline__ Pages page_list(const Args &a, int L) {
     return p;
 }
 
-// group: (sequence, KV head, 16 of its heads); part: a run of a.part pages of its
-// list.  Units of UK keys: a page, or half of one where a page's operands would
-// fill the registers.  DW waves take the part's units in turn.
+// gi: 16 heads of a KV head of sequence s; pages p0 .. p1 - 1 of its list.  Head i of
+// the 16 writes part at + i step, or its row of the output (at < 0).
+// Units of UK keys: a page, or half of one where a page's operands would fill the
+// registers.  DW waves take the pages' units in turn.
 template <int DT, int D> constexpr int UNIT = DT == 1 && D == 64 ? 64 : 32;
 template <int D> struct DecodeLds {
     float o[4][16][D + 4], m[4][16], l[4][16];
 };
 template <int DT, int D, int DW>
-__device__ __forceinline__ void decode_part(const Args &a, DecodeLds<D> &lds, int group, int part) {
+__device__ __forceinline__ void decode_part(const Args &a, DecodeLds<D> &lds, int s, int gi, int p0, int p1,
+                                            int64_t at, int step) {
     typedef typename Op<DT>::F F;
     constexpr int ESZ = DT == 1 ? 2 : 4, UK = UNIT<DT, D>;
     constexpr int NKS = D / 32, NDT = D / 16, NH = UK / 32, UP = rows::PAGE / UK;
@@ -145,10 +149,10 @@ __device__ __forceinline__ void decode_part(const Args &a, DecodeLds<D> &lds, in
     const int lane = threadIdx.x & 63, l16 = lane & 15, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ct = (a.G + 15) / 16;
-    const int s = group / (a.Hkv * ct), g = group / ct % a.Hkv, c0 = group % ct * 16;
+    const int g = gi / ct, c0 = gi % ct * 16;
     const int L = length(a, s);
     const Pages pg = page_list(a, L);
-    const int u0 = part * a.part * UP, u1 = min(pg.n, (part + 1) * a.part) * UP;
+    const int u0 = p0 * UP, u1 = min(pg.n, p1) * UP;
     const int hl = c0 + l16, head = g * a.G + min(hl, a.G - 1);
     const char *kb = a.kr + (int64_t)g * rows::PAGE * D * ESZ, *vb = a.v + (int64_t)g * rows::PAGE * D * ESZ;
     const int64_t pstep = (int64_t)a.Hkv * rows::PAGE * D * ESZ;
@@ -177,7 +181,7 @@ __device__ __forceinline__ void decode_part(const Args &a, DecodeLds<D> &lds, in
             for (int h = 0; h < NH; ++h) x.v[dt][h] = Op<DT>::load(vp + ((dt * 2 + h0 + h) * 64 + lane) * 8 * ESZ);
     };
     int u = u0 + wave;
-    Unit xa, xb;
+    Unit xa;
     int64_t next = 0;   // the place of unit u + DW
     if (u < u1) {
         load(xa, u, place(u));
@@ -264,26 +268,28 @@ __device__ __forceinline__ void decode_part(const Args &a, DecodeLds<D> &lds, in
     };
     if constexpr (DT == 0 && D == 128) {   // two units would fill the registers
 #pragma unroll 1
-        while (u < u1) {
+        for (; u < u1; u += DW) {
             use(xa, u);
-            u += DW;
-            if (u < u1) load(xa, u, next);
-            if (u < u1) next = place(u + DW);
-        }
-    }
-#pragma unroll 1
-    for (; u < u1; u += 2 * DW) {
-        if (u + DW < u1) {
-            load(xb, u + DW, next);
+            if (u + DW >= u1) break;
+            load(xa, u + DW, next);
             next = place(u + 2 * DW);
         }
-        use(xa, u);
-        if (u + DW >= u1) break;
-        if (u + 2 * DW < u1) {
-            load(xa, u + 2 * DW, next);
-            next = place(u + 3 * DW);
+    } else {
+        Unit xb;
+#pragma unroll 1
+        for (; u < u1; u += 2 * DW) {
+            if (u + DW < u1) {
+                load(xb, u + DW, next);
+                next = place(u + 2 * DW);
+            }
+            use(xa, u);
+            if (u + DW >= u1) break;
+            if (u + 2 * DW < u1) {
+                load(xa, u + 2 * DW, next);
+                next = place(u + 3 * DW);
+            }
+            use(xb, u + DW);
         }
-        use(xb, u + DW);
     }
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
@@ -328,7 +334,7 @@ __device__ __forceinline__ void decode_part(const Args &a, DecodeLds<D> &lds, in
             o = o + *reinterpret_cast<const f32x4 *>(&lds.o[w][hc][e]) * f;
         }
         const int64_t row = (int64_t)s * a.Hq + g * a.G + c0 + hc;
-        if (a.slots == 1) {
+        if (at < 0) {
             // nothing seen: 0; keys whose scores are all -inf: NaN, as a softmax of them
             const f32x4 r = L > 0 ? o / ll : f32x4{0.f, 0.f, 0.f, 0.f};
             if constexpr (DT == 1)
@@ -337,20 +343,65 @@ __device__ __forceinline__ void decode_part(const Args &a, DecodeLds<D> &lds, in
             else
                 *reinterpret_cast<f32x4 *>(a.out + (row * D + e) * 4) = r;
         } else {
-            const int64_t at = row * a.slots + a.slot0 + part;
-            *reinterpret_cast<f32x4 *>(a.po + at * D + e) = o;
+            const int64_t to = at + (int64_t)hc * step;
+            *reinterpret_cast<f32x4 *>(a.po + to * D + e) = o;
             if (e == 0) {
-                a.pml[2 * at] = mm;
-                a.pml[2 * at + 1] = ll;
+                a.pml[2 * to] = mm;
+                a.pml[2 * to + 1] = ll;
             }
         }
     }
 }
 
 constexpr int DW = 8;   // waves of a decode workgroup
+// group: (sequence, KV head, 16 of its heads), part: a run of a.part pages.
+template <int DT, int D, int DW>
+__device__ __forceinline__ void decode_run(const Args &a, DecodeLds<D> &lds, int group, int part) {
+    const int ct = (a.G + 15) / 16, ng = a.Hkv * ct, s = group / ng, gi = group % ng;
+    const int64_t row = (int64_t)s * a.Hq + gi / ct * a.G + gi % ct * 16;
+    decode_part<DT, D, DW>(a, lds, s, gi, part * a.part, (part + 1) * a.part,
+                           a.slots == 1 ? -1 : row * a.slots + a.slot0 + part, a.slots);
+}
 template <int DT, int D> __global__ __launch_bounds__(64 * DW) void decode_kernel(const Args a) {
     __shared__ DecodeLds<D> lds;
-    decode_part<DT, D, DW>(a, lds, blockIdx.x, blockIdx.y);
+    decode_run<DT, D, DW>(a, lds, blockIdx.x, blockIdx.y);
+}
+
+// Even shares.  All pages of all groups (a group: 16 heads of a sequence) make one
+// list, in the order of sequences; workgroup w takes share w of it, whatever the
+// sequences' lengths.  A group inside one share is written at once; of the others
+// a share holds two at most, one that began before it (or with it) and one that
+// ends after it: parts 2 w and 2 w + 1.
+struct Shares {
+    int units, per;   // pages of all groups, of one share
+};
+__device__ __forceinline__ int list_pages(const Args &a, int s) { return max(1, page_list(a, length(a, s)).n); }
+__device__ __forceinline__ int groups_of(const Args &a) { return a.Hkv * ((a.G + 15) / 16); }
+template <int NT> __device__ __forceinline__ Shares shares(const Args &a) {
+    Shares x;
+    x.units = ragged::total<NT>(a.Bd, [&](int s) { return list_pages(a, s); }) * groups_of(a);
+    x.per = max(a.part, (x.units + a.slots - 1) / a.slots);
+    return x;
+}
+template <int DT, int D> __global__ __launch_bounds__(64 * DW) void even_kernel(const Args a) {
+    __shared__ DecodeLds<D> lds;
+    const Shares sh = shares<64 * DW>(a);
+    const int ng = groups_of(a), w = blockIdx.x;
+    const int64_t u0 = (int64_t)w * sh.per;
+    if (u0 >= sh.units) return;
+    int left = (int)min((int64_t)sh.per, sh.units - u0), at;
+    int s = ragged::find<64 * DW>((int)u0, a.Bd, [&](int i) { return list_pages(a, i) * ng; }, at);
+    for (int part = 2 * w; left > 0 && s < a.Bd; part = 2 * w + 1) {
+        const int n = list_pages(a, s), p0 = at % n, p1 = min(n, p0 + left);
+        decode_part<DT, D, DW>(a, lds, s, at / n, p0, p1, p1 - p0 == n ? -1 : (int64_t)part * 16, 1);
+        __syncthreads();   // lds is free again
+        left -= p1 - p0;
+        at += p1 - p0;
+        if (at == n * ng) {
+            at = 0;
+            ++s;
+        }
+    }
 }
 
 // -------------------------------------------------------------------- rows ----
@@ -490,35 +541,50 @@ __global__ __launch_bounds__(64 * rows::NW, (rows::WAVES<DT, D>)) void shared_ke
     if (i < nshared)
         rows_part<DT, D, true>(a, smem, i % ptiles, i / ptiles % a.Hkv, i / (ptiles * a.Hkv));
     else
-        decode_part<DT, D, rows::NW>(own, *reinterpret_cast<DecodeLds<D> *>(smem), (i - nshared) % groups,
-                                     (i - nshared) / groups);
+        decode_run<DT, D, rows::NW>(own, *reinterpret_cast<DecodeLds<D> *>(smem), (i - nshared) % groups,
+                                    (i - nshared) / groups);
 }
 
 // out = sum of the parts' O 2^(m - max) over sum of their l 2^(m - max); a row
 // without keys 0.  D / 4 threads a part, SG parts of a row at a time (all of a
 // workgroup where a row has many parts, one where rows are many), each with sums
-// of its own that LDS joins.
-template <int DT, int D, int SG> __global__ __launch_bounds__(256) void join_kernel(const Args a, int64_t nrows) {
+// of its own that LDS joins.  EVEN: the parts are those of even shares.
+template <int DT, int D, int SG, bool EVEN>
+__global__ __launch_bounds__(256) void join_kernel(const Args a, int64_t nrows) {
     constexpr int TP = D / 4, RB = 256 / (TP * SG);   // threads of a part, rows of a workgroup
     __shared__ float so[SG > 1 ? SG : 1][SG > 1 ? D : 1];
     __shared__ float sm[SG], sl[SG];
     const int x = threadIdx.x % TP * 4, sg = threadIdx.x / TP % SG;
     const int64_t row = (int64_t)blockIdx.x * RB + threadIdx.x / (TP * SG);
     if (row >= nrows) return;                         // SG > 1: the workgroup's one row
-    const float *ml = a.pml + row * a.slots * 2, *po = a.po + row * a.slots * D + x;
+    int slots = a.slots, step = 1;                    // part p at first + p step, the row's first part at part0
+    int64_t first_part = row * a.slots, part0 = first_part;
+    if constexpr (EVEN) {
+        static_assert(RB == 1, "the scans are a workgroup's");
+        const Shares sh = shares<256>(a);
+        const int s = (int)(row / a.Hq), h = (int)(row % a.Hq), ct = (a.G + 15) / 16, n = list_pages(a, s);
+        const int before = ragged::total<256>(s, [&](int i) { return list_pages(a, i); }) * groups_of(a);
+        const int u = before + (h / a.G * ct + h % a.G / 16) * n, w0 = u / sh.per, w1 = (u + n - 1) / sh.per;
+        if (w0 == w1) return;                         // written already
+        slots = w1 - w0 + 1;
+        step = 32;
+        first_part = (int64_t)w0 * 32 + h % a.G % 16;
+        part0 = first_part + (w0 * sh.per < u ? 16 : 0);
+    }
+    const auto place = [&](int p) { return p ? first_part + (int64_t)p * step : part0; };
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.0f;
-    for (int i = sg; i < a.slots; i += 4 * SG) {      // four parts at a time
+    for (int i = sg; i < slots; i += 4 * SG) {      // four parts at a time
         float pm[4], pl[4];
         f32x4 px[4];
         float mn = m;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int p = min(i + e * SG, a.slots - 1);
-            const bool in = i + e * SG < a.slots;
-            pm[e] = in ? ml[2 * p] : -INFINITY;
-            pl[e] = in ? ml[2 * p + 1] : 0.0f;
-            px[e] = *reinterpret_cast<const f32x4 *>(po + (int64_t)p * D);
+            const int64_t p = place(min(i + e * SG, slots - 1));
+            const bool in = i + e * SG < slots;
+            pm[e] = in ? a.pml[2 * p] : -INFINITY;
+            pl[e] = in ? a.pml[2 * p + 1] : 0.0f;
+            px[e] = *reinterpret_cast<const f32x4 *>(a.po + p * D + x);
             mn = fmaxf(mn, pm[e]);
         }
         const float al = m == -INFINITY ? 0.0f : ex2(m - mn);
@@ -568,24 +634,21 @@ template <int DT, int D, int SG> __global__ __launch_bounds__(256) void join_ker
 
 // ------------------------------------------------------------------- plan ----
 // How the rows' keys are cut into parts: runs of pages, so that long sequences have
-// more of them than short ones.
+// more of them than short ones, or even shares of everything.
 struct Plan {
     int prefix, own;              // parts over the shared pages, and over each sequence's own, at most
     int prefix_pages, own_pages;  // pages of one
+    int shares;                   // even shares (0: parts), of own_pages at least
     int64_t tiles, ptiles;        // 128-row tiles: of the ragged batch (at most), of all tokens
     int slots() const { return prefix + own; }
 };
-#ifndef AIMR
-#define AIMR 1024
-#endif
-#ifndef AIMP
-#define AIMP 512
-#endif
-#ifndef MINP
-#define MINP 4
-#endif
-static int parts_of(int64_t pages, int64_t parts, int64_t least, int &per) {
-    if (parts > pages / least) parts = pages / least;
+// `base` workgroups a part: parts of one page while they find CUs of their own, then
+// of `least` pages as long as there are no more than `most` workgroups.
+constexpr int CUS = 256;
+static int parts_of(int64_t pages, int64_t base, int64_t most, int64_t least, int &per) {
+    int64_t parts = most / base < pages / least ? most / base : pages / least;
+    if (parts < CUS / base) parts = CUS / base;
+    if (parts > pages) parts = pages;
     if (parts < 1) parts = 1;
     per = (int)((pages + parts - 1) / parts);
     return (int)((pages + per - 1) / per);
@@ -602,16 +665,31 @@ static Plan plan(int64_t T, int64_t Bd, int64_t Hq, int64_t Hkv, int64_t W, int6
     const int64_t all = (max_len + KT - 1) / KT;
     if (pages > all) pages = all > 0 ? all : 1;
     p.ptiles = (T * G + rows::RT - 1) / rows::RT;
-    if (one) {
-        const int64_t groups = Bd * Hkv * ((G + 15) / 16);
-        // some 1024 workgroups of 8 waves; but up to 32 pages, 4 a wave, need no join
-        p.own = parts_of(pages, (1024 + groups - 1) / groups, shared ? 4 : pages <= 32 ? 32 : 8, p.own_pages);
-    } else {
+    const int64_t groups = Bd * Hkv * ((G + 15) / 16);
+    if (!one) {
         p.tiles = p.ptiles + Bd;
-        p.own = parts_of(pages, AIMR / (p.ptiles * Hkv), 8, p.own_pages);
+        // 4 sequences, 1560 tokens, 9000 keys, d = 64: 72 us at 1024 workgroups, 110 at 512, 77 at 1536
+        p.own = parts_of(pages, p.ptiles * Hkv, 1024, 8, p.own_pages);
+    } else if (shared) {
+        p.own = parts_of(pages, groups, 1024, 4, p.own_pages);
+    } else if (pages > 32 && groups < 1024 && groups * pages < (1 << 30)) {
+        // Up to 32 pages are 4 a wave and need no join; from 1024 groups on, the card's
+        // workgroups even out by themselves.  24 sequences of 4000 to 32000 keys, 4 KV
+        // heads, d = 128: 155 us (5.8 TB/s), and 188 in runs of pages, 11 a sequence.
+        p.shares = (int)(groups * pages / 8 < CUS ? groups * pages / 8 + 1 : CUS);
+        p.own = 1;
+        p.own_pages = 8;
+    } else {
+        p.own = 1;
+        p.own_pages = (int)pages;
     }
-    if (shared) p.prefix = parts_of(shared, AIMP / (p.ptiles * Hkv), MINP, p.prefix_pages);
+    // 64 sequences' 8192 shared keys, d = 64: 14.5 us at 256 workgroups, 20 at 512, 17.5 at 128
+    if (shared) p.prefix = parts_of(shared, p.ptiles * Hkv, CUS, 1, p.prefix_pages);
     return p;
+}
+static size_t workspace(const Plan &p, int64_t T, int64_t Hq, int64_t d) {
+    const int64_t parts = p.shares ? (int64_t)p.shares * 32 : p.slots() > 1 ? T * Hq * p.slots() : 0;
+    return (size_t)parts * (d + 2) * 4;
 }
 
 template <int DT, int D> static int launch(Args a, const Plan &p, hipStream_t s) {
@@ -619,6 +697,16 @@ template <int DT, int D> static int launch(Args a, const Plan &p, hipStream_t s)
     static_assert(sizeof(DecodeLds<D>) <= 65536 && lds <= 65536, "LDS without an attribute");
     const int64_t groups = (int64_t)a.Bd * a.Hkv * ((a.G + 15) / 16);
     a.slots = p.slots();
+    if (p.shares) {
+        a.slots = p.shares;
+        a.part = p.own_pages;
+        const int64_t nrows = (int64_t)a.T * a.Hq;
+        hipLaunchKernelGGL((even_kernel<DT, D>), dim3((unsigned)p.shares), dim3(64 * DW), 0, s, a);
+        HBA_LAUNCH_CHECK();
+        hipLaunchKernelGGL((join_kernel<DT, D, 1024 / D, true>), dim3((unsigned)nrows), dim3(256), 0, s, a, nrows);
+        HBA_LAUNCH_CHECK();
+        return HBA_OK;
+    }
     Args own = a;
     own.slot0 = p.prefix;
     own.part = p.own_pages;
@@ -647,9 +735,9 @@ template <int DT, int D> static int launch(Args a, const Plan &p, hipStream_t s)
         const int64_t nrows = (int64_t)a.T * a.Hq;
         constexpr int SG = 1024 / D, RB = 1024 / D;   // parts at a time, or rows
         if (a.slots > 8)
-            hipLaunchKernelGGL((join_kernel<DT, D, SG>), dim3((unsigned)nrows), dim3(256), 0, s, a, nrows);
+            hipLaunchKernelGGL((join_kernel<DT, D, SG, false>), dim3((unsigned)nrows), dim3(256), 0, s, a, nrows);
         else
-            hipLaunchKernelGGL((join_kernel<DT, D, 1>), dim3((unsigned)((nrows + RB - 1) / RB)), dim3(256), 0, s, a,
+            hipLaunchKernelGGL((join_kernel<DT, D, 1, false>), dim3((unsigned)((nrows + RB - 1) / RB)), dim3(256), 0, s, a,
                                nrows);
         HBA_LAUNCH_CHECK();
     }
@@ -681,7 +769,7 @@ extern "C" int hba_paged_attn_workspace_bytes(int64_t T, int64_t Bd, int64_t Hq,
     if (!bytes) return HBA_ERR_INVALID_ARG;
     if (int st = paged::check(T, Bd, Hq, Hkv, d, W, S, shared_pages, one_each, max_len, 1 << 24)) return st;
     const paged::Plan p = paged::plan(T, Bd, Hq, Hkv, W, S, shared_pages, one_each != 0, max_len);
-    *bytes = p.slots() > 1 ? (size_t)(T * Hq) * p.slots() * (d + 2) * 4 : 0;
+    *bytes = paged::workspace(p, T, Hq, d);
     return HBA_OK;
 }
 
@@ -703,7 +791,7 @@ extern "C" int hba_paged_attn(int dtype, const void *q, const int64_t q_strides[
         !abi::aligned16(v_pages) || !abi::aligned16(out))
         return HBA_ERR_UNSUPPORTED;
     const paged::Plan p = paged::plan(T, Bd, Hq, Hkv, W, S, shared_pages, cu == nullptr, max_len);
-    const size_t need = p.slots() > 1 ? (size_t)(T * Hq) * p.slots() * (d + 2) * 4 : 0;
+    const size_t need = paged::workspace(p, T, Hq, d);
     if (need && (!workspace || ws_bytes < need)) return HBA_ERR_INVALID_ARG;
     if (need && !abi::aligned16(workspace)) return HBA_ERR_UNSUPPORTED;
     paged::Args a = {};
@@ -734,7 +822,7 @@ extern "C" int hba_paged_attn(int dtype, const void *q, const int64_t q_strides[
     a.shared = (int)shared_pages;
     a.out = (char *)out;
     a.po = (float *)workspace;
-    a.pml = need ? (float *)workspace + T * Hq * p.slots() * d : nullptr;
+    a.pml = need ? (float *)workspace + need / 4 / (d + 2) * d : nullptr;
     int st = HBA_OK;
 #define HBA_PAGED(DT, D) st = paged::launch<DT, D>(a, p, (hipStream_t)stream)
     HBA_DISPATCH_DT_D(dtype, d, HBA_PAGED);

@@ -15,13 +15,13 @@ __device__ __forceinline__ int tokens(const int32_t *cu, int s, int T, int &firs
 }
 
 // The sequence and the place in it of workgroup `slot`, where sequence s has
-// count(s) workgroups; -1 past the last.  Every thread of a workgroup of 256
-// calls it: thread i counts the i-th of 256 runs of sequences, a scan over the
+// count(s) workgroups; -1 past the last.  Every thread of a workgroup of NT
+// calls it: thread i counts the i-th of NT runs of sequences, a scan over the
 // threads finds the run, and its thread walks it.
-template <class F> __device__ __forceinline__ int find(int slot, int Bd, const F &count, int &place) {
-    __shared__ int wsum[4], found[2];
+template <int NT = 256, class F> __device__ __forceinline__ int find(int slot, int Bd, const F &count, int &place) {
+    __shared__ int wsum[NT / 64], found[2];
     const int tid = threadIdx.x, lane = tid & 63;
-    const int per = (Bd + 255) / 256, s0 = min(tid * per, Bd), s1 = min(s0 + per, Bd);
+    const int per = (Bd + NT - 1) / NT, s0 = min(tid * per, Bd), s1 = min(s0 + per, Bd);
     int mine = 0;
     for (int s = s0; s < s1; ++s) mine += count(s);
     int upto = mine;
@@ -48,6 +48,22 @@ template <class F> __device__ __forceinline__ int find(int slot, int Bd, const F
     __syncthreads();
     place = found[1];
     return __builtin_amdgcn_readfirstlane(found[0]);
+}
+
+// The sum of count(s) over sequences 0 .. n - 1, by a workgroup of NT threads.
+template <int NT, class F> __device__ __forceinline__ int total(int n, const F &count) {
+    __shared__ int wsum[NT / 64];
+    int mine = 0;
+    for (int s = threadIdx.x; s < n; s += NT) mine += count(s);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) mine += __shfl_xor(mine, o, 64);
+    __syncthreads();   // an earlier call's sums are read
+    if (threadIdx.x % 64 == 0) wsum[threadIdx.x / 64] = mine;
+    __syncthreads();
+    mine = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) mine += wsum[w];
+    return __builtin_amdgcn_readfirstlane(mine);
 }
 
 // The sequence of token t (the last s with cu[s] <= t).

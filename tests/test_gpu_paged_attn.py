@@ -91,6 +91,23 @@ def test_decode(lens, W, S, dt, d):
     check(setup(DT[dt], d, 4, 2, lens, seed=len(lens)), W, S)
 
 
+@pytest.mark.parametrize("dt,d", [("f32", 64), ("f32", 128), ("bf16", 64), ("bf16", 128)])
+@pytest.mark.parametrize("W,S", [(0, 0), (2100, 0), (2200, 70)])
+@pytest.mark.parametrize("lens,Hq,Hkv", [([2049], 2, 1), ([0, 4000, 1, 63, 2600], 6, 2), ([0, 0, 2200, 0], 17, 1),
+                                         ([2100] * 9, 3, 3)])
+def test_long_sequences_in_even_shares(lens, Hq, Hkv, W, S, dt, d):
+    """More than 32 pages: all sequences' pages are cut evenly, shares begin and end inside sequences."""
+    check(setup(DT[dt], d, Hq, Hkv, lens, seed=len(lens)), W, S)
+
+
+@pytest.mark.parametrize("bd", [300, 1100])
+def test_many_sequences_under_a_long_bound(bd):
+    """More sequences than the scan has threads for a run each; the bound is far above every length."""
+    s = setup(torch.bfloat16, 64, 2, 1, [(37 * i) % 130 for i in range(bd)], seed=3)
+    s["cos"], s["sin"] = hba_amd.rope_tables(4000, 64, 1e4, "cpu")
+    check({**s, "table": torch.cat([s["table"], torch.zeros(bd, 60, dtype=torch.int32)], 1), "max_len": 4000})
+
+
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
 @pytest.mark.parametrize("Hq,Hkv", [(1, 1), (7, 1), (14, 2), (16, 1), (17, 1), (40, 2), (6, 6)])
 def test_groups(Hq, Hkv, dt):
