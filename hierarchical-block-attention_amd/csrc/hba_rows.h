@@ -48,6 +48,10 @@ constexpr float MOST = 65536.0f;  // sum of a tile's probabilities that calls fo
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 
+// The thread's place among the NW waves of its rows (a workgroup may have two such
+// sets, for halves of the keys).
+__device__ __forceinline__ int thread() { return threadIdx.x % (64 * NW); }
+
 // The value of lane l ^ 32.
 __device__ __forceinline__ float other_half(float v) {
     const uint32_t x = __float_as_uint(v);
@@ -175,21 +179,21 @@ template <int DT, int D> struct Tile {
     }
     // The thread's first chunk of a staging pass, as an offset from the first row.
     static __device__ __forceinline__ uint32_t offset(int64_t bytes) {
-        const int r = threadIdx.x / NCH;
-        return (uint32_t)(r * (int)bytes) + ((threadIdx.x % NCH) ^ swz(r)) * 16;
+        const int r = thread() / NCH;
+        return (uint32_t)(r * (int)bytes) + ((thread() % NCH) ^ swz(r)) * 16;
     }
     // Stage rows j0 .. j0 + R - 1 of a strided array (`bytes` from row to row, off =
     // offset(bytes)); rows past `last` read row `last`.  Called by all NW waves.
     template <int R>
     static __device__ __forceinline__ void stage(const char *base, int64_t bytes, uint32_t off, int j0, int last,
                                                  uint32_t lds) {
-        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int wave = __builtin_amdgcn_readfirstlane(thread() >> 6);
         if (j0 + R - 1 <= last) {
             const char *p = base + j0 * bytes;
 #pragma unroll
             for (int i = 0; i < R / RPI; ++i) dma16s(p + i * RPI * bytes, off, lds + (i * NW + wave) * 1024);
         } else {
-            const int r = threadIdx.x / NCH, c = (threadIdx.x % NCH) ^ swz(r);
+            const int r = thread() / NCH, c = (thread() % NCH) ^ swz(r);
 #pragma unroll
             for (int i = 0; i < R / RPI; ++i)
                 dma16(base + (int64_t)min(j0 + r + i * RPI, last) * bytes + c * 16, lds + (i * NW + wave) * 1024);

@@ -58,7 +58,7 @@ template <int D> __device__ __forceinline__ bool find_rows(const Args &a, Rows &
     x.g = combo % a.Hkv;
     x.len = seq_len(a, x.b);
     const int nr = a.n * a.G, vr = x.len * a.G;          // rows there are, rows of the sequence
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(rows::thread() >> 6);
     const int r0 = tile * RT, rw = r0 + wave * RW, r = rw + (threadIdx.x & 31);
     x.in = r < nr;
     x.valid = r < vr;
@@ -136,6 +136,58 @@ __global__ __launch_bounds__(64 * NW, (DT == 1 && D == 64 ? 3 : WAVES<DT, D>)) v
     load_rows<DT, D>(q_row<DT, D>(a, x), x.valid, q);
     RowAcc<DT, D> acc;
     attend<DT, D, false>(src, smem, q, nullptr, a.c, 0, nt, ns, wt0, x.w, acc);
+    float l = acc.l + other_half(acc.l);
+    if (__ballot(x.valid && (any_bad<D>(acc.O) || !finite(l)))) {
+        attend_each<DT, D, false>(src, q, nullptr, a.c, 0, nt, ns, wt0, x.w, acc);
+        l = acc.l + other_half(acc.l);
+    }
+    store_fwd<DT, D>(a, x, acc, l);
+}
+
+// swa_fwd where its workgroups leave CUs free: two sets of waves have the same rows,
+// each half of the tiles, and meet in LDS.  1001 tokens, 14 heads, d = 64, W = 1024
+// (110 workgroups): 17 us against 20; 28 heads, d = 128 (220) 26 against 31; fp32,
+// d = 64, whose matrix products bound it, 72 against 75.
+template <int DT, int D> constexpr size_t halves_lds() {
+    constexpr size_t tiles = 4 * DenseKV<DT, D>::BYTES, sums = (size_t)64 * NW * (D / 2 + 2) * 4;
+    return tiles > sums ? tiles : sums;
+}
+template <int DT, int D> __global__ __launch_bounds__(2 * 64 * NW) void swa_fwd_halves(const Args a) {
+    extern __shared__ __align__(16) char smem[];
+    Rows x;
+    if (!find_rows<D>(a, x)) return;
+    const int half = __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * NW));
+    DenseKV<DT, D> src = keys<DT, D>(a, x);
+    int ns, wt0;
+    const int nt = tile_list<KEYS<DT, D>>(x.lo, x.hi, a.S, ns, wt0), mid = (nt + 1) / 2;
+    const int it0 = half ? mid : 0, it1 = half ? nt : mid;
+    char *mine = smem + half * 2 * DenseKV<DT, D>::BYTES;
+    attend_begin(src, mine, it0, it1, ns, wt0);
+    typename Op<DT>::F q[D / 16];
+    load_rows<DT, D>(q_row<DT, D>(a, x), x.valid, q);
+    RowAcc<DT, D> acc;
+    attend<DT, D, false>(src, mine, q, nullptr, a.c, it0, it1, ns, wt0, x.w, acc);
+    if (it1 - it0 < mid) __syncthreads();   // the other half's last tile: as many barriers for both
+    float *sums = reinterpret_cast<float *>(smem) + rows::thread();
+    constexpr int T = 64 * NW;
+    if (half) {
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sums[(16 * dt + r) * T] = acc.O[dt][r];
+        sums[D / 2 * T] = acc.m;
+        sums[(D / 2 + 1) * T] = acc.l;
+    }
+    __syncthreads();
+    if (half) return;
+    const float om = sums[D / 2 * T], m = fmaxf(acc.m, om);
+    const float fa = acc.m == -INFINITY ? 0.0f : ex2(acc.m - m), fb = om == -INFINITY ? 0.0f : ex2(om - m);
+    acc.m = m;
+    acc.l = fmaf(sums[(D / 2 + 1) * T], fb, acc.l * fa);
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc.O[dt][r] = fmaf(sums[(16 * dt + r) * T], fb, acc.O[dt][r] * fa);
     float l = acc.l + other_half(acc.l);
     if (__ballot(x.valid && (any_bad<D>(acc.O) || !finite(l)))) {
         attend_each<DT, D, false>(src, q, nullptr, a.c, 0, nt, ns, wt0, x.w, acc);
@@ -573,6 +625,17 @@ template <int DT, int D, class K> static int lds_room(K kern, size_t bytes) {
 
 template <int DT, int D> static int launch_fwd(const Args &a, int64_t grid, hipStream_t s) {
     constexpr size_t lds = 2 * DenseKV<DT, D>::BYTES;
+    if constexpr (WAVES<DT, D> >= 2) {   // 8 waves on a CU
+        // the meeting costs what some 200 keys do: 300 tokens, d = 64, W = 128 takes 8.7 us either way, d = 128 12.2
+        // in one set and 12.4 in two; W = 256 9.7 and 9.4, 14.0 and 13.6
+        if (grid <= 256 && (a.W < a.n ? a.W : a.n) >= 256) {
+            if (int st = lds_room<DT, D>(swa_fwd_halves<DT, D>, halves_lds<DT, D>())) return st;
+            hipLaunchKernelGGL((swa_fwd_halves<DT, D>), dim3((unsigned)grid), dim3(2 * 64 * NW),
+                               (halves_lds<DT, D>()), s, a);
+            HBA_LAUNCH_CHECK();
+            return HBA_OK;
+        }
+    }
     if (int st = lds_room<DT, D>(swa_fwd<DT, D>, lds)) return st;
     hipLaunchKernelGGL((swa_fwd<DT, D>), dim3((unsigned)grid), dim3(64 * NW), lds, s, a);
     HBA_LAUNCH_CHECK();

@@ -54,6 +54,36 @@ def test_forward_and_gradients(n, W, S, dt, d):
     compare(run(q, k, v, W, S, dout=do), q, k, v, W, S, None, None, do)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("n,W,S", [(255, 255, 0), (256, 256, 0), (320, 256, 70), (700, 600, 3), (961, 2000, 0)])
+@pytest.mark.parametrize("lens", [None, [0, 255], [100, 64]])
+def test_few_rows_and_many_keys(n, W, S, lens, dt, d):
+    """Two sets of waves share the keys: odd and even tile counts, and workgroups without any."""
+    q, k, v, _ = make(DT[dt], 2, n, 3, 1, d, seed=n)
+    x = [t.clone() for t in (q, k, v)]
+    for b, m in enumerate(lens or []):
+        for t in x:
+            t[b, m:] = float("nan")
+    compare(run(*x, W, S, lens=lens), q, k, v, W, S, None, lens)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_few_rows_spoiled(bad, dt):
+    """A non-finite key or value spoils the rows that see it, whichever set of waves has it."""
+    for at in (5, 300, 590):
+        q, k, v, _ = make(DT[dt], 1, 600, 2, 1, 64, seed=at)
+        want, bound = sliding(q, k, v, 300, 2, 64 ** -0.5, None, unit(q.dtype))
+        k2, v2 = k.clone(), v.clone()
+        k2[0, at], v2[0, at] = bad, bad
+        got = run(q, k2, v2, 300, 2).cpu()
+        sees = torch.arange(600)
+        sees = (sees >= at) & (sees < at + 300)
+        assert not got[0, sees].isfinite().any()
+        assert_within(got[:, ~sees], want[:, ~sees], bound[:, ~sees], "out")
+
+
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
 @pytest.mark.parametrize("Hq,Hkv", [(1, 1), (3, 3), (14, 2), (8, 1), (33, 1), (6, 2)])
 def test_groups(Hq, Hkv, dt):
