@@ -405,6 +405,18 @@ template <int DT, int D> __global__ __launch_bounds__(64 * DW) void even_kernel(
 }
 
 // -------------------------------------------------------------------- rows ----
+// The rows, of KV head g, of tokens before cu[0] or behind cu[Bd]: 0, by workgroups
+// left over (there are some: no batch fills its last Bd tiles).
+template <int DT, int D> __device__ __forceinline__ void zero_strays(const Args &a, int g, int w, int of) {
+    constexpr int V = DT == 1 ? 8 : 4;   // elements of 16 bytes
+    const int lo = max(0, min(a.T, a.cu[0])), hi = max(lo, min(a.T, a.cu[a.Bd]));
+    const int64_t n = (int64_t)(lo + a.T - hi) * a.G * (D / V), step = (int64_t)of * (64 * rows::NW);
+    for (int64_t i = (int64_t)w * (64 * rows::NW) + threadIdx.x; i < n; i += step) {
+        const int64_t k = i / (D / V) / a.G, t = k < lo ? k : k - lo + hi, head = g * a.G + i / (D / V) % a.G;
+        *reinterpret_cast<uint4 *>(a.out + ((t * a.Hq + head) * D + i % (D / V) * V) * (16 / V)) = uint4{0, 0, 0, 0};
+    }
+}
+
 // SHARED: the rows of all tokens over the shared pages (x: 128-row tile); else the
 // rows of one sequence's tokens over its own pages (x: tile of the ragged batch).
 // g: KV head, z: part, a run of a.part pages.
@@ -426,11 +438,18 @@ __device__ __forceinline__ void rows_part(const Args &a, char *smem, int x, int 
         it1 = min(a.shared * TP, it0 + a.part * TP);
         rows::attend_begin(src, smem, it0, it1, 0, 0);
     } else {
-        s = ragged::find(x, a.Bd, [&](int i) {
+        const auto tiles = [&](int i) {
             int f;
             return (ragged::tokens(a.cu, i, a.T, f) * a.G + rows::RT - 1) / rows::RT;
-        }, tile);
-        if (s < 0) return;
+        };
+        s = ragged::find(x, a.Bd, tiles, tile);
+        if (s < 0) {
+            if (a.slots == 1) {   // else the join does it
+                const int used = ragged::total<64 * rows::NW>(a.Bd, tiles);
+                zero_strays<DT, D>(a, g, x - used, gridDim.x - used);
+            }
+            return;
+        }
         cnt = ragged::tokens(a.cu, s, a.T, first);
         src.table = a.table + (int64_t)s * a.maxp;
     }
@@ -620,11 +639,12 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a, int64_t nrows) 
             o = o + *reinterpret_cast<const f32x4 *>(&so[i][x]) * f;
         }
     }
-    // what the row sees: nothing gives 0, scores that are all -inf NaN
+    // what the row sees: nothing, or a token of no sequence, gives 0, scores that are all -inf NaN
     const int t = (int)(row / a.Hq), s = a.cu ? ragged::sequence(a.cu, a.Bd, t) : t;
     int first = t, cnt = 1;
     if (a.cu) cnt = ragged::tokens(a.cu, s, a.T, first);
-    const f32x4 r = length(a, s) - cnt + t - first >= 0 ? o / l : f32x4{0.f, 0.f, 0.f, 0.f};
+    const bool sees = t >= first && t - first < cnt && length(a, s) - cnt + t - first >= 0;
+    const f32x4 r = sees ? o / l : f32x4{0.f, 0.f, 0.f, 0.f};
     char *to = a.out + (row * D + x) * (DT == 1 ? 2 : 4);
     if constexpr (DT == 1)
         *reinterpret_cast<uint2 *>(to) = make_uint2(pk_bf16(r[0], r[1]), pk_bf16(r[2], r[3]));

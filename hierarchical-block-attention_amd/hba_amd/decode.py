@@ -212,6 +212,7 @@ class PagedKVCache:
         """Begin the empty sequences dsts with the first `tokens` tokens of
         sequence src (whole pages): the same pages, their summaries included,
         without a copy.  Appends go to pages of each sequence's own."""
+        dsts = list(dsts)
         if tokens < 0 or tokens % PAGE or tokens > self.lens[src]:
             raise ValueError(f"share: whole pages of {PAGE} tokens that sequence {src} holds; got {tokens}")
         if any(s == src or self.lens[s] or self._table[s] for s in dsts) or len(set(dsts)) != len(dsts):
@@ -291,7 +292,9 @@ def cache_attention(q, cache, cfg, qkn, cos, sin, window=None, sinks=0, cu=None,
     kernel, as hba_decode_step).  One token per sequence, or with cu (extend's
     result) several.  window None: every key; else the last `window` keys and
     the first `sinks`.  shared: tokens whose pages every sequence shares
-    (PagedKVCache.share), read once for the batch.  Returns [T, Hq, d]."""
+    (PagedKVCache.share), read once for the batch.  max_len bounds the lengths
+    (default: the longest one now, so a captured call that is to serve longer
+    ones gives it).  Returns [T, Hq, d]."""
     qg = qkn.q.gain if getattr(cfg, "qknorm", False) else None
     qeps = float(qkn.q.eps) if qg is not None else 1e-6
     if window is not None and window < 1:

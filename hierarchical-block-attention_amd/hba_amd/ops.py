@@ -939,8 +939,9 @@ def kv_append_ragged(k, v, cu, k_gain, eps, cos, sin, page_table, seq_lens, kc_p
     and summ_pages (with probes and proj) may be None: a cache without the
     unrotated keys or the summaries.  cu int32 [Bd + 1], page_table int32 [Bd,
     max_pages], seq_lens int32 [Bd] on the device; cos/sin fp32 [n_tab, d].
-    Positions past the page table or the cos/sin tables are not appended; a
-    page belongs to one sequence while tokens are appended to it."""
+    Positions past the page table or the cos/sin tables, and tokens behind
+    cu[Bd] (a padded batch), are not appended; a page belongs to one sequence
+    while tokens are appended to it."""
     if torch.compiler.is_compiling():
         return torch.ops.hba.kv_append_ragged(k, v, cu, k_gain, eps, cos, sin, page_table, seq_lens, kc_pages,
                                               kr_pages, v_pages, probes, proj, summ_pages)
@@ -1004,7 +1005,7 @@ def paged_attn(q, q_gain, eps, kr_pages, v_pages, page_table, seq_lens, cos, sin
     `shared` tokens (whole pages) are the same pages in every sequence; they
     are read through page_table[0], once for the batch.  max_len bounds every
     seq_lens[s] (a longer one is read as max_len).  Returns [T, Hq, d]; a
-    token that sees nothing gives 0."""
+    token that sees nothing, or is behind cu[Bd] (a padded batch), gives 0."""
     if torch.compiler.is_compiling():
         return torch.ops.hba.paged_attn(q, q_gain, eps, kr_pages, v_pages, page_table, seq_lens, cos, sin, scales,
                                         max_len, window, sinks, cu, shared)

@@ -501,9 +501,9 @@ int hba_attn_bwd_workspace_size(int64_t B, int64_t n, int64_t Hq, int64_t d, siz
  * bits of hba_kv_append and hba_summarize_pages; a bf16 kr is rounded once, from
  * the fp32 normalised key (hba_kv_append's after every step).  Everything else
  * in the pages stays as it is.  kc_pages and summ_pages may be NULL (summ_pages
- * needs kc_pages, probes and proj).  cu int32 [Bd+1] rises from 0 to T; tokens
- * at positions < 0, past the page table, at/after n_tab, or on a page outside
- * 0 .. num_pages-1 are not appended.  A page is appended to by one sequence.
+ * needs kc_pages, probes and proj).  cu int32 [Bd+1] rises from 0 to at most T;
+ * tokens behind cu[Bd] (a padded batch), at positions < 0, past the page table,
+ * at/after n_tab, or on a page outside 0 .. num_pages-1 are not appended.  A page is appended to by one sequence.
  * The call changes no length, so repeating it gives the same cache.  No
  * counterpart in the reference, which has no KV cache.
  */
@@ -531,7 +531,7 @@ int hba_kv_append_ragged(int dtype, const void *k, const int64_t k_strides[2], c
  * batch, and joined with each sequence's own by their log-sum-exps.  max_len
  * bounds every seq_lens[s] (a longer one is read as max_len).  A page id outside
  * 0 .. num_pages-1 is clamped into it.  out [T, Hq, d] contiguous; a token that
- * sees nothing (position < 0) gives 0.  Whatever lies in the pages at or past a
+ * sees nothing (position < 0) or is behind cu[Bd] (a padded batch) gives 0.  Whatever lies in the pages at or past a
  * sequence's length has no effect.  bf16: logits from queries of two bf16 parts
  * (16 bits of mantissa), probabilities rounded to bf16, sums in fp32.
  * workspace: 16-byte aligned, no initial contents, at least

@@ -164,6 +164,18 @@ def test_places_that_are_not_there():
     assert all(torch.equal(bits(c2[n]), bits(want[n])) for n in c2)
 
 
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_padded_batch(dt):
+    """Tokens behind the last sequence go nowhere."""
+    s = setup(dt, 64, 2, [10, 60], [50, 5])
+    want = {n: s[n].clone() for n in ("kc", "kr", "vp", "summ")}
+    append(s, **want)
+    got = {n: s[n].clone() for n in want}
+    pad = torch.full((77, *s["k"].shape[1:]), float("nan"), dtype=dt, device="cuda")
+    append(s, k=torch.cat([s["k"], pad]), v=torch.cat([s["v"], pad]), **got)
+    assert all(torch.equal(bits(got[n]), bits(want[n])) for n in got)
+
+
 def test_graph_replays():
     old, new = [50, 3], [90, 61]
     s = setup(torch.bfloat16, 64, 2, old, new)

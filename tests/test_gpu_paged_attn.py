@@ -139,6 +139,22 @@ def test_shared_prefix_with_parts(dt):
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("shared,lens,new", [(0, [40, 20], [30, 1]), (0, [900, 700], [60, 65]), (0, [5, 0], [0, 0]),
+                                             (64, [200, 130], [9, 66])])
+def test_padded_batch(shared, lens, new, dt):
+    """Tokens behind the last sequence give 0, whatever they hold."""
+    s = setup(DT[dt], 64, 6, 2, lens, new, shared=shared, seed=3)
+    T = sum(new)
+    s["q"] = torch.cat([s["q"], torch.full((300, 6, 64), float("nan"), dtype=DT[dt])])
+    torch.full((T + 300, 6, 64), float("nan"), dtype=DT[dt], device="cuda")   # the output's memory, perhaps
+    got = call(s)
+    assert not got[T:].any() and got.shape[0] == T + 300
+    if T:
+        want, bound = expect({**s, "q": s["q"][:T]})
+        assert_within(got[:T], want, bound, "out")
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
 @pytest.mark.parametrize("new", [None, [3, 60]])
 def test_no_norm_no_rotation_and_sharp_logits(new, dt):
     s = setup(DT[dt], 64, 4, 2, [200, 90], new, gain=False)
