@@ -659,7 +659,7 @@ template <int DT, int D> static int launch_bwd(Args a, int64_t grid, const Cut &
 }
 
 // Rows whose strides the kernels' 32-bit offsets within a tile can span.
-static bool rows_near(const int64_t *st, int64_t esz) { return st[1] * esz < (1 << 24); }
+static bool rows_near(const int64_t *st, int64_t esz) { return st[1] >= 0 && st[1] * esz < (1 << 24); }
 
 static void set_strides(int64_t (&to)[3], const int64_t *from, int64_t esz) {
     for (int i = 0; i < 3; ++i) to[i] = from[i] * esz;
@@ -790,7 +790,9 @@ extern "C" int hba_swa_bwd(int dtype, const void *q, const int64_t q_strides[3],
     a.Ps = c.Ps;
     a.Pn = c.Pn;
     a.chunk = c.chunk;
-    if (c.slots * a.Cn * rows::NW > 0x7fffffff || (int64_t)c.ntiles * a.Cn * (swa::KB * 2 * d / swa::JE) > 0x7fffffff) return HBA_ERR_UNSUPPORTED;
+    if (c.slots * a.Cn * rows::NW > 0x7fffffff ||
+        (int64_t)c.ntiles * a.Cn * (swa::KB * 2 * d / swa::JE) > 0x7fffffff)
+        return HBA_ERR_UNSUPPORTED;
     int st = HBA_OK;
 #define HBA_SWA(DT, D) st = swa::launch_bwd<DT, D>(a, grid, c, (hipStream_t)stream)
     HBA_DISPATCH_DT_D(dtype, d, HBA_SWA);

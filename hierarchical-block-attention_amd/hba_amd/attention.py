@@ -255,7 +255,8 @@ class _Sliding(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, lens, window, sinks, scale):
-        out, lse = ops._swa_fwd(q, k, v, lens, window, sinks, scale)
+        fwd = ops.swa_fwd if torch.compiler.is_compiling() else ops._swa_fwd
+        out, lse = fwd(q, k, v, lens, window, sinks, scale)
         ctx.save_for_backward(q, k, v, out, lse, lens)
         ctx.meta = (window, sinks, scale)
         return out
@@ -264,7 +265,8 @@ class _Sliding(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse, lens = ctx.saved_tensors
-        return (*ops._swa_bwd(q, k, v, out, lse, dout, lens, *ctx.meta), None, None, None, None)
+        bwd = ops.swa_bwd if torch.compiler.is_compiling() else ops._swa_bwd
+        return (*bwd(q, k, v, out, lse, dout, lens, *ctx.meta), None, None, None, None)
 
 
 def sliding_attention(q, k, v, window, sinks=0, scale=None, lens=None):
@@ -280,7 +282,8 @@ def sliding_attention(q, k, v, window, sinks=0, scale=None, lens=None):
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _Sliding.apply(q, k, v, lens, int(window), int(sinks), scale)
-    return ops._swa_fwd(q, k, v, lens, int(window), int(sinks), scale)[0]
+    fwd = ops.swa_fwd if torch.compiler.is_compiling() else ops._swa_fwd
+    return fwd(q, k, v, lens, int(window), int(sinks), scale)[0]
 
 
 def hba_attention_eval(q, k, v, cos, sin, cfg, summ, qkn, cap=None, hier=False, equiv=False):

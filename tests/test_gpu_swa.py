@@ -274,6 +274,23 @@ def test_custom_ops_agree():
     assert all(torch.equal(a, b) for a, b in zip(want, got))
 
 
+def test_traced():
+    """In a traced graph the registered operators stand for the calls."""
+    q, k, v, do = (t.cuda() for t in make(torch.bfloat16, 2, 70, 4, 2, 64))
+    lens = torch.tensor([70, 33], device="cuda")
+
+    def f(q, k, v):
+        return hba_amd.sliding_attention(q, k, v, 20, 3, lens=lens)
+
+    torch.compiler.reset()
+    traced = torch.compile(f, backend="aot_eager", fullgraph=True)
+    assert torch.equal(traced(q, k, v), f(q, k, v))
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    want = torch.autograd.grad(f(*leaves), leaves, do)
+    got = torch.autograd.grad(traced(*leaves), leaves, do)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_lse():
     q, k, v, _ = make(torch.float32, 1, 150, 2, 1, 64)
     _, lse = ops.swa_fwd(q.cuda(), k.cuda(), v.cuda(), None, 40, 1, 0.125)

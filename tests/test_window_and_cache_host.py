@@ -19,15 +19,18 @@ def size(fn, *args):
     return fn(*args, ctypes.byref(n)), n.value
 
 
-def swa(B=1, n=5, Hq=4, Hkv=2, d=64, W=3, S=1, scale=0.1, dtype=1, q=FAKE, k=FAKE, out=FAKE, st=S3):
-    return _lib.lib().hba_swa_fwd(dtype, q, st, k, S3, FAKE, S3, None, B, n, Hq, Hkv, d, W, S, scale, out, None, None)
+def swa(B=1, n=5, Hq=4, Hkv=2, d=64, W=3, S=1, scale=0.1, dtype=1, q=FAKE, k=FAKE, out=FAKE, st=S3,
+        kst=S3):
+    return _lib.lib().hba_swa_fwd(dtype, q, st, k, kst, FAKE, S3, None, B, n, Hq, Hkv, d, W, S, scale, out, None,
+                                  None)
 
 
 @pytest.mark.parametrize("bad,status", [
     (dict(B=0), -1), (dict(n=0), -1), (dict(Hq=3), -1), (dict(Hkv=0), -1), (dict(W=0), -1), (dict(S=-1), -1),
     (dict(scale=0.0), -1), (dict(scale=-1.0), -1), (dict(scale=float("nan")), -1), (dict(scale=float("inf")), -1),
     (dict(q=None), -1), (dict(out=None), -1), (dict(dtype=7), -2), (dict(d=96), -2), (dict(d=32), -2),
-    (dict(q=OFF), -2), (dict(k=OFF), -2), (dict(st=(ctypes.c_int64 * 3)(64, 64, 63)), -2)])
+    (dict(q=OFF), -2), (dict(k=OFF), -2), (dict(st=(ctypes.c_int64 * 3)(64, 64, 63)), -2),
+    (dict(kst=(ctypes.c_int64 * 3)(64, -64, 64)), -2), (dict(kst=(ctypes.c_int64 * 3)(64, 1 << 24, 64)), -2)])
 def test_swa_refuses(bad, status):
     assert swa(**bad) == status
 
