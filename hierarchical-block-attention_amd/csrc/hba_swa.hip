@@ -123,6 +123,11 @@ __device__ __forceinline__ const char *dout_row(const Args &a, const Rows &x) {
     return a.dout + x.b * a.dos[0] + x.tok * a.dos[1] + x.head * a.dos[2];
 }
 
+// 32768 tokens, 14 heads, d = 64, W = 1024, bf16: 165 us, 0.72 PFLOP/s (98 us at the
+// 1.21 of a large product).  Bound by issue: per 32 rows and 32 keys 16 exponentials
+// and as many multiply-adds and conversions a lane stand beside 8 matrix
+// instructions (without the exponentials 144 us, without reading operands from LDS
+// 150).  fp32, 2 x 2047 tokens, W = 512: 80 to 89 us, 37 at the fp32 matrix rate.
 template <int DT, int D>
 __global__ __launch_bounds__(64 * NW, (DT == 1 && D == 64 ? 3 : WAVES<DT, D>)) void swa_fwd(const Args a) {
     extern __shared__ __align__(16) char smem[];
@@ -258,6 +263,9 @@ template <int DT, int D> __device__ __forceinline__ void dq_each(const Args a) {
     store_dq<DT, D>(a, x, acc);
 }
 
+// Rows as swa_fwd, three products a tile (q . k again, do . v, ds . k).  8192 tokens,
+// 28 heads, d = 128, W = 1024, bf16: 200 us, 110 at the rate of a large product.
+constexpr int FEW = 256;   // keys: see swa_dq
 template <int DT, int D> __global__ __launch_bounds__(64 * NW, DT == 1 ? 2 : 1) void swa_dq(const Args a) {
     extern __shared__ __align__(16) char smem[];
     typedef Tile<DT, D> TL;
@@ -278,6 +286,11 @@ template <int DT, int D> __global__ __launch_bounds__(64 * NW, DT == 1 ? 2 : 1) 
     const float delta = row_delta<DT, D>(a, x, dO);
     if (x.valid && hf == 0) a.delta[hrow] = delta;
     const float lse = x.valid ? a.lse[hrow] : INFINITY;
+    // Rows with few keys have the largest gradients (as 1 / sqrt(keys)) and so most of
+    // the whole's rounding error: their ds enters the product with its rest.  1999
+    // tokens, W = 512, N(0, 1), d = 64: dq is off by 2.2e-3 of its norm, 2.47e-3
+    // without (2.28e-3 for 128 keys; its own rounding alone 1.66e-3), for 1 us of 31.
+    const bool few = x.w.hi_max <= FEW;
     const f32x16 zero = {0.0f};
     f32x16 acc[NDT];
 #pragma unroll
@@ -315,6 +328,16 @@ template <int DT, int D> __global__ __launch_bounds__(64 * NW, DT == 1 ? 2 : 1) 
 #pragma unroll
                 for (int dt = 0; dt < NDT; ++dt)
                     acc[dt] = Op<DT>::mma(TL::col(t, 32 * kt + 16 * u, dt, lane), df, acc[dt]);
+                if (DT == 1 && few) {
+                    float y[8];
+                    Op<DT>::unpack(df, y);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[e] = s[8 * u + e] - y[e];
+                    const F rest = Op<DT>::pack(y);
+#pragma unroll
+                    for (int dt = 0; dt < NDT; ++dt)
+                        acc[dt] = Op<DT>::mma(TL::col(t, 32 * kt + 16 * u, dt, lane), rest, acc[dt]);
+                }
             }
         }
     }
@@ -402,6 +425,10 @@ __device__ __forceinline__ void store_keys(const Args &a, const Keys &x, f32x16 
     store_rows<DT, D>(a.dv + row, dv, 1.0f);
 }
 
+// Four products a step of 32 tokens.  Same case as swa_dq: 320 to 340 us, 146 at the
+// rate of a large product; each operand that a wave reads from LDS serves one matrix
+// instruction (its 32 keys are the other one), which is what bounds it beside the
+// exponentials.
 template <int DT, int D> __global__ __launch_bounds__(64 * NW, DT == 1 ? 2 : 1) void swa_dkv(const Args a) {
     extern __shared__ __align__(16) char smem[];
     typedef Tile<DT, D> TL;
@@ -511,7 +538,7 @@ template <int DT, int D> __global__ __launch_bounds__(64 * NW, DT == 1 ? 2 : 1) 
 
 // dk and dv of the tiles in several parts: the parts' sums, in order.  A workgroup
 // takes 1024 elements of one key tile and KV head, 4 a thread, so that there
-// are enough of them to keep HBM busy.
+// are enough of them to keep HBM busy (8192 tokens, 4 KV heads, d = 128, 3 parts: 20 us).
 //
 // Keys of a wave that swa_dkv marked are computed here instead, token by token,
 // the masked ones left out: 2D / 4 threads a key, those of its dk with q . k, those
@@ -578,7 +605,7 @@ template <int DT, int D> __global__ __launch_bounds__(JE / 4) void swa_join(cons
 // steps of a part (and a part's start and end, worth some 4 steps), and the
 // traffic of the parts' sums, take least.  A step takes about 0.9 us at d = 64,
 // 1.8 at d = 128 (bf16; fp32 eight times that).  Measured at 8192 tokens, 28 / 4
-// heads, d = 128, kernel and join: 2 parts 481 us, 3 (taken) 370, 4 410, 8 412.
+// heads, d = 128, kernel and join: 2 parts 481 us, 3 (taken) 360, 4 410, 8 412.
 struct Cut {
     int ntiles, nst, Ps, Pn, chunk;
     int64_t slots;
