@@ -265,7 +265,6 @@ template <int DT, int D> __device__ __forceinline__ void dq_each(const Args a) {
 
 // Rows as swa_fwd, three products a tile (q . k again, do . v, ds . k).  8192 tokens,
 // 28 heads, d = 128, W = 1024, bf16: 200 us, 110 at the rate of a large product.
-constexpr int FEW = 256;   // keys: see swa_dq
 template <int DT, int D> __global__ __launch_bounds__(64 * NW, DT == 1 ? 2 : 1) void swa_dq(const Args a) {
     extern __shared__ __align__(16) char smem[];
     typedef Tile<DT, D> TL;
@@ -286,6 +285,7 @@ template <int DT, int D> __global__ __launch_bounds__(64 * NW, DT == 1 ? 2 : 1) 
     const float delta = row_delta<DT, D>(a, x, dO);
     if (x.valid && hf == 0) a.delta[hrow] = delta;
     const float lse = x.valid ? a.lse[hrow] : INFINITY;
+    constexpr int FEW = 256;
     // Rows with few keys have the largest gradients (as 1 / sqrt(keys)) and so most of
     // the whole's rounding error: their ds enters the product with its rest.  1999
     // tokens, W = 512, N(0, 1), d = 64: dq is off by 2.2e-3 of its norm, 2.47e-3
