@@ -176,6 +176,20 @@ def test_padded_batch(dt):
     assert all(torch.equal(bits(got[n]), bits(want[n])) for n in got)
 
 
+def test_pages_far_apart():
+    """The same pages at the end of a cache of over 4 GiB."""
+    s = setup(torch.bfloat16, 64, 2, [10, 60], [150, 5])
+    near = {n: s[n].clone() for n in ("kc", "kr", "vp", "summ")}
+    append(s, **near)
+    extra = 270000
+    far = {}
+    for n in near:
+        far[n] = torch.empty(extra + s[n].shape[0], *s[n].shape[1:], dtype=torch.bfloat16, device="cuda")
+        far[n][extra:] = s[n]
+    append(s, table=s["table"] + extra, **far)
+    assert all(torch.equal(bits(far[n][extra:]), bits(near[n])) for n in near)
+
+
 def test_graph_replays():
     old, new = [50, 3], [90, 61]
     s = setup(torch.bfloat16, 64, 2, old, new)

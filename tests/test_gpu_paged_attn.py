@@ -204,6 +204,20 @@ def test_masked_values_have_no_effect(dt):
                 assert not bool(torch.isfinite(got[sees]).any())
 
 
+@pytest.mark.parametrize("new", [None, [70, 3]])
+def test_pages_far_apart(new):
+    """The same pages at the end of a cache of over 4 GiB."""
+    s = setup(torch.bfloat16, 64, 4, 2, [2300, 190], new)
+    near = call(s)
+    P, extra = s["kr"].shape[0], 270000
+    far = {**s, "table": s["table"] + extra}
+    for n in ("kr", "vp"):
+        far[n] = torch.empty(P + extra, *s[n].shape[1:], dtype=torch.bfloat16, device="cuda")
+        far[n][extra:] = s[n].cuda()
+    assert far["kr"].numel() * 2 > 2 ** 32
+    assert torch.equal(call(far), near)
+
+
 def test_strides_streams_and_graphs():
     s = setup(torch.bfloat16, 64, 4, 2, [300, 65, 700, 1])
     want = call(s)

@@ -189,6 +189,20 @@ def test_strided_views(dt):
     assert all(torch.equal(s, t) for s, t in zip(a, b))
 
 
+def test_rows_far_apart():
+    """Rows just under 16 MiB apart: offsets within a sequence pass 32 bits."""
+    q, k, v, do = make(torch.bfloat16, 1, 290, 4, 2, 64)
+    far = torch.empty(290, 2 ** 23 - 64, dtype=torch.bfloat16, device="cuda")
+    views = []
+    for i, t in enumerate((q, k, v, do)):
+        x = far[:, 1024 * i:1024 * i + t.shape[2] * 64].unflatten(1, (t.shape[2], 64))[None]
+        x.copy_(t)
+        views.append(x)
+    leaves = [x.detach().requires_grad_() for x in views[:3]]
+    out = hba_amd.sliding_attention(*leaves, 100, 3)
+    compare((out, *torch.autograd.grad(out, leaves, views[3])), q, k, v, 100, 3, None, None, do)
+
+
 def test_gradients_match_differences():
     q, k, v, do = make(torch.float32, 1, 70, 2, 1, 64, seed=10)
     _, *grads = run(q, k, v, 30, 2, dout=do)
