@@ -36,7 +36,7 @@ struct Args {
     char *dq, *dk, *dv;
     float *part;                        // dk / dv sums of tiles in several parts
     int32_t *marks;                     // waves of swa_dkv whose sums are not finite
-    int nst, Ps, Pn, chunk;             // tiles of sinks, parts of those and of the others, steps of a part
+    int nst, Ps, Pn, schunk, chunk;     // tiles of sinks, parts of those and of the others, steps of a part of either
 };
 
 __device__ __forceinline__ int seq_len(const Args &a, int b) {
@@ -396,8 +396,9 @@ __device__ __forceinline__ void find_keys(const Args &a, Keys &x) {
     x.j = x.kw + (lane & 31);
     x.nst = steps(x.k0, x.len, a.W, a.S);
     x.parts = tile < a.nst ? a.Ps : a.Pn;
-    x.i0 = part * a.chunk;
-    x.i1 = min(x.nst * a.G, x.i0 + a.chunk);
+    const int chunk = tile < a.nst ? a.schunk : a.chunk;
+    x.i0 = part * chunk;
+    x.i1 = min(x.nst * a.G, x.i0 + chunk);
     x.at = ((int64_t)combo * (a.nst * a.Ps + (a.ntiles - a.nst) * a.Pn) + slot) * KB + 32 * wave + (lane & 31);
 }
 
@@ -554,7 +555,8 @@ template <int DT, int D> __global__ __launch_bounds__(JE / 4) void swa_join(cons
     const int P = tile < a.nst ? a.Ps : a.Pn;
     const int slot = tile < a.nst ? tile * a.Ps : a.nst * a.Ps + (tile - a.nst) * a.Pn;
     const int b = combo / a.Hkv, g = combo % a.Hkv, len = seq_len(a, b), k0 = tile * KB, j = k0 + r;
-    const int used = min(P, (steps(k0, len, a.W, a.S) * a.G + a.chunk - 1) / a.chunk);
+    const int chunk = tile < a.nst ? a.schunk : a.chunk;
+    const int used = min(P, (steps(k0, len, a.W, a.S) * a.G + chunk - 1) / chunk);
     bool marked = false;   // the same for the threads of a key
     for (int i = 0; i < used; ++i) marked |= a.marks[((slot + i) * a.Cn + combo) * NW + r / 32] != 0;
     if (j >= a.n || (P == 1 && !marked)) return;
@@ -608,7 +610,7 @@ template <int DT, int D> __global__ __launch_bounds__(JE / 4) void swa_join(cons
 // 1.8 at d = 128 (bf16; fp32 eight times that).  Measured at 8192 tokens, 28 / 4
 // heads, d = 128, kernel and join: 2 parts 481 us, 3 (taken) 360, 4 410, 8 412.
 struct Cut {
-    int ntiles, nst, Ps, Pn, chunk;
+    int ntiles, nst, Ps, Pn, schunk, chunk;
     int64_t slots;
 };
 static Cut cut(int dtype, int64_t d, int64_t Cn, int64_t n, int64_t G, int64_t W, int64_t S) {
@@ -623,12 +625,20 @@ static Cut cut(int dtype, int64_t d, int64_t Cn, int64_t n, int64_t G, int64_t W
     double least = 0;
     for (int64_t P = 1; P <= 32 && P <= usual; ++P) {
         const int64_t ch = (usual + P - 1) / P;
+        // Tiles of sinks, which every later row sees, get parts of as many steps; where
+        // that were more than four rounds of parts, longer ones (a workspace of four
+        // rounds at most, where thousands of sinks would ask for many GB).
+        const int64_t even = (c.nst * Cn * most + 4 * room - 1) / (4 * room), sch = even > ch ? even : ch;
         c.chunk = (int)ch;
+        c.schunk = (int)sch;
         c.Pn = (int)((usual + ch - 1) / ch);
-        c.Ps = (int)((most + ch - 1) / ch);
+        c.Ps = (int)((most + sch - 1) / sch);
         c.slots = (int64_t)c.nst * c.Ps + (int64_t)(c.ntiles - c.nst) * c.Pn;
         const int64_t parts = (c.Ps > 1 ? (int64_t)c.nst * c.Ps : 0) + (c.Pn > 1 ? (int64_t)(c.ntiles - c.nst) * c.Pn : 0);
-        const double us = (double)((c.slots * Cn + room - 1) / room) * (ch + 4) * step +
+        const auto rounds = [&](int64_t slots) { return (double)((slots * Cn + room - 1) / room); };
+        const int64_t sinks = (int64_t)c.nst * c.Ps;
+        const double us = (sch == ch ? rounds(c.slots) * (ch + 4)
+                                     : rounds(sinks) * (sch + 4) + rounds(c.slots - sinks) * (ch + 4)) * step +
                           (double)(parts * Cn) * KB * 2 * d * 8 / 4e6;
         if (P == 1 || us < least) {
             least = us;
@@ -817,6 +827,7 @@ extern "C" int hba_swa_bwd(int dtype, const void *q, const int64_t q_strides[3],
     a.nst = c.nst;
     a.Ps = c.Ps;
     a.Pn = c.Pn;
+    a.schunk = c.schunk;
     a.chunk = c.chunk;
     if (c.slots * a.Cn * rows::NW > 0x7fffffff ||
         (int64_t)c.ntiles * a.Cn * (swa::KB * 2 * d / swa::JE) > 0x7fffffff)

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import hba_amd
-from attn64 import assert_within, sliding, unit
+from attn64 import assert_within, attend, sliding, unit
 from hba_amd import ops
 
 pytestmark = pytest.mark.gpu
@@ -201,6 +201,20 @@ def test_rows_far_apart():
     leaves = [x.detach().requires_grad_() for x in views[:3]]
     out = hba_amd.sliding_attention(*leaves, 100, 3)
     compare((out, *torch.autograd.grad(out, leaves, views[3])), q, k, v, 100, 3, None, None, do)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_thousands_of_sinks(dt):
+    """As many sinks as keys: tiles of sinks have longer parts than the others would."""
+    n = 9000
+    q, k, v, do = make(DT[dt], 1, n, 1, 1, 64, seed=9)
+    got = run(q, k, v, 1, n, dout=do)
+    i = torch.arange(n, device="cuda")
+    want, bound = attend(q[0].cuda(), k[0, :, 0].cuda(), v[0, :, 0].cuda(), i[None] <= i[:, None], 64 ** -0.5,
+                         unit(DT[dt]), do[0].cuda())
+    for name, x, y, z in zip(("out", "dq", "dk", "dv"), got, want, bound):
+        x = x[0] if name in ("out", "dq") else x[0, :, 0]
+        assert_within(x, y.cpu(), z.cpu(), name)
 
 
 def test_gradients_match_differences():

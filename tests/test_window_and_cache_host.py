@@ -51,10 +51,14 @@ def test_swa_backward_refuses_a_short_workspace():
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("n", [1, 63, 1000, 8192, 100000])
 def test_swa_backward_workspace(n, d, dtype):
-    """At least every row's <dout, out>; no more than 33 parts of every key tile's sums."""
-    for W, S in ((1, 0), (64, 4), (1024, 8), (n, 0), (n, n)):
-        st, need = size(_lib.lib().hba_swa_bwd_workspace_bytes, dtype, 2, n, 8, 2, d, min(W, n), min(S, n))
-        assert st == 0 and 2 * 8 * n * 4 <= need
+    """Every row's <dout, out>; of parts no more than four rounds of sink tiles' (768
+    workgroups of 128 keys at most), one for every such tile and 32 for every other."""
+    for W, S in ((1, 0), (64, 4), (1024, 8), (1, n), (64, n // 2), (1024, 4096), (n, 0), (n, n)):
+        W, S = min(W, n), min(S, n)
+        st, need = size(_lib.lib().hba_swa_bwd_workspace_bytes, dtype, 2, n, 8, 2, d, W, S)
+        tiles, sinks = -(-n // 128), -(-S // 128)
+        parts = 4 * 768 + 2 * sinks * 4 + 32 * (tiles - sinks) * 4
+        assert st == 0 and 2 * 8 * n * 4 <= need <= 2 * 8 * n * 4 + parts * (128 * 2 * d * 4 + 16) + 1024
 
 
 def paged(T=2, Bd=2, Hq=4, Hkv=2, d=64, Bk=64, W=0, S=0, shared=0, max_len=1000, maxp=16, pages=40, dtype=1, q=FAKE,
