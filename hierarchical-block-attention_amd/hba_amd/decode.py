@@ -74,6 +74,7 @@ class PagedKVCache:
         self._table = [[] for _ in range(batch)]
         self._free = list(range(P - 1, -1, -1))
         self._held = set()               # pages that several sequences begin with
+        self._common = 0                 # pages that all sequences are known to begin with (tables only grow)
         self._scale_tabs = {}
         self._scales = torch.zeros(batch, dtype=torch.float32, device=device)   # written by append
         self._scales_ok = False          # _scales holds the scales of the current lengths
@@ -300,9 +301,12 @@ def cache_attention(q, cache, cfg, qkn, cos, sin, window=None, sinks=0, cu=None,
     if window is not None and window < 1:
         raise ValueError(f"window must be at least 1, got {window}")
     if shared:
-        head = cache._table[0][:shared // PAGE]
-        if shared % PAGE or len(head) < shared // PAGE or any(t[:len(head)] != head for t in cache._table):
-            raise ValueError(f"the sequences do not share their first {shared} tokens' pages")
+        n = shared // PAGE
+        if shared % PAGE or n > cache._common:
+            head = cache._table[0][:n]
+            if shared % PAGE or len(head) < n or any(t[:n] != head for t in cache._table):
+                raise ValueError(f"the sequences do not share their first {shared} tokens' pages")
+            cache._common = n
     longest = max(cache.lens)
     if max_len is None:
         max_len = max(longest, 1)
