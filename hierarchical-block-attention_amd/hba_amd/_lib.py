@@ -119,9 +119,11 @@ def strides3(t):
 
 def used_strides3(t):
     """strides3 with 0 for dims of one element, whose stride no address uses."""
-    return _I64X3(*(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape)))
+    (a, b, c, _), (n, m, h, _) = t.stride(), t.shape
+    return _I64X3(a if n > 1 else 0, b if m > 1 else 0, c if h > 1 else 0)
 
 
 def used_strides2(t):
     """First two strides of a 3-D [T, H, d] view, 0 for dims of one element."""
-    return _I64X2(*(s if n > 1 else 0 for s, n in zip(t.stride()[:2], t.shape)))
+    (a, b, _), (n, h, _) = t.stride(), t.shape
+    return _I64X2(a if n > 1 else 0, b if h > 1 else 0)

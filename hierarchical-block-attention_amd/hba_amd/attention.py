@@ -282,8 +282,9 @@ def sliding_attention(q, k, v, window, sinks=0, scale=None, lens=None):
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _Sliding.apply(q, k, v, lens, int(window), int(sinks), scale)
-    fwd = ops.swa_fwd if torch.compiler.is_compiling() else ops._swa_fwd
-    return fwd(q, k, v, lens, int(window), int(sinks), scale)[0]
+    if torch.compiler.is_compiling():
+        return ops.swa_fwd(q, k, v, lens, int(window), int(sinks), scale)[0]
+    return ops._swa_fwd(q, k, v, lens, int(window), int(sinks), scale, want_lse=False)[0]
 
 
 def hba_attention_eval(q, k, v, cos, sin, cfg, summ, qkn, cap=None, hier=False, equiv=False):

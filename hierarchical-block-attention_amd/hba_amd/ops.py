@@ -563,10 +563,11 @@ def _(q, k, v, kc, kr, q_gain, k_gain, eps, cos, sin, idx, cnt, out, dout, sinks
 def _rows16(t):
     """t, or a copy of it, with a contiguous last dim, rows on 16-byte boundaries and less
     than 16 MiB from token to token."""
-    q = 16 // t.element_size()
-    st, sz = t.stride(), t.shape
-    if (st[-1] == 1 and t.data_ptr() % 16 == 0 and st[-3] * t.element_size() < 1 << 24
-            and all(s % q == 0 or n == 1 for s, n in zip(st[:-1], sz[:-1]))):
+    e = t.element_size()
+    st, sz, q = t.stride(), t.shape, 16 // e
+    if st[-1] == 1 and t.data_ptr() % 16 == 0 and st[-3] * e < 1 << 24 and (
+            (t.is_contiguous() and sz[-1] % q == 0)     # the usual case, without the loop's microsecond
+            or all(s % q == 0 or n == 1 for s, n in zip(st[:-1], sz[:-1]))):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -595,11 +596,11 @@ def _swa_args(q, k, v, lens, window, sinks, scale):
     return dev, B, n, Hq, Hkv, d, lens
 
 
-def _swa_fwd(q, k, v, lens, window, sinks, scale):
+def _swa_fwd(q, k, v, lens, window, sinks, scale, want_lse=True):
     dev, B, n, Hq, Hkv, d, lens = _swa_args(q, k, v, lens, window, sinks, scale)
     code = _code(q)
     out = torch.empty(B, n, Hq, d, dtype=q.dtype, device=dev)
-    lse = torch.empty(B, Hq, n, dtype=torch.float32, device=dev)
+    lse = torch.empty(B, Hq, n, dtype=torch.float32, device=dev) if want_lse else None
     if out.numel() == 0:
         return out, lse
     q, k, v = _rows16(q), _rows16(k), _rows16(v)
