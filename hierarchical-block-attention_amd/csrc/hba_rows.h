@@ -48,8 +48,8 @@ constexpr float MOST = 65536.0f;  // sum of a tile's probabilities that calls fo
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 
-// The thread's place among the NW waves of its rows (a workgroup may have two such
-// sets, for halves of the keys).
+// The thread's place among the NW waves that stage tiles together (a workgroup may
+// have two such groups, for halves of the keys).
 __device__ __forceinline__ int thread() { return threadIdx.x % (64 * NW); }
 
 // The value of lane l ^ 32.
@@ -202,10 +202,10 @@ template <int DT, int D> struct Tile {
 };
 
 // Keys and values of one KV head as strided rows.
-template <int DT, int D> struct DenseKV {
+template <int DT, int D, int KEYS_ = KEYS<DT, D>> struct DenseKV {
     typedef typename Op<DT>::F F;
     typedef Tile<DT, D> TL;
-    static constexpr int KT = KEYS<DT, D>, BYTES = 2 * KT * TL::ROWB;   // a staged tile: keys, then values
+    static constexpr int KT = KEYS_, BYTES = 2 * KT * TL::ROWB;   // a staged tile: keys, then values
     const char *k, *v;
     int64_t kb, vb;                                   // bytes from row to row
     int last;                                         // the last row that may be read
@@ -382,10 +382,11 @@ __device__ __forceinline__ void attend_begin(Src &src, char *smem, int it0, int 
 // units.  LO: the queries come as two parts in log2 units already (c = 1); their
 // products then start from -m instead of 0.  Every wave of the workgroup calls
 // it; it leaves no wave reading LDS.
-template <int DT, int D, bool LO, class Src>
+// ONE: of each tile the wave takes the 32 keys `which` only (another one has the rest).
+template <int DT, int D, bool LO, bool ONE = false, class Src>
 __device__ __forceinline__ void attend(Src &src, char *smem, const typename Op<DT>::F (&q)[D / 16],
                                        const typename Op<DT>::F *qlo, float c, int it0, int it1, int ns, int wt0,
-                                       const Sees &w, RowAcc<DT, D> &a) {
+                                       const Sees &w, RowAcc<DT, D> &a, int which = 0) {
     typedef typename Op<DT>::F F;
     constexpr int NKS = D / 16, NDT = D / 32, KT = Src::KT;
     const int lane = threadIdx.x & 63, hf = lane >> 5;
@@ -410,8 +411,8 @@ __device__ __forceinline__ void attend(Src &src, char *smem, const typename Op<D
         if (j0 >= w.hi_max || (j0 + KT <= w.lo_min && j0 >= w.S)) continue;   // nothing the wave's rows see
         const char *t = smem + cur * Src::BYTES;
 #pragma unroll
-        for (int kt = 0; kt < KT / 32; ++kt) {   // 32 keys at a time: fewer registers, and halves that no row sees cost nothing
-            const int jh = j0 + 32 * kt;
+        for (int i = 0; i < (ONE ? 1 : KT / 32); ++i) {   // 32 keys at a time: fewer registers, and halves that no row sees cost nothing
+            const int kt = ONE ? which : i, jh = j0 + 32 * kt;
             if (jh >= w.hi_max || (jh + 32 <= w.lo_min && jh >= w.S)) continue;
             f32x16 s = zero;
             if constexpr (LO) s = s + shift;
@@ -499,13 +500,13 @@ __device__ __forceinline__ void add_row(f32x16 (&o)[D / 32], const char *p, floa
     }
 }
 
-template <int DT, int D>
+template <int DT, int D, int KT>
 template <bool LO>
-__device__ __forceinline__ float DenseKV<DT, D>::dot(const F (&q)[D / 16], const F *, int j, int hf) const {
+__device__ __forceinline__ float DenseKV<DT, D, KT>::dot(const F (&q)[D / 16], const F *, int j, int hf) const {
     return dot_rows<DT, D>(q, k + (int64_t)min(j, last) * kb, hf);
 }
-template <int DT, int D>
-__device__ __forceinline__ void DenseKV<DT, D>::add(f32x16 (&o)[D / 32], int j, float p, int hf) const {
+template <int DT, int D, int KT>
+__device__ __forceinline__ void DenseKV<DT, D, KT>::add(f32x16 (&o)[D / 32], int j, float p, int hf) const {
     add_row<DT, D>(o, v + (int64_t)min(j, last) * vb, p, hf);
 }
 

@@ -50,7 +50,9 @@ struct Rows {
     Sees w;
 };
 
-template <int D> __device__ __forceinline__ bool find_rows(const Args &a, Rows &x) {
+// Of 32 R rows a workgroup, wave i those of i % R.
+template <int D, int R = NW> __device__ __forceinline__ bool find_rows(const Args &a, Rows &x) {
+    constexpr int RT = 32 * R;
     int combo, tile;
     xcd_map(blockIdx.x, a.Cn, a.ntiles, a.xmap, combo, tile);
     if (tile >= a.ntiles || combo >= a.Cn) return false;
@@ -58,7 +60,7 @@ template <int D> __device__ __forceinline__ bool find_rows(const Args &a, Rows &
     x.g = combo % a.Hkv;
     x.len = seq_len(a, x.b);
     const int nr = a.n * a.G, vr = x.len * a.G;          // rows there are, rows of the sequence
-    const int wave = __builtin_amdgcn_readfirstlane(rows::thread() >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64 % R);
     const int r0 = tile * RT, rw = r0 + wave * RW, r = rw + (threadIdx.x & 31);
     x.in = r < nr;
     x.valid = r < vr;
@@ -89,8 +91,9 @@ __device__ __forceinline__ void load_rows(const char *p, bool ok, typename Op<DT
     }
 }
 
-template <int DT, int D> __device__ __forceinline__ DenseKV<DT, D> keys(const Args &a, const Rows &x) {
-    DenseKV<DT, D> s;
+template <int DT, int D, int KT = KEYS<DT, D>>
+__device__ __forceinline__ DenseKV<DT, D, KT> keys(const Args &a, const Rows &x) {
+    DenseKV<DT, D, KT> s;
     s.k = a.k + x.b * a.ks[0] + x.g * a.ks[2];
     s.v = a.v + x.b * a.vs[0] + x.g * a.vs[2];
     s.kb = a.ks[1];
@@ -149,50 +152,61 @@ __global__ __launch_bounds__(64 * NW, (DT == 1 && D == 64 ? 3 : WAVES<DT, D>)) v
     store_fwd<DT, D>(a, x, acc, l);
 }
 
-// swa_fwd where its workgroups leave CUs free: two sets of waves have the same rows,
-// each half of the tiles, and meet in LDS.  1001 tokens, 14 heads, d = 64, W = 1024
-// (110 workgroups): 17 us against 20; 28 heads, d = 128 (220) 26 against 31; fp32,
-// d = 64, whose matrix products bound it, 72 against 75.
-template <int DT, int D> constexpr size_t halves_lds() {
-    constexpr size_t tiles = 4 * DenseKV<DT, D>::BYTES, sums = (size_t)64 * NW * (D / 2 + 2) * 4;
+// swa_fwd where its workgroups leave CUs free: 8 waves of which `sets` have the same
+// rows and share their keys, and meet in LDS.  Two sets of 4 waves (128 rows) have
+// half of the tiles each; of four sets of 2 waves (64 rows, and so twice as many
+// workgroups) a pair has half of the tiles of 64 keys and one of the pair 32 keys
+// of each.  1001 tokens, 14 heads, W = 1024, d = 64: 20 us as one set (110 workgroups),
+// 17 as two, 13 as four (220); fp32 75, 72 and 42; d = 128 25 as two and 19 as four.
+template <int DT, int D, int SETS> using SetsKV = DenseKV<DT, D, (SETS == 4 ? 64 : KEYS<DT, D>)>;
+template <int DT, int D, int SETS> constexpr size_t sets_lds() {
+    constexpr size_t tiles = 4 * SetsKV<DT, D, SETS>::BYTES, sums = (size_t)(SETS - 1) * 512 / SETS * (D / 2 + 2) * 4;
     return tiles > sums ? tiles : sums;
 }
-template <int DT, int D> __global__ __launch_bounds__(2 * 64 * NW) void swa_fwd_halves(const Args a) {
+template <int DT, int D, int SETS> __global__ __launch_bounds__(512) void swa_fwd_sets(const Args a) {
     extern __shared__ __align__(16) char smem[];
+    constexpr int R = 8 / SETS, T = 64 * R;   // waves, lanes of a set
     Rows x;
-    if (!find_rows<D>(a, x)) return;
-    const int half = __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * NW));
-    DenseKV<DT, D> src = keys<DT, D>(a, x);
+    if (!find_rows<D, R>(a, x)) return;
+    const int half = __builtin_amdgcn_readfirstlane(threadIdx.x / 256);
+    const int set = __builtin_amdgcn_readfirstlane(threadIdx.x / T);
+    constexpr int KT = SetsKV<DT, D, SETS>::KT;
+    auto src = keys<DT, D, KT>(a, x);
     int ns, wt0;
-    const int nt = tile_list<KEYS<DT, D>>(x.lo, x.hi, a.S, ns, wt0), mid = (nt + 1) / 2;
+    const int nt = tile_list<KT>(x.lo, x.hi, a.S, ns, wt0), mid = (nt + 1) / 2;
     const int it0 = half ? mid : 0, it1 = half ? nt : mid;
-    char *mine = smem + half * 2 * DenseKV<DT, D>::BYTES;
+    char *mine = smem + half * 2 * src.BYTES;
     attend_begin(src, mine, it0, it1, ns, wt0);
     typename Op<DT>::F q[D / 16];
     load_rows<DT, D>(q_row<DT, D>(a, x), x.valid, q);
     RowAcc<DT, D> acc;
-    attend<DT, D, false>(src, mine, q, nullptr, a.c, it0, it1, ns, wt0, x.w, acc);
+    attend<DT, D, false, SETS == 4>(src, mine, q, nullptr, a.c, it0, it1, ns, wt0, x.w, acc, set % 2);
     if (it1 - it0 < mid) __syncthreads();   // the other half's last tile: as many barriers for both
-    float *sums = reinterpret_cast<float *>(smem) + rows::thread();
-    constexpr int T = 64 * NW;
-    if (half) {
+    // element i of set s: sums[(i (SETS - 1) + s - 1) T]
+    float *sums = reinterpret_cast<float *>(smem) + threadIdx.x % T;
+    constexpr int E = (SETS - 1) * T;
+    if (set) {
+        sums += (set - 1) * T;
 #pragma unroll
         for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) sums[(16 * dt + r) * T] = acc.O[dt][r];
-        sums[D / 2 * T] = acc.m;
-        sums[(D / 2 + 1) * T] = acc.l;
+            for (int r = 0; r < 16; ++r) sums[(16 * dt + r) * E] = acc.O[dt][r];
+        sums[D / 2 * E] = acc.m;
+        sums[(D / 2 + 1) * E] = acc.l;
     }
     __syncthreads();
-    if (half) return;
-    const float om = sums[D / 2 * T], m = fmaxf(acc.m, om);
-    const float fa = acc.m == -INFINITY ? 0.0f : ex2(acc.m - m), fb = om == -INFINITY ? 0.0f : ex2(om - m);
-    acc.m = m;
-    acc.l = fmaf(sums[(D / 2 + 1) * T], fb, acc.l * fa);
+    if (set) return;
 #pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
+    for (int s = 0; s < SETS - 1; ++s, sums += T) {
+        const float om = sums[D / 2 * E], m = fmaxf(acc.m, om);
+        const float fa = acc.m == -INFINITY ? 0.0f : ex2(acc.m - m), fb = om == -INFINITY ? 0.0f : ex2(om - m);
+        acc.m = m;
+        acc.l = fmaf(sums[(D / 2 + 1) * E], fb, acc.l * fa);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc.O[dt][r] = fmaf(sums[(16 * dt + r) * T], fb, acc.O[dt][r] * fa);
+        for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc.O[dt][r] = fmaf(sums[(16 * dt + r) * E], fb, acc.O[dt][r] * fa);
+    }
     float l = acc.l + other_half(acc.l);
     if (__ballot(x.valid && (any_bad<D>(acc.O) || !finite(l)))) {
         attend_each<DT, D, false>(src, q, nullptr, a.c, 0, nt, ns, wt0, x.w, acc);
@@ -661,18 +675,25 @@ template <int DT, int D, class K> static int lds_room(K kern, size_t bytes) {
                : HBA_ERR_LAUNCH;
 }
 
+template <int DT, int D, int SETS> static int launch_sets(const Args &a, int64_t grid, hipStream_t s) {
+    if (int st = lds_room<DT, D>(swa_fwd_sets<DT, D, SETS>, sets_lds<DT, D, SETS>())) return st;
+    hipLaunchKernelGGL((swa_fwd_sets<DT, D, SETS>), dim3((unsigned)grid), dim3(512), (sets_lds<DT, D, SETS>()), s, a);
+    HBA_LAUNCH_CHECK();
+    return HBA_OK;
+}
 template <int DT, int D> static int launch_fwd(const Args &a, int64_t grid, hipStream_t s) {
     constexpr size_t lds = 2 * DenseKV<DT, D>::BYTES;
     if constexpr (WAVES<DT, D> >= 2) {   // 8 waves on a CU
-        // the meeting costs what some 200 keys do: 300 tokens, d = 64, W = 128 takes 8.7 us either way, d = 128 12.2
-        // in one set and 12.4 in two; W = 256 9.7 and 9.4, 14.0 and 13.6
-        if (grid <= 256 && (a.W < a.n ? a.W : a.n) >= 256) {
-            if (int st = lds_room<DT, D>(swa_fwd_halves<DT, D>, halves_lds<DT, D>())) return st;
-            hipLaunchKernelGGL((swa_fwd_halves<DT, D>), dim3((unsigned)grid), dim3(2 * 64 * NW),
-                               (halves_lds<DT, D>()), s, a);
-            HBA_LAUNCH_CHECK();
-            return HBA_OK;
-        }
+        // What the meeting costs, in keys: 300 tokens, d = 64, W = 64, 128 and 256 take 7.8, 8.6 and 9.7 us as one
+        // set, the last 9.4 as two, and all 7.7, 7.9 and 8.2 as four; d = 128, W = 128 and 256: 12.2 and 14.0 as one,
+        // 12.4 and 13.6 as two.  100 tokens: 6.3 as one, 6.6 as four.
+        const int seen = a.W < a.n ? a.W : a.n;
+        Args b = a;
+        int64_t more;
+        b.ntiles = (int)(((int64_t)a.n * a.G + 63) / 64);
+        b.xmap = xcd_pick(b.Cn, b.ntiles, more);
+        if (more <= 256 && seen >= 128) return launch_sets<DT, D, 4>(b, more, s);
+        if (grid <= 256 && seen >= 256) return launch_sets<DT, D, 2>(a, grid, s);
     }
     if (int st = lds_room<DT, D>(swa_fwd<DT, D>, lds)) return st;
     hipLaunchKernelGGL((swa_fwd<DT, D>), dim3((unsigned)grid), dim3(64 * NW), lds, s, a);

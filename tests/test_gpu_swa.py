@@ -59,7 +59,7 @@ def test_forward_and_gradients(n, W, S, dt, d):
 @pytest.mark.parametrize("n,W,S", [(255, 255, 0), (256, 256, 0), (320, 256, 70), (700, 600, 3), (961, 2000, 0)])
 @pytest.mark.parametrize("lens", [None, [0, 255], [100, 64]])
 def test_few_rows_and_many_keys(n, W, S, lens, dt, d):
-    """Two sets of waves share the keys: odd and even tile counts, and workgroups without any."""
+    """Sets of waves share the keys: odd and even tile counts, and workgroups without any."""
     q, k, v, _ = make(DT[dt], 2, n, 3, 1, d, seed=n)
     x = [t.clone() for t in (q, k, v)]
     for b, m in enumerate(lens or []):
