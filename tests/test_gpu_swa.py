@@ -56,8 +56,9 @@ def test_forward_and_gradients(n, W, S, dt, d):
 
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
-@pytest.mark.parametrize("n,W,S", [(255, 255, 0), (256, 256, 0), (320, 256, 70), (700, 600, 3), (961, 2000, 0)])
-@pytest.mark.parametrize("lens", [None, [0, 255], [100, 64]])
+@pytest.mark.parametrize("n,W,S", [(128, 128, 0), (190, 129, 66), (255, 255, 0), (256, 256, 0), (320, 256, 70), (700, 600, 3),
+                                   (961, 2000, 0)])
+@pytest.mark.parametrize("lens", [None, [0, 128], [100, 64]])
 def test_few_rows_and_many_keys(n, W, S, lens, dt, d):
     """Sets of waves share the keys: odd and even tile counts, and workgroups without any."""
     q, k, v, _ = make(DT[dt], 2, n, 3, 1, d, seed=n)
@@ -66,6 +67,14 @@ def test_few_rows_and_many_keys(n, W, S, lens, dt, d):
         for t in x:
             t[b, m:] = float("nan")
     compare(run(*x, W, S, lens=lens), q, k, v, W, S, None, lens)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_two_sets_of_waves(dt, d):
+    """More rows than four sets would have workgroups for."""
+    q, k, v, _ = make(DT[dt], 2, 900, 14, 2, d, seed=5)
+    compare(run(q, k, v, 300, 2, lens=[900, 511]), q, k, v, 300, 2, None, [900, 511])
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
