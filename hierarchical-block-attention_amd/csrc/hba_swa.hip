@@ -277,6 +277,17 @@ template <int DT, int D> __device__ __forceinline__ void dq_each(const Args a) {
     store_dq<DT, D>(a, x, acc);
 }
 
+// What half16's rounding left of p.
+template <int DT>
+__device__ __forceinline__ typename Op<DT>::F rest16(const f32x16 &p, int u, typename Op<DT>::F f) {
+    float y[8];
+    Op<DT>::unpack(f, y);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = p[8 * u + e] - y[e];
+    return Op<DT>::pack(y);
+}
+constexpr int FEW = 256;   // rows (and so keys) whose ds enters its products in two parts, see swa_dq
+
 // Rows as swa_fwd, three products a tile (q . k again, do . v, ds . k).  8192 tokens,
 // 28 heads, d = 128, W = 1024, bf16: 200 us, 140 at the rate of a large product; the
 // matrix cores are busy 44 % of the time (the forward: 43 %).
@@ -300,7 +311,6 @@ template <int DT, int D> __global__ __launch_bounds__(64 * NW, DT == 1 ? 2 : 1) 
     const float delta = row_delta<DT, D>(a, x, dO);
     if (x.valid && hf == 0) a.delta[hrow] = delta;
     const float lse = x.valid ? a.lse[hrow] : INFINITY;
-    constexpr int FEW = 256;
     // Rows with few keys have the largest gradients (as 1 / sqrt(keys)) and so most of
     // the whole's rounding error: their ds enters the product with its rest.  1999
     // tokens, W = 512, N(0, 1), d = 64: dq is off by 2.2e-3 of its norm, 2.47e-3
@@ -344,11 +354,7 @@ template <int DT, int D> __global__ __launch_bounds__(64 * NW, DT == 1 ? 2 : 1) 
                 for (int dt = 0; dt < NDT; ++dt)
                     acc[dt] = Op<DT>::mma(TL::col(t, 32 * kt + 16 * u, dt, lane), df, acc[dt]);
                 if (DT == 1 && few) {
-                    float y[8];
-                    Op<DT>::unpack(df, y);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) y[e] = s[8 * u + e] - y[e];
-                    const F rest = Op<DT>::pack(y);
+                    const F rest = rest16<DT>(s, u, df);
 #pragma unroll
                     for (int dt = 0; dt < NDT; ++dt)
                         acc[dt] = Op<DT>::mma(TL::col(t, 32 * kt + 16 * u, dt, lane), rest, acc[dt]);
@@ -441,11 +447,12 @@ __device__ __forceinline__ void store_keys(const Args &a, const Keys &x, f32x16 
     store_rows<DT, D>(a.dv + row, dv, 1.0f);
 }
 
-// Four products a step of 32 tokens.  Same case as swa_dq: 320 to 340 us, 186 at the
+// Four products a step of 32 tokens.  Same case as swa_dq: 310 to 340 us, 186 at the
 // rate of a large product.  Each operand that a wave reads from LDS serves one matrix
 // instruction (its 32 keys are the other one): LDS is busy some 45 % of the time, the
 // matrix cores 35 %, and two waves a SIMD do not hide one behind the other wholly.
-template <int DT, int D> __global__ __launch_bounds__(64 * NW, DT == 1 ? 2 : 1) void swa_dkv(const Args a) {
+template <int DT, int D>
+__global__ __launch_bounds__(64 * NW, (DT == 1 ? (D == 64 ? 3 : 2) : 1)) void swa_dkv(const Args a) {
     extern __shared__ __align__(16) char smem[];
     typedef Tile<DT, D> TL;
     typedef typename Op<DT>::F F;
@@ -543,6 +550,12 @@ template <int DT, int D> __global__ __launch_bounds__(64 * NW, DT == 1 ? 2 : 1) 
                 for (int dt = 0; dt < NDT; ++dt) {
                     dv[dt] = Op<DT>::mma(TL::col(td, 16 * u, dt, lane), pf, dv[dt]);
                     dk[dt] = Op<DT>::mma(TL::col(tq, 16 * u, dt, lane), df, dk[dt]);
+                }
+                if (DT == 1 && th < FEW) {   // as in swa_dq; dk: 1.46 times its own rounding without, 1.31 with, 3 us of 44
+                    const F rest = rest16<DT>(dp, u, df);
+#pragma unroll
+                    for (int dt = 0; dt < NDT; ++dt)
+                        dk[dt] = Op<DT>::mma(TL::col(tq, 16 * u, dt, lane), rest, dk[dt]);
                 }
             }
         }

@@ -580,8 +580,8 @@ int hba_swa_bwd_workspace_bytes(int dtype, int64_t B, int64_t n, int64_t Hq, int
  * (contiguous) and lse, and the cotangent dout (element strides).  workspace:
  * 16-byte aligned, no initial contents.  Every sum runs in a fixed order, so
  * the gradients are the same bits from run to run.  bf16: the probabilities
- * and their gradients enter the products rounded to bf16 (those of dq's rows
- * with up to 256 keys in two bf16 parts), sums in fp32.
+ * and their gradients enter the products rounded to bf16 (in dq and dk
+ * those of the first 256 rows in two bf16 parts), sums in fp32.
  */
 int hba_swa_bwd(int dtype, const void *q, const int64_t q_strides[3], const void *k,
                 const int64_t k_strides[3], const void *v, const int64_t v_strides[3],
