@@ -255,7 +255,7 @@ class _Sliding(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, lens, window, sinks, scale):
-        fwd = ops.swa_fwd if torch.compiler.is_compiling() else ops._swa_fwd
+        fwd = ops._swa_fwd if ops._plain(q, k, v, lens) else ops.swa_fwd
         out, lse = fwd(q, k, v, lens, window, sinks, scale)
         ctx.save_for_backward(q, k, v, out, lse, lens)
         ctx.meta = (window, sinks, scale)
@@ -265,7 +265,7 @@ class _Sliding(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse, lens = ctx.saved_tensors
-        bwd = ops.swa_bwd if torch.compiler.is_compiling() else ops._swa_bwd
+        bwd = ops._swa_bwd if ops._plain(q, k, v, dout, lens) else ops.swa_bwd
         return (*bwd(q, k, v, out, lse, dout, lens, *ctx.meta), None, None, None, None)
 
 
@@ -279,12 +279,12 @@ def sliding_attention(q, k, v, window, sinks=0, scale=None, lens=None):
     [B]: rows at and past lens[b] are padding, whose output and gradients are
     0.  Returns a new tensor of q's shape and dtype; differentiable in q, k
     and v, with gradients that are the same bits from run to run."""
-    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    scale = float(q.shape[-1]) ** -0.5 if scale is None else float(scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _Sliding.apply(q, k, v, lens, int(window), int(sinks), scale)
-    if torch.compiler.is_compiling():
-        return ops.swa_fwd(q, k, v, lens, int(window), int(sinks), scale)[0]
-    return ops._swa_fwd(q, k, v, lens, int(window), int(sinks), scale, want_lse=False)[0]
+    if ops._plain(q, k, v, lens):
+        return ops._swa_fwd(q, k, v, lens, int(window), int(sinks), scale, want_lse=False)[0]
+    return ops.swa_fwd(q, k, v, lens, int(window), int(sinks), scale)[0]
 
 
 def hba_attention_eval(q, k, v, cos, sin, cfg, summ, qkn, cap=None, hier=False, equiv=False):

@@ -25,8 +25,9 @@ device.
     hba::paged_attn       attention of new tokens over the paged cache: decode and
                           parts of prompts, whole or windowed, shared first pages
 
-The last two also run without the dispatcher, under their plain Python names (a
-call through it costs some 20 us of host time).
+The last four run past the dispatcher where nothing but the call itself happens
+(_plain; a call through it costs some 20 us of host time), and through it
+wherever something records or transforms operators.
 """
 import ctypes
 from typing import Optional, Tuple
@@ -87,6 +88,25 @@ def _dev(t):
             check(lib().hba_device_check(), "hba_device_check")
         _CHECKED.add(idx)
     return t.device
+
+
+# What the dispatcher's thread state includes in an eager call.  Whatever records or
+# transforms operators adds a key to it: dispatch modes (make_fx, fake tensors,
+# counters), the jit tracer, vmap and the other function transforms.
+_keys = torch._C.DispatchKeySet
+_EAGER = (_keys(torch._C.DispatchKey.BackendSelect) | _keys(torch._C.DispatchKey.ADInplaceOrView)).raw_repr()
+_TENSORS = frozenset((Tensor, torch.nn.Parameter, type(None)))
+
+
+def _plain(*tensors):
+    """Whether a call with these tensors may go past the dispatcher: nothing would
+    see it there, and no tensor has a dispatch of its own.  (1.5 us.)"""
+    if torch.compiler.is_dynamo_compiling() or torch._C._dispatch_tls_local_include_set().raw_repr() & ~_EAGER:
+        return False
+    for t in tensors:
+        if type(t) not in _TENSORS:
+            return False
+    return True
 
 
 def _f32c(t, dev, n=None, what="tensor"):
@@ -929,23 +949,8 @@ def _pages(t, dt, dev, P, Hkv, width, what):
         raise ValueError(f"{what}: expected {P} pages of {Hkv} KV heads, {width} elements each")
 
 
-def kv_append_ragged(k, v, cu, k_gain, eps, cos, sin, page_table, seq_lens, kc_pages, kr_pages, v_pages, probes, proj,
-                     summ_pages):
-    """Append a ragged batch of tokens to the paged cache: tokens cu[s] ..
-    cu[s + 1] - 1 of k, v [T, Hkv, d] (raw; any strides) are the last ones of
-    sequence s, whose length seq_lens[s] counts them already, so they go to
-    positions seq_lens[s] - (cu[s + 1] - cu[s]) ...: QKNorm (k_gain None: none)
-    into kc_pages, its rotation at the position into kr_pages, v into v_pages,
-    and the summaries of every page that they fill into summ_pages.  kc_pages
-    and summ_pages (with probes and proj) may be None: a cache without the
-    unrotated keys or the summaries.  cu int32 [Bd + 1], page_table int32 [Bd,
-    max_pages], seq_lens int32 [Bd] on the device; cos/sin fp32 [n_tab, d].
-    Positions past the page table or the cos/sin tables, and tokens behind
-    cu[Bd] (a padded batch), are not appended; a page belongs to one sequence
-    while tokens are appended to it."""
-    if torch.compiler.is_compiling():
-        return torch.ops.hba.kv_append_ragged(k, v, cu, k_gain, eps, cos, sin, page_table, seq_lens, kc_pages,
-                                              kr_pages, v_pages, probes, proj, summ_pages)
+def _kv_append_ragged(k, v, cu, k_gain, eps, cos, sin, page_table, seq_lens, kc_pages, kr_pages, v_pages, probes, proj,
+                      summ_pages):
     dev = _dev(k)
     if k.dim() != 3 or v.shape != k.shape or v.dtype != k.dtype or v.device != dev:
         raise ValueError("k and v: expected two [T, Hkv, d] tensors of one type and device")
@@ -984,32 +989,38 @@ def kv_append_ragged(k, v, cu, k_gain, eps, cos, sin, page_table, seq_lens, kc_p
     check(st, "hba_kv_append_ragged")
 
 
+def kv_append_ragged(k, v, cu, k_gain, eps, cos, sin, page_table, seq_lens, kc_pages, kr_pages, v_pages, probes, proj,
+                     summ_pages):
+    """Append a ragged batch of tokens to the paged cache: tokens cu[s] ..
+    cu[s + 1] - 1 of k, v [T, Hkv, d] (raw; any strides) are the last ones of
+    sequence s, whose length seq_lens[s] counts them already, so they go to
+    positions seq_lens[s] - (cu[s + 1] - cu[s]) ...: QKNorm (k_gain None: none)
+    into kc_pages, its rotation at the position into kr_pages, v into v_pages,
+    and the summaries of every page that they fill into summ_pages.  kc_pages
+    and summ_pages (with probes and proj) may be None: a cache without the
+    unrotated keys or the summaries.  cu int32 [Bd + 1], page_table int32 [Bd,
+    max_pages], seq_lens int32 [Bd] on the device; cos/sin fp32 [n_tab, d].
+    Positions past the page table or the cos/sin tables, and tokens behind
+    cu[Bd] (a padded batch), are not appended; a page belongs to one sequence
+    while tokens are appended to it."""
+    args = (k, v, cu, k_gain, eps, cos, sin, page_table, seq_lens, kc_pages, kr_pages, v_pages, probes, proj, summ_pages)
+    if not _plain(k, v, cu, k_gain, cos, sin, page_table, seq_lens, kc_pages, kr_pages, v_pages, probes, proj, summ_pages):
+        return torch.ops.hba.kv_append_ragged(*args)
+    _kv_append_ragged(*args)
+
+
 @torch.library.custom_op("hba::kv_append_ragged", mutates_args=("kc_pages", "kr_pages", "v_pages", "summ_pages"),
                          device_types="cuda")
 def _kv_append_ragged_op(k: Tensor, v: Tensor, cu: Tensor, k_gain: Optional[Tensor], eps: float, cos: Tensor,
                          sin: Tensor, page_table: Tensor, seq_lens: Tensor, kc_pages: Optional[Tensor],
                          kr_pages: Tensor, v_pages: Tensor, probes: Optional[Tensor], proj: Optional[Tensor],
                          summ_pages: Optional[Tensor]) -> None:
-    kv_append_ragged(k, v, cu, k_gain, eps, cos, sin, page_table, seq_lens, kc_pages, kr_pages, v_pages, probes, proj,
-                     summ_pages)
+    _kv_append_ragged(k, v, cu, k_gain, eps, cos, sin, page_table, seq_lens, kc_pages, kr_pages, v_pages, probes, proj,
+                      summ_pages)
 
 
-def paged_attn(q, q_gain, eps, kr_pages, v_pages, page_table, seq_lens, cos, sin, scales, max_len, window=0, sinks=0,
-               cu=None, shared=0):
-    """Attention of each sequence's newest tokens over the paged cache (which
-    holds their keys already): q [T, Hq, d] raw, QKNorm (q_gain None: none),
-    the rotation at each token's position (cos None: none) and the logits'
-    scale scales[s] (fp32 [Bd]) applied in the kernel.  cu None: one token per
-    sequence, T = Bd; cu int32 [Bd + 1]: tokens cu[s] .. cu[s + 1] - 1 are the
-    last ones of sequence s.  The token at position i sees the keys j <= i;
-    with window > 0 those with j > i - window or j < sinks.  shared: the first
-    `shared` tokens (whole pages) are the same pages in every sequence; they
-    are read through page_table[0], once for the batch.  max_len bounds every
-    seq_lens[s] (a longer one is read as max_len).  Returns [T, Hq, d]; a
-    token that sees nothing, or is behind cu[Bd] (a padded batch), gives 0."""
-    if torch.compiler.is_compiling():
-        return torch.ops.hba.paged_attn(q, q_gain, eps, kr_pages, v_pages, page_table, seq_lens, cos, sin, scales,
-                                        max_len, window, sinks, cu, shared)
+def _paged_attn(q, q_gain, eps, kr_pages, v_pages, page_table, seq_lens, cos, sin, scales, max_len, window, sinks, cu,
+                shared):
     dev = _dev(q)
     if q.dim() != 3:
         raise ValueError("q: expected [T, Hq, d]")
@@ -1061,13 +1072,32 @@ def paged_attn(q, q_gain, eps, kr_pages, v_pages, page_table, seq_lens, cos, sin
     return out
 
 
+def paged_attn(q, q_gain, eps, kr_pages, v_pages, page_table, seq_lens, cos, sin, scales, max_len, window=0, sinks=0,
+               cu=None, shared=0):
+    """Attention of each sequence's newest tokens over the paged cache (which
+    holds their keys already): q [T, Hq, d] raw, QKNorm (q_gain None: none),
+    the rotation at each token's position (cos None: none) and the logits'
+    scale scales[s] (fp32 [Bd]) applied in the kernel.  cu None: one token per
+    sequence, T = Bd; cu int32 [Bd + 1]: tokens cu[s] .. cu[s + 1] - 1 are the
+    last ones of sequence s.  The token at position i sees the keys j <= i;
+    with window > 0 those with j > i - window or j < sinks.  shared: the first
+    `shared` tokens (whole pages) are the same pages in every sequence; they
+    are read through page_table[0], once for the batch.  max_len bounds every
+    seq_lens[s] (a longer one is read as max_len).  Returns [T, Hq, d]; a
+    token that sees nothing, or is behind cu[Bd] (a padded batch), gives 0."""
+    args = (q, q_gain, eps, kr_pages, v_pages, page_table, seq_lens, cos, sin, scales, max_len, window, sinks, cu, shared)
+    if not _plain(q, q_gain, kr_pages, v_pages, page_table, seq_lens, cos, sin, scales, cu):
+        return torch.ops.hba.paged_attn(*args)
+    return _paged_attn(*args)
+
+
 @torch.library.custom_op("hba::paged_attn", mutates_args=(), device_types="cuda")
 def _paged_attn_op(q: Tensor, q_gain: Optional[Tensor], eps: float, kr_pages: Tensor, v_pages: Tensor,
                    page_table: Tensor, seq_lens: Tensor, cos: Optional[Tensor], sin: Optional[Tensor],
                    scales: Tensor, max_len: int, window: int = 0, sinks: int = 0, cu: Optional[Tensor] = None,
                    shared: int = 0) -> Tensor:
-    return paged_attn(q, q_gain, eps, kr_pages, v_pages, page_table, seq_lens, cos, sin, scales, max_len, window,
-                      sinks, cu, shared)
+    return _paged_attn(q, q_gain, eps, kr_pages, v_pages, page_table, seq_lens, cos, sin, scales, max_len, window, sinks,
+                       cu, shared)
 
 
 @_paged_attn_op.register_fake

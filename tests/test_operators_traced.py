@@ -1,0 +1,128 @@
+"""The window and cache operators where something records or transforms what runs: a
+recorded graph holds the operator, not the memory of one call's result."""
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+from torch.fx.experimental.proxy_tensor import make_fx
+
+import hba_amd
+from hba_amd import ops
+
+EPS = 1e-6
+
+
+def window(q, k, v):
+    return hba_amd.sliding_attention(q, k, v, 20, 3)
+
+
+def cache(dev, dt=torch.bfloat16, seed=0):
+    """Two sequences of 5 and 100 tokens, 2 and 66 of them new: the arguments of both operators."""
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g).to(dt).to(dev)  # noqa: E731
+    i = lambda x: torch.tensor(x, dtype=torch.int32).to(dev)  # noqa: E731
+    cos, sin = (t.to(dev) for t in hba_amd.rope_tables(128, 64, 1e4, "cpu"))
+    return dict(k=r(68, 2, 64), v=r(68, 2, 64), cu=i([0, 2, 68]), cos=cos, sin=sin, table=i([[3, 0], [1, 2]]),
+                lens=i([5, 100]), kc=r(4, 2, 4096), kr=r(4, 2, 4096), vp=r(4, 2, 4096),
+                probes=r(2, 4, 64).float(), proj=r(2, 64, 64).float(), summ=r(4, 2, 4, 64), q=r(68, 4, 64),
+                gain=torch.ones(4).to(dev), scales=torch.full((2,), 1 / 64).to(dev))
+
+
+def append(a):
+    ops.kv_append_ragged(a["k"], a["v"], a["cu"], a["gain"][:2], EPS, a["cos"], a["sin"], a["table"], a["lens"],
+                         a["kc"], a["kr"], a["vp"], a["probes"], a["proj"], a["summ"])
+    return a["kr"]
+
+
+def attend(a):
+    return ops.paged_attn(a["q"], a["gain"], EPS, a["kr"], a["vp"], a["table"], a["lens"], a["cos"], a["sin"],
+                          a["scales"], 128, cu=a["cu"])
+
+
+def targets(g):
+    return [str(n.target) for n in g.graph.nodes if n.op == "call_function"]
+
+
+def test_eager_calls_go_past_the_dispatcher_and_nothing_else_does():
+    t = torch.zeros(2, 2)
+    assert ops._plain(t, None, torch.nn.Parameter(t))
+    for state in (torch.no_grad(), torch.inference_mode(), torch.autocast("cpu", dtype=torch.bfloat16)):
+        with state:
+            assert ops._plain(t)
+    seen = []
+
+    def f(x):
+        seen.append(ops._plain(x))
+        return x * 2
+
+    make_fx(f)(t)
+    make_fx(f, pre_dispatch=True)(t)
+    make_fx(f, tracing_mode="fake")(t)
+    torch.jit.trace(f, (t,), check_trace=False)
+    torch.func.vmap(f)(t)
+    torch.func.jvp(f, (t,), (t,))
+    torch.func.functionalize(f)(t)
+    with FakeTensorMode() as mode:
+        f(torch.zeros(2))
+    assert not any(seen) and len(seen) == 8
+    assert not ops._plain(mode.from_tensor(t))
+
+
+@pytest.mark.parametrize("pre", [False, True])
+def test_recorded_calls_of_tensors_without_memory(pre):
+    with FakeTensorMode():
+        q, k = torch.empty(1, 30, 4, 64, device="cuda"), torch.empty(1, 30, 2, 64, device="cuda")
+        assert window(q, k, k).shape == q.shape
+        assert "hba.swa_fwd.default" in targets(make_fx(window, pre_dispatch=pre)(q, k, k))
+        a = cache("cuda")
+        assert attend(a).shape == a["q"].shape and append(a) is a["kr"]
+        assert "hba.paged_attn.default" in targets(make_fx(attend, pre_dispatch=pre)(a))
+        assert "hba.kv_append_ragged.default" in targets(make_fx(append, pre_dispatch=pre)(a))
+
+
+def recorded(f, args, how):
+    return torch.jit.trace(f, args, check_trace=False) if how == "jit" else make_fx(f, pre_dispatch=how == "pre")(*args)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("how", ["fx", "pre", "jit"])
+def test_recorded_window(how):
+    x = [torch.randn(1, 70, h, 64, device="cuda") for h in (4, 2, 2)]
+    f = recorded(window, tuple(x), how)
+    for t in x:
+        t.normal_()
+    y = [torch.randn_like(t) for t in x]
+    for z in (x, y):
+        assert torch.equal(f(*z), window(*z))
+
+
+@pytest.mark.gpu
+def test_recorded_gradients():
+    x = [torch.randn(1, 70, h, 64, device="cuda") for h in (4, 2, 2, 4)]
+
+    def step(q, k, v, do):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        o = window(*leaves)
+        return (o.detach(), *torch.autograd.grad(o, leaves, do))
+
+    g = make_fx(step)(*x)
+    assert "hba.swa_fwd.default" in targets(g) and "hba.swa_bwd.default" in targets(g)
+    x = [torch.randn_like(t) for t in x]
+    assert all(torch.equal(a, b) for a, b in zip(g(*x), step(*x)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("how", ["fx", "pre", "jit"])
+def test_recorded_cache_calls(how):
+    names = list(cache("cpu"))
+
+    def both(*ts):
+        a = dict(zip(names, ts))
+        append(a)
+        return attend(a)
+
+    f = recorded(both, tuple(cache("cuda").values()), how)
+    a, b = cache("cuda", seed=1), cache("cuda", seed=1)
+    got, want = f(*a.values()), both(*b.values())
+    assert torch.equal(got, want)
+    assert all(torch.equal(a[n], b[n]) for n in ("kc", "kr", "vp", "summ"))
+    assert not torch.equal(a["kr"], cache("cuda", seed=1)["kr"])
