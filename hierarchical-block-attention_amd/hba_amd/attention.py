@@ -278,9 +278,9 @@ def sliding_attention(q, k, v, window, sinks=0, scale=None, lens=None):
     dim 64 or 128.  scale: of the logits, positive (default d ** -0.5).  lens
     [B]: rows at and past lens[b] are padding, whose output and gradients are
     0.  Returns a new tensor of q's shape and dtype; differentiable in q, k
-    and v, with gradients that are the same bits from run to run."""
+    and v (reverse mode), with gradients that are the same bits from run to run."""
     scale = float(q.shape[-1]) ** -0.5 if scale is None else float(scale)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if ops._differentiated(q, k, v):
         return _Sliding.apply(q, k, v, lens, int(window), int(sinks), scale)
     if ops._plain(q, k, v, lens):
         return ops._swa_fwd(q, k, v, lens, int(window), int(sinks), scale, want_lse=False)[0]

@@ -295,7 +295,7 @@ def cache_attention(q, cache, cfg, qkn, cos, sin, window=None, sinks=0, cu=None,
     the first `sinks`.  shared: tokens whose pages every sequence shares
     (PagedKVCache.share), read once for the batch.  max_len bounds the lengths
     (default: the longest one now, so a captured call that is to serve longer
-    ones gives it).  Returns [T, Hq, d]."""
+    ones gives it).  Returns [T, Hq, d]; there is no backward pass."""
     qg = qkn.q.gain if getattr(cfg, "qknorm", False) else None
     qeps = float(qkn.q.eps) if qg is not None else 1e-6
     if window is not None and window < 1:

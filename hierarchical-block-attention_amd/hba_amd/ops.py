@@ -34,6 +34,7 @@ from typing import Optional, Tuple
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from ._lib import BF16, F32, check, lib, strides3, used_strides2, used_strides3
 
@@ -95,18 +96,25 @@ def _dev(t):
 # counters), the jit tracer, vmap and the other function transforms.
 _keys = torch._C.DispatchKeySet
 _EAGER = (_keys(torch._C.DispatchKey.BackendSelect) | _keys(torch._C.DispatchKey.ADInplaceOrView)).raw_repr()
-_TENSORS = frozenset((Tensor, torch.nn.Parameter, type(None)))
+_ARGS = frozenset((Tensor, torch.nn.Parameter, type(None), int, float))
 
 
-def _plain(*tensors):
-    """Whether a call with these tensors may go past the dispatcher: nothing would
+def _plain(*args):
+    """Whether a call with these arguments may go past the dispatcher: nothing would
     see it there, and no tensor has a dispatch of its own.  (1.5 us.)"""
     if torch.compiler.is_dynamo_compiling() or torch._C._dispatch_tls_local_include_set().raw_repr() & ~_EAGER:
         return False
-    for t in tensors:
-        if type(t) not in _TENSORS:
-            return False
-    return True
+    return _ARGS.issuperset(map(type, args))
+
+
+def _differentiated(*tensors):
+    """Whether a derivative may be asked of a call: a tensor requires grad, or
+    forward-mode tangents are about (and perhaps on these)."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return forward_ad._current_level >= 0
 
 
 def _f32c(t, dev, n=None, what="tensor"):
@@ -1004,9 +1012,7 @@ def kv_append_ragged(k, v, cu, k_gain, eps, cos, sin, page_table, seq_lens, kc_p
     cu[Bd] (a padded batch), are not appended; a page belongs to one sequence
     while tokens are appended to it."""
     args = (k, v, cu, k_gain, eps, cos, sin, page_table, seq_lens, kc_pages, kr_pages, v_pages, probes, proj, summ_pages)
-    if not _plain(k, v, cu, k_gain, cos, sin, page_table, seq_lens, kc_pages, kr_pages, v_pages, probes, proj, summ_pages):
-        return torch.ops.hba.kv_append_ragged(*args)
-    _kv_append_ragged(*args)
+    (_kv_append_ragged if _plain(*args) else torch.ops.hba.kv_append_ragged)(*args)
 
 
 @torch.library.custom_op("hba::kv_append_ragged", mutates_args=("kc_pages", "kr_pages", "v_pages", "summ_pages"),
@@ -1084,11 +1090,25 @@ def paged_attn(q, q_gain, eps, kr_pages, v_pages, page_table, seq_lens, cos, sin
     `shared` tokens (whole pages) are the same pages in every sequence; they
     are read through page_table[0], once for the batch.  max_len bounds every
     seq_lens[s] (a longer one is read as max_len).  Returns [T, Hq, d]; a
-    token that sees nothing, or is behind cu[Bd] (a padded batch), gives 0."""
+    token that sees nothing, or is behind cu[Bd] (a padded batch), gives 0.
+    There is no backward pass: asking for one raises."""
     args = (q, q_gain, eps, kr_pages, v_pages, page_table, seq_lens, cos, sin, scales, max_len, window, sinks, cu, shared)
-    if not _plain(q, q_gain, kr_pages, v_pages, page_table, seq_lens, cos, sin, scales, cu):
-        return torch.ops.hba.paged_attn(*args)
-    return _paged_attn(*args)
+    if _differentiated(q, q_gain, kr_pages, v_pages, cos, sin, scales):
+        return _PagedAttn.apply(*args)
+    return (_paged_attn if _plain(*args) else torch.ops.hba.paged_attn)(*args)
+
+
+class _PagedAttn(torch.autograd.Function):
+    """paged_attn of tensors that a derivative may be asked for: there is none, and
+    neither a gradient nor a tangent is dropped without an error."""
+
+    @staticmethod
+    def forward(ctx, *args):
+        return (_paged_attn if _plain(*args) else torch.ops.hba.paged_attn)(*args)
+
+    @staticmethod
+    def backward(ctx, dout):
+        raise NotImplementedError("paged_attn has no backward pass")
 
 
 @torch.library.custom_op("hba::paged_attn", mutates_args=(), device_types="cuda")

@@ -3,6 +3,7 @@ recorded graph holds the operator, not the memory of one call's result."""
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
+from torch.autograd import forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 
 import hba_amd
@@ -126,3 +127,36 @@ def test_recorded_cache_calls(how):
     assert torch.equal(got, want)
     assert all(torch.equal(a[n], b[n]) for n in ("kc", "kr", "vp", "summ"))
     assert not torch.equal(a["kr"], cache("cuda", seed=1)["kr"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["q", "gain", "kr", "vp", "scales"])
+def test_cache_attention_says_that_it_has_no_gradient(name):
+    a = cache("cuda")
+    want = attend(a)
+    a[name].requires_grad_()
+    got = attend(a)
+    assert torch.equal(got, want) and got.requires_grad
+    with pytest.raises(NotImplementedError):
+        got.sum().backward()
+    with torch.no_grad():
+        assert not attend(a).requires_grad
+
+
+@pytest.mark.gpu
+def test_tangents_are_not_dropped():
+    a = cache("cuda")
+    q, k = torch.randn(1, 30, 4, 64, device="cuda"), torch.randn(1, 30, 2, 64, device="cuda")
+    want = window(q, k, k)
+    with forward_ad.dual_level():
+        assert torch.equal(window(q, k, k), want)
+        with pytest.raises(NotImplementedError):
+            window(forward_ad.make_dual(q, q), k, k)
+        with torch.no_grad(), pytest.raises(NotImplementedError):
+            window(q, k, forward_ad.make_dual(k, k))
+        with pytest.raises(NotImplementedError):
+            attend({**a, "q": forward_ad.make_dual(a["q"], a["q"])})
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda x: window(x, k, k), (q,), (q,))
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda x: attend({**a, "q": x}), (a["q"],), (a["q"],))
