@@ -1012,7 +1012,12 @@ def kv_append_ragged(k, v, cu, k_gain, eps, cos, sin, page_table, seq_lens, kc_p
     cu[Bd] (a padded batch), are not appended; a page belongs to one sequence
     while tokens are appended to it."""
     args = (k, v, cu, k_gain, eps, cos, sin, page_table, seq_lens, kc_pages, kr_pages, v_pages, probes, proj, summ_pages)
-    (_kv_append_ragged if _plain(*args) else torch.ops.hba.kv_append_ragged)(*args)
+    if not _plain(*args):
+        torch.ops.hba.kv_append_ragged(*args)
+        return
+    _kv_append_ragged(*args)
+    written = [t for t in (kc_pages, kr_pages, v_pages, summ_pages) if t is not None and not t.is_inference()]
+    torch.autograd.graph.increment_version(written)   # as the dispatcher does: autograd sees that they changed
 
 
 @torch.library.custom_op("hba::kv_append_ragged", mutates_args=("kc_pages", "kr_pages", "v_pages", "summ_pages"),
