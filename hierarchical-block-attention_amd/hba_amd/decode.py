@@ -193,18 +193,25 @@ class PagedKVCache:
         short = sum(max(0, (n + PAGE - 1) // PAGE - len(t)) for n, t in zip(lens, self._table))
         if short > len(self._free):
             raise RuntimeError("paged KV cache is out of pages")
-        if any([self._ensure_pages(s, n) for s, n in enumerate(lens)]):
+        taken = [self._ensure_pages(s, n) for s, n in enumerate(lens)]
+        if any(taken):
             rows = [t + [0] * (self.max_pages - len(t)) for t in self._table]
             self.page_table.copy_(torch.tensor(rows, dtype=torch.int32))
         # one transfer: the offsets, then the new lengths
         both = torch.tensor(cu + lens, dtype=torch.int32).to(self.kc_pages.device)
-        cu = both[:self.batch + 1]
-        self.seq_lens.copy_(both[self.batch + 1:])
+        cu, new_lens = both[:self.batch + 1], both[self.batch + 1:]
         cfg = self.cfg
         kg = qkn.k.gain if getattr(cfg, "qknorm", False) else None
         keps = float(qkn.k.eps) if kg is not None else 1e-6
-        ops.kv_append_ragged(k, v, cu, kg, keps, cos, sin, self.page_table, self.seq_lens, self.kc_pages,
-                             self.kr_pages, self.v_pages, summ.probes, summ.proj, self.summ_pages)
+        try:
+            ops.kv_append_ragged(k, v, cu, kg, keps, cos, sin, self.page_table, new_lens, self.kc_pages,
+                                 self.kr_pages, self.v_pages, summ.probes, summ.proj, self.summ_pages)
+        except Exception:                # refused: the cache is as it was
+            for s, pages in enumerate(taken):
+                del self._table[s][len(self._table[s]) - len(pages):]
+            self._free += [p for pages in reversed(taken) for p in reversed(pages)]
+            raise
+        self.seq_lens.copy_(new_lens)    # read by whatever is launched after the append
         self.lens = lens
         self._scales_ok = False
         return cu
