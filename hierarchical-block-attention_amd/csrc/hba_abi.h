@@ -18,6 +18,9 @@ inline bool aligned16(const void *p) { return (((uintptr_t)p) & 15u) == 0; }
 
 inline int64_t elem_size(int dtype) { return dtype == HBA_DTYPE_BF16 ? 2 : 4; }
 
+// A launch has fewer than 2^32 threads along its first dimension.
+inline bool launchable(int64_t blocks, int64_t threads) { return blocks <= 0xffffffffll / threads; }
+
 // Rows of a [B, n, H, d] view start on 16-byte boundaries.
 inline bool rows_aligned(int dtype, const void *p, const int64_t s[3]) {
     int64_t q = 16 / elem_size(dtype);

@@ -727,19 +727,27 @@ template <int DT, int D> static int launch(Args a, const Plan &p, hipStream_t s)
         a.slots = p.shares;
         a.part = p.own_pages;
         const int64_t nrows = (int64_t)a.T * a.Hq;
+        if (!abi::launchable(nrows, 256)) return HBA_ERR_UNSUPPORTED;
         hipLaunchKernelGGL((even_kernel<DT, D>), dim3((unsigned)p.shares), dim3(64 * DW), 0, s, a);
         HBA_LAUNCH_CHECK();
         hipLaunchKernelGGL((join_kernel<DT, D, 1024 / D, true>), dim3((unsigned)nrows), dim3(256), 0, s, a, nrows);
         HBA_LAUNCH_CHECK();
         return HBA_OK;
     }
+    const int64_t nrows = (int64_t)a.T * a.Hq, nshared = p.ptiles * a.Hkv * p.prefix;
+    constexpr int SG = 1024 / D, RB = 1024 / D;   // parts at a time, or rows, of a join's workgroup
+    const int64_t joins = a.slots > 8 ? nrows : (nrows + RB - 1) / RB;
+    const bool fits = a.cu ? abi::launchable(p.tiles, 64 * rows::NW)
+                    : p.prefix ? abi::launchable(nshared + groups * p.own, 64 * rows::NW)
+                               : abi::launchable(groups, 64 * DW);
+    if (!fits || (a.slots > 1 && !abi::launchable(joins, 256)))
+        return HBA_ERR_UNSUPPORTED;
     Args own = a;
     own.slot0 = p.prefix;
     own.part = p.own_pages;
     a.part = p.prefix_pages;
     if (p.prefix && !a.cu) {
-        const int64_t nshared = p.ptiles * a.Hkv * p.prefix, grid = nshared + groups * p.own;
-        if (grid > 0x7fffffff) return HBA_ERR_UNSUPPORTED;
+        const int64_t grid = nshared + groups * p.own;
         constexpr size_t both = lds > sizeof(DecodeLds<D>) ? lds : sizeof(DecodeLds<D>);
         hipLaunchKernelGGL((shared_kernel<DT, D>), dim3((unsigned)grid), dim3(64 * rows::NW), both, s, a, own,
                            (int)p.ptiles, (int)nshared, (int)groups);
@@ -758,13 +766,10 @@ template <int DT, int D> static int launch(Args a, const Plan &p, hipStream_t s)
     }
     HBA_LAUNCH_CHECK();
     if (a.slots > 1) {
-        const int64_t nrows = (int64_t)a.T * a.Hq;
-        constexpr int SG = 1024 / D, RB = 1024 / D;   // parts at a time, or rows
         if (a.slots > 8)
-            hipLaunchKernelGGL((join_kernel<DT, D, SG, false>), dim3((unsigned)nrows), dim3(256), 0, s, a, nrows);
+            hipLaunchKernelGGL((join_kernel<DT, D, SG, false>), dim3((unsigned)joins), dim3(256), 0, s, a, nrows);
         else
-            hipLaunchKernelGGL((join_kernel<DT, D, 1, false>), dim3((unsigned)((nrows + RB - 1) / RB)), dim3(256), 0, s, a,
-                               nrows);
+            hipLaunchKernelGGL((join_kernel<DT, D, 1, false>), dim3((unsigned)joins), dim3(256), 0, s, a, nrows);
         HBA_LAUNCH_CHECK();
     }
     return HBA_OK;

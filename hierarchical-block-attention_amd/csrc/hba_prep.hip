@@ -1181,7 +1181,7 @@ extern "C" int hba_kv_append_ragged(int dtype, const void *k, const int64_t k_st
     a.summ = (char *)summ_pages;
     // c tokens touch at most c and at most c / 64 + 2 pages
     const int64_t slots = T < T / 64 + 2 * Bd ? T : T / 64 + 2 * Bd;
-    if ((slots + 7) / 8 * 8 * Hkv > 0x7fffffff) return HBA_ERR_UNSUPPORTED;
+    if (!abi::launchable((slots + 7) / 8 * 8 * Hkv, 256)) return HBA_ERR_UNSUPPORTED;
     const dim3 grid((unsigned)((slots + 7) / 8 * 8 * Hkv));
 #define HBA_APPR(DT, D)                                                                                       \
     do {                                                                                                      \

@@ -37,6 +37,7 @@ struct Args {
     float *part;                        // dk / dv sums of tiles in several parts
     int32_t *marks;                     // waves of swa_dkv whose sums are not finite
     int nst, Ps, Pn, schunk, chunk;     // tiles of sinks, parts of those and of the others, steps of a part of either
+    int first;                          // swa_join: place of the launch's first workgroup
 };
 
 __device__ __forceinline__ int seq_len(const Args &a, int b) {
@@ -577,8 +578,9 @@ constexpr int JE = 1024;
 template <int DT, int D> __global__ __launch_bounds__(JE / 4) void swa_join(const Args a) {
     typedef typename St<DT>::T T;
     constexpr int PER = KB * 2 * D / JE, ESZ = Tile<DT, D>::ESZ;
-    const int e = blockIdx.x % PER * JE + threadIdx.x * 4, r = e / (2 * D), x = e % (2 * D), xd = x % D;
-    const int combo = blockIdx.x / PER % a.Cn, tile = blockIdx.x / PER / a.Cn;
+    const int place = a.first + blockIdx.x;
+    const int e = place % PER * JE + threadIdx.x * 4, r = e / (2 * D), x = e % (2 * D), xd = x % D;
+    const int combo = place / PER % a.Cn, tile = place / PER / a.Cn;
     const int P = tile < a.nst ? a.Ps : a.Pn;
     const int slot = tile < a.nst ? tile * a.Ps : a.nst * a.Ps + (tile - a.nst) * a.Pn;
     const int b = combo / a.Hkv, g = combo % a.Hkv, len = seq_len(a, b), k0 = tile * KB, j = k0 + r;
@@ -724,9 +726,14 @@ template <int DT, int D> static int launch_bwd(Args a, int64_t grid, const Cut &
     a.ntiles = c.ntiles;
     hipLaunchKernelGGL((swa_dkv<DT, D>), dim3((unsigned)(c.slots * a.Cn)), dim3(64 * NW), ldk, s, a);
     HBA_LAUNCH_CHECK();
-    hipLaunchKernelGGL((swa_join<DT, D>), dim3((unsigned)((int64_t)c.ntiles * a.Cn * (KB * 2 * D / JE))), dim3(JE / 4),
-                       0, s, a);
-    HBA_LAUNCH_CHECK();
+    // 16 or 32 workgroups a key tile: more than a launch takes from 2^20 or 2^19 tiles on
+    const int64_t places = (int64_t)c.ntiles * a.Cn * (KB * 2 * D / JE), most = 1 << 23;
+    for (int64_t at = 0; at < places; at += most) {
+        a.first = (int)at;
+        hipLaunchKernelGGL((swa_join<DT, D>), dim3((unsigned)(places - at < most ? places - at : most)), dim3(JE / 4), 0,
+                           s, a);
+        HBA_LAUNCH_CHECK();
+    }
     return HBA_OK;
 }
 
@@ -745,6 +752,7 @@ static int check(int dtype, int64_t B, int64_t n, int64_t Hq, int64_t Hkv, int64
     // rows, steps and workgroups are counted in 32 bits
     if (n > (1 << 28) || n * (Hq / Hkv) > 0x7fffff00 || B * Hq * ((n + 31) / 32 + 8) > 0x7fffffff)
         return HBA_ERR_UNSUPPORTED;
+    if (!abi::launchable(B * Hkv * ((n * (Hq / Hkv) + RT - 1) / RT) + 8, 64 * NW)) return HBA_ERR_UNSUPPORTED;
     return HBA_OK;
 }
 
@@ -863,7 +871,7 @@ extern "C" int hba_swa_bwd(int dtype, const void *q, const int64_t q_strides[3],
     a.Pn = c.Pn;
     a.schunk = c.schunk;
     a.chunk = c.chunk;
-    if (c.slots * a.Cn * rows::NW > 0x7fffffff ||
+    if (!abi::launchable(c.slots * a.Cn, 64 * rows::NW) || c.slots * a.Cn * rows::NW > 0x7fffffff ||
         (int64_t)c.ntiles * a.Cn * (swa::KB * 2 * d / swa::JE) > 0x7fffffff)
         return HBA_ERR_UNSUPPORTED;
     int st = HBA_OK;

@@ -1,11 +1,16 @@
 """Calls of the window and cache operators at the edges of what their documentation
 allows: state after an error, lengths of any type, launches of any size, pages with
 anything behind their sequences, and every form that the gradients' kernels take."""
+import ctypes
+
 import pytest
 import torch
 
 import hba_amd
+import test_gpu_swa as swa
+import test_window_and_cache_host as host
 import test_gpu_append_ragged as ragged
+from attn64 import assert_within, sliding, unit
 from test_gpu_append_ragged import append
 
 
@@ -64,3 +69,34 @@ def test_extend_goes_on_after_a_refusal():
     assert a.lens == a.seq_lens.tolist() == b.lens and a._table == b._table
     for n in ("kc_pages", "kr_pages", "v_pages", "summ_pages", "page_table"):
         assert torch.equal(getattr(a, n), getattr(b, n))
+
+
+def test_launches_of_too_many_threads_are_refused():
+    """A launch has fewer than 2^32 threads; what needs more is refused before any of its work."""
+    s3 = (ctypes.c_int64 * 3)(64, 64, 64)
+    assert host.swa(B=1 << 24, n=1, Hq=1, Hkv=1, st=s3, kst=s3) == -2
+    assert host.paged(T=1 << 23, Bd=1 << 23, Hq=1, Hkv=1, max_len=64, maxp=1) == -2
+    assert host.paged(T=1 << 27, Bd=1, Hq=8, Hkv=8, max_len=128, shared=1, maxp=2, cu=host.FAKE, nbytes=1 << 62) == -2
+    assert host.append(T=1 << 24, Bd=1 << 24, Hkv=1) == -2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,d,Hkv", [("bf16", 64, 16), ("f32", 128, 8)])
+def test_gradients_of_a_million_heads(dt, d, Hkv):
+    """More key tiles than one launch joins; the keys that a NaN of another token's query
+    spoils, which only the join computes, are those of the first and the last launch."""
+    B, n = 65536, 3
+    q, k, v, do = swa.make(swa.DT[dt], 4, n, Hkv, Hkv, d)
+    x = [torch.empty(B, n, Hkv, d, dtype=swa.DT[dt], device="cuda") for _ in range(4)]
+    at = torch.tensor([0, 1, B // 2, B - 1])
+    for t, rows in zip(x, (q, k, v, do)):
+        t[:] = rows[1].cuda()
+        t[at] = rows.cuda()
+    clean = [t.clone() for t in (q, k, v, do)]
+    for b in range(4):
+        x[0][at[b], 0] = float("nan")
+    got = swa.run(*x[:3], 1, 0, dout=x[3])
+    want, bound = sliding(*clean[:3], 1, 0, d ** -0.5, None, unit(swa.DT[dt]), clean[3])
+    for name, a, w, c in zip(("out", "dq", "dk", "dv"), got, want, bound):
+        assert_within(a[at][:, 1:].cpu(), w[:, 1:], c[:, 1:], name)
+        assert torch.equal(a[2:100], a[2:3].expand(98, -1, -1, -1)), name
