@@ -618,8 +618,10 @@ def _swa_args(q, k, v, lens, window, sinks, scale):
     if not 0.0 < scale < float("inf"):
         raise ValueError(f"scale must be positive and finite, got {scale}")
     if lens is not None:
-        if tuple(lens.shape) != (B,) or lens.dtype.is_floating_point or lens.dtype == torch.bool:
+        if tuple(lens.shape) != (B,) or lens.dtype.is_floating_point or lens.dtype.is_complex or lens.dtype == torch.bool:
             raise ValueError(f"lens: expected {B} whole numbers")
+        if lens.dtype != torch.int32:    # before 32 bits wrap it
+            lens = lens.to(dtype=torch.int64).clamp(-1, n)
         lens = lens.to(device=dev, dtype=torch.int32).contiguous()
     return dev, B, n, Hq, Hkv, d, lens
 

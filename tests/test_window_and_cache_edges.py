@@ -100,3 +100,24 @@ def test_gradients_of_a_million_heads(dt, d, Hkv):
     for name, a, w, c in zip(("out", "dq", "dk", "dv"), got, want, bound):
         assert_within(a[at][:, 1:].cpu(), w[:, 1:], c[:, 1:], name)
         assert torch.equal(a[2:100], a[2:3].expand(98, -1, -1, -1)), name
+
+
+@pytest.mark.gpu
+def test_lengths_of_every_type():
+    """Lengths are taken as the numbers they are, past 32 bits too."""
+    q, k, v, do = swa.make(torch.bfloat16, 4, 200, 4, 2, 64, seed=3)
+    x = [t.cuda().requires_grad_() for t in (q, k, v)]
+
+    def run(lens):
+        o = hba_amd.sliding_attention(*x, 70, 5, lens=lens)
+        return (o.detach(), *torch.autograd.grad(o, x, do.cuda()))
+
+    want = run(torch.tensor([200, 0, 130, 200], dtype=torch.int32).cuda())
+    big = torch.tensor([2 ** 32 + 7, -2 ** 32 + 50, 130, 2 ** 31])
+    for lens in (big.cuda(), big):
+        assert all(torch.equal(a, b) for a, b in zip(run(lens), want))
+    for dt in (torch.uint8, torch.int16, torch.int64):
+        lens = torch.tensor([200, 0, 130, 200], dtype=dt).cuda()
+        assert all(torch.equal(a, b) for a, b in zip(run(lens), want))
+    with pytest.raises(ValueError):
+        run(torch.ones(4, dtype=torch.complex64).cuda())
