@@ -654,8 +654,8 @@ def _swa_bwd(q, k, v, out, lse, dout, lens, window, sinks, scale):
     dq = torch.empty(B, n, Hq, d, dtype=q.dtype, device=dev)
     dk = torch.empty(B, n, Hkv, d, dtype=q.dtype, device=dev)
     dv = torch.empty_like(dk)
-    if dq.numel() == 0:
-        return dq, dk, dv
+    if dq.numel() == 0:      # no queries: nothing reaches the keys
+        return dq, dk.zero_(), dv.zero_()
     W, S = min(window, n), min(sinks, n)
     q, k, v, dout, out, lse = _rows16(q), _rows16(k), _rows16(v), _rows16(dout), _c16(out), lse.contiguous()
     nbytes = ctypes.c_size_t(0)

@@ -121,3 +121,14 @@ def test_lengths_of_every_type():
         assert all(torch.equal(a, b) for a, b in zip(run(lens), want))
     with pytest.raises(ValueError):
         run(torch.ones(4, dtype=torch.complex64).cuda())
+
+
+@pytest.mark.gpu
+def test_no_query_heads():
+    """Keys without a query have gradients of 0."""
+    q, k = torch.empty(2, 50, 0, 64, device="cuda"), torch.randn(2, 50, 2, 64, device="cuda").requires_grad_()
+    torch.full((4, 50, 2, 64), float("nan"), device="cuda")       # the gradients' memory, perhaps
+    out = hba_amd.sliding_attention(q, k, k * 2, 5)
+    assert out.shape == q.shape
+    out.sum().backward()
+    assert not k.grad.any()
