@@ -70,7 +70,7 @@ template <> struct Op<1> {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
     }
     // the probabilities enter the product in bf16, as the matrix cores take them: a
-    // relative 2^-9 each, which averages out over a row's keys
+    // relative 2^-8 each at most, which averages out over a row's keys
     static __device__ __forceinline__ F pack(const float (&x)[8]) {
         F r;
 #pragma unroll
@@ -364,6 +364,7 @@ struct Sees {
 template <int DT, int D> struct RowAcc {
     f32x16 O[D / 32];
     float m, l;       // running maximum (log2 units; -inf: nothing seen yet), and this half's part of the sum
+    float le;         // that part before the operands' rounding, of attend<.., SEP> only (else it is l)
 };
 
 // Stages the first of tiles it0 .. it1 - 1 of a list (tile it < ns: sinks, tile it;
@@ -383,7 +384,10 @@ __device__ __forceinline__ void attend_begin(Src &src, char *smem, int it0, int 
 // products then start from -m instead of 0.  Every wave of the workgroup calls
 // it; it leaves no wave reading LDS.
 // ONE: of each tile the wave takes the 32 keys `which` only (another one has the rest).
-template <int DT, int D, bool LO, bool ONE = false, class Src>
+// SEP: the sum of the probabilities as they are, too.  O is divided by the sum of the
+// rounded ones, which its own weights are; a log-sum-exp from that would put a row's
+// gradients off by up to a bf16 rounding (2^-8) in common.
+template <int DT, int D, bool LO, bool ONE = false, bool SEP = false, class Src>
 __device__ __forceinline__ void attend(Src &src, char *smem, const typename Op<DT>::F (&q)[D / 16],
                                        const typename Op<DT>::F *qlo, float c, int it0, int it1, int ns, int wt0,
                                        const Sees &w, RowAcc<DT, D> &a, int which = 0) {
@@ -394,7 +398,7 @@ __device__ __forceinline__ void attend(Src &src, char *smem, const typename Op<D
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) a.O[dt] = zero;
     a.m = -INFINITY;
-    a.l = 0.0f;
+    a.l = a.le = 0.0f;
     float shift = 0.0f;   // -m, or 0 while nothing is seen
     const uint32_t lds = lds_offset(smem);
     const auto tile = [&](int it) { return it < ns ? it : wt0 + it - ns; };
@@ -429,21 +433,28 @@ __device__ __forceinline__ void attend(Src &src, char *smem, const typename Op<D
             }
             // probabilities 2^(c s + by) as operands, and this half's sum of them
             F p[2];
+            struct Sums {
+                float rounded, whole;
+            };
             const auto weights = [&](float by) {
-                float sum = 0.0f;
+                Sums sum = {0.0f, 0.0f};
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     float x[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
                         x[e] = ex2(LO ? s[8 * u + e] : fmaf(s[8 * u + e], c, by));
+                    if constexpr (SEP) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) sum.whole += x[e];
+                    }
                     p[u] = Op<DT>::pack(x);
-                    sum = Op<DT>::sum(p[u], sum);
+                    sum.rounded = Op<DT>::sum(p[u], sum.rounded);
                 }
                 return sum;
             };
-            float sum = weights(shift);
-            if (__ballot(!(sum <= MOST) || a.m == -INFINITY)) {   // a new maximum
+            Sums sum = weights(shift);
+            if (__ballot(!(sum.rounded <= MOST) || a.m == -INFINITY)) {   // a new maximum
                 float mx = s[0];
 #pragma unroll
                 for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[r]);
@@ -451,6 +462,7 @@ __device__ __forceinline__ void attend(Src &src, char *smem, const typename Op<D
                 mx = fmaxf(a.m, LO ? mx - shift : mx * c);
                 const float al = a.m == -INFINITY ? 0.0f : ex2(a.m - mx);   // nothing to rescale yet
                 a.l *= al;
+                if constexpr (SEP) a.le *= al;
 #pragma unroll
                 for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
@@ -461,7 +473,8 @@ __device__ __forceinline__ void attend(Src &src, char *smem, const typename Op<D
                 shift = by;
                 sum = weights(shift);
             }
-            a.l += sum;
+            a.l += sum.rounded;
+            if constexpr (SEP) a.le += sum.whole;
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll

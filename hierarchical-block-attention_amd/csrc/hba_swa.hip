@@ -105,8 +105,9 @@ __device__ __forceinline__ DenseKV<DT, D, KT> keys(const Args &a, const Rows &x)
     return s;
 }
 
+// l: the sum that O is divided by, le: the one of the log-sum-exp.
 template <int DT, int D>
-__device__ __forceinline__ void store_fwd(const Args &a, const Rows &x, RowAcc<DT, D> &acc, float l) {
+__device__ __forceinline__ void store_fwd(const Args &a, const Rows &x, RowAcc<DT, D> &acc, float l, float le) {
     if (!x.in) return;
     if (!x.valid) {   // a row behind its sequence: 0
 #pragma unroll
@@ -115,7 +116,7 @@ __device__ __forceinline__ void store_fwd(const Args &a, const Rows &x, RowAcc<D
     const int64_t row = ((int64_t)x.b * a.n + x.tok) * a.Hq + x.head;
     store_rows<DT, D>(a.out + row * D * Tile<DT, D>::ESZ, acc.O, x.valid ? 1.0f / l : 0.0f);
     if (a.lse && (threadIdx.x & 32) == 0)
-        a.lse[((int64_t)x.b * a.Hq + x.head) * a.n + x.tok] = x.valid ? acc.m + __log2f(l) : INFINITY;
+        a.lse[((int64_t)x.b * a.Hq + x.head) * a.n + x.tok] = x.valid ? acc.m + __log2f(le) : INFINITY;
 }
 
 template <int DT, int D>
@@ -132,8 +133,10 @@ __device__ __forceinline__ const char *dout_row(const Args &a, const Rows &x) {
 // and as many multiply-adds and conversions a lane stand beside 8 matrix
 // instructions (without the exponentials 144 us, without reading operands from LDS
 // 150).  fp32, 2 x 2047 tokens, W = 512: 80 to 89 us, 37 at the fp32 matrix rate.
-template <int DT, int D>
-__global__ __launch_bounds__(64 * NW, (DT == 1 && D == 64 ? 3 : WAVES<DT, D>)) void swa_fwd(const Args a) {
+// SEP: the log-sum-exp has a sum of its own (see attend): 155 us at 8192 tokens, 28
+// heads, d = 128 with three waves per SIMD, 179 with two, 152 without it.
+template <int DT, int D, bool SEP>
+__global__ __launch_bounds__(64 * NW, (DT == 1 ? 3 : WAVES<DT, D>)) void swa_fwd(const Args a) {
     extern __shared__ __align__(16) char smem[];
     Rows x;
     if (!find_rows<D>(a, x)) return;
@@ -144,13 +147,13 @@ __global__ __launch_bounds__(64 * NW, (DT == 1 && D == 64 ? 3 : WAVES<DT, D>)) v
     typename Op<DT>::F q[D / 16];
     load_rows<DT, D>(q_row<DT, D>(a, x), x.valid, q);
     RowAcc<DT, D> acc;
-    attend<DT, D, false>(src, smem, q, nullptr, a.c, 0, nt, ns, wt0, x.w, acc);
-    float l = acc.l + other_half(acc.l);
+    attend<DT, D, false, false, SEP>(src, smem, q, nullptr, a.c, 0, nt, ns, wt0, x.w, acc);
+    float l = acc.l + other_half(acc.l), le = SEP ? acc.le + other_half(acc.le) : l;
     if (__ballot(x.valid && (any_bad<D>(acc.O) || !finite(l)))) {
         attend_each<DT, D, false>(src, q, nullptr, a.c, 0, nt, ns, wt0, x.w, acc);
-        l = acc.l + other_half(acc.l);
+        le = l = acc.l + other_half(acc.l);
     }
-    store_fwd<DT, D>(a, x, acc, l);
+    store_fwd<DT, D>(a, x, acc, l, le);
 }
 
 // swa_fwd where its workgroups leave CUs free: 8 waves of which `sets` have the same
@@ -160,11 +163,12 @@ __global__ __launch_bounds__(64 * NW, (DT == 1 && D == 64 ? 3 : WAVES<DT, D>)) v
 // of each.  1001 tokens, 14 heads, W = 1024, d = 64: 20 us as one set (110 workgroups),
 // 17 as two, 13 as four (220); fp32 75, 72 and 42; d = 128 25 as two and 19 as four.
 template <int DT, int D, int SETS> using SetsKV = DenseKV<DT, D, (SETS == 4 ? 64 : KEYS<DT, D>)>;
-template <int DT, int D, int SETS> constexpr size_t sets_lds() {
-    constexpr size_t tiles = 4 * SetsKV<DT, D, SETS>::BYTES, sums = (size_t)(SETS - 1) * 512 / SETS * (D / 2 + 2) * 4;
+template <int DT, int D, int SETS, bool SEP> constexpr size_t sets_lds() {
+    constexpr size_t tiles = 4 * SetsKV<DT, D, SETS>::BYTES,
+                     sums = (size_t)(SETS - 1) * 512 / SETS * (D / 2 + 2 + SEP) * 4;
     return tiles > sums ? tiles : sums;
 }
-template <int DT, int D, int SETS> __global__ __launch_bounds__(512) void swa_fwd_sets(const Args a) {
+template <int DT, int D, int SETS, bool SEP> __global__ __launch_bounds__(512) void swa_fwd_sets(const Args a) {
     extern __shared__ __align__(16) char smem[];
     constexpr int R = 8 / SETS, T = 64 * R;   // waves, lanes of a set
     Rows x;
@@ -181,7 +185,7 @@ template <int DT, int D, int SETS> __global__ __launch_bounds__(512) void swa_fw
     typename Op<DT>::F q[D / 16];
     load_rows<DT, D>(q_row<DT, D>(a, x), x.valid, q);
     RowAcc<DT, D> acc;
-    attend<DT, D, false, SETS == 4>(src, mine, q, nullptr, a.c, it0, it1, ns, wt0, x.w, acc, set % 2);
+    attend<DT, D, false, SETS == 4, SEP>(src, mine, q, nullptr, a.c, it0, it1, ns, wt0, x.w, acc, set % 2);
     if (it1 - it0 < mid) __syncthreads();   // the other half's last tile: as many barriers for both
     // element i of set s: sums[(i (SETS - 1) + s - 1) T]
     float *sums = reinterpret_cast<float *>(smem) + threadIdx.x % T;
@@ -194,6 +198,7 @@ template <int DT, int D, int SETS> __global__ __launch_bounds__(512) void swa_fw
             for (int r = 0; r < 16; ++r) sums[(16 * dt + r) * E] = acc.O[dt][r];
         sums[D / 2 * E] = acc.m;
         sums[(D / 2 + 1) * E] = acc.l;
+        if constexpr (SEP) sums[(D / 2 + 2) * E] = acc.le;
     }
     __syncthreads();
     if (set) return;
@@ -203,17 +208,18 @@ template <int DT, int D, int SETS> __global__ __launch_bounds__(512) void swa_fw
         const float fa = acc.m == -INFINITY ? 0.0f : ex2(acc.m - m), fb = om == -INFINITY ? 0.0f : ex2(om - m);
         acc.m = m;
         acc.l = fmaf(sums[(D / 2 + 1) * E], fb, acc.l * fa);
+        if constexpr (SEP) acc.le = fmaf(sums[(D / 2 + 2) * E], fb, acc.le * fa);
 #pragma unroll
         for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc.O[dt][r] = fmaf(sums[(16 * dt + r) * E], fb, acc.O[dt][r] * fa);
     }
-    float l = acc.l + other_half(acc.l);
+    float l = acc.l + other_half(acc.l), le = SEP ? acc.le + other_half(acc.le) : l;
     if (__ballot(x.valid && (any_bad<D>(acc.O) || !finite(l)))) {
         attend_each<DT, D, false>(src, q, nullptr, a.c, 0, nt, ns, wt0, x.w, acc);
-        l = acc.l + other_half(acc.l);
+        le = l = acc.l + other_half(acc.l);
     }
-    store_fwd<DT, D>(a, x, acc, l);
+    store_fwd<DT, D>(a, x, acc, l, le);
 }
 
 // The probabilities' gradient from the forward's log-sum-exps, and dq; delta =
@@ -690,13 +696,14 @@ template <int DT, int D, class K> static int lds_room(K kern, size_t bytes) {
                : HBA_ERR_LAUNCH;
 }
 
-template <int DT, int D, int SETS> static int launch_sets(const Args &a, int64_t grid, hipStream_t s) {
-    if (int st = lds_room<DT, D>(swa_fwd_sets<DT, D, SETS>, sets_lds<DT, D, SETS>())) return st;
-    hipLaunchKernelGGL((swa_fwd_sets<DT, D, SETS>), dim3((unsigned)grid), dim3(512), (sets_lds<DT, D, SETS>()), s, a);
+template <int DT, int D, int SETS, bool SEP> static int launch_sets(const Args &a, int64_t grid, hipStream_t s) {
+    constexpr size_t lds = sets_lds<DT, D, SETS, SEP>();
+    if (int st = lds_room<DT, D>(swa_fwd_sets<DT, D, SETS, SEP>, lds)) return st;
+    hipLaunchKernelGGL((swa_fwd_sets<DT, D, SETS, SEP>), dim3((unsigned)grid), dim3(512), lds, s, a);
     HBA_LAUNCH_CHECK();
     return HBA_OK;
 }
-template <int DT, int D> static int launch_fwd(const Args &a, int64_t grid, hipStream_t s) {
+template <int DT, int D, bool SEP> static int launch_fwd(const Args &a, int64_t grid, hipStream_t s) {
     constexpr size_t lds = 2 * DenseKV<DT, D>::BYTES;
     if constexpr (WAVES<DT, D> >= 2) {   // 8 waves on a CU
         // What the meeting costs, in keys: 300 tokens, d = 64, W = 64, 128 and 256 take 7.8, 8.6 and 9.7 us as one
@@ -707,11 +714,11 @@ template <int DT, int D> static int launch_fwd(const Args &a, int64_t grid, hipS
         int64_t more;
         b.ntiles = (int)(((int64_t)a.n * a.G + 63) / 64);
         b.xmap = xcd_pick(b.Cn, b.ntiles, more);
-        if (more <= 256 && seen >= 128) return launch_sets<DT, D, 4>(b, more, s);
-        if (grid <= 256 && seen >= 256) return launch_sets<DT, D, 2>(a, grid, s);
+        if (more <= 256 && seen >= 128) return launch_sets<DT, D, 4, SEP>(b, more, s);
+        if (grid <= 256 && seen >= 256) return launch_sets<DT, D, 2, SEP>(a, grid, s);
     }
-    if (int st = lds_room<DT, D>(swa_fwd<DT, D>, lds)) return st;
-    hipLaunchKernelGGL((swa_fwd<DT, D>), dim3((unsigned)grid), dim3(64 * NW), lds, s, a);
+    if (int st = lds_room<DT, D>(swa_fwd<DT, D, SEP>, lds)) return st;
+    hipLaunchKernelGGL((swa_fwd<DT, D, SEP>), dim3((unsigned)grid), dim3(64 * NW), lds, s, a);
     HBA_LAUNCH_CHECK();
     return HBA_OK;
 }
@@ -795,7 +802,9 @@ extern "C" int hba_swa_fwd(int dtype, const void *q, const int64_t q_strides[3],
     a.out = (char *)out;
     a.lse = lse;
     int st = HBA_OK;
-#define HBA_SWA(DT, D) st = swa::launch_fwd<DT, D>(a, grid, (hipStream_t)stream)
+#define HBA_SWA(DT, D)                                                                       \
+    st = lse && DT == 1 ? swa::launch_fwd<DT, D, DT == 1>(a, grid, (hipStream_t)stream)      \
+                        : swa::launch_fwd<DT, D, false>(a, grid, (hipStream_t)stream)
     HBA_DISPATCH_DT_D(dtype, d, HBA_SWA);
 #undef HBA_SWA
     return st;

@@ -7,10 +7,12 @@ import pytest
 import torch
 
 import hba_amd
+import test_gpu_paged_attn as paged
 import test_gpu_swa as swa
 import test_window_and_cache_host as host
 import test_gpu_append_ragged as ragged
-from attn64 import assert_within, sliding, unit
+from attn64 import E, assert_within, attend, sliding, unit, visible
+from hba_amd.decode import key_offsets, value_offsets
 from test_gpu_append_ragged import append
 
 
@@ -132,3 +134,71 @@ def test_no_query_heads():
     assert out.shape == q.shape
     out.sum().backward()
     assert not k.grad.any()
+
+
+# Batches whose key tiles are cut into (parts of a tile with sinks, parts of the others):
+# every form that swa_dkv and swa_join take beside the one of small grids, several and several
+CUTS = [("f32", 64, "one, one", 600, 130, 4, 2, 40, 3), ("f32", 128, "one, one", 600, 130, 4, 2, 40, 3),
+        ("bf16", 64, "one, one", 600, 130, 4, 2, 40, 3), ("bf16", 128, "one, one", 600, 130, 4, 2, 40, 3),
+        ("f32", 64, "several, one", 150, 200, 2, 2, 1, 4), ("f32", 128, "several, one", 150, 200, 2, 2, 1, 4),
+        ("bf16", 64, "several, one", 150, 200, 2, 2, 1, 4), ("bf16", 128, "several, one", 150, 200, 2, 2, 1, 4),
+        ("f32", 64, "no sinks, one", 150, 200, 2, 2, 1, 0), ("bf16", 128, "no sinks, one", 150, 200, 2, 2, 1, 0),
+        ("f32", 64, "one, several", 105, 2131, 2, 2, 1, 2000), ("bf16", 128, "one, several", 63, 2125, 6, 3, 2125, 2000)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,d,parts,B,n,Hq,Hkv,W,S", CUTS)
+def test_gradients_of_every_cut(dt, d, parts, B, n, Hq, Hkv, W, S):
+    """Whole, short and empty sequences against 64 bits; in the last one two queries are
+    NaN, which spoils what they see and nothing else."""
+    dtype = swa.DT[dt]
+    g = torch.Generator(device="cuda").manual_seed(n)
+    q, k, v, do = (torch.randn(B, n, h, d, generator=g, device="cuda").to(dtype) for h in (Hq, Hkv, Hkv, Hq))
+    lens = torch.tensor([(n, 0, 7, n // 2, n - 1, 129)[b % 6] for b in range(B)])
+    lens[-1] = n
+    bad = [5, 100]
+    dirty = q.clone()
+    dirty[-1, bad] = float("nan")
+    leaves = [t.requires_grad_() for t in (dirty, k.clone(), v.clone())]
+    out = hba_amd.sliding_attention(*leaves, W, S, lens=lens)
+    got = (out.detach(), *torch.autograd.grad(out, leaves, do))
+    i = torch.arange(n, device="cuda")
+    for b in (0, 1, 2, 3, B - 1):
+        m = int(lens[b])
+        assert not any(t[b, m:].any() for t in got)
+        if not m:
+            continue
+        see = visible(i[:m], i[:m], W, S)
+        rows, keys = torch.ones(m, dtype=torch.bool, device="cuda"), torch.ones(m, dtype=torch.bool, device="cuda")
+        if b == B - 1:
+            rows[bad] = False
+            keys = ~see[bad].any(0)
+        G = Hq // Hkv
+        for h in range(Hkv):
+            hs = slice(h * G, h * G + G)
+            with torch.device("cuda"):
+                want, bound = attend(q[b, :m, hs], k[b, :m, h], v[b, :m, h], see, d ** -0.5, unit(dtype), do[b, :m, hs])
+            for name, x, w, c in zip(("out", "dq", "dk", "dv"), got, want, bound):
+                x, keep = (x[b, :m, hs], rows) if name in ("out", "dq") else (x[b, :m, h], keys)
+                assert_within(x[keep], w[keep].cpu(), c[keep].cpu(), f"{name} of {b}, {h}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("B,n,Hq,Hkv", [(1, 200, 2, 1), (2, 900, 14, 2), (8, 700, 14, 2)])
+def test_log_sum_exps(B, n, Hq, Hkv, dt, d):
+    """Of the probabilities, not of their roundings, in every form of the forward: off by
+    the largest error of a logit (d + 4 roundings of its products), the roundings of the
+    sum and the logarithm, and one of the result."""
+    q, k, v, _ = swa.make(swa.DT[dt], B, n, Hq, Hkv, d, seed=n)
+    _, lse = hba_amd.ops.swa_fwd(q.cuda(), k.cuda(), v.cuda(), None, 300, 2, d ** -0.5)
+    x, K = q[-1].double().transpose(0, 1), k[-1].double().repeat_interleave(Hq // Hkv, 1).transpose(0, 1)
+    i = torch.arange(n)
+    see = visible(i, i, 300, 2)
+    c = d ** -0.5 / torch.log(torch.tensor(2.0, dtype=torch.float64))
+    logits = (x @ K.transpose(1, 2) * c).masked_fill(~see, float("-inf"))
+    want = torch.logsumexp(logits / c * d ** -0.5, -1) * c / d ** -0.5
+    size = (x.abs() @ K.abs().transpose(1, 2) * c).masked_fill(~see, 0.0).amax(-1)
+    bound = E * ((d + 4) * size + 1.4427 * n + 8 + 4 * want.abs())
+    assert_within(lse[-1].cpu(), want, bound, "lse")
