@@ -202,3 +202,57 @@ def test_log_sum_exps(B, n, Hq, Hkv, dt, d):
     size = (x.abs() @ K.abs().transpose(1, 2) * c).masked_fill(~see, 0.0).amax(-1)
     bound = E * ((d + 4) * size + 1.4427 * n + 8 + 4 * want.abs())
     assert_within(lse[-1].cpu(), want, bound, "lse")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("which", range(4))
+def test_masked_places_at_head_dim_128(which, bad, dt):
+    """A non-finite query, key, value or cotangent spoils only what sees it."""
+    W, S, n, at, d = 40, 3, 200, 100, 128
+    x = swa.make(swa.DT[dt], 1, n, 4, 2, d, seed=7)
+    want, bound = sliding(*x[:3], W, S, d ** -0.5, None, unit(swa.DT[dt]), x[3])
+    dirty = [t.clone() for t in x]
+    dirty[which][:, at] = bad
+    i = torch.arange(n)
+    see = visible(i, i, W, S)
+    rows = see[:, at] if which in (1, 2) else i == at
+    keys = see[rows].any(0)
+    got = swa.run(*dirty[:3], W, S, dout=dirty[3])
+    for name, a, w, c in zip(("out", "dq", "dk", "dv"), got, want, bound):
+        keep = ~(rows if name in ("out", "dq") else keys)
+        assert_within(a.detach().cpu()[:, keep], w[:, keep], c[:, keep], name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("at", [5, 300, 590])
+def test_few_rows_spoiled_at_head_dim_128(at, bad, dt):
+    q, k, v, _ = swa.make(swa.DT[dt], 1, 600, 2, 1, 128, seed=at)
+    want, bound = sliding(q, k, v, 300, 2, 128 ** -0.5, None, unit(q.dtype))
+    k[0, at], v[0, at] = bad, bad
+    got = swa.run(q, k, v, 300, 2).cpu()
+    i = torch.arange(600)
+    sees = (i >= at) & (i < at + 300)
+    assert not got[0, sees].isfinite().any()
+    assert_within(got[:, ~sees], want[:, ~sees], bound[:, ~sees], "out")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("name", ["kr", "vp"])
+def test_masked_keys_of_a_cache_at_head_dim_128(name, bad, dt):
+    W, S, n, at = 40, 2, 200, 130
+    s = paged.setup(swa.DT[dt], 128, 4, 2, [n], [100])
+    want, bound = paged.expect(s, W, S)
+    off = (key_offsets if name == "kr" else value_offsets)(128)
+    s[name][int(s["table"][0, at // 64])][:, off[at % 64]] = bad
+    got = paged.call(s, W, S).cpu()
+    pos = torch.arange(100, 200)
+    sees = (pos >= at) & (pos < at + W)
+    assert_within(got[~sees], want[~sees], bound[~sees], "out")
+    if name == "vp":
+        assert not got[sees].isfinite().any()
