@@ -37,6 +37,7 @@ struct Args {
     float *part;                        // dk / dv sums of tiles in several parts
     int32_t *marks;                     // waves of swa_dkv whose sums are not finite
     int nst, Ps, Pn, schunk, chunk;     // tiles of sinks, parts of those and of the others, steps of a part of either
+    int pslot, pslots;                  // first slot that has sums in `part`, and how many there are of one (batch, KV head)
     int first;                          // swa_join: place of the launch's first workgroup
 };
 
@@ -426,7 +427,7 @@ __device__ __forceinline__ void find_keys(const Args &a, Keys &x) {
     const int chunk = tile < a.nst ? a.schunk : a.chunk;
     x.i0 = part * chunk;
     x.i1 = min(x.nst * a.G, x.i0 + chunk);
-    x.at = ((int64_t)combo * (a.nst * a.Ps + (a.ntiles - a.nst) * a.Pn) + slot) * KB + 32 * wave + (lane & 31);
+    x.at = ((int64_t)combo * a.pslots + slot - a.pslot) * KB + 32 * wave + (lane & 31);
 }
 
 template <int DT, int D>
@@ -625,8 +626,7 @@ template <int DT, int D> __global__ __launch_bounds__(JE / 4) void swa_join(cons
                 for (int i = 0; i < 4; ++i) sum[i] = fmaf(w, qo[i], sum[i]);
             }
     } else if (j < len) {
-        const int64_t slots = a.nst * a.Ps + (a.ntiles - a.nst) * a.Pn;
-        const float *p = a.part + ((int64_t)combo * slots + slot) * KB * 2 * D + e;
+        const float *p = a.part + ((int64_t)combo * a.pslots + slot - a.pslot) * KB * 2 * D + e;
 #pragma unroll 4
         for (int i = 0; i < used; ++i) sum = sum + *reinterpret_cast<const f32x4 *>(p + (int64_t)i * KB * 2 * D);
     }
@@ -647,6 +647,8 @@ template <int DT, int D> __global__ __launch_bounds__(JE / 4) void swa_join(cons
 struct Cut {
     int ntiles, nst, Ps, Pn, schunk, chunk;
     int64_t slots;
+    // tiles in one part store dk and dv at once: only the others' slots have sums to join
+    int64_t part_slots() const { return (Ps > 1 ? (int64_t)nst * Ps : 0) + (Pn > 1 ? (int64_t)(ntiles - nst) * Pn : 0); }
 };
 static Cut cut(int dtype, int64_t d, int64_t Cn, int64_t n, int64_t G, int64_t W, int64_t S) {
     Cut c = {}, best = {};
@@ -669,12 +671,11 @@ static Cut cut(int dtype, int64_t d, int64_t Cn, int64_t n, int64_t G, int64_t W
         c.Pn = (int)((usual + ch - 1) / ch);
         c.Ps = (int)((most + sch - 1) / sch);
         c.slots = (int64_t)c.nst * c.Ps + (int64_t)(c.ntiles - c.nst) * c.Pn;
-        const int64_t parts = (c.Ps > 1 ? (int64_t)c.nst * c.Ps : 0) + (c.Pn > 1 ? (int64_t)(c.ntiles - c.nst) * c.Pn : 0);
         const auto rounds = [&](int64_t slots) { return (double)((slots * Cn + room - 1) / room); };
         const int64_t sinks = (int64_t)c.nst * c.Ps;
         const double us = (sch == ch ? rounds(c.slots) * (ch + 4)
                                      : rounds(sinks) * (sch + 4) + rounds(c.slots - sinks) * (ch + 4)) * step +
-                          (double)(parts * Cn) * KB * 2 * d * 8 / 4e6;
+                          (double)(c.part_slots() * Cn) * KB * 2 * d * 8 / 4e6;
         if (P == 1 || us < least) {
             least = us;
             best = c;
@@ -817,8 +818,8 @@ extern "C" int hba_swa_bwd_workspace_bytes(int dtype, int64_t B, int64_t n, int6
     if (W > n) W = n;
     if (S > n) S = n;
     const swa::Cut c = swa::cut(dtype, d, B * Hkv, n, Hq / Hkv, W, S);
-    const size_t part = c.Ps > 1 || c.Pn > 1 ? (size_t)(B * Hkv) * c.slots * swa::KB * 2 * d * 4 : 0;
-    *bytes = swa::delta_bytes(B, n, Hq) + swa::mark_bytes(B * Hkv, c) + part;
+    *bytes = swa::delta_bytes(B, n, Hq) + swa::mark_bytes(B * Hkv, c) +
+             (size_t)(B * Hkv) * c.part_slots() * swa::KB * 2 * d * 4;
     return HBA_OK;
 }
 
@@ -878,6 +879,8 @@ extern "C" int hba_swa_bwd(int dtype, const void *q, const int64_t q_strides[3],
     a.nst = c.nst;
     a.Ps = c.Ps;
     a.Pn = c.Pn;
+    a.pslot = c.Ps > 1 ? 0 : c.nst;
+    a.pslots = (int)c.part_slots();
     a.schunk = c.schunk;
     a.chunk = c.chunk;
     if (!abi::launchable(c.slots * a.Cn, 64 * rows::NW) || c.slots * a.Cn * rows::NW > 0x7fffffff ||

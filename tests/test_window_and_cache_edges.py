@@ -82,6 +82,24 @@ def test_launches_of_too_many_threads_are_refused():
     assert host.append(T=1 << 24, Bd=1 << 24, Hkv=1) == -2
 
 
+@pytest.mark.parametrize("B,n,Hq,Hkv,d,W,S,parts", [
+    (8, 8192, 28, 4, 128, 1024, 8, 7 * 32),         # a tile of sinks in 7 parts, the others whole
+    (4, 32768, 56, 8, 128, 1024, 8, 28 * 32),
+    (1, 8192, 28, 4, 128, 1024, 8, None),           # every tile in parts
+    (600, 130, 4, 2, 64, 40, 3, 0)])
+def test_gradients_workspace_has_room_for_what_is_written(B, n, Hq, Hkv, d, W, S, parts):
+    """Each row's <dout, out>, a mark a wave, and the sums of those key tiles that are cut."""
+    st, need = host.size(host._lib.lib().hba_swa_bwd_workspace_bytes, 1, B, n, Hq, Hkv, d, W, S)
+    rows = 4 * B * Hq * n
+    assert st == 0 and need >= rows
+    tiles = B * Hkv * -(-n // 128)
+    if parts is not None:
+        marks = 16 * (tiles + parts)
+        assert parts * 128 * 2 * d * 4 <= need - rows <= marks + 512 + parts * 128 * 2 * d * 4
+    else:
+        assert need - rows >= 2 * tiles * 128 * 2 * d * 4
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt,d,Hkv", [("bf16", 64, 16), ("f32", 128, 8)])
 def test_gradients_of_a_million_heads(dt, d, Hkv):
