@@ -437,6 +437,7 @@ __device__ __forceinline__ void rows_part(const Args &a, char *smem, int x, int 
     int s = 0, tile = x, first = 0, cnt = a.T, it1 = 0, ns = 0, wt0 = 0;
     if constexpr (SHARED) {   // every tile of the part, whatever the rows see of it: it can be staged at once
         src.table = a.table;
+        src.len = a.shared * rows::PAGE;
         it1 = min(a.shared * TP, it0 + a.part * TP);
         rows::attend_begin(src, smem, it0, it1, 0, 0);
     } else {
@@ -454,6 +455,7 @@ __device__ __forceinline__ void rows_part(const Args &a, char *smem, int x, int 
         }
         cnt = ragged::tokens(a.cu, s, a.T, first);
         src.table = a.table + (int64_t)s * a.maxp;
+        src.len = length(a, s);
     }
     const int nr = cnt * a.G, r0 = tile * rows::RT, rw = r0 + wave * rows::RW, r = rw + (lane & 31);
     const bool in = r < nr;

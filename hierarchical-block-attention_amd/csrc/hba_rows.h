@@ -19,7 +19,8 @@
 // would still spoil 0 * V.  Whether that happened shows in the result, so a
 // workgroup whose rows come out non-finite computes them once more key by key,
 // where a masked key takes no part (attend_each).  Finite inputs pay nothing but
-// the check of the result.
+// the check of the result; values behind a sequence in its last page, which may be
+// anything, are cleared in LDS first.
 #pragma once
 
 #include "hba_common.h"
@@ -206,6 +207,7 @@ template <int DT, int D, int KEYS_ = KEYS<DT, D>> struct DenseKV {
     typedef typename Op<DT>::F F;
     typedef Tile<DT, D> TL;
     static constexpr int KT = KEYS_, BYTES = 2 * KT * TL::ROWB;   // a staged tile: keys, then values
+    static constexpr bool TAIL = false;               // no rows past `last` are read
     const char *k, *v;
     int64_t kb, vb;                                   // bytes from row to row
     int last;                                         // the last row that may be read
@@ -241,7 +243,9 @@ template <int DT, int D> struct PageKV {
     const char *k, *v;            // the KV head's place in page 0
     int64_t page;                 // bytes from page to page
     const int32_t *table;         // the sequence's pages
+    int len;                      // its keys: what lies behind them in a page may be anything
     int64_t pages;                // pages there are
+    static constexpr bool TAIL = true;
     int64_t id;                   // the page of the tile that is staged next
     int half;                     // and the tile's place in it
 
@@ -277,6 +281,18 @@ template <int DT, int D> struct PageKV {
     static __device__ __forceinline__ F vf(const char *t, int kt, int dt, int u, int lane) {
         const int x = 32 * dt + (lane & 31);
         return Op<DT>::load(t + HALF + (((x >> 4) * (KT / 32) + kt) * 64 + (x & 15) + 16 * (2 * u + (lane >> 5))) * 8 * ESZ);
+    }
+    // Clears the values at and past place n of a staged tile: a weight of 0 would make
+    // NaN of a NaN there.  A chunk of 8 is as many keys of one column (see vf).
+    static __device__ __forceinline__ void clear(char *t, int n) {
+        typedef typename St<DT>::T T;
+        for (int c = threadIdx.x; c < KT * D / 8; c += 64 * NW) {
+            const int first = n - (32 * (c / 64 % (KT / 32)) + 8 * (c % 64 / 16));   // the chunk's first to clear
+            T *p = reinterpret_cast<T *>(t + HALF) + 8 * c;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e >= first) St<DT>::st(p, e, 0.0f);
+        }
     }
     // one key, for attend_each
     __device__ __forceinline__ float dot_one(const F (&q)[D / 16], int j, int hf) const {
@@ -412,6 +428,12 @@ __device__ __forceinline__ void attend(Src &src, char *smem, const typename Op<D
             src.next(tile(min(nx + 1, it1 - 1)));
         }
         const int j0 = tile(it) * KT;
+        if constexpr (Src::TAIL) {
+            if (j0 + KT > src.len) {   // the same for the workgroup
+                src.clear(smem + cur * Src::BYTES, src.len - j0);
+                __syncthreads();
+            }
+        }
         if (j0 >= w.hi_max || (j0 + KT <= w.lo_min && j0 >= w.S)) continue;   // nothing the wave's rows see
         const char *t = smem + cur * Src::BYTES;
 #pragma unroll

@@ -274,3 +274,21 @@ def test_masked_keys_of_a_cache_at_head_dim_128(name, bad, dt):
     assert_within(got[~sees], want[~sees], bound[~sees], "out")
     if name == "vp":
         assert not got[sees].isfinite().any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,d", [("f32", 64), ("f32", 128), ("bf16", 64), ("bf16", 128)])
+@pytest.mark.parametrize("W,S", [(0, 0), (70, 4)])
+@pytest.mark.parametrize("lens,new,shared", [([1], [1], 0), ([40, 70, 129, 350], [40, 3, 128, 1], 0),
+                                             ([65, 96, 31, 959], [1, 33, 31, 300], 0), ([135, 200], [7, 20], 128)])
+def test_what_lies_behind_a_sequence_changes_no_bit(lens, new, shared, W, S, dt, d):
+    """Parts of prompts: the rest of a last page may be anything, and no row takes
+    another way for it."""
+    if shared and W:
+        W, S = 0, 0
+    s = paged.setup(swa.DT[dt], d, 6, 2, lens, new, shared=shared, seed=len(lens))
+    want = paged.call({**s, "kr": s["kr"].nan_to_num(), "vp": s["vp"].nan_to_num()}, W, S)
+    assert s["vp"].isnan().any()
+    for fill in (float("nan"), float("inf"), torch.finfo(swa.DT[dt]).max):
+        kr, vp = (torch.where(s[n].isnan(), fill, s[n]) for n in ("kr", "vp"))
+        assert torch.equal(paged.call({**s, "kr": kr, "vp": vp}, W, S), want), fill
