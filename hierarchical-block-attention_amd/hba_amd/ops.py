@@ -1100,8 +1100,8 @@ def paged_attn(q, q_gain, eps, kr_pages, v_pages, page_table, seq_lens, cos, sin
     token that sees nothing, or is behind cu[Bd] (a padded batch), gives 0.
     There is no backward pass: asking for one raises."""
     args = (q, q_gain, eps, kr_pages, v_pages, page_table, seq_lens, cos, sin, scales, max_len, window, sinks, cu, shared)
-    if _differentiated(q, q_gain, kr_pages, v_pages, cos, sin, scales):
-        return _PagedAttn.apply(*args)
+    if _differentiated(q, q_gain, kr_pages, v_pages, cos, sin, scales) and not torch.compiler.is_dynamo_compiling():
+        return _PagedAttn.apply(*args)   # torch.compile would trace its backward; the registered operator's raises too
     return (_paged_attn if _plain(*args) else torch.ops.hba.paged_attn)(*args)
 
 

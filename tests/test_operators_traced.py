@@ -160,3 +160,22 @@ def test_tangents_are_not_dropped():
         torch.func.jvp(lambda x: window(x, k, k), (q,), (q,))
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda x: attend({**a, "q": x}), (a["q"],), (a["q"],))
+
+
+@pytest.mark.gpu
+def test_compiled_cache_calls():
+    """As the registered operators; a graph with a gradient through paged_attn is refused."""
+    def both(a):
+        append(a)
+        return attend(a)
+
+    torch.compiler.reset()
+    f = torch.compile(both, backend="aot_eager", fullgraph=True)
+    a, b = cache("cuda", seed=1), cache("cuda", seed=1)
+    for x in (a, b):
+        x["gain"].requires_grad_()
+    with torch.no_grad():
+        assert torch.equal(f(a), both(b))
+    assert all(torch.equal(a[n], b[n]) for n in ("kc", "kr", "vp", "summ"))
+    with pytest.raises(Exception, match="backward through hba.paged_attn"):
+        f(a)
