@@ -261,7 +261,7 @@ __device__ __forceinline__ void decode_part(const Args &a, DecodeLds<D> &lds, in
                 p[e] = ex2(S[2 * h + (e >> 2)][e & 3] - mc);
                 l += p[e];
             }
-            const F pf = Op<DT>::pack(p);
+            const F pf = Op<DT>::pack(p);   // bf16: a relative 2^-8 each at most; l has them as they are
 #pragma unroll
             for (int dt = 0; dt < NDT; ++dt) O[dt] = Mma16<DT>::mma(x.v[dt][h], pf, O[dt]);
         }
@@ -356,7 +356,8 @@ __device__ __forceinline__ void decode_part(const Args &a, DecodeLds<D> &lds, in
 constexpr int DW = 8;   // waves of a decode workgroup
 // group: (sequence, KV head, 16 of its heads), part: a run of a.part pages.
 // 64 sequences' windows of 1024 keys, 14 / 2 heads, d = 64: 11 us, 7 at a copy's rate.
-// Eight waves, so that two pages each cover a window: chains of round trips bound it.
+// Eight waves, so that a window of 17 or 18 pages takes a wave two pages, or three:
+// chains of round trips bound it.
 template <int DT, int D, int DW>
 __device__ __forceinline__ void decode_run(const Args &a, DecodeLds<D> &lds, int group, int part) {
     const int ct = (a.G + 15) / 16, ng = a.Hkv * ct, s = group / ng, gi = group % ng;
@@ -687,7 +688,9 @@ static Plan plan(int64_t T, int64_t Bd, int64_t Hq, int64_t Hkv, int64_t W, int6
     const int64_t G = Hq / Hkv, KT = rows::PAGE;
     int64_t keys = max_len - shared * KT;
     if (W > 0 && W < keys) keys = W;
-    if (W > 0 && !one) keys = max_len;   // a part of a prompt may span any number of windows
+    // A part of a prompt may span any number of windows.  (The parts cut the list of one
+    // 128-row tile, which has W + 128 / G tokens and the sinks, so of a window's parts most are empty.)
+    if (W > 0 && !one) keys = max_len;
     if (keys < 1) keys = 1;
     int64_t pages = (keys + KT - 1) / KT + 1 + (W > 0 ? (S + KT - 1) / KT : 0);
     const int64_t all = (max_len + KT - 1) / KT;
@@ -704,6 +707,10 @@ static Plan plan(int64_t T, int64_t Bd, int64_t Hq, int64_t Hkv, int64_t W, int6
         // Up to 32 pages are 4 a wave and need no join; from 1024 groups on, the card's
         // workgroups even out by themselves.  24 sequences of 4000 to 32000 keys, 4 KV
         // heads, d = 128: 155 us (5.8 TB/s), and 188 in runs of pages, 11 a sequence.
+        // Lengths that are alike have less to even out.  Shares and one workgroup a group,
+        // d = 64: 8 groups of 2000, 4096 and 8192 keys 13, 12, 13 and 9, 12, 20 us; 128
+        // groups 21, 31, 51 and 15, 23, 40; d = 128: 16 groups 14, 15, 21 and 14, 25, 46;
+        // 256 groups 51, 102, 192 and 44, 96, 187.
         p.shares = (int)(groups * pages / 8 < CUS ? groups * pages / 8 + 1 : CUS);
         p.own = 1;
         p.own_pages = 8;

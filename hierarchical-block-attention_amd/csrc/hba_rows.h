@@ -476,7 +476,9 @@ __device__ __forceinline__ void attend(Src &src, char *smem, const typename Op<D
                 return sum;
             };
             Sums sum = weights(shift);
-            if (__ballot(!(sum.rounded <= MOST) || a.m == -INFINITY)) {   // a new maximum
+            // A new maximum.  (A row that sees nothing, as those behind a tile's last have
+            // nothing to see, has none and keeps its wave here: exponentials twice.)
+            if (__ballot(!(sum.rounded <= MOST) || a.m == -INFINITY)) {
                 float mx = s[0];
 #pragma unroll
                 for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[r]);

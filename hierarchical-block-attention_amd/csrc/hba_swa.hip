@@ -9,7 +9,7 @@
 // Forward and dq: a workgroup has 128 rows of one KV head's query heads
 // (hba_rows.h) and walks the tiles of keys that they see.  dk and dv: a workgroup
 // has 128 keys as the columns of S = Q . K^T and walks its KV head's query heads
-// and their 64-token tiles, so the sum over the heads of a group stays in
+// and their tokens, 32 a step, so the sum over the heads of a group stays in
 // registers and nothing is added by atomics: the gradients are the same bits
 // from run to run.  A tile whose keys many rows see (sinks: every later row) is
 // cut into parts that sum into a workspace and are joined in order by a second
@@ -133,7 +133,9 @@ __device__ __forceinline__ const char *dout_row(const Args &a, const Rows &x) {
 // 1.21 of a large product).  Bound by issue: per 32 rows and 32 keys 16 exponentials
 // and as many multiply-adds and conversions a lane stand beside 8 matrix
 // instructions (without the exponentials 144 us, without reading operands from LDS
-// 150).  fp32, 2 x 2047 tokens, W = 512: 80 to 89 us, 37 at the fp32 matrix rate.
+// 150).  fp32, 2 x 2047 tokens, W = 512: 80 to 89 us, 37 at the fp32 matrix rate: 392
+// workgroups with rows for 256 CUs, so some CUs have two and some one, and masked halves
+// of tiles at the windows' ends.
 // SEP: the log-sum-exp has a sum of its own (see attend): 155 us at 8192 tokens, 28
 // heads, d = 128 with three waves per SIMD, 179 with two, 152 without it.
 template <int DT, int D, bool SEP>
@@ -224,7 +226,9 @@ template <int DT, int D, int SETS, bool SEP> __global__ __launch_bounds__(512) v
 }
 
 // The probabilities' gradient from the forward's log-sum-exps, and dq; delta =
-// do . o on the way, for dk and dv.
+// do . o on the way, for dk and dv.  o is the output as stored, so in bf16 delta has
+// its rounding (2^-8 of sum |do||o| at most): o is what there is of the forward, and
+// delta weighs on a ds only with the probability of its key.
 template <int DT, int D>
 __device__ __forceinline__ float row_delta(const Args &a, const Rows &x, const typename Op<DT>::F (&dO)[D / 16]) {
     typename Op<DT>::F o[D / 16];
@@ -294,11 +298,12 @@ __device__ __forceinline__ typename Op<DT>::F rest16(const f32x16 &p, int u, typ
     for (int e = 0; e < 8; ++e) y[e] = p[8 * u + e] - y[e];
     return Op<DT>::pack(y);
 }
-constexpr int FEW = 256;   // rows (and so keys) whose ds enters its products in two parts, see swa_dq
+constexpr int FEW = 256;   // first rows of a sequence whose ds enters its products in two parts, see swa_dq
 
 // Rows as swa_fwd, three products a tile (q . k again, do . v, ds . k).  8192 tokens,
 // 28 heads, d = 128, W = 1024, bf16: 200 us, 140 at the rate of a large product; the
-// matrix cores are busy 44 % of the time (the forward: 43 %).
+// matrix cores are busy 44 % of the time (the forward: 42 %).  fp32: 1.64 ms, 1.12 at
+// the fp32 matrix rate.
 template <int DT, int D> __global__ __launch_bounds__(64 * NW, DT == 1 ? 2 : 1) void swa_dq(const Args a) {
     extern __shared__ __align__(16) char smem[];
     typedef Tile<DT, D> TL;
@@ -319,10 +324,13 @@ template <int DT, int D> __global__ __launch_bounds__(64 * NW, DT == 1 ? 2 : 1) 
     const float delta = row_delta<DT, D>(a, x, dO);
     if (x.valid && hf == 0) a.delta[hrow] = delta;
     const float lse = x.valid ? a.lse[hrow] : INFINITY;
-    // Rows with few keys have the largest gradients (as 1 / sqrt(keys)) and so most of
-    // the whole's rounding error: their ds enters the product with its rest.  1999
-    // tokens, W = 512, N(0, 1), d = 64: dq is off by 2.2e-3 of its norm, 2.47e-3
-    // without (2.28e-3 for 128 keys; its own rounding alone 1.66e-3), for 1 us of 31.
+    // ds enters the product rounded to bf16 (2^-8 at most).  A sequence's first rows see
+    // few keys, so they have its largest gradients (as 1 / sqrt(keys)) and most of the
+    // whole tensor's rounding error: their ds enters with its rest.  The rule goes by a
+    // row's place, so it does little where a window leaves every row few keys, and a
+    // later row's own relative error is what it was.  Its border was chosen at 1999
+    // tokens, W = 512, N(0, 1), d = 64: dq is off by 2.2e-3 of its norm, 2.46e-3
+    // without (2.26e-3 for 128 rows; its own rounding alone 1.66e-3), for 1 us of 31.
     const bool few = x.w.hi_max <= FEW;
     const f32x16 zero = {0.0f};
     f32x16 acc[NDT];
@@ -455,10 +463,10 @@ __device__ __forceinline__ void store_keys(const Args &a, const Keys &x, f32x16 
     store_rows<DT, D>(a.dv + row, dv, 1.0f);
 }
 
-// Four products a step of 32 tokens.  Same case as swa_dq: 310 to 340 us, 186 at the
-// rate of a large product.  Each operand that a wave reads from LDS serves one matrix
+// Four products a step of 32 tokens.  Same case as swa_dq: 310 to 350 us, 186 at the
+// rate of a large product (fp32: 2.5 ms, 1.49).  Each operand that a wave reads from LDS serves one matrix
 // instruction (its 32 keys are the other one): LDS is busy some 45 % of the time, the
-// matrix cores 35 %, and two waves a SIMD do not hide one behind the other wholly.
+// matrix cores 36 %, and two waves a SIMD do not hide one behind the other wholly.
 template <int DT, int D>
 __global__ __launch_bounds__(64 * NW, (DT == 1 ? (D == 64 ? 3 : 2) : 1)) void swa_dkv(const Args a) {
     extern __shared__ __align__(16) char smem[];
@@ -551,6 +559,7 @@ __global__ __launch_bounds__(64 * NW, (DT == 1 ? (D == 64 ? 3 : 2) : 1)) void sw
                     dp[r] = keep(dp[r], see, 8 * (r >> 2) + (r & 3), 0.0f);
                 }
             }
+            // p and ds rounded to bf16 (2^-8 each at most), as the matrix cores take them; sums in fp32
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const F pf = half16<DT>(s, u), df = half16<DT>(dp, u);
@@ -710,6 +719,10 @@ template <int DT, int D, bool SEP> static int launch_fwd(const Args &a, int64_t 
         // What the meeting costs, in keys: 300 tokens, d = 64, W = 64, 128 and 256 take 7.8, 8.6 and 9.7 us as one
         // set, the last 9.4 as two, and all 7.7, 7.9 and 8.2 as four; d = 128, W = 128 and 256: 12.2 and 14.0 as one,
         // 12.4 and 13.6 as two.  100 tokens: 6.3 as one, 6.6 as four.
+        // And in workgroups, one, two and four sets at d = 64, W = 1024: 110 (of 128 rows) 20, 17 and 13; 166 23, 19
+        // and 15; 220 23, 20 and 19 (with W = 128 9.4, 9.3 and 11.3); 308 24, 21 and 25; 660, W = 512 26, 31 and 26.
+        // d = 128: 220 31, 26 and 26; 332 37, 31 and 44; 440 40, 48 and 39.  So the borders are safe rather than best
+        // between 128 and 320 workgroups.  Sinks are not counted in `seen`.
         const int seen = a.W < a.n ? a.W : a.n;
         Args b = a;
         int64_t more;

@@ -503,9 +503,9 @@ int hba_attn_bwd_workspace_size(int64_t B, int64_t n, int64_t Hq, int64_t d, siz
  * in the pages stays as it is.  kc_pages and summ_pages may be NULL (summ_pages
  * needs kc_pages, probes and proj).  cu int32 [Bd+1] rises from 0 to at most T;
  * tokens behind cu[Bd] (a padded batch), at positions < 0, past the page table,
- * at/after n_tab, or on a page outside 0 .. num_pages-1 are not appended.  A page is appended to by one sequence.
- * The call changes no length, so repeating it gives the same cache.  No
- * counterpart in the reference, which has no KV cache.
+ * at/after n_tab, or on a page outside 0 .. num_pages-1 are not appended.  A page
+ * is appended to by one sequence.  The call changes no length, so repeating it
+ * gives the same cache.  No counterpart in the reference, which has no KV cache.
  */
 int hba_kv_append_ragged(int dtype, const void *k, const int64_t k_strides[2], const void *v,
                          const int64_t v_strides[2], const int32_t *cu, int64_t T,
@@ -531,9 +531,12 @@ int hba_kv_append_ragged(int dtype, const void *k, const int64_t k_strides[2], c
  * batch, and joined with each sequence's own by their log-sum-exps.  max_len
  * bounds every seq_lens[s] (a longer one is read as max_len).  A page id outside
  * 0 .. num_pages-1 is clamped into it.  out [T, Hq, d] contiguous; a token that
- * sees nothing (position < 0) or is behind cu[Bd] (a padded batch) gives 0.  Whatever lies in the pages at or past a
- * sequence's length has no effect.  bf16: logits from queries of two bf16 parts
- * (16 bits of mantissa), probabilities rounded to bf16, sums in fp32.
+ * sees nothing (position < 0) or is behind cu[Bd] (a padded batch) gives 0.
+ * Whatever lies in the pages at or past a sequence's length has no effect, and a
+ * NaN or infinity before it none on the tokens that do not see it (with cu, tokens
+ * that share a workgroup with one that sees it are computed again key by key,
+ * which is slow).  bf16: logits from queries of two bf16 parts (16 bits of
+ * mantissa), probabilities rounded to bf16, sums in fp32.
  * workspace: 16-byte aligned, no initial contents, at least
  * hba_paged_attn_workspace_bytes (one_each: cu is NULL); 0 means none is needed.
  * No counterpart in the reference, which has no KV cache.
@@ -552,16 +555,21 @@ int hba_paged_attn(int dtype, const void *q, const int64_t q_strides[2], const f
 /*
  * Sliding-window attention with sinks (a model's window layers): query i of
  * q [B, n, Hq, d] attends to the keys j <= i with j > i - W or j < S of k, v
- * [B, n, Hkv, d], all with element strides (rows on 16-byte boundaries).
+ * [B, n, Hkv, d], all with element strides (rows on 16-byte boundaries; keys and
+ * values of a head 0 bytes to less than 16 MiB from token to token, in the backward
+ * queries and dout as well).
  * Queries and keys enter as they are (no norm, no rotation).  Any n >= 1, any
  * Hq / Hkv, d = 64 or 128, W >= 1, S >= 0, scale > 0.  lens int32 [B] (NULL: n
  * each; values are clamped to 0 .. n): rows at and past lens[b] are padding,
  * whose out is 0; their q, k and v are not used and may hold anything.  out
  * [B, n, Hq, d] contiguous; lse (NULL to skip) fp32 [B, Hq, n]: log2 of the sum
  * of 2^(log2(e) scale q.k) over the keys a row sees, +inf for padding.  A NaN
- * or infinity of a key or value that a row does not see has no effect on it.
- * bf16: products on bf16 matrix cores, the probabilities rounded to bf16, sums
- * in fp32.  No counterpart in the reference.
+ * or infinity of a key or value that a row does not see has no effect on it (rows
+ * that share a workgroup with one that sees it are computed again key by key,
+ * which is slow).  bf16: products on bf16 matrix cores, the probabilities rounded
+ * to bf16 for the product with the values (lse has them as they are), sums in
+ * fp32.  A batch of 2^24 row tiles (128 rows of a KV head's queries) and more is
+ * HBA_ERR_UNSUPPORTED.  No counterpart in the reference.
  */
 int hba_swa_fwd(int dtype, const void *q, const int64_t q_strides[3], const void *k,
                 const int64_t k_strides[3], const void *v, const int64_t v_strides[3],
@@ -569,8 +577,8 @@ int hba_swa_fwd(int dtype, const void *q, const int64_t q_strides[3], const void
                 int64_t W, int64_t S, float scale, void *out, float *lse, void *stream);
 
 /* Scratch bytes of hba_swa_bwd: <dout, out> of every row (fp32 [B, Hq, n]), marks of
- * sums that are not finite, and the partial sums of dk and dv where key tiles are
- * cut into parts. */
+ * sums that are not finite, and the partial sums of dk and dv of those key tiles that
+ * are cut into parts. */
 int hba_swa_bwd_workspace_bytes(int dtype, int64_t B, int64_t n, int64_t Hq, int64_t Hkv,
                                 int64_t d, int64_t W, int64_t S, size_t *bytes);
 
