@@ -11,7 +11,7 @@ import test_gpu_paged_attn as paged
 import test_gpu_swa as swa
 import test_window_and_cache_host as host
 import test_gpu_append_ragged as ragged
-from attn64 import E, assert_within, attend, sliding, unit, visible
+from attn64 import E, assert_within, attend, norm_rotate, sliding, unit, visible
 from hba_amd.decode import key_offsets, value_offsets
 from test_gpu_append_ragged import append
 
@@ -292,3 +292,45 @@ def test_what_lies_behind_a_sequence_changes_no_bit(lens, new, shared, W, S, dt,
     for fill in (float("nan"), float("inf"), torch.finfo(swa.DT[dt]).max):
         kr, vp = (torch.where(s[n].isnan(), fill, s[n]) for n in ("kr", "vp"))
         assert torch.equal(paged.call({**s, "kr": kr, "vp": vp}, W, S), want), fill
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_how_far_extend_and_append_are_apart(dt):
+    """The rotated keys of both ways into the cache, and what a decode makes of the
+    difference.  In bf16 append rounds the key, the table, both products and their sum (4
+    roundings of the products' magnitudes, and what they make of one another), extend the
+    sum alone; in fp32 both do the same.  A logit moves by the keys' differences times
+    |q|, its probability by at most twice that relative to it."""
+    x = ragged.Knobs(dt, batch=1)
+    a, b = x.cache(), x.cache()
+    n, d = 200, 64
+    k, v = x.kv(n)
+    a.extend(k, v, [n], x.qkn, x.summ, x.cos, x.sin)
+    for i in range(n):
+        b.append(k[i:i + 1], v[i:i + 1], x.qkn, x.summ, x.cos, x.sin)
+    ra, rb = (c.key_rows(torch.tensor(c._table[0]).cuda(), rotated=True).transpose(1, 2).reshape(-1, 2, d)[:n]
+              .double().cpu() for c in (a, b))
+    gain, eps = x.qkn.k.gain.detach().cpu(), x.qkn.k.eps
+    cos, sin = x.cos.cpu()[:n], x.sin.cpu()[:n]
+    y, want, _ = norm_rotate(k.cpu(), gain, eps, cos, sin, 0.0)
+    other = torch.cat((y[..., d // 2:], y[..., :d // 2]), -1)
+    size = y.abs() * cos.double()[:, None].abs() + other.abs() * sin.double()[:, None].abs()
+    u = unit(dt)
+    one = (d / 2 + 12) * E * size
+    ea, eb = (one + u * size, one + (4.1 * u if dt == torch.bfloat16 else u) * size)
+    assert_within(ra, want, ea, "extend's kr")
+    assert_within(rb, want, eb, "append's kr")
+    q = torch.randn(1, 4, d).to(dt).cuda()
+    oa, ob = (hba_amd.cache_attention(q, c, x.cfg, x.qkn, x.cos, x.sin).detach().cpu() for c in (a, b))
+    _, qr, qe = norm_rotate(q.cpu(), x.qkn.q.gain.detach().cpu(), x.qkn.q.eps, cos[-1:], sin[-1:],
+                            u * u if dt == torch.bfloat16 else 0.0)
+    scale = float(a.scales()[0])
+    see = torch.ones(1, n, dtype=torch.bool)
+    for h in range(2):
+        hs, vals = slice(2 * h, 2 * h + 2), v[:, h].cpu()
+        move = 2 * scale * (qr[:, hs].abs() @ (ea + eb)[:, h].T).amax(-1, keepdim=True)
+        middle, bound = attend(qr[:, hs], want[:, h], vals, see, scale, u, qerr=qe[:, hs])
+        weight, _ = attend(qr[:, hs], want[:, h], vals.abs(), see, scale, u)
+        assert_within(oa[:, hs], middle, bound + move * weight, "over extend's keys")
+        assert_within(ob[:, hs], middle, bound + move * weight, "over append's keys")
