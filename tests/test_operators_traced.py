@@ -179,3 +179,24 @@ def test_compiled_cache_calls():
     assert all(torch.equal(a[n], b[n]) for n in ("kc", "kr", "vp", "summ"))
     with pytest.raises(Exception, match="backward through hba.paged_attn"):
         f(a)
+
+
+@pytest.mark.gpu
+def test_mapped_calls():
+    """vmap runs the registered operator for each; what it cannot map it refuses."""
+    x = [torch.randn(3, 1, 30, h, 64, device="cuda") for h in (4, 2, 2)]
+    want = torch.stack([window(*(t[i] for t in x)) for i in range(3)])
+    assert torch.equal(torch.func.vmap(window)(*x), want)
+    assert torch.equal(torch.func.vmap(window, (0, None, None))(x[0], x[1][0], x[2][0]),
+                       torch.stack([window(x[0][i], x[1][0], x[2][0]) for i in range(3)]))
+    a = cache("cuda")
+    q = torch.randn(3, *a["q"].shape, device="cuda").bfloat16()
+    got = torch.func.vmap(lambda t: attend({**a, "q": t}))(q)
+    assert torch.equal(got, torch.stack([attend({**a, "q": t}) for t in q]))
+    before = {n: a[n].clone() for n in ("kc", "kr", "vp", "summ")}
+    k = torch.randn(3, *a["k"].shape, device="cuda").bfloat16()
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda t: append({**a, "k": t}))(k)
+    assert all(torch.equal(a[n], before[n]) for n in before)
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda t: window(t, x[1][0], x[2][0]).sum())(x[0][0])
