@@ -1,0 +1,485 @@
+// The paged cache in 4 or 8 bits (hba_mx.h): writing new tokens into it, and reading
+// tokens back as rows.
+//
+//   append_kernel   QKNorm, the rotation at each token's position, quantised keys and
+//                   values into their pages
+//   read_kernel     the last tokens of every sequence as rows of fp32 or bf16
+#include "hba_abi.h"
+#include "hba_common.h"
+#include "hba_mx.h"
+#include "hba_ragged.h"
+
+namespace hba {
+namespace mx {
+
+struct AppendArgs {
+    const char *k, *v;                  // [T, Hkv, D]; byte strides of token and head
+    int64_t kst, ksh, vst, vsh;
+    const int32_t *cu;                  // nullptr: one token per sequence
+    int T, Bd, Hkv, maxp;
+    const float *gain, *cos, *sin;      // nullptr: no norm, no rotation
+    float eps;
+    int64_t n_tab, pages;               // positions at/after n_tab are not appended
+    const int32_t *table, *lens;
+    char *kp, *vp;
+};
+
+// Tokens of sequence s and those of them that lie in its pages: positions first ..
+// last - 1, from place c0 of the batch on.  (Not in them: positions below 0, past the
+// page table or the rotation tables.)
+struct Span {
+    int from, n, c0, first, last;
+    __device__ __forceinline__ int tiles() const { return last > first ? (last - 1) / 64 - first / 64 + 1 : 0; }
+};
+__device__ __forceinline__ Span span(const int32_t *cu, const int32_t *lens, int T, int64_t most, int s) {
+    Span x;
+    if (cu) {
+        x.n = ragged::tokens(cu, s, T, x.from);
+    } else {
+        x.from = s;
+        x.n = 1;
+    }
+    x.c0 = x.from;
+    const int64_t L = lens[s];
+    int64_t first = L - x.n;
+    if (first < 0) {
+        x.c0 += (int)min(-first, (int64_t)x.n);
+        first = 0;
+    }
+    x.first = (int)min(first, most);
+    x.last = (int)max((int64_t)x.first, min(L, most));
+    return x;
+}
+
+// The scale of a group whose largest magnitude has the bits `big`: the smallest 2^(b - 127)
+// that takes it to at most 1.75 2^EMAX (e2m1 7, of which 6 is left; e4m3 448).  Of the
+// energy of normal values e2m1 then loses 1.25% (with the limit 6 1.33%, with 8 1.32%,
+// with the better of two scales in each group 1.245%).
+template <int F> __device__ __forceinline__ int scale_byte(uint32_t big) {
+    constexpr int EMAX = F == 4 ? 2 : 8;
+    const int b = (int)(big >> 23) - EMAX + ((big & 0x7fffffu) > 0x600000u);
+    // (over 1.75 2^127 the nearest code would stand for 2^128, which fp32 has not)
+    return big == 0 ? 0 : big > 0x7f600000u ? 255 : max(b, 1);
+}
+// Four elements of such a group as codes (rounded to nearest, ties to even), F / 2 bytes.
+template <int F> __device__ __forceinline__ uint32_t four(const float (&x)[4], int b) {
+    typedef short s16x2 __attribute__((ext_vector_type(2)));
+    if (b == 0 || b == 255) return 0;
+    const float to = __uint_as_float((uint32_t)(254 - b) << 23);   // b is at most 252
+    float y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = x[i] * to;   // exact, or far below the smallest code
+    if constexpr (F == 4) {
+        const uint32_t w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0, y[0], y[1], 1.0f, 0);
+        return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[2], y[3], 1.0f, 1) & 0xffffu;
+    } else {
+        const s16x2 w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(s16x2{0, 0}, y[0], y[1], 1.0f, false);
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, y[2], y[3], 1.0f, true));
+    }
+}
+// The largest magnitude's bits over the 8 lanes of a group (32 elements, 4 each); a NaN's
+// are above all.
+__device__ __forceinline__ uint32_t largest(const float (&x)[4]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
+    return m;
+}
+template <int DT> __device__ __forceinline__ void load4(float (&x)[4], const char *p) {
+    if constexpr (DT == 1) {
+        const uint2 w = *reinterpret_cast<const uint2 *>(p);
+        x[0] = __uint_as_float(w.x << 16);
+        x[1] = __uint_as_float(w.x & 0xffff0000u);
+        x[2] = __uint_as_float(w.y << 16);
+        x[3] = __uint_as_float(w.y & 0xffff0000u);
+    } else {
+        const float4 w = *reinterpret_cast<const float4 *>(p);
+        x[0] = w.x;
+        x[1] = w.y;
+        x[2] = w.z;
+        x[3] = w.w;
+    }
+}
+
+// One workgroup per (page that gets tokens, KV head).  D / 8 lanes a row, each with 4
+// elements of its first half and the 4 that they are rotated with.  The norm and the
+// rotation run in 64 bits (at half a rate that nothing here needs) and are rounded to
+// 32 once: next to a border between two codes the last bit of an fp32 sum would decide
+// which one it is, and a key's code would depend on the order of that sum.
+// Codes go to LDS in the page's order (the values' a byte each, by columns) and from
+// there in whole 16-byte pieces.  Two tokens' values share a byte (F = 4): where only
+// some of a piece's tokens are new, the others are read and put back, by the one
+// workgroup that writes this page.
+template <int DT, int D, int F> __global__ __launch_bounds__(256) void append_kernel(const AppendArgs a) {
+    typedef Place<D, F> At;
+    constexpr int TPH = D / 8, RPP = 256 / TPH, NP = 64 / RPP, ESZ = DT == 1 ? 2 : 4, NG = D / GROUP;
+    constexpr int CB = (int)code_bytes(D, F), VS = 68;
+    __shared__ __align__(16) uint8_t kcodes[CB];
+    __shared__ __align__(16) uint8_t vcodes[D * VS];
+    __shared__ uint8_t scales[4 * D];   // as in the page: the keys', then the values'
+    const int tid = threadIdx.x, g = blockIdx.x / 8 % a.Hkv, slot = blockIdx.x / 8 / a.Hkv * 8 + blockIdx.x % 8;
+    const int64_t most = min((int64_t)a.maxp * 64, a.n_tab);
+    int s, tile = 0;
+    if (a.cu) {
+        s = ragged::find(slot, a.Bd, [&](int i) { return span(a.cu, a.lens, a.T, most, i).tiles(); }, tile);
+        if (s < 0) return;
+    } else {
+        s = slot;
+        if (s >= a.Bd) return;
+    }
+    const Span x = span(a.cu, a.lens, a.T, most, s);
+    if (x.last <= x.first) return;
+    const int lp = x.first / 64 + tile, p0 = lp * 64;
+    const int ja = max(x.first - p0, 0), jb = min(x.last - p0, 64);   // the page's new tokens
+    const int64_t page = a.table[(int64_t)s * a.maxp + lp];
+    if (page < 0 || page >= a.pages) return;                          // not a page of this cache
+    char *kp = a.kp + (page * a.Hkv + g) * page_bytes(D, F), *vp = a.vp + (page * a.Hkv + g) * page_bytes(D, F);
+    const int jl = tid % TPH, t0 = 4 * jl;
+    const double gain = a.gain ? (double)a.gain[g] : 0.0;
+    float kx[NP][2][4], vx[NP][2][4];
+#pragma unroll
+    for (int pass = 0; pass < NP; ++pass) {
+        if (pass * RPP >= jb || pass * RPP + RPP <= ja) continue;     // uniform
+        const int64_t tok = x.c0 + (p0 + min(max(pass * RPP + tid / TPH, ja), jb - 1) - x.first);
+        const char *kr = a.k + tok * a.kst + g * a.ksh, *vr = a.v + tok * a.vst + g * a.vsh;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            load4<DT>(kx[pass][i], kr + (t0 + i * (D / 2)) * ESZ);
+            load4<DT>(vx[pass][i], vr + (t0 + i * (D / 2)) * ESZ);
+        }
+    }
+#pragma unroll
+    for (int pass = 0; pass < NP; ++pass) {
+        if (pass * RPP >= jb || pass * RPP + RPP <= ja) continue;
+        const int j = pass * RPP + tid / TPH;
+        float(&y)[2][4] = kx[pass];
+        if (a.gain || a.cos) {
+            double z[2][4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) z[i][e] = (double)y[i][e];
+            if (a.gain) {
+                double ss = 0.0;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) ss = fma(z[i][e], z[i][e], ss);
+#pragma unroll
+                for (int o = 1; o < TPH; o <<= 1) ss += __shfl_xor(ss, o, 64);
+                const double f = gain / sqrt(fmax(ss * (1.0 / D), (double)a.eps));
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) z[i][e] *= f;
+            }
+            if (a.cos) {
+                const int64_t pos = (int64_t)(p0 + min(max(j, ja), jb - 1)) * D;
+                float cs[2][4], sn[2][4];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    load4<0>(cs[i], reinterpret_cast<const char *>(a.cos + pos + t0 + i * (D / 2)));
+                    load4<0>(sn[i], reinterpret_cast<const char *>(a.sin + pos + t0 + i * (D / 2)));
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const double lo = z[0][e], hi = z[1][e];
+                    z[0][e] = fma(lo, (double)cs[0][e], -(hi * (double)sn[0][e]));
+                    z[1][e] = fma(hi, (double)cs[1][e], lo * (double)sn[1][e]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[i][e] = (float)z[i][e];
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int t = t0 + i * (D / 2), grp = t / GROUP;
+            const int kb = scale_byte<F>(largest(y[i])), vb = scale_byte<F>(largest(vx[pass][i]));
+            const uint32_t kc = four<F>(y[i], kb), vc = four<F>(vx[pass][i], vb);
+            if constexpr (F == 4) *reinterpret_cast<uint16_t *>(kcodes + At::key(j, t)) = (uint16_t)kc;
+            else *reinterpret_cast<uint32_t *>(kcodes + At::key(j, t)) = kc;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) vcodes[(t + e) * VS + j] = (uint8_t)(F == 4 ? vc >> (4 * e) & 15u : vc >> (8 * e));
+            if (jl % 8 == 0) {
+                scales[At::key_scale(j, grp) - CB] = (uint8_t)kb;
+                scales[2 * D + At::val_scale(j, grp) - CB] = (uint8_t)vb;
+            }
+        }
+    }
+    __syncthreads();
+    for (int c = tid; c < CB / 16; c += 256) {
+        // keys: 8 bytes are of one token
+        constexpr int TB = D / 4 * F / 8;   // bytes of a lane in a tile
+        const int lane = c % 64, b0 = c / 64 * 16;
+        bool in[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int mt = (b0 + 8 * i) / TB, l16 = lane % 16;
+            const int j = 32 * (mt >> 1) + 8 * (l16 >> 2) + 4 * (mt & 1) + (l16 & 3);
+            in[i] = j >= ja && j < jb;
+        }
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(kcodes + 16 * c);
+        if (in[0] && in[1]) {
+            *reinterpret_cast<u32x4 *>(kp + 16 * c) = w;
+        } else {
+            if (in[0]) *reinterpret_cast<u32x2 *>(kp + 16 * c) = u32x2{w[0], w[1]};
+            if (in[1]) *reinterpret_cast<u32x2 *>(kp + 16 * c + 8) = u32x2{w[2], w[3]};
+        }
+        // values: eight tokens of 4 columns, or 2
+        constexpr int PH = D * F / 256;     // pieces of a half
+        const int h = c / 64 / PH, pc = c / 64 % PH, j0 = 32 * h + 8 * (lane / 16);
+        if (j0 + 8 <= ja || j0 >= jb) continue;
+        u32x4 v;
+#pragma unroll
+        for (int i = 0; i < 16 / F; ++i) {
+            const uint32_t *col = reinterpret_cast<const uint32_t *>(vcodes + (16 * (16 / F * pc + i) + lane % 16) * VS + j0);
+            if constexpr (F == 4) {
+                uint32_t lo = col[0], hi = col[1];
+                lo = (lo | lo >> 4) & 0x00ff00ffu;
+                hi = (hi | hi >> 4) & 0x00ff00ffu;
+                v[i] = ((lo | lo >> 8) & 0xffffu) | (hi | hi >> 8) << 16;
+            } else {
+                v[2 * i] = col[0];
+                v[2 * i + 1] = col[1];
+            }
+        }
+        if (j0 < ja || j0 + 8 > jb) {       // the other tokens' codes stay
+            const int lo = max(ja - j0, 0) * F, hi = min(jb - j0, 8) * F;   // bits of the new ones
+            const uint64_t m = (hi == 64 ? ~0ull : (1ull << hi) - 1) & ~((1ull << lo) - 1);
+            const u32x4 old = *reinterpret_cast<const u32x4 *>(vp + 16 * c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t mi = F == 4 || i % 2 == 0 ? (uint32_t)m : (uint32_t)(m >> 32);
+                v[i] = (v[i] & mi) | (old[i] & ~mi);
+            }
+        }
+        *reinterpret_cast<u32x4 *>(vp + 16 * c) = v;
+    }
+    for (int c = tid; c < 2 * D; c += 256) {
+        const int mt = c % 4, l16 = c / 4 % 16;
+        const int jk = 32 * (mt >> 1) + 8 * (l16 >> 2) + 4 * (mt & 1) + (l16 & 3), jv = c / (8 * NG) * 8 + c % 8;
+        if (jk >= ja && jk < jb) kp[CB + c] = (char)scales[c];
+        if (jv >= ja && jv < jb) vp[CB + c] = (char)scales[2 * D + c];
+    }
+}
+
+struct ReadArgs {
+    const char *kp, *vp;
+    const int32_t *cu, *table, *lens;
+    int T, Bd, Hkv, maxp;
+    int64_t pages;
+    char *k, *v;                        // [T, Hkv, D]
+};
+
+// n rows of zeros, the i-th at place at(i) of the batch.
+template <int DT, int D, class At> __device__ __forceinline__ void zero_rows(const ReadArgs &a, int g, int n, const At &at) {
+    constexpr int ESZ = DT == 1 ? 2 : 4, C = D * ESZ / 16;
+    for (int64_t i = threadIdx.x; i < (int64_t)n * C; i += 256) {
+        const int64_t to = ((at((int)(i / C)) * a.Hkv + g) * D) * ESZ + i % C * 16;
+        *reinterpret_cast<uint4 *>(a.k + to) = uint4{0, 0, 0, 0};
+        *reinterpret_cast<uint4 *>(a.v + to) = uint4{0, 0, 0, 0};
+    }
+}
+
+// One workgroup per (page that holds some of the tokens, KV head).  Keys, then values, go
+// through LDS as rows, so that whole rows are written.  Tokens that lie in no page give
+// 0: those of a sequence are tiles behind its pages', those of no sequence (before
+// cu[0], behind cu[Bd]) are left to the workgroups that have nothing else.
+template <int DT, int D, int F> __global__ __launch_bounds__(256) void read_kernel(const ReadArgs a) {
+    typedef typename St<DT>::T T;
+    constexpr int ESZ = DT == 1 ? 2 : 4, NG = D / GROUP, CB = (int)code_bytes(D, F), RS = D + 16 / ESZ;
+    __shared__ __align__(16) T rows[64 * RS];
+    const int tid = threadIdx.x, g = blockIdx.y;
+    const int64_t most = (int64_t)a.maxp * 64;
+    const auto tiles = [&](int i) {
+        const Span x = span(a.cu, a.lens, a.T, most, i);
+        return x.tiles() + (x.n - (x.last - x.first) + 63) / 64;
+    };
+    int tile = 0, s = blockIdx.x;
+    if (a.cu) {
+        s = ragged::find(blockIdx.x, a.Bd, tiles, tile);
+        if (s < 0) {
+            const int used = ragged::total<256>(a.Bd, tiles), w = blockIdx.x - used, of = gridDim.x - used;
+            const int lo = max(0, min(a.T, a.cu[0])), hi = max(lo, min(a.T, a.cu[a.Bd]));
+            const int n = lo + a.T - hi, per = (n + of - 1) / of, i0 = min((int64_t)w * per, (int64_t)n);
+            zero_rows<DT, D>(a, g, min(per, n - i0), [&](int i) { return (int64_t)(i0 + i < lo ? i0 + i : i0 + i - lo + hi); });
+            return;
+        }
+    }
+    const Span x = span(a.cu, a.lens, a.T, most, s);
+    const int np = x.tiles(), lp = x.first / 64 + tile, p0 = lp * 64;
+    const int64_t page = tile < np ? a.table[(int64_t)s * a.maxp + lp] : -1;
+    const int ja = max(x.first - p0, 0), jb = min(x.last - p0, 64);
+    const int64_t at = x.c0 + p0 - x.first;               // the place of the page's token 0
+    if (tile >= np) {
+        const int front = x.c0 - x.from, have = x.last - x.first, i0 = (tile - np) * 64;
+        zero_rows<DT, D>(a, g, min(64, x.n - have - i0),
+                         [&](int i) { return (int64_t)(i0 + i < front ? x.from + i0 + i : x.from + i0 + i + have); });
+        return;
+    }
+    if (page < 0 || page >= a.pages) {                    // not a page of this cache
+        zero_rows<DT, D>(a, g, jb - ja, [&](int i) { return at + ja + i; });
+        return;
+    }
+    const char *kp = a.kp + (page * a.Hkv + g) * page_bytes(D, F), *vp = a.vp + (page * a.Hkv + g) * page_bytes(D, F);
+    const auto write = [&](char *out) {
+        constexpr int C = D * ESZ / 16;
+        for (int i = ja * C + tid; i < jb * C; i += 256)
+            *reinterpret_cast<uint4 *>(out + (((at + i / C) * a.Hkv + g) * D) * ESZ + i % C * 16) =
+                *reinterpret_cast<const uint4 *>(rows + i / C * RS + i % C * (16 / ESZ));
+    };
+    constexpr int TB = D / 4 * F / 8, N8 = 32 / F / 2;    // bytes of a lane in a key tile; runs of 8 codes in a piece
+    for (int c = tid; c < CB / 16; c += 256) {
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(kp + 16 * c);
+        const int lane = c % 64, l16 = lane % 16, lg = lane / 16;
+        const uint32_t sc = *reinterpret_cast<const uint32_t *>(kp + CB + (l16 + 16 * (lg * (D / 4) / GROUP)) * 4);
+#pragma unroll
+        for (int r = 0; r < N8; ++r) {
+            const int b = c / 64 * 16 + r * F, mt = b / TB, t = D / 4 * lg + b % TB * 8 / F;
+            const int j = 32 * (mt >> 1) + 8 * (l16 >> 2) + 4 * (mt & 1) + (l16 & 3);
+            const float scale = __uint_as_float((sc >> (8 * mt) & 255u) << 23);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                St<DT>::st(rows, j * RS + t + e, one<F>(w[F == 4 ? r : 2 * r + (e >> 2)] >> (F * e % 32), scale));
+        }
+    }
+    __syncthreads();
+    write(a.k);
+    __syncthreads();
+    constexpr int PH = D * F / 256;
+    for (int c = tid; c < CB / 16; c += 256) {
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(vp + 16 * c);
+        const int lane = c % 64, h = c / 64 / PH, pc = c / 64 % PH, j0 = 32 * h + 8 * (lane / 16);
+#pragma unroll
+        for (int r = 0; r < N8; ++r) {
+            const int dt = N8 * pc + r, t = 16 * dt + lane % 16;
+            const u32x2 sc = *reinterpret_cast<const u32x2 *>(vp + CB + (j0 / 8 * NG + dt / 2) * 8);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                St<DT>::st(rows, (j0 + e) * RS + t,
+                           one<F>(w[F == 4 ? r : 2 * r + (e >> 2)] >> (F * e % 32),
+                                  __uint_as_float((sc[e >> 2] >> (8 * (e & 3)) & 255u) << 23)));
+        }
+    }
+    __syncthreads();
+    write(a.v);
+}
+
+static int check(int64_t T, int64_t Bd, int64_t Hkv, int64_t d, int64_t Bk, int64_t bits, int64_t max_pages,
+                 int64_t num_pages, const int32_t *cu) {
+    if (d != 64 && d != 128) return HBA_ERR_UNSUPPORTED;
+    if (T < 0 || Bd <= 0 || Hkv <= 0 || max_pages <= 0 || num_pages <= 0 || (!cu && T != Bd)) return HBA_ERR_INVALID_ARG;
+    if (Bk != 64 || (bits != 4 && bits != 8)) return HBA_ERR_UNSUPPORTED;
+    if (T > (1 << 30) || Bd > (1 << 24) || Hkv > 65535 || max_pages > (1 << 24)) return HBA_ERR_UNSUPPORTED;
+    return HBA_OK;
+}
+
+}  // namespace mx
+}  // namespace hba
+
+using namespace hba;
+
+#define HBA_DISPATCH_BITS(dtype, d, bits, M)            \
+    do {                                                \
+        if ((dtype) == HBA_DTYPE_F32) {                 \
+            if ((d) == 64 && (bits) == 4) M(0, 64, 4);  \
+            else if ((d) == 64) M(0, 64, 8);            \
+            else if ((bits) == 4) M(0, 128, 4);         \
+            else M(0, 128, 8);                          \
+        } else {                                        \
+            if ((d) == 64 && (bits) == 4) M(1, 64, 4);  \
+            else if ((d) == 64) M(1, 64, 8);            \
+            else if ((bits) == 4) M(1, 128, 4);         \
+            else M(1, 128, 8);                          \
+        }                                               \
+    } while (0)
+
+extern "C" int hba_kv_append_mx(int dtype, const void *k, const int64_t k_strides[2], const void *v,
+                                const int64_t v_strides[2], const int32_t *cu, int64_t T, const float *k_gain, float eps,
+                                const float *cos_tab, const float *sin_tab, int64_t n_tab, const int32_t *page_table,
+                                int64_t max_pages, const int32_t *seq_lens, int64_t Bd, int64_t Hkv, int64_t d,
+                                int64_t Bk, int64_t bits, int64_t num_pages, void *k_pages, void *v_pages,
+                                void *stream) {
+    if (int st = abi::check_dtype_dim(dtype, d)) return st;
+    if (int st = mx::check(T, Bd, Hkv, d, Bk, bits, max_pages, num_pages, cu)) return st;
+    if (!k || !k_strides || !v || !v_strides || !page_table || !seq_lens || !k_pages || !v_pages || !cos_tab != !sin_tab ||
+        (cos_tab && n_tab <= 0))
+        return HBA_ERR_INVALID_ARG;
+    const int64_t e = abi::elem_size(dtype), al = 16 / e;
+    if (!abi::aligned16(k) || !abi::aligned16(v) || k_strides[0] % al || k_strides[1] % al || v_strides[0] % al ||
+        v_strides[1] % al || !abi::aligned16(cos_tab) || !abi::aligned16(sin_tab) || !abi::aligned16(k_pages) ||
+        !abi::aligned16(v_pages))
+        return HBA_ERR_UNSUPPORTED;
+    if (T == 0) return HBA_OK;
+    mx::AppendArgs a = {};
+    a.k = (const char *)k;
+    a.v = (const char *)v;
+    a.kst = k_strides[0] * e;
+    a.ksh = k_strides[1] * e;
+    a.vst = v_strides[0] * e;
+    a.vsh = v_strides[1] * e;
+    a.cu = cu;
+    a.T = (int)T;
+    a.Bd = (int)Bd;
+    a.Hkv = (int)Hkv;
+    a.maxp = (int)max_pages;
+    a.gain = k_gain;
+    a.cos = cos_tab;
+    a.sin = sin_tab;
+    a.eps = eps;
+    a.n_tab = cos_tab ? n_tab : INT64_MAX;
+    a.pages = num_pages;
+    a.table = page_table;
+    a.lens = seq_lens;
+    a.kp = (char *)k_pages;
+    a.vp = (char *)v_pages;
+    // c tokens touch at most c and at most c / 64 + 2 pages
+    const int64_t slots = !cu || T < T / 64 + 2 * Bd ? T : T / 64 + 2 * Bd, blocks = (slots + 7) / 8 * 8 * Hkv;
+    if (!abi::launchable(blocks, 256)) return HBA_ERR_UNSUPPORTED;
+#define HBA_APPEND_MX(DT, D, F) \
+    hipLaunchKernelGGL((mx::append_kernel<DT, D, F>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a)
+    HBA_DISPATCH_BITS(dtype, d, bits, HBA_APPEND_MX);
+#undef HBA_APPEND_MX
+    HBA_LAUNCH_CHECK();
+    return HBA_OK;
+}
+
+extern "C" int hba_kv_read_mx(int dtype, const void *k_pages, const void *v_pages, int64_t num_pages,
+                              const int32_t *page_table, int64_t max_pages, const int32_t *seq_lens, const int32_t *cu,
+                              int64_t T, int64_t Bd, int64_t Hkv, int64_t d, int64_t Bk, int64_t bits, void *k, void *v,
+                              void *stream) {
+    if (int st = abi::check_dtype_dim(dtype, d)) return st;
+    if (int st = mx::check(T, Bd, Hkv, d, Bk, bits, max_pages, num_pages, cu)) return st;
+    if (!k_pages || !v_pages || !page_table || !seq_lens || !k || !v) return HBA_ERR_INVALID_ARG;
+    if (!abi::aligned16(k) || !abi::aligned16(v) || !abi::aligned16(k_pages) || !abi::aligned16(v_pages))
+        return HBA_ERR_UNSUPPORTED;
+    if (T == 0) return HBA_OK;
+    mx::ReadArgs a = {};
+    a.kp = (const char *)k_pages;
+    a.vp = (const char *)v_pages;
+    a.cu = cu;
+    a.table = page_table;
+    a.lens = seq_lens;
+    a.T = (int)T;
+    a.Bd = (int)Bd;
+    a.Hkv = (int)Hkv;
+    a.maxp = (int)max_pages;
+    a.pages = num_pages;
+    a.k = (char *)k;
+    a.v = (char *)v;
+    // A sequence's c tokens are at most c tiles, and at most c / 64 + 3: pages, and those in
+    // none.  One workgroup more, for tokens of no sequence.
+    const int64_t slots = !cu ? Bd : (T < T / 64 + 3 * Bd ? T : T / 64 + 3 * Bd) + 1;
+    if (!abi::launchable(slots, 256)) return HBA_ERR_UNSUPPORTED;
+#define HBA_READ_MX(DT, D, F)                                                                                      \
+    hipLaunchKernelGGL((mx::read_kernel<DT, D, F>), dim3((unsigned)slots, (unsigned)Hkv), dim3(256), 0,            \
+                       (hipStream_t)stream, a)
+    HBA_DISPATCH_BITS(dtype, d, bits, HBA_READ_MX);
+#undef HBA_READ_MX
+    HBA_LAUNCH_CHECK();
+    return HBA_OK;
+}

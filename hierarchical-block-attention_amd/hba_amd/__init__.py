@@ -11,7 +11,7 @@ from .attention import (aux_kl, build_super, equiv_attention, forward_stages, hb
                         grouped_query, hba_attention_eval, hba_attention_fused, hier_select, selected_mask, sliding_attention)
 from .config import (HBAConfig, content_scale, log_len_tau, resolve_backend, rope_tables,
                      route_scale, union_scale, yarn_theta)
-from .decode import DecodeLoop, PagedKVCache, cache_attention, hba_decode_step
+from .decode import DecodeLoop, MXKVCache, PagedKVCache, cache_attention, hba_decode_step
 from .layer import HBAAttention, attention_by_mode
 from .modules import QKNorm, SlotSummarizer
 
@@ -20,5 +20,5 @@ __all__ = [
     "route_scale", "rope_tables", "yarn_theta", "QKNorm", "SlotSummarizer", "hba_attention_eval",
     "hba_attention_dense", "hba_attention_fused", "build_super", "hier_select", "grouped_query", "forward_stages",
     "selected_mask", "equiv_attention", "aux_kl", "PagedKVCache", "hba_decode_step", "DecodeLoop", "HBAAttention", "attention_by_mode",
-    "sliding_attention", "cache_attention",
+    "sliding_attention", "cache_attention", "MXKVCache",
 ]

@@ -56,11 +56,7 @@ def value_offsets(d, device=None):
 
 class PagedKVCache:
     def __init__(self, cfg, batch, max_len, dtype, device, num_pages=None):
-        self.cfg = cfg
-        self.batch = batch
-        self.max_len = max_len
-        self.max_pages = (max_len + PAGE - 1) // PAGE
-        P = num_pages if num_pages is not None else batch * self.max_pages
+        P = self._init_tables(cfg, batch, max_len, dtype, device, num_pages)
         Hkv, d, m = cfg.n_kv, cfg.head_dim, cfg.slots
         self.kc_pages = torch.zeros(P, Hkv, PAGE * d, dtype=dtype, device=device)
         self.kr_pages = torch.zeros(P, Hkv, PAGE * d, dtype=dtype, device=device)
@@ -68,7 +64,18 @@ class PagedKVCache:
         self._koff = key_offsets(d, device).reshape(-1)
         self._voff = value_offsets(d, device).reshape(-1)
         self.summ_pages = torch.zeros(P, Hkv, m, d, dtype=dtype, device=device)
+        self.scale_table()
+
+    def _init_tables(self, cfg, batch, max_len, dtype, device, num_pages):
+        """Page table, lengths and the host's mirror of both; returns the number of pages."""
+        self.cfg = cfg
+        self.batch = batch
+        self.max_len = max_len
+        self.max_pages = (max_len + PAGE - 1) // PAGE
+        self.dtype = dtype
+        P = num_pages if num_pages is not None else batch * self.max_pages
         self.page_table = torch.zeros(batch, self.max_pages, dtype=torch.int32, device=device)
+        self.device = self.page_table.device
         self.seq_lens = torch.zeros(batch, dtype=torch.int32, device=device)
         self.lens = [0] * batch
         self._table = [[] for _ in range(batch)]
@@ -78,7 +85,7 @@ class PagedKVCache:
         self._scale_tabs = {}
         self._scales = torch.zeros(batch, dtype=torch.float32, device=device)   # written by append
         self._scales_ok = False          # _scales holds the scales of the current lengths
-        self.scale_table()
+        return P
 
     def _ensure_pages(self, s, length):
         need = (length + PAGE - 1) // PAGE
@@ -92,6 +99,12 @@ class PagedKVCache:
             self._table[s].append(p)
             new.append(p)
         return new
+
+    def _give_back(self, taken):
+        """Undo _ensure_pages: its results, for each sequence."""
+        for s, pages in enumerate(taken):
+            del self._table[s][len(self._table[s]) - len(pages):]
+        self._free += [p for pages in reversed(taken) for p in reversed(pages)]
 
     def _sync_table(self):
         self._scales_ok = False
@@ -170,13 +183,24 @@ class PagedKVCache:
         many appends, but that a bf16 kr is rounded once from the fp32 normalised
         key (append: after every step).  Returns the int32 [batch + 1] offsets
         of the sequences' tokens on the device, as cache_attention takes them."""
+        kg, keps = self._key_norm(qkn)
+        return self._extend(k, v, counts, cos, lambda cu, lens: ops.kv_append_ragged(
+            k, v, cu, kg, keps, cos, sin, self.page_table, lens, self.kc_pages, self.kr_pages, self.v_pages, summ.probes,
+            summ.proj, self.summ_pages))
+
+    def _key_norm(self, qkn):
+        """Gains (None: no QKNorm) and epsilon of the keys."""
+        kg = qkn.k.gain if getattr(self.cfg, "qknorm", False) else None
+        return kg, float(qkn.k.eps) if kg is not None else 1e-6
+
+    def _extend(self, k, v, counts, cos, write):
+        """extend, with write(cu, new lengths) to append the tokens to their pages."""
         counts = [int(c) for c in counts]
-        kp = self.kr_pages
         for x, what in ((k, "k"), (v, "v")):
             if x.dim() != 3 or tuple(x.shape[1:]) != (self.cfg.n_kv, self.cfg.head_dim) or x.shape[0] != k.shape[0] \
-                    or x.dtype != kp.dtype or x.device != kp.device:
-                raise ValueError(f"{what}: expected a {kp.dtype} tensor [tokens, {self.cfg.n_kv}, "
-                                 f"{self.cfg.head_dim}] on {kp.device}")
+                    or x.dtype != self.dtype or x.device != self.device:
+                raise ValueError(f"{what}: expected a {self.dtype} tensor [tokens, {self.cfg.n_kv}, "
+                                 f"{self.cfg.head_dim}] on {self.device}")
         if len(counts) != self.batch or min(counts) < 0 or sum(counts) != k.shape[0]:
             raise ValueError(f"counts: expected {self.batch} numbers that sum to the {k.shape[0]} tokens of k")
         need = max(n + c for n, c in zip(self.lens, counts))
@@ -188,7 +212,7 @@ class PagedKVCache:
         for c in counts:
             cu.append(cu[-1] + c)
         if cu[-1] == 0:
-            return torch.zeros(self.batch + 1, dtype=torch.int32, device=self.kc_pages.device)
+            return torch.zeros(self.batch + 1, dtype=torch.int32, device=self.device)
         lens = [n + c for n, c in zip(self.lens, counts)]
         short = sum(max(0, (n + PAGE - 1) // PAGE - len(t)) for n, t in zip(lens, self._table))
         if short > len(self._free):
@@ -198,18 +222,12 @@ class PagedKVCache:
             rows = [t + [0] * (self.max_pages - len(t)) for t in self._table]
             self.page_table.copy_(torch.tensor(rows, dtype=torch.int32))
         # one transfer: the offsets, then the new lengths
-        both = torch.tensor(cu + lens, dtype=torch.int32).to(self.kc_pages.device)
+        both = torch.tensor(cu + lens, dtype=torch.int32).to(self.device)
         cu, new_lens = both[:self.batch + 1], both[self.batch + 1:]
-        cfg = self.cfg
-        kg = qkn.k.gain if getattr(cfg, "qknorm", False) else None
-        keps = float(qkn.k.eps) if kg is not None else 1e-6
         try:
-            ops.kv_append_ragged(k, v, cu, kg, keps, cos, sin, self.page_table, new_lens, self.kc_pages,
-                                 self.kr_pages, self.v_pages, summ.probes, summ.proj, self.summ_pages)
+            write(cu, new_lens)
         except Exception:                # refused: the cache is as it was
-            for s, pages in enumerate(taken):
-                del self._table[s][len(self._table[s]) - len(pages):]
-            self._free += [p for pages in reversed(taken) for p in reversed(pages)]
+            self._give_back(taken)
             raise
         self.seq_lens.copy_(new_lens)    # read by whatever is launched after the append
         self.lens = lens
@@ -262,7 +280,7 @@ class PagedKVCache:
                 first = max(int(n_cal), 1)
                 vals[first:] = [cs * (1.0 + c * math.log(max(L / n_cal, 1.0)))
                                 for L in range(first, self.max_len + 1)]
-            tab = torch.tensor(vals, dtype=torch.float32, device=self.kc_pages.device)
+            tab = torch.tensor(vals, dtype=torch.float32, device=self.device)
             self._scale_tabs[key] = tab
         return tab
 
@@ -274,12 +292,132 @@ class PagedKVCache:
         return torch.index_select(self.scale_table(cfg), 0, self.seq_lens)
 
 
+class MXKVCache(PagedKVCache):
+    """The paged cache in 4 or 8 bits, for dense and window layers: the same page table,
+    lengths, sharing and calls, 4.25 or 8.25 bits an element.
+
+      k_pages [P, Hkv, bytes]  keys, rotated at their own positions, quantised on append
+      v_pages [P, Hkv, bytes]  values
+
+    uint8, ops.mx_page_bytes(head_dim, bits) a page and KV head (hba_amd.h has the
+    format: e2m1 or e4m3 codes with a power of two for every 32 elements).  dtype is the
+    type of the keys, values and queries that come.  cache_attention reads it; the
+    selection's unrotated keys and summaries are not held, so hba_decode_step and
+    DecodeLoop refuse it."""
+
+    def __init__(self, cfg, batch, max_len, dtype, device, bits=4, num_pages=None):
+        if bits not in (4, 8):
+            raise ValueError(f"bits must be 4 or 8, got {bits}")
+        P = self._init_tables(cfg, batch, max_len, dtype, device, num_pages)
+        self.bits = bits
+        nbytes = ops.mx_page_bytes(cfg.head_dim, bits)
+        self.k_pages = torch.zeros(P, cfg.n_kv, nbytes, dtype=torch.uint8, device=device)
+        self.v_pages = torch.zeros(P, cfg.n_kv, nbytes, dtype=torch.uint8, device=device)
+        self.scale_table()
+
+    def load(self, s, kr_seq, v_seq):
+        """Fill sequence s with rotated keys kr_seq and values v_seq [L, Hkv, d] (a
+        prefill's outputs), quantised as they are."""
+        L = kr_seq.shape[0]
+        if self._held.intersection(self._table[s]):
+            raise ValueError(f"sequence {s} begins with pages that others read; load would overwrite them")
+        taken = [[] for _ in range(self.batch)]
+        taken[s] = self._ensure_pages(s, L)
+        rows = torch.tensor(self._table[s] + [0] * (self.max_pages - len(self._table[s])) + [0, L, L], dtype=torch.int32)
+        rows = rows.to(self.device)
+        try:
+            ops.kv_append_mx(kr_seq, v_seq, rows[-3:-1], None, 0.0, None, None, rows[None, :-3], rows[-1:], self.k_pages,
+                             self.v_pages)
+        except Exception:
+            self._give_back(taken)
+            raise
+        self.lens[s] = L
+        self._sync_table()
+
+    def append(self, k_new, v_new, qkn, cos, sin):
+        """Append one token per sequence (raw k_new, v_new [batch, Hkv, d]): no host round
+        trip but for the page-table entry of a page that is allocated."""
+        need = max(self.lens) + 1
+        if need > self.max_len:
+            raise ValueError(f"length {need} exceeds max_len {self.max_len}")
+        if cos.shape[0] < need:
+            raise ValueError(f"cos/sin tables cover {cos.shape[0]} positions, need {need}")
+        if k_new.dtype != self.dtype:
+            raise ValueError(f"k_new: expected {self.dtype}, got {k_new.dtype}")
+        if sum(n % PAGE == 0 and len(t) == n // PAGE for n, t in zip(self.lens, self._table)) > len(self._free):
+            raise RuntimeError("paged KV cache is out of pages")
+        taken = []
+        for s in range(self.batch):
+            first = len(self._table[s])
+            taken.append(self._ensure_pages(s, self.lens[s] + 1))
+            for i, p in enumerate(taken[s]):
+                self.page_table[s, first + i] = p
+        kg, keps = self._key_norm(qkn)
+        lens = self.seq_lens + 1
+        try:
+            ops.kv_append_mx(k_new, v_new, None, kg, keps, cos, sin, self.page_table, lens, self.k_pages, self.v_pages)
+        except Exception:
+            self._give_back(taken)
+            raise
+        self.seq_lens.copy_(lens)
+        self._scales_ok = False
+        for s in range(self.batch):
+            self.lens[s] += 1
+
+    def extend(self, k, v, counts, qkn, cos, sin):
+        """Append counts[s] tokens to each sequence s (raw k, v [sum(counts), Hkv, d], one
+        sequence behind the other; any strides) in one launch.  Returns the int32 [batch +
+        1] offsets of the sequences' tokens on the device, as cache_attention takes them."""
+        kg, keps = self._key_norm(qkn)
+        return self._extend(k, v, counts, cos, lambda cu, lens: ops.kv_append_mx(
+            k, v, cu, kg, keps, cos, sin, self.page_table, lens, self.k_pages, self.v_pages))
+
+    def read(self, counts=None, dtype=None):
+        """The last counts[s] tokens of every sequence (default: all of them) as rows: (k
+        rotated, v, offsets), k and v [sum(counts), Hkv, d] in dtype (default: the cache's)."""
+        counts = list(self.lens) if counts is None else [int(c) for c in counts]
+        if len(counts) != self.batch or any(c < 0 or c > n for c, n in zip(counts, self.lens)):
+            raise ValueError(f"counts: expected {self.batch} numbers from 0 to the sequences' lengths")
+        cu = [0]
+        for c in counts:
+            cu.append(cu[-1] + c)
+        at = torch.tensor(cu, dtype=torch.int32).to(self.device)
+        k, v = ops.kv_read_mx(self.k_pages, self.v_pages, self.page_table, self.seq_lens, at, cu[-1], self.cfg.head_dim,
+                              dtype or self.dtype)
+        return k, v, at
+
+    def _page_rows(self, pages, which):
+        ids = torch.as_tensor(pages, device=self.device).to(torch.int32)
+        n = ids.numel()
+        full = torch.full((n,), PAGE, dtype=torch.int32, device=self.device)
+        cu = torch.arange(0, PAGE * n + 1, PAGE, dtype=torch.int32, device=self.device)
+        rows = ops.kv_read_mx(self.k_pages, self.v_pages, ids.reshape(n, 1).contiguous(), full, cu, PAGE * n,
+                              self.cfg.head_dim, self.dtype)[which]
+        rows = rows.unflatten(0, (n, PAGE)).transpose(1, 2)
+        return rows.reshape(*ids.shape, *rows.shape[1:])
+
+    def key_rows(self, pages, rotated=True):
+        """Rotated keys of physical pages (int or index tensor) as token rows [..., Hkv, 64, d]."""
+        if not rotated:
+            raise ValueError("the cache in 4 or 8 bits holds rotated keys only")
+        return self._page_rows(pages, 0)
+
+    def value_rows(self, pages):
+        return self._page_rows(pages, 1)
+
+
+def _full_precision(cache):
+    if isinstance(cache, MXKVCache):
+        raise TypeError("the block selection needs unrotated keys and summaries: PagedKVCache has them, MXKVCache does not")
+
+
 def hba_decode_step(q, cache, cfg, qkn, cos, sin, scales=None, max_len=None):
     """Union attention of each sequence's new query q [batch, Hq, d] (raw;
     QKNorm and RoPE at position L-1 in the kernel) over the cache.  Returns
     (out [batch, Hq, d], selected page ids [batch, Hkv, k], counts [batch, Hkv]).
     max_len sizes the step's launch (default: the longest sequence; any
     value >= it gives the same selection and an output within rounding)."""
+    _full_precision(cache)
     qg = qkn.q.gain if getattr(cfg, "qknorm", False) else None
     qeps = float(qkn.q.eps) if qg is not None else 1e-6
     sc = cache.scales(cfg) if scales is None else scales
@@ -294,8 +432,8 @@ def hba_decode_step(q, cache, cfg, qkn, cos, sin, scales=None, max_len=None):
 
 def cache_attention(q, cache, cfg, qkn, cos, sin, window=None, sinks=0, cu=None, shared=0, scales=None, max_len=None):
     """Attention of each sequence's newest tokens over the paged cache, no
-    selection: the equiv mode's and a window layer's serving form.  The cache
-    holds the tokens' keys already (append or extend first).  q [T, Hq, d] raw
+    selection: the equiv mode's and a window layer's serving form.  The cache (a
+    PagedKVCache or an MXKVCache) holds the tokens' keys already (append or extend first).  q [T, Hq, d] raw
     (QKNorm, rotation and the union scale of each sequence's length in the
     kernel, as hba_decode_step).  One token per sequence, or with cu (extend's
     result) several.  window None: every key; else the last `window` keys and
@@ -320,6 +458,9 @@ def cache_attention(q, cache, cfg, qkn, cos, sin, window=None, sinks=0, cu=None,
     elif max_len < longest:
         raise ValueError(f"max_len {max_len} is below the longest sequence ({longest})")
     sc = cache.scales(cfg) if scales is None else scales
+    if isinstance(cache, MXKVCache):
+        return ops.paged_attn_mx(q, qg, qeps, cache.k_pages, cache.v_pages, cache.page_table, cache.seq_lens, cos, sin, sc,
+                                 max_len, 0 if window is None else window, sinks, cu, shared)
     return ops.paged_attn(q, qg, qeps, cache.kr_pages, cache.v_pages, cache.page_table, cache.seq_lens, cos, sin, sc,
                           max_len, 0 if window is None else window, sinks, cu, shared)
 
@@ -341,6 +482,7 @@ class DecodeLoop:
     current stream of the cache's device."""
 
     def __init__(self, cache, cfg, qkn, summ, cos, sin, graph=False):
+        _full_precision(cache)
         dev = cache.kc_pages.device
         ops._dev(cache.kc_pages)
         B, Hq, Hkv, d, k = cache.batch, cfg.n_heads, cfg.n_kv, cfg.head_dim, cfg.k_blocks

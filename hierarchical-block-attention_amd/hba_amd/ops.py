@@ -24,8 +24,11 @@ device.
                           (mutates the pages and their summaries)
     hba::paged_attn       attention of new tokens over the paged cache: decode and
                           parts of prompts, whole or windowed, shared first pages
+    hba::kv_append_mx     append to the paged cache in 4 or 8 bits (mutates the pages)
+    hba::kv_read_mx       its tokens as rows
+    hba::paged_attn_mx    paged_attn over it
 
-The last four run past the dispatcher where nothing but the call itself happens
+The last seven run past the dispatcher where nothing but the call itself happens
 (_plain; a call through it costs some 20 us of host time), and through it
 wherever something records or transforms operators.
 """
@@ -96,7 +99,7 @@ def _dev(t):
 # counters), the jit tracer, vmap and the other function transforms.
 _keys = torch._C.DispatchKeySet
 _EAGER = (_keys(torch._C.DispatchKey.BackendSelect) | _keys(torch._C.DispatchKey.ADInplaceOrView)).raw_repr()
-_ARGS = frozenset((Tensor, torch.nn.Parameter, type(None), int, float))
+_ARGS = frozenset((Tensor, torch.nn.Parameter, type(None), int, float, torch.dtype))
 
 
 def _plain(*args):
@@ -1034,14 +1037,24 @@ def _kv_append_ragged_op(k: Tensor, v: Tensor, cu: Tensor, k_gain: Optional[Tens
 
 def _paged_attn(q, q_gain, eps, kr_pages, v_pages, page_table, seq_lens, cos, sin, scales, max_len, window, sinks, cu,
                 shared):
+    return _attend_pages(0, q, q_gain, eps, kr_pages, v_pages, page_table, seq_lens, cos, sin, scales, max_len, window,
+                         sinks, cu, shared)
+
+
+def _attend_pages(mx, q, q_gain, eps, kr_pages, v_pages, page_table, seq_lens, cos, sin, scales, max_len, window, sinks,
+                  cu, shared):
+    """paged_attn, and with mx paged_attn_mx."""
     dev = _dev(q)
     if q.dim() != 3:
         raise ValueError("q: expected [T, Hq, d]")
     T, Hq, d = q.shape
-    P, Hkv = kr_pages.shape[:2]
     code = _code(q)
-    _pages(kr_pages, q.dtype, dev, P, Hkv, BLOCK * d, "kr_pages")
-    _pages(v_pages, q.dtype, dev, P, Hkv, BLOCK * d, "v_pages")
+    if mx:
+        P, Hkv, bits = _mx_pages(kr_pages, v_pages, d, dev)
+    else:
+        P, Hkv = kr_pages.shape[:2]
+        _pages(kr_pages, q.dtype, dev, P, Hkv, BLOCK * d, "kr_pages")
+        _pages(v_pages, q.dtype, dev, P, Hkv, BLOCK * d, "v_pages")
     if Hkv == 0 or Hq % Hkv:
         raise ValueError(f"{Hq} query heads do not divide over {Hkv} KV heads")
     if page_table.dim() != 2:
@@ -1078,10 +1091,16 @@ def _paged_attn(q, q_gain, eps, kr_pages, v_pages, page_table, seq_lens, cos, si
     nbytes = nbytes.value
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     with _on(dev):
-        st = L.hba_paged_attn(code, _p(q), used_strides2(q), _p(qg), eps, _p(cos), _p(sin), n_tab, _p(kr_pages),
-                              _p(v_pages), P, _p(page_table), maxp, _p(seq_lens), _p(sc), _p(cu), T, Bd, Hq, Hkv, d,
-                              BLOCK, window, sinks, shared // BLOCK, max_len, _p(ws), nbytes, _p(out), _stream(dev))
-    check(st, "hba_paged_attn")
+        if mx:
+            st = L.hba_paged_attn_mx(code, _p(q), used_strides2(q), _p(qg), eps, _p(cos), _p(sin), n_tab, bits,
+                                     _p(kr_pages), _p(v_pages), P, _p(page_table), maxp, _p(seq_lens), _p(sc), _p(cu), T,
+                                     Bd, Hq, Hkv, d, BLOCK, window, sinks, shared // BLOCK, max_len, _p(ws), nbytes,
+                                     _p(out), _stream(dev))
+        else:
+            st = L.hba_paged_attn(code, _p(q), used_strides2(q), _p(qg), eps, _p(cos), _p(sin), n_tab, _p(kr_pages),
+                                  _p(v_pages), P, _p(page_table), maxp, _p(seq_lens), _p(sc), _p(cu), T, Bd, Hq, Hkv, d,
+                                  BLOCK, window, sinks, shared // BLOCK, max_len, _p(ws), nbytes, _p(out), _stream(dev))
+    check(st, "hba_paged_attn_mx" if mx else "hba_paged_attn")
     return out
 
 
@@ -1101,21 +1120,24 @@ def paged_attn(q, q_gain, eps, kr_pages, v_pages, page_table, seq_lens, cos, sin
     There is no backward pass: asking for one raises."""
     args = (q, q_gain, eps, kr_pages, v_pages, page_table, seq_lens, cos, sin, scales, max_len, window, sinks, cu, shared)
     if _differentiated(q, q_gain, kr_pages, v_pages, cos, sin, scales) and not torch.compiler.is_dynamo_compiling():
-        return _PagedAttn.apply(*args)   # torch.compile would trace its backward; the registered operator's raises too
+        return _PagedAttn.apply(0, *args)   # torch.compile would trace its backward; the registered operator's raises too
     return (_paged_attn if _plain(*args) else torch.ops.hba.paged_attn)(*args)
 
 
 class _PagedAttn(torch.autograd.Function):
-    """paged_attn of tensors that a derivative may be asked for: there is none, and
-    neither a gradient nor a tangent is dropped without an error."""
+    """paged_attn (mx: paged_attn_mx) of tensors that a derivative may be asked for: there
+    is none, and neither a gradient nor a tangent is dropped without an error."""
 
     @staticmethod
-    def forward(ctx, *args):
+    def forward(ctx, mx, *args):
+        ctx.name = "paged_attn_mx" if mx else "paged_attn"
+        if mx:
+            return (_paged_attn_mx if _plain(*args) else torch.ops.hba.paged_attn_mx)(*args)
         return (_paged_attn if _plain(*args) else torch.ops.hba.paged_attn)(*args)
 
     @staticmethod
     def backward(ctx, dout):
-        raise NotImplementedError("paged_attn has no backward pass")
+        raise NotImplementedError(f"{ctx.name} has no backward pass")
 
 
 @torch.library.custom_op("hba::paged_attn", mutates_args=(), device_types="cuda")
@@ -1129,5 +1151,165 @@ def _paged_attn_op(q: Tensor, q_gain: Optional[Tensor], eps: float, kr_pages: Te
 
 @_paged_attn_op.register_fake
 def _(q, q_gain, eps, kr_pages, v_pages, page_table, seq_lens, cos, sin, scales, max_len, window=0, sinks=0, cu=None,
+      shared=0):
+    return q.new_empty(q.shape)
+
+
+# ------------------------------------------------- the paged cache in 4 or 8 bits ----
+def mx_page_bytes(d, bits):
+    """Bytes of a page and KV head (64 tokens) of the cache in 4 or 8 bits: the codes, and
+    a scale byte for every 32 elements."""
+    return BLOCK * d * bits // 8 + 2 * d
+
+
+def _mx_pages(k_pages, v_pages, d, dev):
+    """Checks the pages; returns (pages, KV heads, bits)."""
+    for t, what in ((k_pages, "k_pages"), (v_pages, "v_pages")):
+        if t.dtype != torch.uint8 or t.device != dev or not t.is_contiguous() or t.dim() != 3:
+            raise ValueError(f"{what} must be a contiguous uint8 tensor [pages, KV heads, bytes] on {dev}")
+        if t.shape != k_pages.shape or t.shape[0] == 0 or t.shape[1] == 0:
+            raise ValueError(f"{what}: expected the shape of k_pages, and a page and a KV head at least")
+    for bits in (4, 8):
+        if k_pages.shape[2] == mx_page_bytes(d, bits):
+            return k_pages.shape[0], k_pages.shape[1], bits
+    raise ValueError(f"k_pages: {k_pages.shape[2]} bytes per page and KV head; head dim {d} has {mx_page_bytes(d, 4)} "
+                     f"(4 bits) or {mx_page_bytes(d, 8)} (8 bits)")
+
+
+def _mx_batch(page_table, seq_lens, cu, T, dev):
+    """Checks a ragged batch's page table, lengths and offsets; returns (sequences, max_pages)."""
+    if page_table.dim() != 2:
+        raise ValueError("page_table: expected [Bd, max_pages]")
+    Bd, maxp = page_table.shape
+    _i32(page_table, (Bd, maxp), dev, "page_table")
+    _i32(seq_lens, (Bd,), dev, "seq_lens")
+    if cu is not None:
+        _i32(cu, (Bd + 1,), dev, "cu")
+    elif T != Bd:
+        raise ValueError(f"one token per sequence expected: {T} tokens, {Bd} sequences (give cu for more)")
+    return Bd, maxp
+
+
+def _kv_append_mx(k, v, cu, k_gain, eps, cos, sin, page_table, seq_lens, k_pages, v_pages):
+    dev = _dev(k)
+    if k.dim() != 3 or v.shape != k.shape or v.dtype != k.dtype or v.device != dev:
+        raise ValueError("k and v: expected two [T, Hkv, d] tensors of one type and device")
+    T, Hkv, d = k.shape
+    code = _code(k)
+    P, heads, bits = _mx_pages(k_pages, v_pages, d, dev)
+    if heads != Hkv:
+        raise ValueError(f"the pages have {heads} KV heads, k and v {Hkv}")
+    Bd, maxp = _mx_batch(page_table, seq_lens, cu, T, dev)
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin go together")
+    n_tab = 0
+    if cos is not None:
+        cos, sin = _tables(cos, sin, 1, d, dev)
+        n_tab = cos.shape[0]
+    kg = _f32c(k_gain, dev, Hkv, "k_gain")
+    if T == 0 or Bd == 0:
+        return
+    k, v = _rows16(k), _rows16(v)
+    with _on(dev):
+        st = lib().hba_kv_append_mx(code, _p(k), used_strides2(k), _p(v), used_strides2(v), _p(cu), T, _p(kg), eps, _p(cos),
+                                    _p(sin), n_tab, _p(page_table), maxp, _p(seq_lens), Bd, Hkv, d, BLOCK, bits, P,
+                                    _p(k_pages), _p(v_pages), _stream(dev))
+    check(st, "hba_kv_append_mx")
+
+
+def kv_append_mx(k, v, cu, k_gain, eps, cos, sin, page_table, seq_lens, k_pages, v_pages):
+    """Append tokens to the paged cache in 4 or 8 bits (k_pages, v_pages uint8 [P, Hkv,
+    mx_page_bytes(d, bits)]; hba_amd.h has the format): k, v [T, Hkv, d] raw, any
+    strides; QKNorm (k_gain None: none), the rotation at each token's position (cos
+    None: none), quantised.  cu int32 [Bd + 1]: tokens cu[s] .. cu[s + 1] - 1 are the last
+    ones of sequence s, whose length seq_lens[s] counts them already; None: one token per
+    sequence, T = Bd.  Positions past the page table or the cos/sin tables, and tokens
+    behind cu[Bd] (a padded batch), are not appended; a page belongs to one sequence
+    while tokens are appended to it."""
+    args = (k, v, cu, k_gain, eps, cos, sin, page_table, seq_lens, k_pages, v_pages)
+    if not _plain(*args):
+        torch.ops.hba.kv_append_mx(*args)
+        return
+    _kv_append_mx(*args)
+    written = [t for t in (k_pages, v_pages) if not t.is_inference()]
+    torch.autograd.graph.increment_version(written)
+
+
+@torch.library.custom_op("hba::kv_append_mx", mutates_args=("k_pages", "v_pages"), device_types="cuda")
+def _kv_append_mx_op(k: Tensor, v: Tensor, cu: Optional[Tensor], k_gain: Optional[Tensor], eps: float,
+                     cos: Optional[Tensor], sin: Optional[Tensor], page_table: Tensor, seq_lens: Tensor, k_pages: Tensor,
+                     v_pages: Tensor) -> None:
+    _kv_append_mx(k, v, cu, k_gain, eps, cos, sin, page_table, seq_lens, k_pages, v_pages)
+
+
+def _kv_read_mx(k_pages, v_pages, page_table, seq_lens, cu, tokens, head_dim, dtype):
+    dev = _dev(k_pages)
+    if dtype not in _DT:
+        raise TypeError(f"unsupported dtype {dtype}: rows are float32 or bfloat16")
+    if tokens < 0:
+        raise ValueError(f"tokens must not be negative, got {tokens}")
+    P, Hkv, bits = _mx_pages(k_pages, v_pages, head_dim, dev)
+    Bd, maxp = _mx_batch(page_table, seq_lens, cu, tokens, dev)
+    k, v = (torch.empty(tokens, Hkv, head_dim, dtype=dtype, device=dev) for _ in range(2))
+    if tokens == 0:
+        return k, v
+    if Bd == 0:
+        return k.zero_(), v.zero_()
+    with _on(dev):
+        st = lib().hba_kv_read_mx(_DT[dtype], _p(k_pages), _p(v_pages), P, _p(page_table), maxp, _p(seq_lens), _p(cu),
+                                  tokens, Bd, Hkv, head_dim, BLOCK, bits, _p(k), _p(v), _stream(dev))
+    check(st, "hba_kv_read_mx")
+    return k, v
+
+
+def kv_read_mx(k_pages, v_pages, page_table, seq_lens, cu, tokens, head_dim, dtype):
+    """The cache in 4 or 8 bits as rows (k, v) [tokens, Hkv, head_dim] of float32 or
+    bfloat16 (which holds every value): tokens cu[s] .. cu[s + 1] - 1 are the last ones of
+    sequence s, as kv_append_mx takes them; cu None: the newest of each.  Keys come as they
+    lie there, rotated.  Tokens that lie in no page of the cache give 0."""
+    args = (k_pages, v_pages, page_table, seq_lens, cu, tokens, head_dim, dtype)
+    return (_kv_read_mx if _plain(*args) else torch.ops.hba.kv_read_mx)(*args)
+
+
+@torch.library.custom_op("hba::kv_read_mx", mutates_args=(), device_types="cuda")
+def _kv_read_mx_op(k_pages: Tensor, v_pages: Tensor, page_table: Tensor, seq_lens: Tensor, cu: Optional[Tensor], tokens: int,
+                   head_dim: int, dtype: torch.dtype) -> Tuple[Tensor, Tensor]:
+    return _kv_read_mx(k_pages, v_pages, page_table, seq_lens, cu, tokens, head_dim, dtype)
+
+
+@_kv_read_mx_op.register_fake
+def _(k_pages, v_pages, page_table, seq_lens, cu, tokens, head_dim, dtype):
+    shape = (tokens, k_pages.shape[1], head_dim)
+    return k_pages.new_empty(shape, dtype=dtype), k_pages.new_empty(shape, dtype=dtype)
+
+
+def _paged_attn_mx(q, q_gain, eps, k_pages, v_pages, page_table, seq_lens, cos, sin, scales, max_len, window, sinks, cu,
+                   shared):
+    return _attend_pages(1, q, q_gain, eps, k_pages, v_pages, page_table, seq_lens, cos, sin, scales, max_len, window,
+                         sinks, cu, shared)
+
+
+def paged_attn_mx(q, q_gain, eps, k_pages, v_pages, page_table, seq_lens, cos, sin, scales, max_len, window=0, sinks=0,
+                  cu=None, shared=0):
+    """paged_attn over the cache in 4 or 8 bits (k_pages, v_pages as kv_append_mx writes
+    them): the same arguments and result.  There is no backward pass: asking for one
+    raises."""
+    args = (q, q_gain, eps, k_pages, v_pages, page_table, seq_lens, cos, sin, scales, max_len, window, sinks, cu, shared)
+    if _differentiated(q, q_gain, cos, sin, scales) and not torch.compiler.is_dynamo_compiling():
+        return _PagedAttn.apply(1, *args)
+    return (_paged_attn_mx if _plain(*args) else torch.ops.hba.paged_attn_mx)(*args)
+
+
+@torch.library.custom_op("hba::paged_attn_mx", mutates_args=(), device_types="cuda")
+def _paged_attn_mx_op(q: Tensor, q_gain: Optional[Tensor], eps: float, k_pages: Tensor, v_pages: Tensor,
+                      page_table: Tensor, seq_lens: Tensor, cos: Optional[Tensor], sin: Optional[Tensor],
+                      scales: Tensor, max_len: int, window: int = 0, sinks: int = 0, cu: Optional[Tensor] = None,
+                      shared: int = 0) -> Tensor:
+    return _paged_attn_mx(q, q_gain, eps, k_pages, v_pages, page_table, seq_lens, cos, sin, scales, max_len, window, sinks,
+                          cu, shared)
+
+
+@_paged_attn_mx_op.register_fake
+def _(q, q_gain, eps, k_pages, v_pages, page_table, seq_lens, cos, sin, scales, max_len, window=0, sinks=0, cu=None,
       shared=0):
     return q.new_empty(q.shape)

@@ -553,6 +553,66 @@ int hba_paged_attn(int dtype, const void *q, const int64_t q_strides[2], const f
                    int64_t max_len, void *workspace, size_t ws_bytes, void *out, void *stream);
 
 /*
+ * The paged cache in 4 or 8 bits (bits): k_pages, v_pages uint8 [P, Hkv,
+ * 64*d*bits/8 + 2*d], rotated keys and values; the page table, the lengths and cu are
+ * the paged cache's.  Elements are e2m1 (4 bits) or e4m3 (8 bits) codes, times a power
+ * of two 2^(b - 127) that the elements 32 g .. 32 g + 31 of a token's head share (the
+ * formats of the OCP Microscaling specification).  b is the smallest byte >= 1 for which
+ * the group's largest magnitude is at most 1.75 * 2^emax times it (e2m1: 7, where more
+ * than 6 becomes 6; e4m3: 448), codes are the nearest ones (ties to even); a group of
+ * zeros has b = 0 and codes 0, one that holds a NaN, an infinity or a magnitude over
+ * 1.75 * 2^127 b = 255 and codes 0 and reads as NaN.  Within a page and KV head, token j's element t, and its group's byte:
+ *   keys    mt = 2*(j/32) + (j/4)%2, l16 = 4*((j%32)/8) + j%4: byte x = (mt*(d/4) + t%(d/4))
+ *           * bits/8 of lane l16 + 16*(t/(d/4)); b at 64*d*bits/8 + (l16 + 16*(t/32))*4 + mt;
+ *   values  byte x = (j/32)*(d*bits/16) + ((t/16)*8 + j%8) * bits/8 of lane t%16 +
+ *           16*((j%32)/8); b at 64*d*bits/8 + ((j/8)*(d/32) + t/32)*8 + j%8;
+ * byte x of lane L lies at (x/16*64 + L)*16 + x%16; in 4 bits the even element of a key
+ * (token of a value) is the low half.
+ */
+
+/*
+ * Append tokens to it: QKNorm of k (k_gain; NULL: none), its rotation at the token's
+ * position (cos_tab, sin_tab; NULL: none), both in fp64 and rounded to fp32 once, quantised
+ * into k_pages, v quantised into v_pages.  k, v: element strides of token and head, rows
+ * on 16-byte boundaries.  cu int32 [Bd+1]: tokens cu[s] .. cu[s+1]-1 are the last ones of
+ * sequence s, whose seq_lens[s] counts them already; NULL: one token per sequence (T =
+ * Bd), the newest.  What is not appended, and what stays, is as for hba_kv_append_ragged.
+ * No counterpart in the reference, which has no KV cache.
+ */
+int hba_kv_append_mx(int dtype, const void *k, const int64_t k_strides[2], const void *v,
+                     const int64_t v_strides[2], const int32_t *cu, int64_t T, const float *k_gain,
+                     float eps, const float *cos_tab, const float *sin_tab, int64_t n_tab,
+                     const int32_t *page_table, int64_t max_pages, const int32_t *seq_lens,
+                     int64_t Bd, int64_t Hkv, int64_t d, int64_t Bk, int64_t bits, int64_t num_pages,
+                     void *k_pages, void *v_pages, void *stream);
+
+/*
+ * Read tokens back as rows k, v [T, Hkv, d] (contiguous; fp32, or bf16, which holds
+ * every value): those that hba_kv_append_mx would write with the same cu and seq_lens.
+ * Tokens at positions < 0 or past the page table, on a page outside 0 .. num_pages-1,
+ * before cu[0] or behind cu[Bd] (a padded batch) give 0.
+ */
+int hba_kv_read_mx(int dtype, const void *k_pages, const void *v_pages, int64_t num_pages,
+                   const int32_t *page_table, int64_t max_pages, const int32_t *seq_lens,
+                   const int32_t *cu, int64_t T, int64_t Bd, int64_t Hkv, int64_t d, int64_t Bk,
+                   int64_t bits, void *k, void *v, void *stream);
+
+/*
+ * hba_paged_attn over it: the same arguments (workspace: hba_paged_attn_workspace_bytes),
+ * the same rules.  Keys and values enter the products as they are (bf16 holds them);
+ * fp32: queries and probabilities in three bf16 parts (24 bits of mantissa).  Values
+ * behind a sequence's length may be anything.  A NaN before it has no effect on tokens
+ * that do not see it (with cu as there: slow for those beside it).
+ */
+int hba_paged_attn_mx(int dtype, const void *q, const int64_t q_strides[2], const float *q_gain,
+                      float eps, const float *cos_tab, const float *sin_tab, int64_t n_tab,
+                      int64_t bits, const void *k_pages, const void *v_pages, int64_t num_pages,
+                      const int32_t *page_table, int64_t max_pages, const int32_t *seq_lens,
+                      const float *scales, const int32_t *cu, int64_t T, int64_t Bd, int64_t Hq,
+                      int64_t Hkv, int64_t d, int64_t Bk, int64_t W, int64_t S, int64_t shared_pages,
+                      int64_t max_len, void *workspace, size_t ws_bytes, void *out, void *stream);
+
+/*
  * Sliding-window attention with sinks (a model's window layers): query i of
  * q [B, n, Hq, d] attends to the keys j <= i with j > i - W or j < S of k, v
  * [B, n, Hkv, d], all with element strides (rows on 16-byte boundaries; keys and
