@@ -30,6 +30,13 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x6 __attribute__((ext_vector_type(6)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+using hba::f32x16;
+typedef float f32x32 __attribute__((ext_vector_type(32)));
+template <int N> struct number {
+    static constexpr int value = N;
+};
 
 constexpr int GROUP = 32;
 constexpr int64_t code_bytes(int64_t d, int bits) { return 64 * d * bits / 8; }
@@ -79,12 +86,37 @@ template <int F> __device__ __forceinline__ bf16x8 eight(const uint32_t *w, floa
     const auto a = __builtin_shufflevector(p[0], p[1], 0, 1, 2, 3), b = __builtin_shufflevector(p[2], p[3], 0, 1, 2, 3);
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
+// c + a 16x16 product over 128 elements: e2m1 codes with byte KB of ks as their scale
+// (lane l: row l % 16, elements 32 (l / 16) ..), e2m3 with byte QB of qs (columns).
+template <int KB, int QB> __device__ __forceinline__ f32x4 product6(u32x4 k, i32x8 q, f32x4 c, int ks, int qs) {
+    const i32x8 a = {(int)k[0], (int)k[1], (int)k[2], (int)k[3], 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q, c, 4, 2, KB, ks, QB, qs);
+}
 // One code (the low F bits) as fp32, exact.
 template <int F> __device__ __forceinline__ float one(uint32_t code, float scale) {
     f32x2 r;
     if constexpr (F == 4) r = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, scale, 0);
     else r = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(code, scale, false);
     return r[0];
+}
+
+// `bytes` of memory from a wave-uniform address on, for loads at a lane's 32-bit offset: no
+// 64-bit addresses in vector registers, whose reuse would have to wait for loads.
+typedef __amdgpu_buffer_rsrc_t Buffer;
+__device__ __forceinline__ Buffer buffer(const char *p, int bytes) {
+    const uint64_t a = (uint64_t)(uintptr_t)p;
+    const uint64_t u = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(a >> 32)) << 32 |
+                       (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)a);
+    return __builtin_amdgcn_make_buffer_rsrc((void *)(uintptr_t)u, 0, bytes, 0x00027000);
+}
+__device__ __forceinline__ u32x4 load16(Buffer b, uint32_t lane, uint32_t at) {
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(b, lane + at, 0, 0));
+}
+__device__ __forceinline__ u32x2 load8(Buffer b, uint32_t lane, uint32_t at) {
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(b, lane + at, 0, 0));
+}
+__device__ __forceinline__ uint32_t load4(Buffer b, uint32_t lane, uint32_t at) {
+    return __builtin_amdgcn_raw_buffer_load_b32(b, lane + at, 0, 0);
 }
 
 // ------------------------------------------------------------ staged tiles --

@@ -87,7 +87,7 @@ __device__ __forceinline__ uint32_t largest(const float (&x)[4]) {
     for (int o = 1; o < 8; o <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
     return m;
 }
-template <int DT> __device__ __forceinline__ void load4(float (&x)[4], const char *p) {
+template <int DT> __device__ __forceinline__ void four_of(float (&x)[4], const char *p) {
     if constexpr (DT == 1) {
         const uint2 w = *reinterpret_cast<const uint2 *>(p);
         x[0] = __uint_as_float(w.x << 16);
@@ -146,8 +146,8 @@ template <int DT, int D, int F> __global__ __launch_bounds__(256) void append_ke
         const char *kr = a.k + tok * a.kst + g * a.ksh, *vr = a.v + tok * a.vst + g * a.vsh;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            load4<DT>(kx[pass][i], kr + (t0 + i * (D / 2)) * ESZ);
-            load4<DT>(vx[pass][i], vr + (t0 + i * (D / 2)) * ESZ);
+            four_of<DT>(kx[pass][i], kr + (t0 + i * (D / 2)) * ESZ);
+            four_of<DT>(vx[pass][i], vr + (t0 + i * (D / 2)) * ESZ);
         }
     }
 #pragma unroll
@@ -180,8 +180,8 @@ template <int DT, int D, int F> __global__ __launch_bounds__(256) void append_ke
                 float cs[2][4], sn[2][4];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    load4<0>(cs[i], reinterpret_cast<const char *>(a.cos + pos + t0 + i * (D / 2)));
-                    load4<0>(sn[i], reinterpret_cast<const char *>(a.sin + pos + t0 + i * (D / 2)));
+                    four_of<0>(cs[i], reinterpret_cast<const char *>(a.cos + pos + t0 + i * (D / 2)));
+                    four_of<0>(sn[i], reinterpret_cast<const char *>(a.sin + pos + t0 + i * (D / 2)));
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {

@@ -61,6 +61,7 @@ struct Args {
     // parts: [T, Hq, slots, D] sums, [T, Hq, slots, 2] maximum (log2 units) and sum; of even shares (slots of
     // them, part pages at least): [slots, 2, 16, D] and [slots, 2, 16, 2], see even_kernel
     float *po, *pml;
+    int *records;                       // of even shares of codes, see even_codes_kernel
 };
 
 // A row's position and what it sees of its sequence.
@@ -141,30 +142,99 @@ __device__ __forceinline__ Pages page_list(const Args &a, int L) {
     return p;
 }
 
-// The same over codes.  A unit's codes are a few registers; they become operands as they
-// are used.  Keys: with their scales, by one instruction a pair.  Values: a lane's eight
-// tokens have eight scales in each group, so those go into the weights instead (a
-// power of two: nothing is rounded), a set of weights for each group.  A key that is
-// not seen has logit -infinity; its value, a weight and a scale of 0.  So what is not
-// finite there has no effect, at no cost.
-template <int DT, int D, int DW, int FMT>
+// ------------------------------------------------------------ decode, codes --
+// A query's 32 elements of a group as N parts of e2m3 (6 bits), each with a power of two
+// of its own: the largest magnitude goes to (3.75, 7.5], what the rounding leaves (1/4 of
+// the first unit at most) times 2^4, of every later one times 2^5.  N parts leave at most
+// 2^-(5 N - 1.1) of the largest magnitude (3 of bf16 queries: 2^-13.9).
+template <int N> struct Query6 {
+    mx::u32x6 q[N];
+    int scale[N];   // bytes
+};
+template <int N> __device__ __forceinline__ Query6<N> parts6(const float (&y)[32]) {
+    Query6<N> r;
+    uint32_t big = 0;
+#pragma unroll
+    for (int e = 0; e < 32; ++e) big = max(big, __float_as_uint(y[e]) & 0x7fffffffu);
+    const int b = (int)(big >> 23) - 2 + ((big & 0x7fffffu) > 0x700000u);
+    const bool bad = big >= 0x7f800000u;   // 255 makes every logit NaN
+    mx::f32x16 x[2];                       // even and odd elements, as the conversion takes them
+#pragma unroll
+    for (int e = 0; e < 32; ++e) x[e & 1][e >> 1] = bad ? 0.0f : y[e];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        r.scale[n] = bad ? 255 : max(n == 0 ? b : b + 1 - 5 * n, 1);
+        const float f = __uint_as_float((uint32_t)(bad ? 127 : r.scale[n]) << 23);
+        r.q[n] = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(x[0], x[1], f);
+        const mx::f32x32 back = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(r.q[n], f);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) x[e & 1][e >> 1] -= back[e];
+    }
+    return r;
+}
+
+// QKNorm, rotation (cs, sn: the lane's; y: the elements half a head away) and scale of a
+// lane's N consecutive elements x of a head; lanes 16 and (ALL) 32 away have the others.
+template <int D, int N, bool ALL>
+__device__ __forceinline__ void finish_group(float (&x)[N], const float (&y)[N], bool first_half, const float *gain,
+                                             float eps, bool turn, const float (&cs)[N], const float (&sn)[N],
+                                             float scale) {
+    if (gain) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int e = 0; e < N; ++e) ss = fmaf(x[e], x[e], ss);
+        ss += rows::other_row(ss);
+        if constexpr (ALL) ss += rows::other_half(ss);
+        scale *= *gain / sqrtf(fmaxf(ss / (float)D, eps));
+    }
+    if (turn) {
+        const float sign = first_half ? -1.0f : 1.0f;
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] = x[e] * cs[e] + y[e] * (sign * sn[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] *= scale;
+}
+
+// decode_part's walk over codes.  A unit's codes are a few registers; they become
+// operands as they are used.
+//   keys, 4 bits   go to the matrix cores as they are, with their scales; the queries are
+//                  e2m3 parts, whose products with e2m1 are summed like fp32's.  (e4m3
+//                  products are not: they lose bits below 2^-14 of the largest.)
+//   keys, 8 bits   bf16 by one instruction a pair, scales included; queries in bf16 parts
+//   values         bf16, without their scales: a lane's eight tokens have eight in each
+//                  group, which go into the weights instead (a power of two: nothing is
+//                  rounded), a set of weights for each group.
+// With 8 heads or less (NS = 2) the columns 8 .. 15 are the same heads again: their lanes
+// make the weights of the other half of the groups.
+// A key that is not seen has logit -infinity; its value's codes and scale are 0.  So
+// what is not finite there has no effect, at no cost.
+template <int DT, int D, int DW, int FMT, int NS>
 __device__ __forceinline__ void decode_codes(const Args &a, int s, int g, int head, int L, int p0, int p1,
                                              f32x4 (&O)[D / 16], float &m, float &l) {
     constexpr int ESZ = DT == 1 ? 2 : 4, UK = FMT == 8 && D == 128 ? 32 : 64;
-    constexpr int NKS = D / 32, NDT = D / 16, NG = D / mx::GROUP, NH = UK / 32, UP = rows::PAGE / UK;
-    constexpr int NQ = DT == 1 ? 2 : 3, NP = DT == 1 ? 1 : 3;   // bf16 parts of a query, of a weight
-    constexpr int E = D / 4, KP = D * FMT / 256;                // codes of a lane in a tile; its 16-byte pieces of 32 tokens
+    constexpr int NDT = D / 16, NG = D / mx::GROUP, NH = UK / 32, UP = rows::PAGE / UK, NL = NG / NS;
+    constexpr int NP = DT == 1 ? 1 : 3;                  // bf16 parts of a weight
+    constexpr int NQ = FMT == 8 ? (DT == 1 ? 2 : 3) : DT == 0 ? 6 : D == 128 ? 3 : 4;   // parts of a query
+    constexpr int NM = FMT == 4 && D == 64 ? NQ / 2 : NQ;   // D = 64: two parts in one product's 128 elements
+    constexpr int NKS = FMT == 8 ? D / 32 : 1;
+    constexpr int E = D / 4, KP = D * FMT / 256;         // codes of a lane in a tile; its 16-byte pieces of 32 tokens
     typedef const __attribute__((address_space(4))) int32_t *uniform;
     const int lane = threadIdx.x & 63, l16 = lane & 15, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kg = FMT == 4 ? lg % NG : lg * E / mx::GROUP;   // the group of a lane's key elements
     const Pages pg = page_list(a, L);
     const int u0 = p0 * UP, u1 = min(pg.n, p1) * UP;
     const char *kb = a.kr + (int64_t)g * HEAD_BYTES<DT, D, FMT>, *vb = a.v + (int64_t)g * HEAD_BYTES<DT, D, FMT>;
     const int64_t pstep = (int64_t)a.Hkv * HEAD_BYTES<DT, D, FMT>;
     const uniform table = (uniform)(uintptr_t)(a.table + (int64_t)s * a.maxp);
+    // a lane's offsets in a page: codes (of 4-bit keys at D = 64 the halves of a group), scales
+    const uint32_t co = lane * 16, k64 = (l16 + 32 * kg) * 16, ko = (l16 + 16 * kg) * 4;
+    const uint32_t vo = (lg * NG + (NS == 2 ? (l16 >> 3) * NL : 0)) * 8;
 
     struct Unit {
-        mx::u32x4 k[NH * KP], v[NH * KP], vs[NH][NG / 2];
+        mx::u32x4 k[FMT == 4 ? 2 * NH : NH * KP], v[NH * KP];
+        mx::u32x2 vs[NH][NL];
         uint32_t ks;
     };
     const auto logical = [&](int u) {
@@ -174,60 +244,133 @@ __device__ __forceinline__ void decode_codes(const Args &a, int s, int g, int he
     const auto place = [&](int u) { return max((int64_t)0, min((int64_t)table[logical(u)], a.pages - 1)); };
     const auto load = [&](Unit &x, int u, int64_t id) {
         const int h0 = UP == 1 ? 0 : u % UP;
-        const char *kp = kb + id * pstep, *vp = vb + id * pstep;
+        constexpr int HB = (int)HEAD_BYTES<DT, D, FMT>, CB = (int)mx::code_bytes(D, FMT);
+        const mx::Buffer kp = mx::buffer(kb + id * pstep, HB), vp = mx::buffer(vb + id * pstep, HB);
+        const uint32_t from = co + h0 * (KP * 1024);
+        if constexpr (FMT == 4 && D == 64) {
 #pragma unroll
-        for (int i = 0; i < NH * KP; ++i) {
-            x.k[i] = *reinterpret_cast<const mx::u32x4 *>(kp + ((h0 * KP + i) * 64 + lane) * 16);
-            x.v[i] = *reinterpret_cast<const mx::u32x4 *>(vp + ((h0 * KP + i) * 64 + lane) * 16);
+            for (int mt = 0; mt < 4; ++mt) {
+                const mx::u32x2 lo = mx::load8(kp, k64, mt / 2 * 1024 + mt % 2 * 8);
+                const mx::u32x2 hi = mx::load8(kp, k64, mt / 2 * 1024 + mt % 2 * 8 + 256);
+                x.k[mt] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NH * KP; ++i) x.k[i] = mx::load16(kp, from, i * 1024);
         }
-        x.ks = *reinterpret_cast<const uint32_t *>(kp + mx::code_bytes(D, FMT) + (l16 + 16 * (lg * E / mx::GROUP)) * 4);
+        x.ks = mx::load4(kp, ko, CB);
+#pragma unroll
+        for (int i = 0; i < NH * KP; ++i) x.v[i] = mx::load16(vp, from, i * 1024);
 #pragma unroll
         for (int h = 0; h < NH; ++h)
 #pragma unroll
-            for (int i = 0; i < NG / 2; ++i)
-                x.vs[h][i] = *reinterpret_cast<const mx::u32x4 *>(vp + mx::code_bytes(D, FMT) +
-                                                                  (((h0 + h) * 4 + lg) * NG + 2 * i) * 8);
+            for (int i = 0; i < NL; ++i) x.vs[h][i] = mx::load8(vp, vo + h0 * (32 * NG), CB + (h * 4 * NG + i) * 8);
     };
-    int u = u0 + wave;
-    Unit xa, xb;
-    int64_t next = 0;   // the place of unit u + DW
-    if (u < u1) {
-        load(xa, u, place(u));
-        next = place(u + DW);
-    }
-
-    // the lane's elements E lg .. of the query, as of a key: those 8 ks .. + 7 in step ks
-    bf16x8 q[NKS][NQ];
-    {
-        float x[NKS][8];
+    // Wave 0 makes the query's operand for all (and takes the units' turns last).
+    constexpr int NE = FMT == 4 ? 32 : E;                 // a lane's elements of the query, from `first` on
+    constexpr int QR = FMT == 4 ? 6 * NM : 4 * NKS * NQ;  // registers of the operand
+    __shared__ uint32_t qlds[QR][64];
+    __shared__ int slds[2][64];
+    const int first = FMT == 4 ? 32 * kg : E * lg;
+    if (wave == 0) {
+        float qx[NE], qy[NE], cs[NE], sn[NE];
         const char *row = a.q + (int64_t)s * a.qst + head * a.qsh;
+        const int64_t pos = max((int64_t)0, min((int64_t)L - 1, a.n_tab - 1)) * D;
 #pragma unroll
-        for (int ks = 0; ks < NKS; ++ks) Op<DT>::unpack(Op<DT>::load(row + (E * lg + 8 * ks) * ESZ), x[ks]);
-        float scale = a.scales[s] * LOG2E;
-        if (a.gain) {
-            float ss = 0.0f;
+        for (int i = 0; i < NE / 8; ++i) {
+            float t[8];
+            Op<DT>::unpack(Op<DT>::load(row + (first + 8 * i) * ESZ), t);
 #pragma unroll
-            for (int ks = 0; ks < NKS; ++ks)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) ss = fmaf(x[ks][e], x[ks][e], ss);
-            ss += __shfl_xor(ss, 16, 64);
-            ss += __shfl_xor(ss, 32, 64);
-            scale *= a.gain[head] / sqrtf(fmaxf(ss / (float)D, a.eps));
+            for (int e = 0; e < 8; ++e) qx[8 * i + e] = t[e];
         }
-        const int64_t pos = max((int64_t)0, min((int64_t)L - 1, a.n_tab - 1)) * D + E * lg;
+        if (a.cos) {
 #pragma unroll
-        for (int ks = 0; ks < NKS; ++ks) {
+            for (int i = 0; i < NE / 8; ++i) {
+                float t[8];
+                Op<DT>::unpack(Op<DT>::load(row + ((first + D / 2) % D + 8 * i) * ESZ), t);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[ks][e] *= scale;
-            if (a.cos) {   // the rotation's partner is half a head away, in the other half of the wave
+                for (int e = 0; e < 8; ++e) qy[8 * i + e] = t[e];
+            }
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float y = rows::other_half(x[ks][e]), sn = a.sin[pos + 8 * ks + e];
-                    x[ks][e] = x[ks][e] * a.cos[pos + 8 * ks + e] + y * (lg < 2 ? -sn : sn);
+            for (int e = 0; e < NE; e += 4) {
+                *reinterpret_cast<f32x4 *>(cs + e) = *reinterpret_cast<const f32x4 *>(a.cos + pos + first + e);
+                *reinterpret_cast<f32x4 *>(sn + e) = *reinterpret_cast<const f32x4 *>(a.sin + pos + first + e);
+            }
+        }
+        finish_group<D, NE, FMT == 8 || D == 128>(qx, qy, first < D / 2, a.gain ? a.gain + head : nullptr, a.eps,
+                                                  a.cos != nullptr, cs, sn, a.scales[s] * LOG2E);
+        if constexpr (FMT == 4) {
+            const Query6<NQ> r = parts6<NQ>(qx);
+            int qs[2] = {0, 0};
+#pragma unroll
+            for (int n = 0; n < NM; ++n) {
+                mx::u32x6 w = r.q[n];
+                int b = r.scale[n];
+                if constexpr (D == 64) {   // elements 0 .. 63 and again, of the next part
+                    b = lg < 2 ? r.scale[2 * n] : r.scale[2 * n + 1];
+#pragma unroll
+                    for (int i = 0; i < 6; ++i) w[i] = lg < 2 ? r.q[2 * n][i] : r.q[2 * n + 1][i];
+                }
+#pragma unroll
+                for (int i = 0; i < 6; ++i) qlds[6 * n + i][lane] = w[i];
+                qs[n / 4] |= b << (8 * (n % 4));
+            }
+            slds[0][lane] = qs[0];
+            slds[1][lane] = qs[1];
+        } else {
+#pragma unroll
+            for (int ks = 0; ks < NKS; ++ks) {
+                float t[8];
+                bf16x8 p[NQ];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) t[e] = qx[8 * ks + e];
+                rows::parts<NQ>(t, p);
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) {
+                    const mx::u32x4 w = __builtin_bit_cast(mx::u32x4, p[n]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) qlds[4 * (ks * NQ + n) + i][lane] = w[i];
                 }
             }
-            rows::parts<NQ>(x[ks], q[ks]);
         }
+    }
+    // Three units: one is worked on while two are on their way.  Past the end the last one
+    // is loaded again (it is in the cache): a load that some passes of the loop leave out
+    // would make all of them wait for every load there is.
+    int u = u0 + (wave + DW - 1) % DW;
+    Unit xa, xb, xc;
+    int64_t next = 0;   // the place of the unit that is loaded next
+    if (u < u1) {
+        __builtin_amdgcn_sched_barrier(0);
+        load(xa, u, place(u));
+        __builtin_amdgcn_sched_barrier(0);
+        load(xb, min(u + DW, u1 - 1), place(u + DW));
+        __builtin_amdgcn_sched_barrier(0);
+        next = place(u + 2 * DW);
+    }
+    __syncthreads();
+    mx::i32x8 q6[FMT == 4 ? NM : 1];
+    int qs[2] = {0, 0};           // scales of the parts, a byte each
+    bf16x8 q16[NKS][FMT == 8 ? NQ : 1];
+    if constexpr (FMT == 4) {
+#pragma unroll
+        for (int n = 0; n < NM; ++n) {
+            q6[n] = mx::i32x8{0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < 6; ++i) q6[n][i] = (int)qlds[6 * n + i][lane];
+        }
+        qs[0] = slds[0][lane];
+        qs[1] = slds[1][lane];
+    } else {
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks)
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                mx::u32x4 w;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = qlds[4 * (ks * NQ + n) + i][lane];
+                q16[ks][n] = __builtin_bit_cast(bf16x8, w);
+            }
     }
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) O[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -237,35 +380,54 @@ __device__ __forceinline__ void decode_codes(const Args &a, int s, int g, int he
         const int h0 = UP == 1 ? 0 : at % UP, j0 = logical(at) * rows::PAGE + h0 * UK;
         f32x4 S[2 * NH];
 #pragma unroll
-        for (int mt = 0; mt < 2 * NH; ++mt) {
-            S[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
-            const float sc = __uint_as_float((x.ks >> (8 * (2 * h0 + mt)) & 255u) << 23);
+        for (int mt = 0; mt < 2 * NH; ++mt) S[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if constexpr (FMT == 4) {
+            // part by part over the tiles: a tile's sums wait for one another
+            const auto part = [&](auto N) {
+                constexpr int n = N.value;
+                if constexpr (n < NM) {
+                    S[0] = mx::product6<0, n % 4>(x.k[0], q6[n], S[0], x.ks, qs[n / 4]);
+                    S[1] = mx::product6<1, n % 4>(x.k[1], q6[n], S[1], x.ks, qs[n / 4]);
+                    S[2] = mx::product6<2, n % 4>(x.k[2], q6[n], S[2], x.ks, qs[n / 4]);
+                    S[3] = mx::product6<3, n % 4>(x.k[3], q6[n], S[3], x.ks, qs[n / 4]);
+                }
+            };
+            part(mx::number<0>());
+            part(mx::number<1>());
+            part(mx::number<2>());
+            part(mx::number<3>());
+            part(mx::number<4>());
+            part(mx::number<5>());
+        } else {
 #pragma unroll
-            for (int ks = 0; ks < NKS; ++ks) {
-                constexpr int W = FMT / 4;              // words of 8 codes
-                const int w = (mt * NKS + ks) * W;      // the first of these
-                uint32_t c[2] = {x.k[w / 4][w % 4], W == 2 ? x.k[w / 4][w % 4 + W - 1] : 0u};
-                const bf16x8 kf = mx::eight<FMT>(c, sc);
+            for (int ks = 0; ks < NKS; ++ks)
 #pragma unroll
-                for (int n = 0; n < NQ; ++n) S[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[ks][n], S[mt], 0, 0, 0);
-            }
+                for (int mt = 0; mt < 2 * NH; ++mt) {
+                    const float sc = __uint_as_float((x.ks >> (8 * (2 * h0 + mt)) & 255u) << 23);
+                    const int w = 2 * (mt * NKS + ks);   // the first of the two words of 8 codes
+                    const uint32_t c[2] = {x.k[w / 4][w % 4], x.k[w / 4][w % 4 + 1]};
+                    const bf16x8 kf = mx::eight<8>(c, sc);
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n)
+                        S[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q16[ks][n], S[mt], 0, 0, 0);
+                }
         }
         // S[mt][e]: key j0 + 32 (mt / 2) + 8 lg + 4 (mt % 2) + e
         const bool whole = j0 + UK <= L && (j0 >= pg.lo || j0 + UK <= a.S);
         if (!whole) {
 #pragma unroll
             for (int h = 0; h < NH; ++h) {
-                uint32_t see[2] = {0, 0};   // bytes of the tokens that are seen
+                const uint32_t bits = (uint32_t)(rows::seen_bits(pg.lo, L, a.S, j0 + 32 * h) >> (8 * lg));
+                // four bits as four bytes
+                const uint32_t see[2] = {((bits & 15u) * 0x00204081u & 0x01010101u) * 255u,
+                                         ((bits >> 4 & 15u) * 0x00204081u & 0x01010101u) * 255u};
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int j = j0 + 32 * h + 8 * lg + e;
-                    if (j < L && (j >= pg.lo || j < a.S)) see[e >> 2] |= 255u << (8 * (e & 3));
-                    else S[2 * h + (e >> 2)][e & 3] = -INFINITY;
-                }
+                for (int e = 0; e < 8; ++e)
+                    S[2 * h + (e >> 2)][e & 3] = rows::keep(S[2 * h + (e >> 2)][e & 3], bits, e, -INFINITY);
 #pragma unroll
-                for (int i = 0; i < NG / 2; ++i)
+                for (int i = 0; i < NL; ++i)
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) x.vs[h][i][w] &= see[w & 1];
+                    for (int w = 0; w < 2; ++w) x.vs[h][i][w] &= see[w];
                 if constexpr (FMT == 8) {   // a code may be a NaN
 #pragma unroll
                     for (int i = 0; i < KP; ++i)
@@ -279,8 +441,8 @@ __device__ __forceinline__ void decode_codes(const Args &a, int s, int g, int he
         for (int mt = 0; mt < 2 * NH; ++mt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) top = fmaxf(top, S[mt][e]);
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        top = fmaxf(top, rows::other_row(top));
+        top = fmaxf(top, rows::other_half(top));
         if (__ballot(top > m)) {
             const float mn = fmaxf(m, top), al = m == -INFINITY ? 0.0f : ex2(m - mn);
             l *= al;
@@ -298,17 +460,18 @@ __device__ __forceinline__ void decode_codes(const Args &a, int s, int g, int he
                 l += p[e];
             }
 #pragma unroll
-            for (int vg = 0; vg < NG; ++vg) {
+            for (int i = 0; i < NL; ++i) {   // the lane's i-th group
                 float y[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = p[e] * mx::power(x.vs[h][vg / 2][vg % 2 * 2 + (e >> 2)], e & 3);
+                for (int e = 0; e < 8; ++e) y[e] = p[e] * mx::power(x.vs[h][i][e >> 2], e & 3);
                 bf16x8 pf[NP];   // bf16 output: a relative 2^-8 each at most; l has them as they are
                 rows::parts<NP>(y, pf);
 #pragma unroll
-                for (int dt = 2 * vg; dt < 2 * vg + 2; ++dt) {
+                for (int k = 0; k < 2 * NS; ++k) {   // the columns of that group in each set
+                    const int dt = 2 * (k / 2 * NL + i) + k % 2;
                     constexpr int W = FMT / 4;
                     const int w = dt * W;
-                    uint32_t c[2] = {x.v[h * KP + w / 4][w % 4], W == 2 ? x.v[h * KP + w / 4][w % 4 + W - 1] : 0u};
+                    const uint32_t c[2] = {x.v[h * KP + w / 4][w % 4], W == 2 ? x.v[h * KP + w / 4][w % 4 + W - 1] : 0u};
                     const bf16x8 vf = mx::eight<FMT>(c, 1.0f);
 #pragma unroll
                     for (int n = 0; n < NP; ++n) O[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[n], O[dt], 0, 0, 0);
@@ -316,21 +479,20 @@ __device__ __forceinline__ void decode_codes(const Args &a, int s, int g, int he
             }
         }
     };
+    const auto step = [&](Unit &now, Unit &free) {
+        load(free, min(u + 2 * DW, u1 - 1), next);
+        next = place(u + 3 * DW);
+        __builtin_amdgcn_sched_barrier(0);
+        use(now, u);
+        __builtin_amdgcn_sched_barrier(0);
+        u += DW;
+        return u < u1;
+    };
+    if (u >= u1) return;
 #pragma unroll 1
-    for (; u < u1; u += 2 * DW) {
-        if (u + DW < u1) {
-            load(xb, u + DW, next);
-            next = place(u + 2 * DW);
-        }
-        use(xa, u);
-        if (u + DW >= u1) break;
-        if (u + 2 * DW < u1) {
-            load(xa, u + 2 * DW, next);
-            next = place(u + 3 * DW);
-        }
-        use(xb, u + DW);
-    }
+    while (step(xa, xc) && step(xb, xa) && step(xc, xb)) {}
 }
+
 // gi: 16 heads of a KV head of sequence s; pages p0 .. p1 - 1 of its list.  Head i of
 // the 16 writes part at + i step, or its row of the output (at < 0).
 // Units of UK keys: a page, or half of one where a page's operands would fill the
@@ -339,9 +501,9 @@ template <int DT, int D> constexpr int UNIT = DT == 1 && D == 64 ? 64 : 32;
 template <int D> struct DecodeLds {
     float o[4][16][D + 4], m[4][16], l[4][16];
 };
-template <int DT, int D, int DW, int FMT>
+template <int DT, int D, int DW, int FMT, int NS>
 __device__ __forceinline__ void decode_part(const Args &a, DecodeLds<D> &lds, int s, int gi, int p0, int p1,
-                                            int64_t at, int step) {
+                                            int64_t at, int step, int known = -1) {   // known: the length, if it is
     typedef typename Op<DT>::F F;
     constexpr int ESZ = DT == 1 ? 2 : 4, UK = UNIT<DT, D>;
     constexpr int NKS = D / 32, NDT = D / 16, NH = UK / 32, UP = rows::PAGE / UK;
@@ -350,12 +512,13 @@ __device__ __forceinline__ void decode_part(const Args &a, DecodeLds<D> &lds, in
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ct = (a.G + 15) / 16;
     const int g = gi / ct, c0 = gi % ct * 16;
-    const int L = length(a, s);
-    const int hl = c0 + l16, head = g * a.G + min(hl, a.G - 1);
+    const int L = FMT != 0 && known >= 0 ? known : length(a, s);
+    const int hr = NS == 2 ? l16 & 7 : l16;   // the lane's head of the 16 (or 8, twice)
+    const int hl = c0 + hr, head = g * a.G + min(hl, a.G - 1);
     f32x4 O[NDT];
     float m, l;
     if constexpr (FMT != 0) {
-        decode_codes<DT, D, DW, FMT>(a, s, g, head, L, p0, p1, O, m, l);
+        decode_codes<DT, D, DW, FMT, NS>(a, s, g, head, L, p0, p1, O, m, l);
     } else {
         const Pages pg = page_list(a, L);
         const int u0 = p0 * UP, u1 = min(pg.n, p1) * UP;
@@ -502,22 +665,25 @@ __device__ __forceinline__ void decode_part(const Args &a, DecodeLds<D> &lds, in
     // the waves' sums meet in LDS: those of waves 4 and up fold into the first four's
     const auto put = [&](int w) {
         if (lg == 0) {
-            lds.m[w][l16] = m;
-            lds.l[w][l16] = l;
+            lds.m[w][hr] = m;
+            lds.l[w][hr] = l;
         }
 #pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) *reinterpret_cast<f32x4 *>(&lds.o[w][l16][16 * dt + 4 * lg]) = O[dt];
+        for (int dt = 0; dt < NDT; ++dt) {
+            if (NS == 2 && l16 >> 3 != dt / (NDT / 2)) continue;   // the other set has these columns
+            *reinterpret_cast<f32x4 *>(&lds.o[w][hr][16 * dt + 4 * lg]) = O[dt];
+        }
     };
     if constexpr (DW > 4) {
         if (wave >= 4) put(wave - 4);
         __syncthreads();
         if (wave < 4) {
-            const float om = lds.m[wave][l16], ol = lds.l[wave][l16], mn = fmaxf(m, om);
+            const float om = lds.m[wave][hr], ol = lds.l[wave][hr], mn = fmaxf(m, om);
             const float fa = m == -INFINITY ? 0.0f : ex2(m - mn), fb = om == -INFINITY ? 0.0f : ex2(om - mn);
             l = fmaf(ol, fb, l * fa);
 #pragma unroll
             for (int dt = 0; dt < NDT; ++dt)
-                O[dt] = O[dt] * fa + *reinterpret_cast<const f32x4 *>(&lds.o[wave][l16][16 * dt + 4 * lg]) * fb;
+                O[dt] = O[dt] * fa + *reinterpret_cast<const f32x4 *>(&lds.o[wave][hr][16 * dt + 4 * lg]) * fb;
             m = mn;
         }
     }
@@ -564,16 +730,16 @@ constexpr int DW = 8;   // waves of a decode workgroup
 // 64 sequences' windows of 1024 keys, 14 / 2 heads, d = 64: 11 us, 7 at a copy's rate.
 // Eight waves, so that a window of 17 or 18 pages takes a wave two pages, or three:
 // chains of round trips bound it.
-template <int DT, int D, int DW, int FMT>
+template <int DT, int D, int DW, int FMT, int NS>
 __device__ __forceinline__ void decode_run(const Args &a, DecodeLds<D> &lds, int group, int part) {
     const int ct = (a.G + 15) / 16, ng = a.Hkv * ct, s = group / ng, gi = group % ng;
     const int64_t row = (int64_t)s * a.Hq + gi / ct * a.G + gi % ct * 16;
-    decode_part<DT, D, DW, FMT>(a, lds, s, gi, part * a.part, (part + 1) * a.part,
+    decode_part<DT, D, DW, FMT, NS>(a, lds, s, gi, part * a.part, (part + 1) * a.part,
                            a.slots == 1 ? -1 : row * a.slots + a.slot0 + part, a.slots);
 }
-template <int DT, int D, int FMT> __global__ __launch_bounds__(64 * DW) void decode_kernel(const Args a) {
+template <int DT, int D, int FMT, int NS> __global__ __launch_bounds__(64 * DW) void decode_kernel(const Args a) {
     __shared__ DecodeLds<D> lds;
-    decode_run<DT, D, DW, FMT>(a, lds, blockIdx.x, blockIdx.y);
+    decode_run<DT, D, DW, FMT, NS>(a, lds, blockIdx.x, blockIdx.y);
 }
 
 // Even shares.  All pages of all groups (a group: 16 heads of a sequence) make one
@@ -592,7 +758,69 @@ template <int NT> __device__ __forceinline__ Shares shares(const Args &a) {
     x.per = max(a.part, (x.units + a.slots - 1) / a.slots);
     return x;
 }
-template <int DT, int D, int FMT> __global__ __launch_bounds__(64 * DW) void even_kernel(const Args a) {
+// The same for codes (at most MOST sequences), where a share's own work is short: the pages
+// before each sequence are found once, in LDS, and for the join a group's first share
+// writes down which parts are its own (records: [groups][2], the first one and how
+// many, 0 if the group is done).
+constexpr int MOST = 1024;
+template <int DT, int D, int FMT, int NS> __global__ __launch_bounds__(64 * DW) void even_codes_kernel(const Args a) {
+    constexpr int NT = 64 * DW;
+    __shared__ DecodeLds<D> lds;
+    __shared__ int before[MOST + 1], len[MOST], wsum[DW], found;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int sum = 0;
+    for (int base = 0; base < a.Bd; base += NT) {
+        const int i = base + tid, L = i < a.Bd ? length(a, i) : 0, n = i < a.Bd ? max(1, page_list(a, L).n) : 0;
+        int upto = n;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int x = __shfl_up(upto, o, 64);
+            if (lane >= o) upto += x;
+        }
+        if (lane == 63) wsum[wave] = upto;
+        __syncthreads();
+        int all = 0;
+#pragma unroll
+        for (int w = 0; w < DW; ++w) {
+            if (w < wave) upto += wsum[w];
+            all += wsum[w];
+        }
+        if (i < a.Bd) {
+            before[i] = sum + upto - n;
+            len[i] = L;
+        }
+        sum += all;
+        __syncthreads();
+    }
+    const int ng = groups_of(a), w = blockIdx.x, units = sum * ng, per = max(a.part, (units + a.slots - 1) / a.slots);
+    const int64_t u0 = (int64_t)w * per;
+    if (tid == 0) before[a.Bd] = sum;
+    __syncthreads();
+    if (u0 >= units) return;
+    for (int i = tid; i < a.Bd; i += NT)
+        if (u0 >= (int64_t)before[i] * ng && u0 < (int64_t)before[i + 1] * ng) found = i;
+    __syncthreads();
+    int s = __builtin_amdgcn_readfirstlane(found);
+    int left = (int)min((int64_t)per, units - u0), at = (int)u0 - before[s] * ng;
+    for (int part = 2 * w; left > 0 && s < a.Bd; part = 2 * w + 1) {
+        const int n = __builtin_amdgcn_readfirstlane(before[s + 1] - before[s]), L = __builtin_amdgcn_readfirstlane(len[s]);
+        const int gi = at / n, p0 = at % n, p1 = min(n, p0 + left);
+        if (p0 == 0 && tid == 0) {
+            const int last = (int)((u0 + (int)min((int64_t)per, units - u0) - left + n - 1) / per);
+            a.records[2 * (s * ng + gi)] = part;
+            a.records[2 * (s * ng + gi) + 1] = p1 == n ? 0 : last - w + 1;
+        }
+        decode_part<DT, D, DW, FMT, NS>(a, lds, s, gi, p0, p1, p1 - p0 == n ? -1 : (int64_t)part * 16, 1, L);
+        __syncthreads();   // lds is free again
+        left -= p1 - p0;
+        at += p1 - p0;
+        if (at == n * ng) {
+            at = 0;
+            ++s;
+        }
+    }
+}
+template <int DT, int D> __global__ __launch_bounds__(64 * DW) void even_kernel(const Args a) {
     __shared__ DecodeLds<D> lds;
     const Shares sh = shares<64 * DW>(a);
     const int ng = groups_of(a), w = blockIdx.x;
@@ -602,7 +830,7 @@ template <int DT, int D, int FMT> __global__ __launch_bounds__(64 * DW) void eve
     int s = ragged::find<64 * DW>((int)u0, a.Bd, [&](int i) { return list_pages(a, i) * ng; }, at);
     for (int part = 2 * w; left > 0 && s < a.Bd; part = 2 * w + 1) {
         const int n = list_pages(a, s), p0 = at % n, p1 = min(n, p0 + left);
-        decode_part<DT, D, DW, FMT>(a, lds, s, at / n, p0, p1, p1 - p0 == n ? -1 : (int64_t)part * 16, 1);
+        decode_part<DT, D, DW, 0, 1>(a, lds, s, at / n, p0, p1, p1 - p0 == n ? -1 : (int64_t)part * 16, 1);
         __syncthreads();   // lds is free again
         left -= p1 - p0;
         at += p1 - p0;
@@ -774,7 +1002,7 @@ __global__ __launch_bounds__(64 * rows::NW, (DT == 1 && D == 64 ? 3 : rows::WAVE
 // The shared pages for all rows (the first nshared workgroups, which take longest)
 // and every sequence's own pages for its newest token: 64 sequences, 8192 shared
 // keys, d = 64: 14.5 us, and 5 of the join.
-template <int DT, int D, int FMT>
+template <int DT, int D, int FMT, int NS>
 __global__ __launch_bounds__(64 * rows::NW, (rows::WAVES<DT, D>)) void shared_kernel(
     const Args a, const Args own, int ptiles, int nshared, int groups) {
     extern __shared__ __align__(16) char smem[];
@@ -782,15 +1010,15 @@ __global__ __launch_bounds__(64 * rows::NW, (rows::WAVES<DT, D>)) void shared_ke
     if (i < nshared)
         rows_part<DT, D, FMT, true>(a, smem, i % ptiles, i / ptiles % a.Hkv, i / (ptiles * a.Hkv));
     else
-        decode_run<DT, D, rows::NW, FMT>(own, *reinterpret_cast<DecodeLds<D> *>(smem), (i - nshared) % groups,
+        decode_run<DT, D, rows::NW, FMT, NS>(own, *reinterpret_cast<DecodeLds<D> *>(smem), (i - nshared) % groups,
                                     (i - nshared) / groups);
 }
 
 // out = sum of the parts' O 2^(m - max) over sum of their l 2^(m - max); a row
 // without keys 0.  D / 4 threads a part, SG parts of a row at a time (all of a
 // workgroup where a row has many parts, one where rows are many), each with sums
-// of its own that LDS joins.  EVEN: the parts are those of even shares.
-template <int DT, int D, int SG, bool EVEN>
+// of its own that LDS joins.  EVEN: the parts are those of even shares (2: written down).
+template <int DT, int D, int SG, int EVEN>
 __global__ __launch_bounds__(256) void join_kernel(const Args a, int64_t nrows) {
     constexpr int TP = D / 4, RB = 256 / (TP * SG);   // threads of a part, rows of a workgroup
     __shared__ float so[SG > 1 ? SG : 1][SG > 1 ? D : 1];
@@ -800,7 +1028,15 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a, int64_t nrows) 
     if (row >= nrows) return;                         // SG > 1: the workgroup's one row
     int slots = a.slots, step = 1;                    // part p at first + p step, the row's first part at part0
     int64_t first_part = row * a.slots, part0 = first_part;
-    if constexpr (EVEN) {
+    if constexpr (EVEN == 2) {
+        const int s = (int)(row / a.Hq), h = (int)(row % a.Hq), ct = (a.G + 15) / 16, hc = h % a.G;
+        const int *r = a.records + 2 * ((s * a.Hkv + h / a.G) * ct + hc / 16);
+        slots = r[1];
+        if (slots == 0) return;                       // written already
+        step = 32;
+        first_part = (int64_t)(r[0] / 2) * 32 + hc % 16;
+        part0 = (int64_t)r[0] * 16 + hc % 16;
+    } else if constexpr (EVEN) {
         static_assert(RB == 1, "the scans are a workgroup's");
         const Shares sh = shares<256>(a);
         const int s = (int)(row / a.Hq), h = (int)(row % a.Hq), ct = (a.G + 15) / 16, n = list_pages(a, s);
@@ -865,7 +1101,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a, int64_t nrows) 
     const int t = (int)(row / a.Hq), s = a.cu ? ragged::sequence(a.cu, a.Bd, t) : t;
     int first = t, cnt = 1;
     if (a.cu) cnt = ragged::tokens(a.cu, s, a.T, first);
-    const bool sees = t >= first && t - first < cnt && length(a, s) - cnt + t - first >= 0;
+    const bool sees = EVEN == 2 || (t >= first && t - first < cnt && length(a, s) - cnt + t - first >= 0);
     const f32x4 r = sees ? o / l : f32x4{0.f, 0.f, 0.f, 0.f};
     char *to = a.out + (row * D + x) * (DT == 1 ? 2 : 4);
     if constexpr (DT == 1)
@@ -896,7 +1132,7 @@ static int parts_of(int64_t pages, int64_t base, int64_t most, int64_t least, in
     return (int)((pages + per - 1) / per);
 }
 static Plan plan(int64_t T, int64_t Bd, int64_t Hq, int64_t Hkv, int64_t W, int64_t S, int64_t shared, bool one,
-                 int64_t max_len) {
+                 int64_t max_len, bool codes) {
     Plan p = {};
     const int64_t G = Hq / Hkv, KT = rows::PAGE;
     int64_t keys = max_len - shared * KT;
@@ -904,6 +1140,7 @@ static Plan plan(int64_t T, int64_t Bd, int64_t Hq, int64_t Hkv, int64_t W, int6
     // A part of a prompt may span any number of windows.  (The parts cut the list of one
     // 128-row tile, which has W + 128 / G tokens and the sinks, so of a window's parts most are empty.)
     if (W > 0 && !one) keys = max_len;
+    if (codes && W > 0 && !one && W + rows::RT / G + 1 < max_len) keys = W + rows::RT / G + 1;   // that list
     if (keys < 1) keys = 1;
     int64_t pages = (keys + KT - 1) / KT + 1 + (W > 0 ? (S + KT - 1) / KT : 0);
     const int64_t all = (max_len + KT - 1) / KT;
@@ -935,12 +1172,17 @@ static Plan plan(int64_t T, int64_t Bd, int64_t Hq, int64_t Hkv, int64_t W, int6
     if (shared) p.prefix = parts_of(shared, p.ptiles * Hkv, CUS, 1, p.prefix_pages);
     return p;
 }
-static size_t workspace(const Plan &p, int64_t T, int64_t Hq, int64_t d) {
+static size_t parts_bytes(const Plan &p, int64_t T, int64_t Hq, int64_t d) {
     const int64_t parts = p.shares ? (int64_t)p.shares * 32 : p.slots() > 1 ? T * Hq * p.slots() : 0;
     return (size_t)parts * (d + 2) * 4;
 }
+static size_t workspace(const Plan &p, int64_t T, int64_t Bd, int64_t Hq, int64_t Hkv, int64_t d, bool codes) {
+    const size_t records = codes && p.shares ? (size_t)(Bd * Hkv * ((Hq / Hkv + 15) / 16) * 8) : 0;
+    return parts_bytes(p, T, Hq, d) + records;
+}
 
-template <int DT, int D, int FMT> static int launch(Args a, const Plan &p, hipStream_t s) {
+// NS: sets of columns, 2 where a KV head of a cache in 4 or 8 bits has 8 query heads at most
+template <int DT, int D, int FMT, int NS> static int launch(Args a, const Plan &p, hipStream_t s) {
     constexpr size_t lds = 2 * RowSource<DT, D, FMT>::T::BYTES;
     static_assert(sizeof(DecodeLds<D>) <= 65536 && lds <= 65536, "LDS without an attribute");
     const int64_t groups = (int64_t)a.Bd * a.Hkv * ((a.G + 15) / 16);
@@ -950,9 +1192,13 @@ template <int DT, int D, int FMT> static int launch(Args a, const Plan &p, hipSt
         a.part = p.own_pages;
         const int64_t nrows = (int64_t)a.T * a.Hq;
         if (!abi::launchable(nrows, 256)) return HBA_ERR_UNSUPPORTED;
-        hipLaunchKernelGGL((even_kernel<DT, D, FMT>), dim3((unsigned)p.shares), dim3(64 * DW), 0, s, a);
+        if constexpr (FMT == 0)
+            hipLaunchKernelGGL((even_kernel<DT, D>), dim3((unsigned)p.shares), dim3(64 * DW), 0, s, a);
+        else
+            hipLaunchKernelGGL((even_codes_kernel<DT, D, FMT, NS>), dim3((unsigned)p.shares), dim3(64 * DW), 0, s, a);
         HBA_LAUNCH_CHECK();
-        hipLaunchKernelGGL((join_kernel<DT, D, 1024 / D, true>), dim3((unsigned)nrows), dim3(256), 0, s, a, nrows);
+        hipLaunchKernelGGL((join_kernel<DT, D, 1024 / D, FMT == 0 ? 1 : 2>), dim3((unsigned)nrows), dim3(256), 0, s, a,
+                           nrows);
         HBA_LAUNCH_CHECK();
         return HBA_OK;
     }
@@ -971,7 +1217,7 @@ template <int DT, int D, int FMT> static int launch(Args a, const Plan &p, hipSt
     if (p.prefix && !a.cu) {
         const int64_t grid = nshared + groups * p.own;
         constexpr size_t both = lds > sizeof(DecodeLds<D>) ? lds : sizeof(DecodeLds<D>);
-        hipLaunchKernelGGL((shared_kernel<DT, D, FMT>), dim3((unsigned)grid), dim3(64 * rows::NW), both, s, a, own,
+        hipLaunchKernelGGL((shared_kernel<DT, D, FMT, NS>), dim3((unsigned)grid), dim3(64 * rows::NW), both, s, a, own,
                            (int)p.ptiles, (int)nshared, (int)groups);
     } else {
         if (p.prefix)
@@ -983,15 +1229,15 @@ template <int DT, int D, int FMT> static int launch(Args a, const Plan &p, hipSt
             hipLaunchKernelGGL((rows_kernel<DT, D, FMT, false>), dim3((unsigned)p.tiles, (unsigned)a.Hkv, (unsigned)p.own),
                                dim3(64 * rows::NW), lds, s, own);
         else
-            hipLaunchKernelGGL((decode_kernel<DT, D, FMT>), dim3((unsigned)groups, (unsigned)p.own), dim3(64 * DW), 0, s,
+            hipLaunchKernelGGL((decode_kernel<DT, D, FMT, NS>), dim3((unsigned)groups, (unsigned)p.own), dim3(64 * DW), 0, s,
                                own);
     }
     HBA_LAUNCH_CHECK();
     if (a.slots > 1) {
         if (a.slots > 8)
-            hipLaunchKernelGGL((join_kernel<DT, D, SG, false>), dim3((unsigned)joins), dim3(256), 0, s, a, nrows);
+            hipLaunchKernelGGL((join_kernel<DT, D, SG, 0>), dim3((unsigned)joins), dim3(256), 0, s, a, nrows);
         else
-            hipLaunchKernelGGL((join_kernel<DT, D, 1, false>), dim3((unsigned)joins), dim3(256), 0, s, a, nrows);
+            hipLaunchKernelGGL((join_kernel<DT, D, 1, 0>), dim3((unsigned)joins), dim3(256), 0, s, a, nrows);
         HBA_LAUNCH_CHECK();
     }
     return HBA_OK;
@@ -1017,7 +1263,7 @@ static int setup(Args &a, Plan &p, int dtype, const void *q, const int64_t q_str
                  int64_t num_pages, const int32_t *page_table, int64_t max_pages, const int32_t *seq_lens,
                  const float *scales, const int32_t *cu, int64_t T, int64_t Bd, int64_t Hq, int64_t Hkv, int64_t d,
                  int64_t Bk, int64_t W, int64_t S, int64_t shared_pages, int64_t max_len, void *workspace,
-                 size_t ws_bytes, void *out) {
+                 size_t ws_bytes, void *out, bool codes) {
     if (int st = abi::check_dtype_dim(dtype, d)) return st;
     if (Bk != rows::PAGE) return HBA_ERR_UNSUPPORTED;
     if (int st = check(T, Bd, Hq, Hkv, d, W, S, shared_pages, cu == nullptr, max_len, max_pages)) return st;
@@ -1028,8 +1274,8 @@ static int setup(Args &a, Plan &p, int dtype, const void *q, const int64_t q_str
     if (!abi::aligned16(q) || q_strides[0] % al || q_strides[1] % al || !abi::aligned16(kr_pages) ||
         !abi::aligned16(v_pages) || !abi::aligned16(out))
         return HBA_ERR_UNSUPPORTED;
-    p = plan(T, Bd, Hq, Hkv, W, S, shared_pages, cu == nullptr, max_len);
-    const size_t need = paged::workspace(p, T, Hq, d);
+    p = plan(T, Bd, Hq, Hkv, W, S, shared_pages, cu == nullptr, max_len, codes);
+    const size_t need = paged::workspace(p, T, Bd, Hq, Hkv, d, codes), parts = parts_bytes(p, T, Hq, d);
     if (need && (!workspace || ws_bytes < need)) return HBA_ERR_INVALID_ARG;
     if (need && !abi::aligned16(workspace)) return HBA_ERR_UNSUPPORTED;
     a = {};
@@ -1060,7 +1306,8 @@ static int setup(Args &a, Plan &p, int dtype, const void *q, const int64_t q_str
     a.shared = (int)shared_pages;
     a.out = (char *)out;
     a.po = (float *)workspace;
-    a.pml = need ? (float *)workspace + need / 4 / (d + 2) * d : nullptr;
+    a.pml = need ? (float *)workspace + parts / 4 / (d + 2) * d : nullptr;
+    a.records = need ? (int *)((char *)workspace + parts) : nullptr;
     return HBA_OK;
 }
 

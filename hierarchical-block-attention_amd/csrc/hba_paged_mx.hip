@@ -3,6 +3,16 @@
 
 using namespace hba;
 
+extern "C" int hba_paged_attn_mx_workspace_bytes(int64_t T, int64_t Bd, int64_t Hq, int64_t Hkv, int64_t d, int64_t W,
+                                                 int64_t S, int64_t shared_pages, int one_each, int64_t max_len,
+                                                 size_t *bytes) {
+    if (!bytes) return HBA_ERR_INVALID_ARG;
+    if (int st = paged::check(T, Bd, Hq, Hkv, d, W, S, shared_pages, one_each, max_len, 1 << 24)) return st;
+    const paged::Plan p = paged::plan(T, Bd, Hq, Hkv, W, S, shared_pages, one_each != 0, max_len, true);
+    *bytes = paged::workspace(p, T, Bd, Hq, Hkv, d, true);
+    return HBA_OK;
+}
+
 extern "C" int hba_paged_attn_mx(int dtype, const void *q, const int64_t q_strides[2], const float *q_gain, float eps,
                                  const float *cos_tab, const float *sin_tab, int64_t n_tab, int64_t bits,
                                  const void *k_pages, const void *v_pages, int64_t num_pages, const int32_t *page_table,
@@ -15,12 +25,16 @@ extern "C" int hba_paged_attn_mx(int dtype, const void *q, const int64_t q_strid
     paged::Plan p;
     if (int st = paged::setup(a, p, dtype, q, q_strides, q_gain, eps, cos_tab, sin_tab, n_tab, k_pages, v_pages, num_pages,
                               page_table, max_pages, seq_lens, scales, cu, T, Bd, Hq, Hkv, d, Bk, W, S, shared_pages,
-                              max_len, workspace, ws_bytes, out))
+                              max_len, workspace, ws_bytes, out, true))
         return st;
     int st = HBA_OK;
 #define HBA_PAGED_MX(DT, D)                                                             \
-    st = bits == 4 ? paged::launch<DT, D, 4>(a, p, (hipStream_t)stream)                 \
-                   : paged::launch<DT, D, 8>(a, p, (hipStream_t)stream)
+    if (bits == 4)                                                                      \
+        st = a.G <= 8 ? paged::launch<DT, D, 4, 2>(a, p, (hipStream_t)stream)           \
+                      : paged::launch<DT, D, 4, 1>(a, p, (hipStream_t)stream);          \
+    else                                                                                \
+        st = a.G <= 8 ? paged::launch<DT, D, 8, 2>(a, p, (hipStream_t)stream)           \
+                      : paged::launch<DT, D, 8, 1>(a, p, (hipStream_t)stream)
     HBA_DISPATCH_DT_D(dtype, d, HBA_PAGED_MX);
 #undef HBA_PAGED_MX
     return st;

@@ -60,6 +60,13 @@ __device__ __forceinline__ float other_half(float v) {
     return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
 }
 
+// The value of lane l ^ 16.
+__device__ __forceinline__ float other_row(float v) {
+    const uint32_t x = __float_as_uint(v);
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return __uint_as_float((threadIdx.x & 16) ? r[0] : r[1]);
+}
+
 // Operand fragments of a 16-deep step: 8 elements of one row or column, lane l
 // those of its half, elements 8 (l / 32) .. + 7.  mma adds a 32x32 product.
 // Lane l of the result: column l % 32, rows 8 (r / 4) + 4 (l / 32) + r % 4.

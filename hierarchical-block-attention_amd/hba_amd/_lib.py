@@ -75,6 +75,8 @@ SIGNATURES = {
     "hba_kv_append_mx": [_i, _vp, _c_i64p, _vp, _c_i64p, _vp, _i64, _vp, _f, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i64,
                          _i64, _i64, _i64, _i64, _vp, _vp, _vp],
     "hba_kv_read_mx": [_i, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp],
+    "hba_paged_attn_mx_workspace_bytes": [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i, _i64,
+                                          ctypes.POINTER(ctypes.c_size_t)],
     "hba_paged_attn_mx": [_i, _vp, _c_i64p, _vp, _f, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64,
                           _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, ctypes.c_size_t, _vp, _vp],
     "hba_swa_fwd": [_i, _vp, _c_i64p, _vp, _c_i64p, _vp, _c_i64p, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f,

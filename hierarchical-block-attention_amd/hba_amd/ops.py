@@ -33,13 +33,14 @@ The last seven run past the dispatcher where nothing but the call itself happens
 wherever something records or transforms operators.
 """
 import ctypes
+import functools
 from typing import Optional, Tuple
 
 import torch
 from torch import Tensor
 from torch.autograd import forward_ad
 
-from ._lib import BF16, F32, check, lib, strides3, used_strides2, used_strides3
+from ._lib import _I64X2, BF16, F32, check, lib, strides3, used_strides2, used_strides3
 
 BLOCK = 64
 _DT = {torch.float32: F32, torch.bfloat16: BF16}
@@ -124,7 +125,7 @@ def _f32c(t, dev, n=None, what="tensor"):
     """fp32 contiguous copy/view on `dev` (gains, probes, proj, tables)."""
     if t is None:
         return None
-    if t.dtype != torch.float32 or t.device != dev or not t.is_contiguous():
+    if t.dtype is not torch.float32 or t.get_device() != dev.index or not t.is_contiguous():
         t = t.detach().to(device=dev, dtype=torch.float32).contiguous()
     if n is not None and t.numel() != n:
         raise ValueError(f"{what}: expected {n} elements, got {t.numel()}")
@@ -144,8 +145,9 @@ def _rows(t, what):
 
 
 def _tables(cos, sin, n, d, dev):
-    if cos.shape[-1] != d or cos.shape[0] < n or sin.shape != cos.shape:
-        raise ValueError(f"cos/sin: expected [>= {n}, {d}] tables, got {tuple(cos.shape)}")
+    shape = cos.shape
+    if shape[-1] != d or shape[0] < n or sin.shape != shape:
+        raise ValueError(f"cos/sin: expected [>= {n}, {d}] tables, got {tuple(shape)}")
     return _f32c(cos, dev), _f32c(sin, dev)
 
 
@@ -951,7 +953,7 @@ def _(q, q_gain, eps, kc_pages, kr_pages, v_pages, summ_pages, page_table, seq_l
 
 # ------------------------------------------------- ragged append, paged attention ----
 def _i32(t, shape, dev, what):
-    if t.dtype != torch.int32 or t.device != dev or not t.is_contiguous() or tuple(t.shape) != shape:
+    if t.dtype is not torch.int32 or t.shape != shape or t.get_device() != dev.index or not t.is_contiguous():
         raise ValueError(f"{what}: expected a contiguous int32 tensor {list(shape)} on {dev}")
 
 
@@ -1041,6 +1043,26 @@ def _paged_attn(q, q_gain, eps, kr_pages, v_pages, page_table, seq_lens, cos, si
                          sinks, cu, shared)
 
 
+@functools.lru_cache(maxsize=1024)
+def _paged_workspace(mx, T, Bd, Hq, Hkv, d, window, sinks, pages, one_each, max_len):
+    """Workspace bytes of these sizes (a query of the library costs 1.5 us)."""
+    n = ctypes.c_size_t(0)
+    L = lib()
+    f = L.hba_paged_attn_mx_workspace_bytes if mx else L.hba_paged_attn_workspace_bytes
+    check(f(T, Bd, Hq, Hkv, d, window, sinks, pages, one_each, max_len, ctypes.byref(n)), "hba_paged_attn_workspace_bytes")
+    return n.value
+
+
+def _rows_of_tokens(t):
+    """_rows16 of a [T, H, d] tensor, and its used_strides2."""
+    (a, b, c), (n, h, _), e = t.stride(), t.shape, t.element_size()
+    a, b, q = a if n > 1 else 0, b if h > 1 else 0, 16 // e
+    if c != 1 or t.data_ptr() % 16 or a % q or b % q or a * e >= 1 << 24:
+        t = t.clone(memory_format=torch.contiguous_format)
+        return t, used_strides2(t)
+    return t, _I64X2(a, b)
+
+
 def _attend_pages(mx, q, q_gain, eps, kr_pages, v_pages, page_table, seq_lens, cos, sin, scales, max_len, window, sinks,
                   cu, shared):
     """paged_attn, and with mx paged_attn_mx."""
@@ -1083,23 +1105,22 @@ def _attend_pages(mx, q, q_gain, eps, kr_pages, v_pages, page_table, seq_lens, c
     out = torch.empty(T, Hq, d, dtype=q.dtype, device=dev)
     if out.numel() == 0:
         return out
-    q = _rows16(q)
+    q, strides = _rows_of_tokens(q)
     L = lib()
-    nbytes = ctypes.c_size_t(0)
-    check(L.hba_paged_attn_workspace_bytes(T, Bd, Hq, Hkv, d, window, sinks, shared // BLOCK, cu is None, max_len,
-                                           ctypes.byref(nbytes)), "hba_paged_attn_workspace_bytes")
-    nbytes = nbytes.value
+    pages = shared // BLOCK
+    nbytes = _paged_workspace(mx, T, Bd, Hq, Hkv, d, window, sinks, pages, cu is None, max_len)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     with _on(dev):
         if mx:
-            st = L.hba_paged_attn_mx(code, _p(q), used_strides2(q), _p(qg), eps, _p(cos), _p(sin), n_tab, bits,
-                                     _p(kr_pages), _p(v_pages), P, _p(page_table), maxp, _p(seq_lens), _p(sc), _p(cu), T,
-                                     Bd, Hq, Hkv, d, BLOCK, window, sinks, shared // BLOCK, max_len, _p(ws), nbytes,
-                                     _p(out), _stream(dev))
+            st = L.hba_paged_attn_mx(code, q.data_ptr(), strides, _p(qg), eps, _p(cos), _p(sin), n_tab, bits,
+                                     kr_pages.data_ptr(), v_pages.data_ptr(), P, page_table.data_ptr(), maxp,
+                                     seq_lens.data_ptr(), sc.data_ptr(), _p(cu), T, Bd, Hq, Hkv, d, BLOCK, window, sinks,
+                                     pages, max_len, _p(ws), nbytes, out.data_ptr(), _stream(dev))
         else:
-            st = L.hba_paged_attn(code, _p(q), used_strides2(q), _p(qg), eps, _p(cos), _p(sin), n_tab, _p(kr_pages),
-                                  _p(v_pages), P, _p(page_table), maxp, _p(seq_lens), _p(sc), _p(cu), T, Bd, Hq, Hkv, d,
-                                  BLOCK, window, sinks, shared // BLOCK, max_len, _p(ws), nbytes, _p(out), _stream(dev))
+            st = L.hba_paged_attn(code, q.data_ptr(), strides, _p(qg), eps, _p(cos), _p(sin), n_tab, kr_pages.data_ptr(),
+                                  v_pages.data_ptr(), P, page_table.data_ptr(), maxp, seq_lens.data_ptr(), sc.data_ptr(),
+                                  _p(cu), T, Bd, Hq, Hkv, d, BLOCK, window, sinks, pages, max_len, _p(ws), nbytes,
+                                  out.data_ptr(), _stream(dev))
     check(st, "hba_paged_attn_mx" if mx else "hba_paged_attn")
     return out
 
@@ -1162,18 +1183,22 @@ def mx_page_bytes(d, bits):
     return BLOCK * d * bits // 8 + 2 * d
 
 
+_MX_BITS = {(d, mx_page_bytes(d, bits)): bits for d in (64, 128) for bits in (4, 8)}
+
+
 def _mx_pages(k_pages, v_pages, d, dev):
     """Checks the pages; returns (pages, KV heads, bits)."""
+    shape = k_pages.shape
     for t, what in ((k_pages, "k_pages"), (v_pages, "v_pages")):
-        if t.dtype != torch.uint8 or t.device != dev or not t.is_contiguous() or t.dim() != 3:
+        if t.dtype is not torch.uint8 or t.get_device() != dev.index or not t.is_contiguous() or len(shape) != 3:
             raise ValueError(f"{what} must be a contiguous uint8 tensor [pages, KV heads, bytes] on {dev}")
-        if t.shape != k_pages.shape or t.shape[0] == 0 or t.shape[1] == 0:
-            raise ValueError(f"{what}: expected the shape of k_pages, and a page and a KV head at least")
-    for bits in (4, 8):
-        if k_pages.shape[2] == mx_page_bytes(d, bits):
-            return k_pages.shape[0], k_pages.shape[1], bits
-    raise ValueError(f"k_pages: {k_pages.shape[2]} bytes per page and KV head; head dim {d} has {mx_page_bytes(d, 4)} "
-                     f"(4 bits) or {mx_page_bytes(d, 8)} (8 bits)")
+    if v_pages.shape != shape or shape[0] == 0 or shape[1] == 0:
+        raise ValueError("v_pages: expected the shape of k_pages, and a page and a KV head at least")
+    bits = _MX_BITS.get((d, shape[2]))
+    if bits is None:
+        raise ValueError(f"k_pages: {shape[2]} bytes per page and KV head; head dim {d} has {mx_page_bytes(d, 4)} "
+                         f"(4 bits) or {mx_page_bytes(d, 8)} (8 bits)")
+    return shape[0], shape[1], bits
 
 
 def _mx_batch(page_table, seq_lens, cu, T, dev):
@@ -1192,7 +1217,7 @@ def _mx_batch(page_table, seq_lens, cu, T, dev):
 
 def _kv_append_mx(k, v, cu, k_gain, eps, cos, sin, page_table, seq_lens, k_pages, v_pages):
     dev = _dev(k)
-    if k.dim() != 3 or v.shape != k.shape or v.dtype != k.dtype or v.device != dev:
+    if k.dim() != 3 or v.shape != k.shape or v.dtype != k.dtype or v.get_device() != dev.index:
         raise ValueError("k and v: expected two [T, Hkv, d] tensors of one type and device")
     T, Hkv, d = k.shape
     code = _code(k)
@@ -1209,11 +1234,11 @@ def _kv_append_mx(k, v, cu, k_gain, eps, cos, sin, page_table, seq_lens, k_pages
     kg = _f32c(k_gain, dev, Hkv, "k_gain")
     if T == 0 or Bd == 0:
         return
-    k, v = _rows16(k), _rows16(v)
+    (k, ks), (v, vs) = _rows_of_tokens(k), _rows_of_tokens(v)
     with _on(dev):
-        st = lib().hba_kv_append_mx(code, _p(k), used_strides2(k), _p(v), used_strides2(v), _p(cu), T, _p(kg), eps, _p(cos),
-                                    _p(sin), n_tab, _p(page_table), maxp, _p(seq_lens), Bd, Hkv, d, BLOCK, bits, P,
-                                    _p(k_pages), _p(v_pages), _stream(dev))
+        st = lib().hba_kv_append_mx(code, k.data_ptr(), ks, v.data_ptr(), vs, _p(cu), T, _p(kg), eps, _p(cos), _p(sin), n_tab,
+                                    page_table.data_ptr(), maxp, seq_lens.data_ptr(), Bd, Hkv, d, BLOCK, bits, P,
+                                    k_pages.data_ptr(), v_pages.data_ptr(), _stream(dev))
     check(st, "hba_kv_append_mx")
 
 
@@ -1250,14 +1275,16 @@ def _kv_read_mx(k_pages, v_pages, page_table, seq_lens, cu, tokens, head_dim, dt
         raise ValueError(f"tokens must not be negative, got {tokens}")
     P, Hkv, bits = _mx_pages(k_pages, v_pages, head_dim, dev)
     Bd, maxp = _mx_batch(page_table, seq_lens, cu, tokens, dev)
-    k, v = (torch.empty(tokens, Hkv, head_dim, dtype=dtype, device=dev) for _ in range(2))
+    k = torch.empty(tokens, Hkv, head_dim, dtype=dtype, device=dev)
+    v = torch.empty_like(k)
     if tokens == 0:
         return k, v
     if Bd == 0:
         return k.zero_(), v.zero_()
     with _on(dev):
-        st = lib().hba_kv_read_mx(_DT[dtype], _p(k_pages), _p(v_pages), P, _p(page_table), maxp, _p(seq_lens), _p(cu),
-                                  tokens, Bd, Hkv, head_dim, BLOCK, bits, _p(k), _p(v), _stream(dev))
+        st = lib().hba_kv_read_mx(_DT[dtype], k_pages.data_ptr(), v_pages.data_ptr(), P, page_table.data_ptr(), maxp,
+                                  seq_lens.data_ptr(), _p(cu), tokens, Bd, Hkv, head_dim, BLOCK, bits, k.data_ptr(),
+                                  v.data_ptr(), _stream(dev))
     check(st, "hba_kv_read_mx")
     return k, v
 

@@ -598,12 +598,15 @@ int hba_kv_read_mx(int dtype, const void *k_pages, const void *v_pages, int64_t 
                    int64_t bits, void *k, void *v, void *stream);
 
 /*
- * hba_paged_attn over it: the same arguments (workspace: hba_paged_attn_workspace_bytes),
+ * hba_paged_attn over it: the same arguments (workspace: hba_paged_attn_mx_workspace_bytes),
  * the same rules.  Keys and values enter the products as they are (bf16 holds them);
  * fp32: queries and probabilities in three bf16 parts (24 bits of mantissa).  Values
  * behind a sequence's length may be anything.  A NaN before it has no effect on tokens
  * that do not see it (with cu as there: slow for those beside it).
  */
+int hba_paged_attn_mx_workspace_bytes(int64_t T, int64_t Bd, int64_t Hq, int64_t Hkv, int64_t d,
+                                      int64_t W, int64_t S, int64_t shared_pages, int one_each,
+                                      int64_t max_len, size_t *bytes);
 int hba_paged_attn_mx(int dtype, const void *q, const int64_t q_strides[2], const float *q_gain,
                       float eps, const float *cos_tab, const float *sin_tab, int64_t n_tab,
                       int64_t bits, const void *k_pages, const void *v_pages, int64_t num_pages,

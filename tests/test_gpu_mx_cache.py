@@ -306,10 +306,14 @@ def call(s, W=0, S=0, **kw):
 
 
 def expect(s, W=0, S=0):
-    """Results and bounds (attn64).  Keys and values are exact.  bf16: a query in two bf16
-    parts, u^2 of it lost at most; fp32: in three, 2^-24.  A product of parts is two or
-    three fp32 sums where the bounds count one: 2 d E more of a logit's |q||k|, 2 N E of a
-    result's sum."""
+    """Results and bounds (attn64).  Keys and values are exact.  A query enters in parts.
+    bf16 queries: two of bf16, u^2 of it lost at most, or (4 bits) three of e2m3 at least;
+    fp32: three of bf16, 2^-24, or six of e2m3.  N parts of e2m3 (steps of 1/8 up to 2, of
+    1/4 up to 4, of 1/2 up to 7.5) of a group whose largest magnitude is taken to (3.75,
+    7.5]: the first leaves 1/4 at most, which 2^4 takes to 4, and the second 1/8 of its unit,
+    which 2^5 takes to 4, and so on: 2^-(7 + 5 (N - 2)) of the first unit, over 3.75 of
+    them.  A product of parts is up to six fp32 sums where the bounds count one: 5 d E more
+    of a logit's |q||k|, 2 N E of a result's sum."""
     dt, (T, Hq, d) = s["q"].dtype, s["q"].shape
     Hkv = s["kp"].shape[1]
     G, u = Hq // Hkv, unit(dt)
@@ -322,7 +326,10 @@ def expect(s, W=0, S=0):
         at = pos.clamp(0, s["cos"].shape[0] - 1) if s["cos"] is not None else None
         cs, sn = (None, None) if at is None else (s["cos"][at], s["sin"][at])
         _, q, qe = norm_rotate(s["q"][t:t + c], s["gain"], EPS, cs, sn, u * u if dt == torch.bfloat16 else E)
-        qe = qe + 2 * d * E * q.abs()
+        qe = qe + 5 * d * E * q.abs()
+        if s["bits"] == 4:
+            n6 = 3 if dt == torch.bfloat16 else 6
+            qe = qe + 2.0 ** -(7 + 5 * (n6 - 2)) / 3.75 * q.unflatten(-1, (-1, 32)).abs().amax(-1).repeat_interleave(32, -1)
         see = visible(pos, torch.arange(max(n, 0)), W or None, S)
         for h in range(Hkv):
             if n > 0 and c > 0:
