@@ -119,18 +119,90 @@ __device__ __forceinline__ uint32_t load4(Buffer b, uint32_t lane, uint32_t at) 
     return __builtin_amdgcn_raw_buffer_load_b32(b, lane + at, 0, 0);
 }
 
+// c + a 32x32 product over 64 elements: e2m1 codes with byte KB of ks as their scale (lane
+// l: row l % 32, elements 32 (l / 32) ..), e2m3 with byte QB of qs (columns).
+template <int KB, int QB> __device__ __forceinline__ f32x16 product6(u32x4 k, i32x8 q, f32x16 c, int ks, int qs) {
+    const i32x8 a = {(int)k[0], (int)k[1], (int)k[2], (int)k[3], 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, q, c, 4, 2, KB, ks, QB, qs);
+}
+// A query's 32 elements of a group as N parts of e2m3 (6 bits), each with a power of two
+// of its own: the largest magnitude goes to (3.75, 7.5], what the rounding leaves (1/4 of
+// the first unit at most) times 2^4, of every later one times 2^5.  N parts leave at most
+// 2^-(5 N - 1.1) of the largest magnitude (3 of bf16 queries: 2^-13.9).
+template <int N> struct Query6 {
+    u32x6 q[N];
+    int scale[N];   // bytes
+};
+template <int N> __device__ __forceinline__ Query6<N> parts6(const float (&y)[32]) {
+    Query6<N> r;
+    uint32_t big = 0;
+#pragma unroll
+    for (int e = 0; e < 32; ++e) big = max(big, __float_as_uint(y[e]) & 0x7fffffffu);
+    const int b = (int)(big >> 23) - 2 + ((big & 0x7fffffu) > 0x700000u);
+    const bool bad = big >= 0x7f800000u;   // 255 makes every logit NaN
+    f32x16 x[2];                           // even and odd elements, as the conversion takes them
+#pragma unroll
+    for (int e = 0; e < 32; ++e) x[e & 1][e >> 1] = bad ? 0.0f : y[e];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        r.scale[n] = bad ? 255 : max(n == 0 ? b : b + 1 - 5 * n, 1);
+        const float f = __uint_as_float((uint32_t)(bad ? 127 : r.scale[n]) << 23);
+        r.q[n] = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(x[0], x[1], f);
+        const f32x32 back = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(r.q[n], f);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) x[e & 1][e >> 1] -= back[e];
+    }
+    return r;
+}
+// The columns of a 32x32 product: lane l has column l % 32, and of every 64 elements
+// those 32 (l / 32) .. + 31, in N parts.
+template <int D, int N> struct Rows6 {
+    i32x8 q[D / 64][N];
+    int qs[D / 64][2];   // scales, a byte each
+    // x[s]: the elements 64 s + 32 (l / 32) .. of the column
+    __device__ __forceinline__ void set(const float (&x)[D / 64][32]) {
+#pragma unroll
+        for (int s = 0; s < D / 64; ++s) {
+            const Query6<N> r = parts6<N>(x[s]);
+            qs[s][0] = qs[s][1] = 0;
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                q[s][n] = i32x8{(int)r.q[n][0], (int)r.q[n][1], (int)r.q[n][2], (int)r.q[n][3], (int)r.q[n][4],
+                                (int)r.q[n][5], 0, 0};
+                qs[s][n / 4] |= r.scale[n] << (8 * (n % 4));
+            }
+        }
+    }
+    // element e of x[s] again
+    __device__ __forceinline__ void get(int s, float (&x)[32]) const {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) x[e] = 0.0f;
+#pragma unroll
+        for (int n = N - 1; n >= 0; --n) {
+            const u32x6 w = {(uint32_t)q[s][n][0], (uint32_t)q[s][n][1], (uint32_t)q[s][n][2],
+                             (uint32_t)q[s][n][3], (uint32_t)q[s][n][4], (uint32_t)q[s][n][5]};
+            const uint32_t b = (uint32_t)qs[s][n / 4] >> (8 * (n % 4)) & 255u;
+            const f32x32 y = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(w, __uint_as_float(b << 23));
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[e] += y[e];
+        }
+    }
+};
+
 // ------------------------------------------------------------ staged tiles --
 // Keys and values of one KV head, for rows::attend: a tile's codes are loaded into
-// registers while the tile before it is worked on, and become the bf16 tile that
-// rows::PageKV stages.  A thread has 16 codes of the keys and 16 of the values: of a
-// key, half a group at most; of the values, eight tokens in two columns of a group.
+// registers while the tile before it is worked on.  Values, and keys of 8 bits, become
+// the bf16 tile that rows::PageKV stages; keys of 4 bits stay codes (CODES), with their
+// scales behind them, and the queries are Rows6.  A thread has 16 codes of the keys and
+// 16 of the values: of a key, half a group at most; of the values, eight tokens in two
+// columns of a group.
 template <int DT, int D, int F> struct TileKV {
     typedef typename rows::Op<DT>::F Q;    // the queries' operand
     typedef rows::PageKV<1, D> Bf16;
     typedef Place<D, F> At;
-    static constexpr int KT = Bf16::KT, TP = Bf16::TP, HALF = Bf16::HALF, BYTES = Bf16::BYTES;
-    static constexpr int NG = D / GROUP, NB = 16 * F / 8;   // a thread's bytes of codes
-    static constexpr bool TAIL = false;                     // stage clears what lies behind the sequence
+    static constexpr bool CODES = F == 4, TAIL = false;     // stage clears what lies behind the sequence
+    static constexpr int KT = Bf16::KT, TP = Bf16::TP, NG = D / GROUP, NB = 16 * F / 8;   // NB: a thread's bytes of codes
+    static constexpr int KEYB = CODES ? KT * D / 2 + 256 : KT * D * 2, BYTES = KEYB + KT * D * 2;
     const char *k, *v;            // the KV head's place in page 0
     int64_t page;                 // bytes from page to page
     const int32_t *table;
@@ -148,36 +220,49 @@ template <int DT, int D, int F> struct TileKV {
     // The thread's 16 codes q = thread / 64 of its lane's stream in this tile: a tile of
     // 16 keys (D = 64) or half of one (128); columns 32 g .. of 32 tokens.
     static __device__ __forceinline__ int unit() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
-    template <class T> static __device__ __forceinline__ void get(uint32_t (&to)[NB / 4], const char *p) {
-        const T x = *reinterpret_cast<const T *>(p);
-        __builtin_memcpy(to, &x, sizeof x);
+    static __device__ __forceinline__ void get(uint32_t (&to)[NB / 4], Buffer b, uint32_t lane, uint32_t at) {
+        if constexpr (F == 4) {
+            const u32x2 x = load8(b, lane, at);
+            __builtin_memcpy(to, &x, sizeof x);
+        } else {
+            const u32x4 x = load16(b, lane, at);
+            __builtin_memcpy(to, &x, sizeof x);
+        }
     }
     __device__ __forceinline__ void next(int tile) {
-        typedef __attribute__((ext_vector_type(NB / 4))) uint32_t V;
+        constexpr int HB = (int)page_bytes(D, F), CB = (int)code_bytes(D, F);
         id = at(tile / TP);
         half = tile % TP;
-        const int q = unit(), lane = threadIdx.x & 63, x = q * NB, first = half * (4 * NB) * 64;
-        const char *kp = k + id * page, *vp = v + id * page;
-        get<V>(kc, kp + first + (x / 16 * 64 + lane) * 16 + x % 16);
-        get<V>(vc, vp + first + (x / 16 * 64 + lane) * 16 + x % 16);
-        const int g = (lane >> 4) * (D / 4) / GROUP;
-        ks = *reinterpret_cast<const uint32_t *>(kp + code_bytes(D, F) + ((lane & 15) + 16 * g) * 4);
+        const int q = unit(), lane = threadIdx.x & 63, lg = lane >> 4, x = q * NB;
+        const uint32_t first = half * (4 * NB) * 64 + x / 16 * 1024 + x % 16;
+        const Buffer kp = buffer(k + id * page, HB), vp = buffer(v + id * page, HB);
+        get(kc, kp, lane * 16, first);
+        get(vc, vp, lane * 16, first);
+        // the scales: as they lie there, for a tile of codes
+        ks = load4(kp, (CODES ? lane % (16 * NG) : (lane & 15) + 16 * (lg * (D / 4) / GROUP)) * 4, CB);
         const int h = D == 64 ? q >> 1 : half, vg = D == 64 ? q & 1 : q;
-        const u32x2 s = *reinterpret_cast<const u32x2 *>(vp + code_bytes(D, F) + ((h * 4 + (lane >> 4)) * NG + vg) * 8);
+        const u32x2 s = load8(vp, lg * (NG * 8), CB + (h * 4 * NG + vg) * 8);
         vs[0] = s[0];
         vs[1] = s[1];
     }
     __device__ __forceinline__ void stage(int tile, uint32_t lds) {
         typedef __attribute__((address_space(3))) u32x4 *out;
         const int q = unit(), lane = threadIdx.x & 63, l16 = lane & 15, lg = lane >> 4;
-        const int mt = D == 64 ? q : q >> 1, t0 = D / 4 * lg + (D == 64 ? 0 : 16 * (q & 1));   // key tile here, first element
-        const int pt = D == 64 ? mt : 2 * half + mt;                                           // and in its page
-        const float sc = __uint_as_float((ks >> (8 * pt) & 255u) << 23);
+        if constexpr (CODES) {
+            const int x = q * NB;
+            *(__attribute__((address_space(3))) u32x2 *)(uintptr_t)(lds + (x / 16 * 64 + lane) * 16 + x % 16) = u32x2{kc[0], kc[1]};
+            // the tile's scales in the low bytes, by all waves alike
+            *(__attribute__((address_space(3))) uint32_t *)(uintptr_t)(lds + KT * D / 2 + lane % (16 * NG) * 4) = ks >> (16 * half);
+        } else {
+            const int mt = D == 64 ? q : q >> 1, t0 = D / 4 * lg + (D == 64 ? 0 : 16 * (q & 1));   // key tile here, first element
+            const int pt = D == 64 ? mt : 2 * half + mt;                                           // and in its page
+            const float sc = __uint_as_float((ks >> (8 * pt) & 255u) << 23);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const int t = t0 + 8 * c;
-            *(out)(uintptr_t)(lds + ((mt * (D / 32) + (t >> 5)) * 64 + l16 + 16 * ((t >> 3) & 3)) * 16) =
-                __builtin_bit_cast(u32x4, eight<F>(kc + c * (F / 4), sc));
+            for (int c = 0; c < 2; ++c) {
+                const int t = t0 + 8 * c;
+                *(out)(uintptr_t)(lds + ((mt * (D / 32) + (t >> 5)) * 64 + l16 + 16 * ((t >> 3) & 3)) * 16) =
+                    __builtin_bit_cast(u32x4, eight<F>(kc + c * (F / 4), sc));
+            }
         }
         const int h = D == 64 ? q >> 1 : 0, g = D == 64 ? q & 1 : q;
         const int left = len - tile * KT - 32 * h - 8 * lg;   // of the thread's eight tokens, those of the sequence
@@ -207,18 +292,65 @@ template <int DT, int D, int F> struct TileKV {
                 const uint32_t hi = __builtin_bit_cast(uint32_t, two<F>(w, s[2 * i + 1], p));
                 r[i] = __builtin_amdgcn_perm(hi, lo, 0x07060100);
             }
-            *(out)(uintptr_t)(lds + HALF + (((2 * g + c) * (KT / 32) + h) * 64 + lane) * 16) = r;
+            *(out)(uintptr_t)(lds + KEYB + (((2 * g + c) * (KT / 32) + h) * 64 + lane) * 16) = r;
         }
     }
     static __device__ __forceinline__ int key(int r, int hf) { return Bf16::key(r, hf); }
     static __device__ __forceinline__ bf16x8 kf(const char *t, int kt, int ks, int lane) { return Bf16::kf(t, kt, ks, lane); }
     static __device__ __forceinline__ bf16x8 vf(const char *t, int kt, int dt, int u, int lane) {
-        return Bf16::vf(t, kt, dt, u, lane);
+        const int x = 32 * dt + (lane & 31);
+        return rows::Op<1>::load(t + KEYB + (((x >> 4) * (KT / 32) + kt) * 64 + (x & 15) + 16 * (2 * u + (lane >> 5))) * 16);
+    }
+    // c + the products of tile kt's 32 keys (in PageKV's order) with the queries
+    template <int N> static __device__ __forceinline__ f32x16 logits(const char *t, int kt, const Rows6<D, N> &q, f32x16 c, int lane) {
+        const int r = lane & 31, hf = lane >> 5, l16 = 8 * (r >> 4) + 4 * ((r >> 2) & 1) + (r & 3), odd = (r >> 3) & 1;
+#pragma unroll
+        for (int s = 0; s < D / 64; ++s) {
+            const int g = 2 * s + hf;
+            u32x4 k;
+            if constexpr (D == 64) {   // a group is the pieces' halves in two places
+                const char *p = t + kt * 1024 + (l16 + 32 * g) * 16 + 8 * odd;
+                const u32x2 lo = *reinterpret_cast<const u32x2 *>(p), hi = *reinterpret_cast<const u32x2 *>(p + 256);
+                k = __builtin_shufflevector(lo, hi, 0, 1, 2, 3);
+            } else {
+                k = *reinterpret_cast<const u32x4 *>(t + (odd * 64 + l16 + 16 * g) * 16);
+            }
+            const int ks = (int)(*reinterpret_cast<const uint32_t *>(t + KT * D / 2 + (l16 + 16 * g) * 4) >> (8 * odd));
+            c = kt == 0 ? products<0>(k, q.q[s], c, ks, q.qs[s]) : products<2>(k, q.q[s], c, ks, q.qs[s]);
+        }
+        return c;
+    }
+    template <int KB, int N> static __device__ __forceinline__ f32x16 products(u32x4 k, const i32x8 (&q)[N], f32x16 c, int ks,
+                                                                               const int (&qs)[2]) {
+        c = product6<KB, 0>(k, q[0], c, ks, qs[0]);
+        if constexpr (N > 1) c = product6<KB, 1>(k, q[1], c, ks, qs[0]);
+        if constexpr (N > 2) c = product6<KB, 2>(k, q[2], c, ks, qs[0]);
+        if constexpr (N > 3) c = product6<KB, 3>(k, q[3], c, ks, qs[0]);
+        if constexpr (N > 4) c = product6<KB, 0>(k, q[4], c, ks, qs[1]);
+        if constexpr (N > 5) c = product6<KB, 1>(k, q[5], c, ks, qs[1]);
+        return c;
     }
     // one key, for attend_each
     static __device__ __forceinline__ float value(const char *p, int at_code, int at_scale, int odd) {
         const uint32_t c = (uint8_t)p[at_code];
         return one<F>(F == 4 ? c >> (4 * odd) : c, __uint_as_float((uint32_t)(uint8_t)p[at_scale] << 23));
+    }
+    template <bool LO, int N> __device__ __forceinline__ float dot(const Rows6<D, N> &q, const Q *, int j, int hf) const {
+        const char *p = k + at(j / rows::PAGE) * page;
+        const int jp = j % rows::PAGE;
+        float sum = 0.0f;
+#pragma unroll
+        for (int s = 0; s < D / 64; ++s) {
+            float x[32];
+            q.get(s, x);
+            const int g = 2 * s + hf;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+                sum = fmaf(x[e], value(p, At::key(jp, 32 * g + e), At::key_scale(jp, g), e & 1), sum);
+                if (e % 8 == 7) __builtin_amdgcn_sched_barrier(0);   // few registers, not speed
+            }
+        }
+        return sum + rows::other_half(sum);
     }
     template <bool LO> __device__ __forceinline__ float dot(const Q (&q)[D / 16], const Q *qlo, int j, int hf) const {
         const char *p = k + at(j / rows::PAGE) * page;
@@ -235,7 +367,7 @@ template <int DT, int D, int F> struct TileKV {
                 sum = fmaf(a[e], x, sum);
                 if constexpr (DT == 1 && LO) sum = fmaf(b[e], x, sum);
             }
-            __builtin_amdgcn_sched_barrier(0);   // few registers, not speed
+            __builtin_amdgcn_sched_barrier(0);
         }
         return sum + rows::other_half(sum);
     }

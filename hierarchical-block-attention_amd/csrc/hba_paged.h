@@ -143,36 +143,6 @@ __device__ __forceinline__ Pages page_list(const Args &a, int L) {
 }
 
 // ------------------------------------------------------------ decode, codes --
-// A query's 32 elements of a group as N parts of e2m3 (6 bits), each with a power of two
-// of its own: the largest magnitude goes to (3.75, 7.5], what the rounding leaves (1/4 of
-// the first unit at most) times 2^4, of every later one times 2^5.  N parts leave at most
-// 2^-(5 N - 1.1) of the largest magnitude (3 of bf16 queries: 2^-13.9).
-template <int N> struct Query6 {
-    mx::u32x6 q[N];
-    int scale[N];   // bytes
-};
-template <int N> __device__ __forceinline__ Query6<N> parts6(const float (&y)[32]) {
-    Query6<N> r;
-    uint32_t big = 0;
-#pragma unroll
-    for (int e = 0; e < 32; ++e) big = max(big, __float_as_uint(y[e]) & 0x7fffffffu);
-    const int b = (int)(big >> 23) - 2 + ((big & 0x7fffffu) > 0x700000u);
-    const bool bad = big >= 0x7f800000u;   // 255 makes every logit NaN
-    mx::f32x16 x[2];                       // even and odd elements, as the conversion takes them
-#pragma unroll
-    for (int e = 0; e < 32; ++e) x[e & 1][e >> 1] = bad ? 0.0f : y[e];
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-        r.scale[n] = bad ? 255 : max(n == 0 ? b : b + 1 - 5 * n, 1);
-        const float f = __uint_as_float((uint32_t)(bad ? 127 : r.scale[n]) << 23);
-        r.q[n] = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(x[0], x[1], f);
-        const mx::f32x32 back = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(r.q[n], f);
-#pragma unroll
-        for (int e = 0; e < 32; ++e) x[e & 1][e >> 1] -= back[e];
-    }
-    return r;
-}
-
 // QKNorm, rotation (cs, sn: the lane's; y: the elements half a head away) and scale of a
 // lane's N consecutive elements x of a head; lanes 16 and (ALL) 32 away have the others.
 template <int D, int N, bool ALL>
@@ -300,7 +270,7 @@ __device__ __forceinline__ void decode_codes(const Args &a, int s, int g, int he
         finish_group<D, NE, FMT == 8 || D == 128>(qx, qy, first < D / 2, a.gain ? a.gain + head : nullptr, a.eps,
                                                   a.cos != nullptr, cs, sn, a.scales[s] * LOG2E);
         if constexpr (FMT == 4) {
-            const Query6<NQ> r = parts6<NQ>(qx);
+            const mx::Query6<NQ> r = mx::parts6<NQ>(qx);
             int qs[2] = {0, 0};
 #pragma unroll
             for (int n = 0; n < NM; ++n) {
@@ -758,19 +728,20 @@ template <int NT> __device__ __forceinline__ Shares shares(const Args &a) {
     x.per = max(a.part, (x.units + a.slots - 1) / a.slots);
     return x;
 }
-// The same for codes (at most MOST sequences), where a share's own work is short: the pages
-// before each sequence are found once, in LDS, and for the join a group's first share
-// writes down which parts are its own (records: [groups][2], the first one and how
-// many, 0 if the group is done).
-constexpr int MOST = 1024;
-template <int DT, int D, int FMT, int NS> __global__ __launch_bounds__(64 * DW) void even_codes_kernel(const Args a) {
-    constexpr int NT = 64 * DW;
-    __shared__ DecodeLds<D> lds;
-    __shared__ int before[MOST + 1], len[MOST], wsum[DW], found;
+// The same for codes (at most MOST sequences), where a share's own work is short: what
+// comes before each sequence is found once, in LDS, and for the join a group's first
+// share writes down which parts are its own (records: [groups][2], the first one and how
+// many, 0 if the group is done).  A second part costs a workgroup as much as
+// EXTRA pages (5 us: its query, first loads and sums).  So where parts of up to so many
+// pages more make no more of them than there are shares, each workgroup has one part.
+constexpr int MOST = 1024, EXTRA = 16;
+// The sums of count(i) over the sequences before each i, and over all, by a workgroup.
+template <int NT, class F> __device__ __forceinline__ int sums_before(int Bd, int (&before)[MOST + 1], const F &count) {
+    __shared__ int wsum[NT / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int sum = 0;
-    for (int base = 0; base < a.Bd; base += NT) {
-        const int i = base + tid, L = i < a.Bd ? length(a, i) : 0, n = i < a.Bd ? max(1, page_list(a, L).n) : 0;
+    for (int base = 0; base < Bd; base += NT) {
+        const int i = base + tid, n = i < Bd ? count(i) : 0;
         int upto = n;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -781,36 +752,71 @@ template <int DT, int D, int FMT, int NS> __global__ __launch_bounds__(64 * DW) 
         __syncthreads();
         int all = 0;
 #pragma unroll
-        for (int w = 0; w < DW; ++w) {
+        for (int w = 0; w < NT / 64; ++w) {
             if (w < wave) upto += wsum[w];
             all += wsum[w];
         }
-        if (i < a.Bd) {
-            before[i] = sum + upto - n;
-            len[i] = L;
-        }
+        if (i < Bd) before[i] = sum + upto - n;
         sum += all;
         __syncthreads();
     }
-    const int ng = groups_of(a), w = blockIdx.x, units = sum * ng, per = max(a.part, (units + a.slots - 1) / a.slots);
-    const int64_t u0 = (int64_t)w * per;
-    if (tid == 0) before[a.Bd] = sum;
+    if (tid == 0) before[Bd] = sum;
     __syncthreads();
-    if (u0 >= units) return;
-    for (int i = tid; i < a.Bd; i += NT)
-        if (u0 >= (int64_t)before[i] * ng && u0 < (int64_t)before[i + 1] * ng) found = i;
+    return __builtin_amdgcn_readfirstlane(sum);
+}
+template <int DT, int D, int FMT, int NS> __global__ __launch_bounds__(64 * DW) void even_codes_kernel(const Args a) {
+    constexpr int NT = 64 * DW;
+    __shared__ DecodeLds<D> lds;
+    __shared__ int before[MOST + 1], pages[MOST], len[MOST], counts[EXTRA], found;
+    const int tid = threadIdx.x, w = blockIdx.x, ng = groups_of(a);
+    const auto find = [&](int64_t x) {   // the sequence with place x
+        for (int i = tid; i < a.Bd; i += NT)
+            if (x >= (int64_t)before[i] * ng && x < (int64_t)before[i + 1] * ng) found = i;
+        __syncthreads();
+        return __builtin_amdgcn_readfirstlane(found);
+    };
+    const int units = sums_before<NT>(a.Bd, before, [&](int i) {
+        len[i] = length(a, i);
+        return pages[i] = max(1, page_list(a, len[i]).n);
+    }) * ng;
+    int per = max(a.part, (units + a.slots - 1) / a.slots);
+    {   // the parts there are at per + c pages
+        static_assert(NT % EXTRA == 0 && NT / EXTRA <= 64, "a candidate's threads are lanes of a wave");
+        const int c = tid / (NT / EXTRA);
+        int n = 0;
+        for (int i = tid % (NT / EXTRA); i < a.Bd; i += NT / EXTRA) n += (pages[i] + per + c - 1) / (per + c);
+#pragma unroll
+        for (int o = 1; o < NT / EXTRA; o <<= 1) n += __shfl_xor(n, o, 64);
+        counts[c] = n * ng;
+    }
     __syncthreads();
-    int s = __builtin_amdgcn_readfirstlane(found);
-    int left = (int)min((int64_t)per, units - u0), at = (int)u0 - before[s] * ng;
-    for (int part = 2 * w; left > 0 && s < a.Bd; part = 2 * w + 1) {
-        const int n = __builtin_amdgcn_readfirstlane(before[s + 1] - before[s]), L = __builtin_amdgcn_readfirstlane(len[s]);
-        const int gi = at / n, p0 = at % n, p1 = min(n, p0 + left);
-        if (p0 == 0 && tid == 0) {
-            const int last = (int)((u0 + (int)min((int64_t)per, units - u0) - left + n - 1) / per);
-            a.records[2 * (s * ng + gi)] = part;
-            a.records[2 * (s * ng + gi) + 1] = p1 == n ? 0 : last - w + 1;
+    int more = 0;
+    while (more < EXTRA && counts[more] > a.slots) ++more;
+    if (more < EXTRA) {
+        per += more;
+        const int parts = sums_before<NT>(a.Bd, before, [&](int i) { return (pages[i] + per - 1) / per; }) * ng;
+        if (w >= parts) return;
+        const int s = find(w), n = __builtin_amdgcn_readfirstlane(pages[s]), k = (n + per - 1) / per;
+        const int x = w - __builtin_amdgcn_readfirstlane(before[s]) * ng, gi = x / k, z = x % k, run = (n + k - 1) / k;
+        if (z == 0 && tid == 0) {
+            a.records[2 * (s * ng + gi)] = 2 * w;
+            a.records[2 * (s * ng + gi) + 1] = k == 1 ? 0 : k;
         }
-        decode_part<DT, D, DW, FMT, NS>(a, lds, s, gi, p0, p1, p1 - p0 == n ? -1 : (int64_t)part * 16, 1, L);
+        decode_part<DT, D, DW, FMT, NS>(a, lds, s, gi, z * run, (z + 1) * run, k == 1 ? -1 : (int64_t)w * 32, 1,
+                                        __builtin_amdgcn_readfirstlane(len[s]));
+        return;
+    }
+    const int64_t u0 = (int64_t)w * per, u1 = min(u0 + per, (int64_t)units);
+    if (u0 >= units) return;
+    int s = find(u0), left = (int)(u1 - u0), at = (int)u0 - __builtin_amdgcn_readfirstlane(before[s]) * ng;
+    for (int part = 2 * w; left > 0 && s < a.Bd; part = 2 * w + 1) {
+        const int n = __builtin_amdgcn_readfirstlane(pages[s]), gi = at / n, p0 = at % n, p1 = min(n, p0 + left);
+        if (p0 == 0 && tid == 0) {
+            a.records[2 * (s * ng + gi)] = part;
+            a.records[2 * (s * ng + gi) + 1] = p1 == n ? 0 : (int)((u1 - left + n - 1) / per) - w + 1;
+        }
+        decode_part<DT, D, DW, FMT, NS>(a, lds, s, gi, p0, p1, p1 - p0 == n ? -1 : (int64_t)part * 16, 1,
+                                        __builtin_amdgcn_readfirstlane(len[s]));
         __syncthreads();   // lds is free again
         left -= p1 - p0;
         at += p1 - p0;
@@ -857,6 +863,35 @@ template <int DT, int D> __device__ __forceinline__ void zero_strays(const Args 
 // SHARED: the rows of all tokens over the shared pages (x: 128-row tile); else the
 // rows of one sequence's tokens over its own pages (x: tile of the ragged batch).
 // g: KV head, z: part, a run of a.part pages.
+// finish_q for Rows6: x[s] are the elements 64 s + 32 hf .. of the row; cs, sn begin at 32 hf.
+template <int D>
+__device__ __forceinline__ void finish_rows(float (&x)[D / 64][32], int hf, const float *gain, float eps, const float *cs,
+                                            const float *sn, float scale) {
+    if (gain) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int s = 0; s < D / 64; ++s)
+#pragma unroll
+            for (int e = 0; e < 32; ++e) ss = fmaf(x[s][e], x[s][e], ss);
+        ss += rows::other_half(ss);
+        scale *= *gain / sqrtf(fmaxf(ss / (float)D, eps));
+    }
+#pragma unroll
+    for (int e = 0; e < 32; ++e) {
+        if constexpr (D == 64) {
+            x[0][e] *= scale;
+            if (cs) {
+                const float y = rows::other_half(x[0][e]);
+                x[0][e] = x[0][e] * cs[e] + y * (hf ? sn[e] : -sn[e]);
+            }
+        } else {
+            const float lo = x[0][e] * scale, hi = x[1][e] * scale;
+            x[0][e] = cs ? lo * cs[e] - hi * sn[e] : lo;
+            x[1][e] = cs ? hi * cs[64 + e] + lo * sn[64 + e] : hi;
+        }
+    }
+}
+
 template <int DT, int D, int FMT> struct RowSource { typedef mx::TileKV<OPS<DT, FMT>, D, FMT> T; };
 template <int DT, int D> struct RowSource<DT, D, 0> { typedef rows::PageKV<DT, D> T; };
 template <int DT, int D, int FMT, bool SHARED>
@@ -948,8 +983,26 @@ __device__ __forceinline__ void rows_part(const Args &a, char *smem, int x, int 
         }
         rows::attend_begin(src, smem, it0, it1, ns, wt0);
     }
-    F qh[NKS], ql[OP == 2 ? 1 : NKS];   // OP 2 has all parts in qh
-    {
+    // the queries: operands of the product with bf16 or fp32 keys (OP 2 has all parts in
+    // qh), or with codes
+    constexpr int N6 = DT == 1 ? 3 : 6;
+    F qh[Source::CODES ? 1 : NKS], ql[Source::CODES || OP == 2 ? 1 : NKS];
+    mx::Rows6<D, N6> q6;
+    if constexpr (Source::CODES) {
+        float y[D / 64][32];
+        const char *q = a.q + (int64_t)t * a.qst + head * a.qsh;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+            float z[8];
+            Op<DT>::unpack(Op<DT>::load(q + (64 * (i / 4) + 32 * hf + 8 * (i % 4)) * ESZ), z);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[i / 4][8 * (i % 4) + e] = z[e];
+        }
+        const int64_t turn = max((int64_t)0, min((int64_t)pos, a.n_tab - 1)) * D + 32 * hf;
+        finish_rows<D>(y, hf, a.gain ? a.gain + head : nullptr, a.eps, a.cos ? a.cos + turn : nullptr,
+                       a.sin ? a.sin + turn : nullptr, a.scales[sq] * LOG2E);
+        q6.set(y);
+    } else {
         float y[NKS][8];
         const char *q = a.q + (int64_t)t * a.qst + head * a.qsh;
 #pragma unroll
@@ -964,11 +1017,15 @@ __device__ __forceinline__ void rows_part(const Args &a, char *smem, int x, int 
         }
     }
     rows::RowAcc<OP, D> acc;
-    rows::attend<OP, D, LO>(src, smem, qh, ql, 1.0f, it0, it1, ns, wt0, w, acc);
+    const auto &keys = [&]() -> const auto & {
+        if constexpr (Source::CODES) return q6;
+        else return qh;
+    }();
+    rows::attend<OP, D, LO>(src, smem, keys, ql, 1.0f, it0, it1, ns, wt0, w, acc);
     float l = acc.l + rows::other_half(acc.l);
     const bool valid = w.hi > 0;
     if (__ballot(valid && (rows::any_bad<D>(acc.O) || !rows::finite(l)))) {
-        rows::attend_each<OP, D, LO>(src, qh, ql, 1.0f, it0, it1, ns, wt0, w, acc);
+        rows::attend_each<OP, D, LO>(src, keys, ql, 1.0f, it0, it1, ns, wt0, w, acc);
         l = acc.l + rows::other_half(acc.l);
     }
     if (!in) return;

@@ -257,6 +257,7 @@ template <int DT, int D, int KEYS_ = KEYS<DT, D>> struct DenseKV {
     typedef Tile<DT, D> TL;
     static constexpr int KT = KEYS_, BYTES = 2 * KT * TL::ROWB;   // a staged tile: keys, then values
     static constexpr bool TAIL = false;               // no rows past `last` are read
+    static constexpr bool CODES = false;              // keys are operands of Op (else logits() takes the product)
     const char *k, *v;
     int64_t kb, vb;                                   // bytes from row to row
     int last;                                         // the last row that may be read
@@ -294,7 +295,7 @@ template <int DT, int D> struct PageKV {
     const int32_t *table;         // the sequence's pages
     int len;                      // its keys: what lies behind them in a page may be anything
     int64_t pages;                // pages there are
-    static constexpr bool TAIL = true;
+    static constexpr bool TAIL = true, CODES = false;
     int64_t id;                   // the page of the tile that is staged next
     int half;                     // and the tile's place in it
 
@@ -452,10 +453,10 @@ __device__ __forceinline__ void attend_begin(Src &src, char *smem, int it0, int 
 // SEP: the sum of the probabilities as they are, too.  O is divided by the sum of the
 // rounded ones, which its own weights are; a log-sum-exp from that would put a row's
 // gradients off by up to a bf16 rounding (2^-8) in common.
-template <int DT, int D, bool LO, bool ONE = false, bool SEP = false, class Src>
-__device__ __forceinline__ void attend(Src &src, char *smem, const typename Op<DT>::F (&q)[D / 16],
-                                       const typename Op<DT>::F *qlo, float c, int it0, int it1, int ns, int wt0,
-                                       const Sees &w, RowAcc<DT, D> &a, int which = 0) {
+template <int DT, int D, bool LO, bool ONE = false, bool SEP = false, class Src, class Q>
+__device__ __forceinline__ void attend(Src &src, char *smem, const Q &q, const typename Op<DT>::F *qlo, float c,
+                                       int it0, int it1, int ns, int wt0, const Sees &w, RowAcc<DT, D> &a,
+                                       int which = 0) {
     typedef typename Op<DT>::F F;
     constexpr int NKS = D / 16, NDT = D / 32, KT = Src::KT;
     const int lane = threadIdx.x & 63, hf = lane >> 5;
@@ -491,11 +492,15 @@ __device__ __forceinline__ void attend(Src &src, char *smem, const typename Op<D
             if (jh >= w.hi_max || (jh + 32 <= w.lo_min && jh >= w.S)) continue;
             f32x16 s = zero;
             if constexpr (LO) s = s + shift;
+            if constexpr (Src::CODES) {
+                s = src.logits(t, kt, q, s, lane);
+            } else {
 #pragma unroll
-            for (int ks = 0; ks < NKS; ++ks) {
-                const auto kf = src.kf(t, kt, ks, lane);
-                s = Op<DT>::mma(kf, q[ks], s);
-                if constexpr (LO && DT == 1) s = Op<DT>::mma(kf, qlo[ks], s);
+                for (int ks = 0; ks < NKS; ++ks) {
+                    const auto kf = src.kf(t, kt, ks, lane);
+                    s = Op<DT>::mma(kf, q[ks], s);
+                    if constexpr (LO && DT == 1) s = Op<DT>::mma(kf, qlo[ks], s);
+                }
             }
             if (!(jh + 32 <= w.hi_min && (jh >= w.lo_max || jh + 32 <= w.S))) {
                 const uint64_t see = seen_bits(w.lo, w.hi, w.S, jh) >> Src::key(0, hf);
@@ -599,10 +604,9 @@ __device__ __forceinline__ void DenseKV<DT, D, KT>::add(f32x16 (&o)[D / 32], int
 // attend, one key at a time: for rows that came out non-finite.  Each lane adds
 // the visible keys only, so nothing of a masked key reaches its row.  It is kept
 // from loading ahead: its registers would cost the kernels that hold it waves.
-template <int DT, int D, bool LO, class Src>
-__device__ __forceinline__ void attend_each(const Src &src, const typename Op<DT>::F (&q)[D / 16],
-                                         const typename Op<DT>::F *qlo, float c, int it0, int it1, int ns, int wt0,
-                                         const Sees &w, RowAcc<DT, D> &a) {
+template <int DT, int D, bool LO, class Src, class Q>
+__device__ __forceinline__ void attend_each(const Src &src, const Q &q, const typename Op<DT>::F *qlo, float c, int it0,
+                                            int it1, int ns, int wt0, const Sees &w, RowAcc<DT, D> &a) {
     const int hf = (threadIdx.x & 63) >> 5;
     const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
