@@ -200,7 +200,9 @@ template <int DT, int D, int F> struct TileKV {
     typedef typename rows::Op<DT>::F Q;    // the queries' operand
     typedef rows::PageKV<1, D> Bf16;
     typedef Place<D, F> At;
+    typedef bf16x8 V;
     static constexpr bool CODES = F == 4, TAIL = false;     // stage clears what lies behind the sequence
+    static constexpr bool EARLY = CODES && D == 64 && DT == 1;
     static constexpr int KT = Bf16::KT, TP = Bf16::TP, NG = D / GROUP, NB = 16 * F / 8;   // NB: a thread's bytes of codes
     static constexpr int KEYB = CODES ? KT * D / 2 + 256 : KT * D * 2, BYTES = KEYB + KT * D * 2;
     const char *k, *v;            // the KV head's place in page 0
@@ -208,8 +210,9 @@ template <int DT, int D, int F> struct TileKV {
     const int32_t *table;
     int len;
     int64_t pages;
-    int64_t id;                   // the page of the tile that is staged next
-    int half;                     // and the tile's place in it
+    int half;                     // the place in its page of the tile that is staged next
+    int expected;                 // the tile after it, and (in all lanes) its page's number as it lies in the table
+    uint32_t number;
     uint32_t kc[NB / 4], vc[NB / 4], ks, vs[2];   // its codes and scales
 
     __device__ __forceinline__ int64_t at(int lp) const {
@@ -229,9 +232,14 @@ template <int DT, int D, int F> struct TileKV {
             __builtin_memcpy(to, &x, sizeof x);
         }
     }
-    __device__ __forceinline__ void next(int tile) {
+    // Page numbers come a tile ahead, and by vector loads: a scalar load would be waited for
+    // with the next LDS read.
+    __device__ __forceinline__ void next(int tile, int after) {
         constexpr int HB = (int)page_bytes(D, F), CB = (int)code_bytes(D, F);
-        id = at(tile / TP);
+        const int p = __builtin_amdgcn_readfirstlane((int)number);
+        const int64_t id = tile == expected ? max((int64_t)0, min((int64_t)p, pages - 1)) : at(tile / TP);
+        expected = after;
+        number = load4(buffer((const char *)table, 0x7fffffff), after / TP * 4, 0);
         half = tile % TP;
         const int q = unit(), lane = threadIdx.x & 63, lg = lane >> 4, x = q * NB;
         const uint32_t first = half * (4 * NB) * 64 + x / 16 * 1024 + x % 16;

@@ -907,6 +907,7 @@ __device__ __forceinline__ void rows_part(const Args &a, char *smem, int x, int 
     src.k = a.kr + (int64_t)g * HEAD_BYTES<DT, D, FMT>;
     src.v = a.v + (int64_t)g * HEAD_BYTES<DT, D, FMT>;
     src.pages = a.pages;
+    if constexpr (FMT != 0) src.expected = -1;   // no tile is
     const int it0 = z * a.part * TP;
     int s = 0, tile = x, first = 0, cnt = a.T, it1 = 0, ns = 0, wt0 = 0;
     if constexpr (SHARED) {   // every tile of the part, whatever the rows see of it: it can be staged at once

@@ -254,16 +254,18 @@ template <int DT, int D> struct Tile {
 // Keys and values of one KV head as strided rows.
 template <int DT, int D, int KEYS_ = KEYS<DT, D>> struct DenseKV {
     typedef typename Op<DT>::F F;
+    typedef F V;
     typedef Tile<DT, D> TL;
     static constexpr int KT = KEYS_, BYTES = 2 * KT * TL::ROWB;   // a staged tile: keys, then values
     static constexpr bool TAIL = false;               // no rows past `last` are read
+    static constexpr bool EARLY = false;              // values' operands are loaded before the logits
     static constexpr bool CODES = false;              // keys are operands of Op (else logits() takes the product)
     const char *k, *v;
     int64_t kb, vb;                                   // bytes from row to row
     int last;                                         // the last row that may be read
     uint32_t ko, vo;                                  // TL::offset of kb, vb
 
-    __device__ __forceinline__ void next(int) {}
+    __device__ __forceinline__ void next(int, int) {}
     __device__ __forceinline__ void stage(int tile, uint32_t lds) const {
         TL::template stage<KT>(k, kb, ko, tile * KT, last, lds);
         TL::template stage<KT>(v, vb, vo, tile * KT, last, lds + KT * TL::ROWB);
@@ -288,6 +290,7 @@ template <int DT, int D, int KEYS_ = KEYS<DT, D>> struct DenseKV {
 // 16 u + 8 h .. + 7, the order in which the pages hold values.
 template <int DT, int D> struct PageKV {
     typedef typename Op<DT>::F F;
+    typedef F V;
     static constexpr int KT = KEYS<DT, D>, TP = PAGE / KT;   // tiles of a page
     static constexpr int ESZ = DT == 1 ? 2 : 4, HALF = KT * D * ESZ, BYTES = 2 * HALF;
     const char *k, *v;            // the KV head's place in page 0
@@ -295,7 +298,7 @@ template <int DT, int D> struct PageKV {
     const int32_t *table;         // the sequence's pages
     int len;                      // its keys: what lies behind them in a page may be anything
     int64_t pages;                // pages there are
-    static constexpr bool TAIL = true, CODES = false;
+    static constexpr bool TAIL = true, CODES = false, EARLY = false;
     int64_t id;                   // the page of the tile that is staged next
     int half;                     // and the tile's place in it
 
@@ -305,7 +308,7 @@ template <int DT, int D> struct PageKV {
         const int p = ((uniform)(uintptr_t)table)[__builtin_amdgcn_readfirstlane(lp)];
         return p < 0 ? 0 : (p < pages ? p : pages - 1);   // never outside the cache
     }
-    __device__ __forceinline__ void next(int tile) {
+    __device__ __forceinline__ void next(int tile, int) {
         id = at(tile / TP);
         half = tile % TP;
     }
@@ -433,6 +436,8 @@ template <int DT, int D> struct RowAcc {
     float le;         // that part before the operands' rounding, of attend<.., SEP> only (else it is l)
 };
 
+// (Sources: next(tile, after) makes ready what stage(tile) then writes to LDS; `after` is the
+// tile whose turn is next.)
 // Stages the first of tiles it0 .. it1 - 1 of a list (tile it < ns: sinks, tile it;
 // else tile wt0 + it - ns): attend goes on from there.  What a kernel loads in
 // between comes while the tile does.
@@ -440,9 +445,9 @@ template <class Src>
 __device__ __forceinline__ void attend_begin(Src &src, char *smem, int it0, int it1, int ns, int wt0) {
     const auto tile = [&](int it) { return it < ns ? it : wt0 + it - ns; };
     if (it0 >= it1) return;
-    src.next(tile(it0));
+    src.next(tile(it0), tile(min(it0 + 1, it1 - 1)));
     src.stage(tile(it0), lds_offset(smem));
-    src.next(tile(min(it0 + 1, it1 - 1)));
+    src.next(tile(min(it0 + 1, it1 - 1)), tile(min(it0 + 2, it1 - 1)));
 }
 
 // One pass of the workgroup's rows over the tiles.  c: logits to log2
@@ -475,7 +480,7 @@ __device__ __forceinline__ void attend(Src &src, char *smem, const Q &q, const t
         const int cur = (it - it0) & 1, nx = it + 1;
         if (nx < it1) {
             src.stage(tile(nx), lds + (cur ^ 1) * Src::BYTES);
-            src.next(tile(min(nx + 1, it1 - 1)));
+            src.next(tile(min(nx + 1, it1 - 1)), tile(min(nx + 2, it1 - 1)));
         }
         const int j0 = tile(it) * KT;
         if constexpr (Src::TAIL) {
@@ -490,6 +495,13 @@ __device__ __forceinline__ void attend(Src &src, char *smem, const Q &q, const t
         for (int i = 0; i < (ONE ? 1 : KT / 32); ++i) {   // 32 keys at a time: fewer registers, and halves that no row sees cost nothing
             const int kt = ONE ? which : i, jh = j0 + 32 * kt;
             if (jh >= w.hi_max || (jh + 32 <= w.lo_min && jh >= w.S)) continue;
+            typename Src::V vk[Src::EARLY ? 2 : 1][NDT];   // the values' operands, early where registers are left
+            if constexpr (Src::EARLY) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int dt = 0; dt < NDT; ++dt) vk[u][dt] = src.vf(t, kt, dt, u, lane);
+            }
             f32x16 s = zero;
             if constexpr (LO) s = s + shift;
             if constexpr (Src::CODES) {
@@ -556,7 +568,10 @@ __device__ __forceinline__ void attend(Src &src, char *smem, const Q &q, const t
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int dt = 0; dt < NDT; ++dt) a.O[dt] = Op<DT>::mma(src.vf(t, kt, dt, u, lane), p[u], a.O[dt]);
+                for (int dt = 0; dt < NDT; ++dt) {
+                    if constexpr (Src::EARLY) a.O[dt] = Op<DT>::mma(vk[u][dt], p[u], a.O[dt]);
+                    else a.O[dt] = Op<DT>::mma(src.vf(t, kt, dt, u, lane), p[u], a.O[dt]);
+                }
         }
     }
     __syncthreads();
