@@ -173,6 +173,12 @@ template <int D, int N> struct Rows6 {
             }
         }
     }
+    // word w of what it holds
+    static constexpr int SCALES = (N + 3) / 4, WORDS = D / 64 * (6 * N + SCALES);
+    __device__ __forceinline__ int &word(int w) {
+        const int s = w / (6 * N + SCALES), i = w % (6 * N + SCALES);
+        return i < 6 * N ? reinterpret_cast<int *>(&q[s][i / 6])[i % 6] : qs[s][i - 6 * N];
+    }
     // element e of x[s] again
     __device__ __forceinline__ void get(int s, float (&x)[32]) const {
 #pragma unroll
@@ -200,9 +206,7 @@ template <int DT, int D, int F> struct TileKV {
     typedef typename rows::Op<DT>::F Q;    // the queries' operand
     typedef rows::PageKV<1, D> Bf16;
     typedef Place<D, F> At;
-    typedef bf16x8 V;
-    static constexpr bool CODES = F == 4, TAIL = false;     // stage clears what lies behind the sequence
-    static constexpr bool EARLY = CODES && D == 64 && DT == 1;
+    static constexpr bool CODES = F == 4;
     static constexpr int KT = Bf16::KT, TP = Bf16::TP, NG = D / GROUP, NB = 16 * F / 8;   // NB: a thread's bytes of codes
     static constexpr int KEYB = CODES ? KT * D / 2 + 256 : KT * D * 2, BYTES = KEYB + KT * D * 2;
     const char *k, *v;            // the KV head's place in page 0
@@ -214,7 +218,15 @@ template <int DT, int D, int F> struct TileKV {
     int expected;                 // the tile after it, and (in all lanes) its page's number as it lies in the table
     uint32_t number;
     uint32_t kc[NB / 4], vc[NB / 4], ks, vs[2];   // its codes and scales
+    // The tiles: of a list (place i < ns: sinks, tile i; else tile wt0 + i - ns) the places from,
+    // from + by .. last.
+    int ns, wt0, from, by, last;
 
+    __device__ __forceinline__ int tile(int it) const {
+        const int i = min(from + it * by, last);
+        return i < ns ? i : wt0 + i - ns;
+    }
+    __device__ __forceinline__ bool past(int it) const { return from + it * by > last; }
     __device__ __forceinline__ int64_t at(int lp) const {
         typedef const __attribute__((address_space(4))) int32_t *uniform;
         const int p = ((uniform)(uintptr_t)table)[__builtin_amdgcn_readfirstlane(lp)];
@@ -222,7 +234,7 @@ template <int DT, int D, int F> struct TileKV {
     }
     // The thread's 16 codes q = thread / 64 of its lane's stream in this tile: a tile of
     // 16 keys (D = 64) or half of one (128); columns 32 g .. of 32 tokens.
-    static __device__ __forceinline__ int unit() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+    static __device__ __forceinline__ int unit() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % rows::NW; }
     static __device__ __forceinline__ void get(uint32_t (&to)[NB / 4], Buffer b, uint32_t lane, uint32_t at) {
         if constexpr (F == 4) {
             const u32x2 x = load8(b, lane, at);
@@ -234,7 +246,8 @@ template <int DT, int D, int F> struct TileKV {
     }
     // Page numbers come a tile ahead, and by vector loads: a scalar load would be waited for
     // with the next LDS read.
-    __device__ __forceinline__ void next(int tile, int after) {
+    __device__ __forceinline__ void next(int it) {
+        const int tile = this->tile(it), after = this->tile(it + 1);
         constexpr int HB = (int)page_bytes(D, F), CB = (int)code_bytes(D, F);
         const int p = __builtin_amdgcn_readfirstlane((int)number);
         const int64_t id = tile == expected ? max((int64_t)0, min((int64_t)p, pages - 1)) : at(tile / TP);
@@ -253,7 +266,8 @@ template <int DT, int D, int F> struct TileKV {
         vs[0] = s[0];
         vs[1] = s[1];
     }
-    __device__ __forceinline__ void stage(int tile, uint32_t lds) {
+    __device__ __forceinline__ void stage(int it, uint32_t lds) {
+        const int tile = this->tile(it);
         typedef __attribute__((address_space(3))) u32x4 *out;
         const int q = unit(), lane = threadIdx.x & 63, l16 = lane & 15, lg = lane >> 4;
         if constexpr (CODES) {
@@ -304,13 +318,22 @@ template <int DT, int D, int F> struct TileKV {
         }
     }
     static __device__ __forceinline__ int key(int r, int hf) { return Bf16::key(r, hf); }
-    static __device__ __forceinline__ bf16x8 kf(const char *t, int kt, int ks, int lane) { return Bf16::kf(t, kt, ks, lane); }
     static __device__ __forceinline__ bf16x8 vf(const char *t, int kt, int dt, int u, int lane) {
         const int x = 32 * dt + (lane & 31);
         return rows::Op<1>::load(t + KEYB + (((x >> 4) * (KT / 32) + kt) * 64 + (x & 15) + 16 * (2 * u + (lane >> 5))) * 16);
     }
-    // c + the products of tile kt's 32 keys (in PageKV's order) with the queries
-    template <int N> static __device__ __forceinline__ f32x16 logits(const char *t, int kt, const Rows6<D, N> &q, f32x16 c, int lane) {
+    // c + the products of tile kt's 32 keys (in PageKV's order) with the queries; kept in
+    // registers from one to the other, the operands spill at D = 128
+    static __device__ __forceinline__ f32x16 logits(const char *t, int kt, const Q (&q)[D / 16], const Q *qlo, f32x16 c, int lane) {
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+            const bf16x8 kf = Bf16::kf(t, kt, ks, lane);
+            c = rows::Op<DT>::mma(kf, q[ks], c);
+            if constexpr (DT == 1) c = rows::Op<DT>::mma(kf, qlo[ks], c);
+        }
+        return c;
+    }
+    template <int N> static __device__ __forceinline__ f32x16 logits(const char *t, int kt, const Rows6<D, N> &q, const Q *, f32x16 c, int lane) {
         const int r = lane & 31, hf = lane >> 5, l16 = 8 * (r >> 4) + 4 * ((r >> 2) & 1) + (r & 3), odd = (r >> 3) & 1;
 #pragma unroll
         for (int s = 0; s < D / 64; ++s) {
@@ -343,7 +366,7 @@ template <int DT, int D, int F> struct TileKV {
         const uint32_t c = (uint8_t)p[at_code];
         return one<F>(F == 4 ? c >> (4 * odd) : c, __uint_as_float((uint32_t)(uint8_t)p[at_scale] << 23));
     }
-    template <bool LO, int N> __device__ __forceinline__ float dot(const Rows6<D, N> &q, const Q *, int j, int hf) const {
+    template <int N> __device__ __forceinline__ float dot(const Rows6<D, N> &q, const Q *, int j, int hf) const {
         const char *p = k + at(j / rows::PAGE) * page;
         const int jp = j % rows::PAGE;
         float sum = 0.0f;
@@ -360,20 +383,20 @@ template <int DT, int D, int F> struct TileKV {
         }
         return sum + rows::other_half(sum);
     }
-    template <bool LO> __device__ __forceinline__ float dot(const Q (&q)[D / 16], const Q *qlo, int j, int hf) const {
+    __device__ __forceinline__ float dot(const Q (&q)[D / 16], const Q *qlo, int j, int hf) const {
         const char *p = k + at(j / rows::PAGE) * page;
         float sum = 0.0f;
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
             float a[8], b[8];
             rows::Op<DT>::unpack(q[ks], a);
-            if constexpr (DT == 1 && LO) rows::Op<DT>::unpack(qlo[ks], b);
+            if constexpr (DT == 1) rows::Op<DT>::unpack(qlo[ks], b);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const int t = 16 * ks + 8 * hf + e, jp = j % rows::PAGE;
                 const float x = value(p, At::key(jp, t), At::key_scale(jp, t / GROUP), e & 1);
                 sum = fmaf(a[e], x, sum);
-                if constexpr (DT == 1 && LO) sum = fmaf(b[e], x, sum);
+                if constexpr (DT == 1) sum = fmaf(b[e], x, sum);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -392,6 +415,144 @@ template <int DT, int D, int F> struct TileKV {
             }
     }
 };
+
+// One pass of a group of NW waves over n of src's tiles, whose first are in registers (next(0)):
+// the queries are in log2 units, in parts.  All groups of the workgroup call it with the same n.
+// The logits count from a reference of the row's own, O and l are sums of 2^(s - m):
+// m is 0 as long as no row of the wave leaves +-BAND (fp32 and bf16 hold 2^-126 .. 2^127 with the
+// same number of bits: nothing is lost, and the products begin at 0 without a register), else
+// the largest logit when it was last set.  All the tile's logits are taken before the first
+// exponential: the next 32 keys' matrix products run beside the exponentials of these.
+constexpr float BAND = 32.0f, ABOVE = 0x1p40f;   // ABOVE: a sum over a tile's keys that sets m anew
+template <int DT, int D, class Src, class Keys>
+__device__ __forceinline__ void attend(Src &src, char *smem, const Keys &q, const typename Src::Q *qlo, int n,
+                                       const rows::Sees &w, rows::RowAcc<DT, D> &a) {
+    typedef rows::Op<DT> Op;
+    constexpr int NDT = D / 32, KT = Src::KT, SUBS = KT / 32;
+    const int lane = threadIdx.x & 63, hf = lane >> 5;
+    const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) a.O[dt] = zero;
+    a.m = -INFINITY;
+    a.l = 0.0f;
+    float shift = 0.0f;    // -m, or 0 while nothing is seen
+    bool plain = true;     // it is 0 in all lanes
+    const uint32_t lds = lds_offset(smem);
+    if (n > 0) {
+        src.stage(0, lds);
+        src.next(1);
+    }
+#pragma unroll 1
+    for (int it = 0; it < n; ++it) {
+        __syncthreads();   // this tile is staged, and the other buffer is read no more
+        const int cur = it & 1;
+        if (it + 1 < n) {
+            src.stage(it + 1, lds + (cur ^ 1) * Src::BYTES);
+            src.next(it + 2);
+        }
+        const int j0 = src.tile(it) * KT;
+        const auto blind = [&](int j) { return j >= w.hi_max || (j + KT / SUBS <= w.lo_min && j >= w.S); };
+        if (src.past(it) || (j0 >= w.hi_max || (j0 + KT <= w.lo_min && j0 >= w.S))) continue;   // nothing the wave's rows see
+        const char *t = smem + cur * Src::BYTES;
+        f32x16 s[SUBS];
+        if (plain) {
+#pragma unroll
+            for (int i = 0; i < SUBS; ++i) s[i] = src.logits(t, i, q, qlo, zero, lane);
+        } else {
+#pragma unroll
+            for (int i = 0; i < SUBS; ++i) s[i] = src.logits(t, i, q, qlo, zero + shift, lane);
+        }
+#pragma unroll
+        for (int i = 0; i < SUBS; ++i) {
+            const int jh = j0 + 32 * i;
+            if (blind(jh)) continue;
+            if (!(jh + 32 <= w.hi_min && (jh >= w.lo_max || jh + 32 <= w.S))) {
+                const uint64_t see = rows::seen_bits(w.lo, w.hi, w.S, jh) >> Src::key(0, hf);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[i][r] = rows::keep(s[i][r], see, Src::key(r, 0), -INFINITY);
+            }
+            typename Op::F p[2];
+            const auto weights = [&]() {   // as operands, and this half's sum of them
+                float sum = 0.0f;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = rows::ex2(s[i][8 * u + e]);
+                    p[u] = Op::pack(x);
+                    if constexpr (DT == 1) {
+                        sum = Op::sum(p[u], sum);
+                    } else {   // the parts have all their bits
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) sum += x[e];
+                    }
+                }
+                return sum;
+            };
+            float sum = weights();
+            if (__ballot(!(sum <= ABOVE) || a.m == -INFINITY)) {
+                float mx = s[i][0];
+#pragma unroll
+                for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[i][r]);
+                mx = fmaxf(a.m, fmaxf(mx, rows::other_half(mx)) - shift);
+                if (fabsf(mx) <= BAND) mx = 0.0f;
+                const float al = a.m == -INFINITY ? 0.0f : rows::ex2(a.m - mx);   // nothing to rescale yet
+                a.l *= al;
+#pragma unroll
+                for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) a.O[dt][r] *= al;
+                a.m = mx;
+                const float by = mx == -INFINITY ? 0.0f : -mx;   // rows that still see nothing: 2^-inf
+#pragma unroll
+                for (int k = i; k < SUBS; ++k) s[k] = s[k] + (by - shift);
+                shift = by;
+                plain = !__ballot(!(shift == 0.0f));
+                sum = weights();
+            }
+            a.l += sum;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int dt = 0; dt < NDT; ++dt) a.O[dt] = Op::mma(src.vf(t, i, dt, u, lane), p[u], a.O[dt]);
+        }
+    }
+    __syncthreads();
+}
+
+// attend, one key at a time: for rows that came out non-finite.  Each lane adds the visible
+// keys only, so nothing of a masked key reaches its row.
+template <int DT, int D, class Src, class Keys>
+__device__ __forceinline__ void attend_each(const Src &src, const Keys &q, const typename Src::Q *qlo, int n,
+                                            const rows::Sees &w, rows::RowAcc<DT, D> &a) {
+    const int hf = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) a.O[dt] = f32x16{0.0f};
+    a.m = -INFINITY;
+    a.l = 0.0f;
+#pragma unroll 1
+    for (int it = 0; it < n && !src.past(it); ++it) {
+        const int j0 = src.tile(it) * Src::KT;
+#pragma unroll 1
+        for (int j = j0; j < min(j0 + Src::KT, w.hi_max); ++j) {
+            const float s = src.dot(q, qlo, j, hf);
+            if (!(j < w.hi && (j >= w.lo || j < w.S))) continue;
+            if (s != s) {   // a NaN makes the row NaN
+                a.l = s;
+                continue;
+            }
+            const float mn = fmaxf(a.m, s), al = a.m == -INFINITY ? 0.0f : rows::ex2(a.m - mn);
+            const float p = mn == -INFINITY ? 0.0f : rows::ex2(s - mn);   // +inf: inf - inf, a NaN
+            a.l = fmaf(a.l, al, hf ? 0.0f : p);
+#pragma unroll
+            for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) a.O[dt][r] *= al;
+            a.m = mn;
+            src.add(a.O, j, p, hf);
+        }
+    }
+}
 
 }  // namespace mx
 }  // namespace hba

@@ -736,7 +736,7 @@ template <int NT> __device__ __forceinline__ Shares shares(const Args &a) {
 // pages more make no more of them than there are shares, each workgroup has one part.
 constexpr int MOST = 1024, EXTRA = 16;
 // The sums of count(i) over the sequences before each i, and over all, by a workgroup.
-template <int NT, class F> __device__ __forceinline__ int sums_before(int Bd, int (&before)[MOST + 1], const F &count) {
+template <int NT, class F> __device__ __forceinline__ int sums_before(int Bd, int *before, const F &count) {
     __shared__ int wsum[NT / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int sum = 0;
@@ -864,30 +864,112 @@ template <int DT, int D> __device__ __forceinline__ void zero_strays(const Args 
 // rows of one sequence's tokens over its own pages (x: tile of the ragged batch).
 // g: KV head, z: part, a run of a.part pages.
 // finish_q for Rows6: x[s] are the elements 64 s + 32 hf .. of the row; cs, sn begin at 32 hf.
+// The table's rows are loaded at once, in 16 bytes (wherever the tensor begins): an element at
+// a time, each behind a branch, they were 12 us of a workgroup of 128 rows.
 template <int D>
 __device__ __forceinline__ void finish_rows(float (&x)[D / 64][32], int hf, const float *gain, float eps, const float *cs,
                                             const float *sn, float scale) {
-    if (gain) {
-        float ss = 0.0f;
+    typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+    const auto norm = [&]() {
+        if (gain) {
+            float ss = 0.0f;
+#pragma unroll
+            for (int s = 0; s < D / 64; ++s)
+#pragma unroll
+                for (int e = 0; e < 32; ++e) ss = fmaf(x[s][e], x[s][e], ss);
+            ss += rows::other_half(ss);
+            scale *= *gain / sqrtf(fmaxf(ss / (float)D, eps));
+        }
 #pragma unroll
         for (int s = 0; s < D / 64; ++s)
 #pragma unroll
-            for (int e = 0; e < 32; ++e) ss = fmaf(x[s][e], x[s][e], ss);
-        ss += rows::other_half(ss);
-        scale *= *gain / sqrtf(fmaxf(ss / (float)D, eps));
+            for (int e = 0; e < 32; ++e) x[s][e] *= scale;
+    };
+    if (!cs) {
+        norm();
+        return;
     }
+    constexpr int M = 2048 / D;   // elements at a time: 64 registers
+    float first[2][D / 64][M];
+    const auto load = [&](int e0, float (&to)[2][D / 64][M]) {
 #pragma unroll
-    for (int e = 0; e < 32; ++e) {
-        if constexpr (D == 64) {
-            x[0][e] *= scale;
-            if (cs) {
-                const float y = rows::other_half(x[0][e]);
-                x[0][e] = x[0][e] * cs[e] + y * (hf ? sn[e] : -sn[e]);
+        for (int s = 0; s < D / 64; ++s)
+#pragma unroll
+            for (int i = 0; i < M; i += 4) {
+                *reinterpret_cast<f32x4 *>(&to[0][s][i]) = *reinterpret_cast<const f32x4u *>(cs + 64 * s + e0 + i);
+                *reinterpret_cast<f32x4 *>(&to[1][s][i]) = *reinterpret_cast<const f32x4u *>(sn + 64 * s + e0 + i);
             }
-        } else {
-            const float lo = x[0][e] * scale, hi = x[1][e] * scale;
-            x[0][e] = cs ? lo * cs[e] - hi * sn[e] : lo;
-            x[1][e] = cs ? hi * cs[64 + e] + lo * sn[64 + e] : hi;
+    };
+    const auto turn = [&](int e0, const float (&by)[2][D / 64][M]) {
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            float &lo = x[0][e0 + i];
+            if constexpr (D == 64) {
+                const float y = rows::other_half(lo);
+                lo = lo * by[0][0][i] + y * (hf ? by[1][0][i] : -by[1][0][i]);
+            } else {
+                float &hi = x[1][e0 + i];
+                const float y = lo * by[0][0][i] - hi * by[1][0][i];
+                hi = hi * by[0][1][i] + lo * by[1][1][i];
+                lo = y;
+            }
+        }
+    };
+    load(0, first);
+    norm();
+    turn(0, first);
+    if constexpr (M < 32) {
+        load(M, first);
+        turn(M, first);
+    }
+}
+
+// A row's query: operands of the product with bf16 or fp32 keys (h; fp32 ones of codes have
+// all parts there), and with 4-bit codes (q6).
+template <int DT, int D, int FMT> struct Queries {
+    typedef typename Op<OPS<DT, FMT>>::F F;
+    static constexpr int NKS = D / 16;
+    F h[FMT == 4 ? 1 : NKS], l[FMT == 4 || OPS<DT, FMT> == 2 ? 1 : NKS];
+    mx::Rows6<FMT == 4 ? D : 64, FMT != 4 ? 1 : DT == 1 ? 3 : 6> q6;
+    __device__ __forceinline__ const auto &keys() const {
+        if constexpr (FMT == 4) return q6;
+        else return h;
+    }
+    // word w of the parts that are used
+    static constexpr int HW = sizeof(h) / 4, WORDS = FMT == 4 ? decltype(q6)::WORDS : (sizeof(h) + (OPS<DT, FMT> == 2 ? 0 : sizeof(l))) / 4;
+    __device__ __forceinline__ int &word(int w) {
+        if constexpr (FMT == 4) return q6.word(w);
+        else return w < HW ? reinterpret_cast<int *>(h)[w] : reinterpret_cast<int *>(l)[w - HW];
+    }
+};
+template <int DT, int D, int FMT>
+__device__ __forceinline__ void row_queries(const Args &a, int t, int head, int pos, int s, Queries<DT, D, FMT> &to) {
+    constexpr int ESZ = DT == 1 ? 2 : 4, N = D / 16, OP = OPS<DT, FMT>;
+    const int hf = (threadIdx.x & 63) >> 5;
+    const char *q = a.q + (int64_t)t * a.qst + head * a.qsh;
+    const int64_t turn = max((int64_t)0, min((int64_t)pos, a.n_tab - 1)) * D + (FMT == 4 ? 32 * hf : 0);
+    const float *gain = a.gain ? a.gain + head : nullptr, *cs = a.cos ? a.cos + turn : nullptr;
+    const float *sn = a.sin ? a.sin + turn : nullptr, scale = a.scales[s] * LOG2E;
+    if constexpr (FMT == 4) {
+        float y[D / 64][32];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float z[8];
+            Op<DT>::unpack(Op<DT>::load(q + (64 * (i / 4) + 32 * hf + 8 * (i % 4)) * ESZ), z);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[i / 4][8 * (i % 4) + e] = z[e];
+        }
+        finish_rows<D>(y, hf, gain, a.eps, cs, sn, scale);
+        to.q6.set(y);
+    } else {
+        float y[N][8];
+#pragma unroll
+        for (int ks = 0; ks < N; ++ks) Op<DT>::unpack(Op<DT>::load(q + (16 * ks + 8 * hf) * ESZ), y[ks]);
+        finish_q<D, 16>(y, 8 * hf, gain, a.eps, cs, sn, scale);
+#pragma unroll
+        for (int ks = 0; ks < N; ++ks) {
+            if constexpr (OP == 2) to.h[ks] = Op<OP>::pack(y[ks]);
+            else split<DT>(y[ks], to.h[ks], to.l[ks]);
         }
     }
 }
@@ -907,14 +989,28 @@ __device__ __forceinline__ void rows_part(const Args &a, char *smem, int x, int 
     src.k = a.kr + (int64_t)g * HEAD_BYTES<DT, D, FMT>;
     src.v = a.v + (int64_t)g * HEAD_BYTES<DT, D, FMT>;
     src.pages = a.pages;
-    if constexpr (FMT != 0) src.expected = -1;   // no tile is
+    if constexpr (FMT != 0) {
+        src.expected = -1;   // no tile is
+        src.by = 1;
+    }
+    const auto begin = [&](int it0, int it1, int ns, int wt0) {
+        if constexpr (FMT == 0) {
+            rows::attend_begin(src, smem, it0, it1, ns, wt0);
+        } else {
+            src.ns = ns;
+            src.wt0 = wt0;
+            src.from = it0;
+            src.last = it1 - 1;
+            if (it0 < it1) src.next(0);
+        }
+    };
     const int it0 = z * a.part * TP;
     int s = 0, tile = x, first = 0, cnt = a.T, it1 = 0, ns = 0, wt0 = 0;
     if constexpr (SHARED) {   // every tile of the part, whatever the rows see of it: it can be staged at once
         src.table = a.table;
         src.len = a.shared * rows::PAGE;
         it1 = min(a.shared * TP, it0 + a.part * TP);
-        rows::attend_begin(src, smem, it0, it1, 0, 0);
+        begin(it0, it1, 0, 0);
     } else {
         const auto tiles = [&](int i) {
             int f;
@@ -982,51 +1078,30 @@ __device__ __forceinline__ void rows_part(const Args &a, char *smem, int x, int 
             }
             return;
         }
-        rows::attend_begin(src, smem, it0, it1, ns, wt0);
+        begin(it0, it1, ns, wt0);
     }
-    // the queries: operands of the product with bf16 or fp32 keys (OP 2 has all parts in
-    // qh), or with codes
-    constexpr int N6 = DT == 1 ? 3 : 6;
-    F qh[Source::CODES ? 1 : NKS], ql[Source::CODES || OP == 2 ? 1 : NKS];
-    mx::Rows6<D, N6> q6;
-    if constexpr (Source::CODES) {
-        float y[D / 64][32];
-        const char *q = a.q + (int64_t)t * a.qst + head * a.qsh;
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-            float z[8];
-            Op<DT>::unpack(Op<DT>::load(q + (64 * (i / 4) + 32 * hf + 8 * (i % 4)) * ESZ), z);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) y[i / 4][8 * (i % 4) + e] = z[e];
-        }
-        const int64_t turn = max((int64_t)0, min((int64_t)pos, a.n_tab - 1)) * D + 32 * hf;
-        finish_rows<D>(y, hf, a.gain ? a.gain + head : nullptr, a.eps, a.cos ? a.cos + turn : nullptr,
-                       a.sin ? a.sin + turn : nullptr, a.scales[sq] * LOG2E);
-        q6.set(y);
-    } else {
+    Queries<DT, D, FMT> q;
+    if constexpr (FMT == 0) {
         float y[NKS][8];
-        const char *q = a.q + (int64_t)t * a.qst + head * a.qsh;
+        const char *qp = a.q + (int64_t)t * a.qst + head * a.qsh;
 #pragma unroll
-        for (int ks = 0; ks < NKS; ++ks) Op<DT>::unpack(Op<DT>::load(q + (16 * ks + 8 * hf) * ESZ), y[ks]);
+        for (int ks = 0; ks < NKS; ++ks) Op<DT>::unpack(Op<DT>::load(qp + (16 * ks + 8 * hf) * ESZ), y[ks]);
         const int64_t turn = max((int64_t)0, min((int64_t)pos, a.n_tab - 1)) * D;
         finish_q<D, 16>(y, 8 * hf, a.gain ? a.gain + head : nullptr, a.eps, a.cos ? a.cos + turn : nullptr,
                         a.sin ? a.sin + turn : nullptr, a.scales[sq] * LOG2E);
 #pragma unroll
-        for (int ks = 0; ks < NKS; ++ks) {
-            if constexpr (OP == 2) qh[ks] = Op<OP>::pack(y[ks]);
-            else split<DT>(y[ks], qh[ks], ql[ks]);
-        }
+        for (int ks = 0; ks < NKS; ++ks) split<DT>(y[ks], q.h[ks], q.l[ks]);
+    } else {
+        row_queries(a, t, head, pos, sq, q);
     }
     rows::RowAcc<OP, D> acc;
-    const auto &keys = [&]() -> const auto & {
-        if constexpr (Source::CODES) return q6;
-        else return qh;
-    }();
-    rows::attend<OP, D, LO>(src, smem, keys, ql, 1.0f, it0, it1, ns, wt0, w, acc);
+    if constexpr (FMT == 0) rows::attend<OP, D, LO>(src, smem, q.h, q.l, 1.0f, it0, it1, ns, wt0, w, acc);
+    else mx::attend<OP, D>(src, smem, q.keys(), q.l, it1 - it0, w, acc);
     float l = acc.l + rows::other_half(acc.l);
     const bool valid = w.hi > 0;
     if (__ballot(valid && (rows::any_bad<D>(acc.O) || !rows::finite(l)))) {
-        rows::attend_each<OP, D, LO>(src, keys, ql, 1.0f, it0, it1, ns, wt0, w, acc);
+        if constexpr (FMT == 0) rows::attend_each<OP, D, LO>(src, q.h, q.l, 1.0f, it0, it1, ns, wt0, w, acc);
+        else mx::attend_each<OP, D>(src, q.keys(), q.l, it1 - it0, w, acc);
         l = acc.l + rows::other_half(acc.l);
     }
     if (!in) return;
@@ -1057,6 +1132,307 @@ __global__ __launch_bounds__(64 * rows::NW, (DT == 1 && D == 64 ? 3 : rows::WAVE
     rows_part<DT, D, FMT, SHARED>(a, smem, blockIdx.x, blockIdx.y, blockIdx.z);
 }
 
+// ---------------------------------------------------------- rows, even shares ----
+// Parts of prompts over codes.  All (128-row tile of a KV head, tile of its keys) make one
+// list; each workgroup takes an even share of it, as decode's do, whatever the
+// sequences' lengths.  SETS sets of four waves work on the same rows and take the key
+// tiles in turn, each with buffers of its own, and join in LDS: as many waves as the
+// registers leave room for, without their parts in memory.
+constexpr int TILES = 2048;    // row tiles of a KV head, at most
+template <int DT, int D, int FMT> constexpr int SETS = DT == 0 && D == 128 ? 1 : 2;
+constexpr int BEGIN = 8;   // what a row tile's beginning and end cost, in tiles of keys
+// What the tile of sequence s, of length L with cnt new tokens, sees: keys lo .. hi - 1 and sinks.
+__device__ __forceinline__ void tile_sees(const Args &a, int L, int cnt, int tile, int &lo, int &hi) {
+    const int r0 = tile * rows::RT, r1 = min(r0 + rows::RT, cnt * a.G) - 1;
+    hi = max(0, L - cnt + r1 / a.G + 1);
+    lo = a.W > 0 ? max(0, max(0, L - cnt + r0 / a.G) + 1 - a.W) : 0;
+}
+// A piece of the list, in LDS: what is needed again after its keys would spill in registers.
+struct Piece {
+    int s, tile, g, p0, p1, part;    // sequence, its row tile, KV head, key tiles p0 .. p1 - 1, part (-1: all keys)
+    int first, count, len;           // of the sequence: its first new token, their number, all keys
+    int next, at, left, head;        // where the next piece begins, and how many key tiles are left
+    int tiles, per;                  // row tiles of a KV head, key tiles of a workgroup
+};
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+// The kernel's first argument, read once more for the same reason.
+__device__ __forceinline__ const Args &again() {
+    uint64_t p = reinterpret_cast<uint64_t>(__builtin_amdgcn_kernarg_segment_ptr());
+    asm("" : "+s"(p));
+    return *(const Args *)reinterpret_cast<const __attribute__((address_space(4))) Args *>(p);
+}
+template <int DT, int D, int FMT, int SETS>
+__device__ __forceinline__ void rows_codes(const Args &a, char *smem, const Piece &job) {
+    const int s = uniform(job.s), tile = uniform(job.tile), g = uniform(job.g), p0 = uniform(job.p0), p1 = uniform(job.p1);
+    typedef typename RowSource<DT, D, FMT>::T Source;
+    constexpr int OP = OPS<DT, FMT>;
+    typedef typename Op<OP>::F F;
+    constexpr int ESZ = DT == 1 ? 2 : 4, NKS = D / 16, KT = Source::KT;
+    const int lane = threadIdx.x & 63, hf = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % rows::NW;
+    const int set = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / rows::NW;
+    const int first = uniform(job.first), cnt = uniform(job.count), L = uniform(job.len);
+    int lo, hi, ns = 0, wt0 = 0;
+    tile_sees(a, L, cnt, tile, lo, hi);
+    const int nt = hi > 0 ? rows::tile_list<KT>(lo, hi, a.W > 0 ? a.S : 0, ns, wt0) : 0;
+    Source src;
+    src.page = (int64_t)a.Hkv * HEAD_BYTES<DT, D, FMT>;
+    src.k = a.kr + (int64_t)g * HEAD_BYTES<DT, D, FMT>;
+    src.v = a.v + (int64_t)g * HEAD_BYTES<DT, D, FMT>;
+    src.pages = a.pages;
+    src.table = a.table + (int64_t)s * a.maxp;
+    src.len = L;
+    src.expected = -1;
+    src.ns = ns;
+    src.wt0 = wt0;
+    src.from = p0 + set;
+    src.by = SETS;
+    src.last = min(p1, nt) - 1;
+    const int n = nt > 0 ? (p1 - p0 + SETS - 1) / SETS : 0;
+    char *mine = smem + set * (2 * Source::BYTES);
+    if (n > 0) src.next(0);
+
+    const int nr = cnt * a.G, r = tile * rows::RT + wave * rows::RW + (lane & 31);
+    const bool in = r < nr;
+    const int t = first + min(r, nr - 1) / a.G, head = g * a.G + min(r, nr - 1) % a.G, pos = L - cnt + t - first;
+    rows::Sees w;
+    w.S = a.W > 0 ? a.S : 0;
+    w.hi = in && pos >= 0 ? pos + 1 : 0;
+    w.lo = a.W > 0 ? max(0, pos + 1 - a.W) : 0;
+    int v[4] = {w.hi ? w.lo : 0x7fffffff, w.hi ? w.lo : 0, in ? w.hi : 0x7fffffff, w.hi};
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        v[0] = min(v[0], __shfl_xor(v[0], o, 64));
+        v[1] = max(v[1], __shfl_xor(v[1], o, 64));
+        v[2] = min(v[2], __shfl_xor(v[2], o, 64));
+        v[3] = max(v[3], __shfl_xor(v[3], o, 64));
+    }
+    w.lo_min = __builtin_amdgcn_readfirstlane(v[0]);
+    w.lo_max = __builtin_amdgcn_readfirstlane(v[1]);
+    w.hi_min = __builtin_amdgcn_readfirstlane(v[2]);
+    w.hi_max = __builtin_amdgcn_readfirstlane(v[3]);
+    // Set 0 makes the queries for all.
+    Queries<DT, D, FMT> q;
+    if (set == 0) row_queries(a, t, head, pos, s, q);
+    if constexpr (SETS > 1) {
+        static_assert(q.WORDS * 1024 <= SETS * 2 * Source::BYTES, "before the tiles, in their place");
+        int *at = reinterpret_cast<int *>(smem) + (threadIdx.x & 255);
+        if (set == 0) {
+#pragma unroll
+            for (int i = 0; i < q.WORDS; ++i) at[i * 256] = q.word(i);
+        }
+        __syncthreads();
+        if (set > 0) {
+#pragma unroll
+            for (int i = 0; i < q.WORDS; ++i) q.word(i) = at[i * 256];
+        }
+        __syncthreads();
+    }
+    rows::RowAcc<OP, D> acc;
+    mx::attend<OP, D>(src, mine, q.keys(), q.l, n, w, acc);
+    float l = acc.l + rows::other_half(acc.l);
+    const bool valid = w.hi > 0;
+    if (__ballot(valid && (rows::any_bad<D>(acc.O) || !rows::finite(l)))) {
+        mx::attend_each<OP, D>(src, q.keys(), q.l, n, w, acc);
+        l = acc.l + rows::other_half(acc.l);
+    }
+    if (!valid) {
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) acc.O[dt] = f32x16{0.0f};
+        acc.m = -INFINITY;
+        l = 0.0f;
+    }
+    if constexpr (SETS > 1) {   // into set 0, 32 columns at a time
+        __shared__ float ml[SETS][rows::RT][2];
+        const int row = wave * rows::RW + (lane & 31);
+        if (hf == 0) {
+            ml[set][row][0] = acc.m;
+            ml[set][row][1] = l;
+        }
+        __syncthreads();
+        float f[SETS], top = acc.m;
+#pragma unroll
+        for (int i = 0; i < SETS; ++i) top = fmaxf(top, ml[i][row][0]);
+        l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < SETS; ++i) {
+            // a set without keys has zeros; scores that are all -inf have them too, and l 0
+            f[i] = ml[i][row][0] == -INFINITY ? 0.0f : ex2(ml[i][row][0] - top);
+            l = fmaf(ml[i][row][1], ml[i][row][0] == -INFINITY ? 1.0f : f[i], l);
+        }
+        acc.m = top;
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) {
+            f32x4 *buf = reinterpret_cast<f32x4 *>(smem) + wave * 256 + lane;
+            if (set > 0) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    buf[(set - 1) * 1024 + i * 64] =
+                        f32x4{acc.O[dt][4 * i], acc.O[dt][4 * i + 1], acc.O[dt][4 * i + 2], acc.O[dt][4 * i + 3]};
+            }
+            __syncthreads();
+            if (set == 0) {
+                acc.O[dt] = acc.O[dt] * f[0];
+#pragma unroll
+                for (int j = 1; j < SETS; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const f32x4 x = buf[(j - 1) * 1024 + i * 64] * f[j];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc.O[dt][4 * i + e] += x[e];
+                    }
+            }
+            __syncthreads();
+        }
+    }
+    if (set == 0) {
+        const Args &b = again();
+        const int part = uniform(job.part), k = wave * rows::RW + (lane & 31), cnt = uniform(job.count);
+        const int r = uniform(job.tile) * rows::RT + k;
+        if (r < cnt * b.G) {
+            if (part < 0) {
+                const int64_t row = (int64_t)(uniform(job.first) + r / b.G) * b.Hq + uniform(job.g) * b.G + r % b.G;
+                const bool valid = uniform(job.len) - cnt + r / b.G >= 0;
+                rows::store_rows<DT, D>(b.out + row * D * ESZ, acc.O, valid ? 1.0f / l : 0.0f);
+            } else {
+                const int64_t at = (int64_t)part * rows::RT + k;
+                rows::store_rows<0, D>(reinterpret_cast<char *>(b.po + at * D), acc.O, 1.0f);
+                if (hf == 0) {
+                    b.pml[2 * at] = acc.m;
+                    b.pml[2 * at + 1] = l;
+                }
+            }
+        }
+    }
+}
+// records: the number of row tiles, then from [4] on four for each (KV head, row tile of
+// `tiles`): the first part, how many (0: done), sequence, tile of the sequence.
+template <int DT, int D, int FMT>
+__global__ __launch_bounds__((256 * SETS<DT, D, FMT>)) void rows_even_kernel(const Args a, int tiles) {
+    constexpr int NS = SETS<DT, D, FMT>, NT = 256 * NS, KT = RowSource<DT, D, FMT>::T::KT;
+    extern __shared__ __align__(16) char smem[];
+    __shared__ int before[MOST + 1], upto[TILES + 1], first[MOST], count[MOST], len[MOST];
+    __shared__ Piece job;
+    const int tid = threadIdx.x, w = blockIdx.x;
+    const int nt = min(tiles, sums_before<NT>(a.Bd, before, [&](int i) {
+        len[i] = length(a, i);
+        count[i] = ragged::tokens(a.cu, i, a.T, first[i]);
+        return (count[i] * a.G + rows::RT - 1) / rows::RT;
+    }));
+    const auto sequence = [&](int tile) {   // the last one that begins at the tile or before: it has tiles
+        int lo = 0, hi = again().Bd - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (before[mid] <= tile) lo = mid;
+            else hi = mid - 1;
+        }
+        return lo;
+    };
+    const int U = sums_before<NT>(nt, upto, [&](int i) {
+        const int s = sequence(i);
+        int lo, hi, ns, wt0;
+        tile_sees(a, len[s], count[s], i - before[s], lo, hi);
+        return BEGIN + max(1, hi > 0 ? rows::tile_list<KT>(lo, hi, a.W > 0 ? a.S : 0, ns, wt0) : 0);
+    });
+    const int64_t units = (int64_t)U * a.Hkv;
+    const int per = (int)max((int64_t)(BEGIN + 2 * NS), (units + a.slots - 1) / a.slots);
+    if (w == 0 && tid == 0) a.records[0] = nt;
+    if (tid < 256)
+        for (int g = 0; g < a.Hkv; ++g) zero_strays<DT, D>(a, g, w, gridDim.x);
+    const int64_t u0 = (int64_t)w * per, u1 = min(u0 + per, units);
+    if (u0 >= units) return;
+    for (int i = tid; i < nt; i += NT) {
+        const int at = (int)(u0 % U) - upto[i];
+        if (at < 0 || at >= upto[i + 1] - upto[i]) continue;
+        job.next = i;
+        job.at = at;
+        job.left = (int)(u1 - u0);
+        job.head = (int)(u0 / U);
+        job.tiles = nt;
+        job.per = per;
+    }
+    __syncthreads();
+    for (int turn = 0; uniform(job.left) > 0; turn = 1) {
+        __syncthreads();
+        if (tid == 0) {
+            const Args &b = again();
+            const int i = job.next, n = upto[i + 1] - upto[i] - BEGIN, at = job.at, to = min(n + BEGIN, at + job.left);
+            const int p0 = max(0, at - BEGIN), p1 = max(0, to - BEGIN);   // p1 0: the next workgroup has the first keys
+            const int g = job.head, s = sequence(i), tile = i - before[s], part = 2 * (int)blockIdx.x + turn;
+            if (p0 == 0 && p1 > 0) {
+                int *r = b.records + 4 + ((int64_t)g * tiles + i) * 4;
+                r[0] = part;
+                r[1] = p1 == n ? 0 : 2 + (n - p1 - 1) / job.per;
+                r[2] = s;
+                r[3] = tile;
+            }
+            job.s = s;
+            job.tile = tile;
+            job.g = g;
+            job.first = first[s];
+            job.count = count[s];
+            job.len = len[s];
+            job.p0 = p0;
+            job.p1 = p1;
+            job.part = p0 == 0 && p1 == n ? -1 : part;
+            const bool end = p1 == n && i + 1 == job.tiles;
+            job.next = end ? 0 : i + (p1 == n);
+            job.at = p1 == n ? 0 : to;
+            job.head = g + end;
+            job.left -= to - at;
+        }
+        __syncthreads();
+        if (uniform(job.p1) == 0) break;
+        rows_codes<DT, D, FMT, NS>(a, smem, job);
+    }
+}
+// The parts of a row tile's 128 rows, as join_kernel.
+template <int DT, int D> __global__ __launch_bounds__(256) void rows_join_kernel(const Args a, int tiles) {
+    constexpr int TP = D / 4;
+    const int i = blockIdx.x, g = blockIdx.y;
+    if (i >= a.records[0]) return;
+    const int *rec = a.records + 4 + ((int64_t)g * tiles + i) * 4;
+    const int parts = rec[1], w0 = rec[0] / 2, s = rec[2], tile = rec[3];
+    if (parts == 0) return;
+    int first;
+    const int cnt = ragged::tokens(a.cu, s, a.T, first), L = length(a, s);
+    const int x = threadIdx.x % TP * 4, k = blockIdx.z * (256 / TP) + threadIdx.x / TP, r = tile * rows::RT + k;
+    if (r >= cnt * a.G) return;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.0f;
+    for (int p = 0; p < parts; p += 4) {
+        float pm[4], pl[4];
+        f32x4 px[4];
+        float mn = m;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int q = min(p + e, parts - 1);
+            const int64_t at = (int64_t)(q == 0 ? rec[0] : 2 * (w0 + q)) * rows::RT + k;
+            pm[e] = p + e < parts ? a.pml[2 * at] : -INFINITY;
+            pl[e] = p + e < parts ? a.pml[2 * at + 1] : 0.0f;
+            px[e] = *reinterpret_cast<const f32x4 *>(a.po + at * D + x);
+            mn = fmaxf(mn, pm[e]);
+        }
+        const float al = m == -INFINITY ? 0.0f : ex2(m - mn);
+        l *= al;
+        o = o * al;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (pm[e] == -INFINITY && pl[e] == 0.0f) continue;   // no keys here, or none that counts
+            const float f = ex2(pm[e] - mn);
+            l = fmaf(pl[e], f, l);
+            o = o + px[e] * f;
+        }
+        m = mn;
+    }
+    const int t = first + r / a.G;
+    const int64_t row = (int64_t)t * a.Hq + g * a.G + r % a.G;
+    const f32x4 y = L - cnt + r / a.G >= 0 ? o / l : f32x4{0.f, 0.f, 0.f, 0.f};   // it sees nothing: 0
+    char *to = a.out + (row * D + x) * (DT == 1 ? 2 : 4);
+    if constexpr (DT == 1)
+        *reinterpret_cast<uint2 *>(to) = make_uint2(pk_bf16(y[0], y[1]), pk_bf16(y[2], y[3]));
+    else
+        *reinterpret_cast<f32x4 *>(to) = y;
+}
 // The shared pages for all rows (the first nshared workgroups, which take longest)
 // and every sequence's own pages for its newest token: 64 sequences, 8192 shared
 // keys, d = 64: 14.5 us, and 5 of the join.
@@ -1175,6 +1551,7 @@ struct Plan {
     int prefix, own;              // parts over the shared pages, and over each sequence's own, at most
     int prefix_pages, own_pages;  // pages of one
     int shares;                   // even shares (0: parts), of own_pages at least
+    bool even_rows;               // shares of row tiles' lists of keys
     int64_t tiles, ptiles;        // 128-row tiles: of the ragged batch (at most), of all tokens
     int slots() const { return prefix + own; }
 };
@@ -1209,6 +1586,11 @@ static Plan plan(int64_t T, int64_t Bd, int64_t Hq, int64_t Hkv, int64_t W, int6
         p.tiles = p.ptiles + Bd;
         // 4 sequences, 1560 tokens, 9000 keys, d = 64: 72 us at 1024 workgroups, 110 at 512, 77 at 1536
         p.own = parts_of(pages, p.ptiles * Hkv, 1024, 8, p.own_pages);
+        if (codes && !shared && Bd <= MOST && p.tiles <= TILES && p.tiles * pages < (1 << 28)) {
+            const int64_t shares = p.tiles * Hkv * pages / 2 + 1;   // of 4 tiles of 32 keys at least
+            p.even_rows = true;
+            p.shares = (int)(shares < CUS ? shares : CUS);
+        }
     } else if (shared) {
         p.own = parts_of(pages, groups, 1024, 4, p.own_pages);
     } else if (pages > 32 && groups < 1024 && groups * pages < (1 << 30)) {
@@ -1231,11 +1613,15 @@ static Plan plan(int64_t T, int64_t Bd, int64_t Hq, int64_t Hkv, int64_t W, int6
     return p;
 }
 static size_t parts_bytes(const Plan &p, int64_t T, int64_t Hq, int64_t d) {
-    const int64_t parts = p.shares ? (int64_t)p.shares * 32 : p.slots() > 1 ? T * Hq * p.slots() : 0;
+    const int64_t parts = p.even_rows ? (int64_t)p.shares * 2 * rows::RT
+                          : p.shares  ? (int64_t)p.shares * 32
+                                      : (p.slots() > 1 ? T * Hq * p.slots() : 0);
     return (size_t)parts * (d + 2) * 4;
 }
 static size_t workspace(const Plan &p, int64_t T, int64_t Bd, int64_t Hq, int64_t Hkv, int64_t d, bool codes) {
-    const size_t records = codes && p.shares ? (size_t)(Bd * Hkv * ((Hq / Hkv + 15) / 16) * 8) : 0;
+    const size_t records = p.even_rows           ? (size_t)(1 + p.tiles * Hkv) * 16
+                           : codes && p.shares   ? (size_t)(Bd * Hkv * ((Hq / Hkv + 15) / 16) * 8)
+                                                 : 0;
     return parts_bytes(p, T, Hq, d) + records;
 }
 
@@ -1245,6 +1631,23 @@ template <int DT, int D, int FMT, int NS> static int launch(Args a, const Plan &
     static_assert(sizeof(DecodeLds<D>) <= 65536 && lds <= 65536, "LDS without an attribute");
     const int64_t groups = (int64_t)a.Bd * a.Hkv * ((a.G + 15) / 16);
     a.slots = p.slots();
+    if constexpr (FMT != 0) {
+        if (p.even_rows) {
+            constexpr int bytes = SETS<DT, D, FMT> * 2 * RowSource<DT, D, FMT>::T::BYTES;
+            static_assert(bytes >= (SETS<DT, D, FMT> - 1) * 16384, "the sets join in the tiles' place");
+            a.slots = p.shares;
+            if (hipFuncSetAttribute(reinterpret_cast<const void *>(rows_even_kernel<DT, D, FMT>),
+                                    hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
+                return HBA_ERR_LAUNCH;
+            hipLaunchKernelGGL((rows_even_kernel<DT, D, FMT>), dim3((unsigned)p.shares), dim3(256 * SETS<DT, D, FMT>), bytes, s,
+                               a, (int)p.tiles);
+            HBA_LAUNCH_CHECK();
+            hipLaunchKernelGGL((rows_join_kernel<DT, D>), dim3((unsigned)p.tiles, (unsigned)a.Hkv, rows::RT * D / 1024),
+                               dim3(256), 0, s, a, (int)p.tiles);
+            HBA_LAUNCH_CHECK();
+            return HBA_OK;
+        }
+    }
     if (p.shares) {
         a.slots = p.shares;
         a.part = p.own_pages;

@@ -254,18 +254,15 @@ template <int DT, int D> struct Tile {
 // Keys and values of one KV head as strided rows.
 template <int DT, int D, int KEYS_ = KEYS<DT, D>> struct DenseKV {
     typedef typename Op<DT>::F F;
-    typedef F V;
     typedef Tile<DT, D> TL;
     static constexpr int KT = KEYS_, BYTES = 2 * KT * TL::ROWB;   // a staged tile: keys, then values
     static constexpr bool TAIL = false;               // no rows past `last` are read
-    static constexpr bool EARLY = false;              // values' operands are loaded before the logits
-    static constexpr bool CODES = false;              // keys are operands of Op (else logits() takes the product)
     const char *k, *v;
     int64_t kb, vb;                                   // bytes from row to row
     int last;                                         // the last row that may be read
     uint32_t ko, vo;                                  // TL::offset of kb, vb
 
-    __device__ __forceinline__ void next(int, int) {}
+    __device__ __forceinline__ void next(int) {}
     __device__ __forceinline__ void stage(int tile, uint32_t lds) const {
         TL::template stage<KT>(k, kb, ko, tile * KT, last, lds);
         TL::template stage<KT>(v, vb, vo, tile * KT, last, lds + KT * TL::ROWB);
@@ -290,7 +287,6 @@ template <int DT, int D, int KEYS_ = KEYS<DT, D>> struct DenseKV {
 // 16 u + 8 h .. + 7, the order in which the pages hold values.
 template <int DT, int D> struct PageKV {
     typedef typename Op<DT>::F F;
-    typedef F V;
     static constexpr int KT = KEYS<DT, D>, TP = PAGE / KT;   // tiles of a page
     static constexpr int ESZ = DT == 1 ? 2 : 4, HALF = KT * D * ESZ, BYTES = 2 * HALF;
     const char *k, *v;            // the KV head's place in page 0
@@ -298,7 +294,7 @@ template <int DT, int D> struct PageKV {
     const int32_t *table;         // the sequence's pages
     int len;                      // its keys: what lies behind them in a page may be anything
     int64_t pages;                // pages there are
-    static constexpr bool TAIL = true, CODES = false, EARLY = false;
+    static constexpr bool TAIL = true;
     int64_t id;                   // the page of the tile that is staged next
     int half;                     // and the tile's place in it
 
@@ -308,7 +304,7 @@ template <int DT, int D> struct PageKV {
         const int p = ((uniform)(uintptr_t)table)[__builtin_amdgcn_readfirstlane(lp)];
         return p < 0 ? 0 : (p < pages ? p : pages - 1);   // never outside the cache
     }
-    __device__ __forceinline__ void next(int tile, int) {
+    __device__ __forceinline__ void next(int tile) {
         id = at(tile / TP);
         half = tile % TP;
     }
@@ -436,8 +432,6 @@ template <int DT, int D> struct RowAcc {
     float le;         // that part before the operands' rounding, of attend<.., SEP> only (else it is l)
 };
 
-// (Sources: next(tile, after) makes ready what stage(tile) then writes to LDS; `after` is the
-// tile whose turn is next.)
 // Stages the first of tiles it0 .. it1 - 1 of a list (tile it < ns: sinks, tile it;
 // else tile wt0 + it - ns): attend goes on from there.  What a kernel loads in
 // between comes while the tile does.
@@ -445,23 +439,23 @@ template <class Src>
 __device__ __forceinline__ void attend_begin(Src &src, char *smem, int it0, int it1, int ns, int wt0) {
     const auto tile = [&](int it) { return it < ns ? it : wt0 + it - ns; };
     if (it0 >= it1) return;
-    src.next(tile(it0), tile(min(it0 + 1, it1 - 1)));
+    src.next(tile(it0));
     src.stage(tile(it0), lds_offset(smem));
-    src.next(tile(min(it0 + 1, it1 - 1)), tile(min(it0 + 2, it1 - 1)));
+    src.next(tile(min(it0 + 1, it1 - 1)));
 }
 
 // One pass of the workgroup's rows over the tiles.  c: logits to log2
-// units.  LO: the queries come in parts (DT 1: a second one in qlo) in log2 units
-// already (c = 1); their products then start from -m instead of 0.  Every wave of the workgroup calls
+// units.  LO: the queries come as two parts in log2 units already (c = 1); their
+// products then start from -m instead of 0.  Every wave of the workgroup calls
 // it; it leaves no wave reading LDS.
 // ONE: of each tile the wave takes the 32 keys `which` only (another one has the rest).
 // SEP: the sum of the probabilities as they are, too.  O is divided by the sum of the
 // rounded ones, which its own weights are; a log-sum-exp from that would put a row's
 // gradients off by up to a bf16 rounding (2^-8) in common.
-template <int DT, int D, bool LO, bool ONE = false, bool SEP = false, class Src, class Q>
-__device__ __forceinline__ void attend(Src &src, char *smem, const Q &q, const typename Op<DT>::F *qlo, float c,
-                                       int it0, int it1, int ns, int wt0, const Sees &w, RowAcc<DT, D> &a,
-                                       int which = 0) {
+template <int DT, int D, bool LO, bool ONE = false, bool SEP = false, class Src>
+__device__ __forceinline__ void attend(Src &src, char *smem, const typename Op<DT>::F (&q)[D / 16],
+                                       const typename Op<DT>::F *qlo, float c, int it0, int it1, int ns, int wt0,
+                                       const Sees &w, RowAcc<DT, D> &a, int which = 0) {
     typedef typename Op<DT>::F F;
     constexpr int NKS = D / 16, NDT = D / 32, KT = Src::KT;
     const int lane = threadIdx.x & 63, hf = lane >> 5;
@@ -480,7 +474,7 @@ __device__ __forceinline__ void attend(Src &src, char *smem, const Q &q, const t
         const int cur = (it - it0) & 1, nx = it + 1;
         if (nx < it1) {
             src.stage(tile(nx), lds + (cur ^ 1) * Src::BYTES);
-            src.next(tile(min(nx + 1, it1 - 1)), tile(min(nx + 2, it1 - 1)));
+            src.next(tile(min(nx + 1, it1 - 1)));
         }
         const int j0 = tile(it) * KT;
         if constexpr (Src::TAIL) {
@@ -495,24 +489,13 @@ __device__ __forceinline__ void attend(Src &src, char *smem, const Q &q, const t
         for (int i = 0; i < (ONE ? 1 : KT / 32); ++i) {   // 32 keys at a time: fewer registers, and halves that no row sees cost nothing
             const int kt = ONE ? which : i, jh = j0 + 32 * kt;
             if (jh >= w.hi_max || (jh + 32 <= w.lo_min && jh >= w.S)) continue;
-            typename Src::V vk[Src::EARLY ? 2 : 1][NDT];   // the values' operands, early where registers are left
-            if constexpr (Src::EARLY) {
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int dt = 0; dt < NDT; ++dt) vk[u][dt] = src.vf(t, kt, dt, u, lane);
-            }
             f32x16 s = zero;
             if constexpr (LO) s = s + shift;
-            if constexpr (Src::CODES) {
-                s = src.logits(t, kt, q, s, lane);
-            } else {
 #pragma unroll
-                for (int ks = 0; ks < NKS; ++ks) {
-                    const auto kf = src.kf(t, kt, ks, lane);
-                    s = Op<DT>::mma(kf, q[ks], s);
-                    if constexpr (LO && DT == 1) s = Op<DT>::mma(kf, qlo[ks], s);
-                }
+            for (int ks = 0; ks < NKS; ++ks) {
+                const F kf = src.kf(t, kt, ks, lane);
+                s = Op<DT>::mma(kf, q[ks], s);
+                if constexpr (LO) s = Op<DT>::mma(kf, qlo[ks], s);
             }
             if (!(jh + 32 <= w.hi_min && (jh >= w.lo_max || jh + 32 <= w.S))) {
                 const uint64_t see = seen_bits(w.lo, w.hi, w.S, jh) >> Src::key(0, hf);
@@ -568,10 +551,7 @@ __device__ __forceinline__ void attend(Src &src, char *smem, const Q &q, const t
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int dt = 0; dt < NDT; ++dt) {
-                    if constexpr (Src::EARLY) a.O[dt] = Op<DT>::mma(vk[u][dt], p[u], a.O[dt]);
-                    else a.O[dt] = Op<DT>::mma(src.vf(t, kt, dt, u, lane), p[u], a.O[dt]);
-                }
+                for (int dt = 0; dt < NDT; ++dt) a.O[dt] = Op<DT>::mma(src.vf(t, kt, dt, u, lane), p[u], a.O[dt]);
         }
     }
     __syncthreads();
@@ -619,9 +599,10 @@ __device__ __forceinline__ void DenseKV<DT, D, KT>::add(f32x16 (&o)[D / 32], int
 // attend, one key at a time: for rows that came out non-finite.  Each lane adds
 // the visible keys only, so nothing of a masked key reaches its row.  It is kept
 // from loading ahead: its registers would cost the kernels that hold it waves.
-template <int DT, int D, bool LO, class Src, class Q>
-__device__ __forceinline__ void attend_each(const Src &src, const Q &q, const typename Op<DT>::F *qlo, float c, int it0,
-                                            int it1, int ns, int wt0, const Sees &w, RowAcc<DT, D> &a) {
+template <int DT, int D, bool LO, class Src>
+__device__ __forceinline__ void attend_each(const Src &src, const typename Op<DT>::F (&q)[D / 16],
+                                         const typename Op<DT>::F *qlo, float c, int it0, int it1, int ns, int wt0,
+                                         const Sees &w, RowAcc<DT, D> &a) {
     const int hf = (threadIdx.x & 63) >> 5;
     const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
