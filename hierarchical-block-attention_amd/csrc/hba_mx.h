@@ -322,33 +322,46 @@ template <int DT, int D, int F> struct TileKV {
         const int x = 32 * dt + (lane & 31);
         return rows::Op<1>::load(t + KEYB + (((x >> 4) * (KT / 32) + kt) * 64 + (x & 15) + 16 * (2 * u + (lane >> 5))) * 16);
     }
-    // c + the products of tile kt's 32 keys (in PageKV's order) with the queries; kept in
-    // registers from one to the other, the operands spill at D = 128
-    static __device__ __forceinline__ f32x16 logits(const char *t, int kt, const Q (&q)[D / 16], const Q *qlo, f32x16 c, int lane) {
+    // Operands of 32 keys (in PageKV's order), and c + their products with the queries.
+    struct Keys {
+        u32x4 k[CODES ? D / 64 : D / 16];
+        int scale[CODES ? D / 64 : 1];
+    };
+    static __device__ __forceinline__ Keys keys(const char *t, int kt, int lane) {
+        Keys r;
+        if constexpr (CODES) {
+            const int x = lane & 31, hf = lane >> 5, l16 = 8 * (x >> 4) + 4 * ((x >> 2) & 1) + (x & 3), odd = (x >> 3) & 1;
+#pragma unroll
+            for (int s = 0; s < D / 64; ++s) {
+                const int g = 2 * s + hf;
+                if constexpr (D == 64) {   // a group is the pieces' halves in two places
+                    const char *p = t + kt * 1024 + (l16 + 32 * g) * 16 + 8 * odd;
+                    const u32x2 lo = *reinterpret_cast<const u32x2 *>(p), hi = *reinterpret_cast<const u32x2 *>(p + 256);
+                    r.k[s] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3);
+                } else {
+                    r.k[s] = *reinterpret_cast<const u32x4 *>(t + (odd * 64 + l16 + 16 * g) * 16);
+                }
+                r.scale[s] = (int)(*reinterpret_cast<const uint32_t *>(t + KT * D / 2 + (l16 + 16 * g) * 4) >> (8 * odd));
+            }
+        } else {
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks) r.k[ks] = __builtin_bit_cast(u32x4, Bf16::kf(t, kt, ks, lane));
+        }
+        return r;
+    }
+    static __device__ __forceinline__ f32x16 logits(const Keys &k, int, const Q (&q)[D / 16], const Q *qlo, f32x16 c) {
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
-            const bf16x8 kf = Bf16::kf(t, kt, ks, lane);
+            const bf16x8 kf = __builtin_bit_cast(bf16x8, k.k[ks]);
             c = rows::Op<DT>::mma(kf, q[ks], c);
             if constexpr (DT == 1) c = rows::Op<DT>::mma(kf, qlo[ks], c);
         }
         return c;
     }
-    template <int N> static __device__ __forceinline__ f32x16 logits(const char *t, int kt, const Rows6<D, N> &q, const Q *, f32x16 c, int lane) {
-        const int r = lane & 31, hf = lane >> 5, l16 = 8 * (r >> 4) + 4 * ((r >> 2) & 1) + (r & 3), odd = (r >> 3) & 1;
+    template <int N> static __device__ __forceinline__ f32x16 logits(const Keys &k, int kt, const Rows6<D, N> &q, const Q *, f32x16 c) {
 #pragma unroll
-        for (int s = 0; s < D / 64; ++s) {
-            const int g = 2 * s + hf;
-            u32x4 k;
-            if constexpr (D == 64) {   // a group is the pieces' halves in two places
-                const char *p = t + kt * 1024 + (l16 + 32 * g) * 16 + 8 * odd;
-                const u32x2 lo = *reinterpret_cast<const u32x2 *>(p), hi = *reinterpret_cast<const u32x2 *>(p + 256);
-                k = __builtin_shufflevector(lo, hi, 0, 1, 2, 3);
-            } else {
-                k = *reinterpret_cast<const u32x4 *>(t + (odd * 64 + l16 + 16 * g) * 16);
-            }
-            const int ks = (int)(*reinterpret_cast<const uint32_t *>(t + KT * D / 2 + (l16 + 16 * g) * 4) >> (8 * odd));
-            c = kt == 0 ? products<0>(k, q.q[s], c, ks, q.qs[s]) : products<2>(k, q.q[s], c, ks, q.qs[s]);
-        }
+        for (int s = 0; s < D / 64; ++s)
+            c = kt == 0 ? products<0>(k.k[s], q.q[s], c, k.scale[s], q.qs[s]) : products<2>(k.k[s], q.q[s], c, k.scale[s], q.qs[s]);
         return c;
     }
     template <int KB, int N> static __device__ __forceinline__ f32x16 products(u32x4 k, const i32x8 (&q)[N], f32x16 c, int ks,
@@ -445,27 +458,38 @@ __device__ __forceinline__ void attend(Src &src, char *smem, const Keys &q, cons
 #pragma unroll 1
     for (int it = 0; it < n; ++it) {
         __syncthreads();   // this tile is staged, and the other buffer is read no more
-        const int cur = it & 1;
-        if (it + 1 < n) {
+        const int cur = it & 1, j0 = src.tile(it) * KT;
+        const char *t = smem + cur * Src::BYTES;
+        const auto blind = [&](int j, int n) { return j >= w.hi_max || (j + n <= w.lo_min && j >= w.S); };
+        const bool skip = src.past(it) || blind(j0, KT);   // nothing the wave's rows see
+        f32x16 s[SUBS];
+        if (!skip) {
+            typename Src::Keys k[SUBS];
+#pragma unroll
+            for (int i = 0; i < SUBS; ++i) k[i] = src.keys(t, i, lane);
+            if (plain) {
+#pragma unroll
+                for (int i = 0; i < SUBS; ++i) s[i] = src.logits(k[i], i, q, qlo, zero);
+            } else {
+#pragma unroll
+                for (int i = 0; i < SUBS; ++i) s[i] = src.logits(k[i], i, q, qlo, zero + shift);
+            }
+        }
+        if (it + 1 < n) {   // beside the products
             src.stage(it + 1, lds + (cur ^ 1) * Src::BYTES);
             src.next(it + 2);
         }
-        const int j0 = src.tile(it) * KT;
-        const auto blind = [&](int j) { return j >= w.hi_max || (j + KT / SUBS <= w.lo_min && j >= w.S); };
-        if (src.past(it) || (j0 >= w.hi_max || (j0 + KT <= w.lo_min && j0 >= w.S))) continue;   // nothing the wave's rows see
-        const char *t = smem + cur * Src::BYTES;
-        f32x16 s[SUBS];
-        if (plain) {
-#pragma unroll
-            for (int i = 0; i < SUBS; ++i) s[i] = src.logits(t, i, q, qlo, zero, lane);
-        } else {
-#pragma unroll
-            for (int i = 0; i < SUBS; ++i) s[i] = src.logits(t, i, q, qlo, zero + shift, lane);
-        }
+        if (skip) continue;
 #pragma unroll
         for (int i = 0; i < SUBS; ++i) {
             const int jh = j0 + 32 * i;
-            if (blind(jh)) continue;
+            if (blind(jh, 32)) continue;
+            bf16x8 vk[2][NDT];   // while the products and exponentials take their time
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int dt = 0; dt < NDT; ++dt) vk[u][dt] = src.vf(t, i, dt, u, lane);
+            __builtin_amdgcn_sched_barrier(0);
             if (!(jh + 32 <= w.hi_min && (jh >= w.lo_max || jh + 32 <= w.S))) {
                 const uint64_t see = rows::seen_bits(w.lo, w.hi, w.S, jh) >> Src::key(0, hf);
 #pragma unroll
@@ -514,7 +538,7 @@ __device__ __forceinline__ void attend(Src &src, char *smem, const Keys &q, cons
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int dt = 0; dt < NDT; ++dt) a.O[dt] = Op::mma(src.vf(t, i, dt, u, lane), p[u], a.O[dt]);
+                for (int dt = 0; dt < NDT; ++dt) a.O[dt] = Op::mma(vk[u][dt], p[u], a.O[dt]);
         }
     }
     __syncthreads();

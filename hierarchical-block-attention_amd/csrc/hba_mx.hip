@@ -12,6 +12,8 @@
 namespace hba {
 namespace mx {
 
+constexpr int HALF = 32;                // tokens of half a page, whose codes lie apart from the other half's
+
 struct AppendArgs {
     const char *k, *v;                  // [T, Hkv, D]; byte strides of token and head
     int64_t kst, ksh, vst, vsh;
@@ -29,7 +31,7 @@ struct AppendArgs {
 // page table or the rotation tables.)
 struct Span {
     int from, n, c0, first, last;
-    __device__ __forceinline__ int tiles() const { return last > first ? (last - 1) / 64 - first / 64 + 1 : 0; }
+    __device__ __forceinline__ int halves() const { return last > first ? (last - 1) / HALF - first / HALF + 1 : 0; }   // of pages
 };
 __device__ __forceinline__ Span span(const int32_t *cu, const int32_t *lens, int T, int64_t most, int s) {
     Span x;
@@ -103,7 +105,8 @@ template <int DT> __device__ __forceinline__ void four_of(float (&x)[4], const c
     }
 }
 
-// One workgroup per (page that gets tokens, KV head).  D / 8 lanes a row, each with 4
+// One workgroup per (half of a page that gets tokens, KV head): twice as many as pages, and
+// half the rows one after the other in each.  D / 8 lanes a row, each with 4
 // elements of its first half and the 4 that they are rotated with.  The norm and the
 // rotation run in 64 bits (at half a rate that nothing here needs) and are rounded to
 // 32 once: next to a border between two codes the last bit of an fp32 sum would decide
@@ -111,19 +114,19 @@ template <int DT> __device__ __forceinline__ void four_of(float (&x)[4], const c
 // Codes go to LDS in the page's order (the values' a byte each, by columns) and from
 // there in whole 16-byte pieces.  Two tokens' values share a byte (F = 4): where only
 // some of a piece's tokens are new, the others are read and put back, by the one
-// workgroup that writes this page.
+// workgroup that writes this half.
 template <int DT, int D, int F> __global__ __launch_bounds__(256) void append_kernel(const AppendArgs a) {
     typedef Place<D, F> At;
-    constexpr int TPH = D / 8, RPP = 256 / TPH, NP = 64 / RPP, ESZ = DT == 1 ? 2 : 4, NG = D / GROUP;
-    constexpr int CB = (int)code_bytes(D, F), VS = 68;
-    __shared__ __align__(16) uint8_t kcodes[CB];
+    constexpr int TPH = D / 8, RPP = 256 / TPH, NP = HALF / RPP, ESZ = DT == 1 ? 2 : 4, NG = D / GROUP;
+    constexpr int CB = (int)code_bytes(D, F), VS = HALF + 4;
+    __shared__ __align__(16) uint8_t kcodes[CB / 2];
     __shared__ __align__(16) uint8_t vcodes[D * VS];
-    __shared__ uint8_t scales[4 * D];   // as in the page: the keys', then the values'
+    __shared__ uint8_t scales[4 * D];   // as in the page, with the first half's: the keys', then the values'
     const int tid = threadIdx.x, g = blockIdx.x / 8 % a.Hkv, slot = blockIdx.x / 8 / a.Hkv * 8 + blockIdx.x % 8;
     const int64_t most = min((int64_t)a.maxp * 64, a.n_tab);
     int s, tile = 0;
     if (a.cu) {
-        s = ragged::find(slot, a.Bd, [&](int i) { return span(a.cu, a.lens, a.T, most, i).tiles(); }, tile);
+        s = ragged::find(slot, a.Bd, [&](int i) { return span(a.cu, a.lens, a.T, most, i).halves(); }, tile);
         if (s < 0) return;
     } else {
         s = slot;
@@ -131,9 +134,9 @@ template <int DT, int D, int F> __global__ __launch_bounds__(256) void append_ke
     }
     const Span x = span(a.cu, a.lens, a.T, most, s);
     if (x.last <= x.first) return;
-    const int lp = x.first / 64 + tile, p0 = lp * 64;
-    const int ja = max(x.first - p0, 0), jb = min(x.last - p0, 64);   // the page's new tokens
-    const int64_t page = a.table[(int64_t)s * a.maxp + lp];
+    const int half = x.first / HALF + tile, p0 = half * HALF, h = half % 2;
+    const int ja = max(x.first - p0, 0), jb = min(x.last - p0, HALF);   // its new tokens
+    const int64_t page = a.table[(int64_t)s * a.maxp + half / 2];
     if (page < 0 || page >= a.pages) return;                          // not a page of this cache
     char *kp = a.kp + (page * a.Hkv + g) * page_bytes(D, F), *vp = a.vp + (page * a.Hkv + g) * page_bytes(D, F);
     const int jl = tid % TPH, t0 = 4 * jl;
@@ -211,7 +214,8 @@ template <int DT, int D, int F> __global__ __launch_bounds__(256) void append_ke
         }
     }
     __syncthreads();
-    for (int c = tid; c < CB / 16; c += 256) {
+    char *kh = kp + h * (CB / 2), *vh = vp + h * (CB / 2);
+    for (int c = tid; c < CB / 32; c += 256) {
         // keys: 8 bytes are of one token
         constexpr int TB = D / 4 * F / 8;   // bytes of a lane in a tile
         const int lane = c % 64, b0 = c / 64 * 16;
@@ -219,24 +223,23 @@ template <int DT, int D, int F> __global__ __launch_bounds__(256) void append_ke
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int mt = (b0 + 8 * i) / TB, l16 = lane % 16;
-            const int j = 32 * (mt >> 1) + 8 * (l16 >> 2) + 4 * (mt & 1) + (l16 & 3);
+            const int j = 8 * (l16 >> 2) + 4 * mt + (l16 & 3);
             in[i] = j >= ja && j < jb;
         }
         const u32x4 w = *reinterpret_cast<const u32x4 *>(kcodes + 16 * c);
         if (in[0] && in[1]) {
-            *reinterpret_cast<u32x4 *>(kp + 16 * c) = w;
+            *reinterpret_cast<u32x4 *>(kh + 16 * c) = w;
         } else {
-            if (in[0]) *reinterpret_cast<u32x2 *>(kp + 16 * c) = u32x2{w[0], w[1]};
-            if (in[1]) *reinterpret_cast<u32x2 *>(kp + 16 * c + 8) = u32x2{w[2], w[3]};
+            if (in[0]) *reinterpret_cast<u32x2 *>(kh + 16 * c) = u32x2{w[0], w[1]};
+            if (in[1]) *reinterpret_cast<u32x2 *>(kh + 16 * c + 8) = u32x2{w[2], w[3]};
         }
         // values: eight tokens of 4 columns, or 2
-        constexpr int PH = D * F / 256;     // pieces of a half
-        const int h = c / 64 / PH, pc = c / 64 % PH, j0 = 32 * h + 8 * (lane / 16);
+        const int j0 = 8 * (lane / 16);
         if (j0 + 8 <= ja || j0 >= jb) continue;
         u32x4 v;
 #pragma unroll
         for (int i = 0; i < 16 / F; ++i) {
-            const uint32_t *col = reinterpret_cast<const uint32_t *>(vcodes + (16 * (16 / F * pc + i) + lane % 16) * VS + j0);
+            const uint32_t *col = reinterpret_cast<const uint32_t *>(vcodes + (16 * (16 / F * (c / 64) + i) + lane % 16) * VS + j0);
             if constexpr (F == 4) {
                 uint32_t lo = col[0], hi = col[1];
                 lo = (lo | lo >> 4) & 0x00ff00ffu;
@@ -250,20 +253,19 @@ template <int DT, int D, int F> __global__ __launch_bounds__(256) void append_ke
         if (j0 < ja || j0 + 8 > jb) {       // the other tokens' codes stay
             const int lo = max(ja - j0, 0) * F, hi = min(jb - j0, 8) * F;   // bits of the new ones
             const uint64_t m = (hi == 64 ? ~0ull : (1ull << hi) - 1) & ~((1ull << lo) - 1);
-            const u32x4 old = *reinterpret_cast<const u32x4 *>(vp + 16 * c);
+            const u32x4 old = *reinterpret_cast<const u32x4 *>(vh + 16 * c);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint32_t mi = F == 4 || i % 2 == 0 ? (uint32_t)m : (uint32_t)(m >> 32);
                 v[i] = (v[i] & mi) | (old[i] & ~mi);
             }
         }
-        *reinterpret_cast<u32x4 *>(vp + 16 * c) = v;
+        *reinterpret_cast<u32x4 *>(vh + 16 * c) = v;
     }
-    for (int c = tid; c < 2 * D; c += 256) {
-        const int mt = c % 4, l16 = c / 4 % 16;
-        const int jk = 32 * (mt >> 1) + 8 * (l16 >> 2) + 4 * (mt & 1) + (l16 & 3), jv = c / (8 * NG) * 8 + c % 8;
-        if (jk >= ja && jk < jb) kp[CB + c] = (char)scales[c];
-        if (jv >= ja && jv < jb) vp[CB + c] = (char)scales[2 * D + c];
+    for (int c = tid; c < D; c += 256) {
+        const int l = c / 2, mt = c % 2, jk = 8 * (l % 16 >> 2) + 4 * mt + (l & 3), jv = c / (8 * NG) * 8 + c % 8;
+        if (jk >= ja && jk < jb) kp[CB + l * 4 + 2 * h + mt] = (char)scales[l * 4 + mt];
+        if (jv >= ja && jv < jb) vp[CB + h * D + c] = (char)scales[2 * D + c];
     }
 }
 
@@ -285,19 +287,19 @@ template <int DT, int D, class At> __device__ __forceinline__ void zero_rows(con
     }
 }
 
-// One workgroup per (page that holds some of the tokens, KV head).  Keys, then values, go
+// One workgroup per (half of a page that holds some of the tokens, KV head).  Keys and values go
 // through LDS as rows, so that whole rows are written.  Tokens that lie in no page give
 // 0: those of a sequence are tiles behind its pages', those of no sequence (before
 // cu[0], behind cu[Bd]) are left to the workgroups that have nothing else.
 template <int DT, int D, int F> __global__ __launch_bounds__(256) void read_kernel(const ReadArgs a) {
     typedef typename St<DT>::T T;
     constexpr int ESZ = DT == 1 ? 2 : 4, NG = D / GROUP, CB = (int)code_bytes(D, F), RS = D + 16 / ESZ;
-    __shared__ __align__(16) T rows[64 * RS];
+    __shared__ __align__(16) T krows[HALF * RS], vrows[HALF * RS];
     const int tid = threadIdx.x, g = blockIdx.y;
     const int64_t most = (int64_t)a.maxp * 64;
     const auto tiles = [&](int i) {
         const Span x = span(a.cu, a.lens, a.T, most, i);
-        return x.tiles() + (x.n - (x.last - x.first) + 63) / 64;
+        return x.halves() + (x.n - (x.last - x.first) + 63) / 64;
     };
     int tile = 0, s = blockIdx.x;
     if (a.cu) {
@@ -311,10 +313,10 @@ template <int DT, int D, int F> __global__ __launch_bounds__(256) void read_kern
         }
     }
     const Span x = span(a.cu, a.lens, a.T, most, s);
-    const int np = x.tiles(), lp = x.first / 64 + tile, p0 = lp * 64;
-    const int64_t page = tile < np ? a.table[(int64_t)s * a.maxp + lp] : -1;
-    const int ja = max(x.first - p0, 0), jb = min(x.last - p0, 64);
-    const int64_t at = x.c0 + p0 - x.first;               // the place of the page's token 0
+    const int np = x.halves(), half = x.first / HALF + tile, p0 = half * HALF, h = half % 2;
+    const int64_t page = tile < np ? a.table[(int64_t)s * a.maxp + half / 2] : -1;
+    const int ja = max(x.first - p0, 0), jb = min(x.last - p0, HALF);
+    const int64_t at = x.c0 + p0 - x.first;               // the place of the half's token 0
     if (tile >= np) {
         const int front = x.c0 - x.from, have = x.last - x.first, i0 = (tile - np) * 64;
         zero_rows<DT, D>(a, g, min(64, x.n - have - i0),
@@ -326,47 +328,43 @@ template <int DT, int D, int F> __global__ __launch_bounds__(256) void read_kern
         return;
     }
     const char *kp = a.kp + (page * a.Hkv + g) * page_bytes(D, F), *vp = a.vp + (page * a.Hkv + g) * page_bytes(D, F);
-    const auto write = [&](char *out) {
-        constexpr int C = D * ESZ / 16;
-        for (int i = ja * C + tid; i < jb * C; i += 256)
-            *reinterpret_cast<uint4 *>(out + (((at + i / C) * a.Hkv + g) * D) * ESZ + i % C * 16) =
-                *reinterpret_cast<const uint4 *>(rows + i / C * RS + i % C * (16 / ESZ));
-    };
+    const char *kh = kp + h * (CB / 2), *vh = vp + h * (CB / 2);
     constexpr int TB = D / 4 * F / 8, N8 = 32 / F / 2;    // bytes of a lane in a key tile; runs of 8 codes in a piece
-    for (int c = tid; c < CB / 16; c += 256) {
-        const u32x4 w = *reinterpret_cast<const u32x4 *>(kp + 16 * c);
+    for (int c = tid; c < CB / 32; c += 256) {
         const int lane = c % 64, l16 = lane % 16, lg = lane / 16;
-        const uint32_t sc = *reinterpret_cast<const uint32_t *>(kp + CB + (l16 + 16 * (lg * (D / 4) / GROUP)) * 4);
+        const u32x4 kw = *reinterpret_cast<const u32x4 *>(kh + 16 * c), vw = *reinterpret_cast<const u32x4 *>(vh + 16 * c);
+        const uint32_t ks = *reinterpret_cast<const uint32_t *>(kp + CB + (l16 + 16 * (lg * (D / 4) / GROUP)) * 4) >> (16 * h);
+        u32x2 vs[N8];
+#pragma unroll
+        for (int r = 0; r < N8; ++r)
+            vs[r] = *reinterpret_cast<const u32x2 *>(vp + CB + ((4 * h + lg) * NG + (N8 * (c / 64) + r) / 2) * 8);
 #pragma unroll
         for (int r = 0; r < N8; ++r) {
             const int b = c / 64 * 16 + r * F, mt = b / TB, t = D / 4 * lg + b % TB * 8 / F;
-            const int j = 32 * (mt >> 1) + 8 * (l16 >> 2) + 4 * (mt & 1) + (l16 & 3);
-            const float scale = __uint_as_float((sc >> (8 * mt) & 255u) << 23);
+            const int j = 8 * (l16 >> 2) + 4 * mt + (l16 & 3);
+            const float scale = __uint_as_float((ks >> (8 * mt) & 255u) << 23);
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                St<DT>::st(rows, j * RS + t + e, one<F>(w[F == 4 ? r : 2 * r + (e >> 2)] >> (F * e % 32), scale));
+                St<DT>::st(krows, j * RS + t + e, one<F>(kw[F == 4 ? r : 2 * r + (e >> 2)] >> (F * e % 32), scale));
         }
-    }
-    __syncthreads();
-    write(a.k);
-    __syncthreads();
-    constexpr int PH = D * F / 256;
-    for (int c = tid; c < CB / 16; c += 256) {
-        const u32x4 w = *reinterpret_cast<const u32x4 *>(vp + 16 * c);
-        const int lane = c % 64, h = c / 64 / PH, pc = c / 64 % PH, j0 = 32 * h + 8 * (lane / 16);
 #pragma unroll
         for (int r = 0; r < N8; ++r) {
-            const int dt = N8 * pc + r, t = 16 * dt + lane % 16;
-            const u32x2 sc = *reinterpret_cast<const u32x2 *>(vp + CB + (j0 / 8 * NG + dt / 2) * 8);
+            const int t = 16 * (N8 * (c / 64) + r) + l16;
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                St<DT>::st(rows, (j0 + e) * RS + t,
-                           one<F>(w[F == 4 ? r : 2 * r + (e >> 2)] >> (F * e % 32),
-                                  __uint_as_float((sc[e >> 2] >> (8 * (e & 3)) & 255u) << 23)));
+                St<DT>::st(vrows, (8 * lg + e) * RS + t,
+                           one<F>(vw[F == 4 ? r : 2 * r + (e >> 2)] >> (F * e % 32),
+                                  __uint_as_float((vs[r][e >> 2] >> (8 * (e & 3)) & 255u) << 23)));
         }
     }
     __syncthreads();
-    write(a.v);
+    constexpr int C = D * ESZ / 16;
+    for (int i = ja * C + tid; i < jb * C; i += 256) {
+        const int64_t to = (((at + i / C) * a.Hkv + g) * D) * ESZ + i % C * 16;
+        const int from = i / C * RS + i % C * (16 / ESZ);
+        *reinterpret_cast<uint4 *>(a.k + to) = *reinterpret_cast<const uint4 *>(krows + from);
+        *reinterpret_cast<uint4 *>(a.v + to) = *reinterpret_cast<const uint4 *>(vrows + from);
+    }
 }
 
 static int check(int64_t T, int64_t Bd, int64_t Hkv, int64_t d, int64_t Bk, int64_t bits, int64_t max_pages,
@@ -437,8 +435,8 @@ extern "C" int hba_kv_append_mx(int dtype, const void *k, const int64_t k_stride
     a.lens = seq_lens;
     a.kp = (char *)k_pages;
     a.vp = (char *)v_pages;
-    // c tokens touch at most c and at most c / 64 + 2 pages
-    const int64_t slots = !cu || T < T / 64 + 2 * Bd ? T : T / 64 + 2 * Bd, blocks = (slots + 7) / 8 * 8 * Hkv;
+    // c tokens touch at most c and at most c / 32 + 2 halves of pages
+    const int64_t slots = !cu || T < T / mx::HALF + 2 * Bd ? T : T / mx::HALF + 2 * Bd, blocks = (slots + 7) / 8 * 8 * Hkv;
     if (!abi::launchable(blocks, 256)) return HBA_ERR_UNSUPPORTED;
 #define HBA_APPEND_MX(DT, D, F) \
     hipLaunchKernelGGL((mx::append_kernel<DT, D, F>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a)
@@ -471,9 +469,9 @@ extern "C" int hba_kv_read_mx(int dtype, const void *k_pages, const void *v_page
     a.pages = num_pages;
     a.k = (char *)k;
     a.v = (char *)v;
-    // A sequence's c tokens are at most c tiles, and at most c / 64 + 3: pages, and those in
-    // none.  One workgroup more, for tokens of no sequence.
-    const int64_t slots = !cu ? Bd : (T < T / 64 + 3 * Bd ? T : T / 64 + 3 * Bd) + 1;
+    // A sequence's c tokens are at most c tiles, and at most c / 32 + 3: halves of pages, and those
+    // in none.  One workgroup more, for tokens of no sequence.
+    const int64_t slots = !cu ? Bd : (T < T / mx::HALF + 3 * Bd ? T : T / mx::HALF + 3 * Bd) + 1;
     if (!abi::launchable(slots, 256)) return HBA_ERR_UNSUPPORTED;
 #define HBA_READ_MX(DT, D, F)                                                                                      \
     hipLaunchKernelGGL((mx::read_kernel<DT, D, F>), dim3((unsigned)slots, (unsigned)Hkv), dim3(256), 0,            \

@@ -1140,7 +1140,7 @@ __global__ __launch_bounds__(64 * rows::NW, (DT == 1 && D == 64 ? 3 : rows::WAVE
 // registers leave room for, without their parts in memory.
 constexpr int TILES = 2048;    // row tiles of a KV head, at most
 template <int DT, int D, int FMT> constexpr int SETS = DT == 0 && D == 128 ? 1 : 2;
-constexpr int BEGIN = 8;   // what a row tile's beginning and end cost, in tiles of keys
+template <int KT> constexpr int BEGIN = 512 / KT;   // what a piece costs besides its keys, in tiles of keys
 // What the tile of sequence s, of length L with cnt new tokens, sees: keys lo .. hi - 1 and sinks.
 __device__ __forceinline__ void tile_sees(const Args &a, int L, int cnt, int tile, int &lo, int &hi) {
     const int r0 = tile * rows::RT, r1 = min(r0 + rows::RT, cnt * a.G) - 1;
@@ -1331,16 +1331,15 @@ __global__ __launch_bounds__((256 * SETS<DT, D, FMT>)) void rows_even_kernel(con
         const int s = sequence(i);
         int lo, hi, ns, wt0;
         tile_sees(a, len[s], count[s], i - before[s], lo, hi);
-        return BEGIN + max(1, hi > 0 ? rows::tile_list<KT>(lo, hi, a.W > 0 ? a.S : 0, ns, wt0) : 0);
+        return BEGIN<KT> + max(1, hi > 0 ? rows::tile_list<KT>(lo, hi, a.W > 0 ? a.S : 0, ns, wt0) : 0);
     });
     const int64_t units = (int64_t)U * a.Hkv;
-    const int per = (int)max((int64_t)(BEGIN + 2 * NS), (units + a.slots - 1) / a.slots);
+    const int per = (int)max((int64_t)(BEGIN<KT> + 2 * NS), (units + a.slots - 1) / a.slots);
     if (w == 0 && tid == 0) a.records[0] = nt;
-    if (tid < 256)
-        for (int g = 0; g < a.Hkv; ++g) zero_strays<DT, D>(a, g, w, gridDim.x);
     const int64_t u0 = (int64_t)w * per, u1 = min(u0 + per, units);
-    if (u0 >= units) return;
-    for (int i = tid; i < nt; i += NT) {
+    if (tid == 0) job.left = 0;
+    __syncthreads();
+    for (int i = tid; i < nt && u0 < units; i += NT) {
         const int at = (int)(u0 % U) - upto[i];
         if (at < 0 || at >= upto[i + 1] - upto[i]) continue;
         job.next = i;
@@ -1355,8 +1354,8 @@ __global__ __launch_bounds__((256 * SETS<DT, D, FMT>)) void rows_even_kernel(con
         __syncthreads();
         if (tid == 0) {
             const Args &b = again();
-            const int i = job.next, n = upto[i + 1] - upto[i] - BEGIN, at = job.at, to = min(n + BEGIN, at + job.left);
-            const int p0 = max(0, at - BEGIN), p1 = max(0, to - BEGIN);   // p1 0: the next workgroup has the first keys
+            const int i = job.next, n = upto[i + 1] - upto[i] - BEGIN<KT>, at = job.at, to = min(n + BEGIN<KT>, at + job.left);
+            const int p0 = max(0, at - BEGIN<KT>), p1 = max(0, to - BEGIN<KT>);   // p1 0: the next workgroup has the first keys
             const int g = job.head, s = sequence(i), tile = i - before[s], part = 2 * (int)blockIdx.x + turn;
             if (p0 == 0 && p1 > 0) {
                 int *r = b.records + 4 + ((int64_t)g * tiles + i) * 4;
@@ -1384,6 +1383,8 @@ __global__ __launch_bounds__((256 * SETS<DT, D, FMT>)) void rows_even_kernel(con
         if (uniform(job.p1) == 0) break;
         rows_codes<DT, D, FMT, NS>(a, smem, job);
     }
+    if (tid < 256)
+        for (int g = 0; g < again().Hkv; ++g) zero_strays<DT, D>(again(), g, blockIdx.x, gridDim.x);
 }
 // The parts of a row tile's 128 rows, as join_kernel.
 template <int DT, int D> __global__ __launch_bounds__(256) void rows_join_kernel(const Args a, int tiles) {
