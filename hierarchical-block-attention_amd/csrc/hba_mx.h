@@ -92,6 +92,17 @@ template <int KB, int QB> __device__ __forceinline__ f32x4 product6(u32x4 k, i32
     const i32x8 a = {(int)k[0], (int)k[1], (int)k[2], (int)k[3], 0, 0, 0, 0};
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q, c, 4, 2, KB, ks, QB, qs);
 }
+// The same in fp32 (exact).
+template <int F> __device__ __forceinline__ f32x2 pair(uint32_t w, float scale, int i) {
+    if constexpr (F == 4)
+        return i == 0   ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 0)
+               : i == 1 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 1)
+               : i == 2 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 2)
+                        : __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 3);
+    else
+        return i == 0 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, scale, false)
+                      : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, scale, true);
+}
 // One code (the low F bits) as fp32, exact.
 template <int F> __device__ __forceinline__ float one(uint32_t code, float scale) {
     f32x2 r;

@@ -12,7 +12,7 @@
 namespace hba {
 namespace mx {
 
-constexpr int HALF = 32;                // tokens of half a page, whose codes lie apart from the other half's
+constexpr int HALF = 32;                // (2^5) tokens of half a page, whose codes lie apart from the other half's
 
 struct AppendArgs {
     const char *k, *v;                  // [T, Hkv, D]; byte strides of token and head
@@ -31,7 +31,8 @@ struct AppendArgs {
 // page table or the rotation tables.)
 struct Span {
     int from, n, c0, first, last;
-    __device__ __forceinline__ int halves() const { return last > first ? (last - 1) / HALF - first / HALF + 1 : 0; }   // of pages
+    // Runs of 2^n tokens, each from a multiple of 2^n on, that they touch.
+    __device__ __forceinline__ int runs(int n) const { return last > first ? ((last - 1) >> n) - (first >> n) + 1 : 0; }
 };
 __device__ __forceinline__ Span span(const int32_t *cu, const int32_t *lens, int T, int64_t most, int s) {
     Span x;
@@ -79,15 +80,35 @@ template <int F> __device__ __forceinline__ uint32_t four(const float (&x)[4], i
         return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, y[2], y[3], 1.0f, true));
     }
 }
+// Of 8 lanes that all call it (16 with the last step): the value of the lane 1 away, 2 away, in
+// the other four, in the other eight, once those that share a value have been taken together.
+template <int STEP> __device__ __forceinline__ uint32_t partner(uint32_t x) {
+    constexpr int CTRL = STEP == 1 ? 0xb1 : STEP == 2 ? 0x4e : STEP == 4 ? 0x141 : 0x140;
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true);
+}
+template <int STEP> __device__ __forceinline__ double partner(double x) {
+    const uint64_t b = (uint64_t)__double_as_longlong(x);
+    return __longlong_as_double((long long)((uint64_t)partner<STEP>((uint32_t)(b >> 32)) << 32 | partner<STEP>((uint32_t)b)));
+}
+// 1 / sqrt(x) to 64 bits' last place or two: each step takes an error e to 5 / 16 e^3.
+__device__ __forceinline__ double inverse_root(double x) {
+    double y = __builtin_amdgcn_rsq(x);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const double e = fma(-x * y, y, 1.0);
+        y = fma(y * e, fma(0.375, e, 0.5), y);
+    }
+    return x == (double)INFINITY ? 0.0 : y;
+}
 // The largest magnitude's bits over the 8 lanes of a group (32 elements, 4 each); a NaN's
 // are above all.
 __device__ __forceinline__ uint32_t largest(const float (&x)[4]) {
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
-    return m;
+    m = max(m, partner<1>(m));
+    m = max(m, partner<2>(m));
+    return max(m, partner<4>(m));
 }
 template <int DT> __device__ __forceinline__ void four_of(float (&x)[4], const char *p) {
     if constexpr (DT == 1) {
@@ -126,7 +147,7 @@ template <int DT, int D, int F> __global__ __launch_bounds__(256) void append_ke
     const int64_t most = min((int64_t)a.maxp * 64, a.n_tab);
     int s, tile = 0;
     if (a.cu) {
-        s = ragged::find(slot, a.Bd, [&](int i) { return span(a.cu, a.lens, a.T, most, i).halves(); }, tile);
+        s = ragged::find(slot, a.Bd, [&](int i) { return span(a.cu, a.lens, a.T, most, i).runs(5); }, tile);
         if (s < 0) return;
     } else {
         s = slot;
@@ -170,9 +191,11 @@ template <int DT, int D, int F> __global__ __launch_bounds__(256) void append_ke
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) ss = fma(z[i][e], z[i][e], ss);
-#pragma unroll
-                for (int o = 1; o < TPH; o <<= 1) ss += __shfl_xor(ss, o, 64);
-                const double f = gain / sqrt(fmax(ss * (1.0 / D), (double)a.eps));
+                ss += partner<1>(ss);
+                ss += partner<2>(ss);
+                ss += partner<4>(ss);
+                if constexpr (TPH == 16) ss += partner<8>(ss);
+                const double f = gain * inverse_root(fmax(ss * (1.0 / D), (double)a.eps));
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -275,6 +298,7 @@ struct ReadArgs {
     int T, Bd, Hkv, maxp;
     int64_t pages;
     char *k, *v;                        // [T, Hkv, D]
+    int run;                            // a workgroup's tokens are 2^run: half a page or all of it
 };
 
 // n rows of zeros, the i-th at place at(i) of the batch.
@@ -287,19 +311,86 @@ template <int DT, int D, class At> __device__ __forceinline__ void zero_rows(con
     }
 }
 
+// Half h of a page: its tokens ja .. jb - 1 to rows at + ja .. of the batch.
+template <int DT, int D, int F>
+__device__ __forceinline__ void read_half(const ReadArgs &a, const char *kp, const char *vp, int h, int g, int64_t at, int ja,
+                                          int jb, typename St<DT>::T *krows, typename St<DT>::T *vrows) {
+    constexpr int ESZ = DT == 1 ? 2 : 4, NG = D / GROUP, CB = (int)code_bytes(D, F), RS = D + 16 / ESZ;
+    constexpr int TB = D / 4 * F / 8, N8 = 32 / F / 2;    // bytes of a lane in a key tile; runs of 8 codes in a piece
+    const int tid = threadIdx.x;
+    const char *kh = kp + h * (CB / 2), *vh = vp + h * (CB / 2);
+    for (int c = tid; c < CB / 32; c += 256) {
+        const int lane = c % 64, l16 = lane % 16, lg = lane / 16;
+        const u32x4 kw = *reinterpret_cast<const u32x4 *>(kh + 16 * c), vw = *reinterpret_cast<const u32x4 *>(vh + 16 * c);
+        const uint32_t ks = *reinterpret_cast<const uint32_t *>(kp + CB + (l16 + 16 * (lg * (D / 4) / GROUP)) * 4) >> (16 * h);
+        u32x2 vs[N8];
+#pragma unroll
+        for (int r = 0; r < N8; ++r)
+            vs[r] = *reinterpret_cast<const u32x2 *>(vp + CB + ((4 * h + lg) * NG + (N8 * (c / 64) + r) / 2) * 8);
+        // keys: runs of 8 elements of a token
+#pragma unroll
+        for (int r = 0; r < N8; ++r) {
+            const int b = c / 64 * 16 + r * F, mt = b / TB, t = D / 4 * lg + b % TB * 8 / F;
+            const float scale = power(ks, mt);
+            const uint32_t w[2] = {kw[F == 4 ? r : 2 * r], kw[F == 4 ? r : 2 * r + 1]};
+            typename St<DT>::T *to = krows + (8 * (l16 >> 2) + 4 * mt + (l16 & 3)) * RS + t;
+            if constexpr (DT == 1) {
+                *reinterpret_cast<u32x4 *>(to) = __builtin_bit_cast(u32x4, eight<F>(w, scale));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const f32x2 x = pair<F>(w[i], scale, F == 4 ? 2 * i : 0), y = pair<F>(w[i], scale, F == 4 ? 2 * i + 1 : 1);
+                    *reinterpret_cast<f32x4 *>(to + 4 * i) = f32x4{x[0], x[1], y[0], y[1]};
+                }
+            }
+        }
+        // values: runs of 8 tokens of a column.  bf16 ones in twos: lanes l and l ^ 1, of two columns,
+        // have the even and the odd token of both.
+#pragma unroll
+        for (int r = 0; r < N8; ++r) {
+            const int t = 16 * (N8 * (c / 64) + r) + l16;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t w = vw[F == 4 ? r : 2 * r + (i >> 1)];
+                const int p = F == 4 ? i : i & 1;
+                const float s0 = power(vs[r][i >> 1], 2 * (i & 1)), s1 = power(vs[r][i >> 1], 2 * (i & 1) + 1);
+                if constexpr (DT == 1) {
+                    const uint32_t lo = __builtin_bit_cast(uint32_t, two<F>(w, s0, p));
+                    const uint32_t hi = __builtin_bit_cast(uint32_t, two<F>(w, s1, p));
+                    const uint32_t mine = __builtin_amdgcn_perm(hi, lo, 0x07060100), other = partner<1>(mine);
+                    const int odd = l16 & 1;
+                    *reinterpret_cast<uint32_t *>(vrows + (8 * lg + 2 * i + odd) * RS + t - odd) =
+                        __builtin_amdgcn_perm(other, mine, odd ? 0x03020706 : 0x05040100);
+                } else {
+                    vrows[(8 * lg + 2 * i) * RS + t] = pair<F>(w, s0, p)[0];
+                    vrows[(8 * lg + 2 * i + 1) * RS + t] = pair<F>(w, s1, p)[1];
+                }
+            }
+        }
+    }
+    __syncthreads();
+    constexpr int C = D * ESZ / 16;
+    for (int i = ja * C + tid; i < jb * C; i += 256) {
+        const int64_t to = (((at + i / C) * a.Hkv + g) * D) * ESZ + i % C * 16;
+        const int from = i / C * RS + i % C * (16 / ESZ);
+        *reinterpret_cast<uint4 *>(a.k + to) = *reinterpret_cast<const uint4 *>(krows + from);
+        *reinterpret_cast<uint4 *>(a.v + to) = *reinterpret_cast<const uint4 *>(vrows + from);
+    }
+}
+
 // One workgroup per (half of a page that holds some of the tokens, KV head).  Keys and values go
 // through LDS as rows, so that whole rows are written.  Tokens that lie in no page give
 // 0: those of a sequence are tiles behind its pages', those of no sequence (before
 // cu[0], behind cu[Bd]) are left to the workgroups that have nothing else.
 template <int DT, int D, int F> __global__ __launch_bounds__(256) void read_kernel(const ReadArgs a) {
     typedef typename St<DT>::T T;
-    constexpr int ESZ = DT == 1 ? 2 : 4, NG = D / GROUP, CB = (int)code_bytes(D, F), RS = D + 16 / ESZ;
+    constexpr int RS = D + (DT == 1 ? 8 : 4);
     __shared__ __align__(16) T krows[HALF * RS], vrows[HALF * RS];
-    const int tid = threadIdx.x, g = blockIdx.y;
+    const int g = blockIdx.y;
     const int64_t most = (int64_t)a.maxp * 64;
     const auto tiles = [&](int i) {
         const Span x = span(a.cu, a.lens, a.T, most, i);
-        return x.halves() + (x.n - (x.last - x.first) + 63) / 64;
+        return x.runs(a.run) + (x.n - (x.last - x.first) + 63) / 64;
     };
     int tile = 0, s = blockIdx.x;
     if (a.cu) {
@@ -313,57 +404,26 @@ template <int DT, int D, int F> __global__ __launch_bounds__(256) void read_kern
         }
     }
     const Span x = span(a.cu, a.lens, a.T, most, s);
-    const int np = x.halves(), half = x.first / HALF + tile, p0 = half * HALF, h = half % 2;
-    const int64_t page = tile < np ? a.table[(int64_t)s * a.maxp + half / 2] : -1;
-    const int ja = max(x.first - p0, 0), jb = min(x.last - p0, HALF);
-    const int64_t at = x.c0 + p0 - x.first;               // the place of the half's token 0
+    const int np = x.runs(a.run), run = (x.first >> a.run) + tile;
     if (tile >= np) {
         const int front = x.c0 - x.from, have = x.last - x.first, i0 = (tile - np) * 64;
         zero_rows<DT, D>(a, g, min(64, x.n - have - i0),
                          [&](int i) { return (int64_t)(i0 + i < front ? x.from + i0 + i : x.from + i0 + i + have); });
         return;
     }
+    const int64_t page = a.table[(int64_t)s * a.maxp + (run << a.run) / 64];
     if (page < 0 || page >= a.pages) {                    // not a page of this cache
-        zero_rows<DT, D>(a, g, jb - ja, [&](int i) { return at + ja + i; });
+        const int ja = max(x.first, run << a.run), jb = min((int64_t)x.last, ((int64_t)run + 1) << a.run);
+        zero_rows<DT, D>(a, g, jb - ja, [&](int i) { return (int64_t)x.c0 + ja + i - x.first; });
         return;
     }
     const char *kp = a.kp + (page * a.Hkv + g) * page_bytes(D, F), *vp = a.vp + (page * a.Hkv + g) * page_bytes(D, F);
-    const char *kh = kp + h * (CB / 2), *vh = vp + h * (CB / 2);
-    constexpr int TB = D / 4 * F / 8, N8 = 32 / F / 2;    // bytes of a lane in a key tile; runs of 8 codes in a piece
-    for (int c = tid; c < CB / 32; c += 256) {
-        const int lane = c % 64, l16 = lane % 16, lg = lane / 16;
-        const u32x4 kw = *reinterpret_cast<const u32x4 *>(kh + 16 * c), vw = *reinterpret_cast<const u32x4 *>(vh + 16 * c);
-        const uint32_t ks = *reinterpret_cast<const uint32_t *>(kp + CB + (l16 + 16 * (lg * (D / 4) / GROUP)) * 4) >> (16 * h);
-        u32x2 vs[N8];
-#pragma unroll
-        for (int r = 0; r < N8; ++r)
-            vs[r] = *reinterpret_cast<const u32x2 *>(vp + CB + ((4 * h + lg) * NG + (N8 * (c / 64) + r) / 2) * 8);
-#pragma unroll
-        for (int r = 0; r < N8; ++r) {
-            const int b = c / 64 * 16 + r * F, mt = b / TB, t = D / 4 * lg + b % TB * 8 / F;
-            const int j = 8 * (l16 >> 2) + 4 * mt + (l16 & 3);
-            const float scale = __uint_as_float((ks >> (8 * mt) & 255u) << 23);
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                St<DT>::st(krows, j * RS + t + e, one<F>(kw[F == 4 ? r : 2 * r + (e >> 2)] >> (F * e % 32), scale));
-        }
-#pragma unroll
-        for (int r = 0; r < N8; ++r) {
-            const int t = 16 * (N8 * (c / 64) + r) + l16;
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                St<DT>::st(vrows, (8 * lg + e) * RS + t,
-                           one<F>(vw[F == 4 ? r : 2 * r + (e >> 2)] >> (F * e % 32),
-                                  __uint_as_float((vs[r][e >> 2] >> (8 * (e & 3)) & 255u) << 23)));
-        }
-    }
-    __syncthreads();
-    constexpr int C = D * ESZ / 16;
-    for (int i = ja * C + tid; i < jb * C; i += 256) {
-        const int64_t to = (((at + i / C) * a.Hkv + g) * D) * ESZ + i % C * 16;
-        const int from = i / C * RS + i % C * (16 / ESZ);
-        *reinterpret_cast<uint4 *>(a.k + to) = *reinterpret_cast<const uint4 *>(krows + from);
-        *reinterpret_cast<uint4 *>(a.v + to) = *reinterpret_cast<const uint4 *>(vrows + from);
+    for (int i = 0; i < (1 << a.run); i += HALF) {
+        const int p0 = (run << a.run) + i, h = p0 / HALF % 2, ja = max(x.first - p0, 0), jb = min(x.last - p0, HALF);
+        if (ja >= jb) continue;
+        const int64_t at = (int64_t)x.c0 + p0 - x.first;   // the place of the half's token 0
+        __syncthreads();                                   // the rows of the other half are written
+        read_half<DT, D, F>(a, kp, vp, h, g, at, ja, jb, krows, vrows);
     }
 }
 
@@ -471,7 +531,8 @@ extern "C" int hba_kv_read_mx(int dtype, const void *k_pages, const void *v_page
     a.v = (char *)v;
     // A sequence's c tokens are at most c tiles, and at most c / 32 + 3: halves of pages, and those
     // in none.  One workgroup more, for tokens of no sequence.
-    const int64_t slots = !cu ? Bd : (T < T / mx::HALF + 3 * Bd ? T : T / mx::HALF + 3 * Bd) + 1;
+    a.run = (T >> 5) * Hkv > 2048 ? 6 : 5;
+    const int64_t tiles = (T >> a.run) + 3 * Bd, slots = !cu ? Bd : (T < tiles ? T : tiles) + 1;
     if (!abi::launchable(slots, 256)) return HBA_ERR_UNSUPPORTED;
 #define HBA_READ_MX(DT, D, F)                                                                                      \
     hipLaunchKernelGGL((mx::read_kernel<DT, D, F>), dim3((unsigned)slots, (unsigned)Hkv), dim3(256), 0,            \
