@@ -110,21 +110,27 @@ __device__ __forceinline__ uint32_t largest(const float (&x)[4]) {
     m = max(m, partner<2>(m));
     return max(m, partner<4>(m));
 }
-template <int DT> __device__ __forceinline__ void four_of(float (&x)[4], const char *p) {
-    if constexpr (DT == 1) {
-        const uint2 w = *reinterpret_cast<const uint2 *>(p);
+// Four elements as they lie in memory, and as fp32.
+template <int DT> struct Four {
+    uint2 w;
+    __device__ __forceinline__ void load(const char *p) { w = *reinterpret_cast<const uint2 *>(p); }
+    __device__ __forceinline__ void get(float (&x)[4]) const {
         x[0] = __uint_as_float(w.x << 16);
         x[1] = __uint_as_float(w.x & 0xffff0000u);
         x[2] = __uint_as_float(w.y << 16);
         x[3] = __uint_as_float(w.y & 0xffff0000u);
-    } else {
-        const float4 w = *reinterpret_cast<const float4 *>(p);
+    }
+};
+template <> struct Four<0> {
+    float4 w;
+    __device__ __forceinline__ void load(const char *p) { w = *reinterpret_cast<const float4 *>(p); }
+    __device__ __forceinline__ void get(float (&x)[4]) const {
         x[0] = w.x;
         x[1] = w.y;
         x[2] = w.z;
         x[3] = w.w;
     }
-}
+};
 
 // One workgroup per (half of a page that gets tokens, KV head): twice as many as pages, and
 // half the rows one after the other in each.  D / 8 lanes a row, each with 4
@@ -136,7 +142,7 @@ template <int DT> __device__ __forceinline__ void four_of(float (&x)[4], const c
 // there in whole 16-byte pieces.  Two tokens' values share a byte (F = 4): where only
 // some of a piece's tokens are new, the others are read and put back, by the one
 // workgroup that writes this half.
-template <int DT, int D, int F> __global__ __launch_bounds__(256) void append_kernel(const AppendArgs a) {
+template <int DT, int D, int F> __global__ __launch_bounds__(256, (DT == 0 && D == 128 ? 5 : 7)) void append_kernel(const AppendArgs a) {
     typedef Place<D, F> At;
     constexpr int TPH = D / 8, RPP = 256 / TPH, NP = HALF / RPP, ESZ = DT == 1 ? 2 : 4, NG = D / GROUP;
     constexpr int CB = (int)code_bytes(D, F), VS = HALF + 4;
@@ -162,23 +168,36 @@ template <int DT, int D, int F> __global__ __launch_bounds__(256) void append_ke
     char *kp = a.kp + (page * a.Hkv + g) * page_bytes(D, F), *vp = a.vp + (page * a.Hkv + g) * page_bytes(D, F);
     const int jl = tid % TPH, t0 = 4 * jl;
     const double gain = a.gain ? (double)a.gain[g] : 0.0;
-    float kx[NP][2][4], vx[NP][2][4];
-#pragma unroll
+#pragma unroll 1
     for (int pass = 0; pass < NP; ++pass) {
         if (pass * RPP >= jb || pass * RPP + RPP <= ja) continue;     // uniform
-        const int64_t tok = x.c0 + (p0 + min(max(pass * RPP + tid / TPH, ja), jb - 1) - x.first);
+        // (a row that is not new stands for the nearest one that is)
+        const int j = pass * RPP + tid / TPH, pos = p0 + min(max(j, ja), jb - 1);
+        const int64_t tok = x.c0 + (pos - x.first);
         const char *kr = a.k + tok * a.kst + g * a.ksh, *vr = a.v + tok * a.vst + g * a.vsh;
+        Four<DT> kx[2], vx[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            four_of<DT>(kx[pass][i], kr + (t0 + i * (D / 2)) * ESZ);
-            four_of<DT>(vx[pass][i], vr + (t0 + i * (D / 2)) * ESZ);
+            kx[i].load(kr + (t0 + i * (D / 2)) * ESZ);
+            vx[i].load(vr + (t0 + i * (D / 2)) * ESZ);
         }
-    }
+        float cs[2][4], sn[2][4];
+        if (a.cos) {
 #pragma unroll
-    for (int pass = 0; pass < NP; ++pass) {
-        if (pass * RPP >= jb || pass * RPP + RPP <= ja) continue;
-        const int j = pass * RPP + tid / TPH;
-        float(&y)[2][4] = kx[pass];
+            for (int i = 0; i < 2; ++i) {
+                Four<0> c, s;
+                c.load(reinterpret_cast<const char *>(a.cos + (int64_t)pos * D + t0 + i * (D / 2)));
+                s.load(reinterpret_cast<const char *>(a.sin + (int64_t)pos * D + t0 + i * (D / 2)));
+                c.get(cs[i]);
+                s.get(sn[i]);
+            }
+        }
+        float y[2][4], v[2][4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            kx[i].get(y[i]);
+            vx[i].get(v[i]);
+        }
         if (a.gain || a.cos) {
             double z[2][4];
 #pragma unroll
@@ -202,13 +221,6 @@ template <int DT, int D, int F> __global__ __launch_bounds__(256) void append_ke
                     for (int e = 0; e < 4; ++e) z[i][e] *= f;
             }
             if (a.cos) {
-                const int64_t pos = (int64_t)(p0 + min(max(j, ja), jb - 1)) * D;
-                float cs[2][4], sn[2][4];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    four_of<0>(cs[i], reinterpret_cast<const char *>(a.cos + pos + t0 + i * (D / 2)));
-                    four_of<0>(sn[i], reinterpret_cast<const char *>(a.sin + pos + t0 + i * (D / 2)));
-                }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const double lo = z[0][e], hi = z[1][e];
@@ -224,8 +236,8 @@ template <int DT, int D, int F> __global__ __launch_bounds__(256) void append_ke
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int t = t0 + i * (D / 2), grp = t / GROUP;
-            const int kb = scale_byte<F>(largest(y[i])), vb = scale_byte<F>(largest(vx[pass][i]));
-            const uint32_t kc = four<F>(y[i], kb), vc = four<F>(vx[pass][i], vb);
+            const int kb = scale_byte<F>(largest(y[i])), vb = scale_byte<F>(largest(v[i]));
+            const uint32_t kc = four<F>(y[i], kb), vc = four<F>(v[i], vb);
             if constexpr (F == 4) *reinterpret_cast<uint16_t *>(kcodes + At::key(j, t)) = (uint16_t)kc;
             else *reinterpret_cast<uint32_t *>(kcodes + At::key(j, t)) = kc;
 #pragma unroll
