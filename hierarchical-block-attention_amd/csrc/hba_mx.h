@@ -136,6 +136,22 @@ template <int KB, int QB> __device__ __forceinline__ f32x16 product6(u32x4 k, i3
     const i32x8 a = {(int)k[0], (int)k[1], (int)k[2], (int)k[3], 0, 0, 0, 0};
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, q, c, 4, 2, KB, ks, QB, qs);
 }
+// 32 elements as e2m3 with the scale f, and back.  The conversions write their results over
+// several cycles: these must not lie where an operand does, as the compiler places them where
+// the operand is needed no more (the scale of a query's last part, whose elements then were of
+// other scales: 0.5% off the outputs of bf16 at d = 128).  So the operands stay in use; the build
+// looks for others.
+template <bool LAST> __device__ __forceinline__ u32x6 to6(f32x16 even, f32x16 odd, float f) {
+    u32x6 r = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, f);
+    asm volatile("" : "+v"(r) : "v"(f));
+    if (LAST) asm volatile("" : "+v"(r) : "v"(even), "v"(odd));   // (else they are used again)
+    return r;
+}
+__device__ __forceinline__ f32x32 from6(u32x6 x, float f) {
+    f32x32 r = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(x, f);
+    asm volatile("" : "+v"(r) : "v"(x), "v"(f));
+    return r;
+}
 // A query's 32 elements of a group as N parts of e2m3 (6 bits), each with a power of two
 // of its own: the largest magnitude goes to (3.75, 7.5], what the rounding leaves (1/4 of
 // the first unit at most) times 2^4, of every later one times 2^5.  N parts leave at most
@@ -158,10 +174,14 @@ template <int N> __device__ __forceinline__ Query6<N> parts6(const float (&y)[32
     for (int n = 0; n < N; ++n) {
         r.scale[n] = bad ? 255 : max(n == 0 ? b : b + 1 - 5 * n, 1);
         const float f = __uint_as_float((uint32_t)(bad ? 127 : r.scale[n]) << 23);
-        r.q[n] = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(x[0], x[1], f);
-        const f32x32 back = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(r.q[n], f);
+        if (n == N - 1) {
+            r.q[n] = to6<true>(x[0], x[1], f);
+        } else {
+            r.q[n] = to6<false>(x[0], x[1], f);
+            const f32x32 back = from6(r.q[n], f);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) x[e & 1][e >> 1] -= back[e];
+            for (int e = 0; e < 32; ++e) x[e & 1][e >> 1] -= back[e];
+        }
     }
     return r;
 }
@@ -199,7 +219,7 @@ template <int D, int N> struct Rows6 {
             const u32x6 w = {(uint32_t)q[s][n][0], (uint32_t)q[s][n][1], (uint32_t)q[s][n][2],
                              (uint32_t)q[s][n][3], (uint32_t)q[s][n][4], (uint32_t)q[s][n][5]};
             const uint32_t b = (uint32_t)qs[s][n / 4] >> (8 * (n % 4)) & 255u;
-            const f32x32 y = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(w, __uint_as_float(b << 23));
+            const f32x32 y = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(w, __uint_as_float(b << 23));   // (not from6: it would spill)
 #pragma unroll
             for (int e = 0; e < 32; ++e) x[e] += y[e];
         }

@@ -427,6 +427,16 @@ def test_no_norm_no_rotation_and_sharp_logits(new, dt, bits):
     check({**s, "scales": s["scales"] * 0})
 
 
+@pytest.mark.parametrize("dt,d,bits", FORMS)
+@pytest.mark.parametrize("n", [2, 40, 200])
+@pytest.mark.parametrize("parts", [False, True])
+def test_all_parts_of_a_query_count(parts, n, dt, d, bits):
+    """Logits so large that a query without its last part is out of bounds, in the form for
+    single tokens and in that for parts of prompts."""
+    s = setup(DT[dt], d, bits, 7, 1, [n] * 16, [1] * 16 if parts else None, seed=n)
+    check({**s, "scales": s["scales"] * 16})
+
+
 def test_max_len_and_long_tables():
     s = setup(torch.bfloat16, 64, 4, 4, 2, [300, 64], maxp=9)
     check({**s, "max_len": 576})

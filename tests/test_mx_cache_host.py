@@ -8,6 +8,7 @@ import torch
 import hba_amd
 import mx64
 from hba_amd import _lib, ops
+from hba_amd.build import overlaps
 
 FAKE, OFF = 0x10000, 0x10008
 S2 = (ctypes.c_int64 * 2)(128, 64)
@@ -159,3 +160,16 @@ def test_the_selection_needs_the_other_cache():
         hba_amd.DecodeLoop(c, cfg, qkn, summ, cos, sin)
     with pytest.raises(ValueError):
         c.key_rows(0, rotated=False)
+
+
+def test_conversions_that_write_over_their_operands_are_found():
+    good = """
+\tv_cvt_scalef32_2xpk16_fp6_f32 v[66:71], v[50:65], v[34:49], v72
+\tv_cvt_scalef32_pk32_f32_fp6 v[2:33], v[66:71], v72
+\tv_cvt_scalef32_pk_bf16_fp4 v3, v3, v4 op_sel:[1,0,0]
+"""
+    assert not overlaps(good)
+    bad = ["\tv_cvt_scalef32_2xpk16_fp6_f32 v[2:7], v[50:65], v[34:49], v2",
+           "\tv_cvt_scalef32_2xpk16_fp6_f32 v[50:55], v[50:65], v[34:49], v72",
+           "\tv_cvt_scalef32_pk32_f32_fp6 v[2:33], v[28:33], v72", "\tv_cvt_scalef32_pk32_f32_fp6 v[2:33], v[66:71], v9"]
+    assert [s for _, s in overlaps(good + "\n".join(bad))] == [b.strip() for b in bad]
