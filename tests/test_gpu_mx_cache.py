@@ -437,6 +437,17 @@ def test_all_parts_of_a_query_count(parts, n, dt, d, bits):
     check({**s, "scales": s["scales"] * 16})
 
 
+@pytest.mark.parametrize("dt,bits", [("bf16", 4), ("f32", 8)])
+@pytest.mark.parametrize("W", [0, 20])
+@pytest.mark.parametrize("lens,new,Hq,Hkv", [
+    ([70 + i % 60 for i in range(1100)], [i % 3 for i in range(1100)], 2, 1),    # more sequences than are shared out
+    ([40, 700, 1], [40, 700, 1], 400, 1),                                        # more row tiles
+    ([300, 9, 0, 1500, 64], [300, 0, 0, 700, 64], 3, 3),                         # a workgroup's share crosses heads
+    ([2000], [1], 32, 2), ([65] * 200, [1] * 200, 2, 2)])                        # a row tile's keys in many shares; pieces of one tile
+def test_parts_shared_out(lens, new, Hq, Hkv, W, dt, bits):
+    check(setup(DT[dt], 64, bits, Hq, Hkv, lens, new, seed=len(lens)), W, 3 if W else 0)
+
+
 def test_max_len_and_long_tables():
     s = setup(torch.bfloat16, 64, 4, 4, 2, [300, 64], maxp=9)
     check({**s, "max_len": 576})

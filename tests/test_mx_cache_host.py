@@ -173,3 +173,30 @@ def test_conversions_that_write_over_their_operands_are_found():
            "\tv_cvt_scalef32_2xpk16_fp6_f32 v[50:55], v[50:65], v[34:49], v72",
            "\tv_cvt_scalef32_pk32_f32_fp6 v[2:33], v[28:33], v72", "\tv_cvt_scalef32_pk32_f32_fp6 v[2:33], v[66:71], v9"]
     assert [s for _, s in overlaps(good + "\n".join(bad))] == [b.strip() for b in bad]
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("Bd", [1, 3, 64, 700, 1500])
+def test_attention_workspace(Bd, d):
+    """Parts of 256 workgroups at most where the lists are shared out evenly (two of 128 rows
+    each, and 16 bytes a row tile), else of every page at most; none for short single tokens."""
+    L = _lib.lib()
+
+    def need(T, W, S, shared, single, max_len, Hq=8, Hkv=2):
+        n = ctypes.c_size_t(0)
+        st = L.hba_paged_attn_mx_workspace_bytes(T, Bd, Hq, Hkv, d, W, S, shared, single, max_len, ctypes.byref(n))
+        return st, n.value
+
+    for max_len in (1, 64, 2048, 2049, 30000, 500000):
+        for W, S in ((0, 0), (1000, 4), (4000, 100)):
+            st, one = need(Bd, W, S, 0, 1, max_len)
+            assert st == 0 and one <= 256 * 32 * (d + 2) * 4 + Bd * 2 * 8
+            if max_len <= 1920:
+                assert one == 0
+            st, many = need(5 * Bd, W, S, 0, 0, max_len)
+            tiles = -(-5 * Bd * 4 // 128) + Bd
+            even = 256 * 2 * 128 * (d + 2) * 4 + (1 + 2 * tiles) * 16
+            assert st == 0 and many <= (even if Bd <= 1024 and tiles <= 2048 else 5 * Bd * 8 * (max_len // 64 + 4) * (d + 2) * 4)
+    st, pre = need(Bd, 0, 0, 16, 1, 2000)
+    assert st == 0 and pre >= 2 * Bd * 8 * (d + 2) * 4
+    assert need(Bd, 0, 0, 0, 1, 100, Hkv=3)[0] == -1
