@@ -227,7 +227,7 @@ template <int D, int N> struct Rows6 {
 };
 
 // ------------------------------------------------------------ staged tiles --
-// Keys and values of one KV head, for rows::attend: a tile's codes are loaded into
+// Keys and values of one KV head, for attend: a tile's codes are loaded into
 // registers while the tile before it is worked on.  Values, and keys of 8 bits, become
 // the bf16 tile that rows::PageKV stages; keys of 4 bits stay codes (CODES), with their
 // scales behind them, and the queries are Rows6.  A thread has 16 codes of the keys and

@@ -1,8 +1,7 @@
 // Attention of new tokens over the paged cache (kr_pages, v_pages; or their form in 4
-// or 8 bits, hba_mx.h): the newest token
-// of each sequence (decode), several (a part of a prompt), whole or through a
-// causal window with sinks; and of a batch whose sequences share their first
-// pages, whose keys are then read once for all.
+// or 8 bits, hba_mx.h): the newest token of each sequence (decode), several (a part of
+// a prompt), whole or through a causal window with sinks; and of a batch whose
+// sequences share their first pages, whose keys are then read once for all.
 //
 // The queries come raw: QKNorm, the rotation at each token's own position and its
 // sequence's scale are applied here in fp32.  For the bf16 matrix cores the
@@ -19,6 +18,11 @@
 //                  (hba_rows.h): parts of prompts, and the shared pages for the
 //                  rows of the whole batch.
 //   join_kernel    the parts of a row, by their maxima and sums.
+//
+// Over codes, decode_codes and mx::attend take the place of the products over rows, and
+//   even_codes_kernel  shares a long decode's pages out (as even_kernel, and by whole parts
+//                      where those are even enough),
+//   rows_even_kernel   shares out the keys of all row tiles of parts of prompts.
 //
 // With shared pages, both parts of the work are one launch (shared_kernel): neither
 // fills the card alone.
@@ -179,6 +183,10 @@ __device__ __forceinline__ void finish_group(float (&x)[N], const float (&y)[N],
 // make the weights of the other half of the groups.
 // A key that is not seen has logit -infinity; its value's codes and scale are 0.  So
 // what is not finite there has no effect, at no cost.
+// Bound by memory: 24 sequences of 4000 to 32000 keys, 28 heads over 4, d = 128, 4 bits, 219 MB
+// in 52 us with the join (a copy's rate: 42), another 24 in 28; 9 of 1000 to 9000 in 8 bits, fp32,
+// 45 MB in 19 + 4.  Below some 20 MB by latency: 64 windows of 1024 in 8 bits 8.4 us, one
+// sequence of 1500 keys 8.6 (page numbers, pages, products, join in LDS, one after the other).
 template <int DT, int D, int DW, int FMT, int NS>
 __device__ __forceinline__ void decode_codes(const Args &a, int s, int g, int head, int L, int p0, int p1,
                                              f32x4 (&O)[D / 16], float &m, float &l) {
@@ -1137,10 +1145,17 @@ __global__ __launch_bounds__(64 * rows::NW, (DT == 1 && D == 64 ? 3 : rows::WAVE
 // list; each workgroup takes an even share of it, as decode's do, whatever the
 // sequences' lengths.  SETS sets of four waves work on the same rows and take the key
 // tiles in turn, each with buffers of its own, and join in LDS: as many waves as the
-// registers leave room for, without their parts in memory.
+// registers leave room for, without their parts in memory.  (1560 tokens behind 1300 to 8500
+// keys, 14 heads over 2, d = 64, 4 bits: 67 us and 5 for the join, 458 TFLOP/s, where 1024
+// workgroups of a run of keys each took 71 and 8; 650 TFLOP/s at four times the tokens.  Three
+// sets have 168 registers, too few: 96.  A window of 1024 in 8 bits, d = 128, 550 tokens: 38 and
+// 6, by runs 44 and 6.)  Of a SIMD's time vector instructions have 60%, half of it exponentials
+// and their rounding to bf16, and the matrix cores 30%; a piece's beginning and end are 10 us.
 constexpr int TILES = 2048;    // row tiles of a KV head, at most
 template <int DT, int D, int FMT> constexpr int SETS = DT == 0 && D == 128 ? 1 : 2;
-template <int KT> constexpr int BEGIN = 512 / KT;   // what a piece costs besides its keys, in tiles of keys
+// What a piece costs besides its keys, in tiles of keys (6 us, and 0.7 a tile; 10 and 0.9 at 32
+// keys a tile).  Not counted, the workgroups with most pieces took half as long again.
+template <int KT> constexpr int BEGIN = 512 / KT;
 // What the tile of sequence s, of length L with cnt new tokens, sees: keys lo .. hi - 1 and sinks.
 __device__ __forceinline__ void tile_sees(const Args &a, int L, int cnt, int tile, int &lo, int &hi) {
     const int r0 = tile * rows::RT, r1 = min(r0 + rows::RT, cnt * a.G) - 1;
@@ -1568,7 +1583,7 @@ static int parts_of(int64_t pages, int64_t base, int64_t most, int64_t least, in
     return (int)((pages + per - 1) / per);
 }
 static Plan plan(int64_t T, int64_t Bd, int64_t Hq, int64_t Hkv, int64_t W, int64_t S, int64_t shared, bool one,
-                 int64_t max_len, bool codes) {
+                 int64_t max_len, int bits) {   // of the cache's codes, or 0
     Plan p = {};
     const int64_t G = Hq / Hkv, KT = rows::PAGE;
     int64_t keys = max_len - shared * KT;
@@ -1576,7 +1591,7 @@ static Plan plan(int64_t T, int64_t Bd, int64_t Hq, int64_t Hkv, int64_t W, int6
     // A part of a prompt may span any number of windows.  (The parts cut the list of one
     // 128-row tile, which has W + 128 / G tokens and the sinks, so of a window's parts most are empty.)
     if (W > 0 && !one) keys = max_len;
-    if (codes && W > 0 && !one && W + rows::RT / G + 1 < max_len) keys = W + rows::RT / G + 1;   // that list
+    if (bits && W > 0 && !one && W + rows::RT / G + 1 < max_len) keys = W + rows::RT / G + 1;   // that list
     if (keys < 1) keys = 1;
     int64_t pages = (keys + KT - 1) / KT + 1 + (W > 0 ? (S + KT - 1) / KT : 0);
     const int64_t all = (max_len + KT - 1) / KT;
@@ -1587,7 +1602,16 @@ static Plan plan(int64_t T, int64_t Bd, int64_t Hq, int64_t Hkv, int64_t W, int6
         p.tiles = p.ptiles + Bd;
         // 4 sequences, 1560 tokens, 9000 keys, d = 64: 72 us at 1024 workgroups, 110 at 512, 77 at 1536
         p.own = parts_of(pages, p.ptiles * Hkv, 1024, 8, p.own_pages);
-        if (codes && !shared && Bd <= MOST && p.tiles <= TILES && p.tiles * pages < (1 << 28)) {
+        // Shares of codes where there are enough keys for them: a share begins and ends in 20 us, a
+        // run in 12, but those of 8-bit keys spill.  Shares and runs, bf16, 4 bits, d = 64: 1560 tokens
+        // behind 1000, 2500, 8000 keys 35, 45, 66 and 35, 49, 77 us, 4900 in 16 sequences 82 and 99,
+        // a window of 1024 in those 76 and 52; 5 tokens behind 16000 keys 25 and 18, 16 times 1 to 6
+        // behind 4000 23 and 26.  8 bits: 1560 tokens alone 26 and 30, behind 8000 keys 70 and 151; 3
+        // windows of 1024, d = 128 44 and 68 (fp32 70 and 61), 64 of 1 to 6 tokens 52 and 81.
+        // (And what LDS holds, the join's grid, sums in 32 bits.)
+        const bool enough = bits == 8 ? p.tiles * Hkv * pages >= 512 : bits == 4 && pages > 32 && p.tiles * Hkv * pages >= 2048;
+        if (enough && !shared && Bd <= MOST && p.tiles <= TILES && p.tiles * Hkv <= (1 << 19) &&
+            p.tiles * pages < (1 << 29) / Hkv) {
             const int64_t shares = p.tiles * Hkv * pages / 2 + 1;   // of 4 tiles of 32 keys at least
             p.even_rows = true;
             p.shares = (int)(shares < CUS ? shares : CUS);
@@ -1725,7 +1749,7 @@ static int setup(Args &a, Plan &p, int dtype, const void *q, const int64_t q_str
                  int64_t num_pages, const int32_t *page_table, int64_t max_pages, const int32_t *seq_lens,
                  const float *scales, const int32_t *cu, int64_t T, int64_t Bd, int64_t Hq, int64_t Hkv, int64_t d,
                  int64_t Bk, int64_t W, int64_t S, int64_t shared_pages, int64_t max_len, void *workspace,
-                 size_t ws_bytes, void *out, bool codes) {
+                 size_t ws_bytes, void *out, int bits) {
     if (int st = abi::check_dtype_dim(dtype, d)) return st;
     if (Bk != rows::PAGE) return HBA_ERR_UNSUPPORTED;
     if (int st = check(T, Bd, Hq, Hkv, d, W, S, shared_pages, cu == nullptr, max_len, max_pages)) return st;
@@ -1736,8 +1760,8 @@ static int setup(Args &a, Plan &p, int dtype, const void *q, const int64_t q_str
     if (!abi::aligned16(q) || q_strides[0] % al || q_strides[1] % al || !abi::aligned16(kr_pages) ||
         !abi::aligned16(v_pages) || !abi::aligned16(out))
         return HBA_ERR_UNSUPPORTED;
-    p = plan(T, Bd, Hq, Hkv, W, S, shared_pages, cu == nullptr, max_len, codes);
-    const size_t need = paged::workspace(p, T, Bd, Hq, Hkv, d, codes), parts = parts_bytes(p, T, Hq, d);
+    p = plan(T, Bd, Hq, Hkv, W, S, shared_pages, cu == nullptr, max_len, bits);
+    const size_t need = paged::workspace(p, T, Bd, Hq, Hkv, d, bits != 0), parts = parts_bytes(p, T, Hq, d);
     if (need && (!workspace || ws_bytes < need)) return HBA_ERR_INVALID_ARG;
     if (need && !abi::aligned16(workspace)) return HBA_ERR_UNSUPPORTED;
     a = {};

@@ -8,7 +8,7 @@ extern "C" int hba_paged_attn_workspace_bytes(int64_t T, int64_t Bd, int64_t Hq,
                                               size_t *bytes) {
     if (!bytes) return HBA_ERR_INVALID_ARG;
     if (int st = paged::check(T, Bd, Hq, Hkv, d, W, S, shared_pages, one_each, max_len, 1 << 24)) return st;
-    const paged::Plan p = paged::plan(T, Bd, Hq, Hkv, W, S, shared_pages, one_each != 0, max_len, false);
+    const paged::Plan p = paged::plan(T, Bd, Hq, Hkv, W, S, shared_pages, one_each != 0, max_len, 0);
     *bytes = paged::workspace(p, T, Bd, Hq, Hkv, d, false);
     return HBA_OK;
 }
@@ -24,7 +24,7 @@ extern "C" int hba_paged_attn(int dtype, const void *q, const int64_t q_strides[
     paged::Plan p;
     if (int st = paged::setup(a, p, dtype, q, q_strides, q_gain, eps, cos_tab, sin_tab, n_tab, kr_pages, v_pages, num_pages,
                               page_table, max_pages, seq_lens, scales, cu, T, Bd, Hq, Hkv, d, Bk, W, S, shared_pages,
-                              max_len, workspace, ws_bytes, out, false))
+                              max_len, workspace, ws_bytes, out, 0))
         return st;
     int st = HBA_OK;
 #define HBA_PAGED(DT, D) st = paged::launch<DT, D, 0, 1>(a, p, (hipStream_t)stream)

@@ -8,8 +8,12 @@ extern "C" int hba_paged_attn_mx_workspace_bytes(int64_t T, int64_t Bd, int64_t 
                                                  size_t *bytes) {
     if (!bytes) return HBA_ERR_INVALID_ARG;
     if (int st = paged::check(T, Bd, Hq, Hkv, d, W, S, shared_pages, one_each, max_len, 1 << 24)) return st;
-    const paged::Plan p = paged::plan(T, Bd, Hq, Hkv, W, S, shared_pages, one_each != 0, max_len, true);
-    *bytes = paged::workspace(p, T, Bd, Hq, Hkv, d, true);
+    *bytes = 0;
+    for (int bits = 4; bits <= 8; bits += 4) {
+        const paged::Plan p = paged::plan(T, Bd, Hq, Hkv, W, S, shared_pages, one_each != 0, max_len, bits);
+        const size_t n = paged::workspace(p, T, Bd, Hq, Hkv, d, true);
+        *bytes = n > *bytes ? n : *bytes;
+    }
     return HBA_OK;
 }
 
@@ -25,7 +29,7 @@ extern "C" int hba_paged_attn_mx(int dtype, const void *q, const int64_t q_strid
     paged::Plan p;
     if (int st = paged::setup(a, p, dtype, q, q_strides, q_gain, eps, cos_tab, sin_tab, n_tab, k_pages, v_pages, num_pages,
                               page_table, max_pages, seq_lens, scales, cu, T, Bd, Hq, Hkv, d, Bk, W, S, shared_pages,
-                              max_len, workspace, ws_bytes, out, true))
+                              max_len, workspace, ws_bytes, out, (int)bits))
         return st;
     int st = HBA_OK;
 #define HBA_PAGED_MX(DT, D)                                                             \

@@ -600,7 +600,9 @@ int hba_kv_read_mx(int dtype, const void *k_pages, const void *v_pages, int64_t 
 /*
  * hba_paged_attn over it: the same arguments (workspace: hba_paged_attn_mx_workspace_bytes),
  * the same rules.  Keys and values enter the products as they are (bf16 holds them);
- * fp32: queries and probabilities in three bf16 parts (24 bits of mantissa).  Values
+ * queries of 4-bit keys in three or four parts of 6 bits (2^-13.9 of a group's largest
+ * magnitude is lost), of 8-bit ones in two of bf16; fp32: in six and three, probabilities
+ * in three bf16 parts (24 bits of mantissa).  Values
  * behind a sequence's length may be anything.  A NaN before it has no effect on tokens
  * that do not see it (with cu as there: slow for those beside it).
  */

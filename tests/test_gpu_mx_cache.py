@@ -448,6 +448,16 @@ def test_parts_shared_out(lens, new, Hq, Hkv, W, dt, bits):
     check(setup(DT[dt], 64, bits, Hq, Hkv, lens, new, seed=len(lens)), W, 3 if W else 0)
 
 
+@pytest.mark.parametrize("dt,d,bits", FORMS)
+@pytest.mark.parametrize("W,S", [(0, 0), (2100, 3)])
+def test_parts_of_long_prompts(W, S, dt, d, bits):
+    """Keys enough for shares in 4 bits too: a tile's keys in several shares, several tiles in
+    one, shares that cross heads, sequences without tokens; and logits that need every part."""
+    s = setup(DT[dt], d, bits, 6, 3, [2200, 9, 0, 3000, 64, 2600], [300, 0, 0, 700, 64, 1], seed=d + bits)
+    check(s, W, S)
+    check({**s, "scales": s["scales"] * 16}, W, S)
+
+
 def test_max_len_and_long_tables():
     s = setup(torch.bfloat16, 64, 4, 4, 2, [300, 64], maxp=9)
     check({**s, "max_len": 576})
