@@ -499,9 +499,65 @@ def test_masked_groups_have_no_effect(which, dt, d, bits):
 
 
 @pytest.mark.parametrize("dt,d,bits", FORMS)
+@pytest.mark.parametrize("which", ["kp", "vp"])
+def test_masked_groups_in_shared_out_keys(which, dt, d, bits):
+    """The same where a tile's keys lie in several workgroups' shares: tokens before the group
+    do not see it, those from it on do."""
+    n, at = 2400, 2250
+    s = setup(DT[dt], d, bits, 32, 2, [n], [300])
+    want, bound = expect(s)
+    sc = mx64.places(d, bits, which == "kp")[2]
+    page = s[which][int(s["table"][0, at // 64])]
+    page[:, sc[at % 64, 1]] = 255
+    if which == "vp":
+        c, high, _ = mx64.places(d, bits, False)
+        for t in range(32, 64):
+            page[:, c[at % 64, t]] &= 0 if bits == 8 else 240 if not high[at % 64, t] else 15
+    got = call(s).cpu()
+    sees = torch.arange(n - 300, n) >= at
+    assert_within(got[~sees], want[~sees], bound[~sees], "out")
+    assert (got[sees][..., 32:64] if which == "vp" else got[sees]).isnan().all()
+    if which == "vp":
+        assert_within(got[sees][..., :32], want[sees][..., :32], bound[sees][..., :32], "out")
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_shared_out_keys_in_graphs_and_streams(bits):
+    """Two graphs, replayed with other queries, lengths and offsets, and both at once on two
+    streams."""
+    s = setup(torch.bfloat16, 64, bits, 32, 2, [2400, 2100, 64], [250, 40, 10])
+    a = dev(s)
+    call(a), call(a, 2100, 3)
+    torch.cuda.synchronize()
+    g1, g2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g1):
+        o1 = call(a)
+    with torch.cuda.graph(g2):
+        o2 = call(a, 2100, 3)
+    for seed in range(3):
+        a["q"].copy_(torch.randn(300, 32, 64, generator=torch.Generator().manual_seed(seed)))
+        a["lens"].copy_(torch.tensor([2400 - 70 * seed, 2100, 64 - seed]))
+        a["cu"].copy_(torch.tensor([0, 250 - seed, 290, 300 - 2 * seed]))
+        want = call(a), call(a, 2100, 3)
+        torch.cuda.synchronize()
+        streams = torch.cuda.Stream(), torch.cuda.Stream()
+        for g, stream in zip((g1, g2), streams):
+            with torch.cuda.stream(stream):
+                g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o1, want[0]) and torch.equal(o2, want[1])
+        for stream in streams:
+            with torch.cuda.stream(stream):
+                got = call(a)
+            stream.synchronize()
+            assert torch.equal(got, want[0])
+
+
+@pytest.mark.parametrize("dt,d,bits", FORMS)
 @pytest.mark.parametrize("W,S", [(0, 0), (70, 4)])
 @pytest.mark.parametrize("lens,new,shared", [([1, 40, 100, 350], None, 0), ([40, 70, 129, 350], [40, 3, 128, 1], 0),
-                                             ([135, 200], [7, 20], 128), ([135, 200, 129], None, 128)])
+                                             ([135, 200], [7, 20], 128), ([135, 200, 129], None, 128),
+                                             ([2410, 70], [1400, 60], 0)])
 def test_what_lies_behind_a_sequence_changes_no_bit(lens, new, shared, W, S, dt, d, bits):
     if shared and W:
         W, S = 0, 0
