@@ -1134,7 +1134,7 @@ __device__ __forceinline__ void rows_part(const Args &a, char *smem, int x, int 
 // 27 at the rate of a large product.  Queries of two bf16 parts double q . k (3
 // products for 2), exponentials and conversions as in the sliding-window kernel.
 template <int DT, int D, int FMT, bool SHARED>
-__global__ __launch_bounds__(64 * rows::NW, (DT == 1 && D == 64 ? 3 : rows::WAVES<DT, D>)) void rows_kernel(
+__global__ __launch_bounds__(64 * rows::NW, (DT == 1 && D == 64 && FMT != 8 ? 3 : rows::WAVES<DT, D>)) void rows_kernel(
     const Args a) {
     extern __shared__ __align__(16) char smem[];
     rows_part<DT, D, FMT, SHARED>(a, smem, blockIdx.x, blockIdx.y, blockIdx.z);
