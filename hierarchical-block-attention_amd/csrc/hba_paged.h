@@ -1583,7 +1583,7 @@ static int parts_of(int64_t pages, int64_t base, int64_t most, int64_t least, in
     return (int)((pages + per - 1) / per);
 }
 static Plan plan(int64_t T, int64_t Bd, int64_t Hq, int64_t Hkv, int64_t W, int64_t S, int64_t shared, bool one,
-                 int64_t max_len, int bits) {   // of the cache's codes, or 0
+                 int64_t max_len, int64_t d, int bits) {   // bits: of the cache's codes, or 0
     Plan p = {};
     const int64_t G = Hq / Hkv, KT = rows::PAGE;
     int64_t keys = max_len - shared * KT;
@@ -1603,13 +1603,16 @@ static Plan plan(int64_t T, int64_t Bd, int64_t Hq, int64_t Hkv, int64_t W, int6
         // 4 sequences, 1560 tokens, 9000 keys, d = 64: 72 us at 1024 workgroups, 110 at 512, 77 at 1536
         p.own = parts_of(pages, p.ptiles * Hkv, 1024, 8, p.own_pages);
         // Shares of codes where there are enough keys for them: a share begins and ends in 20 us, a
-        // run in 12, but those of 8-bit keys spill.  Shares and runs, bf16, 4 bits, d = 64: 1560 tokens
-        // behind 1000, 2500, 8000 keys 35, 45, 66 and 35, 49, 77 us, 4900 in 16 sequences 82 and 99,
-        // a window of 1024 in those 76 and 52; 5 tokens behind 16000 keys 25 and 18, 16 times 1 to 6
-        // behind 4000 23 and 26.  8 bits: 1560 tokens alone 26 and 30, behind 8000 keys 70 and 151; 3
-        // windows of 1024, d = 128 44 and 68 (fp32 70 and 61), 64 of 1 to 6 tokens 52 and 81.
+        // run in 12, but at d = 128 those of 8-bit keys spill.  Shares and runs, bf16, d = 64, 4 bits:
+        // 1560 tokens behind 1000, 2500, 8000 keys 35, 45, 66 and 35, 49, 77 us, 4900 in 16 sequences
+        // 82 and 99, a window of 1024 in those 76 and 52; 5 tokens behind 16000 keys 25 and 18, 16
+        // times 1 to 6 behind 4000 23 and 26; in 8 bits 1560 tokens alone, behind 1000 and 8000 keys
+        // 26, 35, 71 and 19, 34, 101, the windows 80 and 74, the 5 tokens 25 and 17.  d = 128, 8 bits:
+        // 5 tokens behind 16000 keys 34 and 40, 8 times 1 to 6 behind 1600 30 and 48; 3 windows of
+        // 1024 44 and 68 (fp32 70 and 61), 64 of 1 to 6 tokens 52 and 81.
         // (And what LDS holds, the join's grid, sums in 32 bits.)
-        const bool enough = bits == 8 ? p.tiles * Hkv * pages >= 512 : bits == 4 && pages > 32 && p.tiles * Hkv * pages >= 2048;
+        const int64_t all_pages = p.tiles * Hkv * pages;
+        const bool enough = bits && (bits == 8 && d == 128 ? all_pages >= 512 : pages > 32 && all_pages >= 2048);
         if (enough && !shared && Bd <= MOST && p.tiles <= TILES && p.tiles * Hkv <= (1 << 19) &&
             p.tiles * pages < (1 << 29) / Hkv) {
             const int64_t shares = p.tiles * Hkv * pages / 2 + 1;   // of 4 tiles of 32 keys at least
@@ -1760,7 +1763,7 @@ static int setup(Args &a, Plan &p, int dtype, const void *q, const int64_t q_str
     if (!abi::aligned16(q) || q_strides[0] % al || q_strides[1] % al || !abi::aligned16(kr_pages) ||
         !abi::aligned16(v_pages) || !abi::aligned16(out))
         return HBA_ERR_UNSUPPORTED;
-    p = plan(T, Bd, Hq, Hkv, W, S, shared_pages, cu == nullptr, max_len, bits);
+    p = plan(T, Bd, Hq, Hkv, W, S, shared_pages, cu == nullptr, max_len, d, bits);
     const size_t need = paged::workspace(p, T, Bd, Hq, Hkv, d, bits != 0), parts = parts_bytes(p, T, Hq, d);
     if (need && (!workspace || ws_bytes < need)) return HBA_ERR_INVALID_ARG;
     if (need && !abi::aligned16(workspace)) return HBA_ERR_UNSUPPORTED;

@@ -8,7 +8,7 @@ extern "C" int hba_paged_attn_workspace_bytes(int64_t T, int64_t Bd, int64_t Hq,
                                               size_t *bytes) {
     if (!bytes) return HBA_ERR_INVALID_ARG;
     if (int st = paged::check(T, Bd, Hq, Hkv, d, W, S, shared_pages, one_each, max_len, 1 << 24)) return st;
-    const paged::Plan p = paged::plan(T, Bd, Hq, Hkv, W, S, shared_pages, one_each != 0, max_len, 0);
+    const paged::Plan p = paged::plan(T, Bd, Hq, Hkv, W, S, shared_pages, one_each != 0, max_len, d, 0);
     *bytes = paged::workspace(p, T, Bd, Hq, Hkv, d, false);
     return HBA_OK;
 }

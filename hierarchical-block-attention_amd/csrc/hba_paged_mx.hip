@@ -10,7 +10,7 @@ extern "C" int hba_paged_attn_mx_workspace_bytes(int64_t T, int64_t Bd, int64_t 
     if (int st = paged::check(T, Bd, Hq, Hkv, d, W, S, shared_pages, one_each, max_len, 1 << 24)) return st;
     *bytes = 0;
     for (int bits = 4; bits <= 8; bits += 4) {
-        const paged::Plan p = paged::plan(T, Bd, Hq, Hkv, W, S, shared_pages, one_each != 0, max_len, bits);
+        const paged::Plan p = paged::plan(T, Bd, Hq, Hkv, W, S, shared_pages, one_each != 0, max_len, d, bits);
         const size_t n = paged::workspace(p, T, Bd, Hq, Hkv, d, true);
         *bytes = n > *bytes ? n : *bytes;
     }
