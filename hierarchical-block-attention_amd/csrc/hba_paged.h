@@ -1586,6 +1586,9 @@ static Plan plan(int64_t T, int64_t Bd, int64_t Hq, int64_t Hkv, int64_t W, int6
                  int64_t max_len, int64_t d, int bits) {   // bits: of the cache's codes, or 0
     Plan p = {};
     const int64_t G = Hq / Hkv, KT = rows::PAGE;
+    // A window or sinks past every length are every key, and no sum below overflows.
+    W = W < max_len ? W : max_len;
+    S = S < max_len ? S : max_len;
     int64_t keys = max_len - shared * KT;
     if (W > 0 && W < keys) keys = W;
     // A part of a prompt may span any number of windows.  (The parts cut the list of one

@@ -1094,6 +1094,7 @@ def _attend_pages(mx, q, q_gain, eps, kr_pages, v_pages, page_table, seq_lens, c
         raise ValueError(f"shared: whole pages of {BLOCK} tokens within the page table, and no window; got {shared}")
     if max_len < 1:
         raise ValueError(f"max_len must be positive, got {max_len}")
+    window, sinks = min(window, max_len), min(sinks, max_len)   # every key; of a larger int the call would see 64 bits
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin go together")
     n_tab = 0

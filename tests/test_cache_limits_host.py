@@ -1,0 +1,35 @@
+"""Attention over the paged caches, on the host: what it plans for windows, sinks and sizes up
+to the largest there are, and how much workspace each plan asks for.  Nothing here needs a GPU."""
+import ctypes
+
+import pytest
+
+from hba_amd import _lib
+
+LARGEST = 2 ** 63 - 1
+
+
+def workspace(mx, T, Bd, Hq, Hkv, d, W, S, shared, single, max_len):
+    """(status, bytes): the most that 4 and 8 bits need, or (mx false) the cache of rows."""
+    n, L = ctypes.c_size_t(0), _lib.lib()
+    f = L.hba_paged_attn_mx_workspace_bytes if mx else L.hba_paged_attn_workspace_bytes
+    return f(T, Bd, Hq, Hkv, d, W, S, shared, single, max_len, ctypes.byref(n)), n.value
+
+
+@pytest.mark.parametrize("mx", [False, True])
+@pytest.mark.parametrize("single", [0, 1])
+@pytest.mark.parametrize("max_len", [1, 64, 1000, 2000, 8000, 30000, 1 << 30])
+def test_windows_and_sinks_past_every_length(max_len, single, mx):
+    """They mean every key: the same plan as a window, or sinks, of the longest length."""
+    T = 3 if single else 15
+
+    def need(W, S):
+        return workspace(mx, T, 3, 14, 2, 64, W, S, 0, single, max_len)
+
+    every = need(max_len, 0)
+    assert every[0] == 0 and every == need(0, 0)
+    for W in (max_len + 1, 2 ** 31, 2 ** 62, LARGEST - 64, LARGEST):
+        assert need(W, 0) == every and need(W, LARGEST) == need(max_len, max_len)
+    for W in (1, 100, max_len):
+        for S in (max_len + 1, 2 ** 31, LARGEST - 62, LARGEST):
+            assert need(W, S) == need(W, max_len)
