@@ -217,7 +217,8 @@ template <int DT, int D, int F> __global__ __launch_bounds__(256, (DT == 0 && D 
                 ss += partner<2>(ss);
                 ss += partner<4>(ss);
                 if constexpr (TPH == 16) ss += partner<8>(ss);
-                const double f = gain * inverse_root(fmax(ss * (1.0 / D), (double)a.eps));
+                const double ms = ss * (1.0 / D);
+                const double f = gain * inverse_root(ms < (double)a.eps ? (double)a.eps : ms);   // (a maximum would lose a NaN)
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
