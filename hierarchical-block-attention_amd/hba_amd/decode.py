@@ -87,6 +87,10 @@ class PagedKVCache:
         self._scales_ok = False          # _scales holds the scales of the current lengths
         return P
 
+    def _fits(self, s, length):
+        if length > self.max_len:   # (its last page may hold more, but a length past max_len has no scale)
+            raise ValueError(f"sequence {s}: length {length} exceeds max_len {self.max_len}")
+
     def _ensure_pages(self, s, length):
         need = (length + PAGE - 1) // PAGE
         if need > self.max_pages:
@@ -118,6 +122,7 @@ class PagedKVCache:
         outputs: hba_prep_keys' kc and kr), and summarise its full pages.
         Setup path: plain tensor copies."""
         L = kc_seq.shape[0]
+        self._fits(s, L)
         if self._held.intersection(self._table[s]):
             raise ValueError(f"sequence {s} begins with pages that others read; load would overwrite them")
         self._ensure_pages(s, L)
@@ -319,6 +324,7 @@ class MXKVCache(PagedKVCache):
         """Fill sequence s with rotated keys kr_seq and values v_seq [L, Hkv, d] (a
         prefill's outputs), quantised as they are."""
         L = kr_seq.shape[0]
+        self._fits(s, L)
         if self._held.intersection(self._table[s]):
             raise ValueError(f"sequence {s} begins with pages that others read; load would overwrite them")
         taken = [[] for _ in range(self.batch)]

@@ -1,9 +1,11 @@
-"""Attention over the paged caches, on the host: what it plans for windows, sinks and sizes up
-to the largest there are, and how much workspace each plan asks for.  Nothing here needs a GPU."""
+"""The paged caches at their limits, on the host: what attention plans for the largest windows,
+sinks and sizes, and what the cache objects refuse.  Nothing here needs a GPU."""
 import ctypes
 
 import pytest
+import torch
 
+import hba_amd
 from hba_amd import _lib
 
 LARGEST = 2 ** 63 - 1
@@ -33,3 +35,25 @@ def test_windows_and_sinks_past_every_length(max_len, single, mx):
     for W in (1, 100, max_len):
         for S in (max_len + 1, 2 ** 31, LARGEST - 62, LARGEST):
             assert need(W, S) == need(W, max_len)
+
+
+def caches(max_len, num_pages=None, batch=2):
+    cfg = hba_amd.HBAConfig(n_heads=4, n_kv=2, head_dim=64)
+    return [hba_amd.PagedKVCache(cfg, batch, max_len, torch.float32, "cpu", num_pages=num_pages),
+            *(hba_amd.MXKVCache(cfg, batch, max_len, torch.float32, "cpu", bits=b, num_pages=num_pages) for b in (4, 8))]
+
+
+def load(c, s, n, v=None):
+    """n tokens into sequence s; their keys, or (v) other values."""
+    x = torch.zeros(n, 2, 64)
+    v = x if v is None else v
+    c.load(s, x, v) if isinstance(c, hba_amd.MXKVCache) else c.load(s, x, x, v, None)
+
+
+def test_a_load_past_the_longest_length_is_refused():
+    """The last page holds more tokens than max_len allows: a length there has no scale."""
+    for c in caches(50):
+        with pytest.raises(ValueError, match="exceeds max_len"):
+            load(c, 1, 60)
+        assert c.lens == c.seq_lens.tolist() == [0, 0] and c._table == [[], []] and len(c._free) == 2
+        c.scales()
