@@ -95,10 +95,10 @@ class PagedKVCache:
         need = (length + PAGE - 1) // PAGE
         if need > self.max_pages:
             raise ValueError(f"sequence {s}: length {length} exceeds max_len {self.max_len}")
+        if need - len(self._table[s]) > len(self._free):
+            raise RuntimeError("paged KV cache is out of pages")
         new = []
         while len(self._table[s]) < need:
-            if not self._free:
-                raise RuntimeError("paged KV cache is out of pages")
             p = self._free.pop()
             self._table[s].append(p)
             new.append(p)
@@ -125,11 +125,12 @@ class PagedKVCache:
         self._fits(s, L)
         if self._held.intersection(self._table[s]):
             raise ValueError(f"sequence {s} begins with pages that others read; load would overwrite them")
-        self._ensure_pages(s, L)
+        Hkv, d = kc_seq.shape[1], kc_seq.shape[2]
+        taken = [[] for _ in range(self.batch)]
+        taken[s] = self._ensure_pages(s, L)
         pages = torch.tensor(self._table[s], dtype=torch.long, device=self.kc_pages.device)
         npg = (L + PAGE - 1) // PAGE
         pad = npg * PAGE - L
-        Hkv, d = kc_seq.shape[1], kc_seq.shape[2]
 
         def paged(x, off):
             rows = torch.nn.functional.pad(x, (0, 0, 0, 0, 0, pad)).view(npg, PAGE, Hkv, d).transpose(1, 2)
@@ -137,22 +138,31 @@ class PagedKVCache:
             out[:, :, off] = rows.reshape(npg, Hkv, PAGE * d).to(out.dtype)
             return out
 
-        self.kc_pages[pages[:npg]] = paged(kc_seq, self._koff)
-        self.kr_pages[pages[:npg]] = paged(kr_seq, self._koff)
-        self.v_pages[pages[:npg]] = paged(v_seq, self._voff)
+        try:
+            self.kc_pages[pages[:npg]] = paged(kc_seq, self._koff)
+            self.kr_pages[pages[:npg]] = paged(kr_seq, self._koff)
+            self.v_pages[pages[:npg]] = paged(v_seq, self._voff)
+            full = pages[: L // PAGE]
+            if full.numel():
+                ops.summarize_pages(self.kc_pages, full, summ.probes, summ.proj, self.summ_pages)
+        except Exception:                # pages that only the host's table names would be lost to the device's
+            self._give_back(taken)
+            raise
         self.lens[s] = L
         self._sync_table()
-        full = pages[: L // PAGE]
-        if full.numel():
-            ops.summarize_pages(self.kc_pages, full, summ.probes, summ.proj, self.summ_pages)
 
     def reserve(self, length=None):
         """Allocate every sequence's pages up to `length` tokens (default
         max_len) and write the page table, so that later appends allocate
         nothing (a captured decode loop needs this)."""
         length = self.max_len if length is None else length
-        for s in range(self.batch):
-            self._ensure_pages(s, length)
+        taken = []
+        try:
+            for s in range(self.batch):
+                taken.append(self._ensure_pages(s, length))
+        except Exception:
+            self._give_back(taken)
+            raise
         self._sync_table()
 
     def append(self, k_new, v_new, qkn, summ, cos, sin):

@@ -57,3 +57,20 @@ def test_a_load_past_the_longest_length_is_refused():
             load(c, 1, 60)
         assert c.lens == c.seq_lens.tolist() == [0, 0] and c._table == [[], []] and len(c._free) == 2
         c.scales()
+
+
+def test_what_a_refused_call_took_is_given_back():
+    """Pages that only the host's table names would be written as page 0 by the next append."""
+    for c in caches(512, num_pages=3):
+        assert c.max_pages == 8
+        load_zeros = lambda: load(c, 0, 300)   # noqa: E731  five pages of three
+        for f in (load_zeros, lambda: c.reserve(128), lambda: c.reserve(), lambda: c.reserve(600)):
+            with pytest.raises((RuntimeError, ValueError)):
+                f()
+            assert c._table == [[], []] and sorted(c._free) == [0, 1, 2] and c.lens == [0, 0]
+        for bad in (torch.zeros(70, 3, 64), torch.zeros(69, 2, 64)):   # refused once the pages are there
+            with pytest.raises((RuntimeError, ValueError)):
+                load(c, 1, 70, bad)
+            assert c._table == [[], []] and sorted(c._free) == [0, 1, 2] and c.lens == [0, 0]
+        c.reserve(64)
+        assert [len(t) for t in c._table] == [1, 1] and c.page_table[:, 0].tolist() == [t[0] for t in c._table]
