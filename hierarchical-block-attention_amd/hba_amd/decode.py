@@ -403,7 +403,12 @@ class MXKVCache(PagedKVCache):
         return k, v, at
 
     def _page_rows(self, pages, which):
-        ids = torch.as_tensor(pages, device=self.device).to(torch.int32)
+        P = self.k_pages.shape[0]
+        if isinstance(pages, torch.Tensor) and pages.is_cuda and torch.cuda.is_current_stream_capturing():
+            ids = torch.where(pages < 0, pages + P, pages).to(torch.int32)   # (others read as 0)
+        else:                            # an index as any other, but on the host, where one out of range raises
+            at = pages.cpu() if isinstance(pages, torch.Tensor) else pages
+            ids = torch.arange(P, dtype=torch.int32)[at].to(self.device)
         n = ids.numel()
         full = torch.full((n,), PAGE, dtype=torch.int32, device=self.device)
         cu = torch.arange(0, PAGE * n + 1, PAGE, dtype=torch.int32, device=self.device)
@@ -413,7 +418,8 @@ class MXKVCache(PagedKVCache):
         return rows.reshape(*ids.shape, *rows.shape[1:])
 
     def key_rows(self, pages, rotated=True):
-        """Rotated keys of physical pages (int or index tensor) as token rows [..., Hkv, 64, d]."""
+        """Rotated keys of physical pages (an index: int, slice, tensor) as token rows
+        [..., Hkv, 64, d].  Waits for an index tensor on the device, but where it is captured."""
         if not rotated:
             raise ValueError("the cache in 4 or 8 bits holds rotated keys only")
         return self._page_rows(pages, 0)

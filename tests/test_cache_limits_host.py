@@ -74,3 +74,12 @@ def test_what_a_refused_call_took_is_given_back():
             assert c._table == [[], []] and sorted(c._free) == [0, 1, 2] and c.lens == [0, 0]
         c.reserve(64)
         assert [len(t) for t in c._table] == [1, 1] and c.page_table[:, 0].tolist() == [t[0] for t in c._table]
+
+
+@pytest.mark.parametrize("pages", [16, -17, [0, 16], torch.tensor([3, -17]), torch.tensor([[2], [99]])])
+def test_rows_of_pages_that_there_are_none_of(pages):
+    """As of any tensor's index."""
+    for c in caches(512):
+        for f in (lambda: c.key_rows(pages, rotated=True), lambda: c.value_rows(pages)):
+            with pytest.raises(IndexError):
+                f()

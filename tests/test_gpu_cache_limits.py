@@ -2,6 +2,8 @@
 import pytest
 import torch
 
+import hba_amd
+import mx64
 import test_gpu_mx_cache as mxc
 import test_gpu_paged_attn as rows
 from hba_amd import ops
@@ -51,3 +53,30 @@ def test_keys_at_the_edges_with_the_norm(turn, dt, d, bits):
     back = ops.kv_read_mx(got[0].cuda(), got[1].cuda(), a["table"], a["lens"], a["cu"], 120, d, torch.float32)[0].cpu()
     assert back[[6, 7, 10, 12], 0].isnan().all() and back[8, 1].isnan().all() and not back[8, 0].isnan().any()
     assert bool((back[9].isnan().sum(-1) == (64 if turn else 32)).all())
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_rows_of_pages_by_any_index(bits):
+    """What the whole cache's key_rows and value_rows take: numbers from either end, lists,
+    slices, masks, tensors on either side; within a captured graph tensors on the device."""
+    cfg = hba_amd.HBAConfig(n_heads=4, n_kv=2, head_dim=64)
+    c = hba_amd.MXKVCache(cfg, 2, 200, torch.float32, "cuda", bits=bits)
+    for s in range(2):
+        c.load(s, *(torch.randn(200, 2, 64, device="cuda") for _ in range(2)))
+    mask = torch.zeros(8, dtype=torch.bool)
+    mask[[1, 6]] = True
+    for rows_of, pages in ((c.key_rows, c.k_pages), (c.value_rows, c.v_pages)):
+        held = mx64.rows(pages.cpu(), bits, 64, pages is c.k_pages).float().cuda()
+        for i in (3, -1, [0, -8], slice(2, 7, 2), mask, mask.cuda(), torch.tensor([[7, -2]]), torch.tensor([5, 5, 0]).cuda(),
+                  torch.tensor(4).cuda(), torch.zeros(0, dtype=torch.long)):
+            assert torch.equal(rows_of(i), held[i]), i
+        i = torch.tensor([[-1, 2], [0, -8]], device="cuda")
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = rows_of(i)
+        for j in (i.clone(), torch.tensor([[4, -3], [7, 1]], device="cuda")):
+            i.copy_(j)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, held[j])
