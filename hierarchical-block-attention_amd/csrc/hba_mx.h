@@ -34,6 +34,7 @@ typedef uint32_t u32x6 __attribute__((ext_vector_type(6)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 using hba::f32x16;
 typedef float f32x32 __attribute__((ext_vector_type(32)));
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));   // of a table that may begin anywhere
 template <int N> struct number {
     static constexpr int value = N;
 };

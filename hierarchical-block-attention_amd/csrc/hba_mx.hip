@@ -188,11 +188,13 @@ template <int DT, int D, int F> __global__ __launch_bounds__(256, (DT == 0 && D 
         if (a.cos) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                Four<0> c, s;
-                c.load(reinterpret_cast<const char *>(a.cos + (int64_t)pos * D + t0 + i * (D / 2)));
-                s.load(reinterpret_cast<const char *>(a.sin + (int64_t)pos * D + t0 + i * (D / 2)));
-                c.get(cs[i]);
-                s.get(sn[i]);
+                const int64_t at = (int64_t)pos * D + t0 + i * (D / 2);
+                const f32x4 c = *reinterpret_cast<const f32x4u *>(a.cos + at), s = *reinterpret_cast<const f32x4u *>(a.sin + at);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    cs[i][e] = c[e];
+                    sn[i][e] = s[e];
+                }
             }
         }
         float y[2][4], v[2][4];
@@ -488,8 +490,7 @@ extern "C" int hba_kv_append_mx(int dtype, const void *k, const int64_t k_stride
         return HBA_ERR_INVALID_ARG;
     const int64_t e = abi::elem_size(dtype), al = 16 / e;
     if (!abi::aligned16(k) || !abi::aligned16(v) || k_strides[0] % al || k_strides[1] % al || v_strides[0] % al ||
-        v_strides[1] % al || !abi::aligned16(cos_tab) || !abi::aligned16(sin_tab) || !abi::aligned16(k_pages) ||
-        !abi::aligned16(v_pages))
+        v_strides[1] % al || !abi::aligned16(k_pages) || !abi::aligned16(v_pages))
         return HBA_ERR_UNSUPPORTED;
     if (T == 0) return HBA_OK;
     mx::AppendArgs a = {};

@@ -271,8 +271,8 @@ __device__ __forceinline__ void decode_codes(const Args &a, int s, int g, int he
             }
 #pragma unroll
             for (int e = 0; e < NE; e += 4) {
-                *reinterpret_cast<f32x4 *>(cs + e) = *reinterpret_cast<const f32x4 *>(a.cos + pos + first + e);
-                *reinterpret_cast<f32x4 *>(sn + e) = *reinterpret_cast<const f32x4 *>(a.sin + pos + first + e);
+                *reinterpret_cast<f32x4 *>(cs + e) = *reinterpret_cast<const mx::f32x4u *>(a.cos + pos + first + e);
+                *reinterpret_cast<f32x4 *>(sn + e) = *reinterpret_cast<const mx::f32x4u *>(a.sin + pos + first + e);
             }
         }
         finish_group<D, NE, FMT == 8 || D == 128>(qx, qy, first < D / 2, a.gain ? a.gain + head : nullptr, a.eps,
@@ -877,7 +877,6 @@ template <int DT, int D> __device__ __forceinline__ void zero_strays(const Args 
 template <int D>
 __device__ __forceinline__ void finish_rows(float (&x)[D / 64][32], int hf, const float *gain, float eps, const float *cs,
                                             const float *sn, float scale) {
-    typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
     const auto norm = [&]() {
         if (gain) {
             float ss = 0.0f;
@@ -904,8 +903,8 @@ __device__ __forceinline__ void finish_rows(float (&x)[D / 64][32], int hf, cons
         for (int s = 0; s < D / 64; ++s)
 #pragma unroll
             for (int i = 0; i < M; i += 4) {
-                *reinterpret_cast<f32x4 *>(&to[0][s][i]) = *reinterpret_cast<const f32x4u *>(cs + 64 * s + e0 + i);
-                *reinterpret_cast<f32x4 *>(&to[1][s][i]) = *reinterpret_cast<const f32x4u *>(sn + 64 * s + e0 + i);
+                *reinterpret_cast<f32x4 *>(&to[0][s][i]) = *reinterpret_cast<const mx::f32x4u *>(cs + 64 * s + e0 + i);
+                *reinterpret_cast<f32x4 *>(&to[1][s][i]) = *reinterpret_cast<const mx::f32x4u *>(sn + 64 * s + e0 + i);
             }
     };
     const auto turn = [&](int e0, const float (&by)[2][D / 64][M]) {

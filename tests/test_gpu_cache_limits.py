@@ -80,3 +80,23 @@ def test_rows_of_pages_by_any_index(bits):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, held[j])
+
+
+def anywhere(t, by):
+    """t in memory that begins `by` elements behind a 16-byte boundary."""
+    flat = torch.empty(t.numel() + by, dtype=t.dtype, device="cuda")
+    assert flat.data_ptr() % 16 == 0
+    flat[by:] = t.cuda().flatten()
+    return flat[by:].view(t.shape)
+
+
+@pytest.mark.parametrize("by", [1, 2, 3])
+@pytest.mark.parametrize("dt,d,bits", mxc.FORMS)
+def test_tables_that_begin_anywhere(dt, d, bits, by):
+    """cos and sin are read in 16 bytes wherever they begin: append, single tokens, parts."""
+    s = mxc.new_tokens(DT[dt], d, bits, 2, [70, 9], [33, 2])
+    mxc.same(mxc.append(s, cos=anywhere(s["cos"], by), sin=anywhere(s["sin"], (by + 1) % 4)), mxc.append(s))
+    for new, shared in ((None, 0), ([40, 3], 0), (None, 64)):
+        s = mxc.setup(DT[dt], d, bits, 4, 2, [200, 65], new, shared=shared)
+        got = mxc.call(s, cos=anywhere(s["cos"], by), sin=anywhere(s["sin"], (by + 1) % 4))
+        assert torch.equal(got, mxc.call(s))
