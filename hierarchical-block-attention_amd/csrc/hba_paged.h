@@ -1742,9 +1742,10 @@ static int check(int64_t T, int64_t Bd, int64_t Hq, int64_t Hkv, int64_t d, int6
         return HBA_ERR_INVALID_ARG;
     if (W > 0 && shared > 0) return HBA_ERR_INVALID_ARG;   // a window past the prefix would not see it
     if (one && T != Bd) return HBA_ERR_INVALID_ARG;
-    if (max_len > (1 << 30) || max_pages > (1 << 24) || shared > max_pages || T * Hq > (1 << 30) || Hkv > 65535 ||
-        Bd * Hkv * (Hq / Hkv + 16) > 0x7fffffff)
-        return HBA_ERR_UNSUPPORTED;
+    if (max_len > (1 << 30) || max_pages > (1 << 24) || shared > max_pages || T > (1 << 30) || Hq > (1 << 30) ||
+        Bd > 0x7fffffff || Hkv > 65535)
+        return HBA_ERR_UNSUPPORTED;   // (before they are multiplied)
+    if (T * Hq > (1 << 30) || Bd * (Hq + 16 * Hkv) > 0x7fffffff) return HBA_ERR_UNSUPPORTED;
     return HBA_OK;
 }
 

@@ -83,3 +83,10 @@ def test_rows_of_pages_that_there_are_none_of(pages):
         for f in (lambda: c.key_rows(pages, rotated=True), lambda: c.value_rows(pages)):
             with pytest.raises(IndexError):
                 f()
+
+
+@pytest.mark.parametrize("mx", [False, True])
+@pytest.mark.parametrize("T,Bd,Hq,Hkv", [(1, 2 ** 62, 8, 4), (1, 2 ** 60, 16, 16), (2 ** 62, 1, 4, 1), (2 ** 32, 1, 2 ** 32, 1),
+                                         (2 ** 34, 2 ** 34, 2 ** 30, 2 ** 15), (5, 2 ** 58, 32, 2), (2 ** 63 - 1, 3, 2, 1)])
+def test_sizes_whose_products_overflow(T, Bd, Hq, Hkv, mx):
+    assert workspace(mx, T, Bd, Hq, Hkv, 64, 0, 0, 0, int(T == Bd), 1000) == (-2, 0)
