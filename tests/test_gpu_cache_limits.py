@@ -100,3 +100,57 @@ def test_tables_that_begin_anywhere(dt, d, bits, by):
         s = mxc.setup(DT[dt], d, bits, 4, 2, [200, 65], new, shared=shared)
         got = mxc.call(s, cos=anywhere(s["cos"], by), sin=anywhere(s["sin"], (by + 1) % 4))
         assert torch.equal(got, mxc.call(s))
+
+
+@pytest.mark.parametrize("dt,d,bits", [*mxc.FORMS, ("f32", 64, 16), ("bf16", 128, 16)])
+def test_pages_outside_the_cache_are_read_as_the_nearest(dt, d, bits):
+    """Attention clamps page numbers: the same results as with the first and the last page there."""
+    whole = bits == 16
+    m = rows if whole else mxc
+    for lens, new, shared in (([300, 65], None, 0), ([300, 65], [40, 3], 0), ([300, 200], None, 128), ([3000], None, 0),
+                              ([3000, 700], [600, 7], 0)):
+        s = m.setup(DT[dt], d, *(() if whole else (bits,)), 6, 3, lens, new, shared=shared)
+        for name in ("kr", "vp") if whole else ("kp", "vp"):   # the first and the last page: whole, and unlike the others
+            s[name][0], s[name][-1] = s[name][int(s["table"][0, 1])], s[name][int(s["table"][0, 2])]
+        far, near = s["table"].clone(), s["table"].clone()
+        for at, page, there in (((0, 0), -7, 0), ((0, 3), 10 ** 8, -1), ((-1, 1), 2 ** 31 - 1, -1), ((-1, 0), -2 ** 31, 0)):
+            if at[1] < shared // 64:
+                far[:, at[1]], near[:, at[1]] = page, there % len(s["vp"])
+            else:
+                far[at], near[at] = page, there % len(s["vp"])
+        got, want = m.call(s, table=far), m.call(s, table=near)
+        assert torch.isfinite(want).all() and torch.equal(got, want) and not torch.equal(want, m.call(s))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("d", [64, 128])
+def test_read_at_the_smallest_scales(d, bits):
+    """fp32 rows are the values; bf16 rows too, but for 8 bits at 2^-126 and 2^-125, whose smallest
+    codes lie below bf16's last step: those are the nearest, ties to even."""
+    g = torch.Generator().manual_seed(bits)
+    pages = torch.randint(0, 256, (20, 1, mx64.page_bytes(d, bits)), generator=g).to(torch.uint8)
+    if bits == 8:
+        pages[(pages & 127) == 127] = 3                       # no NaN
+    for b in range(20):
+        pages[b, :, 64 * d * bits // 8:] = b + 1
+    a = [torch.arange(20, dtype=torch.int32).view(1, 20).cuda(), torch.tensor([1280], dtype=torch.int32).cuda(),
+         torch.tensor([0, 1280], dtype=torch.int32).cuda()]
+    for dt in (torch.float32, torch.bfloat16):
+        out = ops.kv_read_mx(pages.cuda(), pages.cuda(), *a, 1280, d, dt)
+        for x, keys in zip(out, (True, False)):
+            want = mx64.rows(pages, bits, d, keys).float()    # [20, 1, 64, d]
+            got = x.cpu().view(20, 64, 1, d).transpose(1, 2)
+            assert torch.equal(got, want.to(dt))
+            exact = got.float() == want
+            assert exact[2:].all() and (exact.all() or (bits == 8 and dt == torch.bfloat16))
+
+
+@pytest.mark.parametrize("dt,d,bits", mxc.FORMS)
+def test_calls_repeat_themselves(dt, d, bits):
+    """Bit for bit: no sum's order depends on which workgroup is first."""
+    for lens, new, shared in (([300, 65], None, 0), ([5000, 700, 2100], None, 0), ([3000, 700], [600, 7], 0),
+                              ([300, 200, 1500], None, 128), ([300, 65], [40, 3], 0)):
+        a = mxc.dev(mxc.setup(DT[dt], d, bits, 6, 3, lens, new, shared=shared))
+        want = mxc.call(a)
+        for _ in range(4):
+            assert torch.equal(mxc.call(a), want)
