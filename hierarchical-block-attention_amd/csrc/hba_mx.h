@@ -3,7 +3,8 @@
 // A page (64 tokens of one KV head, D elements each) is 64 D F / 8 bytes of codes
 // and 2 D bytes of scales.  Codes are e2m1 (F = 4) or e4m3 (F = 8); the elements
 // 32 g .. 32 g + 31 of a token share the scale 2^(b - 127), b a byte (b = 255, codes 0:
-// they are NaN).  A value has at most 4 bits of mantissa, so it is exact in bf16, and one
+// they are NaN).  A value has at most 4 bits of mantissa, so it is exact in bf16 (from 2^-130
+// on: the smallest codes of F = 8 at b < 3 are rounded to bf16's last step, 2^-133), and one
 // instruction makes two of them from their codes and scale.
 //
 // The order is that of the decode kernel's MFMA tiles (16 keys; the tile and row of
@@ -93,7 +94,7 @@ template <int KB, int QB> __device__ __forceinline__ f32x4 product6(u32x4 k, i32
     const i32x8 a = {(int)k[0], (int)k[1], (int)k[2], (int)k[3], 0, 0, 0, 0};
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q, c, 4, 2, KB, ks, QB, qs);
 }
-// The same in fp32 (exact).
+// Codes 2 i, 2 i + 1 of a word times a power of two, in fp32 (exact).
 template <int F> __device__ __forceinline__ f32x2 pair(uint32_t w, float scale, int i) {
     if constexpr (F == 4)
         return i == 0   ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 0)
@@ -141,7 +142,9 @@ template <int KB, int QB> __device__ __forceinline__ f32x16 product6(u32x4 k, i3
 // several cycles: these must not lie where an operand does, as the compiler places them where
 // the operand is needed no more (the scale of a query's last part, whose elements then were of
 // other scales: 0.5% off the outputs of bf16 at d = 128).  So the operands stay in use; the build
-// looks for others.
+// looks for others.  (Conversions of two elements may lie there: the compiler places results of
+// theirs on their codes and scales in all of read_kernel's forms, whose rows are the definition's
+// bit for bit.)
 template <bool LAST> __device__ __forceinline__ u32x6 to6(f32x16 even, f32x16 odd, float f) {
     u32x6 r = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, f);
     asm volatile("" : "+v"(r) : "v"(f));
@@ -220,7 +223,7 @@ template <int D, int N> struct Rows6 {
             const u32x6 w = {(uint32_t)q[s][n][0], (uint32_t)q[s][n][1], (uint32_t)q[s][n][2],
                              (uint32_t)q[s][n][3], (uint32_t)q[s][n][4], (uint32_t)q[s][n][5]};
             const uint32_t b = (uint32_t)qs[s][n / 4] >> (8 * (n % 4)) & 255u;
-            const f32x32 y = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(w, __uint_as_float(b << 23));   // (not from6: it would spill)
+            const f32x32 y = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(w, __uint_as_float(b << 23));   // (not from6: it would spill; the build looks here too)
 #pragma unroll
             for (int e = 0; e < 32; ++e) x[e] += y[e];
         }
@@ -465,8 +468,9 @@ template <int DT, int D, int F> struct TileKV {
 // the queries are in log2 units, in parts.  All groups of the workgroup call it with the same n.
 // The logits count from a reference of the row's own, O and l are sums of 2^(s - m):
 // m is 0 as long as no row of the wave leaves +-BAND (fp32 and bf16 hold 2^-126 .. 2^127 with the
-// same number of bits: nothing is lost, and the products begin at 0 without a register), else
-// the largest logit when it was last set.  All the tile's logits are taken before the first
+// same number of bits, and the products begin at 0 without a register; a row whose largest weight
+// is 2^-BAND loses weights below 2^-94 of it, and values below 2^-94 lose bits; what overflows
+// goes to attend_each), else the largest logit when it was last set.  All the tile's logits are taken before the first
 // exponential: the next 32 keys' matrix products run beside the exponentials of these.
 constexpr float BAND = 32.0f, ABOVE = 0x1p40f;   // ABOVE: a sum over a tile's keys that sets m anew
 template <int DT, int D, class Src, class Keys>

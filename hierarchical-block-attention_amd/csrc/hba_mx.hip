@@ -400,9 +400,11 @@ __device__ __forceinline__ void read_half(const ReadArgs &a, const char *kp, con
 // through LDS as rows, so that whole rows are written.  Tokens that lie in no page give
 // 0: those of a sequence are tiles behind its pages', those of no sequence (before
 // cu[0], behind cu[Bd]) are left to the workgroups that have nothing else.  A workgroup's search
-// for its sequence is worth a whole page's work where there are enough of those: 94000 tokens,
-// 2 KV heads, d = 64, 8 bits 17.5 us by pages and 21 by halves, 12800 tokens, 4 heads, d = 128,
-// 4 bits 12.6 and 12.3 (before keys and values were packed in words: 15.2, 4.9 TB/s, and 9.6).
+// for its sequence is worth a whole page's work where there are enough of those: by pages and by
+// halves, bf16, 94000 tokens, 2 KV heads, d = 64, 8 bits 14.8 us (4.9 TB/s) and 16.6, 40000 8.3 and
+// 9.5, 12800 5.3 and 5.3, 3000 4.4 and 4.0; 4 heads, d = 128, 4 bits, 40000 tokens 19.0 and 20.2,
+// 12800 9.0 and 9.3, 3000 5.7 and 5.1.  (Keys and values an element at a time instead of packed in
+// words: 17.5 for the first, 12.6 for 12800 tokens of the second.)
 template <int DT, int D, int F> __global__ __launch_bounds__(256) void read_kernel(const ReadArgs a) {
     typedef typename St<DT>::T T;
     constexpr int RS = D + (DT == 1 ? 8 : 4);

@@ -868,9 +868,6 @@ template <int DT, int D> __device__ __forceinline__ void zero_strays(const Args 
     }
 }
 
-// SHARED: the rows of all tokens over the shared pages (x: 128-row tile); else the
-// rows of one sequence's tokens over its own pages (x: tile of the ragged batch).
-// g: KV head, z: part, a run of a.part pages.
 // finish_q for Rows6: x[s] are the elements 64 s + 32 hf .. of the row; cs, sn begin at 32 hf.
 // The table's rows are loaded at once, in 16 bytes (wherever the tensor begins): an element at
 // a time, each behind a branch, they were 12 us of a workgroup of 128 rows.
@@ -983,6 +980,9 @@ __device__ __forceinline__ void row_queries(const Args &a, int t, int head, int 
 
 template <int DT, int D, int FMT> struct RowSource { typedef mx::TileKV<OPS<DT, FMT>, D, FMT> T; };
 template <int DT, int D> struct RowSource<DT, D, 0> { typedef rows::PageKV<DT, D> T; };
+// SHARED: the rows of all tokens over the shared pages (x: 128-row tile); else the
+// rows of one sequence's tokens over its own pages (x: tile of the ragged batch).
+// g: KV head, z: part, a run of a.part pages.
 template <int DT, int D, int FMT, bool SHARED>
 __device__ __forceinline__ void rows_part(const Args &a, char *smem, int x, int g, int z) {
     typedef typename RowSource<DT, D, FMT>::T Source;
@@ -1129,9 +1129,11 @@ __device__ __forceinline__ void rows_part(const Args &a, char *smem, int x, int 
     }
 }
 
-// 4 sequences, 1560 new tokens behind 1300 to 8500 keys, 14 heads, d = 64, bf16: 73 us,
-// 27 at the rate of a large product.  Queries of two bf16 parts double q . k (3
-// products for 2), exponentials and conversions as in the sliding-window kernel.
+// Over rows (FMT 0): 4 sequences, 1560 new tokens behind 1300 to 8500 keys, 14 heads, d = 64,
+// bf16: 73 us, 27 at the rate of a large product.  Queries of two bf16 parts double q . k (3
+// products for 2), exponentials and conversions as in the sliding-window kernel.  Over codes:
+// `plan` has figures.  Registers are spilled, around the keys' loop or in it, at d = 128 (bf16, 4
+// bits 18, 8 bits 105 of them; fp32, 8 bits 37) and by fp32 over 8 bits at d = 64 (58).
 template <int DT, int D, int FMT, bool SHARED>
 __global__ __launch_bounds__(64 * rows::NW, (DT == 1 && D == 64 && FMT != 8 ? 3 : rows::WAVES<DT, D>)) void rows_kernel(
     const Args a) {
@@ -1148,8 +1150,10 @@ __global__ __launch_bounds__(64 * rows::NW, (DT == 1 && D == 64 && FMT != 8 ? 3 
 // keys, 14 heads over 2, d = 64, 4 bits: 67 us and 5 for the join, 458 TFLOP/s, where 1024
 // workgroups of a run of keys each took 71 and 8; 650 TFLOP/s at four times the tokens.  Three
 // sets have 168 registers, too few: 96.  A window of 1024 in 8 bits, d = 128, 550 tokens: 38 and
-// 6, by runs 44 and 6.)  Of a SIMD's time vector instructions have 60%, half of it exponentials
-// and their rounding to bf16, and the matrix cores 30%; a piece's beginning and end are 10 us.
+// 6, by runs 69 with the join.  No spills of more than 7 registers, but 94 in bf16 over 4 bits at
+// d = 128: 278 us for 1560 tokens behind 8000 keys, 28 heads over 4, by runs 316.)  Of a SIMD's
+// time vector instructions have 60%, half of it exponentials and their rounding to bf16, and the
+// matrix cores 30%; a piece's beginning and end are 10 us.
 constexpr int TILES = 2048;    // row tiles of a KV head, at most
 template <int DT, int D, int FMT> constexpr int SETS = DT == 0 && D == 128 ? 1 : 2;
 // What a piece costs besides its keys, in tiles of keys (6 us, and 0.7 a tile; 10 and 0.9 at 32
@@ -1611,7 +1615,15 @@ static Plan plan(int64_t T, int64_t Bd, int64_t Hq, int64_t Hkv, int64_t W, int6
         // times 1 to 6 behind 4000 23 and 26; in 8 bits 1560 tokens alone, behind 1000 and 8000 keys
         // 26, 35, 71 and 19, 34, 101, the windows 80 and 74, the 5 tokens 25 and 17.  d = 128, 8 bits:
         // 5 tokens behind 16000 keys 34 and 40, 8 times 1 to 6 behind 1600 30 and 48; 3 windows of
-        // 1024 44 and 68 (fp32 70 and 61), 64 of 1 to 6 tokens 52 and 81.
+        // 1024 44 and 68 (fp32 70 and 61), 64 of 1 to 6 tokens 52 and 81.  d = 128, 4 bits, bf16 (and
+        // fp32): 1560 tokens behind 1000, 2500, 8000 keys 84, 126, 278 and 85, 133, 316 (132, 240, 631
+        // and 160, 278, 702), alone 71 and 64 (103 and 122), 4900 in 16 sequences 321 and 296 (661 and
+        // 763), a window of 1024 in those 189 and 149 (320 and 348); 5 tokens behind 16000 keys 38 and
+        // 27 (50 and 51), 16 times 1 to 6 behind 4000 46 and 54 (76 and 116), 8 times behind 1600 34
+        // and 30 (45 and 52).  fp32, d = 64, 4 bits (8 bits): 45, 64, 138 and 47, 71, 150 (47, 69, 155
+        // and 50, 82, 181); 5 tokens 33 and 20 (33 and 21), 16 times 31 and 34 (32 and 40).  So bf16's
+        // borders cost fp32 at d = 128 up to a fifth where it stays in runs, and bf16 in 4 bits a
+        // twelfth where many tokens are shared out.
         // (And what LDS holds, the join's grid, sums in 32 bits.)
         const int64_t all_pages = p.tiles * Hkv * pages;
         const bool enough = bits && (bits == 8 && d == 128 ? all_pages >= 512 : pages > 32 && all_pages >= 2048);

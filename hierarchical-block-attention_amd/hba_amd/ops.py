@@ -1292,7 +1292,7 @@ def _kv_read_mx(k_pages, v_pages, page_table, seq_lens, cu, tokens, head_dim, dt
 
 def kv_read_mx(k_pages, v_pages, page_table, seq_lens, cu, tokens, head_dim, dtype):
     """The cache in 4 or 8 bits as rows (k, v) [tokens, Hkv, head_dim] of float32 or
-    bfloat16 (which holds every value): tokens cu[s] .. cu[s + 1] - 1 are the last ones of
+    bfloat16 (which holds every value of 2^-130 and more): tokens cu[s] .. cu[s + 1] - 1 are the last ones of
     sequence s, as kv_append_mx takes them; cu None: the newest of each.  Keys come as they
     lie there, rotated.  Tokens that lie in no page of the cache give 0."""
     args = (k_pages, v_pages, page_table, seq_lens, cu, tokens, head_dim, dtype)

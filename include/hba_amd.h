@@ -561,7 +561,8 @@ int hba_paged_attn(int dtype, const void *q, const int64_t q_strides[2], const f
  * the group's largest magnitude is at most 1.75 * 2^emax times it (e2m1: 7, where more
  * than 6 becomes 6; e4m3: 448), codes are the nearest ones (ties to even); a group of
  * zeros has b = 0 and codes 0, one that holds a NaN, an infinity or a magnitude over
- * 1.75 * 2^127 b = 255 and codes 0 and reads as NaN.  Within a page and KV head, token j's element t, and its group's byte:
+ * 1.75 * 2^127 b = 255 and codes 0 and reads as NaN.  Within a page and KV head, token j's
+ * element t, and its group's byte:
  *   keys    mt = 2*(j/32) + (j/4)%2, l16 = 4*((j%32)/8) + j%4: byte x = (mt*(d/4) + t%(d/4))
  *           * bits/8 of lane l16 + 16*(t/(d/4)); b at 64*d*bits/8 + (l16 + 16*(t/32))*4 + mt;
  *   values  byte x = (j/32)*(d*bits/16) + ((t/16)*8 + j%8) * bits/8 of lane t%16 +
@@ -573,8 +574,9 @@ int hba_paged_attn(int dtype, const void *q, const int64_t q_strides[2], const f
 /*
  * Append tokens to it: QKNorm of k (k_gain; NULL: none), its rotation at the token's
  * position (cos_tab, sin_tab; NULL: none), both in fp64 and rounded to fp32 once, quantised
- * into k_pages, v quantised into v_pages.  k, v: element strides of token and head, rows
- * on 16-byte boundaries.  cu int32 [Bd+1]: tokens cu[s] .. cu[s+1]-1 are the last ones of
+ * into k_pages, v quantised into v_pages.  (A NaN in a key makes all of its norm, so all of its
+ * groups, NaN.)  k, v: element strides of token and head, rows on 16-byte boundaries; the
+ * tables begin anywhere.  cu int32 [Bd+1]: tokens cu[s] .. cu[s+1]-1 are the last ones of
  * sequence s, whose seq_lens[s] counts them already; NULL: one token per sequence (T =
  * Bd), the newest.  What is not appended, and what stays, is as for hba_kv_append_ragged.
  * No counterpart in the reference, which has no KV cache.
@@ -588,8 +590,8 @@ int hba_kv_append_mx(int dtype, const void *k, const int64_t k_strides[2], const
 
 /*
  * Read tokens back as rows k, v [T, Hkv, d] (contiguous; fp32, or bf16, which holds
- * every value): those that hba_kv_append_mx would write with the same cu and seq_lens.
- * Tokens at positions < 0 or past the page table, on a page outside 0 .. num_pages-1,
+ * every value of 2^-130 and more; below it is rounded): those that hba_kv_append_mx would
+ * write with the same cu and seq_lens.  Tokens at positions < 0 or past the page table, on a page outside 0 .. num_pages-1,
  * before cu[0] or behind cu[Bd] (a padded batch) give 0.
  */
 int hba_kv_read_mx(int dtype, const void *k_pages, const void *v_pages, int64_t num_pages,
